@@ -310,6 +310,71 @@ LLATTN_API int llattn_bwd(const llattn_bwd_args* args, void* stream);
 #define LLATTN_BWD_NOALLOC_SCRATCH_BYTES (32u << 20)
 LLATTN_API int llattn_bwd_noalloc(const llattn_bwd_args* args, void* stream);
 
+/* Softmax cross-entropy of an output projection, and its gradients, without
+ * the [tokens, vocab] logits (models.py:517-518 with the F.cross_entropy of
+ * the reference's training loop):
+ *   l = x w^T,  loss[n] = logsumexp_v l[n, v] - l[n, targets[n]]
+ *   dx = G w, dw = G^T x,  G[n, v] = g[n] (softmax(l[n])[v] - [v == targets[n]])
+ * Tokens whose target is ignore_index have loss 0 and no gradient, and their
+ * rows of x do not reach dw; a target outside [0, vocab) makes its row's loss
+ * and the gradients NaN. g[n] = grad_rows[n] (reduction none), 1 (sum) or
+ * 1 / max(1, counted tokens) (mean).
+ *   x [tokens, d] dtype, row stride ldx; w [vocab, d] dtype, row stride ldw
+ *   (elements; unaligned rows are copied into the workspace); targets int64
+ * Outputs (each may be NULL): losses [tokens] fp32 (only without gradients),
+ * loss (fp32 scalar; reductions mean and sum), dx [tokens, d], dw [vocab, d]
+ * dtype, contiguous. workspace: llattn_xent_workspace_bytes bytes, 256-byte
+ * aligned, no initialisation; it holds half a GiB of exponentials at most
+ * (at least 256 rows), whatever the number of tokens. */
+typedef enum llattn_xent_reduction {
+  LLATTN_XENT_NONE = 0,
+  LLATTN_XENT_MEAN = 1,
+  LLATTN_XENT_SUM = 2
+} llattn_xent_reduction;
+
+typedef struct llattn_xent_args {
+  int32_t tokens, d, vocab, dtype, reduction;
+  int64_t ignore_index;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const int64_t* targets;
+  const float* grad_rows;
+  float* losses;
+  float* loss;
+  void* dx;
+  void* dw;
+  void* workspace;
+  size_t workspace_bytes;
+} llattn_xent_args;
+
+/* pointers are only tested for NULL and alignment (0 on bad arguments) */
+LLATTN_API size_t llattn_xent_workspace_bytes(const llattn_xent_args* args);
+LLATTN_API int llattn_xent(const llattn_xent_args* args, void* stream);
+
+/* buf[i] *= *factor (device scalar) over n elements of dtype; a factor of 1
+ * leaves buf untouched. The upstream gradient of llattn_xent's loss. */
+LLATTN_API int llattn_scale(void* buf, int64_t n, int dtype, const float* factor, void* stream);
+
+/* Orthogonalised updates: per matrix g_i [rows, cols] (contiguous),
+ *   X = g / (|g|_F + eps); `steps` times: S = X X^T, X = a X + (b S + c S^2) X
+ * (on the shorter side), out [count, rows, cols] bf16. g: host array of
+ * count device pointers, read during the call. Computed with 16-bit operands
+ * and fp32 accumulation. workspace: llattn_orth_workspace_bytes bytes,
+ * 256-byte aligned. No counterpart in the reference (AdamW only). */
+typedef struct llattn_orth_args {
+  int32_t rows, cols, count, steps, dtype;
+  float a, b, c, eps;
+  const void* const* g;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+} llattn_orth_args;
+
+LLATTN_API size_t llattn_orth_workspace_bytes(const llattn_orth_args* args);
+LLATTN_API int llattn_orth(const llattn_orth_args* args, void* stream);
+
 /* Per-kernel timing with CUDA events on the launching stream, the native
  * side of the module's set_profile/get_profile_stats (models.py:131-157,
  * which times phases with host syncs instead). enable != 0 turns it on;

@@ -21,7 +21,9 @@ EXPORTED = (
     "llattn_pool_fwd", "llattn_pool_bwd", "llattn_fwd", "llattn_bwd", "llattn_bwd_noalloc", "llattn_decode",
     "llattn_profile_enable", "llattn_profile_read", "llattn_profile_name", "llattn_colsum_workspace_bytes",
     "llattn_colsum", "llattn_fault_inject_host", "llattn_pool_proj_fwd", "llattn_pool_proj_bwd",
+    "llattn_xent_workspace_bytes", "llattn_xent", "llattn_scale", "llattn_orth_workspace_bytes", "llattn_orth",
 )
+XENT_NONE, XENT_MEAN, XENT_SUM = 0, 1, 2
 
 
 class Dims(ctypes.Structure):
@@ -67,6 +69,20 @@ class DecodeArgs(ctypes.Structure):
                 ("mixed_row", _vp)]
 
 
+class XentArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int32), ("d", ctypes.c_int32), ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("reduction", ctypes.c_int32), ("ignore_index", ctypes.c_int64), ("x", _vp), ("ldx", ctypes.c_int64),
+                ("w", _vp), ("ldw", ctypes.c_int64), ("targets", _vp), ("grad_rows", _fp), ("losses", _fp),
+                ("loss", _fp), ("dx", _vp), ("dw", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class OrthArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("count", ctypes.c_int32),
+                ("steps", ctypes.c_int32), ("dtype", ctypes.c_int32), ("a", ctypes.c_float), ("b", ctypes.c_float),
+                ("c", ctypes.c_float), ("eps", ctypes.c_float), ("g", ctypes.POINTER(_vp)), ("out", _vp),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -109,6 +125,16 @@ def lib() -> ctypes.CDLL:
         L.llattn_bwd_noalloc.restype = ctypes.c_int
         L.llattn_decode.argtypes = [ctypes.POINTER(DecodeArgs), _vp]
         L.llattn_decode.restype = ctypes.c_int
+        L.llattn_xent_workspace_bytes.argtypes = [ctypes.POINTER(XentArgs)]
+        L.llattn_xent_workspace_bytes.restype = ctypes.c_size_t
+        L.llattn_xent.argtypes = [ctypes.POINTER(XentArgs), _vp]
+        L.llattn_xent.restype = ctypes.c_int
+        L.llattn_scale.argtypes = [_vp, ctypes.c_int64, ctypes.c_int, _vp, _vp]
+        L.llattn_scale.restype = ctypes.c_int
+        L.llattn_orth_workspace_bytes.argtypes = [ctypes.POINTER(OrthArgs)]
+        L.llattn_orth_workspace_bytes.restype = ctypes.c_size_t
+        L.llattn_orth.argtypes = [ctypes.POINTER(OrthArgs), _vp]
+        L.llattn_orth.restype = ctypes.c_int
         L.llattn_profile_enable.argtypes = [ctypes.c_int]
         L.llattn_profile_enable.restype = ctypes.c_int
         L.llattn_profile_read.argtypes = [ctypes.POINTER(ctypes.c_double),

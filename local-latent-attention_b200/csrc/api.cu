@@ -14,6 +14,7 @@
 #include "common.cuh"
 #include "profile.cuh"
 #include "sm100.cuh"
+#include "xent.cuh"
 
 namespace llattn {
 namespace {
@@ -505,7 +506,7 @@ extern "C" {
 int llattn_version(void) { return LLATTN_VERSION; }
 
 unsigned llattn_fault_status(int reset) {
-  unsigned v = sm100::read_fault_word(reset != 0);
+  unsigned v = sm100::read_fault_word(reset != 0) | xent::read_fault_word(reset != 0) | orth::read_fault_word(reset != 0);
   volatile unsigned* w = fault_host_word();
   if (w) {
     v |= *w;
@@ -688,6 +689,82 @@ int llattn_bwd(const llattn_bwd_args* a, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dims.dtype == LLATTN_BF16) return run_bwd<bf16>(g, a, s);
   return run_bwd<float>(g, a, s);
+}
+
+static int check_xent(const llattn_xent_args* a) {
+  if (!a) return fail(LLATTN_ERR_ARG, "args is NULL");
+  if (a->tokens < 1 || a->d < 1 || a->vocab < 1)
+    return fail(LLATTN_ERR_ARG, "xent: tokens, d and vocab must be >= 1");
+  if (a->d > (1 << 20) || a->vocab > (1 << 21))
+    return fail(LLATTN_ERR_ARG, "xent: d %d or vocab %d too large", a->d, a->vocab);
+  if (a->dtype != LLATTN_F32 && a->dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", a->dtype);
+  if (a->reduction < LLATTN_XENT_NONE || a->reduction > LLATTN_XENT_SUM)
+    return fail(LLATTN_ERR_ARG, "xent: unknown reduction %d", a->reduction);
+  if (a->ldx < a->d || a->ldw < a->d)
+    return fail(LLATTN_ERR_ARG, "xent: row strides (%lld, %lld) below d = %d", (long long)a->ldx, (long long)a->ldw, a->d);
+  return LLATTN_OK;
+}
+
+size_t llattn_xent_workspace_bytes(const llattn_xent_args* a) { return check_xent(a) ? 0 : xent::workspace_bytes(*a); }
+
+int llattn_xent(const llattn_xent_args* a, void* stream) {
+  int rc = check_xent(a);
+  if (rc) return rc;
+  if (!a->x || !a->w || !a->targets) return fail(LLATTN_ERR_ARG, "llattn_xent: NULL pointer in args");
+  const bool grads = a->dx || a->dw;
+  if (!grads && !a->losses && !a->loss) return fail(LLATTN_ERR_ARG, "llattn_xent: no output asked for");
+  if (grads && a->losses) return fail(LLATTN_ERR_ARG, "llattn_xent: losses are written without gradients only");
+  if (a->loss && a->reduction == LLATTN_XENT_NONE)
+    return fail(LLATTN_ERR_ARG, "llattn_xent: reduction none has no scalar loss");
+  if (grads && (a->reduction == LLATTN_XENT_NONE) != (a->grad_rows != nullptr))
+    return fail(LLATTN_ERR_ARG, "llattn_xent: grad_rows goes with reduction none");
+  const size_t need = xent::workspace_bytes(*a);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(LLATTN_ERR_WORKSPACE, "llattn_xent: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
+  if (!al(a->workspace, 256)) return fail(LLATTN_ERR_ALIGN, "llattn_xent: workspace must be 256-byte aligned");
+  Geom g;
+  if ((rc = fault_gate(&g))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prof::Scope ps(prof::XENT, s, xent::launches(*a));
+  return check_launch(xent::launch(*a, g.fault_host, s), "xent");
+}
+
+int llattn_scale(void* buf, int64_t n, int dtype, const float* factor, void* stream) {
+  if (!buf || !factor || n < 1) return fail(LLATTN_ERR_ARG, "scale: NULL pointer or n < 1");
+  if (dtype != LLATTN_F32 && dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", dtype);
+  return check_launch(xent::launch_scale(buf, n, dtype, factor, static_cast<cudaStream_t>(stream)), "scale");
+}
+
+static int check_orth(const llattn_orth_args* a) {
+  if (!a) return fail(LLATTN_ERR_ARG, "args is NULL");
+  if (a->rows < 1 || a->cols < 1 || a->count < 1) return fail(LLATTN_ERR_ARG, "orth: rows, cols and count must be >= 1");
+  if (a->rows > (1 << 20) || a->cols > (1 << 20) || a->count > (1 << 16))
+    return fail(LLATTN_ERR_ARG, "orth: %d x %d x %d too large", a->count, a->rows, a->cols);
+  if (a->steps < 1 || a->steps > 64) return fail(LLATTN_ERR_ARG, "orth: steps %d outside [1, 64]", a->steps);
+  if (a->dtype != LLATTN_F32 && a->dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", a->dtype);
+  if (!(fabsf(a->a) <= 16.f) || !(fabsf(a->b) <= 16.f) || !(fabsf(a->c) <= 16.f))
+    return fail(LLATTN_ERR_ARG, "orth: coefficients (%g, %g, %g) outside [-16, 16]", a->a, a->b, a->c);
+  if (!(a->eps >= 0.f)) return fail(LLATTN_ERR_ARG, "orth: eps must be >= 0");
+  return LLATTN_OK;
+}
+
+size_t llattn_orth_workspace_bytes(const llattn_orth_args* a) { return check_orth(a) ? 0 : orth::workspace_bytes(*a); }
+
+int llattn_orth(const llattn_orth_args* a, void* stream) {
+  int rc = check_orth(a);
+  if (rc) return rc;
+  if (!a->g || !a->out) return fail(LLATTN_ERR_ARG, "llattn_orth: NULL pointer in args");
+  for (int i = 0; i < a->count; ++i)
+    if (!a->g[i]) return fail(LLATTN_ERR_ARG, "llattn_orth: matrix %d is NULL", i);
+  const size_t need = orth::workspace_bytes(*a);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(LLATTN_ERR_WORKSPACE, "llattn_orth: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
+  if (!al(a->workspace, 256)) return fail(LLATTN_ERR_ALIGN, "llattn_orth: workspace must be 256-byte aligned");
+  Geom g;
+  if ((rc = fault_gate(&g))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prof::Scope ps(prof::ORTH, s, orth::launches(*a));
+  return check_launch(orth::launch(*a, g.fault_host, s), "orth");
 }
 
 // ---------------------------------------------------------------------------

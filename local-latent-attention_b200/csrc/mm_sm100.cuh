@@ -1,0 +1,463 @@
+// Persistent tensor-core product of the training operators (included by
+// xent.cu and orth.cu): C[M, N] = A[M, K] B[N, K]^T per batch element z, 16-bit
+// operands (both bf16 or both fp16), fp32 accumulation in TMEM, and an
+// epilogue functor that consumes the accumulator rows in registers.
+//
+// Each operand is K-major (stored [MN, K], K contiguous) or MN-major (stored
+// [K, MN]); tensor maps are 3-D (contiguous, rows, z) with 128-byte-swizzled
+// boxes of 64 x 128 (K-major) or 64 x 64 (MN-major, two panels per 128
+// rows); out-of-range rows, columns and K are zero-filled by the copies.
+//
+// Two tile shapes: CG = 2 runs a 256 x 256 tile on a pair of CTAs (a cluster of
+// two SMs): each CTA copies its own 128 rows of A and 128 of the tile's 256
+// rows of B, the leader (cluster rank 0) issues cta_group::2 MMAs for both,
+// and each CTA ends up with its 128 rows x 256 columns of the accumulator.
+// Per K = 64 step a CTA copies 32 KB for 128 x 256 x 64 products, half the L2
+// traffic per flop of the CG = 1 tile (128 x 128 on one CTA), which small
+// products use because it spreads over more SMs. Both keep a 6-stage ring of
+// 32 KB stages that runs on across tiles and two accumulators in TMEM, so one
+// tile's epilogue overlaps the next tile's MMAs.
+//
+// Warps: 0 copies, 1 issues MMAs, the others (one per 32 rows x 128 columns of
+// the CTA's accumulator) run the epilogue: thread = row, 128 columns.
+// Every wait is bounded (mbar_wait); a CTA whose wait runs out raises the
+// fault word, which ends every other wait, and all warps still meet at the
+// final barriers.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "sm100.cuh"
+#include "sm100_ptx.cuh"
+
+namespace llattn {
+namespace mm {
+namespace {
+
+using namespace ptx;
+
+// as local_sm100.cu's fault word, for the kernels of this translation unit
+__device__ unsigned int g_mm_fault = 0;
+
+unsigned read_fault(bool reset) {
+  unsigned v = 0;
+  cudaMemcpyFromSymbol(&v, g_mm_fault, sizeof(v));
+  if (reset) {
+    const unsigned z = 0;
+    cudaMemcpyToSymbol(g_mm_fault, &z, sizeof(z));
+  }
+  return v;
+}
+
+// One product. M, N, K are the host's sizes; m_dev / k_dev (optional) hold a
+// device-side row count from which M / K are cut: max(0, min(M, *m_dev -
+// dev_base)) (the rows past it are not computed, the K past it not read
+// beyond the next multiple of 64, whose rows the caller keeps at zero).
+struct MmArgs {
+  int M, N, K;
+  int a_mn, b_mn;
+  int nz;                   // batch elements (tensor-map z), 1 for the split forms
+  int splits, k_per_split;  // K ranges (multiples of 64), each its own output
+  int sym;                  // C symmetric: tiles with n <= m only (square tiles)
+  int fp16;                 // operands fp16 instead of bf16
+  // products over planes: operand z coordinates (pa, pb) of n_terms passes
+  // over K, 4 bits each (fp32 operands split into bf16 planes)
+  int n_terms;
+  uint32_t pa, pb;
+  const int* m_dev;
+  const int* k_dev;
+  int dev_base;
+  volatile unsigned* fault_host;
+};
+
+__device__ __forceinline__ void mm_raise(const MmArgs& p, unsigned bit, volatile int* abort) {
+  atomicOr(&g_mm_fault, bit);
+  if (p.fault_host) {
+    *p.fault_host |= bit;
+    __threadfence_system();
+  }
+  *abort = 1;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrive on the barrier at the same shared-memory offset in the cluster's CTA 0
+__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+// tile copy whose bytes count on the leader's barrier (clearing the CTA-rank
+// bit of a shared::cluster address of a pair gives CTA 0's); no multicast
+__device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint64_t* bar, void* dst, int c0, int c1,
+                                                 int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar) & 0xFEFFFFFFu), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if (CG == 1) {
+    mma_bf16(d, a, b, idesc, acc);  // kind::f16; the descriptor names the type
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+// the barrier (in both CTAs of a pair) arrives when the MMAs issued so far are done
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (CG == 1) {
+    mma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void mm_tmem_alloc(uint32_t* dst, uint32_t ncols) {
+  if (CG == 1) {
+    tmem_alloc(dst, ncols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
+  if (CG == 1)
+    tmem_dealloc(t, ncols);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(ncols) : "memory");
+}
+
+template <int CG>
+struct MmShape {
+  static constexpr int BM = 128 * CG, BN = 128 * CG;  // tile of the CTA (pair)
+  static constexpr int EW = 4 * CG;                   // epilogue warps: 32 rows x 128 columns each
+  static constexpr int THREADS = 64 + 32 * EW;
+  static constexpr int ST = 6;
+  static constexpr int OPB = 128 * 64 * 2;  // one CTA's operand tile: 128 rows x 64 K, 16 KB
+  static constexpr int A = 0, B = A + ST * OPB, BAR = B + ST * OPB;
+  static constexpr int BYTES = BAR + 256;
+  static constexpr int SMEM = BYTES + 1024;  // + alignment
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+// work item -> (z or split, first row, first column)
+struct MmTile {
+  int z, m0, n0;
+};
+
+template <int CG>
+struct MmGrid {
+  int n_mt, n_nt, per_z, total;
+  __device__ __forceinline__ MmGrid(const MmArgs& p, int M) {
+    n_mt = cdiv(M, MmShape<CG>::BM);
+    n_nt = cdiv(p.N, MmShape<CG>::BN);
+    per_z = p.sym ? n_mt * (n_mt + 1) / 2 : n_mt * n_nt;
+    total = per_z * p.nz * p.splits;
+  }
+  __device__ __forceinline__ MmTile at(const MmArgs& p, int t) const {
+    MmTile r;
+    r.z = t / per_z;
+    int u = t - r.z * per_z, i, j;
+    if (p.sym) {  // row i of the lower triangle holds i + 1 tiles
+      i = (int)((sqrtf(8.f * u + 1.f) - 1.f) * 0.5f);
+      while (i * (i + 1) / 2 > u) --i;
+      while ((i + 1) * (i + 2) / 2 <= u) ++i;
+      j = u - i * (i + 1) / 2;
+    } else {
+      // bands of 8 row tiles, walked column by column: the tiles in flight
+      // share about 8 row and 9 column strips of the operands in L2
+      const int band = 8 * n_nt, bi = u / band, v = u - bi * band;
+      const int h = min(8, n_mt - bi * 8);
+      j = v / h;
+      i = bi * 8 + (v - j * h);
+    }
+    r.m0 = i * MmShape<CG>::BM;
+    r.n0 = j * MmShape<CG>::BN;
+    return r;
+  }
+};
+
+__device__ __forceinline__ int cut_rows(int n, const int* dev, int base) {
+  if (!dev) return n;
+  const int v = *dev - base;
+  return v < 0 ? 0 : (v < n ? v : n);
+}
+
+// Epi: struct with
+//   __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero) const
+// called by every thread of an epilogue warp (all 32 lanes, converged) for its
+// row and 128 columns [col0, col0 + 128); taddr: TMEM address of the warp's
+// lanes and columns; zero: the K range is empty, the accumulator holds nothing.
+template <int CG, typename Epi>
+__global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
+    mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+              const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
+  using S = MmShape<CG>;
+  constexpr int ST = S::ST;
+  extern __shared__ uint8_t mm_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR);
+  uint64_t *full = bars, *empty = bars + ST, *acc_full = bars + 2 * ST, *acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = CG == 2 ? (int)cluster_rank() : 0;
+  const int unit = blockIdx.x / CG, n_units = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], CG * S::EW);
+    }
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    mm_tmem_alloc<CG>(tmem_slot, 2 * S::BN);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // the peer's barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // accumulator b at columns [b * BN, (b + 1) * BN)
+
+  const int M = cut_rows(p.M, p.m_dev, p.dev_base);
+  const int K = cut_rows(p.K, p.k_dev, p.dev_base);
+  const MmGrid<CG> grid(p, M);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm_a);
+      prefetch_tmap(&tm_b);
+      int it = 0;
+      bool ok = true;
+      for (int t = unit; ok && t < grid.total; t += n_units) {
+        const MmTile w = grid.at(p, t);
+        const int k0 = p.splits > 1 ? w.z * p.k_per_split : 0;
+        const int k1 = p.splits > 1 ? min(K, k0 + p.k_per_split) : K;
+        const int zc = p.splits > 1 ? 0 : w.z;
+        const int ma = w.m0 + rank * 128, nb = w.n0 + rank * 128;
+        for (int term = 0; ok && term < p.n_terms; ++term) {
+          const int za = zc + (int)((p.pa >> (4 * term)) & 15u), zb = zc + (int)((p.pb >> (4 * term)) & 15u);
+          for (int k = k0; k < k1; k += 64, ++it) {
+            const int s = it % ST;
+            if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * CG * S::OPB);
+            uint8_t* sa = smem + S::A + s * S::OPB;
+            uint8_t* sb = smem + S::B + s * S::OPB;
+            auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
+              if (CG == 1)
+                tma_load_3d(map, &full[s], dst, c0, c1, c2);
+              else
+                tma_load_3d_pair(map, &full[s], dst, c0, c1, c2);
+            };
+            if (p.a_mn) {
+              load(&tm_a, sa, ma, k, za);
+              load(&tm_a, sa + S::OPB / 2, ma + 64, k, za);
+            } else {
+              load(&tm_a, sa, k, ma, za);
+            }
+            if (p.b_mn) {
+              load(&tm_b, sb, nb, k, zb);
+              load(&tm_b, sb + S::OPB / 2, nb + 64, k, zb);
+            } else {
+              load(&tm_b, sb, k, nb, zb);
+            }
+          }
+        }
+      }
+      // every stage's last commit has arrived (in a pair, on this CTA's
+      // barrier too): none is in flight when the CTA exits
+      for (int i = it - ST < 0 ? 0 : it - ST; ok && i < it; ++i)
+        ok = mbar_wait(&empty[i % ST], (i / ST) & 1, abort, &g_mm_fault);
+      if (!ok) mm_raise(p, 1u, abort);
+      if (*abort && rank == 0) {  // let the copies already issued land before the CTA (pair) can exit
+        volatile int none = 0;
+        volatile unsigned gnone = 0;
+        for (int i = it - ST < 0 ? 0 : it - ST; i < it; ++i)
+          mbar_wait(&full[i % ST], (i / ST) & 1, &none, &gnone, 100000000ull);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t fmt = p.fp16 ? 0u : 1u;
+      const uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | ((p.a_mn ? 1u : 0u) << 15) |
+                          ((p.b_mn ? 1u : 0u) << 16) | ((uint32_t)(S::BN >> 3) << 17) | ((uint32_t)(S::BM >> 4) << 24);
+      // K-major: a K step of 16 is 32 bytes of the 128-byte rows; MN-major: 16
+      // rows of 128 bytes, panels of 64 rows (MN) 8 KB apart
+      const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+      const uint32_t a_lbo = p.a_mn ? S::OPB / 2 : 16, b_lbo = p.b_mn ? S::OPB / 2 : 16;
+      int it = 0, k = 0;
+      bool ok = true;
+      for (int t = unit; ok && t < grid.total; t += n_units, ++k) {
+        const int z = grid.at(p, t).z, buf = k & 1;
+        const int k0 = p.splits > 1 ? z * p.k_per_split : 0;
+        const int k1 = p.splits > 1 ? min(K, k0 + p.k_per_split) : K;
+        const int steps = k1 > k0 ? cdiv(k1 - k0, 64) * p.n_terms : 0;
+        // the epilogue has read this accumulator's previous tile (k - 2)
+        if (k >= 2 && !(ok = mbar_wait(&acc_empty[buf], ((k >> 1) - 1) & 1, abort, &g_mm_fault))) break;
+        tc_fence_after();
+        for (int i = 0; i < steps; ++i, ++it) {
+          const int s = it % ST;
+          if (!(ok = mbar_wait(&full[s], (it / ST) & 1, abort, &g_mm_fault))) break;
+          tc_fence_after();
+          const uint64_t da = desc_sw128(smem_u32(smem + S::A + s * S::OPB), a_lbo, 1024);
+          const uint64_t db = desc_sw128(smem_u32(smem + S::B + s * S::OPB), b_lbo, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16<CG>(tmem + S::BN * buf, desc_add(da, kk * a_step), desc_add(db, kk * b_step), id,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+          commit<CG>(&empty[s]);
+        }
+        if (!ok) break;
+        commit<CG>(&acc_full[buf]);
+      }
+      if (!ok) mm_raise(p, 2u, abort);
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns 128 half..
+    int k = 0;
+    bool ok = true;
+    for (int t = unit; t < grid.total; t += n_units, ++k) {
+      const int buf = k & 1;
+      const MmTile w = grid.at(p, t);
+      const int k0 = p.splits > 1 ? w.z * p.k_per_split : 0;
+      const int k1 = p.splits > 1 ? min(K, k0 + p.k_per_split) : K;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (k >> 1) & 1, abort, &g_mm_fault));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t ta = tmem + S::BN * buf + 128 * half + ((uint32_t)(32 * quad) << 16);
+      epi.tile(p, w, w.m0 + rank * 128 + 32 * quad + lane, w.n0 + 128 * half, M, ta, k1 <= k0);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {  // this accumulator may take the tile after next
+        if (CG == 1)
+          mbar_arrive(&acc_empty[buf]);
+        else
+          mbar_arrive_leader(&acc_empty[buf]);
+      }
+    }
+    if (!ok) mm_raise(p, 8u, abort);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // the peer reads this CTA's shared memory and arrives on its barriers until here
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    mm_tmem_dealloc<CG>(tmem, 2 * S::BN);
+  }
+}
+
+// 32 accumulator columns of this thread's row
+__device__ __forceinline__ void load32(uint32_t taddr, bool zero, float (&v)[32]) {
+  uint32_t r[32];
+  if (!zero) {
+    tmem_ld32(taddr, r);
+    tmem_ld_wait();
+  }
+#pragma unroll
+  for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : __uint_as_float(r[q]);
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- host side --------------------------------------------------------------
+
+// 3-D operand view: rows x cols with cols contiguous, row stride ld and z
+// stride zs (elements, multiples of 8; 16-byte aligned base)
+struct Operand {
+  const void* p;
+  int64_t rows, cols, ld, nz, zs;
+  int mn;  // stored MN-major (rows = K, cols = MN) instead of K-major (rows = MN, cols = K)
+};
+
+// Which tile: the pair's 256 x 256 tile takes about twice a single 128 x 128
+// tile's time on twice the SMs, so the shorter schedule in tile times wins.
+inline int pick_group(const MmArgs& p) {
+  auto tiles = [&](int b) {
+    const int64_t m = cdiv(p.M, b), n = cdiv(p.N, b);
+    return (p.sym ? m * (m + 1) / 2 : m * n) * p.nz * p.splits;
+  };
+  const int sms = sm_count();
+  const double t1 = (double)((tiles(128) + sms - 1) / sms) * 1.25;
+  const double t2 = (double)((tiles(256) + sms / 2 - 1) / (sms / 2)) * 2.0;
+  return t2 <= t1 ? 2 : 1;
+}
+
+template <int CG, typename Epi>
+cudaError_t launch_mm_cg(const MmArgs& p, const CUtensorMap& ta, const CUtensorMap& tb, const Epi& epi,
+                         cudaStream_t s) {
+  using S = MmShape<CG>;
+  cudaError_t e = set_smem_once(mm_kernel<CG, Epi>, S::SMEM);
+  if (e != cudaSuccess) return e;
+  const int64_t m = cdiv(p.M, S::BM), n = cdiv(p.N, S::BN);
+  const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz * p.splits;
+  if (tiles < 1) return cudaSuccess;
+  if (tiles > 0x3fffffff) return cudaErrorInvalidValue;
+  const int64_t units = std::min<int64_t>(tiles, sm_count() / CG);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * CG));
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {CG, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, mm_kernel<CG, Epi>, ta, tb, p, epi);
+}
+
+template <typename Epi>
+cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
+  CUtensorMap ta, tb;
+  p.a_mn = a.mn;
+  p.b_mn = b.mn;
+  if (p.splits < 1) p.splits = 1;
+  if (p.nz < 1) p.nz = 1;
+  if (p.n_terms < 1) p.n_terms = 1;
+  if (p.M < 1 || p.N < 1 || p.K < 1) return cudaErrorInvalidValue;
+  if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
+      !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : 128))
+    return cudaErrorInvalidValue;
+  return pick_group(p) == 2 ? launch_mm_cg<2>(p, ta, tb, epi, s) : launch_mm_cg<1>(p, ta, tb, epi, s);
+}
+
+}  // namespace
+}  // namespace mm
+}  // namespace llattn

@@ -1,0 +1,666 @@
+// Orthogonalised updates by Newton-Schulz products: for each matrix G of a
+// batch (short side q = min(m, n); written for the short side first)
+//   X0 = G / (|G|_F + eps),  S = X X^T,  B = b S + c S^2,  X <- a X + B X
+// repeated `steps` times, which drives every singular value of X towards 1.
+// (No counterpart in the reference, whose training uses AdamW.)
+//
+// Three products per step on mm_kernel (mm_sm100.cuh) with 16-bit operands
+// and fp32 accumulation. A tall matrix keeps its orientation: S = X^T X reads
+// X with the columns as rows (MN-major), and the update is X B. S and B are
+// symmetric: only tiles on and below the diagonal are computed, the epilogue
+// writes each one's mirror image as well.
+//
+// 16 bits: fp16, whose 11 bits cost the same as bf16's 8; values are kept in
+// its range by powers of two: X * 2^6, S * 2^8 and B * 2^8 (entries of X and S
+// are at most about 1.2, those of B at most |b| + |c| times that). The
+// starting X is G times a power of two near 2^6 / |G| (exact for bf16 G), the
+// rest of the normalisation is a factor s0 in the first step's epilogues.
+//
+// Two roundings matter and are compensated:
+//  * a X: early steps multiply the smallest singular values by a = 3.4 each
+//    time, and the rounding of X with them. The update's linear term reads X
+//    as hi + lo (fp16 and the remainder in bf16); only the products use hi,
+//    where small singular values enter cubed.
+//  * B near the end is close to (b + c) I, and a X + B X cancels to about
+//    (a + b + c) X: rounding B would cost 4 times its 2^-12. The last two
+//    steps therefore hold B + k I with k = -(b + c), near 0, and use
+//    (a - k) X; there hi alone feeds the linear term.
+// Measured on the CPU in the same arithmetic: 0.4 to 1.5e-3 (2-norm) from the
+// exact iteration over spectra from flat to 1 / k, where plain bf16 products
+// give 1 to 4e-2.
+#include <cooperative_groups.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "mm_sm100.cuh"
+#include "xent.cuh"
+
+namespace llattn {
+namespace orth {
+namespace {
+
+using namespace mm;
+
+constexpr float kX = 64.f, kS = 256.f;  // scales of X and of S, B
+constexpr int kCompensated = 2;         // last steps that hold B + k I
+constexpr int kParts = 64;              // partial sums of squares per matrix
+constexpr int kPtrs = 64;               // matrices per conversion launch
+
+struct Ptrs {
+  const void* p[kPtrs];
+};
+
+__device__ __forceinline__ int64_t at2(int64_t z, int64_t zs, int64_t row, int64_t ld) { return z * zs + row * ld; }
+
+// stores 32 fp16 of one row; ld and the column are multiples of 8 where full
+__device__ __forceinline__ void store_half32(__half* dst, const float (&v)[32], int n) {
+  if (n >= 32) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      reinterpret_cast<uint4*>(dst)[q] =
+          make_uint4(pack_half(v[8 * q], v[8 * q + 1]), pack_half(v[8 * q + 2], v[8 * q + 3]),
+                     pack_half(v[8 * q + 4], v[8 * q + 5]), pack_half(v[8 * q + 6], v[8 * q + 7]));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q)
+      if (q < n) dst[q] = __float2half_rn(v[q]);
+  }
+}
+__device__ __forceinline__ void load_half32(const __half* src, float (&v)[32], int n) {
+  if (n >= 32) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 u = reinterpret_cast<const uint4*>(src)[q];
+      const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h[i]);
+        v[8 * q + 2 * i] = f.x;
+        v[8 * q + 2 * i + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = q < n ? __half2float(src[q]) : 0.f;
+  }
+}
+
+// mirror image of 32 columns of a row: element (row, nc + q) -> (nc + q, row);
+// the warp's 32 rows are consecutive, so each q is one 64-byte segment
+__device__ __forceinline__ void store_mirror(__half* base, int64_t ld, int row, int nc, const float (&v)[32], int n) {
+#pragma unroll
+  for (int q = 0; q < 32; ++q)
+    if (q < n) base[(int64_t)(nc + q) * ld + row] = __float2half_rn(v[q]);
+}
+
+// S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
+struct EpiGram {
+  __half* s;
+  int64_t ld, zs;
+  const float* s0;  // first step: X = s0[z] * stored, else null (2^-6)
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
+                                       bool zero) const {
+    const float x = s0 ? s0[w.z] : 1.f / kX;
+    const float f = x * x * kS;
+    __half* base = s + w.z * zs;
+#pragma unroll 1
+    for (int cc = 0; cc < 128; cc += 32) {
+      const int nc = col0 + cc;
+      if (nc >= a.N) break;
+      float v[32];
+      load32(taddr + cc, zero, v);
+      if (row >= M) continue;
+#pragma unroll
+      for (int q = 0; q < 32; ++q) v[q] *= f;
+      store_half32(base + row * ld + nc, v, a.N - nc);
+      if (w.m0 != w.n0) store_mirror(base, ld, row, nc, v, a.N - nc);
+    }
+  }
+};
+
+// B = b S + c S^2 + k I (scaled by kS)
+struct EpiPoly {
+  const __half* s;
+  __half* b;
+  int64_t ld, zs;
+  float cb, cc2, k;  // b, c / kS, k * kS
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
+                                       bool zero) const {
+    __half* base = b + w.z * zs;
+#pragma unroll 1
+    for (int cc = 0; cc < 128; cc += 32) {
+      const int nc = col0 + cc;
+      if (nc >= a.N) break;
+      float v[32], x[32];
+      load32(taddr + cc, zero, v);
+      if (row >= M) continue;
+      load_half32(s + w.z * zs + row * ld + nc, x, a.N - nc);
+#pragma unroll
+      for (int q = 0; q < 32; ++q) v[q] = fmaf(cb, x[q], cc2 * v[q]) + (row == nc + q ? k : 0.f);
+      store_half32(base + row * ld + nc, v, a.N - nc);
+      if (w.m0 != w.n0) store_mirror(base, ld, row, nc, v, a.N - nc);
+    }
+  }
+};
+
+// X <- (a - k) X + (B + k I) X
+struct EpiUpdate {
+  const __half* hi;
+  bf16* lo;          // remainder of X, read where rd_lo, written (in place) where wr_lo
+  __half* next;      // next X (hi), or null in the last step
+  bf16* out;         // last step: [count, rows, cols]
+  int64_t ld, zs, ldo, zso;
+  const float* s0;
+  float ca;          // a - k
+  int rd_lo, wr_lo, vec_out;
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
+                                       bool zero) const {
+    const float x = s0 ? s0[w.z] : 1.f / kX;
+    const float fl = ca * x, fp = x / kS;
+#pragma unroll 1
+    for (int cc = 0; cc < 128; cc += 32) {
+      const int nc = col0 + cc;
+      if (nc >= a.N) break;
+      float v[32], h[32];
+      load32(taddr + cc, zero, v);
+      if (row >= M) continue;
+      const int n = a.N - nc;
+      const int64_t at = at2(w.z, zs, row, ld) + nc;
+      load_half32(hi + at, h, n);
+      if (rd_lo) {
+        if (n >= 32) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float f[8];
+            unpack8(reinterpret_cast<const uint4*>(lo + at)[q], f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[8 * q + i] += f[i];
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (q < n) h[q] += __bfloat162float(lo[at + q]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 32; ++q) v[q] = fmaf(fl, h[q], fp * v[q]);
+      if (out) {
+        bf16* dst = out + at2(w.z, zso, row, ldo) + nc;
+        if (vec_out && n >= 32) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            reinterpret_cast<uint4*>(dst)[q] =
+                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (q < n) dst[q] = __float2bfloat16_rn(v[q]);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int q = 0; q < 32; ++q) v[q] *= kX;
+      store_half32(next + at, v, n);
+      if (wr_lo) {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] -= __half2float(__float2half_rn(v[q]));
+        if (n >= 32) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            reinterpret_cast<uint4*>(lo + at)[q] =
+                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (q < n) lo[at + q] = __float2bfloat16_rn(v[q]);
+        }
+      }
+    }
+  }
+};
+
+// partial sums of squares of matrix blockIdx.y, fixed order
+template <typename T>
+__global__ void __launch_bounds__(256) orth_square(const __grid_constant__ Ptrs g, int64_t n, float* __restrict__ part) {
+  __shared__ float red[8];
+  const T* src = static_cast<const T*>(g.p[blockIdx.y]);
+  float s = 0.f;
+  constexpr int VN = 16 / sizeof(T);
+  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    const int64_t nv = n / VN;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nv; i += (int64_t)gridDim.x * 256) {
+      const uint4 u = reinterpret_cast<const uint4*>(src)[i];
+      if (sizeof(T) == 2) {
+        float f[8];
+        unpack8(u, f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s = fmaf(f[q], f[q], s);
+      } else {
+        const float x = __uint_as_float(u.x), y = __uint_as_float(u.y), z = __uint_as_float(u.z),
+                    t = __uint_as_float(u.w);
+        s = fmaf(x, x, fmaf(y, y, fmaf(z, z, fmaf(t, t, s))));
+      }
+    }
+    if (blockIdx.x == 0 && threadIdx.x < n - nv * VN) {
+      const float x = to_f<T>(src[nv * VN + threadIdx.x]);
+      s = fmaf(x, x, s);
+    }
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+      const float x = to_f<T>(src[i]);
+      s = fmaf(x, x, s);
+    }
+  }
+  s = warp_sum(s);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float r = 0.f;
+    for (int i = 0; i < 8; ++i) r += red[i];
+    part[blockIdx.y * kParts + blockIdx.x] = r;
+  }
+}
+
+// hi = fp16(G 2^e), lo = bf16(G 2^e - hi) (optional), s0 = 2^-e / (|G| + eps)
+template <typename T>
+__global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs g, int rows, int cols,
+                                                    const float* __restrict__ part, int n_parts, float eps,
+                                                    __half* __restrict__ hi, bf16* __restrict__ lo, int64_t ld, int64_t zs,
+                                                    float* __restrict__ s0) {
+  __shared__ float sh[2];
+  const int z = blockIdx.y;
+  if (threadIdx.x == 0) {
+    float sum = 0.f;
+    for (int i = 0; i < n_parts; ++i) sum += part[z * kParts + i];
+    const float inv = 1.f / (sqrtf(sum) + eps);
+    // inv = 0 (the sum overflowed) or NaN: straight through, X = G * inv
+    const bool fine = inv > 0.f && inv < INFINITY;
+    const int e = fine ? min(120, max(-120, ilogbf(inv * kX))) : 0;
+    sh[0] = fine ? ldexpf(1.f, e) : inv;
+    sh[1] = fine ? inv * ldexpf(1.f, -e) : 1.f;
+    if (blockIdx.x == 0) s0[z] = sh[1];
+  }
+  __syncthreads();
+  const float f = sh[0];
+  const T* src = static_cast<const T*>(g.p[z]);
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* r = src + (int64_t)row * cols;
+    __half* h = hi + z * zs + row * ld;
+    bf16* l = lo ? lo + z * zs + row * ld : nullptr;
+    for (int c = threadIdx.x; c < cols; c += 256) {
+      const float v = to_f<T>(r[c]) * f;
+      const __half q = __float2half_rn(v);
+      h[c] = q;
+      if (l) l[c] = __float2bfloat16_rn(v - __half2float(q));
+    }
+  }
+}
+
+// ---- small matrices ---------------------------------------------------------
+// q <= 64: the whole iteration in one launch, in fp32 on the CUDA cores. A
+// cluster of CL CTAs holds one matrix, each CTA a slice of its long side in
+// shared memory as x [q][slice]; per step each CTA takes its slice's part of
+// S, the parts are summed over the cluster's shared memory (fixed order), every
+// CTA forms B for itself and updates its slice. Rows are interleaved over the
+// threads (row = ti + R r) and padded to 4 mod 32 floats, so the 16-byte
+// shared-memory loads of a quarter warp meet all 32 banks.
+constexpr int kSmallQ = 64, kSmallT = 256;
+
+struct SmallShape {
+  int q, R, w, wp, bp;  // short side, row quads, slice, padded slice, padded q
+  __host__ __device__ SmallShape(int q_, int L, int CL) {
+    q = q_;
+    R = cdiv(q, 4);
+    w = cdiv(cdiv(L, CL), 4) * 4;
+    wp = cdiv(w, 32) * 32 + 4;
+    bp = cdiv(4 * R, 32) * 32 + 4;
+  }
+  // x, S, B, this CTA's part of S, group partials
+  __host__ __device__ int floats() const { return 4 * R * (wp + 3 * bp) + kSmallT * 16; }
+};
+
+// out[i][j] (+ epilogue f) = sum_k a[i][k] a[j][k], k < w (a multiple of 4), a
+// [4R][ld]; thread groups share k, joined through part
+template <typename F>
+__device__ __forceinline__ void small_gram(const float* a, int ld, int w, int R, float* part, F f) {
+  const int n_t = R * R, groups = max(1, kSmallT / n_t);
+  const int g = threadIdx.x / n_t, u = threadIdx.x - g * n_t;
+  const bool on = g < groups;
+  const int ti = u / R, tj = u - ti * R;  // R <= 16: R * R <= 256 threads
+  uint64_t acc[4][4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[r][c] = 0;
+  if (on) {
+    for (int k = 4 * g; k < w; k += 4 * groups) {
+      ulonglong2 x[4], y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = *reinterpret_cast<const ulonglong2*>(a + (ti + R * r) * ld + k);
+        y[r] = *reinterpret_cast<const ulonglong2*>(a + (tj + R * r) * ld + k);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] = f2_fma(x[r].y, y[c].y, f2_fma(x[r].x, y[c].x, acc[r][c]));
+    }
+  }
+  __syncthreads();  // the previous readers of part are done
+  if (on) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float lo, hi;
+        f2_unpack(acc[r][c], lo, hi);
+        part[(4 * r + c) * kSmallT + threadIdx.x] = lo + hi;
+      }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 16 * n_t; e += kSmallT) {
+    const int rc = e / n_t, v = e - rc * n_t;
+    float s = 0.f;
+    for (int h = 0; h < groups; ++h) s += part[rc * kSmallT + h * n_t + v];
+    f(v / R + R * (rc / 4), v % R + R * (rc % 4), s);
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Ptrs g, int rows, int cols, int steps,
+                                                      float ca, float cb, float cc, float eps, bf16* __restrict__ out) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = cluster.num_blocks(), rank = cluster.block_rank();
+  const int z = blockIdx.x / CL;
+  const bool tall = rows > cols;
+  const int q = tall ? cols : rows, L = tall ? rows : cols;
+  const SmallShape h(q, L, CL);
+  extern __shared__ float4 orth_smem[];
+  float* x = reinterpret_cast<float*>(orth_smem);
+  float* S = x + 4 * h.R * h.wp;
+  float* B = S + 4 * h.R * h.bp;
+  float* P = B + 4 * h.R * h.bp;
+  float* part = P + 4 * h.R * h.bp;
+  __shared__ float red[8], total;
+  const int tid = threadIdx.x, j0 = rank * h.w, jn = max(0, min(h.w, L - j0));
+  const T* src = static_cast<const T*>(g.p[z]);
+
+  for (int i = tid; i < 4 * h.R * h.wp; i += kSmallT) x[i] = 0.f;
+  __syncthreads();
+  float s = 0.f;
+  if (tall) {  // rows j0.. of the matrix: consecutive memory
+    for (int64_t e = tid; e < (int64_t)jn * q; e += kSmallT) {
+      const int j = (int)(e / q), i = (int)(e - (int64_t)j * q);
+      const float v = to_f<T>(src[(int64_t)j0 * q + e]);
+      x[i * h.wp + j] = v;
+      s = fmaf(v, v, s);
+    }
+  } else {
+    for (int i = 0; i < q; ++i)
+      for (int j = tid; j < jn; j += kSmallT) {
+        const float v = to_f<T>(src[(int64_t)i * cols + j0 + j]);
+        x[i * h.wp + j] = v;
+        s = fmaf(v, v, s);
+      }
+  }
+  s = warp_sum(s);
+  if (tid % 32 == 0) red[tid / 32] = s;
+  __syncthreads();
+  if (tid == 0) {
+    float r = 0.f;
+    for (int i = 0; i < 8; ++i) r += red[i];
+    total = r;
+  }
+  cluster.sync();
+  float sum = 0.f;
+  for (int r = 0; r < CL; ++r) sum += *cluster.map_shared_rank(&total, r);
+  const float inv = 1.f / (sqrtf(sum) + eps);
+  for (int i = tid; i < 4 * h.R * h.wp; i += kSmallT) x[i] *= inv;
+  __syncthreads();
+
+  for (int step = 0; step < steps; ++step) {
+    small_gram(x, h.wp, h.w, h.R, part, [&](int i, int j, float v) { P[i * h.bp + j] = v; });
+    cluster.sync();
+    // every CTA sums its share of the quads over the cluster and gives the
+    // result to all: the next product's parts are written after this second
+    // barrier, the next S after the first one of the next step
+    for (int e = tid * CL + rank; e < 4 * h.R * h.R; e += kSmallT * CL) {
+      const int at = e / h.R * h.bp + e % h.R * 4;
+      float4 v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < CL) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(P, r) + at);
+      float4 t = v[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < CL) t = make_float4(t.x + v[r].x, t.y + v[r].y, t.z + v[r].z, t.w + v[r].w);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < CL) *reinterpret_cast<float4*>(cluster.map_shared_rank(S, r) + at) = t;
+    }
+    cluster.sync();
+    small_gram(S, h.bp, 4 * h.R, h.R, part, [&](int i, int j, float v) { B[i * h.bp + j] = fmaf(cb, S[i * h.bp + j], cc * v); });
+    // x = a x + B x, columns in chunks: every thread holds its results until the chunk has been read
+    const int strips = kSmallT / h.R, tj = tid / h.R, ti = tid - tj * h.R;
+    for (int c0 = 0; c0 < h.w; c0 += 4 * strips) {
+      const int c = c0 + 4 * tj;
+      const bool on = tj < strips && c < h.w;
+      uint64_t acc[4][2];
+      if (on) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float4 v = *reinterpret_cast<const float4*>(x + (ti + h.R * r) * h.wp + c);
+          acc[r][0] = f2_pack(ca * v.x, ca * v.y);
+          acc[r][1] = f2_pack(ca * v.z, ca * v.w);
+        }
+        for (int k = 0; k < 4 * h.R; k += 4) {
+          float4 b[4];
+          ulonglong2 y[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            b[r] = *reinterpret_cast<const float4*>(B + (ti + h.R * r) * h.bp + k);
+            y[r] = *reinterpret_cast<const ulonglong2*>(x + (k + r) * h.wp + c);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float bk[4] = {b[r].x, b[r].y, b[r].z, b[r].w};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const uint64_t d = f2_pack(bk[m], bk[m]);
+              acc[r][0] = f2_fma(d, y[m].x, acc[r][0]);
+              acc[r][1] = f2_fma(d, y[m].y, acc[r][1]);
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (on) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<ulonglong2*>(x + (ti + h.R * r) * h.wp + c) = make_ulonglong2(acc[r][0], acc[r][1]);
+      }
+    }
+    __syncthreads();
+  }
+  bf16* dst = out + (int64_t)z * rows * cols;
+  if (tall) {
+    for (int64_t e = tid; e < (int64_t)jn * q; e += kSmallT) {
+      const int j = (int)(e / q), i = (int)(e - (int64_t)j * q);
+      dst[(int64_t)j0 * q + e] = __float2bfloat16_rn(x[i * h.wp + j]);
+    }
+  } else {
+    for (int i = 0; i < q; ++i)
+      for (int j = tid; j < jn; j += kSmallT) dst[(int64_t)i * cols + j0 + j] = __float2bfloat16_rn(x[i * h.wp + j]);
+  }
+  cluster.sync();  // the others have read this CTA's parts
+}
+
+// CTAs per matrix of the one-launch form, 0 where it does not apply: up to 8,
+// at least 32 columns each
+int small_cluster(const llattn_orth_args& a) {
+  const int q = std::min(a.rows, a.cols), L = std::max(a.rows, a.cols);
+  if (q > kSmallQ) return 0;
+  int cl = 1;
+  while (cl < 8 && L > 32 * cl) cl *= 2;
+  return SmallShape(q, L, cl).floats() * 4 <= 220 * 1024 ? cl : 0;
+}
+
+template <typename T>
+cudaError_t run_small(const llattn_orth_args& a, int cl, cudaStream_t st) {
+  const int smem = SmallShape(std::min(a.rows, a.cols), std::max(a.rows, a.cols), cl).floats() * 4;
+  cudaError_t e = set_smem_once(orth_small<T>, smem);
+  if (e != cudaSuccess) return e;
+  for (int i0 = 0; i0 < a.count; i0 += kPtrs) {
+    const int cnt = std::min(kPtrs, a.count - i0);
+    Ptrs g;
+    for (int i = 0; i < cnt; ++i) g.p[i] = a.g[i0 + i];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cnt * cl));
+    cfg.blockDim = dim3(kSmallT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)cl, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, orth_small<T>, g, (int)a.rows, (int)a.cols, (int)a.steps, a.a, a.b, a.c, a.eps,
+                           static_cast<bf16*>(a.out) + (int64_t)i0 * a.rows * a.cols);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+// ---- host side ------------------------------------------------------------------
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+
+struct Plan {
+  bool tall;
+  int q, slice, n_slices;  // short side; matrices in flight
+  int64_t ldx, xz, ldb, bz;
+  size_t x0, x1, lo, s, b, part, s0, total;
+};
+
+Plan make_plan(const llattn_orth_args& a) {
+  Plan p;
+  p.tall = a.rows > a.cols;
+  p.q = std::min(a.rows, a.cols);
+  p.ldx = up8(a.cols);
+  p.xz = p.ldx * a.rows;
+  p.ldb = up8(p.q);
+  p.bz = p.ldb * p.q;
+  // a GiB of X, its remainder, S and B at a time (at least one matrix)
+  const int64_t each = 6 * p.xz + 4 * p.bz;
+  p.slice = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(a.count, kPtrs), ((int64_t)1 << 30) / each));
+  p.n_slices = cdiv(a.count, p.slice);
+  p.slice = cdiv(a.count, p.n_slices);
+  size_t off = 0;
+  auto take = [&](size_t b) { size_t o = off; off += up256(b); return o; };
+  p.x0 = take(2 * (size_t)p.slice * p.xz);
+  p.x1 = take(2 * (size_t)p.slice * p.xz);
+  p.lo = take(2 * (size_t)p.slice * p.xz);
+  p.s = take(2 * (size_t)p.slice * p.bz);
+  p.b = take(2 * (size_t)p.slice * p.bz);
+  p.part = take(sizeof(float) * (size_t)p.slice * kParts);
+  p.s0 = take(sizeof(float) * p.slice);
+  p.total = off;
+  return p;
+}
+
+#define TRY(x)                        \
+  do {                                \
+    cudaError_t e_ = (x);             \
+    if (e_ != cudaSuccess) return e_; \
+  } while (0)
+
+template <typename T>
+cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fault, cudaStream_t st) {
+  char* ws = static_cast<char*>(a.workspace);
+  __half* x[2] = {reinterpret_cast<__half*>(ws + p.x0), reinterpret_cast<__half*>(ws + p.x1)};
+  bf16* lo = reinterpret_cast<bf16*>(ws + p.lo);
+  __half* S = reinterpret_cast<__half*>(ws + p.s);
+  __half* B = reinterpret_cast<__half*>(ws + p.b);
+  float* part = reinterpret_cast<float*>(ws + p.part);
+  float* s0 = reinterpret_cast<float*>(ws + p.s0);
+  const int m = a.rows, n = a.cols;
+  for (int i0 = 0; i0 < a.count; i0 += p.slice) {
+    const int cnt = std::min(p.slice, a.count - i0);
+    Ptrs g;
+    for (int i = 0; i < cnt; ++i) g.p[i] = a.g[i0 + i];
+    const int n_parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts, (int64_t)m * n / 4096));
+    orth_square<T><<<dim3(n_parts, cnt), 256, 0, st>>>(g, (int64_t)m * n, part);
+    TRY(cudaGetLastError());
+    // steps before the compensated ones read X as hi + lo
+    const int comp0 = a.steps - kCompensated;
+    bf16* lo0 = sizeof(T) == 4 && comp0 > 0 ? lo : nullptr;
+    orth_convert<T><<<dim3(std::min(m, 4 * sm_count()), cnt), 256, 0, st>>>(g, m, n, part, n_parts, a.eps, x[0], lo0,
+                                                                            p.ldx, p.xz, s0);
+    TRY(cudaGetLastError());
+    for (int i = 0; i < a.steps; ++i) {
+      const float* sc = i ? nullptr : s0;
+      const float k = i >= comp0 ? -(a.b + a.c) : 0.f;
+      const bool last = i + 1 == a.steps;
+      const __half* X = x[i & 1];
+      MmArgs ma = {};
+      ma.fp16 = 1;
+      ma.nz = cnt;
+      ma.fault_host = fault;
+      const Operand ok{X, m, n, p.ldx, cnt, p.xz, 0}, on{X, m, n, p.ldx, cnt, p.xz, 1};
+      MmArgs gm = ma;
+      gm.M = gm.N = p.q;
+      gm.K = p.tall ? m : n;
+      gm.sym = 1;
+      const Operand& og = p.tall ? on : ok;
+      TRY(launch_mm(gm, og, og, EpiGram{S, p.ldb, p.bz, sc}, st));
+      gm.K = p.q;
+      const Operand os{S, p.q, p.q, p.ldb, cnt, p.bz, 0}, ob{B, p.q, p.q, p.ldb, cnt, p.bz, 0};
+      TRY(launch_mm(gm, os, os, EpiPoly{S, B, p.ldb, p.bz, a.b, a.c / kS, k * kS}, st));
+      MmArgs um = ma;
+      um.M = m;
+      um.N = n;
+      um.K = p.q;
+      EpiUpdate eu{};
+      eu.hi = X;
+      eu.lo = lo;
+      eu.next = x[(i + 1) & 1];
+      eu.out = last ? static_cast<bf16*>(a.out) + (int64_t)i0 * m * n : nullptr;
+      eu.ld = p.ldx;
+      eu.zs = p.xz;
+      eu.ldo = n;
+      eu.zso = (int64_t)m * n;
+      eu.s0 = sc;
+      eu.ca = a.a - k;
+      eu.rd_lo = i < comp0 && (i > 0 || lo0);
+      eu.wr_lo = i + 1 < comp0;
+      eu.vec_out = n % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
+      TRY(p.tall ? launch_mm(um, ok, ob, eu, st) : launch_mm(um, ob, on, eu, st));
+    }
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+size_t workspace_bytes(const llattn_orth_args& a) { return small_cluster(a) ? 256 : make_plan(a).total; }
+
+int launches(const llattn_orth_args& a) {
+  return small_cluster(a) ? cdiv(a.count, kPtrs) : make_plan(a).n_slices * (2 + 3 * a.steps);
+}
+
+cudaError_t launch(const llattn_orth_args& a, volatile unsigned* fault, cudaStream_t s) {
+  if (const int cl = small_cluster(a)) return a.dtype == LLATTN_F32 ? run_small<float>(a, cl, s) : run_small<bf16>(a, cl, s);
+  const Plan p = make_plan(a);
+  return a.dtype == LLATTN_F32 ? run<float>(a, p, fault, s) : run<bf16>(a, p, fault, s);
+}
+
+unsigned read_fault_word(bool reset) { return read_fault(reset); }
+
+}  // namespace orth
+}  // namespace llattn

@@ -2,6 +2,8 @@
 // activations on sm_100a. The SIMT kernels of local_simt.cu cover the rest.
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace llattn {
@@ -94,6 +96,12 @@ struct GemmOut {
 };
 cudaError_t launch_gemm(const Geom& g, int M, int N, int K, const void* A, int64_t lda, int a_mn, const void* B,
                         int64_t ldb, int b_mn, const GemmOut& o, int splits, cudaStream_t s);
+
+// 3-D map (cols, rows, z) of a 16-bit matrix batch: row stride ld, z stride zs
+// (elements, multiples of 8; 16-byte aligned base), box 64 x box_rows x 1,
+// 128-byte swizzle, zero fill out of range. Cached by its description.
+bool make_operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int64_t nz, int64_t zs,
+                      int box_rows);
 
 // Reads (and optionally clears) the device fault word of the current device:
 // bits set by a tensor-core kernel whose bounded wait ran out.

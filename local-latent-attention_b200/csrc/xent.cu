@@ -1,0 +1,707 @@
+// Softmax cross-entropy of an output projection without its [tokens,
+// vocabulary] logits, and its gradients:
+//   l[n, v] = x[n] . w[v],  loss[n] = log sum_v exp(l[n, v]) - l[n, t(n)]
+//   G[n, v] = g(n) (exp(l[n, v]) / sum_v' exp(l[n, v']) - [v == t(n)])
+//   dx = G w,  dw = G^T x
+// (the head and loss of models.py:505-518 and train.py's F.cross_entropy;
+// the reference materialises the fp32 logits).
+//
+// All three products run on mm_kernel (mm_sm100.cuh). The logits never leave
+// the chip: the first product's epilogue turns each row's 128-column tile
+// into exponentials against the tile's own maximum m, keeps (m, sum) per
+// (row, tile), and, when gradients are wanted, stores the exponentials of a
+// bounded piece of the tokens as fp16 scaled by 2^15: relative to the tile's
+// maximum every stored value above 2^-29 keeps 11 bits, so the later
+// normalisation is the only 8-bit rounding G goes through. xent_rows then
+// joins the tiles' (m, sum) to the row's logsumexp and rewrites the
+// piece in place as bf16 G, which the other two products read. One pass over
+// the exponentials (4 bytes per element) replaces a second 2 N V d product.
+//
+// Gradients run over the tokens that count only: xent_compact lists them (in
+// order), the sizes of the products follow the device-side count, and rows
+// of ignored tokens are never read, so their values cannot reach dw.
+//
+// fp32: x, w and G are split into three bf16 planes each (24 bits) and every
+// product sums the six plane products above 2^-24, smallest first.
+#include <math.h>
+
+#include <algorithm>
+
+#include "mm_sm100.cuh"
+#include "xent.cuh"
+
+namespace llattn {
+namespace xent {
+namespace {
+
+using namespace mm;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kTile = 128;  // columns per (max, sum) statistic
+constexpr int kF32Chain = 1024;  // products per tensor-core sum of the fp32 gradients
+
+// six plane products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u;
+
+// ---- first product: statistics and exponentials ----------------------------
+
+struct EpiStats {
+  float2* stats;       // [rows][n_tiles]: (max, sum of exp(l - max))
+  int n_tiles;
+  const int* tgt;      // [rows] target of row (dev_base already added); < 0: none
+  const int64_t* tgt64;
+  float* lt;           // [rows] target logit
+  void* p;             // exponentials of the rows, or null
+  int64_t ldp;
+  int p_f32;           // fp32 instead of fp16 * 2^15
+
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
+                                       bool zero) const {
+    const int nv = min(kTile, a.N - col0);  // columns of this tile
+    if (nv <= 0) return;                    // warp-uniform
+    const bool row_ok = row < M;
+    int t = -1;
+    if (row_ok) t = tgt ? tgt[row] : (int)max((int64_t)-1, min(tgt64[row], (int64_t)a.N));
+    t -= col0;
+    float m = -INFINITY;
+    float tv = 0.f;
+#pragma unroll 1
+    for (int cc = 0; cc < nv; cc += 32) {
+      float v[32];
+      load32(taddr + cc, zero, v);
+      if (cc + 32 <= nv) {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) m = fmaxf(m, v[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) m = cc + q < nv ? fmaxf(m, v[q]) : m;
+      }
+      if ((unsigned)(t - cc) < 32u) {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) tv = q == t - cc ? v[q] : tv;
+      }
+    }
+    // fmaxf drops NaN: a row of NaN leaves m at -inf, and the sums below carry it
+    // (the maximum itself gives exactly 1: a difference, not a fused product)
+    const float mm = m == -INFINITY ? 0.f : m;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+    for (int cc = 0; cc < nv; cc += 32) {
+      float v[32];
+      load32(taddr + cc, zero, v);
+#pragma unroll
+      for (int q = 0; q < 32; ++q) v[q] = cc + q < nv ? fast_exp2((v[q] - mm) * kLog2e) : 0.f;
+#pragma unroll
+      for (int q = 0; q < 32; q += 2) {
+        s0 += v[q];
+        s1 += v[q + 1];
+      }
+      if (p && row_ok) {
+        const int64_t at = (int64_t)row * ldp + col0 + cc;
+        if (p_f32) {
+          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+          const int n4 = min(8, (nv - cc + 3) / 4);  // ldp is a multiple of 8
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (q < n4) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p) + at);
+          const int n8 = min(4, (nv - cc + 7) / 8);
+          const float k = 32768.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < n8)
+              dst[q] = make_uint4(pack_half(v[8 * q] * k, v[8 * q + 1] * k), pack_half(v[8 * q + 2] * k, v[8 * q + 3] * k),
+                                  pack_half(v[8 * q + 4] * k, v[8 * q + 5] * k),
+                                  pack_half(v[8 * q + 6] * k, v[8 * q + 7] * k));
+        }
+      }
+    }
+    if (row_ok) {
+      // every column -inf: nothing to add
+      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && !(s0 + s1 > 0.f) && !isnan(s0 + s1) ? -INFINITY : mm, s0 + s1);
+      if ((unsigned)t < (unsigned)nv) lt[row] = tv;
+    }
+  }
+};
+
+// ---- second and third product: rows out --------------------------------------
+
+struct EpiOut {
+  void* out;
+  int64_t ldo;
+  int out_bf16;
+  int vec;              // 16-byte stores: base and row stride aligned
+  const float* acc;     // added first (fp32, row stride ldacc), or null
+  int64_t ldacc;
+  const int* idx;       // output row of row m, or null
+  int64_t split_stride;
+
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
+                                       bool zero) const {
+    const bool row_ok = row < M;
+    const int64_t orow = row_ok ? (idx ? idx[row] : row) : 0;
+#pragma unroll 1
+    for (int cc = 0; cc < 128; cc += 32) {
+      const int nc = col0 + cc;
+      if (nc >= a.N) break;  // warp-uniform
+      float v[32];
+      load32(taddr + cc, zero, v);
+      if (!row_ok) continue;
+      const bool full = vec && nc + 32 <= a.N;
+      if (acc) {
+        const float* src = acc + (int64_t)row * ldacc + nc;  // ldacc a multiple of 4
+        if (nc + 32 <= a.N) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 c = reinterpret_cast<const float4*>(src)[q];
+            v[4 * q] += c.x;
+            v[4 * q + 1] += c.y;
+            v[4 * q + 2] += c.z;
+            v[4 * q + 3] += c.w;
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (nc + q < a.N) v[q] += src[q];
+        }
+      }
+      if (out_bf16) {
+        bf16* dst = static_cast<bf16*>(out) + (a.splits > 1 ? w.z * split_stride : 0) + orow * ldo + nc;
+        if (full) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            reinterpret_cast<uint4*>(dst)[q] =
+                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (nc + q < a.N) dst[q] = __float2bfloat16_rn(v[q]);
+        }
+      } else {
+        float* dst = static_cast<float*>(out) + (a.splits > 1 ? w.z * split_stride : 0) + orow * ldo + nc;
+        if (full) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            reinterpret_cast<float4*>(dst)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (nc + q < a.N) dst[q] = v[q];
+        }
+      }
+    }
+  }
+};
+
+// ---- small kernels ------------------------------------------------------------
+
+template <int NT>
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = warp_max(v);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  float r = red[0];
+#pragma unroll
+  for (int i = 1; i < NT / 32; ++i) r = fmaxf(r, red[i]);
+  return r;
+}
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = warp_sum(v);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  float r = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) r += red[i];
+  return r;
+}
+
+// The tokens that count, in order: idx[j] = row of the j-th, tgt[j] = its
+// target (-1: out of range, which makes the row's loss and gradients NaN);
+// count. lt[j] starts at NaN for the same reason. One CTA.
+__global__ void __launch_bounds__(1024) xent_compact(const int64_t* __restrict__ targets, int n, int64_t ignore, int vocab,
+                                                     int* __restrict__ idx, int* __restrict__ tgt,
+                                                     float* __restrict__ lt, int* __restrict__ count) {
+  __shared__ int sums[32];
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += 1024) {
+    const int i = i0 + tid;
+    const int64_t t = i < n ? targets[i] : ignore;
+    const bool keep = t != ignore;
+    const unsigned b = __ballot_sync(0xffffffffu, keep);
+    if (lane == 0) sums[warp] = __popc(b);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      const int c = sums[w];
+      before += w < warp ? c : 0;
+      all += c;
+    }
+    if (keep) {
+      const int j = base + before + __popc(b & ((1u << lane) - 1u));
+      idx[j] = i;
+      tgt[j] = t >= 0 && t < vocab ? (int)t : -1;
+      lt[j] = __int_as_float(0x7fc00000);
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) *count = base;
+}
+
+// fp32 -> three bf16 planes whose sum is the value to 2^-24
+__device__ __forceinline__ void split3(float v, bf16& a, bf16& b, bf16& c) {
+  a = __float2bfloat16_rn(v);
+  const float r = v - __bfloat162float(a);
+  b = __float2bfloat16_rn(r);
+  c = __float2bfloat16_rn(r - __bfloat162float(b));
+}
+
+// One CTA per row of the source: xs[j] = x[idx[j]] (bf16, or three planes of
+// fp32) for j < count, zeros past it and in the padding columns; idx ==
+// nullptr copies rows straight. Also zeros the dx rows of ignored tokens.
+template <typename T>
+__global__ void __launch_bounds__(128) xent_gather(const T* __restrict__ x, int64_t ldx, int d, const int* __restrict__ idx,
+                                                   const int* __restrict__ count, bf16* __restrict__ xs, int64_t lds,
+                                                   int64_t plane, const int64_t* __restrict__ targets, int64_t ignore,
+                                                   T* __restrict__ dx, int64_t lddx) {
+  const int64_t j = blockIdx.x;
+  if (dx && targets[j] == ignore)
+    for (int c = threadIdx.x; c < d; c += 128) dx[j * lddx + c] = from_f<T>(0.f);
+  const bool live = !idx || j < *count;
+  const T* src = x + (live ? (idx ? (int64_t)idx[j] : j) : 0) * ldx;
+  bf16* dst = xs + j * lds;
+  if (sizeof(T) == 2 && live && ldx % 8 == 0 && d % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+    for (int c = threadIdx.x; c < d / 8; c += 128)
+      reinterpret_cast<uint4*>(dst)[c] = reinterpret_cast<const uint4*>(src)[c];
+    return;
+  }
+  for (int c = threadIdx.x; c < lds; c += 128) {
+    const float v = live && c < d ? to_f<T>(src[c]) : 0.f;
+    if (sizeof(T) == 2) {
+      dst[c] = __float2bfloat16_rn(v);
+    } else {
+      bf16 a, b, e;
+      split3(v, a, b, e);
+      dst[c] = a;
+      dst[plane + c] = b;
+      dst[2 * plane + c] = e;
+    }
+  }
+}
+
+// logsumexp of a row from its tiles, as (max, log2 of the sum relative to it)
+template <int NT>
+__device__ __forceinline__ float2 join_tiles(const float2* __restrict__ st, int n_tiles, float* red) {
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < n_tiles; i += NT) m = fmaxf(m, st[i].x);
+  m = block_max<NT>(m, red);
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n_tiles; i += NT) {
+    const float2 v = st[i];
+    s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e);
+  }
+  s = block_sum<NT>(s, red);
+  return make_float2(m, log2f(s));
+}
+
+__device__ __forceinline__ float row_loss(float2 lse, float lt) { return (lse.x - lt) + lse.y * kLn2; }
+
+// Losses without gradients: one warp per row.
+__global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ stats, int n_tiles, int n,
+                                                   const float* __restrict__ lt, const int64_t* __restrict__ targets,
+                                                   int64_t ignore, int vocab, float* __restrict__ losses) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+  if (row >= n) return;
+  const int lane = threadIdx.x % 32;
+  const int64_t t = targets[row];
+  const float2* st = stats + row * n_tiles;
+  float m = -INFINITY;
+  for (int i = lane; i < n_tiles; i += 32) m = fmaxf(m, st[i].x);
+  m = warp_max(m);
+  float s = 0.f;
+  for (int i = lane; i < n_tiles; i += 32) {
+    const float2 v = st[i];
+    s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e);
+  }
+  s = warp_sum(s);
+  if (lane == 0) {
+    float l = t >= 0 && t < vocab ? row_loss(make_float2(m, log2f(s)), lt[row]) : __int_as_float(0x7fc00000);
+    losses[row] = t == ignore ? 0.f : l;
+  }
+}
+
+// One CTA per row of a piece: joins the tiles, writes the row's loss and
+// rewrites the exponentials as G = g (p - onehot) (bf16 in place of fp16, or
+// fp32 -> three bf16 planes). Rows between the count and the next multiple
+// of 64 become zeros: the third product reads them.
+template <bool F32>
+__global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stats, int n_tiles, int rows, int vocab,
+                                                 const int* __restrict__ count, int base, const int* __restrict__ idx,
+                                                 const int* __restrict__ tgt, const float* __restrict__ lt,
+                                                 const float* __restrict__ grad_rows, int mean, float* __restrict__ losses,
+                                                 void* __restrict__ p, int64_t ldp, bf16* __restrict__ planes,
+                                                 int64_t plane) {
+  extern __shared__ float xent_f[];  // [n_tiles]
+  __shared__ float red[8];
+  const int n_all = *count;
+  const int n = cut_rows(rows, count, base);
+  const int64_t row = blockIdx.x;
+  if (row >= n) {
+    if (row < cdiv(n, 64) * 64) {
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      for (int64_t c = threadIdx.x; c < ldp / 8; c += 256) {
+        if (F32) {
+          for (int k = 0; k < 3; ++k) reinterpret_cast<uint4*>(planes + k * plane + row * ldp)[c] = z;
+        } else {
+          reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp)[c] = z;
+        }
+      }
+    }
+    return;
+  }
+  const float2* st = stats + row * n_tiles;
+  const float2 lse = join_tiles<256>(st, n_tiles, red);
+  const int t = tgt[row];
+  if (threadIdx.x == 0 && losses) losses[row] = row_loss(lse, lt[row]);
+  float g = grad_rows ? grad_rows[idx[row]] : (mean ? 1.f / (float)n_all : 1.f);
+  if (t < 0) g = __int_as_float(0x7fc00000);
+  // tile factors: g 2^(m_tile - lse)
+  for (int i = threadIdx.x; i < n_tiles; i += 256) {
+    const float m = st[i].x;
+    xent_f[i] = m == -INFINITY ? 0.f : g * exp2f((m - lse.x) * kLog2e - lse.y) * (F32 ? 1.f : 0x1p-15f);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x * 8; c < vocab; c += 256 * 8) {
+    const float f = xent_f[c / kTile];
+    float v[8];
+    if (F32) {
+      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p) + row * ldp + c);
+      const float4 a = src[0], b = src[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p) + row * ldp + c);
+      const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 x = __half22float2(h[q]);
+        v[2 * q] = x.x;
+        v[2 * q + 1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = v[q] * f - (c + q == t ? g : 0.f);
+    if (F32) {
+      uint32_t o[3][4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        bf16 x[3], y[3];
+        split3(v[2 * q], x[0], x[1], x[2]);
+        split3(v[2 * q + 1], y[0], y[1], y[2]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const __nv_bfloat162 w2 = __halves2bfloat162(x[k], y[k]);
+          o[k][q] = *reinterpret_cast<const uint32_t*>(&w2);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<uint4*>(planes + k * plane + row * ldp + c) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp + c) =
+          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+  }
+}
+
+// loss = sum of the losses (compact list of *count, or all n with the ignored
+// tokens' zeros), over the number that count when mean. One CTA, fixed order.
+__global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ losses, int n, const int* __restrict__ count,
+                                                    const int64_t* __restrict__ targets, int64_t ignore, int mean,
+                                                    float* __restrict__ loss) {
+  __shared__ float red[32];
+  const int m = count ? *count : n;
+  float s = 0.f, c = 0.f;
+  for (int i = threadIdx.x; i < m; i += 1024) {
+    s += losses[i];
+    if (!count && targets[i] != ignore) c += 1.f;  // per thread: exact up to 2^24
+  }
+  s = block_sum<1024>(s, red);
+  if (!count) {
+    c = block_sum<1024>(c, red);
+  } else {
+    c = (float)m;
+  }
+  if (threadIdx.x == 0) *loss = mean ? s / fmaxf(c, 1.f) : s;
+}
+
+// dx[idx[r]] = sum over the splits of part[s][r]
+template <typename T>
+__global__ void __launch_bounds__(256) xent_join(const float* __restrict__ part, int splits, int64_t stride, int rows,
+                                                 const int* __restrict__ count, int base, const int* __restrict__ idx,
+                                                 int d, int64_t ldpart, T* __restrict__ dx, int64_t lddx) {
+  const int row = blockIdx.x;
+  if (row >= cut_rows(rows, count, base)) return;
+  const float* src = part + (int64_t)row * ldpart;
+  T* dst = dx + (int64_t)idx[row] * lddx;
+  for (int c = threadIdx.x; c < d; c += 256) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += src[s * stride + c];
+    dst[c] = from_f<T>(v);
+  }
+}
+
+// buf *= *s unless *s is 1
+template <typename T>
+__global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ buf, int64_t n, const float* __restrict__ s) {
+  const float f = *s;
+  if (f == 1.f) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    buf[i] = from_f<T>(to_f<T>(buf[i]) * f);
+}
+
+// ---- host side ------------------------------------------------------------------
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+
+bool aligned_rows(const void* p, int64_t ld, int64_t rows, int elt) {
+  return ((uintptr_t)p & 15) == 0 && (rows == 1 || ld % (16 / elt) == 0);
+}
+
+struct Plan {
+  bool f32, train, pack_x, pack_w;
+  int elt, planes, n_tiles, piece, n_pieces, dx_splits, dx_k;
+  int64_t ldx, ldw, ldp, ldd;
+  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, acc, part, total;
+};
+
+Plan make_plan(const llattn_xent_args& a) {
+  Plan q;
+  q.f32 = a.dtype == LLATTN_F32;
+  q.elt = q.f32 ? 4 : 2;
+  q.planes = q.f32 ? 3 : 1;
+  q.train = a.dx || a.dw;
+  q.pack_x = q.f32 || q.train || !aligned_rows(a.x, a.ldx, a.tokens, 2);
+  q.pack_w = q.f32 || !aligned_rows(a.w, a.ldw, a.vocab, 2);
+  q.ldx = q.pack_x ? up8(a.d) : (a.tokens == 1 ? up8(a.d) : a.ldx);
+  q.ldw = q.pack_w ? up8(a.d) : (a.vocab == 1 ? up8(a.d) : a.ldw);
+  q.ldp = up8(a.vocab);
+  q.ldd = up8(a.d);
+  q.n_tiles = cdiv(a.vocab, kTile);
+  // rows of exponentials held at a time: half a GiB of them (V = 32000 in
+  // bf16: 8192 rows), whole row tiles. fp32 also bounds the length of each
+  // tensor-core sum: its additions truncate, about 2^-26 of the running sum per
+  // 16 products on average (measured: dx 9.6e-6 off after 8192 products, 1e-6
+  // after 1024), so sums over V run in splits of 1024 and sums over rows in
+  // pieces of 1024, joined by rounded fp32 additions
+  const int64_t row_bytes = q.f32 ? q.ldp * 10 + 4 * q.ldd * cdiv(a.vocab, kF32Chain) : q.ldp * 2;
+  int64_t piece = (int64_t)(512u << 20) / row_bytes / 256 * 256;
+  piece = std::max<int64_t>(256, piece);
+  if (q.f32) piece = std::min<int64_t>(piece, kF32Chain);
+  q.piece = (int)std::min<int64_t>(piece, a.tokens);
+  if (!q.train) q.piece = a.tokens;
+  q.n_pieces = cdiv(a.tokens, q.piece);
+  // few rows: split the long K = V of dx = G w over the SMs
+  const int64_t t = (int64_t)cdiv(q.piece, 128) * cdiv(a.d, 128);
+  const int ksteps = cdiv(a.vocab, 64);
+  int sp = (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / t, ksteps / 8));
+  if (q.f32) sp = std::max(sp, cdiv(a.vocab, kF32Chain));
+  q.dx_k = cdiv(ksteps, sp) * 64;
+  q.dx_splits = cdiv(a.vocab, q.dx_k);
+  size_t off = 0;
+  auto take = [&](size_t b) { size_t o = off; off += up256(b); return o; };
+  const size_t n = a.tokens;
+  q.xs = take(q.pack_x ? 2 * (size_t)q.planes * n * q.ldx : 0);
+  q.ws = take(q.pack_w ? 2 * (size_t)q.planes * a.vocab * q.ldw : 0);
+  q.stats = take(sizeof(float2) * (size_t)q.piece * q.n_tiles);
+  q.lt = take(4 * n);
+  q.idx = take(q.train ? 4 * n : 0);
+  q.tgt = take(q.train ? 4 * n : 0);
+  q.count = take(4);
+  q.losses = take(4 * n);
+  q.p = take(q.train ? (size_t)q.piece * q.ldp * q.elt : 0);
+  q.gplanes = take(q.train && q.f32 ? 6 * (size_t)q.piece * q.ldp : 0);
+  q.acc = take(q.train && a.dw && q.n_pieces > 1 ? 4 * (size_t)a.vocab * q.ldd : 0);
+  q.part = take(q.train && a.dx && q.dx_splits > 1 ? 4 * (size_t)q.dx_splits * q.piece * q.ldd : 0);
+  q.total = off;
+  return q;
+}
+
+MmArgs base_args(const Plan& q, volatile unsigned* fault) {
+  MmArgs p = {};
+  p.n_terms = q.f32 ? 6 : 1;
+  p.pa = q.f32 ? kTermsA : 0;
+  p.pb = q.f32 ? kTermsB : 0;
+  p.nz = p.splits = 1;
+  p.fault_host = fault;
+  return p;
+}
+
+#define TRY(x)                          \
+  do {                                  \
+    cudaError_t e_ = (x);               \
+    if (e_ != cudaSuccess) return e_;   \
+  } while (0)
+
+template <typename T>
+cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fault, cudaStream_t s) {
+  char* ws = static_cast<char*>(a.workspace);
+  bf16* xs = reinterpret_cast<bf16*>(ws + q.xs);
+  bf16* wp = reinterpret_cast<bf16*>(ws + q.ws);
+  float2* stats = reinterpret_cast<float2*>(ws + q.stats);
+  float* lt = reinterpret_cast<float*>(ws + q.lt);
+  int* idx = reinterpret_cast<int*>(ws + q.idx);
+  int* tgt = reinterpret_cast<int*>(ws + q.tgt);
+  int* count = reinterpret_cast<int*>(ws + q.count);
+  const int n = a.tokens, d = a.d, V = a.vocab;
+  const bool mean = a.reduction == LLATTN_XENT_MEAN;
+  const int64_t xplane = (int64_t)n * q.ldx, wplane = (int64_t)V * q.ldw;
+  if (q.pack_w) {
+    xent_gather<T><<<V, 128, 0, s>>>(static_cast<const T*>(a.w), a.ldw, d, nullptr, nullptr, wp, q.ldw, wplane, nullptr,
+                                     0, nullptr, 0);
+    TRY(cudaGetLastError());
+  }
+  const void* wv = q.pack_w ? wp : a.w;
+  if (!q.train) {
+    if (q.pack_x) {
+      xent_gather<T><<<n, 128, 0, s>>>(static_cast<const T*>(a.x), a.ldx, d, nullptr, nullptr, xs, q.ldx, xplane, nullptr,
+                                       0, nullptr, 0);
+      TRY(cudaGetLastError());
+    }
+    MmArgs p = base_args(q, fault);
+    p.M = n;
+    p.N = V;
+    p.K = d;
+    EpiStats ep{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0};
+    TRY(launch_mm(p, Operand{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0},
+                  Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
+    float* losses = a.losses ? a.losses : reinterpret_cast<float*>(ws + q.losses);
+    xent_losses<<<cdiv(n, 4), 128, 0, s>>>(stats, q.n_tiles, n, lt, a.targets, a.ignore_index, V, losses);
+    TRY(cudaGetLastError());
+    if (a.loss) {
+      xent_reduce<<<1, 1024, 0, s>>>(losses, n, nullptr, a.targets, a.ignore_index, mean, a.loss);
+      TRY(cudaGetLastError());
+    }
+    return cudaSuccess;
+  }
+  xent_compact<<<1, 1024, 0, s>>>(a.targets, n, a.ignore_index, V, idx, tgt, lt, count);
+  TRY(cudaGetLastError());
+  T* dx = static_cast<T*>(a.dx);
+  xent_gather<T><<<n, 128, 0, s>>>(static_cast<const T*>(a.x), a.ldx, d, idx, count, xs, q.ldx, xplane, a.targets,
+                                   a.ignore_index, dx, d);
+  TRY(cudaGetLastError());
+  float* losses = reinterpret_cast<float*>(ws + q.losses);
+  void* pbuf = ws + q.p;
+  bf16* gpl = reinterpret_cast<bf16*>(ws + q.gplanes);
+  float* acc = reinterpret_cast<float*>(ws + q.acc);
+  float* part = reinterpret_cast<float*>(ws + q.part);
+  const int64_t gplane = (int64_t)q.piece * q.ldp;
+  for (int c = 0; c < q.n_pieces; ++c) {
+    const int base = c * q.piece, rows = std::min(q.piece, n - base);
+    const Operand ox{xs + (int64_t)base * q.ldx, rows, d, q.ldx, q.planes, xplane, 0};
+    MmArgs p = base_args(q, fault);
+    p.m_dev = count;
+    p.dev_base = base;
+    p.M = rows;
+    p.N = V;
+    p.K = d;
+    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0};
+    TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
+    const size_t sm = sizeof(float) * q.n_tiles;
+    xent_rows<sizeof(T) == 4><<<rows, 256, sm, s>>>(stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
+                                                    lt + base, a.grad_rows, mean, losses + base, pbuf, q.ldp, gpl, gplane);
+    TRY(cudaGetLastError());
+    const void* g = q.f32 ? (const void*)gpl : pbuf;
+    if (dx) {
+      MmArgs m = base_args(q, fault);
+      m.m_dev = count;
+      m.dev_base = base;
+      m.M = rows;
+      m.N = d;
+      m.K = V;
+      m.splits = q.dx_splits;
+      m.k_per_split = q.dx_k;
+      EpiOut eo{};
+      if (q.dx_splits > 1) {
+        eo.out = part;
+        eo.ldo = q.ldd;
+        eo.vec = 1;
+        eo.split_stride = (int64_t)q.piece * q.ldd;
+      } else {
+        eo.out = dx;
+        eo.ldo = d;
+        eo.out_bf16 = !q.f32;
+        eo.vec = aligned_rows(dx, d, 2, q.elt);
+        eo.idx = idx + base;
+      }
+      TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
+                    s));
+      if (q.dx_splits > 1) {
+        xent_join<T><<<rows, 256, 0, s>>>(part, q.dx_splits, eo.split_stride, rows, count, base, idx + base, d, q.ldd, dx,
+                                          d);
+        TRY(cudaGetLastError());
+      }
+    }
+    if (a.dw) {
+      MmArgs m = base_args(q, fault);
+      m.k_dev = count;
+      m.dev_base = base;
+      m.M = V;
+      m.N = d;
+      m.K = rows;
+      EpiOut eo{};
+      const bool last = c + 1 == q.n_pieces;
+      eo.out = last ? a.dw : acc;
+      eo.ldo = last ? d : q.ldd;
+      eo.out_bf16 = last && !q.f32;
+      eo.vec = last ? aligned_rows(a.dw, d, 2, q.elt) : 1;
+      eo.acc = c ? acc : nullptr;
+      eo.ldacc = q.ldd;
+      TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
+                    eo, s));
+    }
+  }
+  if (a.loss) {
+    xent_reduce<<<1, 1024, 0, s>>>(losses, n, count, nullptr, 0, mean, a.loss);
+    TRY(cudaGetLastError());
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+size_t workspace_bytes(const llattn_xent_args& a) { return make_plan(a).total; }
+
+int launches(const llattn_xent_args& a) {
+  const Plan q = make_plan(a);
+  if (!q.train) return q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
+  return q.pack_w + 2 + q.n_pieces * (2 + (a.dx ? 1 + (q.dx_splits > 1) : 0) + (a.dw ? 1 : 0)) + (a.loss ? 1 : 0);
+}
+
+cudaError_t launch(const llattn_xent_args& a, volatile unsigned* fault, cudaStream_t s) {
+  const Plan q = make_plan(a);
+  return q.f32 ? run<float>(a, q, fault, s) : run<bf16>(a, q, fault, s);
+}
+
+cudaError_t launch_scale(void* buf, int64_t n, int dtype, const float* f, cudaStream_t s) {
+  const int64_t blocks = std::min<int64_t>((n + 255) / 256, 8 * sm_count());
+  if (dtype == LLATTN_BF16)
+    scale_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>(static_cast<bf16*>(buf), n, f);
+  else
+    scale_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(static_cast<float*>(buf), n, f);
+  return cudaGetLastError();
+}
+
+unsigned read_fault_word(bool reset) { return read_fault(reset); }
+
+}  // namespace xent
+}  // namespace llattn

@@ -1,0 +1,295 @@
+"""Operators of the training step around the attention block, over
+libllattn.so: the loss of the output head without its logits
+(``linear_cross_entropy``) and the orthogonalised update of the hidden
+matrices (``newton_schulz``).
+
+As in ``ops.py``: custom ops ``llattn_b200::linear_xent / linear_xent_none /
+linear_xent_none_grads / newton_schulz`` for CUDA only with fake
+implementations, torch's current stream, torch-allocated outputs and
+workspaces, ``RuntimeError`` on bad arguments, no CPU implementation. Outside
+``torch.compile`` the same functions are called directly, without the
+dispatcher.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from contextlib import nullcontext
+from typing import Optional, Sequence
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .ops import _dtype_code, _ptr, _require, _stream
+
+_REDUCTIONS = {"none": _lib.XENT_NONE, "mean": _lib.XENT_MEAN, "sum": _lib.XENT_SUM}
+
+
+def _on(device: torch.device):
+    """Makes `device` current where it is not."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
+
+
+# --------------------------------------------------------------------------
+# softmax cross-entropy of the output projection
+
+def _rows(t: Tensor) -> Tensor:
+    """t [R, C] with contiguous columns and non-overlapping rows."""
+    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _check_xent(x: Tensor, w: Tensor, targets: Tensor) -> None:
+    _require(x.is_cuda, "linear_cross_entropy needs CUDA tensors")
+    _require(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1],
+             f"x {tuple(x.shape)} and weight {tuple(w.shape)} must be [tokens, d] and [vocab, d]")
+    _require(x.dtype == w.dtype, f"x is {x.dtype} and weight {w.dtype}: one dtype (or autocast) is needed")
+    _require(targets.dtype == torch.int64 and tuple(targets.shape) == (x.shape[0],),
+             f"targets must be int64 [tokens], got {targets.dtype} {tuple(targets.shape)}")
+    _require(w.device == x.device and targets.device == x.device, "x, weight and targets must be on one device")
+    _require(w.shape[0] >= 1 and w.shape[1] >= 1, "weight must have rows and columns")
+
+
+def _xent(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int, *, grad_rows: Optional[Tensor] = None,
+          losses: Optional[Tensor] = None, loss: Optional[Tensor] = None, dx: Optional[Tensor] = None,
+          dw: Optional[Tensor] = None) -> None:
+    x, w, targets = _rows(x), _rows(w), targets.contiguous()
+    p = lambda t: _ptr(t) if t is not None else None
+    args = _lib.XentArgs(x.shape[0], x.shape[1], w.shape[0], _dtype_code(x), reduction, ignore_index, _ptr(x),
+                         max(x.stride(0), x.shape[1]), _ptr(w), max(w.stride(0), w.shape[1]), _ptr(targets),
+                         p(grad_rows), p(losses), p(loss), p(dx), p(dw), None, 0)
+    L = _lib.lib()
+    with _on(x.device):
+        ws = torch.empty(L.llattn_xent_workspace_bytes(ctypes.byref(args)) or 256, dtype=torch.uint8, device=x.device)
+        args.workspace, args.workspace_bytes = _ptr(ws), ws.numel()
+        _lib.check(L.llattn_xent(ctypes.byref(args), _stream(x)), "llattn_xent")
+
+
+def _linear_xent(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int, need_dx: bool,
+                 need_dw: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """Reductions mean and sum: the loss, and dx / dw of it where needed (else empty)."""
+    _check_xent(x, w, targets)
+    _dtype_code(x)
+    make = torch.empty if x.shape[0] else torch.zeros
+    loss = make((), dtype=torch.float32, device=x.device)
+    dx = make(x.shape if need_dx else (0,), dtype=x.dtype, device=x.device)
+    dw = make(w.shape if need_dw else (0,), dtype=w.dtype, device=x.device)
+    if x.shape[0]:
+        _xent(x, w, targets, ignore_index, reduction, loss=loss, dx=dx if need_dx else None, dw=dw if need_dw else None)
+    return loss, dx, dw
+
+
+def _linear_xent_none(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int) -> Tensor:
+    """Reduction none: per-token losses."""
+    _check_xent(x, w, targets)
+    _dtype_code(x)
+    losses = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    if x.shape[0]:
+        _xent(x, w, targets, ignore_index, _lib.XENT_NONE, losses=losses)
+    return losses
+
+
+def _linear_xent_none_grads(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, grad_rows: Tensor, need_dx: bool,
+                            need_dw: bool) -> tuple[Tensor, Tensor]:
+    """dx / dw of sum_n grad_rows[n] loss[n] (the logits recomputed)."""
+    _check_xent(x, w, targets)
+    make = torch.empty if x.shape[0] else torch.zeros
+    dx = make(x.shape if need_dx else (0,), dtype=x.dtype, device=x.device)
+    dw = make(w.shape if need_dw else (0,), dtype=w.dtype, device=x.device)
+    if x.shape[0] and (need_dx or need_dw):
+        _xent(x, w, targets, ignore_index, _lib.XENT_NONE, grad_rows=grad_rows.float().contiguous(),
+              dx=dx if need_dx else None, dw=dw if need_dw else None)
+    return dx, dw
+
+
+linear_xent_op = torch.library.custom_op("llattn_b200::linear_xent", _linear_xent, mutates_args=(), device_types="cuda")
+linear_xent_none_op = torch.library.custom_op("llattn_b200::linear_xent_none", _linear_xent_none, mutates_args=(),
+                                              device_types="cuda")
+linear_xent_none_grads_op = torch.library.custom_op("llattn_b200::linear_xent_none_grads", _linear_xent_none_grads,
+                                                    mutates_args=(), device_types="cuda")
+
+
+@linear_xent_op.register_fake
+def _linear_xent_fake(x, w, targets, ignore_index, reduction, need_dx, need_dw):
+    return (x.new_empty((), dtype=torch.float32), x.new_empty(x.shape if need_dx else (0,)),
+            w.new_empty(w.shape if need_dw else (0,)))
+
+
+@linear_xent_none_op.register_fake
+def _linear_xent_none_fake(x, w, targets, ignore_index):
+    return x.new_empty(x.shape[0], dtype=torch.float32)
+
+
+@linear_xent_none_grads_op.register_fake
+def _linear_xent_none_grads_fake(x, w, targets, ignore_index, grad_rows, need_dx, need_dw):
+    return x.new_empty(x.shape if need_dx else (0,)), w.new_empty(w.shape if need_dw else (0,))
+
+
+def _scale_(t: Tensor, factor: Tensor) -> Tensor:
+    """t *= factor (device scalar), in one launch that leaves t alone for a factor of 1."""
+    with _on(t.device):
+        _lib.check(_lib.lib().llattn_scale(_ptr(t), t.numel(), _dtype_code(t), _ptr(factor), _stream(t)), "llattn_scale")
+    return t
+
+
+class _XentReduced(torch.autograd.Function):
+    """mean / sum: the gradients for an upstream gradient of 1 are computed
+    with the loss (while the exponentials are at hand) and scaled in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, w, targets, ignore_index, reduction):
+        need = ctx.needs_input_grad
+        f = linear_xent_op if torch.compiler.is_compiling() else _linear_xent
+        loss, dx, dw = f(x, w, targets, ignore_index, reduction, need[0], need[1])
+        ctx.save_for_backward(x, w, targets, dx, dw)
+        ctx.cfg = (ignore_index, reduction)
+        ctx.spent = False
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        need = ctx.needs_input_grad
+        x, w, targets, dx, dw = ctx.saved_tensors
+        if torch.compiler.is_compiling():
+            return ((dx * grad).to(x.dtype) if need[0] else None, (dw * grad).to(w.dtype) if need[1] else None, None, None,
+                    None)
+        if ctx.spent:  # a retained graph's next backward: the first one scaled the stored gradients in place
+            _, dx, dw = _linear_xent(x, w, targets, *ctx.cfg, need[0], need[1])
+        ctx.spent = True
+        g = grad.float()
+        return (_scale_(dx, g) if need[0] and dx.numel() else dx if need[0] else None,
+                _scale_(dw, g) if need[1] and dw.numel() else dw if need[1] else None, None, None, None)
+
+
+class _XentNone(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, targets, ignore_index):
+        f = linear_xent_none_op if torch.compiler.is_compiling() else _linear_xent_none
+        ctx.save_for_backward(x, w, targets)
+        ctx.ignore_index = ignore_index
+        return f(x, w, targets, ignore_index)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, targets = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        f = linear_xent_none_grads_op if torch.compiler.is_compiling() else _linear_xent_none_grads
+        dx, dw = f(x, w, targets, ctx.ignore_index, grad, need[0], need[1])
+        return dx if need[0] else None, dw if need[1] else None, None, None
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
+                         reduction: str = "mean") -> Tensor:
+    """Softmax cross-entropy of the logits x @ weight.T against targets, without
+    the logits: what ``F.cross_entropy(F.linear(x, weight).float(), targets)``
+    returns, differentiable in x and weight.
+
+    x [..., d] and weight [vocab, d], both bfloat16 or both float32 (under
+    autocast both are cast to its dtype, as a linear layer's are); targets
+    [...] int64. Products are summed in fp32; the gradients come back in the
+    inputs' dtype. reduction: "mean" over the tokens whose target is not
+    ignore_index (0 when there is none), "sum", or "none" (losses [...] fp32,
+    0 for ignored tokens). Ignored tokens get zero gradients and their rows of x
+    are not read for weight's. A target outside [0, vocab) makes the loss NaN.
+
+    "mean" and "sum" compute the gradients together with the loss, from at most
+    half a GiB of exponentials at a time, and keep them until the backward;
+    "none" recomputes in the backward. Gradients of gradients are not supported."""
+    _require(reduction in _REDUCTIONS, f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    _require(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
+             f"x {tuple(x.shape)} must end in weight's columns {tuple(weight.shape)}")
+    _require(tuple(targets.shape) == tuple(x.shape[:-1]),
+             f"targets {tuple(targets.shape)} must have x's leading shape {tuple(x.shape[:-1])}")
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight = x.to(dt), weight.to(dt)
+    x2, t = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
+    grads = torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad)
+    if reduction == "none":
+        if grads:
+            out = _XentNone.apply(x2, weight, t, ignore_index)
+        else:
+            out = (linear_xent_none_op if torch.compiler.is_compiling() else _linear_xent_none)(x2, weight, t, ignore_index)
+        return out.view(targets.shape)
+    code = _REDUCTIONS[reduction]
+    if grads:
+        return _XentReduced.apply(x2, weight, t, ignore_index, code)
+    f = linear_xent_op if torch.compiler.is_compiling() else _linear_xent
+    return f(x2, weight, t, ignore_index, code, False, False)[0]
+
+
+# --------------------------------------------------------------------------
+# orthogonalised updates
+
+DEFAULT_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _orth(gs: Sequence[Tensor], steps: int, a: float, b: float, c: float, eps: float) -> Tensor:
+    """gs: matrices of one shape, dtype and device -> [len(gs), m, n] bf16."""
+    g0 = gs[0]
+    m, n = g0.shape
+    out = torch.empty(len(gs), m, n, dtype=torch.bfloat16, device=g0.device)
+    if m == 0 or n == 0:
+        return out
+    gs = [g.contiguous() for g in gs]
+    ptrs = (ctypes.c_void_p * len(gs))(*[g.data_ptr() for g in gs])
+    args = _lib.OrthArgs(m, n, len(gs), steps, _dtype_code(g0), a, b, c, eps, ptrs, _ptr(out), None, 0)
+    L = _lib.lib()
+    with _on(g0.device):
+        ws = torch.empty(L.llattn_orth_workspace_bytes(ctypes.byref(args)) or 256, dtype=torch.uint8, device=g0.device)
+        args.workspace, args.workspace_bytes = _ptr(ws), ws.numel()
+        _lib.check(L.llattn_orth(ctypes.byref(args), _stream(g0)), "llattn_orth")
+    return out
+
+
+def _newton_schulz(g: Tensor, steps: int, a: float, b: float, c: float, eps: float) -> Tensor:
+    return _orth(g.unbind(0), steps, a, b, c, eps)
+
+
+newton_schulz_op = torch.library.custom_op("llattn_b200::newton_schulz", _newton_schulz, mutates_args=(),
+                                           device_types="cuda")
+
+
+@newton_schulz_op.register_fake
+def _newton_schulz_fake(g, steps, a, b, c, eps):
+    return g.new_empty(g.shape, dtype=torch.bfloat16)
+
+
+@torch.no_grad()
+def newton_schulz(g, *, steps: int = 5, coefficients: tuple[float, float, float] = DEFAULT_COEFFICIENTS,
+                  eps: float = 1e-7):
+    """Orthogonalises matrices by Newton-Schulz products, as the Muon optimiser
+    does with its momentum: X = g / (|g|_F + eps), then `steps` times
+    X <- a X + (b S + c S^2) X with S = X X^T, on the shorter side, so that every
+    singular value of X approaches 1.
+
+    g: a matrix [m, n], a batch [..., m, n], or a list of matrices (of any mix
+    of shapes; equal shapes run as one batch), bfloat16 or float32 on CUDA.
+    Returns the same structure in bfloat16 (products of 16-bit operands summed
+    in fp32; not differentiable). An all-zero matrix stays zero."""
+    a, b, c = (float(v) for v in coefficients)
+    steps, eps = int(steps), float(eps)
+    if isinstance(g, Tensor):
+        _require(g.dim() >= 2, f"newton_schulz expects matrices [..., m, n], got {tuple(g.shape)}")
+        _require(g.is_cuda, "newton_schulz needs CUDA tensors")
+        _dtype_code(g)
+        if g.numel() == 0:
+            return torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
+        f = newton_schulz_op if torch.compiler.is_compiling() else _newton_schulz
+        return f(g.reshape(-1, *g.shape[-2:]), steps, a, b, c, eps).view(g.shape)
+    gs = list(g)
+    groups: dict = {}
+    for i, t in enumerate(gs):
+        _require(isinstance(t, Tensor) and t.dim() == 2, "newton_schulz expects a list of matrices")
+        _require(t.is_cuda, "newton_schulz needs CUDA tensors")
+        _dtype_code(t)
+        groups.setdefault((t.shape, t.dtype, t.device), []).append(i)
+    outs: list = [None] * len(gs)
+    for members in groups.values():
+        for i, o in zip(members, _orth([gs[i] for i in members], steps, a, b, c, eps).unbind(0)):
+            outs[i] = o
+    return outs
