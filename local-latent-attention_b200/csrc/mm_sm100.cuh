@@ -159,7 +159,8 @@ struct MmShape {
   static constexpr int THREADS = 64 + 32 * EW;
   static constexpr int ST = 6;
   static constexpr int OPB = 128 * 64 * 2;  // one CTA's operand tile: 128 rows x 64 K, 16 KB
-  static constexpr int A = 0, B = A + ST * OPB, BAR = B + ST * OPB;
+  static constexpr int STG = 4096;          // an epilogue warp's staging block: 32 rows of 128 bytes
+  static constexpr int A = 0, B = A + ST * OPB, STAGE = B + ST * OPB, BAR = STAGE + EW * STG;
   static constexpr int BYTES = BAR + 256;
   static constexpr int SMEM = BYTES + 1024;  // + alignment
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -209,10 +210,12 @@ __device__ __forceinline__ int cut_rows(int n, const int* dev, int base) {
 }
 
 // Epi: struct with
-//   __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero) const
+//   __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
+//                        uint8_t* buf) const
 // called by every thread of an epilogue warp (all 32 lanes, converged) for its
 // row and 128 columns [col0, col0 + 128); taddr: TMEM address of the warp's
-// lanes and columns; zero: the K range is empty, the accumulator holds nothing.
+// lanes and columns; zero: the K range is empty, the accumulator holds
+// nothing; buf: the warp's staging block.
 template <int CG, typename Epi>
 __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
@@ -357,7 +360,8 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
       if (!ok) break;
       tc_fence_after();
       const uint32_t ta = tmem + S::BN * buf + 128 * half + ((uint32_t)(32 * quad) << 16);
-      epi.tile(p, w, w.m0 + rank * 128 + 32 * quad + lane, w.n0 + 128 * half, M, ta, k1 <= k0);
+      epi.tile(p, w, w.m0 + rank * 128 + 32 * quad + lane, w.n0 + 128 * half, M, ta, k1 <= k0,
+               smem + S::STAGE + (warp - 2) * S::STG);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {  // this accumulator may take the tile after next
@@ -391,9 +395,109 @@ __device__ __forceinline__ void load32(uint32_t taddr, bool zero, float (&v)[32]
   for (int q = 0; q < 32; ++q) v[q] = zero ? 0.f : __uint_as_float(r[q]);
 }
 
+// Block transfers of an epilogue warp: thread = row holds CH 16-byte chunks of
+// its row (32 columns of 16 or 32 bits: 4 or 8 chunks); global memory is
+// accessed with CH lanes per row, whole 64- or 128-byte segments, through the
+// staging block (chunks rotated by the row, so both sides meet every bank). A
+// thread-per-row access would touch 32 lines per instruction and half of
+// each 32-byte sector.
+template <int CH>
+__device__ __forceinline__ int stage_at(int r, int c) {
+  return CH == 8 ? r * 128 + ((c ^ (r & 7)) * 16) : r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
+}
+// p: the lane's own row's first byte (16-byte aligned), bytes: valid bytes of
+// the rows (rounded up to 16 in memory), ok: the lane's row exists.
+template <int CH>
+__device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 (&v)[CH], uint8_t* p, int bytes,
+                                            bool ok) {
+#pragma unroll
+  for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
+  __syncwarp();
+  const int c = lane % CH;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = 32 / CH * i + lane / CH;
+    const uint4 u = *reinterpret_cast<const uint4*>(buf + stage_at<CH>(r, c));
+    uint8_t* q = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
+    if (q && 16 * c < bytes) *reinterpret_cast<uint4*>(q + 16 * c) = u;
+  }
+  __syncwarp();
+}
+// The reverse, in two halves so that the caller may have several in flight:
+// fetch reads global memory, spread hands each thread its row (zeros where
+// nothing was read).
+template <int CH>
+__device__ __forceinline__ void block_fetch(int lane, uint4 (&v)[CH], const void* p, int bytes, bool ok) {
+  const int c = lane % CH;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = 32 / CH * i + lane / CH;
+    const uint8_t* q =
+        reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
+    v[i] = q && 16 * c < bytes ? *reinterpret_cast<const uint4*>(q + 16 * c) : make_uint4(0, 0, 0, 0);
+  }
+}
+template <int CH>
+__device__ __forceinline__ void block_spread(uint8_t* buf, int lane, uint4 (&v)[CH]) {
+  const int c = lane % CH;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(32 / CH * i + lane / CH, c)) = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < CH; ++i) v[i] = *reinterpret_cast<const uint4*>(buf + stage_at<CH>(lane, i));
+  __syncwarp();
+}
+// Rows without 16-byte alignment: the staged block written element by
+// element, lanes along the 32 columns (n of them valid).
+template <typename E, int CH>
+__device__ __forceinline__ void block_store_odd(uint8_t* buf, int lane, const uint4 (&v)[CH], E* p, int n, bool ok) {
+#pragma unroll
+  for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
+  __syncwarp();
+  constexpr int PER = 16 / sizeof(E);
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r) {
+    E* q = reinterpret_cast<E*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
+    const E e = *reinterpret_cast<const E*>(buf + stage_at<CH>(r, lane / PER) + (lane % PER) * sizeof(E));
+    if (q && lane < n) q[lane] = e;
+  }
+  __syncwarp();
+}
+
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void half_row(const float (&v)[32], uint4 (&u)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    u[q] = make_uint4(pack_half(v[8 * q], v[8 * q + 1]), pack_half(v[8 * q + 2], v[8 * q + 3]),
+                      pack_half(v[8 * q + 4], v[8 * q + 5]), pack_half(v[8 * q + 6], v[8 * q + 7]));
+}
+__device__ __forceinline__ void bf16_row(const float (&v)[32], uint4 (&u)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    u[q] = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                      pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+}
+__device__ __forceinline__ void f32_row(const float (&v)[32], uint4 (&u)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    u[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
+                      __float_as_uint(v[4 * q + 3]));
+}
+template <int CH>
+__device__ __forceinline__ uint32_t word(const uint4 (&u)[CH], int i) {
+  return i % 4 == 0 ? u[i / 4].x : i % 4 == 1 ? u[i / 4].y : i % 4 == 2 ? u[i / 4].z : u[i / 4].w;
+}
+__device__ __forceinline__ float2 half_pair(const uint4 (&u)[4], int i) {  // values 2i, 2i + 1
+  const uint32_t w = word(u, i);
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 bf16_pair(const uint4 (&u)[4], int i) {
+  const uint32_t w = word(u, i);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
 // ---- host side --------------------------------------------------------------

@@ -51,41 +51,6 @@ struct Ptrs {
   const void* p[kPtrs];
 };
 
-__device__ __forceinline__ int64_t at2(int64_t z, int64_t zs, int64_t row, int64_t ld) { return z * zs + row * ld; }
-
-// stores 32 fp16 of one row; ld and the column are multiples of 8 where full
-__device__ __forceinline__ void store_half32(__half* dst, const float (&v)[32], int n) {
-  if (n >= 32) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      reinterpret_cast<uint4*>(dst)[q] =
-          make_uint4(pack_half(v[8 * q], v[8 * q + 1]), pack_half(v[8 * q + 2], v[8 * q + 3]),
-                     pack_half(v[8 * q + 4], v[8 * q + 5]), pack_half(v[8 * q + 6], v[8 * q + 7]));
-  } else {
-#pragma unroll
-    for (int q = 0; q < 32; ++q)
-      if (q < n) dst[q] = __float2half_rn(v[q]);
-  }
-}
-__device__ __forceinline__ void load_half32(const __half* src, float (&v)[32], int n) {
-  if (n >= 32) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 u = reinterpret_cast<const uint4*>(src)[q];
-      const __half2* h = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(h[i]);
-        v[8 * q + 2 * i] = f.x;
-        v[8 * q + 2 * i + 1] = f.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 32; ++q) v[q] = q < n ? __half2float(src[q]) : 0.f;
-  }
-}
-
 // mirror image of 32 columns of a row: element (row, nc + q) -> (nc + q, row);
 // the warp's 32 rows are consecutive, so each q is one 64-byte segment
 __device__ __forceinline__ void store_mirror(__half* base, int64_t ld, int row, int nc, const float (&v)[32], int n) {
@@ -100,21 +65,23 @@ struct EpiGram {
   int64_t ld, zs;
   const float* s0;  // first step: X = s0[z] * stored, else null (2^-6)
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero) const {
+                                       bool zero, uint8_t* buf) const {
+    const int lane = threadIdx.x % 32;
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float f = x * x * kS;
     __half* base = s + w.z * zs;
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
-      const int nc = col0 + cc;
-      if (nc >= a.N) break;
+      const int nc = col0 + cc, n = a.N - nc;
+      if (n <= 0) break;
       float v[32];
       load32(taddr + cc, zero, v);
-      if (row >= M) continue;
 #pragma unroll
       for (int q = 0; q < 32; ++q) v[q] *= f;
-      store_half32(base + row * ld + nc, v, a.N - nc);
-      if (w.m0 != w.n0) store_mirror(base, ld, row, nc, v, a.N - nc);
+      uint4 u[4];
+      half_row(v, u);
+      block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), n * 2, row < M);
+      if (w.m0 != w.n0 && row < M) store_mirror(base, ld, row, nc, v, n);
     }
   }
 };
@@ -126,20 +93,27 @@ struct EpiPoly {
   int64_t ld, zs;
   float cb, cc2, k;  // b, c / kS, k * kS
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero) const {
+                                       bool zero, uint8_t* buf) const {
+    const int lane = threadIdx.x % 32;
     __half* base = b + w.z * zs;
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
-      const int nc = col0 + cc;
-      if (nc >= a.N) break;
-      float v[32], x[32];
+      const int nc = col0 + cc, n = a.N - nc;
+      if (n <= 0) break;
+      float v[32];
+      uint4 u[4];
+      block_fetch(lane, u, s + w.z * zs + row * ld + nc, n * 2, row < M);
       load32(taddr + cc, zero, v);
-      if (row >= M) continue;
-      load_half32(s + w.z * zs + row * ld + nc, x, a.N - nc);
+      block_spread(buf, lane, u);
 #pragma unroll
-      for (int q = 0; q < 32; ++q) v[q] = fmaf(cb, x[q], cc2 * v[q]) + (row == nc + q ? k : 0.f);
-      store_half32(base + row * ld + nc, v, a.N - nc);
-      if (w.m0 != w.n0) store_mirror(base, ld, row, nc, v, a.N - nc);
+      for (int q = 0; q < 16; ++q) {
+        const float2 x = half_pair(u, q);
+        v[2 * q] = fmaf(cb, x.x, cc2 * v[2 * q]) + (row == nc + 2 * q ? k : 0.f);
+        v[2 * q + 1] = fmaf(cb, x.y, cc2 * v[2 * q + 1]) + (row == nc + 2 * q + 1 ? k : 0.f);
+      }
+      half_row(v, u);
+      block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), n * 2, row < M);
+      if (w.m0 != w.n0 && row < M) store_mirror(base, ld, row, nc, v, n);
     }
   }
 };
@@ -155,68 +129,59 @@ struct EpiUpdate {
   float ca;          // a - k
   int rd_lo, wr_lo, vec_out;
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero) const {
+                                       bool zero, uint8_t* buf) const {
+    const int lane = threadIdx.x % 32;
+    const bool ok = row < M;
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float fl = ca * x, fp = x / kS;
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
-      const int nc = col0 + cc;
-      if (nc >= a.N) break;
-      float v[32], h[32];
+      const int nc = col0 + cc, n = a.N - nc;
+      if (n <= 0) break;
+      const int64_t at = w.z * zs + row * ld + nc;
+      float v[32];
+      uint4 h[4], l[4];
+      block_fetch(lane, h, hi + at, n * 2, ok);
+      if (rd_lo) block_fetch(lane, l, lo + at, n * 2, ok);
       load32(taddr + cc, zero, v);
-      if (row >= M) continue;
-      const int n = a.N - nc;
-      const int64_t at = at2(w.z, zs, row, ld) + nc;
-      load_half32(hi + at, h, n);
+      block_spread(buf, lane, h);
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const float2 y = half_pair(h, q);
+        v[2 * q] = fmaf(fl, y.x, fp * v[2 * q]);
+        v[2 * q + 1] = fmaf(fl, y.y, fp * v[2 * q + 1]);
+      }
       if (rd_lo) {
-        if (n >= 32) {
+        block_spread(buf, lane, l);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float f[8];
-            unpack8(reinterpret_cast<const uint4*>(lo + at)[q], f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[8 * q + i] += f[i];
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (q < n) h[q] += __bfloat162float(lo[at + q]);
+        for (int q = 0; q < 16; ++q) {
+          const float2 y = bf16_pair(l, q);
+          v[2 * q] = fmaf(fl, y.x, v[2 * q]);
+          v[2 * q + 1] = fmaf(fl, y.y, v[2 * q + 1]);
         }
       }
-#pragma unroll
-      for (int q = 0; q < 32; ++q) v[q] = fmaf(fl, h[q], fp * v[q]);
       if (out) {
-        bf16* dst = out + at2(w.z, zso, row, ldo) + nc;
-        if (vec_out && n >= 32) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            reinterpret_cast<uint4*>(dst)[q] =
-                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (q < n) dst[q] = __float2bfloat16_rn(v[q]);
-        }
+        bf16* dst = out + w.z * zso + row * ldo + nc;
+        bf16_row(v, h);
+        if (vec_out)
+          block_store(buf, lane, h, reinterpret_cast<uint8_t*>(dst), n * 2, ok);
+        else
+          block_store_odd(buf, lane, h, dst, n, ok);
         continue;
       }
 #pragma unroll
       for (int q = 0; q < 32; ++q) v[q] *= kX;
-      store_half32(next + at, v, n);
+      half_row(v, h);
+      block_store(buf, lane, h, reinterpret_cast<uint8_t*>(next + at), n * 2, ok);
       if (wr_lo) {
 #pragma unroll
-        for (int q = 0; q < 32; ++q) v[q] -= __half2float(__float2half_rn(v[q]));
-        if (n >= 32) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            reinterpret_cast<uint4*>(lo + at)[q] =
-                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (q < n) lo[at + q] = __float2bfloat16_rn(v[q]);
+        for (int q = 0; q < 16; ++q) {
+          const float2 y = half_pair(h, q);
+          v[2 * q] -= y.x;
+          v[2 * q + 1] -= y.y;
         }
+        bf16_row(v, l);
+        block_store(buf, lane, l, reinterpret_cast<uint8_t*>(lo + at), n * 2, ok);
       }
     }
   }
@@ -286,15 +251,44 @@ __global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs
   __syncthreads();
   const float f = sh[0];
   const T* src = static_cast<const T*>(g.p[z]);
+  __half* h = hi + z * zs;
+  bf16* l = lo ? lo + z * zs : nullptr;
+  if (cols % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {  // ld == cols: one run of 8-element chunks
+    const int64_t n8 = (int64_t)rows * cols / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256) {
+      float v[8];
+      if (sizeof(T) == 2) {
+        unpack8(reinterpret_cast<const uint4*>(src)[i], v);
+      } else {
+        const float4 x = reinterpret_cast<const float4*>(src)[2 * i], y = reinterpret_cast<const float4*>(src)[2 * i + 1];
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= f;
+      const uint4 u = make_uint4(pack_half(v[0], v[1]), pack_half(v[2], v[3]), pack_half(v[4], v[5]), pack_half(v[6], v[7]));
+      reinterpret_cast<uint4*>(h)[i] = u;
+      if (l) {
+        const __half2* k = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 y = __half22float2(k[q]);
+          v[2 * q] -= y.x;
+          v[2 * q + 1] -= y.y;
+        }
+        reinterpret_cast<uint4*>(l)[i] =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+      }
+    }
+    return;
+  }
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* r = src + (int64_t)row * cols;
-    __half* h = hi + z * zs + row * ld;
-    bf16* l = lo ? lo + z * zs + row * ld : nullptr;
     for (int c = threadIdx.x; c < cols; c += 256) {
       const float v = to_f<T>(r[c]) * f;
       const __half q = __float2half_rn(v);
-      h[c] = q;
-      if (l) l[c] = __float2bfloat16_rn(v - __half2float(q));
+      h[row * ld + c] = q;
+      if (l) l[row * ld + c] = __float2bfloat16_rn(v - __half2float(q));
     }
   }
 }
@@ -600,7 +594,7 @@ cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fau
     // steps before the compensated ones read X as hi + lo
     const int comp0 = a.steps - kCompensated;
     bf16* lo0 = sizeof(T) == 4 && comp0 > 0 ? lo : nullptr;
-    orth_convert<T><<<dim3(std::min(m, 4 * sm_count()), cnt), 256, 0, st>>>(g, m, n, part, n_parts, a.eps, x[0], lo0,
+    orth_convert<T><<<dim3((unsigned)std::min<int64_t>(((int64_t)m * n + 2047) / 2048, cdiv(8 * sm_count(), cnt)), cnt), 256, 0, st>>>(g, m, n, part, n_parts, a.eps, x[0], lo0,
                                                                             p.ldx, p.xz, s0);
     TRY(cudaGetLastError());
     for (int i = 0; i < a.steps; ++i) {

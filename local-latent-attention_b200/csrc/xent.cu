@@ -57,9 +57,10 @@ struct EpiStats {
   int p_f32;           // fp32 instead of fp16 * 2^15
 
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero) const {
+                                       bool zero, uint8_t* buf) const {
     const int nv = min(kTile, a.N - col0);  // columns of this tile
     if (nv <= 0) return;                    // warp-uniform
+    const int lane = threadIdx.x % 32;
     const bool row_ok = row < M;
     int t = -1;
     if (row_ok) t = tgt ? tgt[row] : (int)max((int64_t)-1, min(tgt64[row], (int64_t)a.N));
@@ -86,6 +87,7 @@ struct EpiStats {
     // (the maximum itself gives exactly 1: a difference, not a fused product)
     const float mm = m == -INFINITY ? 0.f : m;
     float s0 = 0.f, s1 = 0.f;
+    const int64_t at = (int64_t)row * ldp + col0;
 #pragma unroll 1
     for (int cc = 0; cc < nv; cc += 32) {
       float v[32];
@@ -97,30 +99,23 @@ struct EpiStats {
         s0 += v[q];
         s1 += v[q + 1];
       }
-      if (p && row_ok) {
-        const int64_t at = (int64_t)row * ldp + col0 + cc;
-        if (p_f32) {
-          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-          const int n4 = min(8, (nv - cc + 3) / 4);  // ldp is a multiple of 8
+      if (!p) continue;
+      if (p_f32) {
+        uint4 u[8];
+        f32_row(v, u);
+        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(static_cast<float*>(p) + at + cc), (nv - cc) * 4, row_ok);
+      } else {
+        uint4 u[4];
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q < n4) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p) + at);
-          const int n8 = min(4, (nv - cc + 7) / 8);
-          const float k = 32768.f;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < n8)
-              dst[q] = make_uint4(pack_half(v[8 * q] * k, v[8 * q + 1] * k), pack_half(v[8 * q + 2] * k, v[8 * q + 3] * k),
-                                  pack_half(v[8 * q + 4] * k, v[8 * q + 5] * k),
-                                  pack_half(v[8 * q + 6] * k, v[8 * q + 7] * k));
-        }
+        for (int q = 0; q < 32; ++q) v[q] *= 32768.f;
+        half_row(v, u);
+        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(static_cast<__half*>(p) + at + cc), (nv - cc) * 2, row_ok);
       }
     }
     if (row_ok) {
       // every column -inf: nothing to add
-      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && !(s0 + s1 > 0.f) && !isnan(s0 + s1) ? -INFINITY : mm, s0 + s1);
+      const float sum = s0 + s1;
+      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && sum == 0.f ? -INFINITY : mm, sum);
       if ((unsigned)t < (unsigned)nv) lt[row] = tv;
     }
   }
@@ -132,65 +127,48 @@ struct EpiOut {
   void* out;
   int64_t ldo;
   int out_bf16;
-  int vec;              // 16-byte stores: base and row stride aligned
+  int vec;              // base and row stride 16-byte aligned (whole rows may be padded to 16 bytes)
   const float* acc;     // added first (fp32, row stride ldacc), or null
   int64_t ldacc;
   const int* idx;       // output row of row m, or null
   int64_t split_stride;
 
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero) const {
+                                       bool zero, uint8_t* buf) const {
+    const int lane = threadIdx.x % 32;
     const bool row_ok = row < M;
-    const int64_t orow = row_ok ? (idx ? idx[row] : row) : 0;
+    const int64_t orow = (row_ok ? (idx ? idx[row] : row) : 0) * ldo + (a.splits > 1 ? w.z * split_stride : 0);
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
-      const int nc = col0 + cc;
-      if (nc >= a.N) break;  // warp-uniform
+      const int nc = col0 + cc, n = a.N - nc;
+      if (n <= 0) break;  // warp-uniform
       float v[32];
-      load32(taddr + cc, zero, v);
-      if (!row_ok) continue;
-      const bool full = vec && nc + 32 <= a.N;
       if (acc) {
-        const float* src = acc + (int64_t)row * ldacc + nc;  // ldacc a multiple of 4
-        if (nc + 32 <= a.N) {
+        uint4 x[8];  // ldacc is a multiple of 8
+        block_fetch(lane, x, acc + (row_ok ? (int64_t)row * ldacc : 0) + nc, n * 4, row_ok);
+        load32(taddr + cc, zero, v);
+        block_spread(buf, lane, x);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float4 c = reinterpret_cast<const float4*>(src)[q];
-            v[4 * q] += c.x;
-            v[4 * q + 1] += c.y;
-            v[4 * q + 2] += c.z;
-            v[4 * q + 3] += c.w;
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (nc + q < a.N) v[q] += src[q];
-        }
+        for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(word(x, q));
+      } else {
+        load32(taddr + cc, zero, v);
       }
       if (out_bf16) {
-        bf16* dst = static_cast<bf16*>(out) + (a.splits > 1 ? w.z * split_stride : 0) + orow * ldo + nc;
-        if (full) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            reinterpret_cast<uint4*>(dst)[q] =
-                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (nc + q < a.N) dst[q] = __float2bfloat16_rn(v[q]);
-        }
+        uint4 u[4];
+        bf16* dst = static_cast<bf16*>(out) + orow + nc;
+        bf16_row(v, u);
+        if (vec)
+          block_store(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 2, row_ok);
+        else
+          block_store_odd(buf, lane, u, dst, n, row_ok);
       } else {
-        float* dst = static_cast<float*>(out) + (a.splits > 1 ? w.z * split_stride : 0) + orow * ldo + nc;
-        if (full) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            reinterpret_cast<float4*>(dst)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (nc + q < a.N) dst[q] = v[q];
-        }
+        uint4 u[8];
+        float* dst = static_cast<float*>(out) + orow + nc;
+        f32_row(v, u);
+        if (vec)
+          block_store(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 4, row_ok);
+        else
+          block_store_odd(buf, lane, u, dst, n, row_ok);
       }
     }
   }
@@ -228,14 +206,25 @@ __global__ void __launch_bounds__(1024) xent_compact(const int64_t* __restrict__
                                                      int* __restrict__ idx, int* __restrict__ tgt,
                                                      float* __restrict__ lt, int* __restrict__ count) {
   __shared__ int sums[32];
+  constexpr int PER = 8;  // consecutive targets per thread and round
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   int base = 0;
-  for (int i0 = 0; i0 < n; i0 += 1024) {
-    const int i = i0 + tid;
-    const int64_t t = i < n ? targets[i] : ignore;
-    const bool keep = t != ignore;
-    const unsigned b = __ballot_sync(0xffffffffu, keep);
-    if (lane == 0) sums[warp] = __popc(b);
+  for (int i0 = 0; i0 < n; i0 += 1024 * PER) {
+    int64_t t[PER];
+    int mine = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int i = i0 + tid * PER + q;
+      t[q] = i < n ? targets[i] : ignore;
+      mine += t[q] != ignore;
+    }
+    int upto = mine;  // inclusive scan over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      upto += lane >= o ? v : 0;
+    }
+    if (lane == 31) sums[warp] = upto;
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
@@ -244,11 +233,14 @@ __global__ void __launch_bounds__(1024) xent_compact(const int64_t* __restrict__
       before += w < warp ? c : 0;
       all += c;
     }
-    if (keep) {
-      const int j = base + before + __popc(b & ((1u << lane) - 1u));
-      idx[j] = i;
-      tgt[j] = t >= 0 && t < vocab ? (int)t : -1;
+    int j = base + before + upto - mine;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      if (t[q] == ignore) continue;
+      idx[j] = i0 + tid * PER + q;
+      tgt[j] = t[q] >= 0 && t[q] < vocab ? (int)t[q] : -1;
       lt[j] = __int_as_float(0x7fc00000);
+      ++j;
     }
     base += all;
     __syncthreads();
