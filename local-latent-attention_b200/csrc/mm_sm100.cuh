@@ -57,8 +57,12 @@ unsigned read_fault(bool reset) {
 struct MmArgs {
   int M, N, K;
   int a_mn, b_mn;
-  int nz;                   // batch elements (tensor-map z), 1 for the split forms
-  int splits, k_per_split;  // K ranges (multiples of 64), each its own output
+  int nz;                   // batch elements (tensor-map z)
+  // Split K of the tiles that do not fill a wave (and, min_splits > 1, of
+  // every tile into at least that many ranges): each range's sums go to part
+  // (fp32, one BM x BN block per range) and mm_join adds them up. 0: no split.
+  int split, min_splits;
+  float* part;
   int sym;                  // C symmetric: tiles with n <= m only (square tiles)
   int fp16;                 // operands fp16 instead of bf16
   // products over planes: operand z coordinates (pa, pb) of n_terms passes
@@ -166,23 +170,50 @@ struct MmShape {
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// work item -> (z or split, first row, first column)
 struct MmTile {
   int z, m0, n0;
 };
 
+// The schedule: total tiles, of which the first `full` run whole, one after
+// another on each CTA (pair), and the rest in s ranges of K each.
+struct MmPlan {
+  int total, full, s, items;
+};
+
+// s splits the last, partial wave of `units` so that it costs ceil(tail s /
+// units) / s of a whole one, each range at least 8 steps of K, and a hundredth
+// of a wave per range for the partial sums' way through memory (measured: a
+// 256 x 256 fp32 block costs about what 2 steps of K do).
+__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int min_splits) {
+  MmPlan r{total, total, 1, total};
+  if (!split || total == 0) return r;
+  const int full = min_splits > 1 ? 0 : total / units * units, tail = total - full;
+  if (tail == 0) return r;
+  int best = min_splits;
+  float cost = 1e30f;
+  for (int s = min_splits; s <= 32 || s == min_splits; ++s) {
+    if (s > min_splits && (ksteps < 8 * s || (int64_t)tail * s > 4 * (int64_t)units)) break;
+    const float c = (float)cdiv(tail * s, units) / (float)s + 0.01f * (float)s;
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  if (best == 1) return r;
+  return MmPlan{total, full, best, full + tail * best};
+}
+
 template <int CG>
 struct MmGrid {
-  int n_mt, n_nt, per_z, total;
-  __device__ __forceinline__ MmGrid(const MmArgs& p, int M) {
+  int n_mt, n_nt, per_z;
+  __host__ __device__ __forceinline__ MmGrid(const MmArgs& p, int M) {
     n_mt = cdiv(M, MmShape<CG>::BM);
     n_nt = cdiv(p.N, MmShape<CG>::BN);
     per_z = p.sym ? n_mt * (n_mt + 1) / 2 : n_mt * n_nt;
-    total = per_z * p.nz * p.splits;
   }
   __device__ __forceinline__ MmTile at(const MmArgs& p, int t) const {
     MmTile r;
-    r.z = t / per_z;
+    r.z = p.nz > 1 ? t / per_z : 0;
     int u = t - r.z * per_z, i, j;
     if (p.sym) {  // row i of the lower triangle holds i + 1 tiles
       i = (int)((sqrtf(8.f * u + 1.f) - 1.f) * 0.5f);
@@ -193,7 +224,7 @@ struct MmGrid {
       // bands of 8 row tiles, walked column by column: the tiles in flight
       // share about 8 row and 9 column strips of the operands in L2
       const int band = 8 * n_nt, bi = u / band, v = u - bi * band;
-      const int h = min(8, n_mt - bi * 8);
+      const int h = n_mt - bi * 8 < 8 ? n_mt - bi * 8 : 8;
       j = v / h;
       i = bi * 8 + (v - j * h);
     }
@@ -203,185 +234,22 @@ struct MmGrid {
   }
 };
 
+// item -> tile index, range of K [k0, k1), partial block (-1: whole)
+struct MmItem {
+  int tile, k0, k1, block;
+};
+__device__ __forceinline__ MmItem mm_item(const MmPlan& pl, int t, int K) {
+  if (t < pl.full) return {t, 0, K, -1};
+  const int u = t - pl.full, tile = u / pl.s, j = u - tile * pl.s;
+  const int per = cdiv(cdiv(K, 64), pl.s) * 64;
+  const int k0 = j * per;
+  return {pl.full + tile, k0, min(K, k0 + per), u};
+}
+
 __device__ __forceinline__ int cut_rows(int n, const int* dev, int base) {
   if (!dev) return n;
   const int v = *dev - base;
   return v < 0 ? 0 : (v < n ? v : n);
-}
-
-// Epi: struct with
-//   __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
-//                        uint8_t* buf) const
-// called by every thread of an epilogue warp (all 32 lanes, converged) for its
-// row and 128 columns [col0, col0 + 128); taddr: TMEM address of the warp's
-// lanes and columns; zero: the K range is empty, the accumulator holds
-// nothing; buf: the warp's staging block.
-template <int CG, typename Epi>
-__global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
-    mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-              const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
-  using S = MmShape<CG>;
-  constexpr int ST = S::ST;
-  extern __shared__ uint8_t mm_smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR);
-  uint64_t *full = bars, *empty = bars + ST, *acc_full = bars + 2 * ST, *acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int rank = CG == 2 ? (int)cluster_rank() : 0;
-  const int unit = blockIdx.x / CG, n_units = gridDim.x / CG;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], CG * S::EW);
-    }
-    *abort = 0;
-    fence_barrier_init();
-  }
-  if (warp == 1) {
-    __syncwarp();
-    mm_tmem_alloc<CG>(tmem_slot, 2 * S::BN);
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (CG == 2) cluster_sync();  // the peer's barriers are initialised
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // accumulator b at columns [b * BN, (b + 1) * BN)
-
-  const int M = cut_rows(p.M, p.m_dev, p.dev_base);
-  const int K = cut_rows(p.K, p.k_dev, p.dev_base);
-  const MmGrid<CG> grid(p, M);
-
-  if (warp == 0) {
-    if (lane == 0) {
-      prefetch_tmap(&tm_a);
-      prefetch_tmap(&tm_b);
-      int it = 0;
-      bool ok = true;
-      for (int t = unit; ok && t < grid.total; t += n_units) {
-        const MmTile w = grid.at(p, t);
-        const int k0 = p.splits > 1 ? w.z * p.k_per_split : 0;
-        const int k1 = p.splits > 1 ? min(K, k0 + p.k_per_split) : K;
-        const int zc = p.splits > 1 ? 0 : w.z;
-        const int ma = w.m0 + rank * 128, nb = w.n0 + rank * 128;
-        for (int term = 0; ok && term < p.n_terms; ++term) {
-          const int za = zc + (int)((p.pa >> (4 * term)) & 15u), zb = zc + (int)((p.pb >> (4 * term)) & 15u);
-          for (int k = k0; k < k1; k += 64, ++it) {
-            const int s = it % ST;
-            if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
-            if (rank == 0) mbar_expect_tx(&full[s], 2 * CG * S::OPB);
-            uint8_t* sa = smem + S::A + s * S::OPB;
-            uint8_t* sb = smem + S::B + s * S::OPB;
-            auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
-              if (CG == 1)
-                tma_load_3d(map, &full[s], dst, c0, c1, c2);
-              else
-                tma_load_3d_pair(map, &full[s], dst, c0, c1, c2);
-            };
-            if (p.a_mn) {
-              load(&tm_a, sa, ma, k, za);
-              load(&tm_a, sa + S::OPB / 2, ma + 64, k, za);
-            } else {
-              load(&tm_a, sa, k, ma, za);
-            }
-            if (p.b_mn) {
-              load(&tm_b, sb, nb, k, zb);
-              load(&tm_b, sb + S::OPB / 2, nb + 64, k, zb);
-            } else {
-              load(&tm_b, sb, k, nb, zb);
-            }
-          }
-        }
-      }
-      // every stage's last commit has arrived (in a pair, on this CTA's
-      // barrier too): none is in flight when the CTA exits
-      for (int i = it - ST < 0 ? 0 : it - ST; ok && i < it; ++i)
-        ok = mbar_wait(&empty[i % ST], (i / ST) & 1, abort, &g_mm_fault);
-      if (!ok) mm_raise(p, 1u, abort);
-      if (*abort && rank == 0) {  // let the copies already issued land before the CTA (pair) can exit
-        volatile int none = 0;
-        volatile unsigned gnone = 0;
-        for (int i = it - ST < 0 ? 0 : it - ST; i < it; ++i)
-          mbar_wait(&full[i % ST], (i / ST) & 1, &none, &gnone, 100000000ull);
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t fmt = p.fp16 ? 0u : 1u;
-      const uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | ((p.a_mn ? 1u : 0u) << 15) |
-                          ((p.b_mn ? 1u : 0u) << 16) | ((uint32_t)(S::BN >> 3) << 17) | ((uint32_t)(S::BM >> 4) << 24);
-      // K-major: a K step of 16 is 32 bytes of the 128-byte rows; MN-major: 16
-      // rows of 128 bytes, panels of 64 rows (MN) 8 KB apart
-      const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-      const uint32_t a_lbo = p.a_mn ? S::OPB / 2 : 16, b_lbo = p.b_mn ? S::OPB / 2 : 16;
-      int it = 0, k = 0;
-      bool ok = true;
-      for (int t = unit; ok && t < grid.total; t += n_units, ++k) {
-        const int z = grid.at(p, t).z, buf = k & 1;
-        const int k0 = p.splits > 1 ? z * p.k_per_split : 0;
-        const int k1 = p.splits > 1 ? min(K, k0 + p.k_per_split) : K;
-        const int steps = k1 > k0 ? cdiv(k1 - k0, 64) * p.n_terms : 0;
-        // the epilogue has read this accumulator's previous tile (k - 2)
-        if (k >= 2 && !(ok = mbar_wait(&acc_empty[buf], ((k >> 1) - 1) & 1, abort, &g_mm_fault))) break;
-        tc_fence_after();
-        for (int i = 0; i < steps; ++i, ++it) {
-          const int s = it % ST;
-          if (!(ok = mbar_wait(&full[s], (it / ST) & 1, abort, &g_mm_fault))) break;
-          tc_fence_after();
-          const uint64_t da = desc_sw128(smem_u32(smem + S::A + s * S::OPB), a_lbo, 1024);
-          const uint64_t db = desc_sw128(smem_u32(smem + S::B + s * S::OPB), b_lbo, 1024);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f16<CG>(tmem + S::BN * buf, desc_add(da, kk * a_step), desc_add(db, kk * b_step), id,
-                        (i > 0 || kk > 0) ? 1u : 0u);
-          commit<CG>(&empty[s]);
-        }
-        if (!ok) break;
-        commit<CG>(&acc_full[buf]);
-      }
-      if (!ok) mm_raise(p, 2u, abort);
-    }
-  } else {
-    const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns 128 half..
-    int k = 0;
-    bool ok = true;
-    for (int t = unit; t < grid.total; t += n_units, ++k) {
-      const int buf = k & 1;
-      const MmTile w = grid.at(p, t);
-      const int k0 = p.splits > 1 ? w.z * p.k_per_split : 0;
-      const int k1 = p.splits > 1 ? min(K, k0 + p.k_per_split) : K;
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (k >> 1) & 1, abort, &g_mm_fault));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t ta = tmem + S::BN * buf + 128 * half + ((uint32_t)(32 * quad) << 16);
-      epi.tile(p, w, w.m0 + rank * 128 + 32 * quad + lane, w.n0 + 128 * half, M, ta, k1 <= k0,
-               smem + S::STAGE + (warp - 2) * S::STG);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {  // this accumulator may take the tile after next
-        if (CG == 1)
-          mbar_arrive(&acc_empty[buf]);
-        else
-          mbar_arrive_leader(&acc_empty[buf]);
-      }
-    }
-    if (!ok) mm_raise(p, 8u, abort);
-  }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  if (CG == 2) cluster_sync();  // the peer reads this CTA's shared memory and arrives on its barriers until here
-  if (warp == 1) {
-    __syncwarp();
-    tc_fence_after();
-    mm_tmem_dealloc<CG>(tmem, 2 * S::BN);
-  }
 }
 
 // 32 accumulator columns of this thread's row
@@ -405,14 +273,8 @@ template <int CH>
 __device__ __forceinline__ int stage_at(int r, int c) {
   return CH == 8 ? r * 128 + ((c ^ (r & 7)) * 16) : r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
 }
-// p: the lane's own row's first byte (16-byte aligned), bytes: valid bytes of
-// the rows (rounded up to 16 in memory), ok: the lane's row exists.
 template <int CH>
-__device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 (&v)[CH], uint8_t* p, int bytes,
-                                            bool ok) {
-#pragma unroll
-  for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
-  __syncwarp();
+__device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, uint8_t* p, int bytes, bool ok) {
   const int c = lane % CH;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
@@ -422,6 +284,36 @@ __device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 
     if (q && 16 * c < bytes) *reinterpret_cast<uint4*>(q + 16 * c) = u;
   }
   __syncwarp();
+}
+// p: the lane's own row's first byte (16-byte aligned), bytes: valid bytes of
+// the rows (rounded up to 16 in memory), ok: the lane's row exists.
+template <int CH>
+__device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 (&v)[CH], uint8_t* p, int bytes,
+                                            bool ok) {
+#pragma unroll
+  for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
+  __syncwarp();
+  block_write_out<CH>(buf, lane, p, bytes, ok);
+}
+// After a block_store of 32 x 32 16-bit values: the block's transpose, column c
+// of it (lane = c) as the row at p. 8 x 8 matrices go through registers
+// (transposed on the load) into the second half of the staging block.
+__device__ __forceinline__ void block_mirror(uint8_t* buf, int lane, uint8_t* p, int bytes, bool ok) {
+  uint8_t* tb = buf + 2048;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t a, b, c, d;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+                 : "r"(smem_u32(buf + stage_at<4>(lane, j)))
+                 : "memory");
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     smem_u32(tb + stage_at<4>(8 * j + lane % 8, lane / 8))),
+                 "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+  }
+  __syncwarp();
+  block_write_out<4>(tb, lane, p, bytes, ok);
 }
 // The reverse, in two halves so that the caller may have several in flight:
 // fetch reads global memory, spread hands each thread its row (zeros where
@@ -500,6 +392,234 @@ __device__ __forceinline__ float2 bf16_pair(const uint4 (&u)[4], int i) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// one range's sums of a tile: its fp32 block of part, [BM][BN]
+template <int CG>
+__device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, const MmTile& w, int row, int col, int M,
+                                           uint32_t taddr, uint8_t* buf) {
+  using S = MmShape<CG>;
+  float* dst = p.part + ((int64_t)x.block * S::BM + row) * S::BN + col;
+#pragma unroll 1
+  for (int cc = 0; cc < 128; cc += 32) {
+    const int n = p.N - (w.n0 + col + cc);
+    if (n <= 0) break;  // warp-uniform
+    float v[32];
+    load32(taddr + cc, x.k1 <= x.k0, v);
+    uint4 u[8];
+    f32_row(v, u);
+    block_store(buf, threadIdx.x % 32, u, reinterpret_cast<uint8_t*>(dst + cc), n * 4, w.m0 + row < M);
+  }
+}
+
+// Epi: struct with
+//   __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
+//                        uint8_t* buf) const
+// called by every thread of an epilogue warp (all 32 lanes, converged) for its
+// row and 128 columns [col0, col0 + 128); taddr: TMEM address of the warp's
+// lanes and columns; zero: the K range is empty, the accumulator holds
+// nothing; buf: the warp's staging block.
+template <int CG, typename Epi>
+__global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
+    mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+              const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
+  using S = MmShape<CG>;
+  constexpr int ST = S::ST;
+  extern __shared__ uint8_t mm_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR);
+  uint64_t *full = bars, *empty = bars + ST, *acc_full = bars + 2 * ST, *acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  MmPlan* plan = reinterpret_cast<MmPlan*>(tmem_slot + 2);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = CG == 2 ? (int)cluster_rank() : 0;
+  const int unit = blockIdx.x / CG, n_units = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], CG * S::EW);
+    }
+    *abort = 0;
+    fence_barrier_init();
+    const MmGrid<CG> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
+    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    mm_tmem_alloc<CG>(tmem_slot, 2 * S::BN);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // the peer's barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // accumulator b at columns [b * BN, (b + 1) * BN)
+
+  const int M = cut_rows(p.M, p.m_dev, p.dev_base);
+  const int K = cut_rows(p.K, p.k_dev, p.dev_base);
+  const MmGrid<CG> grid(p, M);
+  const MmPlan pl = *plan;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm_a);
+      prefetch_tmap(&tm_b);
+      int it = 0;
+      bool ok = true;
+      for (int t = unit; ok && t < pl.items; t += n_units) {
+        const MmItem x = mm_item(pl, t, K);
+        const MmTile w = grid.at(p, x.tile);
+        const int ma = w.m0 + rank * 128, nb = w.n0 + rank * 128;
+        for (int term = 0; ok && term < p.n_terms; ++term) {
+          const int za = w.z + (int)((p.pa >> (4 * term)) & 15u), zb = w.z + (int)((p.pb >> (4 * term)) & 15u);
+          for (int k = x.k0; k < x.k1; k += 64, ++it) {
+            const int s = it % ST;
+            if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * CG * S::OPB);
+            uint8_t* sa = smem + S::A + s * S::OPB;
+            uint8_t* sb = smem + S::B + s * S::OPB;
+            auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
+              if (CG == 1)
+                tma_load_3d(map, &full[s], dst, c0, c1, c2);
+              else
+                tma_load_3d_pair(map, &full[s], dst, c0, c1, c2);
+            };
+            if (p.a_mn) {
+              load(&tm_a, sa, ma, k, za);
+              load(&tm_a, sa + S::OPB / 2, ma + 64, k, za);
+            } else {
+              load(&tm_a, sa, k, ma, za);
+            }
+            if (p.b_mn) {
+              load(&tm_b, sb, nb, k, zb);
+              load(&tm_b, sb + S::OPB / 2, nb + 64, k, zb);
+            } else {
+              load(&tm_b, sb, k, nb, zb);
+            }
+          }
+        }
+      }
+      // every stage's last commit has arrived (in a pair, on this CTA's
+      // barrier too): none is in flight when the CTA exits
+      for (int i = it - ST < 0 ? 0 : it - ST; ok && i < it; ++i)
+        ok = mbar_wait(&empty[i % ST], (i / ST) & 1, abort, &g_mm_fault);
+      if (!ok) mm_raise(p, 1u, abort);
+      if (*abort && rank == 0) {  // let the copies already issued land before the CTA (pair) can exit
+        volatile int none = 0;
+        volatile unsigned gnone = 0;
+        for (int i = it - ST < 0 ? 0 : it - ST; i < it; ++i)
+          mbar_wait(&full[i % ST], (i / ST) & 1, &none, &gnone, 100000000ull);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t fmt = p.fp16 ? 0u : 1u;
+      const uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | ((p.a_mn ? 1u : 0u) << 15) |
+                          ((p.b_mn ? 1u : 0u) << 16) | ((uint32_t)(S::BN >> 3) << 17) | ((uint32_t)(S::BM >> 4) << 24);
+      // K-major: a K step of 16 is 32 bytes of the 128-byte rows; MN-major: 16
+      // rows of 128 bytes, panels of 64 rows (MN) 8 KB apart
+      const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+      const uint32_t a_lbo = p.a_mn ? S::OPB / 2 : 16, b_lbo = p.b_mn ? S::OPB / 2 : 16;
+      int it = 0, k = 0;
+      bool ok = true;
+      for (int t = unit; ok && t < pl.items; t += n_units, ++k) {
+        const MmItem x = mm_item(pl, t, K);
+        const int buf = k & 1, steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
+        // the epilogue has read this accumulator's previous tile (k - 2)
+        if (k >= 2 && !(ok = mbar_wait(&acc_empty[buf], ((k >> 1) - 1) & 1, abort, &g_mm_fault))) break;
+        tc_fence_after();
+        for (int i = 0; i < steps; ++i, ++it) {
+          const int s = it % ST;
+          if (!(ok = mbar_wait(&full[s], (it / ST) & 1, abort, &g_mm_fault))) break;
+          tc_fence_after();
+          const uint64_t da = desc_sw128(smem_u32(smem + S::A + s * S::OPB), a_lbo, 1024);
+          const uint64_t db = desc_sw128(smem_u32(smem + S::B + s * S::OPB), b_lbo, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16<CG>(tmem + S::BN * buf, desc_add(da, kk * a_step), desc_add(db, kk * b_step), id,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+          commit<CG>(&empty[s]);
+        }
+        if (!ok) break;
+        commit<CG>(&acc_full[buf]);
+      }
+      if (!ok) mm_raise(p, 2u, abort);
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns 128 half..
+    int k = 0;
+    bool ok = true;
+    for (int t = unit; t < pl.items; t += n_units, ++k) {
+      const int buf = k & 1;
+      const MmItem x = mm_item(pl, t, K);
+      const MmTile w = grid.at(p, x.tile);
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (k >> 1) & 1, abort, &g_mm_fault));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t ta = tmem + S::BN * buf + 128 * half + ((uint32_t)(32 * quad) << 16);
+      uint8_t* stage = smem + S::STAGE + (warp - 2) * S::STG;
+      const int row = rank * 128 + 32 * quad + lane, col = 128 * half;
+      if (x.block < 0)
+        epi.tile(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage);
+      else
+        store_part<CG>(p, x, w, row, col, M, ta, stage);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {  // this accumulator may take the tile after next
+        if (CG == 1)
+          mbar_arrive(&acc_empty[buf]);
+        else
+          mbar_arrive_leader(&acc_empty[buf]);
+      }
+    }
+    if (!ok) mm_raise(p, 8u, abort);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // the peer reads this CTA's shared memory and arrives on its barriers until here
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    mm_tmem_dealloc<CG>(tmem, 2 * S::BN);
+  }
+}
+
+// Adds up the ranges of the split tiles in order, and hands 4 columns of a row
+// at a time to Epi::quad(row, col, n valid, values). grid (split tiles at
+// most, BM / 8), one warp per row.
+template <int CG, typename Epi>
+__global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi, int units) {
+  using S = MmShape<CG>;
+  __shared__ MmPlan plan;
+  const int M = cut_rows(p.M, p.m_dev, p.dev_base);
+  const MmGrid<CG> grid(p, M);
+  if (threadIdx.x == 0)
+    plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
+  __syncthreads();
+  const MmPlan pl = plan;
+  const int tile = pl.full + blockIdx.x;
+  if (tile >= pl.total) return;
+  const MmTile w = grid.at(p, tile);
+  const int r = blockIdx.y * 8 + threadIdx.x / 32, row = w.m0 + r;
+  if (row >= M) return;
+  const float* src = p.part + ((int64_t)blockIdx.x * pl.s * S::BM + r) * S::BN;
+  for (int c = threadIdx.x % 32 * 4; c < S::BN; c += 128) {
+    const int n = p.N - (w.n0 + c);
+    if (n <= 0) break;
+    float4 v = *reinterpret_cast<const float4*>(src + c);
+#pragma unroll 4
+    for (int s = 1; s < pl.s; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(src + (int64_t)s * S::BM * S::BN + c);
+      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+    }
+    epi.quad(row, w.n0 + c, min(4, n), v);
+  }
+}
+
 // ---- host side --------------------------------------------------------------
 
 // 3-D operand view: rows x cols with cols contiguous, row stride ld and z
@@ -510,17 +630,52 @@ struct Operand {
   int mn;  // stored MN-major (rows = K, cols = MN) instead of K-major (rows = MN, cols = K)
 };
 
+inline int mm_units(int cg) { return sm_count() / cg; }
+
+// Waves of a product on `units` CTAs (pairs), the last one split where allowed.
+inline double mm_waves(const MmPlan& pl, int units) {
+  return (double)(pl.full / units) + (pl.full % units ? 1.0 : 0.0) +
+         (pl.items > pl.full ? (double)cdiv(pl.items - pl.full, units) / pl.s + 0.01 * pl.s : 0.0);
+}
+
 // Which tile: the pair's 256 x 256 tile takes about twice a single 128 x 128
-// tile's time on twice the SMs, so the shorter schedule in tile times wins.
+// tile's time on twice the SMs (measured 1.6 against 1.3 PFLOP/s in long
+// products), so the shorter schedule in tile times wins.
 inline int pick_group(const MmArgs& p) {
-  auto tiles = [&](int b) {
-    const int64_t m = cdiv(p.M, b), n = cdiv(p.N, b);
-    return (p.sym ? m * (m + 1) / 2 : m * n) * p.nz * p.splits;
-  };
-  const int sms = sm_count();
-  const double t1 = (double)((tiles(128) + sms - 1) / sms) * 1.25;
-  const double t2 = (double)((tiles(256) + sms / 2 - 1) / (sms / 2)) * 2.0;
+  const MmGrid<1> g1(p, p.M);
+  const MmGrid<2> g2(p, p.M);
+  const int u1 = mm_units(1), u2 = mm_units(2), ks = cdiv(p.K, 64);
+  const double t1 = mm_waves(mm_plan(g1.per_z * p.nz, u1, ks, p.split, p.min_splits), u1) * 1.25;
+  const double t2 = mm_waves(mm_plan(g2.per_z * p.nz, u2, ks, p.split, p.min_splits), u2) * 2.0;
   return t2 <= t1 ? 2 : 1;
+}
+
+// fp32 elements of MmArgs::part for a product of at most these sizes
+inline int64_t mm_part_floats(const MmArgs& p) {
+  if (!p.split) return 0;
+  const MmGrid<1> g1(p, p.M);
+  const MmGrid<2> g2(p, p.M);
+  // below the caps of mm_plan: 4 waves of ranges, or min_splits of every tile
+  const int64_t n1 = std::max<int64_t>(4 * mm_units(1), (int64_t)g1.per_z * p.nz * p.min_splits);
+  const int64_t n2 = std::max<int64_t>(4 * mm_units(2), (int64_t)g2.per_z * p.nz * p.min_splits);
+  return p.min_splits > 1 ? std::max(n1 * 128 * 128, n2 * 256 * 256)
+                          : std::max((int64_t)4 * mm_units(1) * 128 * 128, (int64_t)4 * mm_units(2) * 256 * 256);
+}
+
+template <int CG, typename Epi>
+cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t s, decltype(&Epi::quad)) {
+  using S = MmShape<CG>;
+  const MmGrid<CG> g(p, p.M);
+  const int total = g.per_z * p.nz;
+  // the device may have fewer tiles than the host's sizes say, never more
+  const int tail = p.min_splits > 1 ? total : std::min(total, units - 1);
+  if (tail < 1) return cudaSuccess;
+  mm_join<CG, Epi><<<dim3(tail, S::BM / 8), 256, 0, s>>>(p, epi, units);
+  return cudaGetLastError();
+}
+template <int CG, typename Epi>
+cudaError_t launch_join(const MmArgs&, const Epi&, int, cudaStream_t, ...) {
+  return cudaErrorInvalidValue;  // an epilogue without quad() cannot be split
 }
 
 template <int CG, typename Epi>
@@ -530,10 +685,9 @@ cudaError_t launch_mm_cg(const MmArgs& p, const CUtensorMap& ta, const CUtensorM
   cudaError_t e = set_smem_once(mm_kernel<CG, Epi>, S::SMEM);
   if (e != cudaSuccess) return e;
   const int64_t m = cdiv(p.M, S::BM), n = cdiv(p.N, S::BN);
-  const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz * p.splits;
-  if (tiles < 1) return cudaSuccess;
-  if (tiles > 0x3fffffff) return cudaErrorInvalidValue;
-  const int64_t units = std::min<int64_t>(tiles, sm_count() / CG);
+  const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
+  if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
+  const int units = p.split ? mm_units(CG) : (int)std::min<int64_t>(tiles, mm_units(CG));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * CG));
   cfg.blockDim = dim3(S::THREADS);
@@ -544,7 +698,9 @@ cudaError_t launch_mm_cg(const MmArgs& p, const CUtensorMap& ta, const CUtensorM
   at[0].val.clusterDim = {CG, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = CG == 2 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, mm_kernel<CG, Epi>, ta, tb, p, epi);
+  e = cudaLaunchKernelEx(&cfg, mm_kernel<CG, Epi>, ta, tb, p, epi);
+  if (e != cudaSuccess || !p.split) return e;
+  return launch_join<CG, Epi>(p, epi, units, s, nullptr);
 }
 
 template <typename Epi>
@@ -552,10 +708,10 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
   CUtensorMap ta, tb;
   p.a_mn = a.mn;
   p.b_mn = b.mn;
-  if (p.splits < 1) p.splits = 1;
+  if (p.min_splits < 1) p.min_splits = 1;
   if (p.nz < 1) p.nz = 1;
   if (p.n_terms < 1) p.n_terms = 1;
-  if (p.M < 1 || p.N < 1 || p.K < 1) return cudaErrorInvalidValue;
+  if (p.M < 1 || p.N < 1 || p.K < 1 || (p.split && !p.part)) return cudaErrorInvalidValue;
   if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
       !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : 128))
     return cudaErrorInvalidValue;

@@ -51,12 +51,16 @@ struct Ptrs {
   const void* p[kPtrs];
 };
 
-// mirror image of 32 columns of a row: element (row, nc + q) -> (nc + q, row);
-// the warp's 32 rows are consecutive, so each q is one 64-byte segment
-__device__ __forceinline__ void store_mirror(__half* base, int64_t ld, int row, int nc, const float (&v)[32], int n) {
-#pragma unroll
-  for (int q = 0; q < 32; ++q)
-    if (q < n) base[(int64_t)(nc + q) * ld + row] = __float2half_rn(v[q]);
+// Stores 32 columns of a symmetric matrix's tile, and off the diagonal their
+// mirror image: column nc + lane of the block becomes that row, from row0 on.
+__device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, MmTile w, int row, int nc, int M, int N,
+                                                const float (&v)[32], uint8_t* buf) {
+  const int lane = threadIdx.x % 32, row0 = row - lane;
+  uint4 u[4];
+  half_row(v, u);
+  block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), (N - nc) * 2, row < M);
+  if (w.m0 != w.n0)
+    block_mirror(buf, lane, reinterpret_cast<uint8_t*>(base + (nc + lane) * ld + row0), (M - row0) * 2, nc + lane < N);
 }
 
 // S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
@@ -66,22 +70,18 @@ struct EpiGram {
   const float* s0;  // first step: X = s0[z] * stored, else null (2^-6)
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
-    const int lane = threadIdx.x % 32;
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float f = x * x * kS;
     __half* base = s + w.z * zs;
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
-      const int nc = col0 + cc, n = a.N - nc;
-      if (n <= 0) break;
+      const int nc = col0 + cc;
+      if (nc >= a.N) break;
       float v[32];
       load32(taddr + cc, zero, v);
 #pragma unroll
       for (int q = 0; q < 32; ++q) v[q] *= f;
-      uint4 u[4];
-      half_row(v, u);
-      block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), n * 2, row < M);
-      if (w.m0 != w.n0 && row < M) store_mirror(base, ld, row, nc, v, n);
+      store_symmetric(base, ld, w, row, nc, M, a.N, v, buf);
     }
   }
 };
@@ -111,9 +111,7 @@ struct EpiPoly {
         v[2 * q] = fmaf(cb, x.x, cc2 * v[2 * q]) + (row == nc + 2 * q ? k : 0.f);
         v[2 * q + 1] = fmaf(cb, x.y, cc2 * v[2 * q + 1]) + (row == nc + 2 * q + 1 ? k : 0.f);
       }
-      half_row(v, u);
-      block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), n * 2, row < M);
-      if (w.m0 != w.n0 && row < M) store_mirror(base, ld, row, nc, v, n);
+      store_symmetric(base, ld, w, row, nc, M, a.N, v, buf);
     }
   }
 };

@@ -131,13 +131,37 @@ struct EpiOut {
   const float* acc;     // added first (fp32, row stride ldacc), or null
   int64_t ldacc;
   const int* idx;       // output row of row m, or null
-  int64_t split_stride;
+
+  // 4 columns of a row of a split tile, joined
+  __device__ __forceinline__ void quad(int row, int col, int n, float4 v) const {
+    if (acc) {
+      const float4 c = *reinterpret_cast<const float4*>(acc + (int64_t)row * ldacc + col);
+      v = make_float4(v.x + c.x, v.y + c.y, v.z + c.z, v.w + c.w);
+    }
+    const int64_t at = (int64_t)(idx ? idx[row] : row) * ldo + col;
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    if (out_bf16) {
+      bf16* dst = static_cast<bf16*>(out) + at;
+      if (vec) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+      } else {
+        for (int q = 0; q < n; ++q) dst[q] = __float2bfloat16_rn(x[q]);
+      }
+    } else {
+      float* dst = static_cast<float*>(out) + at;
+      if (vec) {
+        *reinterpret_cast<float4*>(dst) = v;
+      } else {
+        for (int q = 0; q < n; ++q) dst[q] = x[q];
+      }
+    }
+  }
 
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32;
     const bool row_ok = row < M;
-    const int64_t orow = (row_ok ? (idx ? idx[row] : row) : 0) * ldo + (a.splits > 1 ? w.z * split_stride : 0);
+    const int64_t orow = (row_ok ? (idx ? idx[row] : row) : 0) * ldo;
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
@@ -435,22 +459,6 @@ __global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ lo
   if (threadIdx.x == 0) *loss = mean ? s / fmaxf(c, 1.f) : s;
 }
 
-// dx[idx[r]] = sum over the splits of part[s][r]
-template <typename T>
-__global__ void __launch_bounds__(256) xent_join(const float* __restrict__ part, int splits, int64_t stride, int rows,
-                                                 const int* __restrict__ count, int base, const int* __restrict__ idx,
-                                                 int d, int64_t ldpart, T* __restrict__ dx, int64_t lddx) {
-  const int row = blockIdx.x;
-  if (row >= cut_rows(rows, count, base)) return;
-  const float* src = part + (int64_t)row * ldpart;
-  T* dst = dx + (int64_t)idx[row] * lddx;
-  for (int c = threadIdx.x; c < d; c += 256) {
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += src[s * stride + c];
-    dst[c] = from_f<T>(v);
-  }
-}
-
 // buf *= *s unless *s is 1
 template <typename T>
 __global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ buf, int64_t n, const float* __restrict__ s) {
@@ -471,10 +479,39 @@ bool aligned_rows(const void* p, int64_t ld, int64_t rows, int elt) {
 
 struct Plan {
   bool f32, train, pack_x, pack_w;
-  int elt, planes, n_tiles, piece, n_pieces, dx_splits, dx_k;
+  int elt, planes, n_tiles, piece, n_pieces, dx_splits;
   int64_t ldx, ldw, ldp, ldd;
   size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, acc, part, total;
 };
+
+MmArgs base_args(const Plan& q, volatile unsigned* fault) {
+  MmArgs p = {};
+  p.n_terms = q.f32 ? 6 : 1;
+  p.pa = q.f32 ? kTermsA : 0;
+  p.pb = q.f32 ? kTermsB : 0;
+  p.nz = p.min_splits = 1;
+  p.fault_host = fault;
+  return p;
+}
+
+// dx = G w and dw = G^T x of a piece
+MmArgs dx_args(const Plan& q, const llattn_xent_args& a, int rows, volatile unsigned* fault) {
+  MmArgs m = base_args(q, fault);
+  m.M = rows;
+  m.N = a.d;
+  m.K = a.vocab;
+  m.split = 1;
+  m.min_splits = q.dx_splits;
+  return m;
+}
+MmArgs dw_args(const Plan& q, const llattn_xent_args& a, int rows, volatile unsigned* fault) {
+  MmArgs m = base_args(q, fault);
+  m.M = a.vocab;
+  m.N = a.d;
+  m.K = rows;
+  m.split = 1;
+  return m;
+}
 
 Plan make_plan(const llattn_xent_args& a) {
   Plan q;
@@ -502,13 +539,7 @@ Plan make_plan(const llattn_xent_args& a) {
   q.piece = (int)std::min<int64_t>(piece, a.tokens);
   if (!q.train) q.piece = a.tokens;
   q.n_pieces = cdiv(a.tokens, q.piece);
-  // few rows: split the long K = V of dx = G w over the SMs
-  const int64_t t = (int64_t)cdiv(q.piece, 128) * cdiv(a.d, 128);
-  const int ksteps = cdiv(a.vocab, 64);
-  int sp = (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / t, ksteps / 8));
-  if (q.f32) sp = std::max(sp, cdiv(a.vocab, kF32Chain));
-  q.dx_k = cdiv(ksteps, sp) * 64;
-  q.dx_splits = cdiv(a.vocab, q.dx_k);
+  q.dx_splits = q.f32 ? cdiv(a.vocab, kF32Chain) : 1;
   size_t off = 0;
   auto take = [&](size_t b) { size_t o = off; off += up256(b); return o; };
   const size_t n = a.tokens;
@@ -523,19 +554,12 @@ Plan make_plan(const llattn_xent_args& a) {
   q.p = take(q.train ? (size_t)q.piece * q.ldp * q.elt : 0);
   q.gplanes = take(q.train && q.f32 ? 6 * (size_t)q.piece * q.ldp : 0);
   q.acc = take(q.train && a.dw && q.n_pieces > 1 ? 4 * (size_t)a.vocab * q.ldd : 0);
-  q.part = take(q.train && a.dx && q.dx_splits > 1 ? 4 * (size_t)q.dx_splits * q.piece * q.ldd : 0);
+  int64_t part = 0;
+  if (a.dx) part = mm_part_floats(dx_args(q, a, q.piece, nullptr));
+  if (a.dw) part = std::max(part, mm_part_floats(dw_args(q, a, q.piece, nullptr)));
+  q.part = take(q.train ? 4 * (size_t)part : 0);
   q.total = off;
   return q;
-}
-
-MmArgs base_args(const Plan& q, volatile unsigned* fault) {
-  MmArgs p = {};
-  p.n_terms = q.f32 ? 6 : 1;
-  p.pa = q.f32 ? kTermsA : 0;
-  p.pb = q.f32 ? kTermsB : 0;
-  p.nz = p.splits = 1;
-  p.fault_host = fault;
-  return p;
 }
 
 #define TRY(x)                          \
@@ -595,7 +619,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   void* pbuf = ws + q.p;
   bf16* gpl = reinterpret_cast<bf16*>(ws + q.gplanes);
   float* acc = reinterpret_cast<float*>(ws + q.acc);
-  float* part = reinterpret_cast<float*>(ws + q.part);
+  float* part = reinterpret_cast<float*>(ws + q.part);  // split tiles of one product at a time
   const int64_t gplane = (int64_t)q.piece * q.ldp;
   for (int c = 0; c < q.n_pieces; ++c) {
     const int base = c * q.piece, rows = std::min(q.piece, n - base);
@@ -614,42 +638,24 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     TRY(cudaGetLastError());
     const void* g = q.f32 ? (const void*)gpl : pbuf;
     if (dx) {
-      MmArgs m = base_args(q, fault);
+      MmArgs m = dx_args(q, a, rows, fault);
       m.m_dev = count;
       m.dev_base = base;
-      m.M = rows;
-      m.N = d;
-      m.K = V;
-      m.splits = q.dx_splits;
-      m.k_per_split = q.dx_k;
+      m.part = part;
       EpiOut eo{};
-      if (q.dx_splits > 1) {
-        eo.out = part;
-        eo.ldo = q.ldd;
-        eo.vec = 1;
-        eo.split_stride = (int64_t)q.piece * q.ldd;
-      } else {
-        eo.out = dx;
-        eo.ldo = d;
-        eo.out_bf16 = !q.f32;
-        eo.vec = aligned_rows(dx, d, 2, q.elt);
-        eo.idx = idx + base;
-      }
+      eo.out = dx;
+      eo.ldo = d;
+      eo.out_bf16 = !q.f32;
+      eo.vec = aligned_rows(dx, d, 2, q.elt);
+      eo.idx = idx + base;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
                     s));
-      if (q.dx_splits > 1) {
-        xent_join<T><<<rows, 256, 0, s>>>(part, q.dx_splits, eo.split_stride, rows, count, base, idx + base, d, q.ldd, dx,
-                                          d);
-        TRY(cudaGetLastError());
-      }
     }
     if (a.dw) {
-      MmArgs m = base_args(q, fault);
+      MmArgs m = dw_args(q, a, rows, fault);
       m.k_dev = count;
       m.dev_base = base;
-      m.M = V;
-      m.N = d;
-      m.K = rows;
+      m.part = part;
       EpiOut eo{};
       const bool last = c + 1 == q.n_pieces;
       eo.out = last ? a.dw : acc;
@@ -676,7 +682,7 @@ size_t workspace_bytes(const llattn_xent_args& a) { return make_plan(a).total; }
 int launches(const llattn_xent_args& a) {
   const Plan q = make_plan(a);
   if (!q.train) return q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
-  return q.pack_w + 2 + q.n_pieces * (2 + (a.dx ? 1 + (q.dx_splits > 1) : 0) + (a.dw ? 1 : 0)) + (a.loss ? 1 : 0);
+  return q.pack_w + 2 + q.n_pieces * (2 + (a.dx ? 2 : 0) + (a.dw ? 2 : 0)) + (a.loss ? 1 : 0);
 }
 
 cudaError_t launch(const llattn_xent_args& a, volatile unsigned* fault, cudaStream_t s) {
