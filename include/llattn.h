@@ -353,9 +353,10 @@ typedef struct llattn_xent_args {
 LLATTN_API size_t llattn_xent_workspace_bytes(const llattn_xent_args* args);
 LLATTN_API int llattn_xent(const llattn_xent_args* args, void* stream);
 
-/* buf[i] *= *factor (device scalar) over n elements of dtype; a factor of 1
- * leaves buf untouched. The upstream gradient of llattn_xent's loss. */
-LLATTN_API int llattn_scale(void* buf, int64_t n, int dtype, const float* factor, void* stream);
+/* a[i] *= *factor (device scalar) over na elements of dtype, and b over nb
+ * (either may be NULL with 0 elements); a factor of 1 leaves them untouched.
+ * The upstream gradient of llattn_xent's loss, onto dx and dw. */
+LLATTN_API int llattn_scale(void* a, int64_t na, void* b, int64_t nb, int dtype, const float* factor, void* stream);
 
 /* Orthogonalised updates: per matrix g_i [rows, cols] (contiguous),
  *   X = g / (|g|_F + eps); `steps` times: S = X X^T, X = a X + (b S + c S^2) X

@@ -129,7 +129,7 @@ def lib() -> ctypes.CDLL:
         L.llattn_xent_workspace_bytes.restype = ctypes.c_size_t
         L.llattn_xent.argtypes = [ctypes.POINTER(XentArgs), _vp]
         L.llattn_xent.restype = ctypes.c_int
-        L.llattn_scale.argtypes = [_vp, ctypes.c_int64, ctypes.c_int, _vp, _vp]
+        L.llattn_scale.argtypes = [_vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int, _vp, _vp]
         L.llattn_scale.restype = ctypes.c_int
         L.llattn_orth_workspace_bytes.argtypes = [ctypes.POINTER(OrthArgs)]
         L.llattn_orth_workspace_bytes.restype = ctypes.c_size_t

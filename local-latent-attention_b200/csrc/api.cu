@@ -729,10 +729,11 @@ int llattn_xent(const llattn_xent_args* a, void* stream) {
   return check_launch(xent::launch(*a, g.fault_host, s), "xent");
 }
 
-int llattn_scale(void* buf, int64_t n, int dtype, const float* factor, void* stream) {
-  if (!buf || !factor || n < 1) return fail(LLATTN_ERR_ARG, "scale: NULL pointer or n < 1");
+int llattn_scale(void* a, int64_t na, void* b, int64_t nb, int dtype, const float* factor, void* stream) {
+  if (!factor || na < 0 || nb < 0 || (na && !a) || (nb && !b) || na + nb < 1)
+    return fail(LLATTN_ERR_ARG, "scale: NULL pointer or nothing to scale");
   if (dtype != LLATTN_F32 && dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", dtype);
-  return check_launch(xent::launch_scale(buf, n, dtype, factor, static_cast<cudaStream_t>(stream)), "scale");
+  return check_launch(xent::launch_scale(a, na, b, nb, dtype, factor, static_cast<cudaStream_t>(stream)), "scale");
 }
 
 static int check_orth(const llattn_orth_args* a) {

@@ -379,6 +379,18 @@ __device__ __forceinline__ void f32_row(const float (&v)[32], uint4 (&u)[8]) {
     u[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
                       __float_as_uint(v[4 * q + 3]));
 }
+// 64 accumulator columns of this thread's row as bf16
+__device__ __forceinline__ void row64_bf16(uint32_t taddr, bool zero, uint4 (&u)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[32];
+    load32(taddr + 32 * h, zero, v);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      u[4 * h + q] = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                                pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+  }
+}
 template <int CH>
 __device__ __forceinline__ uint32_t word(const uint4 (&u)[CH], int i) {
   return i % 4 == 0 ? u[i / 4].x : i % 4 == 1 ? u[i / 4].y : i % 4 == 2 ? u[i / 4].z : u[i / 4].w;
@@ -662,6 +674,9 @@ inline int64_t mm_part_floats(const MmArgs& p) {
                           : std::max((int64_t)4 * mm_units(1) * 128 * 128, (int64_t)4 * mm_units(2) * 256 * 256);
 }
 
+// whether mm_plan may split anything, whatever the device-side counts
+inline bool joins(const MmArgs& p) { return p.split && (p.min_splits > 1 || cdiv(p.K, 64) >= 16); }
+
 template <int CG, typename Epi>
 cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t s, decltype(&Epi::quad)) {
   using S = MmShape<CG>;
@@ -699,7 +714,7 @@ cudaError_t launch_mm_cg(const MmArgs& p, const CUtensorMap& ta, const CUtensorM
   cfg.attrs = at;
   cfg.numAttrs = CG == 2 ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, mm_kernel<CG, Epi>, ta, tb, p, epi);
-  if (e != cudaSuccess || !p.split) return e;
+  if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<CG, Epi>(p, epi, units, s, nullptr);
 }
 

@@ -292,74 +292,151 @@ __global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs
 }
 
 // ---- small matrices ---------------------------------------------------------
-// q <= 64: the whole iteration in one launch, in fp32 on the CUDA cores. A
-// cluster of CL CTAs holds one matrix, each CTA a slice of its long side in
-// shared memory as x [q][slice]; per step each CTA takes its slice's part of
-// S, the parts are summed over the cluster's shared memory (fixed order), every
-// CTA forms B for itself and updates its slice. Rows are interleaved over the
-// threads (row = ti + R r) and padded to 4 mod 32 floats, so the 16-byte
-// shared-memory loads of a quarter warp meet all 32 banks.
-constexpr int kSmallQ = 64, kSmallT = 256;
+// Short side q <= 128: the whole iteration in one launch. A cluster of CL CTAs
+// holds one matrix, each CTA a slice of its long side in shared memory; per
+// step each CTA forms its slice's part of S, the parts are summed over the
+// cluster's shared memory (fixed order, every CTA a share of the elements
+// handed to all), every CTA forms B for itself and updates its slice. What
+// bounds it is the length of that chain (two cluster barriers a step), not
+// bytes or flops: a few 10 MFLOP, so the products run on mma.sync from
+// shared memory, which needs no descriptors, TMEM or copies in between.
+//
+// X, S and B are fp16 pairs hi + lo (22 bits), scaled by 2^8, and each product
+// sums hi hi + hi lo + lo hi in fp32: the result is exact to about 1e-6
+// before its rounding. Rows are padded by 16 bytes, an odd number of 16-byte
+// slots, so ldmatrix meets all banks.
+constexpr int kSmallQ = 128, kSmallT = 256, kSmallW = kSmallT / 32;
+constexpr float kSm = 256.f;
 
 struct SmallShape {
-  int q, R, w, wp, bp;  // short side, row quads, slice, padded slice, padded q
-  __host__ __device__ SmallShape(int q_, int L, int CL) {
-    q = q_;
-    R = cdiv(q, 4);
-    w = cdiv(cdiv(L, CL), 4) * 4;
-    wp = cdiv(w, 32) * 32 + 4;
-    bp = cdiv(4 * R, 32) * 32 + 4;
+  int q, L, w, wp, qp, fp;  // padded short side, slice, row strides of X, of S / B (halves) and of the parts (floats)
+  int mt, ng, units, groups;
+  __host__ __device__ SmallShape(int q_, int L_, int CL) {
+    q = cdiv(q_, 16) * 16;
+    L = L_;
+    w = cdiv(cdiv(L, CL), 16) * 16;
+    wp = w + 8;
+    qp = q + 8;
+    fp = q + 4;
+    mt = q / 16;
+    ng = cdiv(q / 8, 4);  // groups of up to 4 column tiles of 8
+    units = mt * ng;
+    groups = units >= kSmallW ? 1 : kSmallW / units;  // ranges of K side by side
   }
-  // x, S, B, this CTA's part of S, group partials
-  __host__ __device__ int floats() const { return 4 * R * (wp + 3 * bp) + kSmallT * 16; }
+  // X hi, lo; S (then B) hi, lo; parts of S
+  __host__ __device__ int bytes() const { return 2 * (2 * q * wp + 2 * q * qp) + 4 * groups * q * fp; }
 };
 
-// out[i][j] (+ epilogue f) = sum_k a[i][k] a[j][k], k < w (a multiple of 4), a
-// [4R][ld]; thread groups share k, joined through part
-template <typename F>
-__device__ __forceinline__ void small_gram(const float* a, int ld, int w, int R, float* part, F f) {
-  const int n_t = R * R, groups = max(1, kSmallT / n_t);
-  const int g = threadIdx.x / n_t, u = threadIdx.x - g * n_t;
-  const bool on = g < groups;
-  const int ti = u / R, tj = u - ti * R;  // R <= 16: R * R <= 256 threads
-  uint64_t acc[4][4];
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], const __half* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldm2t(uint32_t (&r)[2], const __half* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(smem_u32(p))
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void split2(float v, __half& h, __half& l) {
+  h = __float2half_rn(v);
+  l = __float2half_rn(v - __half2float(h));
+}
+__device__ __forceinline__ void split2x2(float a, float b, __half2& h, __half2& l) {
+  h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  l = __floats2half2_rn(a - f.x, b - f.y);
+}
+
+// One unit of a symmetric product Y Y^T, Y = hi + lo [.., ld] halves: rows
+// [16 m, 16 m + 16) x columns [32 n, 32 n + 32) (as far as q), K steps of 16
+// from k0 by dk
+__device__ __forceinline__ void small_product(const __half* hi, const __half* lo, int ld, int q, int m, int n, int k0,
+                                              int k1, int dk, float (&acc)[4][4]) {
+  const int lane = threadIdx.x % 32;
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[r][c] = 0;
-  if (on) {
-    for (int k = 4 * g; k < w; k += 4 * groups) {
-      ulonglong2 x[4], y[4];
+    for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+  // A: lane -> row lane % 16, K half lane / 16; B (two column tiles a load):
+  // lane -> row lane % 8 of tile lane / 16, K half (lane / 8) % 2
+  const int ao = (16 * m + lane % 16) * ld + lane / 16 * 8;
+  const int bo = (32 * n + lane / 16 * 8 + lane % 8) * ld + lane / 8 % 2 * 8;
+  const int nt = min(4, (q - 32 * n) / 8);  // 2 or 4
+#pragma unroll 2
+  for (int k = k0; k < k1; k += dk) {
+    uint32_t ah[4], al[4];
+    ldm4(ah, hi + ao + k);
+    ldm4(al, lo + ao + k);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = *reinterpret_cast<const ulonglong2*>(a + (ti + R * r) * ld + k);
-        y[r] = *reinterpret_cast<const ulonglong2*>(a + (tj + R * r) * ld + k);
+    for (int t = 0; t < 4; t += 2) {
+      if (t >= nt) break;
+      uint32_t bh[4], bl[4];
+      ldm4(bh, hi + bo + t * 8 * ld + k);
+      ldm4(bl, lo + bo + t * 8 * ld + k);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mma16816(acc[t + j], al, bh[2 * j], bh[2 * j + 1]);
+        mma16816(acc[t + j], ah, bl[2 * j], bl[2 * j + 1]);
+        mma16816(acc[t + j], ah, bh[2 * j], bh[2 * j + 1]);
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] = f2_fma(x[r].y, y[c].y, f2_fma(x[r].x, y[c].x, acc[r][c]));
     }
   }
-  __syncthreads();  // the previous readers of part are done
-  if (on) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float lo, hi;
-        f2_unpack(acc[r][c], lo, hi);
-        part[(4 * r + c) * kSmallT + threadIdx.x] = lo + hi;
+}
+
+// the slice's elements of the matrix in memory order of the slice, 8 at a
+// time where aligned: f(i, j, value) with i along the short side
+template <typename T, typename F>
+__device__ __forceinline__ void small_read(const T* src, bool tall, int q, int L, int j0, int jn, F f) {
+  // wide: q runs of jn; tall: one run of jn q
+  const int runs = tall ? 1 : q, len = tall ? jn * q : jn;
+  const int64_t start = tall ? (int64_t)j0 * q : j0, step = tall ? 0 : L;
+  const bool vec = len % 8 == 0 && start % 8 == 0 && step % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  if (vec) {
+    const int per = len / 8, n = runs * per;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < n; e += kSmallT) {
+      const int r = e / per, c = (e - r * per) * 8;
+      const T* p = src + start + r * step + c;
+      float v[8];
+      if (sizeof(T) == 2) {
+        unpack8(*reinterpret_cast<const uint4*>(p), v);
+      } else {
+        const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (tall) {
+          const int j = (c + k) / q;
+          f(c + k - j * q, j, v[k]);
+        } else {
+          f(r, c + k, v[k]);
+        }
+      }
+    }
+    return;
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < 16 * n_t; e += kSmallT) {
-    const int rc = e / n_t, v = e - rc * n_t;
-    float s = 0.f;
-    for (int h = 0; h < groups; ++h) s += part[rc * kSmallT + h * n_t + v];
-    f(v / R + R * (rc / 4), v % R + R * (rc % 4), s);
+  const int n = runs * len;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < n; e += kSmallT) {
+    const int r = e / max(len, 1), c = e - r * len;
+    const float v = to_f<T>(src[start + r * step + c]);
+    if (tall) {
+      const int j = c / q;
+      f(c - j * q, j, v);
+    } else {
+      f(r, c, v);
+    }
   }
-  __syncthreads();
 }
 
 template <typename T>
@@ -372,141 +449,200 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
   const bool tall = rows > cols;
   const int q = tall ? cols : rows, L = tall ? rows : cols;
   const SmallShape h(q, L, CL);
-  extern __shared__ float4 orth_smem[];
-  float* x = reinterpret_cast<float*>(orth_smem);
-  float* S = x + 4 * h.R * h.wp;
-  float* B = S + 4 * h.R * h.bp;
-  float* P = B + 4 * h.R * h.bp;
-  float* part = P + 4 * h.R * h.bp;
-  __shared__ float red[8], total;
-  const int tid = threadIdx.x, j0 = rank * h.w, jn = max(0, min(h.w, L - j0));
+  extern __shared__ uint4 orth_smem[];
+  __half* xh = reinterpret_cast<__half*>(orth_smem);
+  __half* xl = xh + h.q * h.wp;
+  __half* sh = xl + h.q * h.wp;
+  __half* sl = sh + h.q * h.qp;
+  float* P = reinterpret_cast<float*>(sl + h.q * h.qp);
+  __shared__ float red[kSmallW], total;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int j0 = rank * h.w, jn = max(0, min(h.w, L - j0));
   const T* src = static_cast<const T*>(g.p[z]);
 
-  for (int i = tid; i < 4 * h.R * h.wp; i += kSmallT) x[i] = 0.f;
-  __syncthreads();
   float s = 0.f;
-  if (tall) {  // rows j0.. of the matrix: consecutive memory
-    for (int64_t e = tid; e < (int64_t)jn * q; e += kSmallT) {
-      const int j = (int)(e / q), i = (int)(e - (int64_t)j * q);
-      const float v = to_f<T>(src[(int64_t)j0 * q + e]);
-      x[i * h.wp + j] = v;
-      s = fmaf(v, v, s);
-    }
-  } else {
-    for (int i = 0; i < q; ++i)
-      for (int j = tid; j < jn; j += kSmallT) {
-        const float v = to_f<T>(src[(int64_t)i * cols + j0 + j]);
-        x[i * h.wp + j] = v;
-        s = fmaf(v, v, s);
-      }
-  }
+  small_read(src, tall, q, L, j0, jn, [&](int, int, float v) { s = fmaf(v, v, s); });
   s = warp_sum(s);
-  if (tid % 32 == 0) red[tid / 32] = s;
+  if (lane == 0) red[warp] = s;
+  for (int i = tid; i < 2 * h.q * h.wp / 8; i += kSmallT) orth_smem[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (tid == 0) {
     float r = 0.f;
-    for (int i = 0; i < 8; ++i) r += red[i];
+    for (int i = 0; i < kSmallW; ++i) r += red[i];
     total = r;
   }
   cluster.sync();
   float sum = 0.f;
   for (int r = 0; r < CL; ++r) sum += *cluster.map_shared_rank(&total, r);
   const float inv = 1.f / (sqrtf(sum) + eps);
-  for (int i = tid; i < 4 * h.R * h.wp; i += kSmallT) x[i] *= inv;
+  small_read(src, tall, q, L, j0, jn,
+             [&](int i, int j, float v) { split2(v * inv * kSm, xh[i * h.wp + j], xl[i * h.wp + j]); });
   __syncthreads();
 
+  const int fr = lane / 4, fc = lane % 4 * 2;  // an accumulator's first row and column
   for (int step = 0; step < steps; ++step) {
-    small_gram(x, h.wp, h.w, h.R, part, [&](int i, int j, float v) { P[i * h.bp + j] = v; });
-    cluster.sync();
-    // every CTA sums its share of the quads over the cluster and gives the
-    // result to all: the next product's parts are written after this second
-    // barrier, the next S after the first one of the next step
-    for (int e = tid * CL + rank; e < 4 * h.R * h.R; e += kSmallT * CL) {
-      const int at = e / h.R * h.bp + e % h.R * 4;
-      float4 v[8];
+    // this slice's part of S, the K ranges' one after another in P
+    for (int u = warp; u < h.units * h.groups; u += kSmallW) {
+      const int gr = u / h.units, v = u - gr * h.units, m = v / h.ng, n = v - m * h.ng;
+      float acc[4][4];
+      small_product(xh, xl, h.wp, h.q, m, n, 16 * gr, h.w, 16 * h.groups, acc);
+      float* dst = P + gr * h.q * h.fp + (16 * m + fr) * h.fp + 32 * n + fc;
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < CL) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(P, r) + at);
-      float4 t = v[0];
-#pragma unroll
-      for (int r = 1; r < 8; ++r)
-        if (r < CL) t = make_float4(t.x + v[r].x, t.y + v[r].y, t.z + v[r].z, t.w + v[r].w);
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < CL) *reinterpret_cast<float4*>(cluster.map_shared_rank(S, r) + at) = t;
+      for (int t = 0; t < 4; ++t) {
+        if (32 * n + 8 * t >= h.q) break;
+        *reinterpret_cast<float2*>(dst + 8 * t) = make_float2(acc[t][0], acc[t][1]);
+        *reinterpret_cast<float2*>(dst + 8 * h.fp + 8 * t) = make_float2(acc[t][2], acc[t][3]);
+      }
+    }
+    if (h.groups > 1) {
+      __syncthreads();
+      for (int e = tid; e < h.q * h.q; e += kSmallT) {
+        const int at = e / h.q * h.fp + e % h.q;
+        float v = P[at];
+        for (int gr = 1; gr < h.groups; ++gr) v += P[gr * h.q * h.fp + at];
+        P[at] = v;
+      }
     }
     cluster.sync();
-    small_gram(S, h.bp, 4 * h.R, h.R, part, [&](int i, int j, float v) { B[i * h.bp + j] = fmaf(cb, S[i * h.bp + j], cc * v); });
-    // x = a x + B x, columns in chunks: every thread holds its results until the chunk has been read
-    const int strips = kSmallT / h.R, tj = tid / h.R, ti = tid - tj * h.R;
-    for (int c0 = 0; c0 < h.w; c0 += 4 * strips) {
-      const int c = c0 + 4 * tj;
-      const bool on = tj < strips && c < h.w;
-      uint64_t acc[4][2];
-      if (on) {
+    // every CTA sums its share of the quads over the cluster and gives the
+    // result to all: the next step's parts are written after the second
+    // barrier, the next S after that step's first one
+    for (int e = tid * CL + rank; e < h.q * h.q / 4; e += kSmallT * CL) {
+      const int i = e / (h.q / 4), j = (e - i * (h.q / 4)) * 4;
+      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int r0 = 0; r0 < CL; r0 += 8) {
+        float4 v[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float4 v = *reinterpret_cast<const float4*>(x + (ti + h.R * r) * h.wp + c);
-          acc[r][0] = f2_pack(ca * v.x, ca * v.y);
-          acc[r][1] = f2_pack(ca * v.z, ca * v.w);
-        }
-        for (int k = 0; k < 4 * h.R; k += 4) {
-          float4 b[4];
-          ulonglong2 y[4];
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r < CL) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(P, r0 + r) + i * h.fp + j);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            b[r] = *reinterpret_cast<const float4*>(B + (ti + h.R * r) * h.bp + k);
-            y[r] = *reinterpret_cast<const ulonglong2*>(x + (k + r) * h.wp + c);
-          }
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r < CL) t = make_float4(t.x + v[r].x, t.y + v[r].y, t.z + v[r].z, t.w + v[r].w);
+      }
+      // products of 2^8 X: S 2^16 -> S 2^8
+      __half2 hi[2], lo[2];
+      split2x2(t.x / kSm, t.y / kSm, hi[0], lo[0]);
+      split2x2(t.z / kSm, t.w / kSm, hi[1], lo[1]);
+      const int at = i * h.qp + j;
+      for (int r = 0; r < CL; ++r) {
+        *reinterpret_cast<uint2*>(cluster.map_shared_rank(sh, r) + at) = *reinterpret_cast<const uint2*>(hi);
+        *reinterpret_cast<uint2*>(cluster.map_shared_rank(sl, r) + at) = *reinterpret_cast<const uint2*>(lo);
+      }
+    }
+    cluster.sync();
+    // B = b S + c S^2 over S, once every warp has read what it needs (up to 4
+    // units a warp, held in registers)
+    {
+      float acc[4][4][4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float bk[4] = {b[r].x, b[r].y, b[r].z, b[r].w};
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const uint64_t d = f2_pack(bk[m], bk[m]);
-              acc[r][0] = f2_fma(d, y[m].x, acc[r][0]);
-              acc[r][1] = f2_fma(d, y[m].y, acc[r][1]);
-            }
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int u = warp + kSmallW * i;
+        if (u < h.units) small_product(sh, sl, h.qp, h.q, u / h.ng, u % h.ng, 0, h.q, 16, acc[i]);
       }
       __syncthreads();
-      if (on) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          *reinterpret_cast<ulonglong2*>(x + (ti + h.R * r) * h.wp + c) = make_ulonglong2(acc[r][0], acc[r][1]);
+      for (int i = 0; i < 4; ++i) {
+        const int u = warp + kSmallW * i;
+        if (u >= h.units) break;
+        const int m = u / h.ng, n = u - m * h.ng, at = (16 * m + fr) * h.qp + 32 * n + fc;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (32 * n + 8 * t >= h.q) break;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            __half2* ph = reinterpret_cast<__half2*>(sh + at + 8 * t + 8 * k * h.qp);
+            __half2* pl = reinterpret_cast<__half2*>(sl + at + 8 * t + 8 * k * h.qp);
+            const float2 x = __half22float2(*ph), y = __half22float2(*pl);
+            split2x2(fmaf(cb, x.x + y.x, cc / kSm * acc[i][t][2 * k]), fmaf(cb, x.y + y.y, cc / kSm * acc[i][t][2 * k + 1]),
+                     *ph, *pl);
+          }
+        }
       }
+    }
+    __syncthreads();
+    // X = a X + B X: a warp owns column tiles of 8 and reads no others, so it
+    // overwrites them in place; 64 rows at a time would read rows already
+    // new, so all row tiles' sums are held (up to 8)
+    for (int c0 = 8 * warp; c0 < h.w; c0 += 8 * kSmallW) {
+      float acc[8][4];
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
+      for (int k = 0; k < h.q; k += 16) {
+        uint32_t bh[2], bl[2];
+        ldm2t(bh, xh + (k + lane % 16) * h.wp + c0);
+        ldm2t(bl, xl + (k + lane % 16) * h.wp + c0);
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          if (m >= h.mt) break;
+          uint32_t ah[4], al[4];
+          const int ao = (16 * m + lane % 16) * h.qp + lane / 16 * 8 + k;
+          ldm4(ah, sh + ao);
+          ldm4(al, sl + ao);
+          mma16816(acc[m], al, bh[0], bh[1]);
+          mma16816(acc[m], ah, bl[0], bl[1]);
+          mma16816(acc[m], ah, bh[0], bh[1]);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        if (m >= h.mt) break;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = (16 * m + fr + 8 * k) * h.wp + c0 + fc;
+          __half2* ph = reinterpret_cast<__half2*>(xh + at);
+          __half2* pl = reinterpret_cast<__half2*>(xl + at);
+          const float2 x = __half22float2(*ph), y = __half22float2(*pl);
+          split2x2(fmaf(ca, x.x + y.x, acc[m][2 * k] / kSm), fmaf(ca, x.y + y.y, acc[m][2 * k + 1] / kSm), *ph, *pl);
+        }
+      }
+      __syncwarp();
     }
     __syncthreads();
   }
   bf16* dst = out + (int64_t)z * rows * cols;
+  auto value = [&](int i, int j) {
+    return __float2bfloat16_rn((__half2float(xh[i * h.wp + j]) + __half2float(xl[i * h.wp + j])) / kSm);
+  };
   if (tall) {
-    for (int64_t e = tid; e < (int64_t)jn * q; e += kSmallT) {
-      const int j = (int)(e / q), i = (int)(e - (int64_t)j * q);
-      dst[(int64_t)j0 * q + e] = __float2bfloat16_rn(x[i * h.wp + j]);
+#pragma unroll 4
+    for (int e = tid; e < jn * q; e += kSmallT) {
+      const int j = e / q;
+      dst[(int64_t)j0 * q + e] = value(e - j * q, j);
     }
   } else {
-    for (int i = 0; i < q; ++i)
-      for (int j = tid; j < jn; j += kSmallT) dst[(int64_t)i * cols + j0 + j] = __float2bfloat16_rn(x[i * h.wp + j]);
+#pragma unroll 4
+    for (int e = tid; e < jn * q; e += kSmallT) {
+      const int i = e / jn, j = e - i * jn;
+      dst[(int64_t)i * cols + j0 + j] = value(i, j);
+    }
   }
   cluster.sync();  // the others have read this CTA's parts
 }
 
-// CTAs per matrix of the one-launch form, 0 where it does not apply: up to 8,
-// at least 32 columns each
+// CTAs per matrix of the one-launch form, 0 where it does not apply: the
+// smallest number whose slices are at most 64 wide or, past 8 (16 needs the
+// opt-in), that fit shared memory.
 int small_cluster(const llattn_orth_args& a) {
   const int q = std::min(a.rows, a.cols), L = std::max(a.rows, a.cols);
   if (q > kSmallQ) return 0;
   int cl = 1;
-  while (cl < 8 && L > 32 * cl) cl *= 2;
-  return SmallShape(q, L, cl).floats() * 4 <= 220 * 1024 ? cl : 0;
+  while (cl < 16 && L > 96 * cl) cl *= 2;
+  return SmallShape(q, L, cl).bytes() <= 220 * 1024 ? cl : 0;
 }
 
 template <typename T>
 cudaError_t run_small(const llattn_orth_args& a, int cl, cudaStream_t st) {
-  const int smem = SmallShape(std::min(a.rows, a.cols), std::max(a.rows, a.cols), cl).floats() * 4;
+  const int smem = SmallShape(std::min(a.rows, a.cols), std::max(a.rows, a.cols), cl).bytes();
   cudaError_t e = set_smem_once(orth_small<T>, smem);
   if (e != cudaSuccess) return e;
+  if (cl > 8) {
+    e = cudaFuncSetAttribute(orth_small<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
   for (int i0 = 0; i0 < a.count; i0 += kPtrs) {
     const int cnt = std::min(kPtrs, a.count - i0);
     Ptrs g;

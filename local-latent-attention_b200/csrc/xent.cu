@@ -17,7 +17,7 @@
 // piece in place as bf16 G, which the other two products read. One pass over
 // the exponentials (4 bytes per element) replaces a second 2 N V d product.
 //
-// Gradients run over the tokens that count only: xent_compact lists them (in
+// Gradients run over the tokens that count only: xent_prep lists them (in
 // order), the sizes of the products follow the device-side count, and rows
 // of ignored tokens are never read, so their values cannot reach dw.
 //
@@ -162,6 +162,17 @@ struct EpiOut {
     const int lane = threadIdx.x % 32;
     const bool row_ok = row < M;
     const int64_t orow = (row_ok ? (idx ? idx[row] : row) : 0) * ldo;
+    if (out_bf16 && vec && !acc) {  // 64 columns, whole 128-byte lines, at a time
+#pragma unroll 1
+      for (int cc = 0; cc < 128; cc += 64) {
+        const int nc = col0 + cc, n = a.N - nc;
+        if (n <= 0) break;
+        uint4 u[8];
+        row64_bf16(taddr + cc, zero, u);
+        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(static_cast<bf16*>(out) + orow + nc), n * 2, row_ok);
+      }
+      return;
+    }
 #pragma unroll 1
     for (int cc = 0; cc < 128; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
@@ -223,55 +234,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return r;
 }
 
-// The tokens that count, in order: idx[j] = row of the j-th, tgt[j] = its
-// target (-1: out of range, which makes the row's loss and gradients NaN);
-// count. lt[j] starts at NaN for the same reason. One CTA.
-__global__ void __launch_bounds__(1024) xent_compact(const int64_t* __restrict__ targets, int n, int64_t ignore, int vocab,
-                                                     int* __restrict__ idx, int* __restrict__ tgt,
-                                                     float* __restrict__ lt, int* __restrict__ count) {
-  __shared__ int sums[32];
-  constexpr int PER = 8;  // consecutive targets per thread and round
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  int base = 0;
-  for (int i0 = 0; i0 < n; i0 += 1024 * PER) {
-    int64_t t[PER];
-    int mine = 0;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int i = i0 + tid * PER + q;
-      t[q] = i < n ? targets[i] : ignore;
-      mine += t[q] != ignore;
-    }
-    int upto = mine;  // inclusive scan over the warp
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      upto += lane >= o ? v : 0;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < 32; ++w) {
-      const int c = sums[w];
-      before += w < warp ? c : 0;
-      all += c;
-    }
-    int j = base + before + upto - mine;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      if (t[q] == ignore) continue;
-      idx[j] = i0 + tid * PER + q;
-      tgt[j] = t[q] >= 0 && t[q] < vocab ? (int)t[q] : -1;
-      lt[j] = __int_as_float(0x7fc00000);
-      ++j;
-    }
-    base += all;
-    __syncthreads();
-  }
-  if (tid == 0) *count = base;
-}
-
 // fp32 -> three bf16 planes whose sum is the value to 2^-24
 __device__ __forceinline__ void split3(float v, bf16& a, bf16& b, bf16& c) {
   a = __float2bfloat16_rn(v);
@@ -280,27 +242,19 @@ __device__ __forceinline__ void split3(float v, bf16& a, bf16& b, bf16& c) {
   c = __float2bfloat16_rn(r - __bfloat162float(b));
 }
 
-// One CTA per row of the source: xs[j] = x[idx[j]] (bf16, or three planes of
-// fp32) for j < count, zeros past it and in the padding columns; idx ==
-// nullptr copies rows straight. Also zeros the dx rows of ignored tokens.
+// A warp's row: dst = src (bf16, or three planes of fp32), zeros from column d
+// to lds, or everywhere where src is null.
 template <typename T>
-__global__ void __launch_bounds__(128) xent_gather(const T* __restrict__ x, int64_t ldx, int d, const int* __restrict__ idx,
-                                                   const int* __restrict__ count, bf16* __restrict__ xs, int64_t lds,
-                                                   int64_t plane, const int64_t* __restrict__ targets, int64_t ignore,
-                                                   T* __restrict__ dx, int64_t lddx) {
-  const int64_t j = blockIdx.x;
-  if (dx && targets[j] == ignore)
-    for (int c = threadIdx.x; c < d; c += 128) dx[j * lddx + c] = from_f<T>(0.f);
-  const bool live = !idx || j < *count;
-  const T* src = x + (live ? (idx ? (int64_t)idx[j] : j) : 0) * ldx;
-  bf16* dst = xs + j * lds;
-  if (sizeof(T) == 2 && live && ldx % 8 == 0 && d % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-    for (int c = threadIdx.x; c < d / 8; c += 128)
-      reinterpret_cast<uint4*>(dst)[c] = reinterpret_cast<const uint4*>(src)[c];
+__device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t lds, int64_t plane, bool vec) {
+  const int lane = threadIdx.x % 32;
+  if (sizeof(T) == 2 && (vec || !src)) {  // d a multiple of 8, 16-byte aligned rows
+#pragma unroll 8
+    for (int c = lane; c < lds / 8; c += 32)
+      reinterpret_cast<uint4*>(dst)[c] = src ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
     return;
   }
-  for (int c = threadIdx.x; c < lds; c += 128) {
-    const float v = live && c < d ? to_f<T>(src[c]) : 0.f;
+  for (int c = lane; c < lds; c += 32) {
+    const float v = src && c < d ? to_f<T>(src[c]) : 0.f;
     if (sizeof(T) == 2) {
       dst[c] = __float2bfloat16_rn(v);
     } else {
@@ -309,6 +263,102 @@ __global__ void __launch_bounds__(128) xent_gather(const T* __restrict__ x, int6
       dst[c] = a;
       dst[plane + c] = b;
       dst[2 * plane + c] = e;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool vec_rows(const T* p, int64_t ld, int d) {
+  return ld % 8 == 0 && d % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// rows of a matrix, packed; one warp per row
+template <typename T>
+__global__ void __launch_bounds__(256) xent_pack(const T* __restrict__ x, int64_t ldx, int n, int d, bf16* __restrict__ xs,
+                                                 int64_t lds, int64_t plane) {
+  const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d));
+}
+
+// Before the products of a training call. Lists the tokens that count, in
+// order: idx[j] = row of the j-th, tgt[j] = its target (-1: out of range, which
+// makes the row's loss and gradients NaN; lt[j] starts at NaN for the same
+// reason), *count; packs their rows of x, xs[j] = x[idx[j]], and zeros the rows
+// past the count and the dx rows of ignored tokens. Each CTA takes `per` rows
+// (a multiple of 8) and counts the targets before them for itself: reading a
+// few hundred KB from L2 again costs less than a second launch or a wait
+// (measured 56 us for one CTA's scan of 32768 targets, 12 us this way with the
+// rows packed as well). The first n_w CTAs pack w instead, 64 rows each.
+template <typename T>
+__global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_t ldx, int d,
+                                                 const int64_t* __restrict__ targets, int n, int64_t ignore, int vocab,
+                                                 int per, int* __restrict__ idx, int* __restrict__ tgt,
+                                                 float* __restrict__ lt, int* __restrict__ count, bf16* __restrict__ xs,
+                                                 int64_t lds, int64_t plane, T* __restrict__ dx, const T* __restrict__ w,
+                                                 int64_t ldw, bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w) {
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  if ((int)blockIdx.x < n_w) {
+    const bool v = vec_rows(w, ldw, d);
+    for (int64_t r = (int64_t)blockIdx.x * 64 + warp; r < min(vocab, ((int)blockIdx.x + 1) * 64); r += 8)
+      pack_row<T>(w + r * ldw, d, wp + r * ldwp, ldwp, wplane, v);
+    return;
+  }
+  __shared__ int red[2][8], pos[256];
+  const int r0 = (blockIdx.x - n_w) * per, r1 = min(n, r0 + per);
+  int before = 0, all = 0;
+#pragma unroll 8
+  for (int i = tid; i < n; i += 256) {
+    const int k = targets[i] != ignore;
+    all += k;
+    before += i < r0 ? k : 0;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (lane == 0) {
+    red[0][warp] = before;
+    red[1][warp] = all;
+  }
+  __syncthreads();
+  before = all = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    before += red[0][i];
+    all += red[1][i];
+  }
+  if (blockIdx.x == n_w && tid == 0) {
+    count[0] = all;
+    count[1] = 0;  // rows done (xent_rows)
+  }
+  const bool vec = vec_rows(x, ldx, d);
+  for (int c0 = r0; c0 < r1; c0 += 256) {
+    const int i = c0 + tid;
+    const int64_t t = i < r1 ? targets[i] : ignore;
+    const bool keep = t != ignore;
+    const unsigned b = __ballot_sync(0xffffffffu, keep);
+    __syncthreads();
+    if (lane == 0) red[0][warp] = __popc(b);
+    __syncthreads();
+    int j = before + __popc(b & ((1u << lane) - 1u));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      j += k < warp ? red[0][k] : 0;
+      before += red[0][k];
+    }
+    pos[tid] = keep ? j : -1;
+    if (keep) {
+      idx[j] = i;
+      tgt[j] = t >= 0 && t < vocab ? (int)t : -1;
+      lt[j] = __int_as_float(0x7fc00000);
+    }
+    __syncthreads();
+    for (int k = warp; k < min(256, r1 - c0); k += 8) {
+      const int64_t row = c0 + k;
+      if (pos[k] >= 0) {
+        pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec);
+      } else if (dx) {
+        for (int c = lane; c < d; c += 32) dx[row * d + c] = from_f<T>(0.f);
+      }
+      if (row >= all) pack_row<T>(nullptr, d, xs + row * lds, lds, plane, vec);
     }
   }
 }
@@ -354,19 +404,40 @@ __global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ st
   }
 }
 
+// The last of the grid's CTAs to come here sums losses[0, n) into *loss.
+__device__ __forceinline__ void sum_losses(int* count, const float* losses, int n, int mean, float* loss, float* red,
+                                           int* last) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    *last = atomicAdd(count + 1, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!*last) return;
+  __threadfence();
+  float s = 0.f;
+#pragma unroll 32
+  for (int i = threadIdx.x; i < n; i += 256) s += __ldcg(losses + i);
+  s = block_sum<256>(s, red);
+  if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
+}
+
 // One CTA per row of a piece: joins the tiles, writes the row's loss and
 // rewrites the exponentials as G = g (p - onehot) (bf16 in place of fp16, or
 // fp32 -> three bf16 planes). Rows between the count and the next multiple
-// of 64 become zeros: the third product reads them.
+// of 64 become zeros: the third product reads them. The last CTA of the last
+// piece to finish sums the losses (thread t those of index t mod 256, then
+// in thread order: the same bits whichever CTA it is).
 template <bool F32>
 __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stats, int n_tiles, int rows, int vocab,
-                                                 const int* __restrict__ count, int base, const int* __restrict__ idx,
+                                                 int* __restrict__ count, int base, const int* __restrict__ idx,
                                                  const int* __restrict__ tgt, const float* __restrict__ lt,
-                                                 const float* __restrict__ grad_rows, int mean, float* __restrict__ losses,
+                                                 const float* __restrict__ grad_rows, int mean, float* losses,
                                                  void* __restrict__ p, int64_t ldp, bf16* __restrict__ planes,
-                                                 int64_t plane) {
+                                                 int64_t plane, float* __restrict__ loss) {
   extern __shared__ float xent_f[];  // [n_tiles]
   __shared__ float red[8];
+  __shared__ int last;
   const int n_all = *count;
   const int n = cut_rows(rows, count, base);
   const int64_t row = blockIdx.x;
@@ -381,12 +452,13 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
         }
       }
     }
+    if (loss) sum_losses(count, losses, n_all, mean, loss, red, &last);
     return;
   }
   const float2* st = stats + row * n_tiles;
   const float2 lse = join_tiles<256>(st, n_tiles, red);
   const int t = tgt[row];
-  if (threadIdx.x == 0 && losses) losses[row] = row_loss(lse, lt[row]);
+  if (threadIdx.x == 0) losses[base + row] = row_loss(lse, lt[row]);
   float g = grad_rows ? grad_rows[idx[row]] : (mean ? 1.f / (float)n_all : 1.f);
   if (t < 0) g = __int_as_float(0x7fc00000);
   // tile factors: g 2^(m_tile - lse)
@@ -436,36 +508,47 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
           make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
     }
   }
+  if (loss) sum_losses(count, losses, n_all, mean, loss, red, &last);
 }
 
-// loss = sum of the losses (compact list of *count, or all n with the ignored
-// tokens' zeros), over the number that count when mean. One CTA, fixed order.
-__global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ losses, int n, const int* __restrict__ count,
+// loss = sum of the losses (ignored tokens' are 0), over the number that count
+// when mean. One CTA, fixed order.
+__global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ losses, int n,
                                                     const int64_t* __restrict__ targets, int64_t ignore, int mean,
                                                     float* __restrict__ loss) {
   __shared__ float red[32];
-  const int m = count ? *count : n;
   float s = 0.f, c = 0.f;
-  for (int i = threadIdx.x; i < m; i += 1024) {
+  for (int i = threadIdx.x; i < n; i += 1024) {
     s += losses[i];
-    if (!count && targets[i] != ignore) c += 1.f;  // per thread: exact up to 2^24
+    c += targets[i] != ignore ? 1.f : 0.f;  // per thread: exact up to 2^24
   }
   s = block_sum<1024>(s, red);
-  if (!count) {
-    c = block_sum<1024>(c, red);
-  } else {
-    c = (float)m;
-  }
+  c = block_sum<1024>(c, red);
   if (threadIdx.x == 0) *loss = mean ? s / fmaxf(c, 1.f) : s;
 }
 
-// buf *= *s unless *s is 1
+// a *= *s, b *= *s, unless *s is 1; whole 16-byte chunks where aligned
 template <typename T>
-__global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ buf, int64_t n, const float* __restrict__ s) {
+__device__ __forceinline__ void scale_run(T* p, int64_t n, float f) {
+  constexpr int PER = 16 / sizeof(T);
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  const int64_t nv = (reinterpret_cast<uintptr_t>(p) & 15) ? 0 : n / PER;
+  for (int64_t i = i0; i < nv; i += step) {
+    uint4 u = reinterpret_cast<uint4*>(p)[i];
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) e[q] = from_f<T>(to_f<T>(e[q]) * f);
+    reinterpret_cast<uint4*>(p)[i] = u;
+  }
+  for (int64_t i = nv * PER + i0; i < n; i += step) p[i] = from_f<T>(to_f<T>(p[i]) * f);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ a, int64_t na, T* __restrict__ b, int64_t nb,
+                                                    const float* __restrict__ s) {
   const float f = *s;
   if (f == 1.f) return;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    buf[i] = from_f<T>(to_f<T>(buf[i]) * f);
+  scale_run(a, na, f);
+  scale_run(b, nb, f);
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -549,7 +632,7 @@ Plan make_plan(const llattn_xent_args& a) {
   q.lt = take(4 * n);
   q.idx = take(q.train ? 4 * n : 0);
   q.tgt = take(q.train ? 4 * n : 0);
-  q.count = take(4);
+  q.count = take(8);
   q.losses = take(4 * n);
   q.p = take(q.train ? (size_t)q.piece * q.ldp * q.elt : 0);
   q.gplanes = take(q.train && q.f32 ? 6 * (size_t)q.piece * q.ldp : 0);
@@ -581,16 +664,14 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   const int n = a.tokens, d = a.d, V = a.vocab;
   const bool mean = a.reduction == LLATTN_XENT_MEAN;
   const int64_t xplane = (int64_t)n * q.ldx, wplane = (int64_t)V * q.ldw;
-  if (q.pack_w) {
-    xent_gather<T><<<V, 128, 0, s>>>(static_cast<const T*>(a.w), a.ldw, d, nullptr, nullptr, wp, q.ldw, wplane, nullptr,
-                                     0, nullptr, 0);
-    TRY(cudaGetLastError());
-  }
   const void* wv = q.pack_w ? wp : a.w;
   if (!q.train) {
+    if (q.pack_w) {
+      xent_pack<T><<<cdiv(V, 8), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane);
+      TRY(cudaGetLastError());
+    }
     if (q.pack_x) {
-      xent_gather<T><<<n, 128, 0, s>>>(static_cast<const T*>(a.x), a.ldx, d, nullptr, nullptr, xs, q.ldx, xplane, nullptr,
-                                       0, nullptr, 0);
+      xent_pack<T><<<cdiv(n, 8), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane);
       TRY(cudaGetLastError());
     }
     MmArgs p = base_args(q, fault);
@@ -604,16 +685,16 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     xent_losses<<<cdiv(n, 4), 128, 0, s>>>(stats, q.n_tiles, n, lt, a.targets, a.ignore_index, V, losses);
     TRY(cudaGetLastError());
     if (a.loss) {
-      xent_reduce<<<1, 1024, 0, s>>>(losses, n, nullptr, a.targets, a.ignore_index, mean, a.loss);
+      xent_reduce<<<1, 1024, 0, s>>>(losses, n, a.targets, a.ignore_index, mean, a.loss);
       TRY(cudaGetLastError());
     }
     return cudaSuccess;
   }
-  xent_compact<<<1, 1024, 0, s>>>(a.targets, n, a.ignore_index, V, idx, tgt, lt, count);
-  TRY(cudaGetLastError());
   T* dx = static_cast<T*>(a.dx);
-  xent_gather<T><<<n, 128, 0, s>>>(static_cast<const T*>(a.x), a.ldx, d, idx, count, xs, q.ldx, xplane, a.targets,
-                                   a.ignore_index, dx, d);
+  const int per = std::max(8, cdiv(cdiv(n, 512), 8) * 8), n_w = q.pack_w ? cdiv(V, 64) : 0;
+  xent_prep<T><<<n_w + cdiv(n, per), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, d, a.targets, n, a.ignore_index, V, per,
+                                                  idx, tgt, lt, count, xs, q.ldx, xplane, dx, static_cast<const T*>(a.w),
+                                                  a.ldw, wp, q.ldw, wplane, n_w);
   TRY(cudaGetLastError());
   float* losses = reinterpret_cast<float*>(ws + q.losses);
   void* pbuf = ws + q.p;
@@ -634,7 +715,8 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
     xent_rows<sizeof(T) == 4><<<rows, 256, sm, s>>>(stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
-                                                    lt + base, a.grad_rows, mean, losses + base, pbuf, q.ldp, gpl, gplane);
+                                                    lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane,
+                                                    c + 1 == q.n_pieces ? a.loss : nullptr);
     TRY(cudaGetLastError());
     const void* g = q.f32 ? (const void*)gpl : pbuf;
     if (dx) {
@@ -668,10 +750,6 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
                     eo, s));
     }
   }
-  if (a.loss) {
-    xent_reduce<<<1, 1024, 0, s>>>(losses, n, count, nullptr, 0, mean, a.loss);
-    TRY(cudaGetLastError());
-  }
   return cudaSuccess;
 }
 
@@ -682,7 +760,8 @@ size_t workspace_bytes(const llattn_xent_args& a) { return make_plan(a).total; }
 int launches(const llattn_xent_args& a) {
   const Plan q = make_plan(a);
   if (!q.train) return q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
-  return q.pack_w + 2 + q.n_pieces * (2 + (a.dx ? 2 : 0) + (a.dw ? 2 : 0)) + (a.loss ? 1 : 0);
+  return 1 + q.n_pieces * (2 + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
+                           (a.dw ? 1 + joins(dw_args(q, a, q.piece, nullptr)) : 0));
 }
 
 cudaError_t launch(const llattn_xent_args& a, volatile unsigned* fault, cudaStream_t s) {
@@ -690,12 +769,12 @@ cudaError_t launch(const llattn_xent_args& a, volatile unsigned* fault, cudaStre
   return q.f32 ? run<float>(a, q, fault, s) : run<bf16>(a, q, fault, s);
 }
 
-cudaError_t launch_scale(void* buf, int64_t n, int dtype, const float* f, cudaStream_t s) {
-  const int64_t blocks = std::min<int64_t>((n + 255) / 256, 8 * sm_count());
+cudaError_t launch_scale(void* a, int64_t na, void* b, int64_t nb, int dtype, const float* f, cudaStream_t s) {
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((std::max(na, nb) + 2047) / 2048, 8 * sm_count()));
   if (dtype == LLATTN_BF16)
-    scale_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>(static_cast<bf16*>(buf), n, f);
+    scale_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>(static_cast<bf16*>(a), na, static_cast<bf16*>(b), nb, f);
   else
-    scale_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(static_cast<float*>(buf), n, f);
+    scale_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(static_cast<float*>(a), na, static_cast<float*>(b), nb, f);
   return cudaGetLastError();
 }
 

@@ -8,7 +8,7 @@ namespace xent {
 size_t workspace_bytes(const llattn_xent_args& a);
 int launches(const llattn_xent_args& a);
 cudaError_t launch(const llattn_xent_args& a, volatile unsigned* fault, cudaStream_t s);
-cudaError_t launch_scale(void* buf, int64_t n, int dtype, const float* f, cudaStream_t s);
+cudaError_t launch_scale(void* a, int64_t na, void* b, int64_t nb, int dtype, const float* f, cudaStream_t s);
 unsigned read_fault_word(bool reset);
 }  // namespace xent
 namespace orth {

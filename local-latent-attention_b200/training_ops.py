@@ -21,9 +21,14 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .ops import _dtype_code, _ptr, _require, _stream
+from .ops import _dtype_code, _ptr, _require
 
 _REDUCTIONS = {"none": _lib.XENT_NONE, "mean": _lib.XENT_MEAN, "sum": _lib.XENT_SUM}
+
+
+def _stream(t: Tensor) -> int:
+    """torch's current stream on t's device (without building a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _on(device: torch.device):
@@ -127,11 +132,12 @@ def _linear_xent_none_grads_fake(x, w, targets, ignore_index, grad_rows, need_dx
     return x.new_empty(x.shape if need_dx else (0,)), w.new_empty(w.shape if need_dw else (0,))
 
 
-def _scale_(t: Tensor, factor: Tensor) -> Tensor:
-    """t *= factor (device scalar), in one launch that leaves t alone for a factor of 1."""
-    with _on(t.device):
-        _lib.check(_lib.lib().llattn_scale(_ptr(t), t.numel(), _dtype_code(t), _ptr(factor), _stream(t)), "llattn_scale")
-    return t
+def _scale_(a: Tensor, b: Tensor, factor: Tensor) -> None:
+    """a *= factor, b *= factor (device scalar), in one launch that leaves them alone for a factor of 1."""
+    if a.numel() + b.numel():
+        with _on(a.device):
+            _lib.check(_lib.lib().llattn_scale(_ptr(a), a.numel(), _ptr(b), b.numel(), _dtype_code(a), _ptr(factor),
+                                               _stream(a)), "llattn_scale")
 
 
 class _XentReduced(torch.autograd.Function):
@@ -149,19 +155,25 @@ class _XentReduced(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        need = ctx.needs_input_grad
-        x, w, targets, dx, dw = ctx.saved_tensors
-        if torch.compiler.is_compiling():
-            return ((dx * grad).to(x.dtype) if need[0] else None, (dw * grad).to(w.dtype) if need[1] else None, None, None,
-                    None)
-        if ctx.spent:  # a retained graph's next backward: the first one scaled the stored gradients in place
-            _, dx, dw = _linear_xent(x, w, targets, *ctx.cfg, need[0], need[1])
-        ctx.spent = True
-        g = grad.float()
-        return (_scale_(dx, g) if need[0] and dx.numel() else dx if need[0] else None,
-                _scale_(dw, g) if need[1] and dw.numel() else dw if need[1] else None, None, None, None)
+        # under create_graph the wrapper refuses to be differentiated; otherwise it only costs time
+        return _reduced_backward_once(ctx, grad) if torch.is_grad_enabled() else _reduced_backward(ctx, grad)
+
+
+def _reduced_backward(ctx, grad):
+    need = ctx.needs_input_grad
+    x, w, targets, dx, dw = ctx.saved_tensors
+    if torch.compiler.is_compiling():
+        return ((dx * grad).to(x.dtype) if need[0] else None, (dw * grad).to(w.dtype) if need[1] else None, None, None,
+                None)
+    if ctx.spent:  # a retained graph's next backward: the first one scaled the stored gradients in place
+        _, dx, dw = _linear_xent(x, w, targets, *ctx.cfg, need[0], need[1])
+    ctx.spent = True
+    _scale_(dx, dw, grad)
+    return dx if need[0] else None, dw if need[1] else None, None, None, None
+
+
+_reduced_backward_once = torch.autograd.function.once_differentiable(_reduced_backward)
 
 
 class _XentNone(torch.autograd.Function):
