@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs
 }
 
 // ---- small matrices ---------------------------------------------------------
-// Short side q <= 128: the whole iteration in one launch. A cluster of CL CTAs
+// Short side q <= 64: the whole iteration in one launch. A cluster of CL CTAs
 // holds one matrix, each CTA a slice of its long side in shared memory; per
 // step each CTA forms its slice's part of S, the parts are summed over the
 // cluster's shared memory (fixed order, every CTA a share of the elements
@@ -305,12 +305,12 @@ __global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs
 // sums hi hi + hi lo + lo hi in fp32: the result is exact to about 1e-6
 // before its rounding. Rows are padded by 16 bytes, an odd number of 16-byte
 // slots, so ldmatrix meets all banks.
-constexpr int kSmallQ = 128, kSmallT = 256, kSmallW = kSmallT / 32;
+constexpr int kSmallQ = 64, kSmallT = 512, kSmallW = kSmallT / 32;
 constexpr float kSm = 256.f;
 
 struct SmallShape {
   int q, L, w, wp, qp, fp;  // padded short side, slice, row strides of X, of S / B (halves) and of the parts (floats)
-  int mt, ng, units, groups;
+  int mt, units, groups;
   __host__ __device__ SmallShape(int q_, int L_, int CL) {
     q = cdiv(q_, 16) * 16;
     L = L_;
@@ -319,9 +319,8 @@ struct SmallShape {
     qp = q + 8;
     fp = q + 4;
     mt = q / 16;
-    ng = cdiv(q / 8, 4);  // groups of up to 4 column tiles of 8
-    units = mt * ng;
-    groups = units >= kSmallW ? 1 : kSmallW / units;  // ranges of K side by side
+    units = mt * mt;           // 16 x 16 blocks of S: at most a warp's each
+    groups = kSmallW / units;  // ranges of K side by side
   }
   // X hi, lo; S (then B) hi, lo; parts of S
   __host__ __device__ int bytes() const { return 2 * (2 * q * wp + 2 * q * qp) + 4 * groups * q * fp; }
@@ -355,38 +354,31 @@ __device__ __forceinline__ void split2x2(float a, float b, __half2& h, __half2& 
   l = __floats2half2_rn(a - f.x, b - f.y);
 }
 
-// One unit of a symmetric product Y Y^T, Y = hi + lo [.., ld] halves: rows
-// [16 m, 16 m + 16) x columns [32 n, 32 n + 32) (as far as q), K steps of 16
-// from k0 by dk
-__device__ __forceinline__ void small_product(const __half* hi, const __half* lo, int ld, int q, int m, int n, int k0,
-                                              int k1, int dk, float (&acc)[4][4]) {
+// A 16 x 16 block of a symmetric product Y Y^T, Y = hi + lo [.., ld] halves:
+// rows 16 m.., columns 16 n.., K steps of 16 from k0 by dk
+__device__ __forceinline__ void small_product(const __half* hi, const __half* lo, int ld, int m, int n, int k0, int k1,
+                                              int dk, float (&acc)[2][4]) {
   const int lane = threadIdx.x % 32;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-  // A: lane -> row lane % 16, K half lane / 16; B (two column tiles a load):
-  // lane -> row lane % 8 of tile lane / 16, K half (lane / 8) % 2
+  // A: lane -> row lane % 16, K half lane / 16; B (both column tiles of 8 in a
+  // load): lane -> row lane % 8 of tile lane / 16, K half (lane / 8) % 2
   const int ao = (16 * m + lane % 16) * ld + lane / 16 * 8;
-  const int bo = (32 * n + lane / 16 * 8 + lane % 8) * ld + lane / 8 % 2 * 8;
-  const int nt = min(4, (q - 32 * n) / 8);  // 2 or 4
-#pragma unroll 2
+  const int bo = (16 * n + lane / 16 * 8 + lane % 8) * ld + lane / 8 % 2 * 8;
+#pragma unroll 4
   for (int k = k0; k < k1; k += dk) {
-    uint32_t ah[4], al[4];
+    uint32_t ah[4], al[4], bh[4], bl[4];
     ldm4(ah, hi + ao + k);
     ldm4(al, lo + ao + k);
+    ldm4(bh, hi + bo + k);
+    ldm4(bl, lo + bo + k);
 #pragma unroll
-    for (int t = 0; t < 4; t += 2) {
-      if (t >= nt) break;
-      uint32_t bh[4], bl[4];
-      ldm4(bh, hi + bo + t * 8 * ld + k);
-      ldm4(bl, lo + bo + t * 8 * ld + k);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        mma16816(acc[t + j], al, bh[2 * j], bh[2 * j + 1]);
-        mma16816(acc[t + j], ah, bl[2 * j], bl[2 * j + 1]);
-        mma16816(acc[t + j], ah, bh[2 * j], bh[2 * j + 1]);
-      }
+    for (int j = 0; j < 2; ++j) {
+      mma16816(acc[j], al, bh[2 * j], bh[2 * j + 1]);
+      mma16816(acc[j], ah, bl[2 * j], bl[2 * j + 1]);
+      mma16816(acc[j], ah, bh[2 * j], bh[2 * j + 1]);
     }
   }
 }
@@ -482,14 +474,13 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
   const int fr = lane / 4, fc = lane % 4 * 2;  // an accumulator's first row and column
   for (int step = 0; step < steps; ++step) {
     // this slice's part of S, the K ranges' one after another in P
-    for (int u = warp; u < h.units * h.groups; u += kSmallW) {
-      const int gr = u / h.units, v = u - gr * h.units, m = v / h.ng, n = v - m * h.ng;
-      float acc[4][4];
-      small_product(xh, xl, h.wp, h.q, m, n, 16 * gr, h.w, 16 * h.groups, acc);
-      float* dst = P + gr * h.q * h.fp + (16 * m + fr) * h.fp + 32 * n + fc;
+    const int gr = warp / h.units, u = warp - gr * h.units, um = u / h.mt, un = u - um * h.mt;
+    float acc[2][4];
+    if (gr < h.groups) {
+      small_product(xh, xl, h.wp, um, un, 16 * gr, h.w, 16 * h.groups, acc);
+      float* dst = P + gr * h.q * h.fp + (16 * um + fr) * h.fp + 16 * un + fc;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (32 * n + 8 * t >= h.q) break;
+      for (int t = 0; t < 2; ++t) {
         *reinterpret_cast<float2*>(dst + 8 * t) = make_float2(acc[t][0], acc[t][1]);
         *reinterpret_cast<float2*>(dst + 8 * h.fp + 8 * t) = make_float2(acc[t][2], acc[t][3]);
       }
@@ -499,96 +490,87 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
       for (int e = tid; e < h.q * h.q; e += kSmallT) {
         const int at = e / h.q * h.fp + e % h.q;
         float v = P[at];
-        for (int gr = 1; gr < h.groups; ++gr) v += P[gr * h.q * h.fp + at];
+        for (int r = 1; r < h.groups; ++r) v += P[r * h.q * h.fp + at];
         P[at] = v;
       }
     }
     cluster.sync();
-    // every CTA sums its share of the quads over the cluster and gives the
-    // result to all: the next step's parts are written after the second
-    // barrier, the next S after that step's first one
-    for (int e = tid * CL + rank; e < h.q * h.q / 4; e += kSmallT * CL) {
-      const int i = e / (h.q / 4), j = (e - i * (h.q / 4)) * 4;
-      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-      for (int r0 = 0; r0 < CL; r0 += 8) {
-        float4 v[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r0 + r < CL) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(P, r0 + r) + i * h.fp + j);
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r0 + r < CL) t = make_float4(t.x + v[r].x, t.y + v[r].y, t.z + v[r].z, t.w + v[r].w);
+    // every CTA sums its share of the quads over the cluster, up to 8 threads
+    // a quad, and gives the result to all: the next step's parts are written
+    // after the second barrier, the next S after that step's first one
+    const int tq = min(CL, 8), per = h.q * h.q / 4 / CL;
+    for (int e0 = 32 * warp; e0 < per * tq; e0 += kSmallT) {
+      const int e = e0 + lane, sub = e % tq, quad = min(rank * per + e / tq, h.q * h.q / 4 - 1);
+      const int i = quad / (h.q / 4), j = (quad - i * (h.q / 4)) * 4;
+      float4 t = *reinterpret_cast<const float4*>(cluster.map_shared_rank(P, sub) + i * h.fp + j);
+      if (CL > 8) {
+        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(P, sub + 8) + i * h.fp + j);
+        t = make_float4(t.x + v.x, t.y + v.y, t.z + v.z, t.w + v.w);
       }
+      for (int o = 1; o < tq; o *= 2) {  // a + b = b + a: every thread gets the same bits
+        t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+        t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+        t.z += __shfl_xor_sync(0xffffffffu, t.z, o);
+        t.w += __shfl_xor_sync(0xffffffffu, t.w, o);
+      }
+      if (e >= per * tq) continue;
       // products of 2^8 X: S 2^16 -> S 2^8
       __half2 hi[2], lo[2];
       split2x2(t.x / kSm, t.y / kSm, hi[0], lo[0]);
       split2x2(t.z / kSm, t.w / kSm, hi[1], lo[1]);
       const int at = i * h.qp + j;
-      for (int r = 0; r < CL; ++r) {
+      for (int r = sub; r < CL; r += 8) {
         *reinterpret_cast<uint2*>(cluster.map_shared_rank(sh, r) + at) = *reinterpret_cast<const uint2*>(hi);
         *reinterpret_cast<uint2*>(cluster.map_shared_rank(sl, r) + at) = *reinterpret_cast<const uint2*>(lo);
       }
     }
     cluster.sync();
-    // B = b S + c S^2 over S, once every warp has read what it needs (up to 4
-    // units a warp, held in registers)
-    {
-      float acc[4][4][4];
+    // B = b S + c S^2 over S, once every warp has read what it needs
+    if (warp < h.units) small_product(sh, sl, h.qp, um, un, 0, h.q, 16, acc);
+    __syncthreads();
+    if (warp < h.units) {
+      const int at = (16 * um + fr) * h.qp + 16 * un + fc;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int u = warp + kSmallW * i;
-        if (u < h.units) small_product(sh, sl, h.qp, h.q, u / h.ng, u % h.ng, 0, h.q, 16, acc[i]);
-      }
-      __syncthreads();
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int u = warp + kSmallW * i;
-        if (u >= h.units) break;
-        const int m = u / h.ng, n = u - m * h.ng, at = (16 * m + fr) * h.qp + 32 * n + fc;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (32 * n + 8 * t >= h.q) break;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            __half2* ph = reinterpret_cast<__half2*>(sh + at + 8 * t + 8 * k * h.qp);
-            __half2* pl = reinterpret_cast<__half2*>(sl + at + 8 * t + 8 * k * h.qp);
-            const float2 x = __half22float2(*ph), y = __half22float2(*pl);
-            split2x2(fmaf(cb, x.x + y.x, cc / kSm * acc[i][t][2 * k]), fmaf(cb, x.y + y.y, cc / kSm * acc[i][t][2 * k + 1]),
-                     *ph, *pl);
-          }
+        for (int k = 0; k < 2; ++k) {
+          __half2* ph = reinterpret_cast<__half2*>(sh + at + 8 * t + 8 * k * h.qp);
+          __half2* pl = reinterpret_cast<__half2*>(sl + at + 8 * t + 8 * k * h.qp);
+          const float2 x = __half22float2(*ph), y = __half22float2(*pl);
+          split2x2(fmaf(cb, x.x + y.x, cc / kSm * acc[t][2 * k]), fmaf(cb, x.y + y.y, cc / kSm * acc[t][2 * k + 1]), *ph,
+                   *pl);
         }
-      }
     }
     __syncthreads();
-    // X = a X + B X: a warp owns column tiles of 8 and reads no others, so it
-    // overwrites them in place; 64 rows at a time would read rows already
-    // new, so all row tiles' sums are held (up to 8)
+    // X = a X + B X: a warp owns column tiles of 8 (it reads no others, so it
+    // overwrites them in place) and holds all their row tiles' sums
     for (int c0 = 8 * warp; c0 < h.w; c0 += 8 * kSmallW) {
-      float acc[8][4];
+      float d[4][4];
 #pragma unroll
-      for (int m = 0; m < 8; ++m)
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
-      for (int k = 0; k < h.q; k += 16) {
+        for (int i = 0; i < 4; ++i) d[m][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kSmallQ; k += 16) {
+        if (k >= h.q) break;
         uint32_t bh[2], bl[2];
         ldm2t(bh, xh + (k + lane % 16) * h.wp + c0);
         ldm2t(bl, xl + (k + lane % 16) * h.wp + c0);
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
+        for (int m = 0; m < 4; ++m) {
           if (m >= h.mt) break;
           uint32_t ah[4], al[4];
           const int ao = (16 * m + lane % 16) * h.qp + lane / 16 * 8 + k;
           ldm4(ah, sh + ao);
           ldm4(al, sl + ao);
-          mma16816(acc[m], al, bh[0], bh[1]);
-          mma16816(acc[m], ah, bl[0], bl[1]);
-          mma16816(acc[m], ah, bh[0], bh[1]);
+          mma16816(d[m], al, bh[0], bh[1]);
+          mma16816(d[m], ah, bl[0], bl[1]);
+          mma16816(d[m], ah, bh[0], bh[1]);
         }
       }
       __syncwarp();
 #pragma unroll
-      for (int m = 0; m < 8; ++m) {
+      for (int m = 0; m < 4; ++m) {
         if (m >= h.mt) break;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -596,7 +578,7 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
           __half2* ph = reinterpret_cast<__half2*>(xh + at);
           __half2* pl = reinterpret_cast<__half2*>(xl + at);
           const float2 x = __half22float2(*ph), y = __half22float2(*pl);
-          split2x2(fmaf(ca, x.x + y.x, acc[m][2 * k] / kSm), fmaf(ca, x.y + y.y, acc[m][2 * k + 1] / kSm), *ph, *pl);
+          split2x2(fmaf(ca, x.x + y.x, d[m][2 * k] / kSm), fmaf(ca, x.y + y.y, d[m][2 * k + 1] / kSm), *ph, *pl);
         }
       }
       __syncwarp();
@@ -623,14 +605,13 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
   cluster.sync();  // the others have read this CTA's parts
 }
 
-// CTAs per matrix of the one-launch form, 0 where it does not apply: the
-// smallest number whose slices are at most 64 wide or, past 8 (16 needs the
-// opt-in), that fit shared memory.
+// CTAs per matrix of the one-launch form (more than 8 need an opt-in), 0 where
+// it does not apply. Slices of at most 128 columns: one column tile per warp.
 int small_cluster(const llattn_orth_args& a) {
   const int q = std::min(a.rows, a.cols), L = std::max(a.rows, a.cols);
   if (q > kSmallQ) return 0;
   int cl = 1;
-  while (cl < 16 && L > 96 * cl) cl *= 2;
+  while (cl < 16 && L > 128 * cl) cl *= 2;
   return SmallShape(q, L, cl).bytes() <= 220 * 1024 ? cl : 0;
 }
 
