@@ -50,6 +50,31 @@ unsigned read_fault(bool reset) {
   return v;
 }
 
+// Programmatic dependent launch: a kernel may start (set up its barriers, TMEM
+// and tensor maps) while the one before it in the stream finishes; pdl_wait
+// returns when everything before is complete and visible, so it comes before
+// the first access to global memory; pdl_next lets the kernel after start.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launches a kernel that calls pdl_wait, in clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // One product. M, N, K are the host's sizes; m_dev / k_dev (optional) hold a
 // device-side row count from which M / K are cut: max(0, min(M, *m_dev -
 // dev_base)) (the rows past it are not computed, the K past it not read
@@ -457,12 +482,18 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
     }
     *abort = 0;
     fence_barrier_init();
-    const MmGrid<CG> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
-    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
   }
   if (warp == 1) {
     __syncwarp();
     mm_tmem_alloc<CG>(tmem_slot, 2 * S::BN);
+  }
+  pdl_next();
+  pdl_wait();
+  if (threadIdx.x == 0) {
+    const MmGrid<CG> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
+    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
   }
   tc_fence_before();
   __syncthreads();
@@ -477,8 +508,6 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      prefetch_tmap(&tm_a);
-      prefetch_tmap(&tm_b);
       int it = 0;
       bool ok = true;
       for (int t = unit; ok && t < pl.items; t += n_units) {
@@ -607,6 +636,8 @@ template <int CG, typename Epi>
 __global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi, int units) {
   using S = MmShape<CG>;
   __shared__ MmPlan plan;
+  pdl_next();
+  pdl_wait();
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const MmGrid<CG> grid(p, M);
   if (threadIdx.x == 0)
@@ -685,8 +716,7 @@ cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t
   // the device may have fewer tiles than the host's sizes say, never more
   const int tail = p.min_splits > 1 ? total : std::min(total, units - 1);
   if (tail < 1) return cudaSuccess;
-  mm_join<CG, Epi><<<dim3(tail, S::BM / 8), 256, 0, s>>>(p, epi, units);
-  return cudaGetLastError();
+  return launch_pdl(mm_join<CG, Epi>, dim3(tail, S::BM / 8), 256, 0, 1, s, p, epi, units);
 }
 template <int CG, typename Epi>
 cudaError_t launch_join(const MmArgs&, const Epi&, int, cudaStream_t, ...) {
@@ -703,17 +733,7 @@ cudaError_t launch_mm_cg(const MmArgs& p, const CUtensorMap& ta, const CUtensorM
   const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
   const int units = p.split ? mm_units(CG) : (int)std::min<int64_t>(tiles, mm_units(CG));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * CG));
-  cfg.blockDim = dim3(S::THREADS);
-  cfg.dynamicSmemBytes = S::SMEM;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {CG, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, mm_kernel<CG, Epi>, ta, tb, p, epi);
+  e = launch_pdl(mm_kernel<CG, Epi>, dim3((unsigned)(units * CG)), S::THREADS, S::SMEM, CG, s, ta, tb, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<CG, Epi>(p, epi, units, s, nullptr);
 }

@@ -189,6 +189,8 @@ struct EpiUpdate {
 template <typename T>
 __global__ void __launch_bounds__(256) orth_square(const __grid_constant__ Ptrs g, int64_t n, float* __restrict__ part) {
   __shared__ float red[8];
+  pdl_next();
+  pdl_wait();
   const T* src = static_cast<const T*>(g.p[blockIdx.y]);
   float s = 0.f;
   constexpr int VN = 16 / sizeof(T);
@@ -234,6 +236,8 @@ __global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs
                                                     __half* __restrict__ hi, bf16* __restrict__ lo, int64_t ld, int64_t zs,
                                                     float* __restrict__ s0) {
   __shared__ float sh[2];
+  pdl_next();
+  pdl_wait();
   const int z = blockIdx.y;
   if (threadIdx.x == 0) {
     float sum = 0.f;
@@ -452,6 +456,8 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
   const int j0 = rank * h.w, jn = max(0, min(h.w, L - j0));
   const T* src = static_cast<const T*>(g.p[z]);
 
+  pdl_next();
+  pdl_wait();
   float s = 0.f;
   small_read(src, tall, q, L, j0, jn, [&](int, int, float v) { s = fmaf(v, v, s); });
   s = warp_sum(s);
@@ -628,18 +634,8 @@ cudaError_t run_small(const llattn_orth_args& a, int cl, cudaStream_t st) {
     const int cnt = std::min(kPtrs, a.count - i0);
     Ptrs g;
     for (int i = 0; i < cnt; ++i) g.p[i] = a.g[i0 + i];
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cnt * cl));
-    cfg.blockDim = dim3(kSmallT);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)cl, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, orth_small<T>, g, (int)a.rows, (int)a.cols, (int)a.steps, a.a, a.b, a.c, a.eps,
-                           static_cast<bf16*>(a.out) + (int64_t)i0 * a.rows * a.cols);
+    e = launch_pdl(orth_small<T>, dim3((unsigned)(cnt * cl)), kSmallT, smem, cl, st, g, (int)a.rows, (int)a.cols, (int)a.steps,
+                   a.a, a.b, a.c, a.eps, static_cast<bf16*>(a.out) + (int64_t)i0 * a.rows * a.cols);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -704,14 +700,12 @@ cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fau
     Ptrs g;
     for (int i = 0; i < cnt; ++i) g.p[i] = a.g[i0 + i];
     const int n_parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts, (int64_t)m * n / 4096));
-    orth_square<T><<<dim3(n_parts, cnt), 256, 0, st>>>(g, (int64_t)m * n, part);
-    TRY(cudaGetLastError());
+    TRY(launch_pdl(orth_square<T>, dim3(n_parts, cnt), 256, 0, 1, st, g, (int64_t)m * n, part));
     // steps before the compensated ones read X as hi + lo
     const int comp0 = a.steps - kCompensated;
     bf16* lo0 = sizeof(T) == 4 && comp0 > 0 ? lo : nullptr;
-    orth_convert<T><<<dim3((unsigned)std::min<int64_t>(((int64_t)m * n + 2047) / 2048, cdiv(8 * sm_count(), cnt)), cnt), 256, 0, st>>>(g, m, n, part, n_parts, a.eps, x[0], lo0,
-                                                                            p.ldx, p.xz, s0);
-    TRY(cudaGetLastError());
+    TRY(launch_pdl(orth_convert<T>, dim3((unsigned)std::min<int64_t>(((int64_t)m * n + 2047) / 2048, cdiv(8 * sm_count(), cnt)), cnt), 256, 0, 1, st, g, m, n, part, n_parts, a.eps, x[0], lo0,
+                                                                            p.ldx, p.xz, s0));
     for (int i = 0; i < a.steps; ++i) {
       const float* sc = i ? nullptr : s0;
       const float k = i >= comp0 ? -(a.b + a.c) : 0.f;

@@ -276,6 +276,8 @@ __device__ __forceinline__ bool vec_rows(const T* p, int64_t ld, int d) {
 template <typename T>
 __global__ void __launch_bounds__(256) xent_pack(const T* __restrict__ x, int64_t ldx, int n, int d, bf16* __restrict__ xs,
                                                  int64_t lds, int64_t plane) {
+  pdl_next();
+  pdl_wait();
   const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d));
 }
@@ -296,6 +298,8 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
                                                  float* __restrict__ lt, int* __restrict__ count, bf16* __restrict__ xs,
                                                  int64_t lds, int64_t plane, T* __restrict__ dx, const T* __restrict__ w,
                                                  int64_t ldw, bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w) {
+  pdl_next();
+  pdl_wait();
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if ((int)blockIdx.x < n_w) {
     const bool v = vec_rows(w, ldw, d);
@@ -384,6 +388,8 @@ __device__ __forceinline__ float row_loss(float2 lse, float lt) { return (lse.x 
 __global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ stats, int n_tiles, int n,
                                                    const float* __restrict__ lt, const int64_t* __restrict__ targets,
                                                    int64_t ignore, int vocab, float* __restrict__ losses) {
+  pdl_next();
+  pdl_wait();
   const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= n) return;
   const int lane = threadIdx.x % 32;
@@ -438,6 +444,8 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   extern __shared__ float xent_f[];  // [n_tiles]
   __shared__ float red[8];
   __shared__ int last;
+  pdl_next();
+  pdl_wait();
   const int n_all = *count;
   const int n = cut_rows(rows, count, base);
   const int64_t row = blockIdx.x;
@@ -516,6 +524,8 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
 __global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ losses, int n,
                                                     const int64_t* __restrict__ targets, int64_t ignore, int mean,
                                                     float* __restrict__ loss) {
+  pdl_next();
+  pdl_wait();
   __shared__ float red[32];
   float s = 0.f, c = 0.f;
   for (int i = threadIdx.x; i < n; i += 1024) {
@@ -545,6 +555,8 @@ __device__ __forceinline__ void scale_run(T* p, int64_t n, float f) {
 template <typename T>
 __global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ a, int64_t na, T* __restrict__ b, int64_t nb,
                                                     const float* __restrict__ s) {
+  pdl_next();
+  pdl_wait();
   const float f = *s;
   if (f == 1.f) return;
   scale_run(a, na, f);
@@ -667,12 +679,10 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   const void* wv = q.pack_w ? wp : a.w;
   if (!q.train) {
     if (q.pack_w) {
-      xent_pack<T><<<cdiv(V, 8), 256, 0, s>>>(static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane);
-      TRY(cudaGetLastError());
+      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(V, 8)), 256, 0, 1, s, static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane));
     }
     if (q.pack_x) {
-      xent_pack<T><<<cdiv(n, 8), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane);
-      TRY(cudaGetLastError());
+      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane));
     }
     MmArgs p = base_args(q, fault);
     p.M = n;
@@ -682,20 +692,17 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     TRY(launch_mm(p, Operand{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0},
                   Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     float* losses = a.losses ? a.losses : reinterpret_cast<float*>(ws + q.losses);
-    xent_losses<<<cdiv(n, 4), 128, 0, s>>>(stats, q.n_tiles, n, lt, a.targets, a.ignore_index, V, losses);
-    TRY(cudaGetLastError());
+    TRY(launch_pdl(xent_losses, dim3(cdiv(n, 4)), 128, 0, 1, s, stats, q.n_tiles, n, lt, a.targets, a.ignore_index, V, losses));
     if (a.loss) {
-      xent_reduce<<<1, 1024, 0, s>>>(losses, n, a.targets, a.ignore_index, mean, a.loss);
-      TRY(cudaGetLastError());
+      TRY(launch_pdl(xent_reduce, dim3(1), 1024, 0, 1, s, losses, n, a.targets, a.ignore_index, mean, a.loss));
     }
     return cudaSuccess;
   }
   T* dx = static_cast<T*>(a.dx);
   const int per = std::max(8, cdiv(cdiv(n, 512), 8) * 8), n_w = q.pack_w ? cdiv(V, 64) : 0;
-  xent_prep<T><<<n_w + cdiv(n, per), 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, d, a.targets, n, a.ignore_index, V, per,
+  TRY(launch_pdl(xent_prep<T>, dim3(n_w + cdiv(n, per)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, d, a.targets, n, a.ignore_index, V, per,
                                                   idx, tgt, lt, count, xs, q.ldx, xplane, dx, static_cast<const T*>(a.w),
-                                                  a.ldw, wp, q.ldw, wplane, n_w);
-  TRY(cudaGetLastError());
+                                                  a.ldw, wp, q.ldw, wplane, n_w));
   float* losses = reinterpret_cast<float*>(ws + q.losses);
   void* pbuf = ws + q.p;
   bf16* gpl = reinterpret_cast<bf16*>(ws + q.gplanes);
@@ -714,10 +721,9 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0};
     TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
-    xent_rows<sizeof(T) == 4><<<rows, 256, sm, s>>>(stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
+    TRY(launch_pdl(xent_rows<sizeof(T) == 4>, dim3(rows), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
                                                     lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane,
-                                                    c + 1 == q.n_pieces ? a.loss : nullptr);
-    TRY(cudaGetLastError());
+                                                    c + 1 == q.n_pieces ? a.loss : nullptr));
     const void* g = q.f32 ? (const void*)gpl : pbuf;
     if (dx) {
       MmArgs m = dx_args(q, a, rows, fault);
@@ -771,11 +777,10 @@ cudaError_t launch(const llattn_xent_args& a, volatile unsigned* fault, cudaStre
 
 cudaError_t launch_scale(void* a, int64_t na, void* b, int64_t nb, int dtype, const float* f, cudaStream_t s) {
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((std::max(na, nb) + 2047) / 2048, 8 * sm_count()));
+  const dim3 grid((unsigned)blocks);
   if (dtype == LLATTN_BF16)
-    scale_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>(static_cast<bf16*>(a), na, static_cast<bf16*>(b), nb, f);
-  else
-    scale_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(static_cast<float*>(a), na, static_cast<float*>(b), nb, f);
-  return cudaGetLastError();
+    return launch_pdl(scale_kernel<bf16>, grid, 256, 0, 1, s, static_cast<bf16*>(a), na, static_cast<bf16*>(b), nb, f);
+  return launch_pdl(scale_kernel<float>, grid, 256, 0, 1, s, static_cast<float*>(a), na, static_cast<float*>(b), nb, f);
 }
 
 unsigned read_fault_word(bool reset) { return read_fault(reset); }
