@@ -8,15 +8,15 @@
 // boxes of 64 x 128 (K-major) or 64 x 64 (MN-major, two panels per 128
 // rows); out-of-range rows, columns and K are zero-filled by the copies.
 //
-// Two tile shapes: CG = 2 runs a 256 x 256 tile on a pair of CTAs (a cluster of
-// two SMs): each CTA copies its own 128 rows of A and 128 of the tile's 256
+// The large tile is 256 x 256 on a pair of CTAs (a cluster of two SMs, CG = 2):
+// each CTA copies its own 128 rows of A and 128 of the tile's 256
 // rows of B, the leader (cluster rank 0) issues cta_group::2 MMAs for both,
 // and each CTA ends up with its 128 rows x 256 columns of the accumulator.
 // Per K = 64 step a CTA copies 32 KB for 128 x 256 x 64 products, half the L2
-// traffic per flop of the CG = 1 tile (128 x 128 on one CTA), which small
-// products use because it spreads over more SMs. Both keep a 6-stage ring of
-// 32 KB stages that runs on across tiles and two accumulators in TMEM, so one
-// tile's epilogue overlaps the next tile's MMAs.
+// traffic per flop of a 128 x 128 tile on one CTA, which smaller products use
+// because it spreads over more SMs. All keep a ring of 6 to 8 stages that
+// runs on across tiles and two accumulators in TMEM, so one tile's epilogue
+// overlaps the next tile's MMAs.
 //
 // Warps: 0 copies, 1 issues MMAs, the others (one per 32 rows x 128 columns of
 // the CTA's accumulator) run the epilogue: thread = row, 128 columns.
@@ -181,15 +181,24 @@ __device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(ncols) : "memory");
 }
 
-template <int CG>
+// Tile shapes: 2 = 256 x 256 on a pair, 1 = 128 x 128 on a CTA, 0 = 128 x 32 on
+// a CTA, for products too small to occupy the SMs otherwise: its epilogue is
+// one block of 32 columns per warp instead of four (4.2 -> 1.1 us at the end
+// of a kernel), and a K step copies 20 KB instead of 32 (a single SM takes in
+// about 64 bytes a cycle, which bounds the 128 x 128 tile at 0.28 us a step).
+template <int SH>
 struct MmShape {
-  static constexpr int BM = 128 * CG, BN = 128 * CG;  // tile of the CTA (pair)
-  static constexpr int EW = 4 * CG;                   // epilogue warps: 32 rows x 128 columns each
+  static constexpr int CG = SH == 2 ? 2 : 1;
+  static constexpr int BM = 128 * CG, BN = SH == 2 ? 256 : SH == 1 ? 128 : 32;  // tile of the CTA (pair)
+  static constexpr int CW = BN < 128 ? BN : 128;  // columns of an epilogue warp (32 rows)
+  static constexpr int EW = 4 * (BN / CW);        // epilogue warps
   static constexpr int THREADS = 64 + 32 * EW;
-  static constexpr int ST = 6;
-  static constexpr int OPB = 128 * 64 * 2;  // one CTA's operand tile: 128 rows x 64 K, 16 KB
+  static constexpr int ST = SH == 0 ? 8 : 6;
+  static constexpr int BR = BN / CG;        // rows of B that a CTA copies
+  static constexpr int AB = 128 * 64 * 2;   // one CTA's A tile: 128 rows x 64 K, 16 KB
+  static constexpr int BB = (BR < 64 ? 64 : BR) * 64 * 2;  // B tile (a whole panel of 64 if MN-major)
   static constexpr int STG = 4096;          // an epilogue warp's staging block: 32 rows of 128 bytes
-  static constexpr int A = 0, B = A + ST * OPB, STAGE = B + ST * OPB, BAR = STAGE + EW * STG;
+  static constexpr int A = 0, B = A + ST * AB, STAGE = B + ST * BB, BAR = STAGE + EW * STG;
   static constexpr int BYTES = BAR + 256;
   static constexpr int SMEM = BYTES + 1024;  // + alignment
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -228,12 +237,12 @@ __host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int 
   return MmPlan{total, full, best, full + tail * best};
 }
 
-template <int CG>
+template <int SH>
 struct MmGrid {
   int n_mt, n_nt, per_z;
   __host__ __device__ __forceinline__ MmGrid(const MmArgs& p, int M) {
-    n_mt = cdiv(M, MmShape<CG>::BM);
-    n_nt = cdiv(p.N, MmShape<CG>::BN);
+    n_mt = cdiv(M, MmShape<SH>::BM);
+    n_nt = cdiv(p.N, MmShape<SH>::BN);
     per_z = p.sym ? n_mt * (n_mt + 1) / 2 : n_mt * n_nt;
   }
   __device__ __forceinline__ MmTile at(const MmArgs& p, int t) const {
@@ -253,8 +262,8 @@ struct MmGrid {
       j = v / h;
       i = bi * 8 + (v - j * h);
     }
-    r.m0 = i * MmShape<CG>::BM;
-    r.n0 = j * MmShape<CG>::BN;
+    r.m0 = i * MmShape<SH>::BM;
+    r.n0 = j * MmShape<SH>::BN;
     return r;
   }
 };
@@ -430,13 +439,13 @@ __device__ __forceinline__ float2 bf16_pair(const uint4 (&u)[4], int i) {
 }
 
 // one range's sums of a tile: its fp32 block of part, [BM][BN]
-template <int CG>
+template <int SH>
 __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, const MmTile& w, int row, int col, int M,
                                            uint32_t taddr, uint8_t* buf) {
-  using S = MmShape<CG>;
+  using S = MmShape<SH>;
   float* dst = p.part + ((int64_t)x.block * S::BM + row) * S::BN + col;
 #pragma unroll 1
-  for (int cc = 0; cc < 128; cc += 32) {
+  for (int cc = 0; cc < S::CW; cc += 32) {
     const int n = p.N - (w.n0 + col + cc);
     if (n <= 0) break;  // warp-uniform
     float v[32];
@@ -448,18 +457,19 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 }
 
 // Epi: struct with
-//   __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
-//                        uint8_t* buf) const
-// called by every thread of an epilogue warp (all 32 lanes, converged) for its
-// row and 128 columns [col0, col0 + 128); taddr: TMEM address of the warp's
+//   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
+//                                          bool zero, uint8_t* buf) const
+//   static constexpr bool kNarrow: the 128 x 32 shape may be used (CW = 32, else 128)
+// tile is called by every thread of an epilogue warp (all 32 lanes,
+// converged) for its row and CW columns [col0, col0 + CW); taddr: TMEM address of the warp's
 // lanes and columns; zero: the K range is empty, the accumulator holds
 // nothing; buf: the warp's staging block.
-template <int CG, typename Epi>
-__global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
+template <int SH, typename Epi>
+__global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
               const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
-  using S = MmShape<CG>;
-  constexpr int ST = S::ST;
+  using S = MmShape<SH>;
+  constexpr int ST = S::ST, CG = S::CG;
   extern __shared__ uint8_t mm_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR);
@@ -492,7 +502,7 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
   pdl_next();
   pdl_wait();
   if (threadIdx.x == 0) {
-    const MmGrid<CG> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
+    const MmGrid<SH> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
     *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
   }
   tc_fence_before();
@@ -503,7 +513,7 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
 
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const int K = cut_rows(p.K, p.k_dev, p.dev_base);
-  const MmGrid<CG> grid(p, M);
+  const MmGrid<SH> grid(p, M);
   const MmPlan pl = *plan;
 
   if (warp == 0) {
@@ -513,15 +523,15 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
       for (int t = unit; ok && t < pl.items; t += n_units) {
         const MmItem x = mm_item(pl, t, K);
         const MmTile w = grid.at(p, x.tile);
-        const int ma = w.m0 + rank * 128, nb = w.n0 + rank * 128;
+        const int ma = w.m0 + rank * 128, nb = w.n0 + rank * S::BR;
         for (int term = 0; ok && term < p.n_terms; ++term) {
           const int za = w.z + (int)((p.pa >> (4 * term)) & 15u), zb = w.z + (int)((p.pb >> (4 * term)) & 15u);
           for (int k = x.k0; k < x.k1; k += 64, ++it) {
             const int s = it % ST;
             if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
-            if (rank == 0) mbar_expect_tx(&full[s], 2 * CG * S::OPB);
-            uint8_t* sa = smem + S::A + s * S::OPB;
-            uint8_t* sb = smem + S::B + s * S::OPB;
+            if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
+            uint8_t* sa = smem + S::A + s * S::AB;
+            uint8_t* sb = smem + S::B + s * S::BB;
             auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
               if (CG == 1)
                 tma_load_3d(map, &full[s], dst, c0, c1, c2);
@@ -530,13 +540,13 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
             };
             if (p.a_mn) {
               load(&tm_a, sa, ma, k, za);
-              load(&tm_a, sa + S::OPB / 2, ma + 64, k, za);
+              load(&tm_a, sa + S::AB / 2, ma + 64, k, za);
             } else {
               load(&tm_a, sa, k, ma, za);
             }
             if (p.b_mn) {
               load(&tm_b, sb, nb, k, zb);
-              load(&tm_b, sb + S::OPB / 2, nb + 64, k, zb);
+              if (S::BR > 64) load(&tm_b, sb + S::BB / 2, nb + 64, k, zb);
             } else {
               load(&tm_b, sb, k, nb, zb);
             }
@@ -563,7 +573,7 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
       // K-major: a K step of 16 is 32 bytes of the 128-byte rows; MN-major: 16
       // rows of 128 bytes, panels of 64 rows (MN) 8 KB apart
       const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-      const uint32_t a_lbo = p.a_mn ? S::OPB / 2 : 16, b_lbo = p.b_mn ? S::OPB / 2 : 16;
+      const uint32_t a_lbo = p.a_mn ? S::AB / 2 : 16, b_lbo = p.b_mn ? S::BB / 2 : 16;
       int it = 0, k = 0;
       bool ok = true;
       for (int t = unit; ok && t < pl.items; t += n_units, ++k) {
@@ -576,8 +586,8 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
           const int s = it % ST;
           if (!(ok = mbar_wait(&full[s], (it / ST) & 1, abort, &g_mm_fault))) break;
           tc_fence_after();
-          const uint64_t da = desc_sw128(smem_u32(smem + S::A + s * S::OPB), a_lbo, 1024);
-          const uint64_t db = desc_sw128(smem_u32(smem + S::B + s * S::OPB), b_lbo, 1024);
+          const uint64_t da = desc_sw128(smem_u32(smem + S::A + s * S::AB), a_lbo, 1024);
+          const uint64_t db = desc_sw128(smem_u32(smem + S::B + s * S::BB), b_lbo, 1024);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             mma_f16<CG>(tmem + S::BN * buf, desc_add(da, kk * a_step), desc_add(db, kk * b_step), id,
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
       if (!ok) mm_raise(p, 2u, abort);
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns 128 half..
+    const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns CW half..
     int k = 0;
     bool ok = true;
     for (int t = unit; t < pl.items; t += n_units, ++k) {
@@ -600,13 +610,13 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (k >> 1) & 1, abort, &g_mm_fault));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t ta = tmem + S::BN * buf + 128 * half + ((uint32_t)(32 * quad) << 16);
+      const uint32_t ta = tmem + S::BN * buf + S::CW * half + ((uint32_t)(32 * quad) << 16);
       uint8_t* stage = smem + S::STAGE + (warp - 2) * S::STG;
-      const int row = rank * 128 + 32 * quad + lane, col = 128 * half;
+      const int row = rank * 128 + 32 * quad + lane, col = S::CW * half;
       if (x.block < 0)
-        epi.tile(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage);
+        epi.template tile<S::CW>(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage);
       else
-        store_part<CG>(p, x, w, row, col, M, ta, stage);
+        store_part<SH>(p, x, w, row, col, M, ta, stage);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {  // this accumulator may take the tile after next
@@ -632,14 +642,14 @@ __global__ void __launch_bounds__(MmShape<CG>::THREADS, 1)
 // Adds up the ranges of the split tiles in order, and hands 4 columns of a row
 // at a time to Epi::quad(row, col, n valid, values). grid (split tiles at
 // most, BM / 8), one warp per row.
-template <int CG, typename Epi>
+template <int SH, typename Epi>
 __global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi, int units) {
-  using S = MmShape<CG>;
+  using S = MmShape<SH>;
   __shared__ MmPlan plan;
   pdl_next();
   pdl_wait();
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
-  const MmGrid<CG> grid(p, M);
+  const MmGrid<SH> grid(p, M);
   if (threadIdx.x == 0)
     plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
   __syncthreads();
@@ -673,84 +683,85 @@ struct Operand {
   int mn;  // stored MN-major (rows = K, cols = MN) instead of K-major (rows = MN, cols = K)
 };
 
-inline int mm_units(int cg) { return sm_count() / cg; }
+inline int mm_units(int sh) { return sh == 2 ? sm_count() / 2 : sm_count(); }
 
-// Waves of a product on `units` CTAs (pairs), the last one split where allowed.
-inline double mm_waves(const MmPlan& pl, int units) {
-  return (double)(pl.full / units) + (pl.full % units ? 1.0 : 0.0) +
-         (pl.items > pl.full ? (double)cdiv(pl.items - pl.full, units) / pl.s + 0.01 * pl.s : 0.0);
-}
-
-// Which tile: the pair's 256 x 256 tile takes about twice a single 128 x 128
-// tile's time on twice the SMs (measured 1.6 against 1.3 PFLOP/s in long
-// products), so the shorter schedule in tile times wins.
-inline int pick_group(const MmArgs& p) {
-  const MmGrid<1> g1(p, p.M);
-  const MmGrid<2> g2(p, p.M);
-  const int u1 = mm_units(1), u2 = mm_units(2), ks = cdiv(p.K, 64);
-  const double t1 = mm_waves(mm_plan(g1.per_z * p.nz, u1, ks, p.split, p.min_splits), u1) * 1.25;
-  const double t2 = mm_waves(mm_plan(g2.per_z * p.nz, u2, ks, p.split, p.min_splits), u2) * 2.0;
-  return t2 <= t1 ? 2 : 1;
+// Estimated time (us) of a product in a shape: waves of tiles (the last one
+// split where allowed), each K / 64 steps and a gap, and the last tile's
+// epilogue. The constants are measured on a B200: a step of the pair's tile
+// takes 0.385 us (tensor cores), one of the others 0.28 and 0.18 (copies).
+template <int SH>
+double mm_time(const MmArgs& p) {
+  constexpr double step = SH == 2 ? 0.385 : SH == 1 ? 0.28 : 0.18, tail = SH == 2 ? 5.5 : SH == 1 ? 4.3 : 1.2;
+  const MmGrid<SH> g(p, p.M);
+  const int units = mm_units(SH), ks = cdiv(p.K, 64);
+  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.min_splits);
+  double waves = pl.full / units + (pl.full % units ? 1.0 : 0.0);
+  if (pl.items > pl.full) waves += (double)cdiv(pl.items - pl.full, units) / pl.s + 0.01 * pl.s;
+  return waves * (ks * p.n_terms * step + 0.5) + tail;
 }
 
 // fp32 elements of MmArgs::part for a product of at most these sizes
 inline int64_t mm_part_floats(const MmArgs& p) {
   if (!p.split) return 0;
-  const MmGrid<1> g1(p, p.M);
-  const MmGrid<2> g2(p, p.M);
-  // below the caps of mm_plan: 4 waves of ranges, or min_splits of every tile
-  const int64_t n1 = std::max<int64_t>(4 * mm_units(1), (int64_t)g1.per_z * p.nz * p.min_splits);
-  const int64_t n2 = std::max<int64_t>(4 * mm_units(2), (int64_t)g2.per_z * p.nz * p.min_splits);
-  return p.min_splits > 1 ? std::max(n1 * 128 * 128, n2 * 256 * 256)
-                          : std::max((int64_t)4 * mm_units(1) * 128 * 128, (int64_t)4 * mm_units(2) * 256 * 256);
+  // the caps of mm_plan: 4 waves of ranges, or min_splits of every tile
+  auto floats = [&](int sh, int64_t tiles, int64_t block) {
+    return std::max<int64_t>(4 * mm_units(sh), p.min_splits > 1 ? tiles * p.nz * p.min_splits : 0) * block;
+  };
+  return std::max({floats(2, MmGrid<2>(p, p.M).per_z, 256 * 256), floats(1, MmGrid<1>(p, p.M).per_z, 128 * 128),
+                   floats(0, MmGrid<0>(p, p.M).per_z, 128 * 32)});
 }
 
 // whether mm_plan may split anything, whatever the device-side counts
 inline bool joins(const MmArgs& p) { return p.split && (p.min_splits > 1 || cdiv(p.K, 64) >= 16); }
 
-template <int CG, typename Epi>
+template <int SH, typename Epi>
 cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t s, decltype(&Epi::quad)) {
-  using S = MmShape<CG>;
-  const MmGrid<CG> g(p, p.M);
+  using S = MmShape<SH>;
+  const MmGrid<SH> g(p, p.M);
   const int total = g.per_z * p.nz;
   // the device may have fewer tiles than the host's sizes say, never more
   const int tail = p.min_splits > 1 ? total : std::min(total, units - 1);
   if (tail < 1) return cudaSuccess;
-  return launch_pdl(mm_join<CG, Epi>, dim3(tail, S::BM / 8), 256, 0, 1, s, p, epi, units);
+  return launch_pdl(mm_join<SH, Epi>, dim3(tail, S::BM / 8), 256, 0, 1, s, p, epi, units);
 }
-template <int CG, typename Epi>
+template <int SH, typename Epi>
 cudaError_t launch_join(const MmArgs&, const Epi&, int, cudaStream_t, ...) {
   return cudaErrorInvalidValue;  // an epilogue without quad() cannot be split
 }
 
-template <int CG, typename Epi>
-cudaError_t launch_mm_cg(const MmArgs& p, const CUtensorMap& ta, const CUtensorMap& tb, const Epi& epi,
-                         cudaStream_t s) {
-  using S = MmShape<CG>;
-  cudaError_t e = set_smem_once(mm_kernel<CG, Epi>, S::SMEM);
+template <int SH, typename Epi>
+cudaError_t launch_mm_sh(const MmArgs& p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
+  using S = MmShape<SH>;
+  CUtensorMap ta, tb;
+  if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
+      !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : S::BR))
+    return cudaErrorInvalidValue;
+  cudaError_t e = set_smem_once(mm_kernel<SH, Epi>, S::SMEM);
   if (e != cudaSuccess) return e;
   const int64_t m = cdiv(p.M, S::BM), n = cdiv(p.N, S::BN);
   const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
-  const int units = p.split ? mm_units(CG) : (int)std::min<int64_t>(tiles, mm_units(CG));
-  e = launch_pdl(mm_kernel<CG, Epi>, dim3((unsigned)(units * CG)), S::THREADS, S::SMEM, CG, s, ta, tb, p, epi);
+  const int units = p.split ? mm_units(SH) : (int)std::min<int64_t>(tiles, mm_units(SH));
+  e = launch_pdl(mm_kernel<SH, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
-  return launch_join<CG, Epi>(p, epi, units, s, nullptr);
+  return launch_join<SH, Epi>(p, epi, units, s, nullptr);
 }
 
 template <typename Epi>
 cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
-  CUtensorMap ta, tb;
   p.a_mn = a.mn;
   p.b_mn = b.mn;
   if (p.min_splits < 1) p.min_splits = 1;
   if (p.nz < 1) p.nz = 1;
   if (p.n_terms < 1) p.n_terms = 1;
   if (p.M < 1 || p.N < 1 || p.K < 1 || (p.split && !p.part)) return cudaErrorInvalidValue;
-  if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
-      !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : 128))
-    return cudaErrorInvalidValue;
-  return pick_group(p) == 2 ? launch_mm_cg<2>(p, ta, tb, epi, s) : launch_mm_cg<1>(p, ta, tb, epi, s);
+  const double t2 = mm_time<2>(p), t1 = mm_time<1>(p);
+  if constexpr (Epi::kNarrow) {
+    MmArgs q = p;
+    q.sym = 0;  // not square: every tile is computed
+    if (mm_time<0>(q) < std::min(t1, t2)) return launch_mm_sh<0>(q, a, b, epi, s);
+  }
+  return t2 <= t1 ? launch_mm_sh<2>(p, a, b, epi, s) : launch_mm_sh<1>(p, a, b, epi, s);
 }
 
 }  // namespace

@@ -51,53 +51,57 @@ struct Ptrs {
   const void* p[kPtrs];
 };
 
-// Stores 32 columns of a symmetric matrix's tile, and off the diagonal their
-// mirror image: column nc + lane of the block becomes that row, from row0 on.
-__device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, MmTile w, int row, int nc, int M, int N,
+// Stores 32 columns of a symmetric matrix's tile, and off the diagonal (of the
+// shapes that skip the tiles above it) their mirror image: column nc + lane of the block becomes that row, from row0 on.
+__device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, bool mirror, int row, int nc, int M, int N,
                                                 const float (&v)[32], uint8_t* buf) {
   const int lane = threadIdx.x % 32, row0 = row - lane;
   uint4 u[4];
   half_row(v, u);
   block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), (N - nc) * 2, row < M);
-  if (w.m0 != w.n0)
+  if (mirror)
     block_mirror(buf, lane, reinterpret_cast<uint8_t*>(base + (nc + lane) * ld + row0), (M - row0) * 2, nc + lane < N);
 }
 
 // S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
 struct EpiGram {
+  static constexpr bool kNarrow = true;
   __half* s;
   int64_t ld, zs;
   const float* s0;  // first step: X = s0[z] * stored, else null (2^-6)
+  template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float f = x * x * kS;
     __half* base = s + w.z * zs;
 #pragma unroll 1
-    for (int cc = 0; cc < 128; cc += 32) {
+    for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc;
       if (nc >= a.N) break;
       float v[32];
       load32(taddr + cc, zero, v);
 #pragma unroll
       for (int q = 0; q < 32; ++q) v[q] *= f;
-      store_symmetric(base, ld, w, row, nc, M, a.N, v, buf);
+      store_symmetric(base, ld, a.sym && w.m0 != w.n0, row, nc, M, a.N, v, buf);
     }
   }
 };
 
 // B = b S + c S^2 + k I (scaled by kS)
 struct EpiPoly {
+  static constexpr bool kNarrow = true;
   const __half* s;
   __half* b;
   int64_t ld, zs;
   float cb, cc2, k;  // b, c / kS, k * kS
+  template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32;
     __half* base = b + w.z * zs;
 #pragma unroll 1
-    for (int cc = 0; cc < 128; cc += 32) {
+    for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
       if (n <= 0) break;
       float v[32];
@@ -111,13 +115,14 @@ struct EpiPoly {
         v[2 * q] = fmaf(cb, x.x, cc2 * v[2 * q]) + (row == nc + 2 * q ? k : 0.f);
         v[2 * q + 1] = fmaf(cb, x.y, cc2 * v[2 * q + 1]) + (row == nc + 2 * q + 1 ? k : 0.f);
       }
-      store_symmetric(base, ld, w, row, nc, M, a.N, v, buf);
+      store_symmetric(base, ld, a.sym && w.m0 != w.n0, row, nc, M, a.N, v, buf);
     }
   }
 };
 
 // X <- (a - k) X + (B + k I) X
 struct EpiUpdate {
+  static constexpr bool kNarrow = true;
   const __half* hi;
   bf16* lo;          // remainder of X, read where rd_lo, written (in place) where wr_lo
   __half* next;      // next X (hi), or null in the last step
@@ -126,6 +131,7 @@ struct EpiUpdate {
   const float* s0;
   float ca;          // a - k
   int rd_lo, wr_lo, vec_out;
+  template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32;
@@ -133,7 +139,7 @@ struct EpiUpdate {
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float fl = ca * x, fp = x / kS;
 #pragma unroll 1
-    for (int cc = 0; cc < 128; cc += 32) {
+    for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
       if (n <= 0) break;
       const int64_t at = w.z * zs + row * ld + nc;

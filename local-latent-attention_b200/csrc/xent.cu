@@ -47,6 +47,7 @@ constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u;
 // ---- first product: statistics and exponentials ----------------------------
 
 struct EpiStats {
+  static constexpr bool kNarrow = false;
   float2* stats;       // [rows][n_tiles]: (max, sum of exp(l - max))
   int n_tiles;
   const int* tgt;      // [rows] target of row (dev_base already added); < 0: none
@@ -56,6 +57,7 @@ struct EpiStats {
   int64_t ldp;
   int p_f32;           // fp32 instead of fp16 * 2^15
 
+  template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const int nv = min(kTile, a.N - col0);  // columns of this tile
@@ -124,6 +126,7 @@ struct EpiStats {
 // ---- second and third product: rows out --------------------------------------
 
 struct EpiOut {
+  static constexpr bool kNarrow = true;
   void* out;
   int64_t ldo;
   int out_bf16;
@@ -157,12 +160,13 @@ struct EpiOut {
     }
   }
 
+  template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32;
     const bool row_ok = row < M;
     const int64_t orow = (row_ok ? (idx ? idx[row] : row) : 0) * ldo;
-    if (out_bf16 && vec && !acc) {  // 64 columns, whole 128-byte lines, at a time
+    if (CW == 128 && out_bf16 && vec && !acc) {  // 64 columns, whole 128-byte lines, at a time
 #pragma unroll 1
       for (int cc = 0; cc < 128; cc += 64) {
         const int nc = col0 + cc, n = a.N - nc;
@@ -174,7 +178,7 @@ struct EpiOut {
       return;
     }
 #pragma unroll 1
-    for (int cc = 0; cc < 128; cc += 32) {
+    for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
       if (n <= 0) break;  // warp-uniform
       float v[32];
