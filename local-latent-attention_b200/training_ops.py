@@ -31,11 +31,12 @@ def _stream(t: Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+_HERE = nullcontext()
+
+
 def _on(device: torch.device):
     """Makes `device` current where it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 # --------------------------------------------------------------------------
@@ -46,37 +47,46 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
+_TYPES = (torch.bfloat16, torch.float32)
+
+
 def _check_xent(x: Tensor, w: Tensor, targets: Tensor) -> None:
+    # one test on the way of every call; the messages are put together only when it fails
+    if (x.is_cuda and x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and x.dtype == w.dtype
+            and x.dtype in _TYPES and targets.dtype == torch.int64 and targets.shape == x.shape[:1]
+            and w.device == x.device and targets.device == x.device and w.shape[0] and w.shape[1]):
+        return
     _require(x.is_cuda, "linear_cross_entropy needs CUDA tensors")
     _require(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1],
              f"x {tuple(x.shape)} and weight {tuple(w.shape)} must be [tokens, d] and [vocab, d]")
     _require(x.dtype == w.dtype, f"x is {x.dtype} and weight {w.dtype}: one dtype (or autocast) is needed")
-    _require(targets.dtype == torch.int64 and tuple(targets.shape) == (x.shape[0],),
+    _require(targets.dtype == torch.int64 and targets.shape == x.shape[:1],
              f"targets must be int64 [tokens], got {targets.dtype} {tuple(targets.shape)}")
     _require(w.device == x.device and targets.device == x.device, "x, weight and targets must be on one device")
-    _require(w.shape[0] >= 1 and w.shape[1] >= 1, "weight must have rows and columns")
+    _dtype_code(x)
+    _require(False, "weight must have rows and columns")
 
 
 def _xent(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int, *, grad_rows: Optional[Tensor] = None,
           losses: Optional[Tensor] = None, loss: Optional[Tensor] = None, dx: Optional[Tensor] = None,
           dw: Optional[Tensor] = None) -> None:
     x, w, targets = _rows(x), _rows(w), targets.contiguous()
-    p = lambda t: _ptr(t) if t is not None else None
-    args = _lib.XentArgs(x.shape[0], x.shape[1], w.shape[0], _dtype_code(x), reduction, ignore_index, _ptr(x),
-                         max(x.stride(0), x.shape[1]), _ptr(w), max(w.stride(0), w.shape[1]), _ptr(targets),
-                         p(grad_rows), p(losses), p(loss), p(dx), p(dw), None, 0)
-    L = _lib.lib()
-    with _on(x.device):
-        ws = torch.empty(L.llattn_xent_workspace_bytes(ctypes.byref(args)) or 256, dtype=torch.uint8, device=x.device)
-        args.workspace, args.workspace_bytes = _ptr(ws), ws.numel()
-        _lib.check(L.llattn_xent(ctypes.byref(args), _stream(x)), "llattn_xent")
+    p = lambda t: t.data_ptr() if t is not None else None
+    (n, d), v, dev = x.shape, w.shape[0], x.device
+    args = _lib.XentArgs(n, d, v, _dtype_code(x), reduction, ignore_index, x.data_ptr(), max(x.stride(0), d), w.data_ptr(),
+                         max(w.stride(0), d), targets.data_ptr(), p(grad_rows), p(losses), p(loss), p(dx), p(dw), None, 0)
+    L, ref = _lib.lib(), ctypes.byref(args)
+    with _on(dev):
+        size = L.llattn_xent_workspace_bytes(ref) or 256
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), size
+        _lib.check(L.llattn_xent(ref, _stream(x)), "llattn_xent")
 
 
 def _linear_xent(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int, need_dx: bool,
                  need_dw: bool) -> tuple[Tensor, Tensor, Tensor]:
     """Reductions mean and sum: the loss, and dx / dw of it where needed (else empty)."""
     _check_xent(x, w, targets)
-    _dtype_code(x)
     make = torch.empty if x.shape[0] else torch.zeros
     loss = make((), dtype=torch.float32, device=x.device)
     dx = make(x.shape if need_dx else (0,), dtype=x.dtype, device=x.device)
@@ -89,7 +99,6 @@ def _linear_xent(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduc
 def _linear_xent_none(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int) -> Tensor:
     """Reduction none: per-token losses."""
     _check_xent(x, w, targets)
-    _dtype_code(x)
     losses = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
     if x.shape[0]:
         _xent(x, w, targets, ignore_index, _lib.XENT_NONE, losses=losses)
@@ -211,23 +220,25 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
     "mean" and "sum" compute the gradients together with the loss, from at most
     half a GiB of exponentials at a time, and keep them until the backward;
     "none" recomputes in the backward. Gradients of gradients are not supported."""
-    _require(reduction in _REDUCTIONS, f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
-    _require(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
-             f"x {tuple(x.shape)} must end in weight's columns {tuple(weight.shape)}")
-    _require(tuple(targets.shape) == tuple(x.shape[:-1]),
-             f"targets {tuple(targets.shape)} must have x's leading shape {tuple(x.shape[:-1])}")
+    code = _REDUCTIONS.get(reduction)
+    if code is None:
+        _require(False, f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        _require(False, f"x {tuple(x.shape)} must end in weight's columns {tuple(weight.shape)}")
+    if targets.shape != x.shape[:-1]:
+        _require(False, f"targets {tuple(targets.shape)} must have x's leading shape {tuple(x.shape[:-1])}")
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dt), weight.to(dt)
-    x2, t = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
+    flat = x.dim() == 2
+    x2, t = (x, targets) if flat else (x.reshape(-1, x.shape[-1]), targets.reshape(-1))
     grads = torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad)
     if reduction == "none":
         if grads:
             out = _XentNone.apply(x2, weight, t, ignore_index)
         else:
             out = (linear_xent_none_op if torch.compiler.is_compiling() else _linear_xent_none)(x2, weight, t, ignore_index)
-        return out.view(targets.shape)
-    code = _REDUCTIONS[reduction]
+        return out if flat else out.view(targets.shape)
     if grads:
         return _XentReduced.apply(x2, weight, t, ignore_index, code)
     f = linear_xent_op if torch.compiler.is_compiling() else _linear_xent
