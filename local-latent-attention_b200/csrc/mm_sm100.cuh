@@ -192,24 +192,34 @@ __device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(ncols) : "memory");
 }
 
-// Tile shapes: 2 = 256 x 256 on a pair, 1 = 128 x 128 on a CTA, 0 = 128 x 32 on
-// a CTA, for products too small to occupy the SMs otherwise: its epilogue is
-// one block of 32 columns per warp instead of four (4.2 -> 1.1 us at the end
-// of a kernel), and a K step copies 20 KB instead of 32 (a single SM takes in
-// about 64 bytes a cycle, which bounds the 128 x 128 tile at 0.28 us a step).
+// Tile shapes:
+//  3 = 256 x 512 on a pair, for long sums: one accumulator fills the TMEM, as two
+//      halves of 256 columns that the epilogue frees one after the other. An
+//      SM takes in about 64 bytes a cycle, which the 32 KB a step of shape 2
+//      need as long as their products take; 48 KB for twice the products do
+//      not hold the tensor cores up.
+//  2 = 256 x 256 on a pair, two accumulators
+//  1 = 128 x 128 on a CTA, two accumulators
+//  0 = 128 x 32 on a CTA, for products too small to occupy the SMs otherwise:
+//      its epilogue is one block of 32 columns per warp instead of four (4.2 ->
+//      1.1 us at the end of a kernel), and a step copies 20 KB instead of 32.
 template <int SH>
 struct MmShape {
-  static constexpr int CG = SH == 2 ? 2 : 1;
-  static constexpr int BM = 128 * CG, BN = SH == 2 ? 256 : SH == 1 ? 128 : 32;  // tile of the CTA (pair)
-  static constexpr int CW = BN < 128 ? BN : 128;  // columns of an epilogue warp (32 rows)
-  static constexpr int EW = 4 * (BN / CW);        // epilogue warps
+  static constexpr int CG = SH >= 2 ? 2 : 1;
+  static constexpr int NH = SH == 3 ? 2 : 1;  // column halves of the accumulator, an MMA each
+  static constexpr int BM = 128 * CG, BN = SH == 3 ? 512 : SH == 2 ? 256 : SH == 1 ? 128 : 32;  // tile of the CTA (pair)
+  static constexpr int HN = BN / NH;              // columns of an MMA
+  static constexpr int CW = HN < 128 ? HN : 128;  // columns of an epilogue warp (32 rows) in a half
+  static constexpr int EW = 4 * (HN / CW);        // epilogue warps
   static constexpr int THREADS = 64 + 32 * EW;
-  static constexpr int ST = SH == 0 ? 8 : 6;
-  static constexpr int BR = BN / CG;        // rows of B that a CTA copies
+  static constexpr int ST = SH == 3 ? 4 : SH == 0 ? 8 : 6;
+  static constexpr int BR = HN / CG;        // rows of B that a CTA copies per half
   static constexpr int AB = 128 * 64 * 2;   // one CTA's A tile: 128 rows x 64 K, 16 KB
-  static constexpr int BB = (BR < 64 ? 64 : BR) * 64 * 2;  // B tile (a whole panel of 64 if MN-major)
+  static constexpr int BB = (BR < 64 ? 64 : BR) * 64 * 2;  // B tile of a half (a whole panel of 64 if MN-major)
   static constexpr int STG = 4096;          // an epilogue warp's staging block: 32 rows of 128 bytes
-  static constexpr int A = 0, B = A + ST * AB, STAGE = B + ST * BB, BAR = STAGE + EW * STG;
+  static constexpr int A = 0, B = A + ST * AB, STAGE = B + ST * NH * BB, BAR = STAGE + EW * STG;
+  static constexpr int ACC = NH == 2 ? 1 : 2;      // accumulators in TMEM
+  static constexpr int TCOLS = NH == 2 ? 512 : 2 * BN;
   static constexpr int BYTES = BAR + 256;
   static constexpr int SMEM = BYTES + 1024;  // + alignment
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -318,7 +328,7 @@ template <int CH>
 __device__ __forceinline__ int stage_at(int r, int c) {
   return CH == 8 ? r * 128 + ((c ^ (r & 7)) * 16) : r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
 }
-template <int CH>
+template <int CH, bool ADD = false>
 __device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, uint8_t* p, int bytes, bool ok) {
   const int c = lane % CH;
 #pragma unroll
@@ -326,19 +336,26 @@ __device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, ui
     const int r = 32 / CH * i + lane / CH;
     const uint4 u = *reinterpret_cast<const uint4*>(buf + stage_at<CH>(r, c));
     uint8_t* q = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
-    if (q && 16 * c < bytes) *reinterpret_cast<uint4*>(q + 16 * c) = u;
+    if (q && 16 * c < bytes) {
+      if (ADD)  // fp32: added in the L2, nothing waits for the old value
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(q + 16 * c), "f"(__uint_as_float(u.x)),
+                     "f"(__uint_as_float(u.y)), "f"(__uint_as_float(u.z)), "f"(__uint_as_float(u.w))
+                     : "memory");
+      else
+        *reinterpret_cast<uint4*>(q + 16 * c) = u;
+    }
   }
   __syncwarp();
 }
 // p: the lane's own row's first byte (16-byte aligned), bytes: valid bytes of
 // the rows (rounded up to 16 in memory), ok: the lane's row exists.
-template <int CH>
+template <int CH, bool ADD = false>
 __device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 (&v)[CH], uint8_t* p, int bytes,
                                             bool ok) {
 #pragma unroll
   for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
   __syncwarp();
-  block_write_out<CH>(buf, lane, p, bytes, ok);
+  block_write_out<CH, ADD>(buf, lane, p, bytes, ok);
 }
 // After a block_store of 32 x 32 16-bit values: the block's transpose, column c
 // of it (lane = c) as the row at p. 8 x 8 matrices go through registers
@@ -470,7 +487,7 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
 //                                          bool zero, uint8_t* buf) const
-//   static constexpr bool kNarrow: the 128 x 32 shape may be used (CW = 32, else 128)
+//   static constexpr bool kNarrow, kWide: the 128 x 32 (CW = 32, else 128) and 256 x 512 shapes may be used
 // tile is called by every thread of an epilogue warp (all 32 lanes,
 // converged) for its row and CW columns [col0, col0 + CW); taddr: TMEM address of the warp's
 // lanes and columns; zero: the K range is empty, the accumulator holds
@@ -508,7 +525,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   }
   if (warp == 1) {
     __syncwarp();
-    mm_tmem_alloc<CG>(tmem_slot, 2 * S::BN);
+    mm_tmem_alloc<CG>(tmem_slot, S::TCOLS);
   }
   pdl_next();
   pdl_wait();
@@ -520,7 +537,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   __syncthreads();
   if (CG == 2) cluster_sync();  // the peer's barriers are initialised
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // accumulator b at columns [b * BN, (b + 1) * BN)
+  const uint32_t tmem = *tmem_slot;  // accumulator (or half) b at columns [b * HN, (b + 1) * HN)
 
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const int K = cut_rows(p.K, p.k_dev, p.dev_base);
@@ -540,9 +557,9 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
           for (int k = x.k0; k < x.k1; k += 64, ++it) {
             const int s = it % ST;
             if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
-            if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
+            if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + S::NH * (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
             uint8_t* sa = smem + S::A + s * S::AB;
-            uint8_t* sb = smem + S::B + s * S::BB;
+            uint8_t* sb = smem + S::B + s * S::NH * S::BB;
             auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
               if (CG == 1)
                 tma_load_3d(map, &full[s], dst, c0, c1, c2);
@@ -555,11 +572,16 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
             } else {
               load(&tm_a, sa, k, ma, za);
             }
-            if (p.b_mn) {
-              load(&tm_b, sb, nb, k, zb);
-              if (S::BR > 64) load(&tm_b, sb + S::BB / 2, nb + 64, k, zb);
-            } else {
-              load(&tm_b, sb, k, nb, zb);
+#pragma unroll
+            for (int h = 0; h < S::NH; ++h) {
+              uint8_t* dst = sb + h * S::BB;
+              const int n = nb + h * S::HN;
+              if (p.b_mn) {
+                load(&tm_b, dst, n, k, zb);
+                if (S::BR > 64) load(&tm_b, dst + S::BB / 2, n + 64, k, zb);
+              } else {
+                load(&tm_b, dst, k, n, zb);
+              }
             }
           }
         }
@@ -585,7 +607,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       // per MMA).
       const uint32_t fmt = p.fp16 ? 0u : 1u;
       const uint32_t id = (1u << 4) | (fmt << 7) | (fmt << 10) | ((p.a_mn ? 1u : 0u) << 15) |
-                          ((p.b_mn ? 1u : 0u) << 16) | ((uint32_t)(S::BN >> 3) << 17) | ((uint32_t)(S::BM >> 4) << 24);
+                          ((p.b_mn ? 1u : 0u) << 16) | ((uint32_t)(S::HN >> 3) << 17) | ((uint32_t)(S::BM >> 4) << 24);
       // K-major: a K step of 16 is 32 bytes of the 128-byte rows; MN-major: 16
       // rows of 128 bytes, panels of 64 rows (MN) 8 KB apart
       const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
@@ -596,25 +618,60 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       bool ok = true;
       for (int t = unit; ok && t < pl.items; t += n_units, ++k) {
         const MmItem x = mm_item(pl, t, K);
-        const int buf = k & 1, steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
-        // the epilogue has read this accumulator's previous tile (k - 2)
-        if (k >= 2 && !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((k >> 1) - 1) & 1, abort, &g_mm_fault))))
-          break;
-        tc_fence_after();
-        const uint32_t d = td + S::BN * buf;
-        for (int i = 0; i < steps; ++i) {
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, &g_mm_fault)))) break;
-          const uint64_t da = da0 + stage * (S::AB >> 4), db = db0 + stage * (S::BB >> 4);
+        const int buf = S::ACC == 2 ? k & 1 : 0, steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
+        auto wait = [&](uint64_t* bar, int parity) {
+          return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_mm_fault));
+        };
+        // 4 MMAs of a stage's K = 64 into accumulator (half) h
+        auto issue = [&](int st, int h, int first) {
+          const uint32_t d = td + S::HN * (S::ACC == 2 ? buf : h);
+          const uint64_t da = da0 + st * (S::AB >> 4), db = db0 + (st * S::NH + h) * (S::BB >> 4);
+          mma_f16<CG>(d, da, db, id, first ? 0u : 1u);
+          mma_f16<CG>(d, da + a_step, db + b_step, id, 1u);
+          mma_f16<CG>(d, da + 2 * a_step, db + 2 * b_step, id, 1u);
+          mma_f16<CG>(d, da + 3 * a_step, db + 3 * b_step, id, 1u);
+        };
+        auto advance = [&] {
+          stage = stage + 1 == ST ? 0 : stage + 1;
+          phase ^= stage == 0;
+        };
+        int i = 0;
+        if (S::NH == 1) {
+          // the epilogue has read this accumulator's previous tile (k - 2)
+          if (k >= 2 && !(ok = wait(&acc_empty[buf], ((k >> 1) - 1) & 1))) break;
+          tc_fence_after();
+        } else {
+          // the first half may start while the epilogue reads the second:
+          // as many stages as the ring holds, whose second halves follow
+          if (k >= 1 && !(ok = wait(&acc_empty[0], (k - 1) & 1))) break;
+          tc_fence_after();
+          const int ahead = min(steps, ST), stage0 = stage;
+          for (; i < ahead; ++i) {
+            if (!(ok = wait(&full[stage], phase))) break;
+            if (elect_one()) issue(stage, 0, i == 0);
+            __syncwarp();
+            advance();
+          }
+          if (!ok || (k >= 1 && !(ok = wait(&acc_empty[1], (k - 1) & 1)))) break;
+          tc_fence_after();
+          for (int j = 0, st = stage0; j < ahead; ++j) {
+            if (elect_one()) {
+              issue(st, 1, j == 0);
+              commit<CG>(&empty[st]);
+            }
+            __syncwarp();
+            st = st + 1 == ST ? 0 : st + 1;
+          }
+        }
+        for (; i < steps; ++i) {
+          if (!(ok = wait(&full[stage], phase))) break;
           if (elect_one()) {
-            mma_f16<CG>(d, da, db, id, i > 0 ? 1u : 0u);
-            mma_f16<CG>(d, da + a_step, db + b_step, id, 1u);
-            mma_f16<CG>(d, da + 2 * a_step, db + 2 * b_step, id, 1u);
-            mma_f16<CG>(d, da + 3 * a_step, db + 3 * b_step, id, 1u);
+            issue(stage, 0, i == 0);
+            if (S::NH == 2) issue(stage, 1, 0);
             commit<CG>(&empty[stage]);
           }
           __syncwarp();
-          stage = stage + 1 == ST ? 0 : stage + 1;
-          phase ^= stage == 0;
+          advance();
         }
         if (!ok) break;
         if (elect_one()) commit<CG>(&acc_full[buf]);
@@ -627,26 +684,31 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     int k = 0;
     bool ok = true;
     for (int t = unit; t < pl.items; t += n_units, ++k) {
-      const int buf = k & 1;
+      const int buf = S::ACC == 2 ? k & 1 : 0;
       const MmItem x = mm_item(pl, t, K);
       const MmTile w = grid.at(p, x.tile);
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (k >> 1) & 1, abort, &g_mm_fault));
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (S::ACC == 2 ? k >> 1 : k) & 1, abort, &g_mm_fault));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t ta = tmem + S::BN * buf + S::CW * half + ((uint32_t)(32 * quad) << 16);
       uint8_t* stage = smem + S::STAGE + (warp - 2) * S::STG;
-      const int row = rank * 128 + 32 * quad + lane, col = S::CW * half;
-      if (x.block < 0)
-        epi.template tile<S::CW>(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage);
-      else
-        store_part<SH>(p, x, w, row, col, M, ta, stage);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {  // this accumulator may take the tile after next
-        if (CG == 1)
-          mbar_arrive(&acc_empty[buf]);
+      const int row = rank * 128 + 32 * quad + lane;
+#pragma unroll
+      for (int h = 0; h < S::NH; ++h) {
+        const int col = S::HN * h + S::CW * half;
+        const uint32_t ta = tmem + S::HN * (S::ACC == 2 ? buf : h) + S::CW * half + ((uint32_t)(32 * quad) << 16);
+        if (x.block < 0)
+          epi.template tile<S::CW>(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage);
         else
-          mbar_arrive_leader(&acc_empty[buf]);
+          store_part<SH>(p, x, w, row, col, M, ta, stage);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {  // this accumulator (half) may take its next tile
+          uint64_t* bar = &acc_empty[S::ACC == 2 ? buf : h];
+          if (CG == 1)
+            mbar_arrive(bar);
+          else
+            mbar_arrive_leader(bar);
+        }
       }
     }
     if (!ok) mm_raise(p, 8u, abort);
@@ -658,7 +720,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    mm_tmem_dealloc<CG>(tmem, 2 * S::BN);
+    mm_tmem_dealloc<CG>(tmem, S::TCOLS);
   }
 }
 
@@ -706,21 +768,22 @@ struct Operand {
   int mn;  // stored MN-major (rows = K, cols = MN) instead of K-major (rows = MN, cols = K)
 };
 
-inline int mm_units(int sh) { return sh == 2 ? sm_count() / 2 : sm_count(); }
+inline int mm_units(int sh) { return sh >= 2 ? sm_count() / 2 : sm_count(); }
 
 // Estimated time (us) of a product in a shape: waves of tiles (the last one
 // split where allowed), each K / 64 steps and a gap, and the last tile's
 // epilogue. The constants are measured on a B200: a step of the pair's tile
-// takes 0.385 us (tensor cores), one of the others 0.28 and 0.18 (copies).
+// takes 0.385 us, of its 512-wide one 0.72, of the others 0.28 and 0.18.
 template <int SH>
 double mm_time(const MmArgs& p) {
-  constexpr double step = SH == 2 ? 0.385 : SH == 1 ? 0.28 : 0.18, tail = SH == 2 ? 5.5 : SH == 1 ? 4.3 : 1.2;
+  constexpr double step = SH == 3 ? 0.72 : SH == 2 ? 0.385 : SH == 1 ? 0.28 : 0.18;
+  constexpr double gap = SH == 3 ? 3.0 : 0.5, tail = SH == 3 ? 8.0 : SH == 2 ? 5.5 : SH == 1 ? 4.3 : 1.2;
   const MmGrid<SH> g(p, p.M);
   const int units = mm_units(SH), ks = cdiv(p.K, 64);
   const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.min_splits);
   double waves = pl.full / units + (pl.full % units ? 1.0 : 0.0);
   if (pl.items > pl.full) waves += (double)cdiv(pl.items - pl.full, units) / pl.s + 0.01 * pl.s;
-  return waves * (ks * p.n_terms * step + 0.5) + tail;
+  return waves * (ks * p.n_terms * step + gap) + tail;
 }
 
 // fp32 elements of MmArgs::part for a product of at most these sizes
@@ -730,7 +793,7 @@ inline int64_t mm_part_floats(const MmArgs& p) {
   auto floats = [&](int sh, int64_t tiles, int64_t block) {
     return std::max<int64_t>(4 * mm_units(sh), p.min_splits > 1 ? tiles * p.nz * p.min_splits : 0) * block;
   };
-  return std::max({floats(2, MmGrid<2>(p, p.M).per_z, 256 * 256), floats(1, MmGrid<1>(p, p.M).per_z, 128 * 128),
+  return std::max({floats(3, MmGrid<3>(p, p.M).per_z, 256 * 512), floats(2, MmGrid<2>(p, p.M).per_z, 256 * 256), floats(1, MmGrid<1>(p, p.M).per_z, 128 * 128),
                    floats(0, MmGrid<0>(p, p.M).per_z, 128 * 32)});
 }
 
@@ -783,6 +846,9 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
     MmArgs q = p;
     q.sym = 0;  // not square: every tile is computed
     if (mm_time<0>(q) < std::min(t1, t2)) return launch_mm_sh<0>(q, a, b, epi, s);
+  }
+  if constexpr (Epi::kWide) {
+    if (mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s);
   }
   return t2 <= t1 ? launch_mm_sh<2>(p, a, b, epi, s) : launch_mm_sh<1>(p, a, b, epi, s);
 }

@@ -47,7 +47,7 @@ constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u;
 // ---- first product: statistics and exponentials ----------------------------
 
 struct EpiStats {
-  static constexpr bool kNarrow = false;
+  static constexpr bool kNarrow = false, kWide = false;  // wide: sums over d are short, its long epilogue shows (757 us for 620)
   float2* stats;       // [rows][n_tiles]: (max, sum of exp(l - max))
   int n_tiles;
   const int* tgt;      // [rows] target of row (dev_base already added); < 0: none
@@ -126,11 +126,12 @@ struct EpiStats {
 // ---- second and third product: rows out --------------------------------------
 
 struct EpiOut {
-  static constexpr bool kNarrow = true;
+  static constexpr bool kNarrow = true, kWide = true;
   void* out;
   int64_t ldo;
   int out_bf16;
   int vec;              // base and row stride 16-byte aligned (whole rows may be padded to 16 bytes)
+  int add;              // fp32, vec: added to what out holds (one writer per element and launch: in order)
   const float* acc;     // added first (fp32, row stride ldacc), or null
   int64_t ldacc;
   const int* idx;       // output row of row m, or null
@@ -153,6 +154,10 @@ struct EpiOut {
     } else {
       float* dst = static_cast<float*>(out) + at;
       if (vec) {
+        if (add) {
+          const float4 c = *reinterpret_cast<const float4*>(dst);
+          v = make_float4(v.x + c.x, v.y + c.y, v.z + c.z, v.w + c.w);
+        }
         *reinterpret_cast<float4*>(dst) = v;
       } else {
         for (int q = 0; q < n; ++q) dst[q] = x[q];
@@ -177,20 +182,22 @@ struct EpiOut {
       }
       return;
     }
+    // what was summed before is fetched one block ahead: its latency passes
+    // during the previous block's stores
+    const float* src = acc + (row_ok ? (int64_t)row * ldacc : 0) + col0;  // ldacc is a multiple of 8
+    uint4 x[8];
+    if (acc && col0 < a.N) block_fetch(lane, x, src, (a.N - col0) * 4, row_ok);
 #pragma unroll 1
     for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
       if (n <= 0) break;  // warp-uniform
       float v[32];
+      load32(taddr + cc, zero, v);
       if (acc) {
-        uint4 x[8];  // ldacc is a multiple of 8
-        block_fetch(lane, x, acc + (row_ok ? (int64_t)row * ldacc : 0) + nc, n * 4, row_ok);
-        load32(taddr + cc, zero, v);
         block_spread(buf, lane, x);
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(word(x, q));
-      } else {
-        load32(taddr + cc, zero, v);
+        if (cc + 32 < CW && n > 32) block_fetch(lane, x, src + cc + 32, (n - 32) * 4, row_ok);
       }
       if (out_bf16) {
         uint4 u[4];
@@ -204,7 +211,9 @@ struct EpiOut {
         uint4 u[8];
         float* dst = static_cast<float*>(out) + orow + nc;
         f32_row(v, u);
-        if (vec)
+        if (add)
+          block_store<8, true>(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 4, row_ok);
+        else if (vec)
           block_store(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 4, row_ok);
         else
           block_store_odd(buf, lane, u, dst, n, row_ok);
@@ -754,7 +763,8 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.ldo = last ? d : q.ldd;
       eo.out_bf16 = last && !q.f32;
       eo.vec = last ? aligned_rows(a.dw, d, 2, q.elt) : 1;
-      eo.acc = c ? acc : nullptr;
+      eo.add = c && !last;
+      eo.acc = c && last ? acc : nullptr;
       eo.ldacc = q.ldd;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
                     eo, s));
