@@ -118,9 +118,9 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Arrive on the barrier at the same shared-memory offset in the cluster's CTA 0.
-// Release at CTA scope: what the leader's MMAs touch after it is this CTA's TMEM
-// and shared memory, whose order the tcgen05 and proxy fences before it see
-// to; a cluster-scope release waits some 1500 cycles for unrelated writes.
+// Release at CTA scope: what the leader's MMAs touch after it is this CTA's
+// TMEM, whose order the tcgen05 fence before it sees to; a cluster-scope
+// release waits some 1500 cycles for unrelated writes.
 __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
   asm volatile(
       "{\n\t.reg .b32 ra;\n\t"
@@ -487,14 +487,6 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
   }
 }
 
-// What mm_kernel's CVT form rewrites A with.
-struct MmConvert {
-  const float* f;
-  int64_t ldf;
-  const int* tgt;
-  const float* g;
-};
-
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
 //                                          bool zero, uint8_t* buf) const
@@ -503,26 +495,17 @@ struct MmConvert {
 // converged) for its row and CW columns [col0, col0 + CW); taddr: TMEM address of the warp's
 // lanes and columns; zero: the K range is empty, the accumulator holds
 // nothing; buf: the warp's staging block.
-//
-// CVT (K-major A, one term): A holds fp16 exponentials that become the bf16 operand
-// in shared memory: a (row, column) f[column / 128][row], minus g[row] at
-// column tgt[row], zeros for the rows past M. Four more warps (thread = row)
-// rewrite each stage in place between its copy and its MMAs, and where the
-// tile is its row's first they also store it (tm_g), so the operand is in
-// memory for another product without a pass of its own.
-template <int SH, typename Epi, bool CVT>
-__global__ void __launch_bounds__(MmShape<SH>::THREADS + (CVT ? 128 : 0), 1)
+template <int SH, typename Epi>
+__global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-              const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ MmArgs p,
-              const __grid_constant__ Epi epi, const __grid_constant__ MmConvert cv) {
+              const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
   using S = MmShape<SH>;
   constexpr int ST = S::ST, CG = S::CG;
   extern __shared__ uint8_t mm_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR);
   uint64_t *full = bars, *empty = bars + ST, *acc_full = bars + 2 * ST, *acc_empty = acc_full + 2;
-  uint64_t* copied = acc_empty + 2;  // CVT: this CTA's A has landed (full: B has, and both CTAs' A is rewritten)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(copied + (CVT ? ST : 0));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   MmPlan* plan = reinterpret_cast<MmPlan*>(tmem_slot + 2);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // (uniform)
@@ -531,9 +514,8 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS + (CVT ? 128 : 0), 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], CVT ? 1 + 4 * CG : 1);
-      mbar_init(&empty[s], CVT ? 5 : 1);
-      if (CVT) mbar_init(&copied[s], 1);
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -578,8 +560,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS + (CVT ? 128 : 0), 1)
           for (int k = x.k0; k < x.k1; k += 64, ++it) {
             const int s = it % ST;
             if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
-            if (rank == 0)
-              mbar_expect_tx(&full[s], CG * ((CVT ? 0 : S::AB) + S::NH * (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
+            if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + S::NH * (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
             uint8_t* sa = smem + S::A + s * S::AB;
             uint8_t* sb = smem + S::B + s * S::NH * S::BB;
             auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
@@ -588,10 +569,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS + (CVT ? 128 : 0), 1)
               else
                 tma_load_3d_pair(map, &full[s], dst, c0, c1, c2);
             };
-            if (CVT) {
-              mbar_expect_tx(&copied[s], S::AB);
-              tma_load_3d(&tm_a, &copied[s], sa, k, ma, za);
-            } else if (p.a_mn) {
+            if (p.a_mn) {
               load(&tm_a, sa, ma, k, za);
               load(&tm_a, sa + S::AB / 2, ma + 64, k, za);
             } else {
@@ -616,13 +594,11 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS + (CVT ? 128 : 0), 1)
       for (int i = it - ST < 0 ? 0 : it - ST; ok && i < it; ++i)
         ok = mbar_wait(&empty[i % ST], (i / ST) & 1, abort, &g_mm_fault);
       if (!ok) mm_raise(p, 1u, abort);
-      if (*abort && (rank == 0 || CVT)) {  // let the copies already issued land before the CTA (pair) can exit
+      if (*abort && rank == 0) {  // let the copies already issued land before the CTA (pair) can exit
         volatile int none = 0;
         volatile unsigned gnone = 0;
-        for (int i = it - ST < 0 ? 0 : it - ST; i < it; ++i) {
-          if (CVT) mbar_wait(&copied[i % ST], (i / ST) & 1, &none, &gnone, 100000000ull);
-          if (rank == 0) mbar_wait(&full[i % ST], (i / ST) & 1, &none, &gnone, 100000000ull);
-        }
+        for (int i = it - ST < 0 ? 0 : it - ST; i < it; ++i)
+          mbar_wait(&full[i % ST], (i / ST) & 1, &none, &gnone, 100000000ull);
       }
     }
   } else if (warp == 1) {
@@ -706,77 +682,6 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS + (CVT ? 128 : 0), 1)
       }
       if (!ok && lane == 0) mm_raise(p, 2u, abort);
     }
-  } else if (CVT && warp >= 2 + S::EW) {
-    const int cw = warp - 2 - S::EW, r = 32 * cw + lane;
-    bool ok = true;
-    int it = 0, held = -1;  // held: the stage that this warp's store may still read (lane 0)
-    for (int t = unit; ok && t < pl.items; t += n_units) {
-      const MmItem x = mm_item(pl, t, K);
-      const MmTile w = grid.at(p, x.tile);
-      const int row = w.m0 + rank * 128 + r;
-      const bool live = row < M, store = w.n0 == 0 && row - lane < p.M;
-      const int target = live ? cv.tgt[row] : -1;
-      const float g = live ? cv.g[row] : 0.f;
-      // the factor of a step is fetched a step ahead: its latency would be
-      // most of a step's time (1.17 against 0.52 ms for a piece)
-      auto factor = [&](int k) { return live && k < x.k1 ? cv.f[(int64_t)(k / 128) * cv.ldf + row] : 0.f; };
-      float next = factor(x.k0);
-      for (int k = x.k0; k < x.k1; k += 64, ++it) {
-        const int s = it % ST;
-        const float f = next;
-        next = factor(k + 64);
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&copied[s], (it / ST) & 1, abort, &g_mm_fault)))) break;
-        uint8_t* line = smem + S::A + s * S::AB + r * 128;
-        const int at = target - k;
-        const bool plain = __all_sync(0xffffffffu, live && (unsigned)at >= 64u);
-        uint4 in[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) in[c] = *reinterpret_cast<const uint4*>(line + ((c ^ (r & 7)) * 16));
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4* q = reinterpret_cast<uint4*>(line + ((c ^ (r & 7)) * 16));
-          const uint4 u = in[c];
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t h = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
-            const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            v[2 * i] = d.x * f;
-            v[2 * i + 1] = d.y * f;
-          }
-          if (!plain) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = live ? v[i] - (8 * c + i == at ? g : 0.f) : 0.f;
-          }
-          *q = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (store) {  // the warp's 32 rows
-            tma_store_3d(&tm_g, smem + S::A + s * S::AB + cw * 4096, k, row, 0);
-            tma_store_commit();
-          }
-          mbar_arrive_leader(&full[s]);
-          // the stage may be copied over once the store has read it: seen one step later
-          if (held >= 0) {
-            if (store)
-              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            else
-              tma_store_wait_read();
-            mbar_arrive(&empty[held]);
-          }
-          held = store ? s : -1;
-          if (!store) mbar_arrive(&empty[s]);
-        }
-        __syncwarp();
-      }
-    }
-    if (lane == 0 && held >= 0) {
-      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      mbar_arrive(&empty[held]);
-    }
-    if (!ok) mm_raise(p, 4u, abort);
   } else {
     const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns CW half..
     int k = 0;
@@ -913,33 +818,22 @@ cudaError_t launch_join(const MmArgs&, const Epi&, int, cudaStream_t, ...) {
   return cudaErrorInvalidValue;  // an epilogue without quad() cannot be split
 }
 
-// g: where the CVT form stores its operand (same sizes as a)
-template <int SH, typename Epi, bool CVT = false>
-cudaError_t launch_mm_sh(const MmArgs& p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s,
-                         const MmConvert& cv = {}, const Operand* g = nullptr) {
+template <int SH, typename Epi>
+cudaError_t launch_mm_sh(const MmArgs& p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
   using S = MmShape<SH>;
-  CUtensorMap ta, tb, tg;
-  if (CVT && (a.mn || p.n_terms != 1 || p.nz != 1 || !g)) return cudaErrorInvalidValue;
+  CUtensorMap ta, tb;
   if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
       !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : S::BR))
     return cudaErrorInvalidValue;
-  tg = ta;
-  if (CVT && !sm100::make_operand_map(&tg, g->p, g->rows, g->cols, g->ld, g->nz, g->zs, 32)) return cudaErrorInvalidValue;
-  cudaError_t e = set_smem_once(mm_kernel<SH, Epi, CVT>, S::SMEM);
+  cudaError_t e = set_smem_once(mm_kernel<SH, Epi>, S::SMEM);
   if (e != cudaSuccess) return e;
   const int64_t m = cdiv(p.M, S::BM), n = cdiv(p.N, S::BN);
   const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
   const int units = p.split ? mm_units(SH) : (int)std::min<int64_t>(tiles, mm_units(SH));
-  e = launch_pdl(mm_kernel<SH, Epi, CVT>, dim3((unsigned)(units * S::CG)), S::THREADS + (CVT ? 128 : 0), S::SMEM, S::CG, s, ta,
-                 tb, tg, p, epi, cv);
+  e = launch_pdl(mm_kernel<SH, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<SH, Epi>(p, epi, units, s, nullptr);
-}
-
-// whether launch_mm would take the 256 x 512 shape (without its sizes' checks)
-inline bool mm_wide(const MmArgs& p) {
-  return mm_time<3>(p) < std::min({mm_time<2>(p), mm_time<1>(p), mm_time<0>(p)});
 }
 
 template <typename Epi>

@@ -26,7 +26,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "mm_sm100.cuh"
 #include "xent.cuh"
@@ -219,44 +218,6 @@ struct EpiOut {
         else
           block_store_odd(buf, lane, u, dst, n, row_ok);
       }
-    }
-  }
-};
-
-// dx of the CVT form: bf16 rows out through idx
-struct EpiRows {
-  bf16* out;
-  int64_t ldo;
-  int vec;
-  const int* idx;
-
-  __device__ __forceinline__ void quad(int row, int col, int n, float4 v) const {
-    bf16* dst = out + (int64_t)idx[row] * ldo + col;
-    if (vec) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-    } else {
-      const float x[4] = {v.x, v.y, v.z, v.w};
-      for (int q = 0; q < n; ++q) dst[q] = __float2bfloat16_rn(x[q]);
-    }
-  }
-  template <int CW>
-  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
-    const int lane = threadIdx.x % 32;
-    const bool row_ok = row < M;
-    bf16* base = out + (row_ok ? (int64_t)idx[row] : 0) * ldo;
-#pragma unroll 1
-    for (int cc = 0; cc < CW; cc += 32) {
-      const int nc = col0 + cc, n = a.N - nc;
-      if (n <= 0) break;  // warp-uniform
-      float v[32];
-      load32(taddr + cc, zero, v);
-      uint4 u[4];
-      bf16_row(v, u);
-      if (vec)
-        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + nc), n * 2, row_ok);
-      else
-        block_store_odd(buf, lane, u, base + nc, n, row_ok);
     }
   }
 };
@@ -589,56 +550,6 @@ __global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ lo
   if (threadIdx.x == 0) *loss = mean ? s / fmaxf(c, 1.f) : s;
 }
 
-// Before the CVT form of dx: joins the tiles of 8 rows (a warp each), writes
-// their losses, gradients g and targets' factors f[tile][row] = g 2^-15
-// exp(m_tile - lse), by which its exponentials become G.
-__global__ void __launch_bounds__(256) xent_factors(const float2* __restrict__ stats, int n_tiles, int rows,
-                                                    int* __restrict__ count, int base, const int* __restrict__ idx,
-                                                    const int* __restrict__ tgt, const float* __restrict__ lt,
-                                                    const float* __restrict__ grad_rows, int mean, float* losses,
-                                                    float* __restrict__ f, int64_t ldf, float* __restrict__ grow,
-                                                    float* __restrict__ loss) {
-  __shared__ float red[8], sm[8], sl[8], sg[8];
-  __shared__ int last;
-  pdl_next();
-  pdl_wait();
-  const int n_all = *count, n = cut_rows(rows, count, base);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row0 = blockIdx.x * 8, row = row0 + warp;
-  if (row < n) {
-    const float2* st = stats + (int64_t)row * n_tiles;
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int i = lane; i < n_tiles; i += 32) m = fmaxf(m, st[i].x);
-    m = warp_max(m);
-    float s = 0.f;
-#pragma unroll 4
-    for (int i = lane; i < n_tiles; i += 32) {
-      const float2 v = st[i];
-      s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e);
-    }
-    const float l = log2f(warp_sum(s));
-    if (lane == 0) {
-      float g = grad_rows ? grad_rows[idx[row]] : (mean ? 1.f / (float)n_all : 1.f);
-      if (tgt[row] < 0) g = __int_as_float(0x7fc00000);
-      losses[base + row] = row_loss(make_float2(m, l), lt[row]);
-      grow[row] = g;
-      sm[warp] = m;
-      sl[warp] = l;
-      sg[warp] = g;
-    }
-  }
-  __syncthreads();
-  const int r = threadIdx.x % 8;
-  if (row0 + r < n) {
-    const float m = sm[r], l = sl[r], g = sg[r] * 0x1p-15f;
-    for (int i = threadIdx.x / 8; i < n_tiles; i += 32) {
-      const float x = stats[(int64_t)(row0 + r) * n_tiles + i].x;
-      f[(int64_t)i * ldf + row0 + r] = x == -INFINITY ? 0.f : g * exp2f((x - m) * kLog2e - l);
-    }
-  }
-  if (loss) sum_losses(count, losses, n_all, mean, loss, red, &last);
-}
-
 // a *= *s, b *= *s, unless *s is 1; whole 16-byte chunks where aligned
 template <typename T>
 __device__ __forceinline__ void scale_run(T* p, int64_t n, float f) {
@@ -678,8 +589,7 @@ struct Plan {
   bool f32, train, pack_x, pack_w;
   int elt, planes, n_tiles, piece, n_pieces, dx_splits;
   int64_t ldx, ldw, ldp, ldd;
-  bool fused;  // dx rewrites the exponentials itself (mm_kernel's CVT form)
-  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, acc, part, f, grow, total;
+  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, acc, part, total;
 };
 
 MmArgs base_args(const Plan& q, volatile unsigned* fault) {
@@ -752,15 +662,6 @@ Plan make_plan(const llattn_xent_args& a) {
   q.p = take(q.train ? (size_t)q.piece * q.ldp * q.elt : 0);
   q.gplanes = take(q.train && q.f32 ? 6 * (size_t)q.piece * q.ldp : 0);
   q.acc = take(q.train && a.dw && q.n_pieces > 1 ? 4 * (size_t)a.vocab * q.ldd : 0);
-  // long products of both gradients: G is written by dx's kernel on its way
-  // (measured 1.60 against 1.77 ms for a piece of 8192 rows); otherwise, and
-  // for fp32's planes, xent_rows makes it
-  q.fused = !q.f32 && a.dx && a.dw && mm_wide(dx_args(q, a, q.piece, nullptr));
-  // LLATTN_XENT_FUSED=0 / 1 overrides the choice where both are possible (tests)
-  if (const char* e = std::getenv("LLATTN_XENT_FUSED")) q.fused = !q.f32 && a.dx && a.dw && e[0] == '1';
-  if (q.fused) q.gplanes = take(2 * (size_t)q.piece * q.ldp);
-  q.f = take(q.fused ? sizeof(float) * (size_t)q.n_tiles * up8(q.piece) : 0);
-  q.grow = take(q.fused ? sizeof(float) * (size_t)q.piece : 0);
   int64_t part = 0;
   if (a.dx) part = mm_part_floats(dx_args(q, a, q.piece, nullptr));
   if (a.dw) part = std::max(part, mm_part_floats(dw_args(q, a, q.piece, nullptr)));
@@ -832,30 +733,12 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     p.K = d;
     EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0};
     TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
-    float* loss = c + 1 == q.n_pieces ? a.loss : nullptr;
-    if (q.fused) {
-      float* f = reinterpret_cast<float*>(ws + q.f);
-      float* grow = reinterpret_cast<float*>(ws + q.grow);
-      const int64_t ldf = up8(q.piece);
-      TRY(launch_pdl(xent_factors, dim3(cdiv(rows, 8)), 256, 0, 1, s, stats, q.n_tiles, rows, count, base, idx + base,
-                     tgt + base, lt + base, a.grad_rows, mean, losses, f, ldf, grow, loss));
-      MmArgs m = dx_args(q, a, rows, fault);
-      m.m_dev = count;
-      m.dev_base = base;
-      m.part = part;
-      m.b_mn = 1;
-      const EpiRows er{static_cast<bf16*>(a.dx), d, aligned_rows(dx, d, 2, 2), idx + base};
-      const Operand og{gpl, rows, V, q.ldp, 1, gplane, 0};
-      TRY((launch_mm_sh<3, EpiRows, true>(m, Operand{pbuf, rows, V, q.ldp, 1, gplane, 0},
-                                          Operand{wv, V, d, q.ldw, 1, wplane, 1}, er, s,
-                                          MmConvert{f, ldf, tgt + base, grow}, &og)));
-    } else {
-      TRY(launch_pdl(xent_rows<sizeof(T) == 4>, dim3(rows), 256, sizeof(float) * q.n_tiles, 1, s, stats, q.n_tiles, rows, V,
-                     count, base, idx + base, tgt + base, lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane,
-                     loss));
-    }
-    const void* g = q.f32 || q.fused ? (const void*)gpl : pbuf;
-    if (dx && !q.fused) {
+    const size_t sm = sizeof(float) * q.n_tiles;
+    TRY(launch_pdl(xent_rows<sizeof(T) == 4>, dim3(rows), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
+                                                    lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane,
+                                                    c + 1 == q.n_pieces ? a.loss : nullptr));
+    const void* g = q.f32 ? (const void*)gpl : pbuf;
+    if (dx) {
       MmArgs m = dx_args(q, a, rows, fault);
       m.m_dev = count;
       m.dev_base = base;
