@@ -222,6 +222,7 @@ struct MmShape {
   static constexpr int STG = 4096;          // an epilogue warp's staging block: 32 rows of 128 bytes
   static constexpr int A = 0, B = A + ST * AB, STAGE = B + ST * NH * BB, BAR = STAGE + EW * STG;
   static constexpr int ACC = NH == 2 ? 1 : 2;      // accumulators in TMEM
+  static constexpr int BLOCK = 205 * (BM * BN / 1024) / 64;  // mm_plan's `block`
   static constexpr int TCOLS = NH == 2 ? 512 : 2 * BN;
   static constexpr int BYTES = BAR + 256;
   static constexpr int SMEM = BYTES + 1024;  // + alignment
@@ -238,20 +239,20 @@ struct MmPlan {
   int total, full, s, items;
 };
 
-// s splits the last, partial wave of `units` so that it costs ceil(tail s /
-// units) / s of a whole one, each range at least 8 steps of K, and a hundredth
-// of a wave per range for the partial sums' way through memory (measured: a
-// 256 x 256 fp32 block costs about what 2 steps of K do).
-__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int min_splits) {
+// s splits the last, partial wave of `units`, each range at least 8 steps of K,
+// by the time of its ceil(tail s / units) rounds in steps: the range's own,
+// 6 for its epilogue, and the partial sums' way through memory (a 256 x 256
+// block written and read takes the memory 0.2 of a step: `block`, in 1/1024).
+__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int min_splits, int block) {
   MmPlan r{total, total, 1, total};
   if (!split || total == 0) return r;
   const int full = min_splits > 1 ? 0 : total / units * units, tail = total - full;
   if (tail == 0) return r;
   int best = min_splits;
-  float cost = 1e30f;
+  int64_t cost = INT64_MAX;  // (integers: the product's and the join's kernel have to agree)
   for (int s = min_splits; s <= 32 || s == min_splits; ++s) {
     if (s > min_splits && (ksteps < 8 * s || (int64_t)tail * s > 4 * (int64_t)units)) break;
-    const float c = (float)cdiv(tail * s, units) / (float)s + 0.01f * (float)s;
+    const int64_t c = 1024 * (int64_t)cdiv(tail * s, units) * (cdiv(ksteps, s) + 6) + (s > 1 ? (int64_t)block * tail * s : 0);
     if (c < cost) {
       cost = c;
       best = s;
@@ -331,14 +332,34 @@ template <int CH>
 __device__ __forceinline__ int stage_at(int r, int c) {
   return CH == 8 ? r * 128 + ((c ^ (r & 7)) * 16) : r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
 }
-template <int CH, bool ADD = false>
-__device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, uint8_t* p, int bytes, bool ok) {
+// The 32 rows of a block in memory (16-byte aligned where not said otherwise):
+// row r at p + r stride (bytes), `rows` of them exist; or each lane's own row.
+// row(r) is null for one that does not exist; at(b): the same rows b bytes on.
+struct Rows {
+  uint8_t* p;
+  int64_t stride;
+  int rows;
+  __device__ __forceinline__ Rows(const void* p_, int64_t stride_, int rows_)
+      : p(static_cast<uint8_t*>(const_cast<void*>(p_))), stride(stride_), rows(rows_) {}
+  __device__ __forceinline__ uint8_t* row(int r) const { return r < rows ? p + r * stride : nullptr; }
+  __device__ __forceinline__ Rows at(int bytes) const { return Rows(p + bytes, stride, rows); }
+};
+struct MappedRows {
+  uint8_t* p;  // this lane's row, or null
+  __device__ __forceinline__ uint8_t* row(int r) const {
+    return reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(p), r));
+  }
+  __device__ __forceinline__ MappedRows at(int bytes) const { return MappedRows{p ? p + bytes : nullptr}; }
+};
+
+template <bool ADD, int CH, typename R>
+__device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, const R& dst, int bytes) {
   const int c = lane % CH;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int r = 32 / CH * i + lane / CH;
     const uint4 u = *reinterpret_cast<const uint4*>(buf + stage_at<CH>(r, c));
-    uint8_t* q = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
+    uint8_t* q = dst.row(r);
     if (q && 16 * c < bytes) {
       if (ADD)  // fp32: added in the L2, nothing waits for the old value
         asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(q + 16 * c), "f"(__uint_as_float(u.x)),
@@ -350,20 +371,18 @@ __device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, ui
   }
   __syncwarp();
 }
-// p: the lane's own row's first byte (16-byte aligned), bytes: valid bytes of
-// the rows (rounded up to 16 in memory), ok: the lane's row exists.
-template <int CH, bool ADD = false>
-__device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 (&v)[CH], uint8_t* p, int bytes,
-                                            bool ok) {
+// bytes: valid bytes of the rows (rounded up to 16 in memory)
+template <bool ADD = false, int CH, typename R>
+__device__ __forceinline__ void block_store(uint8_t* buf, int lane, const uint4 (&v)[CH], const R& dst, int bytes) {
 #pragma unroll
   for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
   __syncwarp();
-  block_write_out<CH, ADD>(buf, lane, p, bytes, ok);
+  block_write_out<ADD, CH>(buf, lane, dst, bytes);
 }
 // After a block_store of 32 x 32 16-bit values: the block's transpose, column c
-// of it (lane = c) as the row at p. 8 x 8 matrices go through registers
-// (transposed on the load) into the second half of the staging block.
-__device__ __forceinline__ void block_mirror(uint8_t* buf, int lane, uint8_t* p, int bytes, bool ok) {
+// of it as row c of dst. 8 x 8 matrices go through registers (transposed on
+// the load) into the second half of the staging block.
+__device__ __forceinline__ void block_mirror(uint8_t* buf, int lane, const Rows& dst, int bytes) {
   uint8_t* tb = buf + 2048;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -378,19 +397,17 @@ __device__ __forceinline__ void block_mirror(uint8_t* buf, int lane, uint8_t* p,
                  : "memory");
   }
   __syncwarp();
-  block_write_out<4>(tb, lane, p, bytes, ok);
+  block_write_out<false, 4>(tb, lane, dst, bytes);
 }
 // The reverse, in two halves so that the caller may have several in flight:
 // fetch reads global memory, spread hands each thread its row (zeros where
 // nothing was read).
 template <int CH>
-__device__ __forceinline__ void block_fetch(int lane, uint4 (&v)[CH], const void* p, int bytes, bool ok) {
+__device__ __forceinline__ void block_fetch(int lane, uint4 (&v)[CH], const Rows& src, int bytes) {
   const int c = lane % CH;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int r = 32 / CH * i + lane / CH;
-    const uint8_t* q =
-        reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
+    const uint8_t* q = src.row(32 / CH * i + lane / CH);
     v[i] = q && 16 * c < bytes ? *reinterpret_cast<const uint4*>(q + 16 * c) : make_uint4(0, 0, 0, 0);
   }
 }
@@ -406,15 +423,15 @@ __device__ __forceinline__ void block_spread(uint8_t* buf, int lane, uint4 (&v)[
 }
 // Rows without 16-byte alignment: the staged block written element by
 // element, lanes along the 32 columns (n of them valid).
-template <typename E, int CH>
-__device__ __forceinline__ void block_store_odd(uint8_t* buf, int lane, const uint4 (&v)[CH], E* p, int n, bool ok) {
+template <typename E, int CH, typename R>
+__device__ __forceinline__ void block_store_odd(uint8_t* buf, int lane, const uint4 (&v)[CH], const R& dst, int n) {
 #pragma unroll
   for (int i = 0; i < CH; ++i) *reinterpret_cast<uint4*>(buf + stage_at<CH>(lane, i)) = v[i];
   __syncwarp();
   constexpr int PER = 16 / sizeof(E);
 #pragma unroll 4
   for (int r = 0; r < 32; ++r) {
-    E* q = reinterpret_cast<E*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(ok ? p : nullptr), r));
+    E* q = reinterpret_cast<E*>(dst.row(r));
     const E e = *reinterpret_cast<const E*>(buf + stage_at<CH>(r, lane / PER) + (lane % PER) * sizeof(E));
     if (q && lane < n) q[lane] = e;
   }
@@ -474,7 +491,8 @@ template <int SH>
 __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, const MmTile& w, int row, int col, int M,
                                            uint32_t taddr, uint8_t* buf) {
   using S = MmShape<SH>;
-  float* dst = p.part + ((int64_t)x.block * S::BM + row) * S::BN + col;
+  const int lane = threadIdx.x % 32, row0 = row - lane;
+  const Rows dst{p.part + ((int64_t)x.block * S::BM + row0) * S::BN + col, S::BN * 4, M - w.m0 - row0};
 #pragma unroll 1
   for (int cc = 0; cc < S::CW; cc += 32) {
     const int n = p.N - (w.n0 + col + cc);
@@ -483,7 +501,7 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
     load32(taddr + cc, x.k1 <= x.k0, v);
     uint4 u[8];
     f32_row(v, u);
-    block_store(buf, threadIdx.x % 32, u, reinterpret_cast<uint8_t*>(dst + cc), n * 4, w.m0 + row < M);
+    block_store(buf, lane, u, dst.at(cc * 4), n * 4);
   }
 }
 
@@ -534,7 +552,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   pdl_wait();
   if (threadIdx.x == 0) {
     const MmGrid<SH> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
-    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
+    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits, S::BLOCK);
   }
   tc_fence_before();
   __syncthreads();
@@ -739,7 +757,7 @@ __global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p,
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const MmGrid<SH> grid(p, M);
   if (threadIdx.x == 0)
-    plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits);
+    plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits, S::BLOCK);
   __syncthreads();
   const MmPlan pl = plan;
   const int tile = pl.full + blockIdx.x;
@@ -776,17 +794,18 @@ inline int mm_units(int sh) { return sh >= 2 ? sm_count() / 2 : sm_count(); }
 // Estimated time (us) of a product in a shape: waves of tiles (the last one
 // split where allowed), each K / 64 steps and a gap, and the last tile's
 // epilogue. The constants are measured on a B200: a step of the pair's tile
-// takes 0.385 us, of its 512-wide one 0.72, of the others 0.28 and 0.18.
+// takes 0.385 us, of its 512-wide one 0.70, of the others 0.28 and 0.18.
 template <int SH>
 double mm_time(const MmArgs& p) {
-  constexpr double step = SH == 3 ? 0.72 : SH == 2 ? 0.385 : SH == 1 ? 0.28 : 0.18;
+  constexpr double step = SH == 3 ? 0.70 : SH == 2 ? 0.385 : SH == 1 ? 0.28 : 0.18;
   constexpr double gap = SH == 3 ? 3.0 : 0.5, tail = SH == 3 ? 8.0 : SH == 2 ? 5.5 : SH == 1 ? 4.3 : 1.2;
   const MmGrid<SH> g(p, p.M);
   const int units = mm_units(SH), ks = cdiv(p.K, 64);
-  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.min_splits);
-  double waves = pl.full / units + (pl.full % units ? 1.0 : 0.0);
-  if (pl.items > pl.full) waves += (double)cdiv(pl.items - pl.full, units) / pl.s + 0.01 * pl.s;
-  return waves * (ks * p.n_terms * step + gap) + tail;
+  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.min_splits, MmShape<SH>::BLOCK);
+  double t = (pl.full / units + (pl.full % units ? 1 : 0)) * (ks * p.n_terms * step + gap);
+  const int split = pl.items - pl.full;
+  if (split) t += cdiv(split, units) * (cdiv(ks, pl.s) * p.n_terms * step + gap) + split * step * MmShape<SH>::BLOCK / 1024;
+  return t + tail;
 }
 
 // fp32 elements of MmArgs::part for a product of at most these sizes

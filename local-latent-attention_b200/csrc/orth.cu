@@ -23,9 +23,9 @@
 //    where small singular values enter cubed.
 //  * B near the end is close to (b + c) I, and a X + B X cancels to about
 //    (a + b + c) X: rounding B would cost 4 times its 2^-12. The last two
-//    steps therefore hold B + k I with k = -(b + c), near 0, and use
-//    (a - k) X; there hi alone feeds the linear term.
-// Measured on the CPU in the same arithmetic: 0.4 to 1.5e-3 (2-norm) from the
+//    steps therefore hold B + a I, about (a + b + c) I, and update by the
+//    product alone, which also saves their epilogues the reading of X.
+// Measured on the CPU in the same arithmetic: 0.5 to 1.6e-3 (2-norm) from the
 // exact iteration over spectra from flat to 1 / k, where plain bf16 products
 // give 1 to 4e-2.
 #include <cooperative_groups.h>
@@ -43,7 +43,7 @@ namespace {
 using namespace mm;
 
 constexpr float kX = 64.f, kS = 256.f;  // scales of X and of S, B
-constexpr int kCompensated = 2;         // last steps that hold B + k I
+constexpr int kFolded = 2;              // last steps that hold B + a I
 constexpr int kParts = 64;              // partial sums of squares per matrix
 constexpr int kPtrs = 64;               // matrices per conversion launch
 
@@ -58,9 +58,8 @@ __device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, bool m
   const int lane = threadIdx.x % 32, row0 = row - lane;
   uint4 u[4];
   half_row(v, u);
-  block_store(buf, lane, u, reinterpret_cast<uint8_t*>(base + row * ld + nc), (N - nc) * 2, row < M);
-  if (mirror)
-    block_mirror(buf, lane, reinterpret_cast<uint8_t*>(base + (nc + lane) * ld + row0), (M - row0) * 2, nc + lane < N);
+  block_store(buf, lane, u, Rows{base + row0 * ld + nc, ld * 2, M - row0}, (N - nc) * 2);
+  if (mirror) block_mirror(buf, lane, Rows{base + nc * ld + row0, ld * 2, N - nc}, (M - row0) * 2);
 }
 
 // S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
@@ -100,13 +99,15 @@ struct EpiPoly {
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32;
     __half* base = b + w.z * zs;
+    const int row0 = row - lane;
+    const Rows src{s + w.z * zs + row0 * ld + col0, ld * 2, M - row0};
+    uint4 u[4];  // fetched a block ahead: its latency passes during the stores
+    if (col0 < a.N) block_fetch(lane, u, src, (a.N - col0) * 2);
 #pragma unroll 1
     for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
       if (n <= 0) break;
       float v[32];
-      uint4 u[4];
-      block_fetch(lane, u, s + w.z * zs + row * ld + nc, n * 2, row < M);
       load32(taddr + cc, zero, v);
       block_spread(buf, lane, u);
 #pragma unroll
@@ -115,12 +116,13 @@ struct EpiPoly {
         v[2 * q] = fmaf(cb, x.x, cc2 * v[2 * q]) + (row == nc + 2 * q ? k : 0.f);
         v[2 * q + 1] = fmaf(cb, x.y, cc2 * v[2 * q + 1]) + (row == nc + 2 * q + 1 ? k : 0.f);
       }
+      if (cc + 32 < CW && n > 32) block_fetch(lane, u, src.at((cc + 32) * 2), (n - 32) * 2);
       store_symmetric(base, ld, a.sym && w.m0 != w.n0, row, nc, M, a.N, v, buf);
     }
   }
 };
 
-// X <- (a - k) X + (B + k I) X
+// X <- a X + B X, or (B + a I) X
 struct EpiUpdate {
   static constexpr bool kNarrow = true, kWide = false;
   const __half* hi;
@@ -129,31 +131,38 @@ struct EpiUpdate {
   bf16* out;         // last step: [count, rows, cols]
   int64_t ld, zs, ldo, zso;
   const float* s0;
-  float ca;          // a - k
-  int rd_lo, wr_lo, vec_out;
+  float ca;          // a
+  int rd_hi, rd_lo, wr_lo, vec_out;
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32;
-    const bool ok = row < M;
+    const int row0 = row - lane, rows = M - row0;
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float fl = ca * x, fp = x / kS;
+    uint4 h[4], l[4];  // fetched a block ahead, as in EpiPoly
+    auto fetch = [&](int64_t at, int n) {
+      if (rd_hi) block_fetch(lane, h, Rows{hi + at, ld * 2, rows}, n * 2);
+      if (rd_lo) block_fetch(lane, l, Rows{lo + at, ld * 2, rows}, n * 2);
+    };
+    if (col0 < a.N) fetch(w.z * zs + row0 * ld + col0, a.N - col0);
 #pragma unroll 1
     for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
       if (n <= 0) break;
-      const int64_t at = w.z * zs + row * ld + nc;
+      const int64_t at = w.z * zs + row0 * ld + nc;
       float v[32];
-      uint4 h[4], l[4];
-      block_fetch(lane, h, hi + at, n * 2, ok);
-      if (rd_lo) block_fetch(lane, l, lo + at, n * 2, ok);
       load32(taddr + cc, zero, v);
-      block_spread(buf, lane, h);
 #pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const float2 y = half_pair(h, q);
-        v[2 * q] = fmaf(fl, y.x, fp * v[2 * q]);
-        v[2 * q + 1] = fmaf(fl, y.y, fp * v[2 * q + 1]);
+      for (int q = 0; q < 32; ++q) v[q] *= fp;
+      if (rd_hi) {
+        block_spread(buf, lane, h);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float2 y = half_pair(h, q);
+          v[2 * q] = fmaf(fl, y.x, v[2 * q]);
+          v[2 * q + 1] = fmaf(fl, y.y, v[2 * q + 1]);
+        }
       }
       if (rd_lo) {
         block_spread(buf, lane, l);
@@ -164,28 +173,30 @@ struct EpiUpdate {
           v[2 * q + 1] = fmaf(fl, y.y, v[2 * q + 1]);
         }
       }
+      if (cc + 32 < CW && n > 32) fetch(at + 32, n - 32);
+      uint4 u[4];
       if (out) {
-        bf16* dst = out + w.z * zso + row * ldo + nc;
-        bf16_row(v, h);
+        const Rows dst{out + w.z * zso + row0 * ldo + nc, ldo * 2, rows};
+        bf16_row(v, u);
         if (vec_out)
-          block_store(buf, lane, h, reinterpret_cast<uint8_t*>(dst), n * 2, ok);
+          block_store(buf, lane, u, dst, n * 2);
         else
-          block_store_odd(buf, lane, h, dst, n, ok);
+          block_store_odd<bf16>(buf, lane, u, dst, n);
         continue;
       }
 #pragma unroll
       for (int q = 0; q < 32; ++q) v[q] *= kX;
-      half_row(v, h);
-      block_store(buf, lane, h, reinterpret_cast<uint8_t*>(next + at), n * 2, ok);
+      half_row(v, u);
+      block_store(buf, lane, u, Rows{next + at, ld * 2, rows}, n * 2);
       if (wr_lo) {
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          const float2 y = half_pair(h, q);
+          const float2 y = half_pair(u, q);
           v[2 * q] -= y.x;
           v[2 * q + 1] -= y.y;
         }
-        bf16_row(v, l);
-        block_store(buf, lane, l, reinterpret_cast<uint8_t*>(lo + at), n * 2, ok);
+        bf16_row(v, u);
+        block_store(buf, lane, u, Rows{lo + at, ld * 2, rows}, n * 2);
       }
     }
   }
@@ -707,14 +718,14 @@ cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fau
     for (int i = 0; i < cnt; ++i) g.p[i] = a.g[i0 + i];
     const int n_parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts, (int64_t)m * n / 4096));
     TRY(launch_pdl(orth_square<T>, dim3(n_parts, cnt), 256, 0, 1, st, g, (int64_t)m * n, part));
-    // steps before the compensated ones read X as hi + lo
-    const int comp0 = a.steps - kCompensated;
+    // steps before the folded ones read X as hi + lo
+    const int comp0 = a.steps - kFolded;
     bf16* lo0 = sizeof(T) == 4 && comp0 > 0 ? lo : nullptr;
     TRY(launch_pdl(orth_convert<T>, dim3((unsigned)std::min<int64_t>(((int64_t)m * n + 2047) / 2048, cdiv(8 * sm_count(), cnt)), cnt), 256, 0, 1, st, g, m, n, part, n_parts, a.eps, x[0], lo0,
                                                                             p.ldx, p.xz, s0));
     for (int i = 0; i < a.steps; ++i) {
       const float* sc = i ? nullptr : s0;
-      const float k = i >= comp0 ? -(a.b + a.c) : 0.f;
+      const bool folded = i >= comp0;
       const bool last = i + 1 == a.steps;
       const __half* X = x[i & 1];
       MmArgs ma = {};
@@ -730,7 +741,7 @@ cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fau
       TRY(launch_mm(gm, og, og, EpiGram{S, p.ldb, p.bz, sc}, st));
       gm.K = p.q;
       const Operand os{S, p.q, p.q, p.ldb, cnt, p.bz, 0}, ob{B, p.q, p.q, p.ldb, cnt, p.bz, 0};
-      TRY(launch_mm(gm, os, os, EpiPoly{S, B, p.ldb, p.bz, a.b, a.c / kS, k * kS}, st));
+      TRY(launch_mm(gm, os, os, EpiPoly{S, B, p.ldb, p.bz, a.b, a.c / kS, folded ? a.a * kS : 0.f}, st));
       MmArgs um = ma;
       um.M = m;
       um.N = n;
@@ -745,8 +756,9 @@ cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fau
       eu.ldo = n;
       eu.zso = (int64_t)m * n;
       eu.s0 = sc;
-      eu.ca = a.a - k;
-      eu.rd_lo = i < comp0 && (i > 0 || lo0);
+      eu.ca = a.a;
+      eu.rd_hi = !folded;
+      eu.rd_lo = !folded && (i > 0 || lo0);
       eu.wr_lo = i + 1 < comp0;
       eu.vec_out = n % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
       TRY(p.tall ? launch_mm(um, ok, ob, eu, st) : launch_mm(um, ob, on, eu, st));

@@ -26,6 +26,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "mm_sm100.cuh"
 #include "xent.cuh"
@@ -89,7 +90,8 @@ struct EpiStats {
     // (the maximum itself gives exactly 1: a difference, not a fused product)
     const float mm = m == -INFINITY ? 0.f : m;
     float s0 = 0.f, s1 = 0.f;
-    const int64_t at = (int64_t)row * ldp + col0;
+    const int row0 = row - lane;
+    const int64_t at = (int64_t)row0 * ldp + col0;
 #pragma unroll 1
     for (int cc = 0; cc < nv; cc += 32) {
       float v[32];
@@ -105,13 +107,13 @@ struct EpiStats {
       if (p_f32) {
         uint4 u[8];
         f32_row(v, u);
-        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(static_cast<float*>(p) + at + cc), (nv - cc) * 4, row_ok);
+        block_store(buf, lane, u, Rows{static_cast<float*>(p) + at + cc, ldp * 4, M - row0}, (nv - cc) * 4);
       } else {
         uint4 u[4];
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] *= 32768.f;
         half_row(v, u);
-        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(static_cast<__half*>(p) + at + cc), (nv - cc) * 2, row_ok);
+        block_store(buf, lane, u, Rows{static_cast<__half*>(p) + at + cc, ldp * 2, M - row0}, (nv - cc) * 2);
       }
     }
     if (row_ok) {
@@ -120,6 +122,40 @@ struct EpiStats {
       stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && sum == 0.f ? -INFINITY : mm, sum);
       if ((unsigned)t < (unsigned)nv) lt[row] = tv;
     }
+  }
+};
+
+// Few tokens, no gradients: the vocabulary on the tile's long side (A = w), up
+// to 32 tokens on its short one, so that w's rows are all that is copied.
+// Statistics per token and 32 rows of w (a warp's).
+constexpr int kFew = 32;
+
+struct EpiScore {
+  static constexpr bool kNarrow = true, kWide = false;
+  float2* stats;  // [tokens][n_tiles]
+  int n_tiles;
+  const int64_t* targets;
+  float* lt;
+
+  template <int CW>
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
+                                       bool zero, uint8_t* buf) const {
+    const int lane = threadIdx.x % 32, n = min(CW, a.N - col0);
+    if (row - lane >= M) return;  // warp-uniform
+    float v[32];
+    load32(taddr, zero, v);
+    const int64_t t = lane < n ? targets[col0 + lane] : -1;
+    float2 mine = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+      if (q >= n) break;
+      const float x = row < M ? v[q] : -INFINITY;
+      const float m = warp_max(x), mm = m == -INFINITY ? 0.f : m;
+      const float s = warp_sum(row < M ? fast_exp2((x - mm) * kLog2e) : 0.f);
+      if (lane == q) mine = make_float2(m == -INFINITY && s == 0.f ? -INFINITY : mm, s);
+      if (__shfl_sync(0xffffffffu, t, q) == row) lt[col0 + q] = v[q];
+    }
+    if (lane < n) stats[(int64_t)(col0 + lane) * n_tiles + row / 32] = mine;
   }
 };
 
@@ -168,28 +204,28 @@ struct EpiOut {
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
                                        bool zero, uint8_t* buf) const {
-    const int lane = threadIdx.x % 32;
-    const bool row_ok = row < M;
-    const int64_t orow = (row_ok ? (idx ? idx[row] : row) : 0) * ldo;
+    const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0;
+    const int64_t at = row < M ? (idx ? (int64_t)idx[row] : row) * ldo + col0 : -1;
+    const MappedRows dst{at < 0 ? nullptr : static_cast<uint8_t*>(out) + at * (out_bf16 ? 2 : 4)};
     if (CW == 128 && out_bf16 && vec && !acc) {  // 64 columns, whole 128-byte lines, at a time
 #pragma unroll 1
-      for (int cc = 0; cc < 128; cc += 64) {
-        const int nc = col0 + cc, n = a.N - nc;
+      for (int cc = 0; cc < CW; cc += 64) {
+        const int n = a.N - col0 - cc;
         if (n <= 0) break;
         uint4 u[8];
         row64_bf16(taddr + cc, zero, u);
-        block_store(buf, lane, u, reinterpret_cast<uint8_t*>(static_cast<bf16*>(out) + orow + nc), n * 2, row_ok);
+        block_store(buf, lane, u, dst.at(cc * 2), n * 2);
       }
       return;
     }
     // what was summed before is fetched one block ahead: its latency passes
     // during the previous block's stores
-    const float* src = acc + (row_ok ? (int64_t)row * ldacc : 0) + col0;  // ldacc is a multiple of 8
+    const Rows src{acc + (int64_t)row0 * ldacc + col0, ldacc * 4, rows};  // ldacc is a multiple of 8
     uint4 x[8];
-    if (acc && col0 < a.N) block_fetch(lane, x, src, (a.N - col0) * 4, row_ok);
+    if (acc && col0 < a.N) block_fetch(lane, x, src, (a.N - col0) * 4);
 #pragma unroll 1
     for (int cc = 0; cc < CW; cc += 32) {
-      const int nc = col0 + cc, n = a.N - nc;
+      const int n = a.N - col0 - cc;
       if (n <= 0) break;  // warp-uniform
       float v[32];
       load32(taddr + cc, zero, v);
@@ -197,26 +233,24 @@ struct EpiOut {
         block_spread(buf, lane, x);
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(word(x, q));
-        if (cc + 32 < CW && n > 32) block_fetch(lane, x, src + cc + 32, (n - 32) * 4, row_ok);
+        if (cc + 32 < CW && n > 32) block_fetch(lane, x, src.at((cc + 32) * 4), (n - 32) * 4);
       }
       if (out_bf16) {
         uint4 u[4];
-        bf16* dst = static_cast<bf16*>(out) + orow + nc;
         bf16_row(v, u);
         if (vec)
-          block_store(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 2, row_ok);
+          block_store(buf, lane, u, dst.at(cc * 2), n * 2);
         else
-          block_store_odd(buf, lane, u, dst, n, row_ok);
+          block_store_odd<bf16>(buf, lane, u, dst.at(cc * 2), n);
       } else {
         uint4 u[8];
-        float* dst = static_cast<float*>(out) + orow + nc;
         f32_row(v, u);
         if (add)
-          block_store<8, true>(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 4, row_ok);
+          block_store<true>(buf, lane, u, dst.at(cc * 4), n * 4);
         else if (vec)
-          block_store(buf, lane, u, reinterpret_cast<uint8_t*>(dst), n * 4, row_ok);
+          block_store(buf, lane, u, dst.at(cc * 4), n * 4);
         else
-          block_store_odd(buf, lane, u, dst, n, row_ok);
+          block_store_odd<float>(buf, lane, u, dst.at(cc * 4), n);
       }
     }
   }
@@ -384,9 +418,11 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
 template <int NT>
 __device__ __forceinline__ float2 join_tiles(const float2* __restrict__ st, int n_tiles, float* red) {
   float m = -INFINITY;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n_tiles; i += NT) m = fmaxf(m, st[i].x);
   m = block_max<NT>(m, red);
   float s = 0.f;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n_tiles; i += NT) {
     const float2 v = st[i];
     s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e);
@@ -397,28 +433,17 @@ __device__ __forceinline__ float2 join_tiles(const float2* __restrict__ st, int 
 
 __device__ __forceinline__ float row_loss(float2 lse, float lt) { return (lse.x - lt) + lse.y * kLn2; }
 
-// Losses without gradients: one warp per row.
-__global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ stats, int n_tiles, int n,
+// Losses without gradients: one CTA per row.
+__global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ stats, int n_tiles,
                                                    const float* __restrict__ lt, const int64_t* __restrict__ targets,
                                                    int64_t ignore, int vocab, float* __restrict__ losses) {
+  __shared__ float red[4];
   pdl_next();
   pdl_wait();
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  if (row >= n) return;
-  const int lane = threadIdx.x % 32;
-  const int64_t t = targets[row];
-  const float2* st = stats + row * n_tiles;
-  float m = -INFINITY;
-  for (int i = lane; i < n_tiles; i += 32) m = fmaxf(m, st[i].x);
-  m = warp_max(m);
-  float s = 0.f;
-  for (int i = lane; i < n_tiles; i += 32) {
-    const float2 v = st[i];
-    s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e);
-  }
-  s = warp_sum(s);
-  if (lane == 0) {
-    float l = t >= 0 && t < vocab ? row_loss(make_float2(m, log2f(s)), lt[row]) : __int_as_float(0x7fc00000);
+  const int64_t row = blockIdx.x, t = targets[row];
+  const float2 lse = join_tiles<128>(stats + row * n_tiles, n_tiles, red);
+  if (threadIdx.x == 0) {
+    const float l = t >= 0 && t < vocab ? row_loss(lse, lt[row]) : __int_as_float(0x7fc00000);
     losses[row] = t == ignore ? 0.f : l;
   }
 }
@@ -429,7 +454,7 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    *last = atomicAdd(count + 1, 1) == (int)gridDim.x - 1;
+    *last = atomicAdd(count + 1, 1) == (int)(gridDim.x * gridDim.y) - 1;
   }
   __syncthreads();
   if (!*last) return;
@@ -441,13 +466,13 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
   if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
 }
 
-// One CTA per row of a piece: joins the tiles, writes the row's loss and
-// rewrites the exponentials as G = g (p - onehot) (bf16 in place of fp16, or
+// One CTA per row of a piece (few rows: SHARES of them, along y, each a share
+// of the columns): joins the tiles, writes the row's loss and rewrites the exponentials as G = g (p - onehot) (bf16 in place of fp16, or
 // fp32 -> three bf16 planes). Rows between the count and the next multiple
 // of 64 become zeros: the third product reads them. The last CTA of the last
 // piece to finish sums the losses (thread t those of index t mod 256, then
 // in thread order: the same bits whichever CTA it is).
-template <bool F32>
+template <bool F32, int SHARES>
 __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stats, int n_tiles, int rows, int vocab,
                                                  int* __restrict__ count, int base, const int* __restrict__ idx,
                                                  const int* __restrict__ tgt, const float* __restrict__ lt,
@@ -465,7 +490,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   if (row >= n) {
     if (row < cdiv(n, 64) * 64) {
       const uint4 z = make_uint4(0, 0, 0, 0);
-      for (int64_t c = threadIdx.x; c < ldp / 8; c += 256) {
+      for (int64_t c = blockIdx.y * 256 + threadIdx.x; c < ldp / 8; c += 256 * SHARES) {
         if (F32) {
           for (int k = 0; k < 3; ++k) reinterpret_cast<uint4*>(planes + k * plane + row * ldp)[c] = z;
         } else {
@@ -479,7 +504,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   const float2* st = stats + row * n_tiles;
   const float2 lse = join_tiles<256>(st, n_tiles, red);
   const int t = tgt[row];
-  if (threadIdx.x == 0) losses[base + row] = row_loss(lse, lt[row]);
+  if (threadIdx.x == 0 && blockIdx.y == 0) losses[base + row] = row_loss(lse, lt[row]);
   float g = grad_rows ? grad_rows[idx[row]] : (mean ? 1.f / (float)n_all : 1.f);
   if (t < 0) g = __int_as_float(0x7fc00000);
   // tile factors: g 2^(m_tile - lse)
@@ -488,7 +513,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
     xent_f[i] = m == -INFINITY ? 0.f : g * exp2f((m - lse.x) * kLog2e - lse.y) * (F32 ? 1.f : 0x1p-15f);
   }
   __syncthreads();
-  for (int c = threadIdx.x * 8; c < vocab; c += 256 * 8) {
+  for (int c = (blockIdx.y * 256 + threadIdx.x) * 8; c < vocab; c += 256 * 8 * SHARES) {
     const float f = xent_f[c / kTile];
     float v[8];
     if (F32) {
@@ -586,7 +611,7 @@ bool aligned_rows(const void* p, int64_t ld, int64_t rows, int elt) {
 }
 
 struct Plan {
-  bool f32, train, pack_x, pack_w;
+  bool f32, train, few, pack_x, pack_w;
   int elt, planes, n_tiles, piece, n_pieces, dx_splits;
   int64_t ldx, ldw, ldp, ldd;
   size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, acc, part, total;
@@ -633,7 +658,8 @@ Plan make_plan(const llattn_xent_args& a) {
   q.ldw = q.pack_w ? up8(a.d) : (a.vocab == 1 ? up8(a.d) : a.ldw);
   q.ldp = up8(a.vocab);
   q.ldd = up8(a.d);
-  q.n_tiles = cdiv(a.vocab, kTile);
+  q.few = !q.train && a.tokens <= kFew;
+  q.n_tiles = cdiv(a.vocab, q.few ? 32 : kTile);
   // rows of exponentials held at a time: half a GiB of them (V = 32000 in
   // bf16: 8192 rows), whole row tiles. fp32 also bounds the length of each
   // tensor-core sum: its additions truncate, about 2^-26 of the running sum per
@@ -698,14 +724,20 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       TRY(launch_pdl(xent_pack<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane));
     }
     MmArgs p = base_args(q, fault);
-    p.M = n;
-    p.N = V;
+    const Operand ox{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0}, ow{wv, V, d, q.ldw, q.planes, wplane, 0};
     p.K = d;
-    EpiStats ep{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0};
-    TRY(launch_mm(p, Operand{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0},
-                  Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
+    if (q.few) {
+      p.M = V;
+      p.N = n;
+      std::swap(p.pa, p.pb);
+      TRY(launch_mm_sh<0>(p, ow, ox, EpiScore{stats, q.n_tiles, a.targets, lt}, s));
+    } else {
+      p.M = n;
+      p.N = V;
+      TRY(launch_mm(p, ox, ow, EpiStats{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0}, s));
+    }
     float* losses = a.losses ? a.losses : reinterpret_cast<float*>(ws + q.losses);
-    TRY(launch_pdl(xent_losses, dim3(cdiv(n, 4)), 128, 0, 1, s, stats, q.n_tiles, n, lt, a.targets, a.ignore_index, V, losses));
+    TRY(launch_pdl(xent_losses, dim3(n), 128, 0, 1, s, stats, q.n_tiles, lt, a.targets, a.ignore_index, V, losses));
     if (a.loss) {
       TRY(launch_pdl(xent_reduce, dim3(1), 1024, 0, 1, s, losses, n, a.targets, a.ignore_index, mean, a.loss));
     }
@@ -734,9 +766,12 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0};
     TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
-    TRY(launch_pdl(xent_rows<sizeof(T) == 4>, dim3(rows), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
-                                                    lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane,
-                                                    c + 1 == q.n_pieces ? a.loss : nullptr));
+    auto rows_pass = [&](auto kernel, int shares) {
+      return launch_pdl(kernel, dim3(rows, shares), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
+                        lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, c + 1 == q.n_pieces ? a.loss : nullptr);
+    };
+    const bool share = rows <= 2 * sm_count() && V >= 4096;  // (129 rows of 32000: 12.7 -> 9.1 us)
+    TRY(share ? rows_pass(xent_rows<sizeof(T) == 4, 4>, 4) : rows_pass(xent_rows<sizeof(T) == 4, 1>, 1));
     const void* g = q.f32 ? (const void*)gpl : pbuf;
     if (dx) {
       MmArgs m = dx_args(q, a, rows, fault);
