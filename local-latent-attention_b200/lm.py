@@ -29,6 +29,8 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 from .module import LocalLatentAttentionB200
+from .optim import Muon, OptimizerPair
+from .training_ops import linear_cross_entropy
 
 
 @dataclass
@@ -111,6 +113,10 @@ class LocalLatentLM(nn.Module):
         self.lm_head = nn.Linear(config.d_model, config.vocab_size, bias=False)
         self.lm_head.weight = self.embedding.weight
         gpt2_init_(self, config.n_layers, skip=self.lm_head)
+        # True: the loss of forward(ids, targets) by linear_cross_entropy, which
+        # never holds the [B T, vocab] logits (CUDA only); False: the logits in
+        # memory and F.cross_entropy, as the reference's training loop
+        self.fused_loss = False
 
     def set_profile(self, enabled: bool) -> None:
         for layer in self.blocks:
@@ -136,6 +142,8 @@ class LocalLatentLM(nn.Module):
         return self.lm_head(self.norm(x))
 
     def loss_head(self, x: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        if self.fused_loss:
+            return linear_cross_entropy(self.norm(x), self.lm_head.weight, targets)
         logits = self.lm_head(self.norm(x))
         return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), targets.reshape(-1))
 
@@ -215,14 +223,26 @@ def _sample(logits: torch.Tensor, temperature: float, top_k: int, generator) -> 
     return torch.multinomial(torch.softmax(logits, dim=-1), 1, generator=generator)
 
 
-def build_optimizer(model: nn.Module, lr: float = 3e-4, weight_decay: float = 0.1):
-    """AdamW(beta 0.9/0.95), decay on >= 2-D params only (train.py:851-859)."""
-    decay, no_decay = [], []
-    for p in model.parameters():
-        if p.requires_grad:
+def build_optimizer(model: nn.Module, lr: float = 3e-4, weight_decay: float = 0.1, hidden: str = "adamw"):
+    """AdamW(beta 0.9/0.95), decay on >= 2-D params only (train.py:851-859).
+    hidden="muon": the layers' matrices (blocks.*, more than one row) by Muon
+    with the same lr and decay, the rest (embeddings, the tied head, biases,
+    norm gains, gate vectors) by AdamW; both step together."""
+    if hidden not in ("adamw", "muon"):
+        raise ValueError(f"build_optimizer: hidden must be 'adamw' or 'muon', got {hidden!r}")
+    decay, no_decay, matrices = [], [], []
+    for name, p in model.named_parameters():
+        if not p.requires_grad:
+            continue
+        if hidden == "muon" and "blocks." in name and p.dim() == 2 and min(p.shape) > 1:
+            matrices.append(p)
+        else:
             (decay if p.dim() >= 2 else no_decay).append(p)
     groups = [{"params": decay, "weight_decay": weight_decay}, {"params": no_decay, "weight_decay": 0.0}]
-    return torch.optim.AdamW(groups, lr=lr, betas=(0.9, 0.95), fused=torch.cuda.is_available())
+    adamw = torch.optim.AdamW(groups, lr=lr, betas=(0.9, 0.95), fused=torch.cuda.is_available())
+    if hidden == "adamw":
+        return adamw
+    return OptimizerPair(Muon(matrices, lr=lr, weight_decay=weight_decay), adamw)
 
 
 def train_step(model: nn.Module, optimizer, ids: torch.Tensor, targets: torch.Tensor, grad_clip: float = 1.0,

@@ -54,3 +54,31 @@ class Muon(torch.optim.Optimizer):
             for p, u in zip(params, updates):
                 p.add_(u, alpha=-group["lr"] * 0.2 * max(p.shape) ** 0.5)
         return loss
+
+
+class OptimizerPair:
+    """Optimisers over disjoint parameters that step together."""
+
+    def __init__(self, *optimizers: torch.optim.Optimizer) -> None:
+        self.optimizers = optimizers
+
+    @property
+    def param_groups(self) -> list[dict]:
+        return [g for o in self.optimizers for g in o.param_groups]
+
+    def step(self) -> None:
+        for o in self.optimizers:
+            o.step()
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for o in self.optimizers:
+            o.zero_grad(set_to_none=set_to_none)
+
+    def state_dict(self) -> list[dict]:
+        return [o.state_dict() for o in self.optimizers]
+
+    def load_state_dict(self, state: list[dict]) -> None:
+        if len(state) != len(self.optimizers):
+            raise ValueError(f"OptimizerPair: {len(state)} states for {len(self.optimizers)} optimisers")
+        for o, s in zip(self.optimizers, state):
+            o.load_state_dict(s)
