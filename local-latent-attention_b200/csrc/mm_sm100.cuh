@@ -461,12 +461,14 @@ __device__ __forceinline__ void f32_row(const float (&v)[32], uint4 (&u)[8]) {
     u[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
                       __float_as_uint(v[4 * q + 3]));
 }
-// 64 accumulator columns of this thread's row as bf16
-__device__ __forceinline__ void row64_bf16(uint32_t taddr, bool zero, uint4 (&u)[8]) {
+// 64 accumulator columns of this thread's row, times f, as bf16
+__device__ __forceinline__ void row64_bf16(uint32_t taddr, bool zero, float f, uint4 (&u)[8]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float v[32];
     load32(taddr + 32 * h, zero, v);
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] *= f;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       u[4 * h + q] = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),

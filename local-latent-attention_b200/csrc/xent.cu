@@ -16,6 +16,9 @@
 // joins the tiles' (m, sum) to the row's logsumexp and rewrites the
 // piece in place as bf16 G, which the other two products read. One pass over
 // the exponentials (4 bytes per element) replaces a second 2 N V d product.
+// The mean's 1 / count stays out of G (a common factor rounded to 8 bits would
+// be a common error of all rows, and p - 1 would not be exact near -1); the
+// gradients' epilogues apply it in fp32.
 //
 // Gradients run over the tokens that count only: xent_prep lists them (in
 // order), the sizes of the products follow the device-side count, and rows
@@ -171,6 +174,9 @@ struct EpiOut {
   const float* acc;     // added first (fp32, row stride ldacc), or null
   int64_t ldacc;
   const int* idx;       // output row of row m, or null
+  const int* count;     // the result is divided by max(1, *count), or null
+
+  __device__ __forceinline__ float scale() const { return count ? 1.f / (float)max(1, *count) : 1.f; }
 
   // 4 columns of a row of a split tile, joined
   __device__ __forceinline__ void quad(int row, int col, int n, float4 v) const {
@@ -178,6 +184,8 @@ struct EpiOut {
       const float4 c = *reinterpret_cast<const float4*>(acc + (int64_t)row * ldacc + col);
       v = make_float4(v.x + c.x, v.y + c.y, v.z + c.z, v.w + c.w);
     }
+    const float f = scale();
+    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
     const int64_t at = (int64_t)(idx ? idx[row] : row) * ldo + col;
     const float x[4] = {v.x, v.y, v.z, v.w};
     if (out_bf16) {
@@ -206,6 +214,7 @@ struct EpiOut {
                                        bool zero, uint8_t* buf) const {
     const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0;
     const int64_t at = row < M ? (idx ? (int64_t)idx[row] : row) * ldo + col0 : -1;
+    const float f = scale();
     const MappedRows dst{at < 0 ? nullptr : static_cast<uint8_t*>(out) + at * (out_bf16 ? 2 : 4)};
     if (CW == 128 && out_bf16 && vec && !acc) {  // 64 columns, whole 128-byte lines, at a time
 #pragma unroll 1
@@ -213,7 +222,7 @@ struct EpiOut {
         const int n = a.N - col0 - cc;
         if (n <= 0) break;
         uint4 u[8];
-        row64_bf16(taddr + cc, zero, u);
+        row64_bf16(taddr + cc, zero, f, u);
         block_store(buf, lane, u, dst.at(cc * 2), n * 2);
       }
       return;
@@ -235,6 +244,8 @@ struct EpiOut {
         for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(word(x, q));
         if (cc + 32 < CW && n > 32) block_fetch(lane, x, src.at((cc + 32) * 4), (n - 32) * 4);
       }
+#pragma unroll
+      for (int q = 0; q < 32; ++q) v[q] *= f;
       if (out_bf16) {
         uint4 u[4];
         bf16_row(v, u);
@@ -467,7 +478,8 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
 }
 
 // One CTA per row of a piece (few rows: SHARES of them, along y, each a share
-// of the columns): joins the tiles, writes the row's loss and rewrites the exponentials as G = g (p - onehot) (bf16 in place of fp16, or
+// of the columns): joins the tiles, writes the row's loss and rewrites the
+// exponentials as G = g (p - onehot), g = 1 or grad_rows (bf16 in place of fp16, or
 // fp32 -> three bf16 planes). Rows between the count and the next multiple
 // of 64 become zeros: the third product reads them. The last CTA of the last
 // piece to finish sums the losses (thread t those of index t mod 256, then
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   const float2 lse = join_tiles<256>(st, n_tiles, red);
   const int t = tgt[row];
   if (threadIdx.x == 0 && blockIdx.y == 0) losses[base + row] = row_loss(lse, lt[row]);
-  float g = grad_rows ? grad_rows[idx[row]] : (mean ? 1.f / (float)n_all : 1.f);
+  float g = grad_rows ? grad_rows[idx[row]] : 1.f;
   if (t < 0) g = __int_as_float(0x7fc00000);
   // tile factors: g 2^(m_tile - lse)
   for (int i = threadIdx.x; i < n_tiles; i += 256) {
@@ -784,6 +796,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.out_bf16 = !q.f32;
       eo.vec = aligned_rows(dx, d, 2, q.elt);
       eo.idx = idx + base;
+      eo.count = mean ? count : nullptr;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
                     s));
     }
@@ -801,6 +814,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.add = c && !last;
       eo.acc = c && last ? acc : nullptr;
       eo.ldacc = q.ldd;
+      eo.count = last && mean ? count : nullptr;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
                     eo, s));
     }
