@@ -203,19 +203,20 @@ __device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
 //      not hold the tensor cores up.
 //  2 = 256 x 256 on a pair, two accumulators
 //  1 = 128 x 128 on a CTA, two accumulators
+//  4 = 128 x 64 on a CTA, between 1 and 0
 //  0 = 128 x 32 on a CTA, for products too small to occupy the SMs otherwise:
 //      its epilogue is one block of 32 columns per warp instead of four (4.2 ->
 //      1.1 us at the end of a kernel), and a step copies 20 KB instead of 32.
 template <int SH>
 struct MmShape {
-  static constexpr int CG = SH >= 2 ? 2 : 1;
+  static constexpr int CG = SH == 2 || SH == 3 ? 2 : 1;
   static constexpr int NH = SH == 3 ? 2 : 1;  // column halves of the accumulator, an MMA each
-  static constexpr int BM = 128 * CG, BN = SH == 3 ? 512 : SH == 2 ? 256 : SH == 1 ? 128 : 32;  // tile of the CTA (pair)
+  static constexpr int BM = 128 * CG, BN = SH == 3 ? 512 : SH == 2 ? 256 : SH == 1 ? 128 : SH == 4 ? 64 : 32;  // tile of the CTA (pair)
   static constexpr int HN = BN / NH;              // columns of an MMA
   static constexpr int CW = HN < 128 ? HN : 128;  // columns of an epilogue warp (32 rows) in a half
   static constexpr int EW = 4 * (HN / CW);        // epilogue warps
   static constexpr int THREADS = 64 + 32 * EW;
-  static constexpr int ST = SH == 3 ? 4 : SH == 0 ? 8 : 6;
+  static constexpr int ST = SH == 3 ? 4 : BN < 128 ? 8 : 6;
   static constexpr int BR = HN / CG;        // rows of B that a CTA copies per half
   static constexpr int AB = 128 * 64 * 2;   // one CTA's A tile: 128 rows x 64 K, 16 KB
   static constexpr int BB = (BR < 64 ? 64 : BR) * 64 * 2;  // B tile of a half (a whole panel of 64 if MN-major)
@@ -510,7 +511,7 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
 //                                          bool zero, uint8_t* buf) const
-//   static constexpr bool kNarrow, kWide: the 128 x 32 (CW = 32, else 128) and 256 x 512 shapes may be used
+//   static constexpr bool kNarrow, kWide: shapes 0 and 4 (CW = 32 and 64, else 128), and 3, may be used
 // tile is called by every thread of an epilogue warp (all 32 lanes,
 // converged) for its row and CW columns [col0, col0 + CW); taddr: TMEM address of the warp's
 // lanes and columns; zero: the K range is empty, the accumulator holds
@@ -791,16 +792,16 @@ struct Operand {
   int mn;  // stored MN-major (rows = K, cols = MN) instead of K-major (rows = MN, cols = K)
 };
 
-inline int mm_units(int sh) { return sh >= 2 ? sm_count() / 2 : sm_count(); }
+inline int mm_units(int sh) { return sh == 2 || sh == 3 ? sm_count() / 2 : sm_count(); }
 
 // Estimated time (us) of a product in a shape: waves of tiles (the last one
 // split where allowed), each K / 64 steps and a gap, and the last tile's
 // epilogue. The constants are measured on a B200: a step of the pair's tile
-// takes 0.385 us, of its 512-wide one 0.70, of the others 0.28 and 0.18.
+// takes 0.385 us, of its 512-wide one 0.70, of the others 0.28, 0.22 and 0.18.
 template <int SH>
 double mm_time(const MmArgs& p) {
-  constexpr double step = SH == 3 ? 0.70 : SH == 2 ? 0.385 : SH == 1 ? 0.28 : 0.18;
-  constexpr double gap = SH == 3 ? 3.0 : 0.5, tail = SH == 3 ? 8.0 : SH == 2 ? 5.5 : SH == 1 ? 4.3 : 1.2;
+  constexpr double step = SH == 3 ? 0.70 : SH == 2 ? 0.385 : SH == 1 ? 0.28 : SH == 4 ? 0.22 : 0.18;
+  constexpr double gap = SH == 3 ? 3.0 : 0.5, tail = SH == 3 ? 8.0 : SH == 2 ? 5.5 : SH == 1 ? 4.3 : SH == 4 ? 2.3 : 1.2;
   const MmGrid<SH> g(p, p.M);
   const int units = mm_units(SH), ks = cdiv(p.K, 64);
   const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.min_splits, MmShape<SH>::BLOCK);
@@ -818,7 +819,7 @@ inline int64_t mm_part_floats(const MmArgs& p) {
     return std::max<int64_t>(4 * mm_units(sh), p.min_splits > 1 ? tiles * p.nz * p.min_splits : 0) * block;
   };
   return std::max({floats(3, MmGrid<3>(p, p.M).per_z, 256 * 512), floats(2, MmGrid<2>(p, p.M).per_z, 256 * 256), floats(1, MmGrid<1>(p, p.M).per_z, 128 * 128),
-                   floats(0, MmGrid<0>(p, p.M).per_z, 128 * 32)});
+                   floats(4, MmGrid<4>(p, p.M).per_z, 128 * 64), floats(0, MmGrid<0>(p, p.M).per_z, 128 * 32)});
 }
 
 // whether mm_plan may split anything, whatever the device-side counts
@@ -869,7 +870,9 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
   if constexpr (Epi::kNarrow) {
     MmArgs q = p;
     q.sym = 0;  // not square: every tile is computed
-    if (mm_time<0>(q) < std::min(t1, t2)) return launch_mm_sh<0>(q, a, b, epi, s);
+    const double t4 = mm_time<4>(q), t0 = mm_time<0>(q);
+    if (std::min(t0, t4) < std::min(t1, t2))
+      return t0 <= t4 ? launch_mm_sh<0>(q, a, b, epi, s) : launch_mm_sh<4>(q, a, b, epi, s);
   }
   if constexpr (Epi::kWide) {
     if (mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s);

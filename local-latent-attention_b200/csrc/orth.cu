@@ -52,7 +52,7 @@ struct Ptrs {
 };
 
 // Stores 32 columns of a symmetric matrix's tile, and off the diagonal (of the
-// shapes that skip the tiles above it) their mirror image: column nc + lane of the block becomes that row, from row0 on.
+// square tile shapes, which skip those above it) their mirror image: column nc + lane of the block becomes that row, from row0 on.
 __device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, bool mirror, int row, int nc, int M, int N,
                                                 const float (&v)[32], uint8_t* buf) {
   const int lane = threadIdx.x % 32, row0 = row - lane;
