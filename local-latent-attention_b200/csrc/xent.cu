@@ -24,8 +24,11 @@
 // order), the sizes of the products follow the device-side count, and rows
 // of ignored tokens are never read, so their values cannot reach dw.
 //
-// fp32: x, w and G are split into three bf16 planes each (24 bits) and every
-// product sums the six plane products above 2^-24, smallest first.
+// fp32: x, w and G are split into two fp16 planes each, hi + lo (22 bits), after
+// a power of two has brought the largest value of each below 2^15 (xent_amax;
+// an element keeps its 22 bits down to 2^-17 of the largest, and an error of
+// 2^-40 of it below), and every product sums lo hi + hi lo + hi hi. Three bf16
+// planes would need six products for 24 bits.
 #include <math.h>
 
 #include <algorithm>
@@ -45,8 +48,12 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 128;  // columns per (max, sum) statistic
 constexpr int kF32Chain = 1024;  // products per tensor-core sum of the fp32 gradients
 
-// six plane products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u;
+constexpr uint32_t kTermsA = 0x001u, kTermsB = 0x010u;  // planes (1,0) (0,1) (0,0)
+
+// fp32's powers of two: of x, w, G, and the inverses that undo them in x w^T,
+// G w and G^T x
+enum { kScX = 0, kScW, kScG, kUnXW, kUnGW, kUnGX, kScales };
+constexpr int kAmax = 128;  // partial maxima each of x, w and the rows' gradients
 
 // ---- first product: statistics and exponentials ----------------------------
 
@@ -60,6 +67,7 @@ struct EpiStats {
   void* p;             // exponentials of the rows, or null
   int64_t ldp;
   int p_f32;           // fp32 instead of fp16 * 2^15
+  const float* un;     // logit = accumulator * *un, or null
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
@@ -91,7 +99,7 @@ struct EpiStats {
     }
     // fmaxf drops NaN: a row of NaN leaves m at -inf, and the sums below carry it
     // (the maximum itself gives exactly 1: a difference, not a fused product)
-    const float mm = m == -INFINITY ? 0.f : m;
+    const float mm = m == -INFINITY ? 0.f : m, f = un ? *un : 1.f, k = f * kLog2e;
     float s0 = 0.f, s1 = 0.f;
     const int row0 = row - lane;
     const int64_t at = (int64_t)row0 * ldp + col0;
@@ -100,7 +108,7 @@ struct EpiStats {
       float v[32];
       load32(taddr + cc, zero, v);
 #pragma unroll
-      for (int q = 0; q < 32; ++q) v[q] = cc + q < nv ? fast_exp2((v[q] - mm) * kLog2e) : 0.f;
+      for (int q = 0; q < 32; ++q) v[q] = cc + q < nv ? fast_exp2((v[q] - mm) * k) : 0.f;
 #pragma unroll
       for (int q = 0; q < 32; q += 2) {
         s0 += v[q];
@@ -122,8 +130,8 @@ struct EpiStats {
     if (row_ok) {
       // every column -inf: nothing to add
       const float sum = s0 + s1;
-      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && sum == 0.f ? -INFINITY : mm, sum);
-      if ((unsigned)t < (unsigned)nv) lt[row] = tv;
+      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && sum == 0.f ? -INFINITY : mm * f, sum);
+      if ((unsigned)t < (unsigned)nv) lt[row] = tv * f;
     }
   }
 };
@@ -139,6 +147,7 @@ struct EpiScore {
   int n_tiles;
   const int64_t* targets;
   float* lt;
+  const float* un;  // as in EpiStats
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
@@ -149,14 +158,15 @@ struct EpiScore {
     load32(taddr, zero, v);
     const int64_t t = lane < n ? targets[col0 + lane] : -1;
     float2 mine = make_float2(0.f, 0.f);
+    const float f = un ? *un : 1.f, k = f * kLog2e;
 #pragma unroll
     for (int q = 0; q < 32; ++q) {
       if (q >= n) break;
       const float x = row < M ? v[q] : -INFINITY;
       const float m = warp_max(x), mm = m == -INFINITY ? 0.f : m;
-      const float s = warp_sum(row < M ? fast_exp2((x - mm) * kLog2e) : 0.f);
-      if (lane == q) mine = make_float2(m == -INFINITY && s == 0.f ? -INFINITY : mm, s);
-      if (__shfl_sync(0xffffffffu, t, q) == row) lt[col0 + q] = v[q];
+      const float s = warp_sum(row < M ? fast_exp2((x - mm) * k) : 0.f);
+      if (lane == q) mine = make_float2(m == -INFINITY && s == 0.f ? -INFINITY : mm * f, s);
+      if (__shfl_sync(0xffffffffu, t, q) == row) lt[col0 + q] = v[q] * f;
     }
     if (lane < n) stats[(int64_t)(col0 + lane) * n_tiles + row / 32] = mine;
   }
@@ -175,8 +185,11 @@ struct EpiOut {
   int64_t ldacc;
   const int* idx;       // output row of row m, or null
   const int* count;     // the result is divided by max(1, *count), or null
+  const float* un;      // and multiplied by *un, or null
 
-  __device__ __forceinline__ float scale() const { return count ? 1.f / (float)max(1, *count) : 1.f; }
+  __device__ __forceinline__ float scale() const {
+    return (count ? 1.f / (float)max(1, *count) : 1.f) * (un ? *un : 1.f);
+  }
 
   // 4 columns of a row of a split tile, joined
   __device__ __forceinline__ void quad(int row, int col, int n, float4 v) const {
@@ -292,18 +305,85 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return r;
 }
 
-// fp32 -> three bf16 planes whose sum is the value to 2^-24
-__device__ __forceinline__ void split3(float v, bf16& a, bf16& b, bf16& c) {
-  a = __float2bfloat16_rn(v);
-  const float r = v - __bfloat162float(a);
-  b = __float2bfloat16_rn(r);
-  c = __float2bfloat16_rn(r - __bfloat162float(b));
+// whether rows can be read in 16-byte chunks (and need no padding columns)
+template <typename T>
+__device__ __forceinline__ bool vec_rows(const T* p, int64_t ld, int d) {
+  return ld % 8 == 0 && d % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-// A warp's row: dst = src (bf16, or three planes of fp32), zeros from column d
-// to lds, or everywhere where src is null.
+// ---- fp32's scales: largest magnitudes of x (the rows that count), w and the
+// rows' gradients, in kAmax partial maxima each
+__global__ void __launch_bounds__(256) xent_amax(const float* __restrict__ x, int64_t ldx, int n, int d,
+                                                 const int64_t* __restrict__ targets, int64_t ignore,
+                                                 const float* __restrict__ w, int64_t ldw, int vocab,
+                                                 const float* __restrict__ grad_rows, float* __restrict__ part) {
+  __shared__ float red[8];
+  pdl_next();
+  pdl_wait();
+  const int what = blockIdx.x / kAmax, i = blockIdx.x % kAmax, lane = threadIdx.x % 32;
+  float m = 0.f;
+  if (what < 2) {
+    const float* p = what ? w : x;
+    const int64_t ld = what ? ldw : ldx, rows = what ? vocab : n;
+    for (int64_t r = i * 8 + threadIdx.x / 32; r < rows; r += 8 * kAmax) {
+      if (!what && targets[r] == ignore) continue;
+      if (vec_rows(p, ld, d)) {
+        const float4* q = reinterpret_cast<const float4*>(p + r * ld);
+#pragma unroll 8
+        for (int c = lane; c < d / 4; c += 32) {
+          const float4 v = q[c];
+          m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+      } else {
+#pragma unroll 8
+        for (int c = lane; c < d; c += 32) m = fmaxf(m, fabsf(p[r * ld + c]));
+      }
+    }
+  } else {
+    for (int64_t r = i * 256 + threadIdx.x; r < n; r += 256 * kAmax)
+      if (targets[r] != ignore) m = fmaxf(m, grad_rows ? fabsf(grad_rows[r]) : 1.f);
+  }
+  m = block_max<256>(m, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = m;
+}
+
+// the power of two that brings a largest magnitude into [2^14, 2^15); 1 for 0,
+// infinities and NaN
+__device__ __forceinline__ float scale_of(float amax) {
+  return amax > 0.f && amax < INFINITY ? ldexpf(1.f, min(100, max(-100, 14 - ilogbf(amax)))) : 1.f;
+}
+
+// The scales, from the partial maxima, for a whole CTA of 256 (sc: shared); the
+// grid's first CTA leaves them in memory for the kernels after it.
+__device__ __forceinline__ void load_scales(const float* __restrict__ part, float* sc, float* __restrict__ out) {
+  static_assert(kAmax == 128, "four partials per lane");
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (warp < 3) {
+    const float4 v = reinterpret_cast<const float4*>(part + warp * kAmax)[lane];
+    const float m = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+    if (lane == 0) sc[warp] = scale_of(m);
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    out[kScX] = sc[0];
+    out[kScW] = sc[1];
+    out[kScG] = sc[2];
+    out[kUnXW] = 1.f / sc[0] / sc[1];
+    out[kUnGW] = 1.f / sc[2] / sc[1];
+    out[kUnGX] = 1.f / sc[2] / sc[0];
+  }
+}
+
+// fp32 -> two fp16 planes
+__device__ __forceinline__ void split2(float v, __half& h, __half& l) {
+  h = __float2half_rn(v);
+  l = __float2half_rn(v - __half2float(h));
+}
+
+// A warp's row: dst = src (bf16, or two planes of fp32 times f), zeros from
+// column d to lds, or everywhere where src is null.
 template <typename T>
-__device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t lds, int64_t plane, bool vec) {
+__device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t lds, int64_t plane, bool vec, float f) {
   const int lane = threadIdx.x % 32;
   if (sizeof(T) == 2 && (vec || !src)) {  // d a multiple of 8, 16-byte aligned rows
 #pragma unroll 8
@@ -311,33 +391,44 @@ __device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t
       reinterpret_cast<uint4*>(dst)[c] = src ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
     return;
   }
+  if (sizeof(T) == 4 && vec && src) {  // lds == d
+#pragma unroll 8
+    for (int c = lane; c < d / 4; c += 32) {
+      const float4 v = reinterpret_cast<const float4*>(src)[c];
+      const __half2 h0 = __floats2half2_rn(v.x * f, v.y * f), h1 = __floats2half2_rn(v.z * f, v.w * f);
+      const float2 y0 = __half22float2(h0), y1 = __half22float2(h1);
+      const __half2 l0 = __floats2half2_rn(v.x * f - y0.x, v.y * f - y0.y), l1 = __floats2half2_rn(v.z * f - y1.x, v.w * f - y1.y);
+      reinterpret_cast<uint2*>(dst)[c] = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+      reinterpret_cast<uint2*>(dst + plane)[c] =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
+    }
+    return;
+  }
+#pragma unroll 4
   for (int c = lane; c < lds; c += 32) {
     const float v = src && c < d ? to_f<T>(src[c]) : 0.f;
     if (sizeof(T) == 2) {
       dst[c] = __float2bfloat16_rn(v);
     } else {
-      bf16 a, b, e;
-      split3(v, a, b, e);
-      dst[c] = a;
-      dst[plane + c] = b;
-      dst[2 * plane + c] = e;
+      __half h, l;
+      split2(v * f, h, l);
+      reinterpret_cast<__half*>(dst)[c] = h;
+      reinterpret_cast<__half*>(dst)[plane + c] = l;
     }
   }
-}
-
-template <typename T>
-__device__ __forceinline__ bool vec_rows(const T* p, int64_t ld, int d) {
-  return ld % 8 == 0 && d % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
 // rows of a matrix, packed; one warp per row
 template <typename T>
 __global__ void __launch_bounds__(256) xent_pack(const T* __restrict__ x, int64_t ldx, int n, int d, bf16* __restrict__ xs,
-                                                 int64_t lds, int64_t plane) {
+                                                 int64_t lds, int64_t plane, const float* __restrict__ amax, int which,
+                                                 float* __restrict__ scales) {
+  __shared__ float sc[3];
   pdl_next();
   pdl_wait();
+  if (sizeof(T) == 4) load_scales(amax, sc, scales);
   const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d));
+  if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d), sizeof(T) == 4 ? sc[which] : 1.f);
 }
 
 // Before the products of a training call. Lists the tokens that count, in
@@ -348,21 +439,25 @@ __global__ void __launch_bounds__(256) xent_pack(const T* __restrict__ x, int64_
 // (a multiple of 8) and counts the targets before them for itself: reading a
 // few hundred KB from L2 again costs less than a second launch or a wait
 // (measured 56 us for one CTA's scan of 32768 targets, 12 us this way with the
-// rows packed as well). The first n_w CTAs pack w instead, 64 rows each.
+// rows packed as well). The first n_w CTAs pack w instead, 16 rows each.
 template <typename T>
 __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_t ldx, int d,
                                                  const int64_t* __restrict__ targets, int n, int64_t ignore, int vocab,
                                                  int per, int* __restrict__ idx, int* __restrict__ tgt,
                                                  float* __restrict__ lt, int* __restrict__ count, bf16* __restrict__ xs,
                                                  int64_t lds, int64_t plane, T* __restrict__ dx, const T* __restrict__ w,
-                                                 int64_t ldw, bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w) {
+                                                 int64_t ldw, bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w,
+                                                 const float* __restrict__ amax, float* __restrict__ scales) {
+  __shared__ float sc[3];
   pdl_next();
   pdl_wait();
+  if (sizeof(T) == 4) load_scales(amax, sc, scales);
+  const float fx = sizeof(T) == 4 ? sc[kScX] : 1.f;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if ((int)blockIdx.x < n_w) {
     const bool v = vec_rows(w, ldw, d);
-    for (int64_t r = (int64_t)blockIdx.x * 64 + warp; r < min(vocab, ((int)blockIdx.x + 1) * 64); r += 8)
-      pack_row<T>(w + r * ldw, d, wp + r * ldwp, ldwp, wplane, v);
+    for (int64_t r = (int64_t)blockIdx.x * 16 + warp; r < min(vocab, ((int)blockIdx.x + 1) * 16); r += 8)
+      pack_row<T>(w + r * ldw, d, wp + r * ldwp, ldwp, wplane, v, sizeof(T) == 4 ? sc[kScW] : 1.f);
     return;
   }
   __shared__ int red[2][8], pos[256];
@@ -416,11 +511,11 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
     for (int k = warp; k < min(256, r1 - c0); k += 8) {
       const int64_t row = c0 + k;
       if (pos[k] >= 0) {
-        pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec);
+        pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec, fx);
       } else if (dx) {
         for (int c = lane; c < d; c += 32) dx[row * d + c] = from_f<T>(0.f);
       }
-      if (row >= all) pack_row<T>(nullptr, d, xs + row * lds, lds, plane, vec);
+      if (row >= all) pack_row<T>(nullptr, d, xs + row * lds, lds, plane, vec, fx);
     }
   }
 }
@@ -480,7 +575,7 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
 // One CTA per row of a piece (few rows: SHARES of them, along y, each a share
 // of the columns): joins the tiles, writes the row's loss and rewrites the
 // exponentials as G = g (p - onehot), g = 1 or grad_rows (bf16 in place of fp16, or
-// fp32 -> three bf16 planes). Rows between the count and the next multiple
+// fp32 -> two fp16 planes, scaled). Rows between the count and the next multiple
 // of 64 become zeros: the third product reads them. The last CTA of the last
 // piece to finish sums the losses (thread t those of index t mod 256, then
 // in thread order: the same bits whichever CTA it is).
@@ -489,8 +584,8 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
                                                  int* __restrict__ count, int base, const int* __restrict__ idx,
                                                  const int* __restrict__ tgt, const float* __restrict__ lt,
                                                  const float* __restrict__ grad_rows, int mean, float* losses,
-                                                 void* __restrict__ p, int64_t ldp, bf16* __restrict__ planes,
-                                                 int64_t plane, float* __restrict__ loss) {
+                                                 void* __restrict__ p, int64_t ldp, __half* __restrict__ planes,
+                                                 int64_t plane, const float* __restrict__ scales, float* __restrict__ loss) {
   extern __shared__ float xent_f[];  // [n_tiles]
   __shared__ float red[8];
   __shared__ int last;
@@ -504,7 +599,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
       const uint4 z = make_uint4(0, 0, 0, 0);
       for (int64_t c = blockIdx.y * 256 + threadIdx.x; c < ldp / 8; c += 256 * SHARES) {
         if (F32) {
-          for (int k = 0; k < 3; ++k) reinterpret_cast<uint4*>(planes + k * plane + row * ldp)[c] = z;
+          for (int k = 0; k < 2; ++k) reinterpret_cast<uint4*>(planes + k * plane + row * ldp)[c] = z;
         } else {
           reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp)[c] = z;
         }
@@ -519,6 +614,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   if (threadIdx.x == 0 && blockIdx.y == 0) losses[base + row] = row_loss(lse, lt[row]);
   float g = grad_rows ? grad_rows[idx[row]] : 1.f;
   if (t < 0) g = __int_as_float(0x7fc00000);
+  if (F32) g *= scales[kScG];
   // tile factors: g 2^(m_tile - lse)
   for (int i = threadIdx.x; i < n_tiles; i += 256) {
     const float m = st[i].x;
@@ -546,20 +642,17 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = v[q] * f - (c + q == t ? g : 0.f);
     if (F32) {
-      uint32_t o[3][4];
+      uint32_t o[2][4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        bf16 x[3], y[3];
-        split3(v[2 * q], x[0], x[1], x[2]);
-        split3(v[2 * q + 1], y[0], y[1], y[2]);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const __nv_bfloat162 w2 = __halves2bfloat162(x[k], y[k]);
-          o[k][q] = *reinterpret_cast<const uint32_t*>(&w2);
-        }
+        const __half2 hi = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
+        const float2 y = __half22float2(hi);
+        const __half2 lo = __floats2half2_rn(v[2 * q] - y.x, v[2 * q + 1] - y.y);
+        o[0][q] = *reinterpret_cast<const uint32_t*>(&hi);
+        o[1][q] = *reinterpret_cast<const uint32_t*>(&lo);
       }
 #pragma unroll
-      for (int k = 0; k < 3; ++k)
+      for (int k = 0; k < 2; ++k)
         *reinterpret_cast<uint4*>(planes + k * plane + row * ldp + c) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
     } else {
       *reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp + c) =
@@ -626,12 +719,13 @@ struct Plan {
   bool f32, train, few, pack_x, pack_w;
   int elt, planes, n_tiles, piece, n_pieces, dx_splits;
   int64_t ldx, ldw, ldp, ldd;
-  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, acc, part, total;
+  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, amax, scales, acc, part, total;
 };
 
 MmArgs base_args(const Plan& q, volatile unsigned* fault) {
   MmArgs p = {};
-  p.n_terms = q.f32 ? 6 : 1;
+  p.n_terms = q.f32 ? 3 : 1;
+  p.fp16 = q.f32;
   p.pa = q.f32 ? kTermsA : 0;
   p.pb = q.f32 ? kTermsB : 0;
   p.nz = p.min_splits = 1;
@@ -655,6 +749,7 @@ MmArgs dw_args(const Plan& q, const llattn_xent_args& a, int rows, volatile unsi
   m.N = a.d;
   m.K = rows;
   m.split = 1;
+  if (q.f32) m.min_splits = cdiv(rows, kF32Chain / 2);
   return m;
 }
 
@@ -662,7 +757,7 @@ Plan make_plan(const llattn_xent_args& a) {
   Plan q;
   q.f32 = a.dtype == LLATTN_F32;
   q.elt = q.f32 ? 4 : 2;
-  q.planes = q.f32 ? 3 : 1;
+  q.planes = q.f32 ? 2 : 1;
   q.train = a.dx || a.dw;
   q.pack_x = q.f32 || q.train || !aligned_rows(a.x, a.ldx, a.tokens, 2);
   q.pack_w = q.f32 || !aligned_rows(a.w, a.ldw, a.vocab, 2);
@@ -676,9 +771,10 @@ Plan make_plan(const llattn_xent_args& a) {
   // bf16: 8192 rows), whole row tiles. fp32 also bounds the length of each
   // tensor-core sum: its additions truncate, about 2^-26 of the running sum per
   // 16 products on average (measured: dx 9.6e-6 off after 8192 products, 1e-6
-  // after 1024), so sums over V run in splits of 1024 and sums over rows in
-  // pieces of 1024, joined by rounded fp32 additions
-  const int64_t row_bytes = q.f32 ? q.ldp * 10 + 4 * q.ldd * cdiv(a.vocab, kF32Chain) : q.ldp * 2;
+  // after 1024), so sums over V run in splits of 1024 and sums over rows, which
+  // cancel less, in splits of 512 of pieces of 1024, joined by rounded fp32
+  // additions
+  const int64_t row_bytes = q.f32 ? q.ldp * 8 + 4 * q.ldd * cdiv(a.vocab, kF32Chain) : q.ldp * 2;
   int64_t piece = (int64_t)(512u << 20) / row_bytes / 256 * 256;
   piece = std::max<int64_t>(256, piece);
   if (q.f32) piece = std::min<int64_t>(piece, kF32Chain);
@@ -698,7 +794,9 @@ Plan make_plan(const llattn_xent_args& a) {
   q.count = take(8);
   q.losses = take(4 * n);
   q.p = take(q.train ? (size_t)q.piece * q.ldp * q.elt : 0);
-  q.gplanes = take(q.train && q.f32 ? 6 * (size_t)q.piece * q.ldp : 0);
+  q.gplanes = take(q.train && q.f32 ? 4 * (size_t)q.piece * q.ldp : 0);
+  q.amax = take(q.f32 ? sizeof(float) * 3 * kAmax : 0);
+  q.scales = take(q.f32 ? sizeof(float) * kScales : 0);
   q.acc = take(q.train && a.dw && q.n_pieces > 1 ? 4 * (size_t)a.vocab * q.ldd : 0);
   int64_t part = 0;
   if (a.dx) part = mm_part_floats(dx_args(q, a, q.piece, nullptr));
@@ -728,12 +826,20 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   const bool mean = a.reduction == LLATTN_XENT_MEAN;
   const int64_t xplane = (int64_t)n * q.ldx, wplane = (int64_t)V * q.ldw;
   const void* wv = q.pack_w ? wp : a.w;
+  float* amax = reinterpret_cast<float*>(ws + q.amax);
+  float* scales = q.f32 ? reinterpret_cast<float*>(ws + q.scales) : nullptr;
+  auto un = [&](int i) { return scales ? scales + i : nullptr; };
+  if (q.f32)
+    TRY(launch_pdl(xent_amax, dim3(3 * kAmax), 256, 0, 1, s, static_cast<const float*>(a.x), a.ldx, n, d, a.targets,
+                   a.ignore_index, static_cast<const float*>(a.w), a.ldw, V, a.grad_rows, amax));
   if (!q.train) {
     if (q.pack_w) {
-      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(V, 8)), 256, 0, 1, s, static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane));
+      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(V, 8)), 256, 0, 1, s, static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane,
+                     amax, (int)kScW, scales));
     }
     if (q.pack_x) {
-      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane));
+      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane,
+                     amax, (int)kScX, scales));
     }
     MmArgs p = base_args(q, fault);
     const Operand ox{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0}, ow{wv, V, d, q.ldw, q.planes, wplane, 0};
@@ -742,11 +848,11 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       p.M = V;
       p.N = n;
       std::swap(p.pa, p.pb);
-      TRY(launch_mm_sh<0>(p, ow, ox, EpiScore{stats, q.n_tiles, a.targets, lt}, s));
+      TRY(launch_mm_sh<0>(p, ow, ox, EpiScore{stats, q.n_tiles, a.targets, lt, un(kUnXW)}, s));
     } else {
       p.M = n;
       p.N = V;
-      TRY(launch_mm(p, ox, ow, EpiStats{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0}, s));
+      TRY(launch_mm(p, ox, ow, EpiStats{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0, un(kUnXW)}, s));
     }
     float* losses = a.losses ? a.losses : reinterpret_cast<float*>(ws + q.losses);
     TRY(launch_pdl(xent_losses, dim3(n), 128, 0, 1, s, stats, q.n_tiles, lt, a.targets, a.ignore_index, V, losses));
@@ -756,13 +862,13 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     return cudaSuccess;
   }
   T* dx = static_cast<T*>(a.dx);
-  const int per = std::max(8, cdiv(cdiv(n, 512), 8) * 8), n_w = q.pack_w ? cdiv(V, 64) : 0;
+  const int per = std::max(8, cdiv(cdiv(n, 512), 8) * 8), n_w = q.pack_w ? cdiv(V, 16) : 0;
   TRY(launch_pdl(xent_prep<T>, dim3(n_w + cdiv(n, per)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, d, a.targets, n, a.ignore_index, V, per,
                                                   idx, tgt, lt, count, xs, q.ldx, xplane, dx, static_cast<const T*>(a.w),
-                                                  a.ldw, wp, q.ldw, wplane, n_w));
+                                                  a.ldw, wp, q.ldw, wplane, n_w, amax, scales));
   float* losses = reinterpret_cast<float*>(ws + q.losses);
   void* pbuf = ws + q.p;
-  bf16* gpl = reinterpret_cast<bf16*>(ws + q.gplanes);
+  __half* gpl = reinterpret_cast<__half*>(ws + q.gplanes);
   float* acc = reinterpret_cast<float*>(ws + q.acc);
   float* part = reinterpret_cast<float*>(ws + q.part);  // split tiles of one product at a time
   const int64_t gplane = (int64_t)q.piece * q.ldp;
@@ -775,12 +881,12 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     p.M = rows;
     p.N = V;
     p.K = d;
-    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0};
+    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0, un(kUnXW)};
     TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
     auto rows_pass = [&](auto kernel, int shares) {
       return launch_pdl(kernel, dim3(rows, shares), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
-                        lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, c + 1 == q.n_pieces ? a.loss : nullptr);
+                        lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, scales, c + 1 == q.n_pieces ? a.loss : nullptr);
     };
     const bool share = rows <= 2 * sm_count() && V >= 4096;  // (129 rows of 32000: 12.7 -> 9.1 us)
     TRY(share ? rows_pass(xent_rows<sizeof(T) == 4, 4>, 4) : rows_pass(xent_rows<sizeof(T) == 4, 1>, 1));
@@ -797,6 +903,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.vec = aligned_rows(dx, d, 2, q.elt);
       eo.idx = idx + base;
       eo.count = mean ? count : nullptr;
+      eo.un = un(kUnGW);
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
                     s));
     }
@@ -815,6 +922,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.acc = c && last ? acc : nullptr;
       eo.ldacc = q.ldd;
       eo.count = last && mean ? count : nullptr;
+      eo.un = last ? un(kUnGX) : nullptr;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
                     eo, s));
     }
@@ -828,8 +936,8 @@ size_t workspace_bytes(const llattn_xent_args& a) { return make_plan(a).total; }
 
 int launches(const llattn_xent_args& a) {
   const Plan q = make_plan(a);
-  if (!q.train) return q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
-  return 1 + q.n_pieces * (2 + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
+  if (!q.train) return q.f32 + q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
+  return q.f32 + 1 + q.n_pieces * (2 + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
                            (a.dw ? 1 + joins(dw_args(q, a, q.piece, nullptr)) : 0));
 }
 

@@ -6,8 +6,8 @@ from the arithmetic:
   * bf16 gradients: G is rounded once to 8 bits (relative error at most 2^-9,
     independent per element) and the result once more: 2 * 2^-9, and a quarter
     on top for what an unlucky sum adds: 5e-3.
-  * fp32 gradients: three bf16 planes hold 24 bits, sums of up to 1024 products
-    on the tensor cores: 1e-5.
+  * fp32 gradients: operands of at least 22 bits, sums of up to 1024 products on
+    the tensor cores: 1e-5.
   * losses: fp32 sums of d products of magnitude |x||w|: 1e-5 of the losses'
     norm, plus 1e-5 absolute where they are near 0.
   * newton_schulz: one rounding to bf16 at the end (2^-9) and what the fp16
