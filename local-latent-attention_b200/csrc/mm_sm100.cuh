@@ -83,11 +83,18 @@ struct MmArgs {
   int M, N, K;
   int a_mn, b_mn;
   int nz;                   // batch elements (tensor-map z)
-  // Split K of the tiles that do not fill a wave (and, min_splits > 1, of
-  // every tile into at least that many ranges): each range's sums go to part
+  // Split K of the tiles that do not fill a wave: each range's sums go to part
   // (fp32, one BM x BN block per range) and mm_join adds them up. 0: no split.
-  int split, min_splits;
+  int split;
   float* part;
+  // The tensor cores' additions drop what lies below the running sum's last
+  // bits: a sum that grows evenly comes out up to 2^-26 per product of 16 short
+  // (measured for bf16 operands, three times that for fp32's planes), always
+  // towards zero. chain > 0 bounds each such sum to that many K = 64 steps (of
+  // the last term's; the terms before it, smaller by 2^-8 and less, make one
+  // more): the epilogue warps add it to the tile's fp32 sum in TMEM, rounded to
+  // nearest, while the next one is under way (Epi::kChain; not shape 3).
+  int chain;
   int sym;                  // C symmetric: tiles with n <= m only (square tiles)
   int fp16;                 // operands fp16 instead of bf16
   // products over planes: operand z coordinates (pa, pb) of n_terms passes
@@ -224,7 +231,7 @@ struct MmShape {
   static constexpr int A = 0, B = A + ST * AB, STAGE = B + ST * NH * BB, BAR = STAGE + EW * STG;
   static constexpr int ACC = NH == 2 ? 1 : 2;      // accumulators in TMEM
   static constexpr int BLOCK = 205 * (BM * BN / 1024) / 64;  // mm_plan's `block`
-  static constexpr int TCOLS = NH == 2 ? 512 : 2 * BN;
+  static constexpr int TCOLS = BN < 256 ? 4 * BN : 512;  // (and with chains a sum, after the accumulators)
   static constexpr int BYTES = BAR + 256;
   static constexpr int SMEM = BYTES + 1024;  // + alignment
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -244,15 +251,15 @@ struct MmPlan {
 // by the time of its ceil(tail s / units) rounds in steps: the range's own,
 // 6 for its epilogue, and the partial sums' way through memory (a 256 x 256
 // block written and read takes the memory 0.2 of a step: `block`, in 1/1024).
-__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int min_splits, int block) {
+__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int block) {
   MmPlan r{total, total, 1, total};
   if (!split || total == 0) return r;
-  const int full = min_splits > 1 ? 0 : total / units * units, tail = total - full;
+  const int full = total / units * units, tail = total - full;
   if (tail == 0) return r;
-  int best = min_splits;
+  int best = 1;
   int64_t cost = INT64_MAX;  // (integers: the product's and the join's kernel have to agree)
-  for (int s = min_splits; s <= 32 || s == min_splits; ++s) {
-    if (s > min_splits && (ksteps < 8 * s || (int64_t)tail * s > 4 * (int64_t)units)) break;
+  for (int s = 1; s <= 32; ++s) {
+    if (s > 1 && (ksteps < 8 * s || (int64_t)tail * s > 4 * (int64_t)units)) break;
     const int64_t c = 1024 * (int64_t)cdiv(tail * s, units) * (cdiv(ksteps, s) + 6) + (s > 1 ? (int64_t)block * tail * s : 0);
     if (c < cost) {
       cost = c;
@@ -489,6 +496,37 @@ __device__ __forceinline__ float2 bf16_pair(const uint4 (&u)[4], int i) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// sum (+)= an accumulator's CW columns of this thread's row
+template <int CW>
+__device__ __forceinline__ void drain(uint32_t acc, uint32_t sum, bool add) {
+#pragma unroll 1
+  for (int cc = 0; cc < CW; cc += 32) {
+    uint32_t a[32], b[32];
+    tmem_ld32(acc + cc, a);
+    if (add) tmem_ld32(sum + cc, b);
+    tmem_ld_wait();
+    if (add) {
+#pragma unroll
+      for (int q = 0; q < 32; ++q) a[q] = __float_as_uint(__uint_as_float(a[q]) + __uint_as_float(b[q]));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t c[16];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) c[q] = a[16 * h + q];
+      tmem_st16(sum + cc + 16 * h, c);
+    }
+  }
+  tmem_st_wait();
+}
+
+// The tensor-core sums of a tile of `steps` K = 64 steps over n_terms terms:
+// the one that starts at step i ends before step chain_end.
+__device__ __forceinline__ int chain_end(int i, int steps, int n_terms, int chain) {
+  const int minor = n_terms > 1 ? steps / n_terms * (n_terms - 1) : 0;
+  return i < minor ? minor : min(steps, i + chain);
+}
+
 // one range's sums of a tile: its fp32 block of part, [BM][BN]
 template <int SH>
 __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, const MmTile& w, int row, int col, int M,
@@ -512,11 +550,13 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
 //                                          bool zero, uint8_t* buf) const
 //   static constexpr bool kNarrow, kWide: shapes 0 and 4 (CW = 32 and 64, else 128), and 3, may be used
+//   static constexpr bool kChain: MmArgs::chain may be set
 // tile is called by every thread of an epilogue warp (all 32 lanes,
 // converged) for its row and CW columns [col0, col0 + CW); taddr: TMEM address of the warp's
 // lanes and columns; zero: the K range is empty, the accumulator holds
 // nothing; buf: the warp's staging block.
-template <int SH, typename Epi>
+// CHAIN: sums are bounded by MmArgs::chain.
+template <int SH, bool CHAIN, typename Epi>
 __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
               const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
@@ -555,7 +595,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   pdl_wait();
   if (threadIdx.x == 0) {
     const MmGrid<SH> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
-    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits, S::BLOCK);
+    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
   }
   tc_fence_before();
   __syncthreads();
@@ -567,6 +607,9 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   const int K = cut_rows(p.K, p.k_dev, p.dev_base);
   const MmGrid<SH> grid(p, M);
   const MmPlan pl = *plan;
+  // one accumulator at a time: both halves of shape 3, or, with chains, where
+  // the sum takes the place of the second
+  constexpr bool one = S::ACC == 1 || (CHAIN && SH == 2);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -638,17 +681,17 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       const uint32_t a_lbo = p.a_mn ? S::AB / 2 : 16, b_lbo = p.b_mn ? S::BB / 2 : 16;
       const uint64_t da0 = desc_sw128(smem_u32(smem + S::A), a_lbo, 1024), db0 = desc_sw128(smem_u32(smem + S::B), b_lbo, 1024);
       const uint32_t td = __shfl_sync(0xffffffffu, tmem, 0);
-      int k = 0, stage = 0, phase = 0;
+      int k = 0, stage = 0, phase = 0;  // k: accumulators filled so far
       bool ok = true;
-      for (int t = unit; ok && t < pl.items; t += n_units, ++k) {
+      for (int t = unit; ok && t < pl.items; t += n_units) {
         const MmItem x = mm_item(pl, t, K);
-        const int buf = S::ACC == 2 ? k & 1 : 0, steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
+        const int steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
         auto wait = [&](uint64_t* bar, int parity) {
           return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_mm_fault));
         };
         // 4 MMAs of a stage's K = 64 into accumulator (half) h
-        auto issue = [&](int st, int h, int first) {
-          const uint32_t d = td + S::HN * (S::ACC == 2 ? buf : h);
+        auto issue = [&](int st, int b, int h, int first) {
+          const uint32_t d = td + S::HN * b;
           const uint64_t da = da0 + st * (S::AB >> 4), db = db0 + (st * S::NH + h) * (S::BB >> 4);
           mma_f16<CG>(d, da, db, id, first ? 0u : 1u);
           mma_f16<CG>(d, da + a_step, db + b_step, id, 1u);
@@ -660,11 +703,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
           phase ^= stage == 0;
         };
         int i = 0;
-        if (S::NH == 1) {
-          // the epilogue has read this accumulator's previous tile (k - 2)
-          if (k >= 2 && !(ok = wait(&acc_empty[buf], ((k >> 1) - 1) & 1))) break;
-          tc_fence_after();
-        } else {
+        if (S::NH == 2) {
           // the first half may start while the epilogue reads the second:
           // as many stages as the ring holds, whose second halves follow
           if (k >= 1 && !(ok = wait(&acc_empty[0], (k - 1) & 1))) break;
@@ -672,7 +711,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
           const int ahead = min(steps, ST), stage0 = stage;
           for (; i < ahead; ++i) {
             if (!(ok = wait(&full[stage], phase))) break;
-            if (elect_one()) issue(stage, 0, i == 0);
+            if (elect_one()) issue(stage, 0, 0, i == 0);
             __syncwarp();
             advance();
           }
@@ -680,26 +719,36 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
           tc_fence_after();
           for (int j = 0, st = stage0; j < ahead; ++j) {
             if (elect_one()) {
-              issue(st, 1, j == 0);
+              issue(st, 1, 1, j == 0);
               commit<CG>(&empty[st]);
             }
             __syncwarp();
             st = st + 1 == ST ? 0 : st + 1;
           }
         }
-        for (; i < steps; ++i) {
-          if (!(ok = wait(&full[stage], phase))) break;
-          if (elect_one()) {
-            issue(stage, 0, i == 0);
-            if (S::NH == 2) issue(stage, 1, 0);
-            commit<CG>(&empty[stage]);
+        do {
+          const int end = CHAIN ? chain_end(i, steps, p.n_terms, p.chain) : steps, begin = i;
+          const int buf = one ? 0 : k & 1, use = one ? k : k >> 1;
+          if (S::NH == 1) {
+            // the epilogue has read what this accumulator held before
+            if (use && !(ok = wait(&acc_empty[buf], (use - 1) & 1))) break;
+            tc_fence_after();
           }
+          for (; i < end; ++i) {
+            if (!(ok = wait(&full[stage], phase))) break;
+            if (elect_one()) {
+              issue(stage, S::NH == 1 ? buf : 0, 0, S::NH == 1 && i == begin);
+              if (S::NH == 2) issue(stage, 1, 1, 0);
+              commit<CG>(&empty[stage]);
+            }
+            __syncwarp();
+            advance();
+          }
+          if (!ok) break;
+          if (elect_one()) commit<CG>(&acc_full[buf]);
           __syncwarp();
-          advance();
-        }
-        if (!ok) break;
-        if (elect_one()) commit<CG>(&acc_full[buf]);
-        __syncwarp();
+          ++k;
+        } while (CHAIN && i < steps);
       }
       if (!ok && lane == 0) mm_raise(p, 2u, abort);
     }
@@ -707,31 +756,55 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns CW half..
     int k = 0;
     bool ok = true;
-    for (int t = unit; t < pl.items; t += n_units, ++k) {
-      const int buf = S::ACC == 2 ? k & 1 : 0;
+    auto release = [&](int b) {  // accumulator (half) b may be filled again
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 1)
+          mbar_arrive(&acc_empty[b]);
+        else
+          mbar_arrive_leader(&acc_empty[b]);
+      }
+    };
+    for (int t = unit; ok && t < pl.items; t += n_units) {
       const MmItem x = mm_item(pl, t, K);
       const MmTile w = grid.at(p, x.tile);
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (S::ACC == 2 ? k >> 1 : k) & 1, abort, &g_mm_fault));
-      if (!ok) break;
-      tc_fence_after();
       uint8_t* stage = smem + S::STAGE + (warp - 2) * S::STG;
       const int row = rank * 128 + 32 * quad + lane;
-#pragma unroll
-      for (int h = 0; h < S::NH; ++h) {
-        const int col = S::HN * h + S::CW * half;
-        const uint32_t ta = tmem + S::HN * (S::ACC == 2 ? buf : h) + S::CW * half + ((uint32_t)(32 * quad) << 16);
+      const uint32_t t0 = tmem + S::CW * half + ((uint32_t)(32 * quad) << 16);
+      auto out = [&](int col, uint32_t ta) {
         if (x.block < 0)
           epi.template tile<S::CW>(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage);
         else
           store_part<SH>(p, x, w, row, col, M, ta, stage);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {  // this accumulator (half) may take its next tile
-          uint64_t* bar = &acc_empty[S::ACC == 2 ? buf : h];
-          if (CG == 1)
-            mbar_arrive(bar);
-          else
-            mbar_arrive_leader(bar);
+      };
+      auto wait = [&] {
+        const int buf = one ? 0 : k & 1, use = one ? k : k >> 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], use & 1, abort, &g_mm_fault));
+        tc_fence_after();
+        ++k;
+        return buf;
+      };
+      if constexpr (CHAIN) {
+        const int steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
+        const uint32_t sum = t0 + (SH == 2 ? 1 : 2) * S::HN;
+        int i = 0;
+        do {
+          const int buf = wait();
+          if (!ok) break;
+          if (steps) drain<S::CW>(t0 + S::HN * buf, sum, i > 0);
+          release(buf);
+          i = chain_end(i, steps, p.n_terms, p.chain);
+        } while (i < steps);
+        if (ok) out(S::CW * half, sum);
+      } else {
+        const int buf = wait();
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < S::NH; ++h) {
+          const int b = S::NH == 2 ? h : buf;
+          out(S::HN * h + S::CW * half, t0 + S::HN * b);
+          release(b);
         }
       }
     }
@@ -760,7 +833,7 @@ __global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p,
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const MmGrid<SH> grid(p, M);
   if (threadIdx.x == 0)
-    plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.min_splits, S::BLOCK);
+    plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
   __syncthreads();
   const MmPlan pl = plan;
   const int tile = pl.full + blockIdx.x;
@@ -804,7 +877,7 @@ double mm_time(const MmArgs& p) {
   constexpr double gap = SH == 3 ? 3.0 : 0.5, tail = SH == 3 ? 8.0 : SH == 2 ? 5.5 : SH == 1 ? 4.3 : SH == 4 ? 2.3 : 1.2;
   const MmGrid<SH> g(p, p.M);
   const int units = mm_units(SH), ks = cdiv(p.K, 64);
-  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.min_splits, MmShape<SH>::BLOCK);
+  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, MmShape<SH>::BLOCK);
   double t = (pl.full / units + (pl.full % units ? 1 : 0)) * (ks * p.n_terms * step + gap);
   const int split = pl.items - pl.full;
   if (split) t += cdiv(split, units) * (cdiv(ks, pl.s) * p.n_terms * step + gap) + split * step * MmShape<SH>::BLOCK / 1024;
@@ -814,16 +887,12 @@ double mm_time(const MmArgs& p) {
 // fp32 elements of MmArgs::part for a product of at most these sizes
 inline int64_t mm_part_floats(const MmArgs& p) {
   if (!p.split) return 0;
-  // the caps of mm_plan: 4 waves of ranges, or min_splits of every tile
-  auto floats = [&](int sh, int64_t tiles, int64_t block) {
-    return std::max<int64_t>(4 * mm_units(sh), p.min_splits > 1 ? tiles * p.nz * p.min_splits : 0) * block;
-  };
-  return std::max({floats(3, MmGrid<3>(p, p.M).per_z, 256 * 512), floats(2, MmGrid<2>(p, p.M).per_z, 256 * 256), floats(1, MmGrid<1>(p, p.M).per_z, 128 * 128),
-                   floats(4, MmGrid<4>(p, p.M).per_z, 128 * 64), floats(0, MmGrid<0>(p, p.M).per_z, 128 * 32)});
+  // mm_plan's cap: 4 waves of ranges
+  return 4 * std::max({mm_units(3) * 256 * 512, mm_units(2) * 256 * 256, mm_units(1) * 128 * 128});
 }
 
 // whether mm_plan may split anything, whatever the device-side counts
-inline bool joins(const MmArgs& p) { return p.split && (p.min_splits > 1 || cdiv(p.K, 64) >= 16); }
+inline bool joins(const MmArgs& p) { return p.split && cdiv(p.K, 64) >= 16; }
 
 template <int SH, typename Epi>
 cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t s, decltype(&Epi::quad)) {
@@ -831,7 +900,7 @@ cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t
   const MmGrid<SH> g(p, p.M);
   const int total = g.per_z * p.nz;
   // the device may have fewer tiles than the host's sizes say, never more
-  const int tail = p.min_splits > 1 ? total : std::min(total, units - 1);
+  const int tail = std::min(total, units - 1);
   if (tail < 1) return cudaSuccess;
   return launch_pdl(mm_join<SH, Epi>, dim3(tail, S::BM / 8), 256, 0, 1, s, p, epi, units);
 }
@@ -840,20 +909,23 @@ cudaError_t launch_join(const MmArgs&, const Epi&, int, cudaStream_t, ...) {
   return cudaErrorInvalidValue;  // an epilogue without quad() cannot be split
 }
 
-template <int SH, typename Epi>
+template <int SH, bool CHAIN = false, typename Epi>
 cudaError_t launch_mm_sh(const MmArgs& p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
+  if constexpr (Epi::kChain && !CHAIN && SH != 3) {
+    if (p.chain) return launch_mm_sh<SH, true>(p, a, b, epi, s);
+  }
   using S = MmShape<SH>;
   CUtensorMap ta, tb;
   if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
       !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : S::BR))
     return cudaErrorInvalidValue;
-  cudaError_t e = set_smem_once(mm_kernel<SH, Epi>, S::SMEM);
+  cudaError_t e = set_smem_once(mm_kernel<SH, CHAIN, Epi>, S::SMEM);
   if (e != cudaSuccess) return e;
   const int64_t m = cdiv(p.M, S::BM), n = cdiv(p.N, S::BN);
   const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
   const int units = p.split ? mm_units(SH) : (int)std::min<int64_t>(tiles, mm_units(SH));
-  e = launch_pdl(mm_kernel<SH, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, p, epi);
+  e = launch_pdl(mm_kernel<SH, CHAIN, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<SH, Epi>(p, epi, units, s, nullptr);
 }
@@ -862,7 +934,6 @@ template <typename Epi>
 cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
   p.a_mn = a.mn;
   p.b_mn = b.mn;
-  if (p.min_splits < 1) p.min_splits = 1;
   if (p.nz < 1) p.nz = 1;
   if (p.n_terms < 1) p.n_terms = 1;
   if (p.M < 1 || p.N < 1 || p.K < 1 || (p.split && !p.part)) return cudaErrorInvalidValue;
@@ -875,7 +946,7 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
       return t0 <= t4 ? launch_mm_sh<0>(q, a, b, epi, s) : launch_mm_sh<4>(q, a, b, epi, s);
   }
   if constexpr (Epi::kWide) {
-    if (mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s);
+    if (!p.chain && mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s);
   }
   return t2 <= t1 ? launch_mm_sh<2>(p, a, b, epi, s) : launch_mm_sh<1>(p, a, b, epi, s);
 }

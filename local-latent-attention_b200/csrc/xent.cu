@@ -46,9 +46,23 @@ using namespace mm;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 128;  // columns per (max, sum) statistic
-constexpr int kF32Chain = 1024;  // products per tensor-core sum of the fp32 gradients
 
-constexpr uint32_t kTermsA = 0x001u, kTermsB = 0x010u;  // planes (1,0) (0,1) (0,0)
+// planes (1,0) (0,1) (0,0) of fp32's products; (1,.) (0,.) of G's two in bf16
+constexpr uint32_t kTermsA = 0x001u, kTermsB = 0x010u, kFineA = 0x01u;
+
+// Calls of few tokens have little to average an error over and time to spare: up
+// to kFine tokens keep G in two bf16 planes (one plane's rounding of p - 1 is an
+// error of the whole row, up to 1.5 times the output's own rounding for a
+// single token), and their tensor-core sums are short chains (MmArgs::chain): of
+// 4 K = 64 steps for bf16 logits (the loss of 1 token at d = 2048: 2e-6 off
+// without chains, 4e-7 with; one token's time is the same, 129 tokens of V = 32000
+// would take 150 instead of 143 us), of 2 for fp32's three products. fp32's sums
+// always run in chains (d = 2048, 300 tokens: gradients 2.4e-6 off at 1024
+// products a sum, 7e-7 at 512), bf16 logits where they are longer than kChain
+// steps (losses of 1024 tokens, d = 2048: 1.0e-6 off in one sum, 5e-7 in two;
+// d = 1536: 7.7e-7 in one, and two would take 148 instead of 142 us for 2048
+// tokens).
+constexpr int kFine = 64, kFineChain = 4, kFineF32Chain = 2, kF32Chain = 8, kChain = 24;
 
 // fp32's powers of two: of x, w, G, and the inverses that undo them in x w^T,
 // G w and G^T x
@@ -58,7 +72,7 @@ constexpr int kAmax = 128;  // partial maxima each of x, w and the rows' gradien
 // ---- first product: statistics and exponentials ----------------------------
 
 struct EpiStats {
-  static constexpr bool kNarrow = false, kWide = false;  // wide: sums over d are short, its long epilogue shows (757 us for 620)
+  static constexpr bool kNarrow = false, kWide = false, kChain = true;  // wide: sums over d are short, its long epilogue shows (757 us for 620)
   float2* stats;       // [rows][n_tiles]: (max, sum of exp(l - max))
   int n_tiles;
   const int* tgt;      // [rows] target of row (dev_base already added); < 0: none
@@ -142,7 +156,7 @@ struct EpiStats {
 constexpr int kFew = 32;
 
 struct EpiScore {
-  static constexpr bool kNarrow = true, kWide = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = true;
   float2* stats;  // [tokens][n_tiles]
   int n_tiles;
   const int64_t* targets;
@@ -175,7 +189,7 @@ struct EpiScore {
 // ---- second and third product: rows out --------------------------------------
 
 struct EpiOut {
-  static constexpr bool kNarrow = true, kWide = true;
+  static constexpr bool kNarrow = true, kWide = true, kChain = true;
   void* out;
   int64_t ldo;
   int out_bf16;
@@ -572,20 +586,24 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
   if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
 }
 
+// What xent_rows leaves: bf16 in place of the fp16 exponentials, or two planes
+// hi + lo, apart from fp32 exponentials: bf16, or fp16 of G times its scale
+enum class GKind { kInPlace, kBf16s, kHalves };
+
 // One CTA per row of a piece (few rows: SHARES of them, along y, each a share
 // of the columns): joins the tiles, writes the row's loss and rewrites the
-// exponentials as G = g (p - onehot), g = 1 or grad_rows (bf16 in place of fp16, or
-// fp32 -> two fp16 planes, scaled). Rows between the count and the next multiple
+// exponentials as G = g (p - onehot), g = 1 or grad_rows. Rows between the count and the next multiple
 // of 64 become zeros: the third product reads them. The last CTA of the last
 // piece to finish sums the losses (thread t those of index t mod 256, then
 // in thread order: the same bits whichever CTA it is).
-template <bool F32, int SHARES>
+template <GKind KIND, int SHARES>
 __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stats, int n_tiles, int rows, int vocab,
                                                  int* __restrict__ count, int base, const int* __restrict__ idx,
                                                  const int* __restrict__ tgt, const float* __restrict__ lt,
                                                  const float* __restrict__ grad_rows, int mean, float* losses,
-                                                 void* __restrict__ p, int64_t ldp, __half* __restrict__ planes,
+                                                 void* __restrict__ p, int64_t ldp, void* __restrict__ planes,
                                                  int64_t plane, const float* __restrict__ scales, float* __restrict__ loss) {
+  constexpr bool SPLIT = KIND != GKind::kInPlace;
   extern __shared__ float xent_f[];  // [n_tiles]
   __shared__ float red[8];
   __shared__ int last;
@@ -598,8 +616,8 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
     if (row < cdiv(n, 64) * 64) {
       const uint4 z = make_uint4(0, 0, 0, 0);
       for (int64_t c = blockIdx.y * 256 + threadIdx.x; c < ldp / 8; c += 256 * SHARES) {
-        if (F32) {
-          for (int k = 0; k < 2; ++k) reinterpret_cast<uint4*>(planes + k * plane + row * ldp)[c] = z;
+        if (SPLIT) {
+          for (int k = 0; k < 2; ++k) reinterpret_cast<uint4*>(static_cast<bf16*>(planes) + k * plane + row * ldp)[c] = z;
         } else {
           reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp)[c] = z;
         }
@@ -614,17 +632,17 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   if (threadIdx.x == 0 && blockIdx.y == 0) losses[base + row] = row_loss(lse, lt[row]);
   float g = grad_rows ? grad_rows[idx[row]] : 1.f;
   if (t < 0) g = __int_as_float(0x7fc00000);
-  if (F32) g *= scales[kScG];
+  if (KIND == GKind::kHalves) g *= scales[kScG];
   // tile factors: g 2^(m_tile - lse)
   for (int i = threadIdx.x; i < n_tiles; i += 256) {
     const float m = st[i].x;
-    xent_f[i] = m == -INFINITY ? 0.f : g * exp2f((m - lse.x) * kLog2e - lse.y) * (F32 ? 1.f : 0x1p-15f);
+    xent_f[i] = m == -INFINITY ? 0.f : g * exp2f((m - lse.x) * kLog2e - lse.y) * (SPLIT ? 1.f : 0x1p-15f);
   }
   __syncthreads();
   for (int c = (blockIdx.y * 256 + threadIdx.x) * 8; c < vocab; c += 256 * 8 * SHARES) {
     const float f = xent_f[c / kTile];
     float v[8];
-    if (F32) {
+    if (SPLIT) {
       const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p) + row * ldp + c);
       const float4 a = src[0], b = src[1];
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -641,19 +659,23 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = v[q] * f - (c + q == t ? g : 0.f);
-    if (F32) {
+    if (SPLIT) {
       uint32_t o[2][4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const __half2 hi = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
-        const float2 y = __half22float2(hi);
-        const __half2 lo = __floats2half2_rn(v[2 * q] - y.x, v[2 * q + 1] - y.y);
-        o[0][q] = *reinterpret_cast<const uint32_t*>(&hi);
-        o[1][q] = *reinterpret_cast<const uint32_t*>(&lo);
+        const float a = v[2 * q], b = v[2 * q + 1];
+        if (KIND == GKind::kHalves) {
+          o[0][q] = pack_half(a, b);
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&o[0][q]));
+          o[1][q] = pack_half(a - y.x, b - y.y);
+        } else {
+          o[0][q] = pack_bf16(a, b);
+          o[1][q] = pack_bf16(a - __uint_as_float(o[0][q] << 16), b - __uint_as_float(o[0][q] & 0xffff0000u));
+        }
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        *reinterpret_cast<uint4*>(planes + k * plane + row * ldp + c) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+        *reinterpret_cast<uint4*>(static_cast<bf16*>(planes) + k * plane + row * ldp + c) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
     } else {
       *reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp + c) =
           make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
@@ -717,9 +739,9 @@ bool aligned_rows(const void* p, int64_t ld, int64_t rows, int elt) {
 
 struct Plan {
   bool f32, train, few, pack_x, pack_w;
-  int elt, planes, n_tiles, piece, n_pieces, dx_splits;
+  int elt, planes, gplanes, n_tiles, piece, n_pieces;
   int64_t ldx, ldw, ldp, ldd;
-  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, gplanes, amax, scales, acc, part, total;
+  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, g, amax, scales, acc, part, total;
 };
 
 MmArgs base_args(const Plan& q, volatile unsigned* fault) {
@@ -728,29 +750,43 @@ MmArgs base_args(const Plan& q, volatile unsigned* fault) {
   p.fp16 = q.f32;
   p.pa = q.f32 ? kTermsA : 0;
   p.pb = q.f32 ? kTermsB : 0;
-  p.nz = p.min_splits = 1;
+  p.nz = 1;
   p.fault_host = fault;
   return p;
 }
 
 // dx = G w and dw = G^T x of a piece
-MmArgs dx_args(const Plan& q, const llattn_xent_args& a, int rows, volatile unsigned* fault) {
+MmArgs grad_args(const Plan& q, const llattn_xent_args& a, volatile unsigned* fault) {
   MmArgs m = base_args(q, fault);
+  if (q.f32) {
+    m.chain = a.tokens <= kFine ? kFineF32Chain : kF32Chain;
+  } else if (q.gplanes == 2) {
+    m.n_terms = 2;
+    m.pa = kFineA;
+  }
+  return m;
+}
+MmArgs dx_args(const Plan& q, const llattn_xent_args& a, int rows, volatile unsigned* fault) {
+  MmArgs m = grad_args(q, a, fault);
   m.M = rows;
   m.N = a.d;
   m.K = a.vocab;
   m.split = 1;
-  m.min_splits = q.dx_splits;
   return m;
 }
 MmArgs dw_args(const Plan& q, const llattn_xent_args& a, int rows, volatile unsigned* fault) {
-  MmArgs m = base_args(q, fault);
+  MmArgs m = grad_args(q, a, fault);
   m.M = a.vocab;
   m.N = a.d;
   m.K = rows;
   m.split = 1;
-  if (q.f32) m.min_splits = cdiv(rows, kF32Chain / 2);
   return m;
+}
+
+int logits_chain(const Plan& q, const llattn_xent_args& a) {
+  const int steps = cdiv(a.d, 64);
+  if (q.f32) return a.tokens <= kFine ? kFineF32Chain : kF32Chain;
+  return a.tokens <= kFine ? kFineChain : steps > kChain ? cdiv(steps, cdiv(steps, kChain)) : 0;
 }
 
 Plan make_plan(const llattn_xent_args& a) {
@@ -759,6 +795,7 @@ Plan make_plan(const llattn_xent_args& a) {
   q.elt = q.f32 ? 4 : 2;
   q.planes = q.f32 ? 2 : 1;
   q.train = a.dx || a.dw;
+  q.gplanes = q.f32 || a.tokens <= kFine ? 2 : 1;
   q.pack_x = q.f32 || q.train || !aligned_rows(a.x, a.ldx, a.tokens, 2);
   q.pack_w = q.f32 || !aligned_rows(a.w, a.ldw, a.vocab, 2);
   q.ldx = q.pack_x ? up8(a.d) : (a.tokens == 1 ? up8(a.d) : a.ldx);
@@ -768,20 +805,12 @@ Plan make_plan(const llattn_xent_args& a) {
   q.few = !q.train && a.tokens <= kFew;
   q.n_tiles = cdiv(a.vocab, q.few ? 32 : kTile);
   // rows of exponentials held at a time: half a GiB of them (V = 32000 in
-  // bf16: 8192 rows), whole row tiles. fp32 also bounds the length of each
-  // tensor-core sum: its additions truncate, about 2^-26 of the running sum per
-  // 16 products on average (measured: dx 9.6e-6 off after 8192 products, 1e-6
-  // after 1024), so sums over V run in splits of 1024 and sums over rows, which
-  // cancel less, in splits of 512 of pieces of 1024, joined by rounded fp32
-  // additions
-  const int64_t row_bytes = q.f32 ? q.ldp * 8 + 4 * q.ldd * cdiv(a.vocab, kF32Chain) : q.ldp * 2;
-  int64_t piece = (int64_t)(512u << 20) / row_bytes / 256 * 256;
-  piece = std::max<int64_t>(256, piece);
-  if (q.f32) piece = std::min<int64_t>(piece, kF32Chain);
+  // bf16: 8192 rows), whole row tiles
+  const int64_t row_bytes = q.gplanes == 2 ? q.ldp * 8 : q.ldp * 2;
+  const int64_t piece = std::max<int64_t>(256, (int64_t)(512u << 20) / row_bytes / 256 * 256);
   q.piece = (int)std::min<int64_t>(piece, a.tokens);
   if (!q.train) q.piece = a.tokens;
   q.n_pieces = cdiv(a.tokens, q.piece);
-  q.dx_splits = q.f32 ? cdiv(a.vocab, kF32Chain) : 1;
   size_t off = 0;
   auto take = [&](size_t b) { size_t o = off; off += up256(b); return o; };
   const size_t n = a.tokens;
@@ -793,8 +822,8 @@ Plan make_plan(const llattn_xent_args& a) {
   q.tgt = take(q.train ? 4 * n : 0);
   q.count = take(8);
   q.losses = take(4 * n);
-  q.p = take(q.train ? (size_t)q.piece * q.ldp * q.elt : 0);
-  q.gplanes = take(q.train && q.f32 ? 4 * (size_t)q.piece * q.ldp : 0);
+  q.p = take(q.train ? (size_t)q.piece * q.ldp * 2 * q.gplanes : 0);
+  q.g = take(q.train && q.gplanes == 2 ? 4 * (size_t)q.piece * q.ldp : 0);
   q.amax = take(q.f32 ? sizeof(float) * 3 * kAmax : 0);
   q.scales = take(q.f32 ? sizeof(float) * kScales : 0);
   q.acc = take(q.train && a.dw && q.n_pieces > 1 ? 4 * (size_t)a.vocab * q.ldd : 0);
@@ -844,6 +873,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     MmArgs p = base_args(q, fault);
     const Operand ox{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0}, ow{wv, V, d, q.ldw, q.planes, wplane, 0};
     p.K = d;
+    p.chain = logits_chain(q, a);
     if (q.few) {
       p.M = V;
       p.N = n;
@@ -868,7 +898,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
                                                   a.ldw, wp, q.ldw, wplane, n_w, amax, scales));
   float* losses = reinterpret_cast<float*>(ws + q.losses);
   void* pbuf = ws + q.p;
-  __half* gpl = reinterpret_cast<__half*>(ws + q.gplanes);
+  void* gpl = ws + q.g;
   float* acc = reinterpret_cast<float*>(ws + q.acc);
   float* part = reinterpret_cast<float*>(ws + q.part);  // split tiles of one product at a time
   const int64_t gplane = (int64_t)q.piece * q.ldp;
@@ -881,7 +911,8 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     p.M = rows;
     p.N = V;
     p.K = d;
-    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.f32 ? 1 : 0, un(kUnXW)};
+    p.chain = logits_chain(q, a);
+    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.gplanes == 2, un(kUnXW)};
     TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
     auto rows_pass = [&](auto kernel, int shares) {
@@ -889,8 +920,19 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
                         lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, scales, c + 1 == q.n_pieces ? a.loss : nullptr);
     };
     const bool share = rows <= 2 * sm_count() && V >= 4096;  // (129 rows of 32000: 12.7 -> 9.1 us)
-    TRY(share ? rows_pass(xent_rows<sizeof(T) == 4, 4>, 4) : rows_pass(xent_rows<sizeof(T) == 4, 1>, 1));
-    const void* g = q.f32 ? (const void*)gpl : pbuf;
+    auto rows_as = [&](auto kind) {
+      constexpr GKind kG = decltype(kind)::value;
+      return share ? rows_pass(xent_rows<kG, 4>, 4) : rows_pass(xent_rows<kG, 1>, 1);
+    };
+    using std::integral_constant;
+    if constexpr (sizeof(T) == 4) {
+      TRY(rows_as(integral_constant<GKind, GKind::kHalves>{}));
+    } else if (q.gplanes == 2) {
+      TRY(rows_as(integral_constant<GKind, GKind::kBf16s>{}));
+    } else {
+      TRY(rows_as(integral_constant<GKind, GKind::kInPlace>{}));
+    }
+    const void* g = q.gplanes == 2 ? gpl : pbuf;
     if (dx) {
       MmArgs m = dx_args(q, a, rows, fault);
       m.m_dev = count;
@@ -904,7 +946,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.idx = idx + base;
       eo.count = mean ? count : nullptr;
       eo.un = un(kUnGW);
-      TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
+      TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.gplanes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
                     s));
     }
     if (a.dw) {
@@ -923,7 +965,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.ldacc = q.ldd;
       eo.count = last && mean ? count : nullptr;
       eo.un = last ? un(kUnGX) : nullptr;
-      TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.planes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
+      TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.gplanes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
                     eo, s));
     }
   }
