@@ -325,12 +325,21 @@ LLATTN_API int llattn_bwd_noalloc(const llattn_bwd_args* args, void* stream);
  * loss (fp32 scalar; reductions mean and sum), dx [tokens, d], dw [vocab, d]
  * dtype, contiguous. workspace: llattn_xent_workspace_bytes bytes, 256-byte
  * aligned, no initialisation; it holds half a GiB of exponentials at most
- * (at least 256 rows), whatever the number of tokens. */
+ * (at least 256 rows), whatever the number of tokens.
+ * stage LLATTN_XENT_ALL: all of it. Where the exponentials fit at once
+ * (llattn_xent_workspace_bytes of LLATTN_XENT_LOSS is not 0), reductions mean and
+ * sum can also run in two calls with the upstream gradient known only to the
+ * second: LLATTN_XENT_LOSS writes loss, and LLATTN_XENT_GRADS, any number of times,
+ * dx and dw times *factor (device scalar; NULL: 1) from the first one's
+ * workspace, unchanged since, as kept, with the other arguments as they were, a
+ * workspace of its own, and loss NULL. */
 typedef enum llattn_xent_reduction {
   LLATTN_XENT_NONE = 0,
   LLATTN_XENT_MEAN = 1,
   LLATTN_XENT_SUM = 2
 } llattn_xent_reduction;
+
+typedef enum llattn_xent_stage { LLATTN_XENT_ALL = 0, LLATTN_XENT_LOSS = 1, LLATTN_XENT_GRADS = 2 } llattn_xent_stage;
 
 typedef struct llattn_xent_args {
   int32_t tokens, d, vocab, dtype, reduction;
@@ -347,6 +356,9 @@ typedef struct llattn_xent_args {
   void* dw;
   void* workspace;
   size_t workspace_bytes;
+  int32_t stage;
+  const float* factor;
+  void* kept;
 } llattn_xent_args;
 
 /* pointers are only tested for NULL and alignment (0 on bad arguments) */

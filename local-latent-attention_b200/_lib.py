@@ -24,6 +24,7 @@ EXPORTED = (
     "llattn_xent_workspace_bytes", "llattn_xent", "llattn_scale", "llattn_orth_workspace_bytes", "llattn_orth",
 )
 XENT_NONE, XENT_MEAN, XENT_SUM = 0, 1, 2
+XENT_ALL, XENT_LOSS, XENT_GRADS = 0, 1, 2  # stages
 
 
 class Dims(ctypes.Structure):
@@ -73,7 +74,8 @@ class XentArgs(ctypes.Structure):
     _fields_ = [("tokens", ctypes.c_int32), ("d", ctypes.c_int32), ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32),
                 ("reduction", ctypes.c_int32), ("ignore_index", ctypes.c_int64), ("x", _vp), ("ldx", ctypes.c_int64),
                 ("w", _vp), ("ldw", ctypes.c_int64), ("targets", _vp), ("grad_rows", _fp), ("losses", _fp),
-                ("loss", _fp), ("dx", _vp), ("dw", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+                ("loss", _fp), ("dx", _vp), ("dw", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+                ("stage", ctypes.c_int32), ("factor", _fp), ("kept", _vp)]
 
 
 class OrthArgs(ctypes.Structure):

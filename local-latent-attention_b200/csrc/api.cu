@@ -700,6 +700,9 @@ static int check_xent(const llattn_xent_args* a) {
   if (a->dtype != LLATTN_F32 && a->dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", a->dtype);
   if (a->reduction < LLATTN_XENT_NONE || a->reduction > LLATTN_XENT_SUM)
     return fail(LLATTN_ERR_ARG, "xent: unknown reduction %d", a->reduction);
+  if (a->stage < LLATTN_XENT_ALL || a->stage > LLATTN_XENT_GRADS) return fail(LLATTN_ERR_ARG, "xent: unknown stage %d", a->stage);
+  if (a->stage != LLATTN_XENT_ALL && a->reduction == LLATTN_XENT_NONE)
+    return fail(LLATTN_ERR_ARG, "xent: stages go with reductions mean and sum");
   if (a->ldx < a->d || a->ldw < a->d)
     return fail(LLATTN_ERR_ARG, "xent: row strides (%lld, %lld) below d = %d", (long long)a->ldx, (long long)a->ldw, a->d);
   return LLATTN_OK;
@@ -712,6 +715,12 @@ int llattn_xent(const llattn_xent_args* a, void* stream) {
   if (rc) return rc;
   if (!a->x || !a->w || !a->targets) return fail(LLATTN_ERR_ARG, "llattn_xent: NULL pointer in args");
   const bool grads = a->dx || a->dw;
+  if (a->stage == LLATTN_XENT_LOSS && (grads || a->losses))
+    return fail(LLATTN_ERR_ARG, "llattn_xent: stage loss writes the loss only");
+  if (a->stage == LLATTN_XENT_GRADS && (!grads || a->loss || !a->kept || !al(a->kept, 256)))
+    return fail(LLATTN_ERR_ARG, "llattn_xent: stage grads writes dx and dw, from the kept workspace of a stage loss");
+  if (a->stage != LLATTN_XENT_GRADS && (a->factor || a->kept))
+    return fail(LLATTN_ERR_ARG, "llattn_xent: factor and kept go with stage grads");
   if (!grads && !a->losses && !a->loss) return fail(LLATTN_ERR_ARG, "llattn_xent: no output asked for");
   if (grads && a->losses) return fail(LLATTN_ERR_ARG, "llattn_xent: losses are written without gradients only");
   if (a->loss && a->reduction == LLATTN_XENT_NONE)
@@ -719,6 +728,7 @@ int llattn_xent(const llattn_xent_args* a, void* stream) {
   if (grads && (a->reduction == LLATTN_XENT_NONE) != (a->grad_rows != nullptr))
     return fail(LLATTN_ERR_ARG, "llattn_xent: grad_rows goes with reduction none");
   const size_t need = xent::workspace_bytes(*a);
+  if (need == 0) return fail(LLATTN_ERR_ARG, "llattn_xent: %d tokens do not fit one piece: no stages", a->tokens);
   if (!a->workspace || a->workspace_bytes < need)
     return fail(LLATTN_ERR_WORKSPACE, "llattn_xent: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
   if (!al(a->workspace, 256)) return fail(LLATTN_ERR_ALIGN, "llattn_xent: workspace must be 256-byte aligned");

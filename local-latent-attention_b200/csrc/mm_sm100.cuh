@@ -551,6 +551,8 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 //                                          bool zero, uint8_t* buf) const
 //   static constexpr bool kNarrow, kWide: shapes 0 and 4 (CW = 32 and 64, else 128), and 3, may be used
 //   static constexpr bool kChain: MmArgs::chain may be set
+//   static constexpr bool kBegin: __device__ void begin(int warp, int warps) const is called once, by every warp
+//     of the grid's epilogue warps, while the first tile's products are under way
 // tile is called by every thread of an epilogue warp (all 32 lanes,
 // converged) for its row and CW columns [col0, col0 + CW); taddr: TMEM address of the warp's
 // lanes and columns; zero: the K range is empty, the accumulator holds
@@ -756,6 +758,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns CW half..
     int k = 0;
     bool ok = true;
+    if constexpr (Epi::kBegin) epi.begin(blockIdx.x * S::EW + warp - 2, gridDim.x * S::EW);
     auto release = [&](int b) {  // accumulator (half) b may be filled again
       tc_fence_before();
       __syncwarp();

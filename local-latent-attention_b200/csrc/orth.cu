@@ -64,7 +64,7 @@ __device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, bool m
 
 // S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
 struct EpiGram {
-  static constexpr bool kNarrow = true, kWide = false, kChain = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = false, kBegin = false;
   __half* s;
   int64_t ld, zs;
   const float* s0;  // first step: X = s0[z] * stored, else null (2^-6)
@@ -89,7 +89,7 @@ struct EpiGram {
 
 // B = b S + c S^2 + k I (scaled by kS)
 struct EpiPoly {
-  static constexpr bool kNarrow = true, kWide = false, kChain = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = false, kBegin = false;
   const __half* s;
   __half* b;
   int64_t ld, zs;
@@ -124,7 +124,7 @@ struct EpiPoly {
 
 // X <- a X + B X, or (B + a I) X
 struct EpiUpdate {
-  static constexpr bool kNarrow = true, kWide = false, kChain = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = false, kBegin = false;
   const __half* hi;
   bf16* lo;          // remainder of X, read where rd_lo, written (in place) where wr_lo
   __half* next;      // next X (hi), or null in the last step

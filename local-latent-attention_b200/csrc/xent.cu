@@ -56,13 +56,13 @@ constexpr uint32_t kTermsA = 0x001u, kTermsB = 0x010u, kFineA = 0x01u;
 // single token), and their tensor-core sums are short chains (MmArgs::chain): of
 // 4 K = 64 steps for bf16 logits (the loss of 1 token at d = 2048: 2e-6 off
 // without chains, 4e-7 with; one token's time is the same, 129 tokens of V = 32000
-// would take 150 instead of 143 us), of 2 for fp32's three products. fp32's sums
+// would take 150 instead of 143 us), of 1 for fp32's three products. fp32's sums
 // always run in chains (d = 2048, 300 tokens: gradients 2.4e-6 off at 1024
 // products a sum, 7e-7 at 512), bf16 logits where they are longer than kChain
 // steps (losses of 1024 tokens, d = 2048: 1.0e-6 off in one sum, 5e-7 in two;
 // d = 1536: 7.7e-7 in one, and two would take 148 instead of 142 us for 2048
 // tokens).
-constexpr int kFine = 64, kFineChain = 4, kFineF32Chain = 2, kF32Chain = 8, kChain = 24;
+constexpr int kFine = 64, kFineChain = 4, kFineF32Chain = 1, kF32Chain = 8, kChain = 24;
 
 // fp32's powers of two: of x, w, G, and the inverses that undo them in x w^T,
 // G w and G^T x
@@ -72,7 +72,7 @@ constexpr int kAmax = 128;  // partial maxima each of x, w and the rows' gradien
 // ---- first product: statistics and exponentials ----------------------------
 
 struct EpiStats {
-  static constexpr bool kNarrow = false, kWide = false, kChain = true;  // wide: sums over d are short, its long epilogue shows (757 us for 620)
+  static constexpr bool kNarrow = false, kWide = false, kChain = true, kBegin = false;  // wide: sums over d are short, its long epilogue shows (757 us for 620)
   float2* stats;       // [rows][n_tiles]: (max, sum of exp(l - max))
   int n_tiles;
   const int* tgt;      // [rows] target of row (dev_base already added); < 0: none
@@ -156,7 +156,7 @@ struct EpiStats {
 constexpr int kFew = 32;
 
 struct EpiScore {
-  static constexpr bool kNarrow = true, kWide = false, kChain = true;
+  static constexpr bool kNarrow = true, kWide = false, kChain = true, kBegin = false;
   float2* stats;  // [tokens][n_tiles]
   int n_tiles;
   const int64_t* targets;
@@ -189,7 +189,7 @@ struct EpiScore {
 // ---- second and third product: rows out --------------------------------------
 
 struct EpiOut {
-  static constexpr bool kNarrow = true, kWide = true, kChain = true;
+  static constexpr bool kNarrow = true, kWide = true, kChain = true, kBegin = true;
   void* out;
   int64_t ldo;
   int out_bf16;
@@ -200,9 +200,25 @@ struct EpiOut {
   const int* idx;       // output row of row m, or null
   const int* count;     // the result is divided by max(1, *count), or null
   const float* un;      // and multiplied by *un, or null
+  const float* factor;  // and by *factor, or null
+  const int64_t* zero;  // rows of out whose target, of zero_n, is `ignore` become zeros; or null
+  int zero_n;
+  int64_t ignore;
 
   __device__ __forceinline__ float scale() const {
-    return (count ? 1.f / (float)max(1, *count) : 1.f) * (un ? *un : 1.f);
+    return (count ? 1.f / (float)max(1, *count) : 1.f) * (un ? *un : 1.f) * (factor ? *factor : 1.f);
+  }
+  __device__ __forceinline__ void begin(int warp, int warps) const {
+    if (!zero) return;
+    for (int64_t r = warp; r < zero_n; r += warps) {
+      if (zero[r] != ignore) continue;
+      for (int64_t c = r * ldo + threadIdx.x % 32; c < (r + 1) * ldo; c += 32) {
+        if (out_bf16)
+          static_cast<bf16*>(out)[c] = __float2bfloat16_rn(0.f);
+        else
+          static_cast<float*>(out)[c] = 0.f;
+      }
+    }
   }
 
   // 4 columns of a row of a split tile, joined
@@ -449,7 +465,7 @@ __global__ void __launch_bounds__(256) xent_pack(const T* __restrict__ x, int64_
 // order: idx[j] = row of the j-th, tgt[j] = its target (-1: out of range, which
 // makes the row's loss and gradients NaN; lt[j] starts at NaN for the same
 // reason), *count; packs their rows of x, xs[j] = x[idx[j]], and zeros the rows
-// past the count and the dx rows of ignored tokens. Each CTA takes `per` rows
+// past the count. Each CTA takes `per` rows
 // (a multiple of 8) and counts the targets before them for itself: reading a
 // few hundred KB from L2 again costs less than a second launch or a wait
 // (measured 56 us for one CTA's scan of 32768 targets, 12 us this way with the
@@ -459,8 +475,8 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
                                                  const int64_t* __restrict__ targets, int n, int64_t ignore, int vocab,
                                                  int per, int* __restrict__ idx, int* __restrict__ tgt,
                                                  float* __restrict__ lt, int* __restrict__ count, bf16* __restrict__ xs,
-                                                 int64_t lds, int64_t plane, T* __restrict__ dx, const T* __restrict__ w,
-                                                 int64_t ldw, bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w,
+                                                 int64_t lds, int64_t plane, const T* __restrict__ w, int64_t ldw,
+                                                 bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w,
                                                  const float* __restrict__ amax, float* __restrict__ scales) {
   __shared__ float sc[3];
   pdl_next();
@@ -524,11 +540,7 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
     __syncthreads();
     for (int k = warp; k < min(256, r1 - c0); k += 8) {
       const int64_t row = c0 + k;
-      if (pos[k] >= 0) {
-        pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec, fx);
-      } else if (dx) {
-        for (int c = lane; c < d; c += 32) dx[row * d + c] = from_f<T>(0.f);
-      }
+      if (pos[k] >= 0) pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec, fx);
       if (row >= all) pack_row<T>(nullptr, d, xs + row * lds, lds, plane, vec, fx);
     }
   }
@@ -741,6 +753,7 @@ struct Plan {
   bool f32, train, few, pack_x, pack_w;
   int elt, planes, gplanes, n_tiles, piece, n_pieces;
   int64_t ldx, ldw, ldp, ldd;
+  size_t part_bytes;
   size_t xs, ws, stats, lt, idx, tgt, count, losses, p, g, amax, scales, acc, part, total;
 };
 
@@ -794,7 +807,7 @@ Plan make_plan(const llattn_xent_args& a) {
   q.f32 = a.dtype == LLATTN_F32;
   q.elt = q.f32 ? 4 : 2;
   q.planes = q.f32 ? 2 : 1;
-  q.train = a.dx || a.dw;
+  q.train = a.dx || a.dw || a.stage != LLATTN_XENT_ALL;
   q.gplanes = q.f32 || a.tokens <= kFine ? 2 : 1;
   q.pack_x = q.f32 || q.train || !aligned_rows(a.x, a.ldx, a.tokens, 2);
   q.pack_w = q.f32 || !aligned_rows(a.w, a.ldw, a.vocab, 2);
@@ -830,7 +843,8 @@ Plan make_plan(const llattn_xent_args& a) {
   int64_t part = 0;
   if (a.dx) part = mm_part_floats(dx_args(q, a, q.piece, nullptr));
   if (a.dw) part = std::max(part, mm_part_floats(dw_args(q, a, q.piece, nullptr)));
-  q.part = take(q.train ? 4 * (size_t)part : 0);
+  q.part_bytes = 4 * (size_t)part;
+  q.part = take(a.stage == LLATTN_XENT_ALL ? q.part_bytes : 0);
   q.total = off;
   return q;
 }
@@ -843,7 +857,8 @@ Plan make_plan(const llattn_xent_args& a) {
 
 template <typename T>
 cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fault, cudaStream_t s) {
-  char* ws = static_cast<char*>(a.workspace);
+  const bool grads = a.stage == LLATTN_XENT_GRADS;  // on what a call of stage LOSS left in its workspace
+  char* ws = static_cast<char*>(grads ? a.kept : a.workspace);
   bf16* xs = reinterpret_cast<bf16*>(ws + q.xs);
   bf16* wp = reinterpret_cast<bf16*>(ws + q.ws);
   float2* stats = reinterpret_cast<float2*>(ws + q.stats);
@@ -858,7 +873,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   float* amax = reinterpret_cast<float*>(ws + q.amax);
   float* scales = q.f32 ? reinterpret_cast<float*>(ws + q.scales) : nullptr;
   auto un = [&](int i) { return scales ? scales + i : nullptr; };
-  if (q.f32)
+  if (q.f32 && !grads)
     TRY(launch_pdl(xent_amax, dim3(3 * kAmax), 256, 0, 1, s, static_cast<const float*>(a.x), a.ldx, n, d, a.targets,
                    a.ignore_index, static_cast<const float*>(a.w), a.ldw, V, a.grad_rows, amax));
   if (!q.train) {
@@ -891,16 +906,16 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     }
     return cudaSuccess;
   }
-  T* dx = static_cast<T*>(a.dx);
   const int per = std::max(8, cdiv(cdiv(n, 512), 8) * 8), n_w = q.pack_w ? cdiv(V, 16) : 0;
-  TRY(launch_pdl(xent_prep<T>, dim3(n_w + cdiv(n, per)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, d, a.targets, n, a.ignore_index, V, per,
-                                                  idx, tgt, lt, count, xs, q.ldx, xplane, dx, static_cast<const T*>(a.w),
-                                                  a.ldw, wp, q.ldw, wplane, n_w, amax, scales));
+  if (!grads)
+    TRY(launch_pdl(xent_prep<T>, dim3(n_w + cdiv(n, per)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, d, a.targets, n,
+                   a.ignore_index, V, per, idx, tgt, lt, count, xs, q.ldx, xplane, static_cast<const T*>(a.w), a.ldw, wp,
+                   q.ldw, wplane, n_w, amax, scales));
   float* losses = reinterpret_cast<float*>(ws + q.losses);
   void* pbuf = ws + q.p;
   void* gpl = ws + q.g;
   float* acc = reinterpret_cast<float*>(ws + q.acc);
-  float* part = reinterpret_cast<float*>(ws + q.part);  // split tiles of one product at a time
+  float* part = reinterpret_cast<float*>(grads ? static_cast<char*>(a.workspace) : ws + q.part);  // split tiles of one product at a time
   const int64_t gplane = (int64_t)q.piece * q.ldp;
   for (int c = 0; c < q.n_pieces; ++c) {
     const int base = c * q.piece, rows = std::min(q.piece, n - base);
@@ -913,7 +928,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     p.K = d;
     p.chain = logits_chain(q, a);
     EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.gplanes == 2, un(kUnXW)};
-    TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
+    if (!grads) TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
     auto rows_pass = [&](auto kernel, int shares) {
       return launch_pdl(kernel, dim3(rows, shares), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
@@ -925,7 +940,8 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       return share ? rows_pass(xent_rows<kG, 4>, 4) : rows_pass(xent_rows<kG, 1>, 1);
     };
     using std::integral_constant;
-    if constexpr (sizeof(T) == 4) {
+    if (grads) {
+    } else if constexpr (sizeof(T) == 4) {
       TRY(rows_as(integral_constant<GKind, GKind::kHalves>{}));
     } else if (q.gplanes == 2) {
       TRY(rows_as(integral_constant<GKind, GKind::kBf16s>{}));
@@ -933,16 +949,20 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       TRY(rows_as(integral_constant<GKind, GKind::kInPlace>{}));
     }
     const void* g = q.gplanes == 2 ? gpl : pbuf;
-    if (dx) {
+    if (a.dx) {
       MmArgs m = dx_args(q, a, rows, fault);
       m.m_dev = count;
       m.dev_base = base;
       m.part = part;
       EpiOut eo{};
-      eo.out = dx;
+      eo.out = a.dx;
       eo.ldo = d;
       eo.out_bf16 = !q.f32;
-      eo.vec = aligned_rows(dx, d, 2, q.elt);
+      eo.vec = aligned_rows(a.dx, d, 2, q.elt);
+      eo.factor = a.factor;
+      eo.zero = c ? nullptr : a.targets;
+      eo.zero_n = n;
+      eo.ignore = a.ignore_index;
       eo.idx = idx + base;
       eo.count = mean ? count : nullptr;
       eo.un = un(kUnGW);
@@ -965,6 +985,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.ldacc = q.ldd;
       eo.count = last && mean ? count : nullptr;
       eo.un = last ? un(kUnGX) : nullptr;
+      eo.factor = a.factor;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.gplanes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
                     eo, s));
     }
@@ -974,12 +995,17 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
 
 }  // namespace
 
-size_t workspace_bytes(const llattn_xent_args& a) { return make_plan(a).total; }
+size_t workspace_bytes(const llattn_xent_args& a) {
+  const Plan q = make_plan(a);
+  if (a.stage != LLATTN_XENT_ALL && q.n_pieces > 1) return 0;
+  return a.stage == LLATTN_XENT_GRADS ? std::max<size_t>(256, up256(q.part_bytes)) : q.total;
+}
 
 int launches(const llattn_xent_args& a) {
   const Plan q = make_plan(a);
   if (!q.train) return q.f32 + q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
-  return q.f32 + 1 + q.n_pieces * (2 + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
+  const int loss = a.stage == LLATTN_XENT_GRADS ? 0 : 1;
+  return loss * (q.f32 + 1) + q.n_pieces * (2 * loss + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
                            (a.dw ? 1 + joins(dw_args(q, a, q.piece, nullptr)) : 0));
 }
 

@@ -48,6 +48,7 @@ def _rows(t: Tensor) -> Tensor:
 
 
 _TYPES = (torch.bfloat16, torch.float32)
+_PLAIN = torch.contiguous_format
 
 
 def _check_xent(x: Tensor, w: Tensor, targets: Tensor) -> None:
@@ -65,6 +66,38 @@ def _check_xent(x: Tensor, w: Tensor, targets: Tensor) -> None:
     _require(w.device == x.device and targets.device == x.device, "x, weight and targets must be on one device")
     _dtype_code(x)
     _require(False, "weight must have rows and columns")
+
+
+def _xent_loss(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int):
+    """The loss, and for _xent_grads the arguments with the workspace kept and
+    what else they point to; None where the tokens do not fit at once."""
+    rows, weight, at = _rows(x), _rows(w), targets.contiguous()
+    (n, d), v, dev = rows.shape, weight.shape[0], rows.device
+    args = _lib.XentArgs(n, d, v, _dtype_code(rows), reduction, ignore_index, rows.data_ptr(), max(rows.stride(0), d),
+                         weight.data_ptr(), max(weight.stride(0), d), at.data_ptr(), None, None, None, None, None, None, 0,
+                         _lib.XENT_LOSS)
+    L, ref = _lib.lib(), ctypes.byref(args)
+    with _on(dev):
+        size = L.llattn_xent_workspace_bytes(ref)
+        if not size:
+            return None
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        kept = torch.empty(size, dtype=torch.uint8, device=dev)
+        args.loss, args.workspace, args.workspace_bytes = loss.data_ptr(), kept.data_ptr(), size
+        _lib.check(L.llattn_xent(ref, _stream(x)), "llattn_xent")
+    args.kept, args.loss, args.stage = args.workspace, None, _lib.XENT_GRADS
+    return loss, kept, args, (weight, at)
+
+
+def _xent_grads(args, dx: Optional[Tensor], dw: Optional[Tensor], factor: Tensor) -> None:
+    """dx and dw of *factor times the loss of _xent_loss."""
+    L, ref, dev = _lib.lib(), ctypes.byref(args), factor.device
+    with _on(dev):
+        args.dx, args.dw = dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None
+        size = L.llattn_xent_workspace_bytes(ref)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        args.factor, args.workspace, args.workspace_bytes = factor.data_ptr(), ws.data_ptr(), size
+        _lib.check(L.llattn_xent(ref, _stream(factor)), "llattn_xent")
 
 
 def _xent(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int, *, grad_rows: Optional[Tensor] = None,
@@ -150,13 +183,24 @@ def _scale_(a: Tensor, b: Tensor, factor: Tensor) -> None:
 
 
 class _XentReduced(torch.autograd.Function):
-    """mean / sum: the gradients for an upstream gradient of 1 are computed
-    with the loss (while the exponentials are at hand) and scaled in the backward."""
+    """mean / sum. Where all tokens' exponentials fit in the workspace it is kept
+    until the backward, whose products apply the upstream gradient; otherwise the
+    gradients for an upstream gradient of 1 are computed with the loss, piece by
+    piece, and scaled in the backward (27 us more for 32003 x 1408 of them)."""
 
     @staticmethod
     def forward(ctx, x, w, targets, ignore_index, reduction):
         need = ctx.needs_input_grad
-        f = linear_xent_op if torch.compiler.is_compiling() else _linear_xent
+        compiling = torch.compiler.is_compiling()
+        ctx.args = None
+        if not compiling:
+            _check_xent(x, w, targets)
+            got = _xent_loss(x, w, targets, ignore_index, reduction) if x.shape[0] else None
+            if got is not None:
+                loss, kept, ctx.args, ctx.hold = got
+                ctx.save_for_backward(x, w, targets, kept)
+                return loss
+        f = linear_xent_op if compiling else _linear_xent
         loss, dx, dw = f(x, w, targets, ignore_index, reduction, need[0], need[1])
         ctx.save_for_backward(x, w, targets, dx, dw)
         ctx.cfg = (ignore_index, reduction)
@@ -171,6 +215,11 @@ class _XentReduced(torch.autograd.Function):
 
 def _reduced_backward(ctx, grad):
     need = ctx.needs_input_grad
+    if ctx.args is not None:
+        x, w = ctx.saved_tensors[:2]
+        dx, dw = torch.empty_like(x, memory_format=_PLAIN) if need[0] else None, torch.empty_like(w, memory_format=_PLAIN) if need[1] else None
+        _xent_grads(ctx.args, dx, dw, grad)
+        return dx, dw, None, None, None
     x, w, targets, dx, dw = ctx.saved_tensors
     if torch.compiler.is_compiling():
         return ((dx * grad).to(x.dtype) if need[0] else None, (dw * grad).to(w.dtype) if need[1] else None, None, None,
@@ -217,9 +266,10 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
     0 for ignored tokens). Ignored tokens get zero gradients and their rows of x
     are not read for weight's. A target outside [0, vocab) makes the loss NaN.
 
-    "mean" and "sum" compute the gradients together with the loss, from at most
-    half a GiB of exponentials at a time, and keep them until the backward;
-    "none" recomputes in the backward. Gradients of gradients are not supported."""
+    "mean" and "sum" keep the exponentials until the backward where they take at
+    most half a GiB; for more tokens they compute the gradients together with the
+    loss, half a GiB of exponentials at a time, and keep those. "none" recomputes
+    in the backward. Gradients of gradients are not supported."""
     code = _REDUCTIONS.get(reduction)
     if code is None:
         _require(False, f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")

@@ -242,6 +242,51 @@ def test_retained_graph():
         assert torch.equal(u, v)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("factor", [0.25, -1.7, 0.0])
+def test_upstream_gradient(dtype, factor):
+    """The upstream gradient scales the products before their only rounding;
+    strided inputs; only one of the gradients wanted."""
+    n, d, v = 130, 72, 301
+    x, w, t = make(n, d, v, dtype, ignored=0.3)
+    _, rdx, rdw = plain(x, w, t)
+    xs = torch.empty(n, d + 9, device="cuda", dtype=dtype)[:, :d].copy_(x).requires_grad_(True)
+    ws = torch.empty(v, d + 5, device="cuda", dtype=dtype)[:, :d].copy_(w).requires_grad_(True)
+    dx, dw = torch.autograd.grad(linear_cross_entropy(xs, ws, t) * factor, (xs, ws))
+    for got, want in ((dx, rdx), (dw, rdw)):
+        if factor:
+            assert rel(got, want * factor) <= GRAD_TOL[dtype]
+        else:
+            assert not got.any()
+    assert not dx[t == -100].any()
+    only_x, = torch.autograd.grad(linear_cross_entropy(xs, ws.detach(), t) * factor, (xs,))
+    only_w, = torch.autograd.grad(linear_cross_entropy(xs.detach(), ws, t) * factor, (ws,))
+    assert torch.equal(only_x, dx) and torch.equal(only_w, dw)
+
+
+def test_changed_inputs_are_refused_in_the_backward():
+    x, w, t = make(40, 64, 200, BF)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, t)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("n,d,v,dtype", [(1, 2048, 4000, FP), (1, 2048, 4000, BF), (200, 2048, 3000, FP), (70, 1700, 900, BF)])
+def test_long_products_keep_fp32(n, d, v, dtype):
+    """Losses of long dot products: the tensor cores' truncating additions run in
+    chains joined in fp32. A chain loses up to 2^-26 (bf16) or 2^-24 (fp32's
+    planes) of itself per 16 products, so a logit of at most 14 is at most 14 x
+    24 x 4 x 2^-26 / 2 = 1e-5 (bf16, 24 steps a chain) or 14 x 8 x 4 x 2^-24 / 2 =
+    1.4e-5 (fp32, 8 steps) off, plus fp32's rounding of the loss itself."""
+    x, w, t = make(n, d, v, dtype)
+    ref = plain(x, w, t, "none")[0]
+    got = linear_cross_entropy(x, w, t, reduction="none").double()
+    assert (got - ref).abs().max().item() <= 2e-5
+
+
 def test_gradient_against_differences():
     """fp32: the directional derivative of the loss by central differences in
     64 bits of the plain loss, at the same point."""

@@ -68,6 +68,26 @@ def test_xent_refusals_on_the_host(bad, msg):
     assert msg in L.llattn_last_error().decode()
 
 
+@pytest.mark.parametrize("bad,msg", [
+    (dict(stage=3), "unknown stage"), (dict(stage=-1), "unknown stage"),
+    (dict(stage=_lib.XENT_LOSS, reduction=_lib.XENT_NONE), "mean and sum"),
+    (dict(stage=_lib.XENT_LOSS, dx=1 << 21), "loss only"), (dict(stage=_lib.XENT_LOSS, losses=1 << 22), "loss only"),
+    (dict(stage=_lib.XENT_GRADS, dx=1 << 21, kept=1 << 23), "kept workspace"),
+    (dict(stage=_lib.XENT_GRADS, loss=None, kept=1 << 23), "kept workspace"),
+    (dict(stage=_lib.XENT_GRADS, loss=None, dx=1 << 21), "kept workspace"),
+    (dict(stage=_lib.XENT_GRADS, loss=None, dx=1 << 21, kept=1), "kept workspace"),
+    (dict(factor=1 << 23), "go with stage grads"), (dict(stage=_lib.XENT_LOSS, kept=1 << 23), "go with stage grads"),
+    (dict(stage=_lib.XENT_LOSS, tokens=100000, vocab=1 << 20), "one piece"),
+    (dict(stage=_lib.XENT_LOSS), "workspace of"), (dict(stage=_lib.XENT_GRADS, loss=None, dw=1 << 21, kept=1 << 23), "workspace of"),
+])
+def test_xent_stage_refusals_on_the_host(bad, msg):
+    L = _lib.lib()
+    args = xent_args(**{k: v for k, v in bad.items() if k not in ("stage", "factor", "kept")})
+    args.stage, args.factor, args.kept = bad.get("stage", _lib.XENT_ALL), bad.get("factor"), bad.get("kept")
+    assert L.llattn_xent(ctypes.byref(args), None) != 0
+    assert msg in L.llattn_last_error().decode()
+
+
 def test_xent_workspace_is_bounded():
     """Half a GiB of exponentials whatever the number of tokens; what grows
     with them is their packed rows and a few words each."""
