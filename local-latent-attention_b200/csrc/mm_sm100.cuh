@@ -363,18 +363,20 @@ struct MappedRows {
 template <bool ADD, int CH, typename R>
 __device__ __forceinline__ void block_write_out(const uint8_t* buf, int lane, const R& dst, int bytes) {
   const int c = lane % CH;
+  // all reads before the first write: the compiler may not move them across it
+  uint4 u[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) u[i] = *reinterpret_cast<const uint4*>(buf + stage_at<CH>(32 / CH * i + lane / CH, c));
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int r = 32 / CH * i + lane / CH;
-    const uint4 u = *reinterpret_cast<const uint4*>(buf + stage_at<CH>(r, c));
-    uint8_t* q = dst.row(r);
+    uint8_t* q = dst.row(32 / CH * i + lane / CH);
     if (q && 16 * c < bytes) {
       if (ADD)  // fp32: added in the L2, nothing waits for the old value
-        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(q + 16 * c), "f"(__uint_as_float(u.x)),
-                     "f"(__uint_as_float(u.y)), "f"(__uint_as_float(u.z)), "f"(__uint_as_float(u.w))
-                     : "memory");
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(q + 16 * c), "f"(__uint_as_float(u[i].x)),
+                     "f"(__uint_as_float(u[i].y)), "f"(__uint_as_float(u[i].z)), "f"(__uint_as_float(u[i].w)));
       else
-        *reinterpret_cast<uint4*>(q + 16 * c) = u;
+        asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(q + 16 * c), "r"(u[i].x), "r"(u[i].y), "r"(u[i].z),
+                     "r"(u[i].w));
     }
   }
   __syncwarp();
