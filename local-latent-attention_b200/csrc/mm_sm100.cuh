@@ -596,7 +596,10 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     mm_tmem_alloc<CG>(tmem_slot, S::TCOLS);
   }
   pdl_next();
-  pdl_wait();
+  // Without device-side counts the schedule is known before the kernels ahead are
+  // done, and only the warps that touch global memory wait for them.
+  const bool counted = p.m_dev || p.k_dev;
+  if (counted) pdl_wait();
   if (threadIdx.x == 0) {
     const MmGrid<SH> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
     *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
@@ -616,6 +619,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   constexpr bool one = S::ACC == 1 || (CHAIN && SH == 2);
 
   if (warp == 0) {
+    if (!counted) pdl_wait();
     if (lane == 0) {
       int it = 0;
       bool ok = true;
@@ -760,6 +764,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns CW half..
     int k = 0;
     bool ok = true;
+    if (!counted) pdl_wait();
     if constexpr (Epi::kBegin) epi.begin(blockIdx.x * S::EW + warp - 2, gridDim.x * S::EW);
     auto release = [&](int b) {  // accumulator (half) b may be filled again
       tc_fence_before();
