@@ -65,12 +65,14 @@ __device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, bool m
 // S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
 struct EpiGram {
   static constexpr bool kNarrow = true, kWide = false, kChain = false, kBegin = false;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
   __half* s;
   int64_t ld, zs;
   const float* s0;  // first step: X = s0[z] * stored, else null (2^-6)
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
+                                       bool zero, uint8_t* buf, Pre&) const {
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float f = x * x * kS;
     __half* base = s + w.z * zs;
@@ -94,15 +96,23 @@ struct EpiPoly {
   __half* b;
   int64_t ld, zs;
   float cb, cc2, k;  // b, c / kS, k * kS
+  struct Pre {
+    uint4 u[4];
+  };
+  __device__ __forceinline__ Rows src(const MmTile& w, int row0, int col0, int M) const {
+    return Rows{s + w.z * zs + row0 * ld + col0, ld * 2, M - row0};
+  }
+  __device__ __forceinline__ void fetch(Pre& pre, const MmArgs& a, MmTile w, int row, int col0, int M) const {
+    const int lane = threadIdx.x % 32;
+    if (col0 < a.N) block_fetch(lane, pre.u, src(w, row - lane, col0, M), (a.N - col0) * 2);
+  }
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
+                                       bool zero, uint8_t* buf, Pre& pre) const {
     const int lane = threadIdx.x % 32;
     __half* base = b + w.z * zs;
-    const int row0 = row - lane;
-    const Rows src{s + w.z * zs + row0 * ld + col0, ld * 2, M - row0};
-    uint4 u[4];  // fetched a block ahead: its latency passes during the stores
-    if (col0 < a.N) block_fetch(lane, u, src, (a.N - col0) * 2);
+    const Rows from = src(w, row - lane, col0, M);
+    uint4(&u)[4] = pre.u;  // fetched a block ahead: its latency passes during the stores
 #pragma unroll 1
     for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
@@ -116,7 +126,7 @@ struct EpiPoly {
         v[2 * q] = fmaf(cb, x.x, cc2 * v[2 * q]) + (row == nc + 2 * q ? k : 0.f);
         v[2 * q + 1] = fmaf(cb, x.y, cc2 * v[2 * q + 1]) + (row == nc + 2 * q + 1 ? k : 0.f);
       }
-      if (cc + 32 < CW && n > 32) block_fetch(lane, u, src.at((cc + 32) * 2), (n - 32) * 2);
+      if (cc + 32 < CW && n > 32) block_fetch(lane, u, from.at((cc + 32) * 2), (n - 32) * 2);
       store_symmetric(base, ld, a.sym && w.m0 != w.n0, row, nc, M, a.N, v, buf);
     }
   }
@@ -133,19 +143,27 @@ struct EpiUpdate {
   const float* s0;
   float ca;          // a
   int rd_hi, rd_lo, wr_lo, vec_out;
+  struct Pre {
+    uint4 h[4], l[4];
+  };
+  // 32 columns of hi and lo, n of them valid
+  __device__ __forceinline__ void block(Pre& pre, int64_t at, int rows, int n) const {
+    const int lane = threadIdx.x % 32;
+    if (rd_hi) block_fetch(lane, pre.h, Rows{hi + at, ld * 2, rows}, n * 2);
+    if (rd_lo) block_fetch(lane, pre.l, Rows{lo + at, ld * 2, rows}, n * 2);
+  }
+  __device__ __forceinline__ void fetch(Pre& pre, const MmArgs& a, MmTile w, int row, int col0, int M) const {
+    const int row0 = row - (int)(threadIdx.x % 32);
+    if (col0 < a.N) block(pre, w.z * zs + row0 * ld + col0, M - row0, a.N - col0);
+  }
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
+                                       bool zero, uint8_t* buf, Pre& pre) const {
     const int lane = threadIdx.x % 32;
     const int row0 = row - lane, rows = M - row0;
     const float x = s0 ? s0[w.z] : 1.f / kX;
     const float fl = ca * x, fp = x / kS;
-    uint4 h[4], l[4];  // fetched a block ahead, as in EpiPoly
-    auto fetch = [&](int64_t at, int n) {
-      if (rd_hi) block_fetch(lane, h, Rows{hi + at, ld * 2, rows}, n * 2);
-      if (rd_lo) block_fetch(lane, l, Rows{lo + at, ld * 2, rows}, n * 2);
-    };
-    if (col0 < a.N) fetch(w.z * zs + row0 * ld + col0, a.N - col0);
+    uint4(&h)[4] = pre.h, (&l)[4] = pre.l;  // fetched a block ahead, as in EpiPoly
 #pragma unroll 1
     for (int cc = 0; cc < CW; cc += 32) {
       const int nc = col0 + cc, n = a.N - nc;
@@ -173,7 +191,7 @@ struct EpiUpdate {
           v[2 * q + 1] = fmaf(fl, y.y, v[2 * q + 1]);
         }
       }
-      if (cc + 32 < CW && n > 32) fetch(at + 32, n - 32);
+      if (cc + 32 < CW && n > 32) block(pre, at + 32, rows, n - 32);
       uint4 u[4];
       if (out) {
         const Rows dst{out + w.z * zso + row0 * ldo + nc, ldo * 2, rows};

@@ -72,7 +72,10 @@ constexpr int kAmax = 256;  // partial maxima each of x, w and the rows' gradien
 // ---- first product: statistics and exponentials ----------------------------
 
 struct EpiStats {
-  static constexpr bool kNarrow = false, kWide = false, kChain = true, kBegin = false;  // wide: sums over d are short, its long epilogue shows (757 us for 620)
+  static constexpr bool kNarrow = false, kWide = false, kChain = true, kBegin = false;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
+  // not wide: sums over d are short, its long epilogue shows (757 us for 620)
   float2* stats;       // [rows][n_tiles]: (max, sum of exp(l - max))
   int n_tiles;
   const int* tgt;      // [rows] target of row (dev_base already added); < 0: none
@@ -85,7 +88,7 @@ struct EpiStats {
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
+                                       bool zero, uint8_t* buf, Pre&) const {
     const int nv = min(kTile, a.N - col0);  // columns of this tile
     if (nv <= 0) return;                    // warp-uniform
     const int lane = threadIdx.x % 32;
@@ -173,6 +176,8 @@ __device__ __forceinline__ float warp_transposed(float (&v)[32], int lane, Op op
 
 struct EpiScore {
   static constexpr bool kNarrow = true, kWide = false, kChain = true, kBegin = false;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
   float2* stats;  // [tokens][n_tiles]
   int n_tiles;
   const int64_t* targets;
@@ -181,7 +186,7 @@ struct EpiScore {
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
+                                       bool zero, uint8_t* buf, Pre&) const {
     const int lane = threadIdx.x % 32, n = min(CW, a.N - col0);
     if (row - lane >= M) return;  // warp-uniform
     float v[32];
@@ -226,6 +231,8 @@ struct EpiScore {
 
 struct EpiOut {
   static constexpr bool kNarrow = true, kWide = true, kChain = true, kBegin = true;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
   void* out;
   int64_t ldo;
   int out_bf16;
@@ -290,7 +297,7 @@ struct EpiOut {
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
-                                       bool zero, uint8_t* buf) const {
+                                       bool zero, uint8_t* buf, Pre&) const {
     const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0;
     const int64_t at = row < M ? (idx ? (int64_t)idx[row] : row) * ldo + col0 : -1;
     const float f = scale();
