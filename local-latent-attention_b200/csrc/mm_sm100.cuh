@@ -599,7 +599,9 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   }
   pdl_next();
   // Without device-side counts the schedule is known before the kernels ahead are
-  // done, and only the warps that touch global memory wait for them.
+  // done, and only the warps that touch global memory wait for them, as late as
+  // they can: what an SM does for the first time, from reading the parameters on,
+  // takes it long (4 x 256^2 update: 88 us with the wait here, 66 so).
   const bool counted = p.m_dev || p.k_dev;
   if (counted) pdl_wait();
   if (threadIdx.x == 0) {
@@ -621,45 +623,55 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   constexpr bool one = S::ACC == 1 || (CHAIN && SH == 2);
 
   if (warp == 0) {
-    if (!counted) pdl_wait();
     if (lane == 0) {
       int it = 0;
       bool ok = true;
+      // the copies of a K = 64 step into stage s
+      auto copy = [&](int s, int ma, int nb, int k, int za, int zb, bool first) {
+        if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + S::NH * (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
+        uint8_t* sa = smem + S::A + s * S::AB;
+        uint8_t* sb = smem + S::B + s * S::NH * S::BB;
+        auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
+          if (CG == 1)
+            tma_load_3d(map, &full[s], dst, c0, c1, c2);
+          else
+            tma_load_3d_pair(map, &full[s], dst, c0, c1, c2);
+        };
+        if (first) pdl_wait();
+        if (p.a_mn) {
+          load(&tm_a, sa, ma, k, za);
+          load(&tm_a, sa + S::AB / 2, ma + 64, k, za);
+        } else {
+          load(&tm_a, sa, k, ma, za);
+        }
+#pragma unroll
+        for (int h = 0; h < S::NH; ++h) {
+          uint8_t* dst = sb + h * S::BB;
+          const int n = nb + h * S::HN;
+          if (p.b_mn) {
+            load(&tm_b, dst, n, k, zb);
+            if (S::BR > 64) load(&tm_b, dst + S::BB / 2, n + 64, k, zb);
+          } else {
+            load(&tm_b, dst, k, n, zb);
+          }
+        }
+      };
       for (int t = unit; ok && t < pl.items; t += n_units) {
         const MmItem x = mm_item(pl, t, K);
         const MmTile w = grid.at(p, x.tile);
         const int ma = w.m0 + rank * 128, nb = w.n0 + rank * S::BR;
         for (int term = 0; ok && term < p.n_terms; ++term) {
           const int za = w.z + (int)((p.pa >> (4 * term)) & 15u), zb = w.z + (int)((p.pb >> (4 * term)) & 15u);
-          for (int k = x.k0; k < x.k1; k += 64, ++it) {
+          int k = x.k0;
+          if (!counted && it == 0 && k < x.k1) {  // (apart: a test in the loop costs a long product 3 %)
+            copy(0, ma, nb, k, za, zb, true);
+            k += 64;
+            ++it;
+          }
+          for (; k < x.k1; k += 64, ++it) {
             const int s = it % ST;
             if (it >= ST && !(ok = mbar_wait(&empty[s], ((it / ST) - 1) & 1, abort, &g_mm_fault))) break;
-            if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + S::NH * (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
-            uint8_t* sa = smem + S::A + s * S::AB;
-            uint8_t* sb = smem + S::B + s * S::NH * S::BB;
-            auto load = [&](const CUtensorMap* map, void* dst, int c0, int c1, int c2) {
-              if (CG == 1)
-                tma_load_3d(map, &full[s], dst, c0, c1, c2);
-              else
-                tma_load_3d_pair(map, &full[s], dst, c0, c1, c2);
-            };
-            if (p.a_mn) {
-              load(&tm_a, sa, ma, k, za);
-              load(&tm_a, sa + S::AB / 2, ma + 64, k, za);
-            } else {
-              load(&tm_a, sa, k, ma, za);
-            }
-#pragma unroll
-            for (int h = 0; h < S::NH; ++h) {
-              uint8_t* dst = sb + h * S::BB;
-              const int n = nb + h * S::HN;
-              if (p.b_mn) {
-                load(&tm_b, dst, n, k, zb);
-                if (S::BR > 64) load(&tm_b, dst + S::BB / 2, n + 64, k, zb);
-              } else {
-                load(&tm_b, dst, k, n, zb);
-              }
-            }
+            copy(s, ma, nb, k, za, zb, false);
           }
         }
       }
@@ -766,7 +778,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     const int quad = warp & 3, half = (warp - 2) / 4;  // TMEM lanes 32 quad.., columns CW half..
     int k = 0;
     bool ok = true;
-    if (!counted) pdl_wait();
+    if (!counted && (Epi::kBegin || unit >= pl.items)) pdl_wait();
     if constexpr (Epi::kBegin) epi.begin(blockIdx.x * S::EW + warp - 2, gridDim.x * S::EW);
     auto release = [&](int b) {  // accumulator (half) b may be filled again
       tc_fence_before();
@@ -784,6 +796,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       uint8_t* stage = smem + S::STAGE + (warp - 2) * S::STG;
       const int row = rank * 128 + 32 * quad + lane;
       const uint32_t t0 = tmem + S::CW * half + ((uint32_t)(32 * quad) << 16);
+      if (!counted && t == unit) pdl_wait();
       typename Epi::Pre pre;
       if (x.block < 0) epi.fetch(pre, p, w, w.m0 + row, w.n0 + S::CW * half, M);
       auto out = [&](int col, uint32_t ta) {
