@@ -593,16 +593,28 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
 // logsumexp of a row from its tiles, as (max, log2 of the sum relative to it)
 template <int NT>
 __device__ __forceinline__ float2 join_tiles(const float2* __restrict__ st, int n_tiles, float* red) {
+  // the first 8 NT tiles (all of them up to V = 32 K a tile of 32 columns) are
+  // read once, together
+  constexpr int KEEP = 8;
+  float2 c[KEEP];
   float m = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < KEEP; ++r) {
+    const int i = threadIdx.x + r * NT;
+    c[r] = i < n_tiles ? st[i] : make_float2(-INFINITY, 0.f);
+  }
+#pragma unroll
+  for (int r = 0; r < KEEP; ++r) m = fmaxf(m, c[r].x);
 #pragma unroll 4
-  for (int i = threadIdx.x; i < n_tiles; i += NT) m = fmaxf(m, st[i].x);
+  for (int i = threadIdx.x + KEEP * NT; i < n_tiles; i += NT) m = fmaxf(m, st[i].x);
   m = block_max<NT>(m, red);
   float s = 0.f;
+  auto add = [&](float2 v) { s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e); };
+#pragma unroll
+  for (int r = 0; r < KEEP; ++r)
+    if (r * NT < n_tiles) add(c[r]);
 #pragma unroll 4
-  for (int i = threadIdx.x; i < n_tiles; i += NT) {
-    const float2 v = st[i];
-    s += v.x == -INFINITY ? 0.f : v.y * exp2f((v.x - m) * kLog2e);
-  }
+  for (int i = threadIdx.x + KEEP * NT; i < n_tiles; i += NT) add(st[i]);
   s = block_sum<NT>(s, red);
   return make_float2(m, log2f(s));
 }
@@ -617,9 +629,10 @@ __global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ st
   pdl_next();
   pdl_wait();
   const int64_t row = blockIdx.x, t = targets[row];
+  const float at = lt[row];
   const float2 lse = join_tiles<128>(stats + row * n_tiles, n_tiles, red);
   if (threadIdx.x == 0) {
-    const float l = t >= 0 && t < vocab ? row_loss(lse, lt[row]) : __int_as_float(0x7fc00000);
+    const float l = t >= 0 && t < vocab ? row_loss(lse, at) : __int_as_float(0x7fc00000);
     losses[row] = t == ignore ? 0.f : l;
   }
 }
