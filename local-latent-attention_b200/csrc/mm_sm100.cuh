@@ -98,7 +98,7 @@ struct MmArgs {
   int sym;                  // C symmetric: tiles with n <= m only (square tiles)
   int fp16;                 // operands fp16 instead of bf16
   // products over planes: operand z coordinates (pa, pb) of n_terms passes
-  // over K, 4 bits each (fp32 operands split into bf16 planes)
+  // over K, 4 bits each (fp32 operands in two fp16 planes, G in two of bf16)
   int n_terms;
   uint32_t pa, pb;
   const int* m_dev;

@@ -989,6 +989,10 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     if (!grads) TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
     auto rows_pass = [&](auto kernel, int shares) {
+      if (sm > 48 * 1024) {  // V past 1.5 M, of at most 2 M
+        const cudaError_t e = set_smem_once(kernel, 64 * 1024);
+        if (e != cudaSuccess) return e;
+      }
       return launch_pdl(kernel, dim3(rows, shares), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
                         lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, scales, c + 1 == q.n_pieces ? a.loss : nullptr);
     };

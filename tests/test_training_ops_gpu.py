@@ -264,6 +264,15 @@ def test_upstream_gradient(dtype, factor):
     assert torch.equal(only_x, dx) and torch.equal(only_w, dw)
 
 
+@pytest.mark.parametrize("n,v", [(9, 1_600_001), (20, 2_097_152)])
+def test_largest_vocabularies(n, v):
+    x, w, t = make(n, 16, v, BF)
+    loss, dx, dw = run(x, w, t)
+    rl, rdx, rdw = plain(x, w, t)
+    assert abs(loss.item() - rl.item()) <= 1e-5 * rl.item()
+    assert rel(dx, rdx) <= GRAD_TOL[BF] and rel(dw, rdw) <= GRAD_TOL[BF]
+
+
 def test_changed_inputs_are_refused_in_the_backward():
     x, w, t = make(40, 64, 200, BF)
     x, w = x.requires_grad_(True), w.requires_grad_(True)
