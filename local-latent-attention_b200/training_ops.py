@@ -69,8 +69,9 @@ def _check_xent(x: Tensor, w: Tensor, targets: Tensor) -> None:
 
 
 def _xent_loss(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reduction: int):
-    """The loss, and for _xent_grads the arguments with the workspace kept and
-    what else they point to; None where the tokens do not fit at once."""
+    """The loss, and for _xent_grads the arguments and the tensors that they
+    point to (weight, targets, kept workspace); None where the tokens do not fit
+    at once."""
     rows, weight, at = _rows(x), _rows(w), targets.contiguous()
     (n, d), v, dev = rows.shape, weight.shape[0], rows.device
     args = _lib.XentArgs(n, d, v, _dtype_code(rows), reduction, ignore_index, rows.data_ptr(), max(rows.stride(0), d),
@@ -85,14 +86,24 @@ def _xent_loss(x: Tensor, w: Tensor, targets: Tensor, ignore_index: int, reducti
         kept = torch.empty(size, dtype=torch.uint8, device=dev)
         args.loss, args.workspace, args.workspace_bytes = loss.data_ptr(), kept.data_ptr(), size
         _lib.check(L.llattn_xent(ref, _stream(x)), "llattn_xent")
-    args.kept, args.loss, args.stage = args.workspace, None, _lib.XENT_GRADS
-    return loss, kept, args, (weight, at)
+    return loss, args, weight, at, kept
 
 
-def _xent_grads(args, dx: Optional[Tensor], dw: Optional[Tensor], factor: Tensor) -> None:
-    """dx and dw of *factor times the loss of _xent_loss."""
-    L, ref, dev = _lib.lib(), ctypes.byref(args), factor.device
+def _xent_grads(made, x: Tensor, w: Tensor, targets: Tensor, kept: Tensor, dx: Optional[Tensor], dw: Optional[Tensor],
+                factor: Tensor) -> None:
+    """dx and dw of *factor times the loss that _xent_loss made with the arguments
+    `made`. Their addresses are those of then: x, w, targets and kept, the saved
+    tensors, are where they are now, or copies (an offload's, a checkpoint's)."""
+    L, dev = _lib.lib(), factor.device
+    weight, at = _rows(w), targets.contiguous()
+    args = _lib.XentArgs.from_buffer_copy(made)
+    ref = ctypes.byref(args)
+    args.x, args.w, args.ldw, args.targets = x.data_ptr(), weight.data_ptr(), max(weight.stride(0), args.d), at.data_ptr()
     with _on(dev):
+        if L.llattn_xent_workspace_bytes(ref) != kept.numel():
+            # weight's rows are aligned otherwise than kept was made for (with or without a packed copy of them)
+            kept = _xent_loss(x, weight, at, args.ignore_index, args.reduction)[-1]
+        args.kept, args.loss, args.stage = kept.data_ptr(), None, _lib.XENT_GRADS
         args.dx, args.dw = dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None
         size = L.llattn_xent_workspace_bytes(ref)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
@@ -197,8 +208,8 @@ class _XentReduced(torch.autograd.Function):
             _check_xent(x, w, targets)
             got = _xent_loss(x, w, targets, ignore_index, reduction) if x.shape[0] else None
             if got is not None:
-                loss, kept, ctx.args, ctx.hold = got
-                ctx.save_for_backward(x, w, targets, kept)
+                loss, ctx.args, *saved = got
+                ctx.save_for_backward(x, *saved)
                 return loss
         f = linear_xent_op if compiling else _linear_xent
         loss, dx, dw = f(x, w, targets, ignore_index, reduction, need[0], need[1])
@@ -216,9 +227,10 @@ class _XentReduced(torch.autograd.Function):
 def _reduced_backward(ctx, grad):
     need = ctx.needs_input_grad
     if ctx.args is not None:
-        x, w = ctx.saved_tensors[:2]
-        dx, dw = torch.empty_like(x, memory_format=_PLAIN) if need[0] else None, torch.empty_like(w, memory_format=_PLAIN) if need[1] else None
-        _xent_grads(ctx.args, dx, dw, grad)
+        x, w, targets, kept = ctx.saved_tensors
+        dx = torch.empty_like(x, memory_format=_PLAIN) if need[0] else None
+        dw = torch.empty_like(w, memory_format=_PLAIN) if need[1] else None
+        _xent_grads(ctx.args, x, w, targets, kept, dx, dw, grad)
         return dx, dw, None, None, None
     x, w, targets, dx, dw = ctx.saved_tensors
     if torch.compiler.is_compiling():

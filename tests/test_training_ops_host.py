@@ -1,0 +1,105 @@
+"""The training operators' host side without a GPU: what the backward of
+linear_cross_entropy hands to the C calls, with stand-ins for them."""
+
+import contextlib
+import ctypes
+import gc
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import llattn_b200
+from llattn_b200 import _lib, training_ops
+
+KEPT = 4096
+
+
+class StandIn:
+    """llattn_xent by its arguments alone: records the addresses that each call
+    is given, and at the gradients' which of them belong to a live tensor."""
+
+    def __init__(self):
+        self.calls = []
+
+    def llattn_xent_workspace_bytes(self, ref):
+        return 256 if ref._obj.stage == _lib.XENT_GRADS else KEPT
+
+    def llattn_xent(self, ref, stream):
+        a = ref._obj
+        if a.stage == _lib.XENT_LOSS:
+            ctypes.memset(a.loss, 0, 4)
+            self.calls.append(("loss", a.workspace))
+        else:
+            assert a.stage == _lib.XENT_GRADS
+            live = {t.data_ptr() for t in gc.get_objects() if type(t) in (torch.Tensor, torch.nn.Parameter)}
+            self.calls.append(("grads", a.kept, a.kept in live, a.w in live, a.targets in live, a.w))
+            for p, n in ((a.dx, a.tokens * a.d), (a.dw, a.vocab * a.d)):
+                if p:
+                    ctypes.memset(p, 0, 4 * n)
+        return 0
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    fake = StandIn()
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    monkeypatch.setattr(training_ops, "_on", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(training_ops, "_stream", lambda t: 0)
+    monkeypatch.setattr(training_ops, "_check_xent", lambda *a: None)
+    return fake.calls
+
+
+def copying_hooks():
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t)
+
+
+def case():
+    x = torch.randn(6, 16, requires_grad=True)
+    w = torch.nn.Parameter(torch.randn(10, 16))
+    return x, w, torch.arange(6)
+
+
+@pytest.mark.parametrize("how", ["plain", "hooks", "checkpoint"])
+def test_backward_reads_live_memory_only(calls, how):
+    """The kept workspace belongs to the graph's saved tensors, which hooks (an
+    offload, a checkpoint) may replace: the backward takes it from there."""
+    x, w, t = case()
+    f = lambda x, w: llattn_b200.linear_cross_entropy(x, w, t)
+    if how == "hooks":
+        with copying_hooks():
+            loss = f(x, w)
+    elif how == "checkpoint":
+        loss = checkpoint(f, x, w, use_reentrant=False)
+    else:
+        loss = f(x, w)
+    gc.collect()
+    loss.backward()
+    grads = [c for c in calls if c[0] == "grads"]
+    assert len(grads) == 1 and grads[0][2:5] == (True, True, True), calls
+    if how == "checkpoint":  # computed again, and taken from there
+        assert [c[0] for c in calls] == ["loss", "loss", "grads"] and grads[0][1] == calls[1][1]
+
+
+def test_backward_follows_the_weight_to_its_new_memory(calls):
+    """A weight whose memory is given up between forward and backward and gathered
+    again elsewhere (sharded parameters) is read where it is then."""
+    x, w, t = case()
+    loss = llattn_b200.linear_cross_entropy(x, w, t)
+    other = torch.randn(10, 16)
+    old = w.data_ptr()
+    w.data = other
+    assert w.data_ptr() != old
+    loss.backward()
+    assert calls[-1][0] == "grads" and calls[-1][5] == other.data_ptr(), calls
+
+
+def test_backward_computes_again_what_does_not_fit_its_inputs(calls, monkeypatch):
+    """A saved weight that comes back in another layout than it was kept for
+    (its packed copy is, or is not, part of the workspace): a loss of its own."""
+    x, w, t = case()
+    loss = llattn_b200.linear_cross_entropy(x, w, t)
+    monkeypatch.setattr(StandIn, "llattn_xent_workspace_bytes",
+                        lambda self, ref: 256 if ref._obj.stage == _lib.XENT_GRADS else 2 * KEPT)
+    loss.backward()
+    assert [c[0] for c in calls] == ["loss", "loss", "grads"] and calls[2][1] == calls[1][1] and calls[2][2]

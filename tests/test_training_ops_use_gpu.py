@@ -1,0 +1,73 @@
+"""The training operators as training programs use them: saved-tensor hooks,
+checkpoints, storage that comes and goes."""
+
+import math
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from llattn_b200 import linear_cross_entropy
+from test_training_ops_gpu import BF, FP, make
+
+pytestmark = pytest.mark.gpu
+
+
+def gradients(loss, *inputs):
+    return loss.detach(), *torch.autograd.grad(loss, inputs)
+
+
+def churn():
+    """Fills the allocator's free blocks, of every size up to 64 MB, with other values."""
+    torch.cuda.synchronize()
+    held = [torch.full((1 << k,), 0x7f, dtype=torch.uint8, device="cuda") for k in range(9, 27) for _ in range(4)]
+    torch.cuda.synchronize()
+    return held
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("how", ["save_on_cpu", "hooks", "checkpoint"])
+def test_saved_tensors_that_move(how, dtype):
+    """The backward of a head whose saved tensors were offloaded, copied or thrown
+    away and computed again: the same bits as the plain call's."""
+    n, d, v = 300, 136, 1003  # (rows of w that are copied where they are, and rows that are packed)
+    for cut in (d, d - 5):
+        x, w, t = make(n, d, v, dtype, ignored=0.1)
+        x, w = x[:, :cut].requires_grad_(True), w[:, :cut].requires_grad_(True)
+        want = gradients(linear_cross_entropy(x, w, t) * 0.7, x, w)
+        f = lambda x, w: linear_cross_entropy(x, w, t)
+        if how == "checkpoint":
+            loss = checkpoint(f, x, w, use_reentrant=False)
+        elif how == "save_on_cpu":
+            with torch.autograd.graph.save_on_cpu():
+                loss = f(x, w)
+        else:
+            with torch.autograd.graph.saved_tensors_hooks(lambda s: s.detach().clone(), lambda s: s):
+                loss = f(x, w)
+        held = churn()
+        got = gradients(loss * 0.7, x, w)
+        del held
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_weight_gathered_again_elsewhere(dtype):
+    """A weight whose storage is freed after the forward and filled again before
+    the backward, as sharded parameters are."""
+    x, w, t = make(200, 64, 700, dtype)
+    x, w = x.requires_grad_(True), torch.nn.Parameter(w)
+    want = gradients(linear_cross_entropy(x, w, t), x, w)
+    loss = linear_cross_entropy(x, w, t)
+    values, store = w.detach().clone(), w.untyped_storage()
+    size = store.size()
+    torch.cuda.synchronize()
+    store.resize_(0)
+    held = churn()
+    store.resize_(size)
+    with torch.no_grad():
+        w.data.copy_(values)
+    got = gradients(loss, x, w)
+    del held
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
