@@ -89,7 +89,7 @@ struct MmArgs {
   float* part;
   // The tensor cores' additions drop what lies below the running sum's last
   // bits: a sum that grows evenly comes out up to 2^-26 per product of 16 short
-  // (measured for bf16 operands, three times that for fp32's planes), always
+  // (measured for bf16 operands, three times that for fp16), always
   // towards zero. chain > 0 bounds each such sum to that many K = 64 steps (of
   // the last term's; the terms before it, smaller by 2^-8 and less, make one
   // more): the epilogue warps add it to the tile's fp32 sum in TMEM, rounded to
@@ -98,7 +98,7 @@ struct MmArgs {
   int sym;                  // C symmetric: tiles with n <= m only (square tiles)
   int fp16;                 // operands fp16 instead of bf16
   // products over planes: operand z coordinates (pa, pb) of n_terms passes
-  // over K, 4 bits each (fp32 operands in two fp16 planes, G in two of bf16)
+  // over K, 4 bits each (fp32 operands in three bf16 planes, G in two)
   int n_terms;
   uint32_t pa, pb;
   const int* m_dev;

@@ -24,11 +24,13 @@
 // order), the sizes of the products follow the device-side count, and rows
 // of ignored tokens are never read, so their values cannot reach dw.
 //
-// fp32: x, w and G are split into two fp16 planes each, hi + lo (22 bits), after
-// a power of two has brought the largest value of each below 2^15 (xent_amax;
-// an element keeps its 22 bits down to 2^-17 of the largest, and an error of
-// 2^-40 of it below), and every product sums lo hi + hi lo + hi hi. Three bf16
-// planes would need six products for 24 bits.
+// fp32: x, w and G are split into three bf16 planes each (24 bits, and fp32's
+// range), and every product sums the six plane products above 2^-24, smallest
+// first. Two fp16 planes and three products take two thirds of the time (step
+// of 2048 x 1024 x 8192: 345 us, these 538), but their 22 bits need a common
+// scale and end 2^-17 below the largest value of the matrix: entries of dw for
+// improbable words, small columns and rows of small upstream gradients lost
+// their bits.
 #include <math.h>
 
 #include <algorithm>
@@ -47,8 +49,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 128;  // columns per (max, sum) statistic
 
-// planes (1,0) (0,1) (0,0) of fp32's products; (1,.) (0,.) of G's two in bf16
-constexpr uint32_t kTermsA = 0x001u, kTermsB = 0x010u, kFineA = 0x01u;
+// fp32's plane products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0); (1,.) (0,.) of G's two in bf16
+constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u, kFineA = 0x01u;
 
 // Calls of few tokens have little to average an error over and time to spare: up
 // to kFineG tokens keep G in two bf16 planes (one plane's rounding of p - 1 is an
@@ -57,18 +59,13 @@ constexpr uint32_t kTermsA = 0x001u, kTermsB = 0x010u, kFineA = 0x01u;
 // planes, 127 in one), and up to kFine tokens' tensor-core sums are short chains
 // (MmArgs::chain): of 4 K = 64 steps for bf16 logits (the loss of 1 token at d = 2048: 2e-6 off
 // without chains, 4e-7 with; one token's time is the same, 129 tokens of V = 32000
-// would take 150 instead of 143 us), of 1 for fp32's three products. fp32's sums
-// always run in chains (d = 2048, 300 tokens: gradients 2.4e-6 off at 1024
-// products a sum, 7e-7 at 512), bf16 logits where they are longer than kChain
+// would take 150 instead of 143 us), of 1 for fp32's. fp32's sums
+// always run in chains (d = 2048, 300 tokens: gradients 1.4e-6 off at 1024
+// products a sum, 7e-7 at 512, in the same time), bf16 logits where they are longer than kChain
 // steps (losses of 1024 tokens, d = 2048: 1.0e-6 off in one sum, 5e-7 in two;
 // d = 1536: 7.7e-7 in one, and two would take 148 instead of 142 us for 2048
 // tokens).
 constexpr int kFineG = 16, kFine = 64, kFineChain = 4, kFineF32Chain = 1, kF32Chain = 8, kChain = 24;
-
-// fp32's powers of two: of x, w, G, and the inverses that undo them in x w^T,
-// G w and G^T x
-enum { kScX = 0, kScW, kScG, kUnXW, kUnGW, kUnGX, kScales };
-constexpr int kAmax = 256;  // partial maxima each of x, w and the rows' gradients
 
 // ---- first product: statistics and exponentials ----------------------------
 
@@ -85,7 +82,6 @@ struct EpiStats {
   void* p;             // exponentials of the rows, or null
   int64_t ldp;
   int p_f32;           // fp32 instead of fp16 * 2^15
-  const float* un;     // logit = accumulator * *un, or null
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
@@ -117,7 +113,7 @@ struct EpiStats {
     }
     // fmaxf drops NaN: a row of NaN leaves m at -inf, and the sums below carry it
     // (the maximum itself gives exactly 1: a difference, not a fused product)
-    const float mm = m == -INFINITY ? 0.f : m, f = un ? *un : 1.f, k = f * kLog2e;
+    const float mm = m == -INFINITY ? 0.f : m;
     float s0 = 0.f, s1 = 0.f;
     const int row0 = row - lane;
     const int64_t at = (int64_t)row0 * ldp + col0;
@@ -126,7 +122,7 @@ struct EpiStats {
       float v[32];
       load32(taddr + cc, zero, v);
 #pragma unroll
-      for (int q = 0; q < 32; ++q) v[q] = cc + q < nv ? fast_exp2((v[q] - mm) * k) : 0.f;
+      for (int q = 0; q < 32; ++q) v[q] = cc + q < nv ? fast_exp2((v[q] - mm) * kLog2e) : 0.f;
 #pragma unroll
       for (int q = 0; q < 32; q += 2) {
         s0 += v[q];
@@ -148,8 +144,8 @@ struct EpiStats {
     if (row_ok) {
       // every column -inf: nothing to add
       const float sum = s0 + s1;
-      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && sum == 0.f ? -INFINITY : mm * f, sum);
-      if ((unsigned)t < (unsigned)nv) lt[row] = tv * f;
+      stats[(int64_t)row * n_tiles + col0 / kTile] = make_float2(m == -INFINITY && sum == 0.f ? -INFINITY : mm, sum);
+      if ((unsigned)t < (unsigned)nv) lt[row] = tv;
     }
   }
 };
@@ -183,7 +179,6 @@ struct EpiScore {
   int n_tiles;
   const int64_t* targets;
   float* lt;
-  const float* un;  // as in EpiStats
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile w, int row, int col0, int M, uint32_t taddr,
@@ -194,7 +189,6 @@ struct EpiScore {
     load32(taddr, zero, v);
     const int64_t t = lane < n ? targets[col0 + lane] : -1;
     float2 mine = make_float2(0.f, 0.f);
-    const float f = un ? *un : 1.f, k = f * kLog2e;
     // (32000 rows of w, 32 tokens: 47 us one token at a time, 39 transposed; 1 token: 34)
     if (n <= 4) {
 #pragma unroll
@@ -202,7 +196,7 @@ struct EpiScore {
         if (q >= n) break;
         const float x = row < M ? v[q] : -INFINITY;
         const float m = warp_max(x), mm = m == -INFINITY ? 0.f : m;
-        const float s = warp_sum(row < M ? fast_exp2((x - mm) * k) : 0.f);
+        const float s = warp_sum(row < M ? fast_exp2((x - mm) * kLog2e) : 0.f);
         if (lane == q) mine = make_float2(m, s);
       }
     } else {
@@ -214,15 +208,15 @@ struct EpiScore {
 #pragma unroll
       for (int q = 0; q < 32; ++q) {
         const float mq = __shfl_sync(0xffffffffu, mm, q);  // (every lane takes part)
-        x[q] = row < M ? fast_exp2((v[q] - mq) * k) : 0.f;
+        x[q] = row < M ? fast_exp2((v[q] - mq) * kLog2e) : 0.f;
       }
       mine.y = warp_transposed(x, lane, [](float a, float b) { return a + b; });
     }
-    mine.x = mine.x == -INFINITY && mine.y != 0.f ? 0.f : mine.x * f;
+    mine.x = mine.x == -INFINITY && mine.y != 0.f ? 0.f : mine.x;
 #pragma unroll
     for (int q = 0; q < 32; ++q) {
       if (q >= n) break;
-      if (__shfl_sync(0xffffffffu, t, q) == row) lt[col0 + q] = v[q] * f;
+      if (__shfl_sync(0xffffffffu, t, q) == row) lt[col0 + q] = v[q];
     }
     if (lane < n) stats[(int64_t)(col0 + lane) * n_tiles + row / 32] = mine;
   }
@@ -243,14 +237,13 @@ struct EpiOut {
   int64_t ldacc;
   const int* idx;       // output row of row m, or null
   const int* count;     // the result is divided by max(1, *count), or null
-  const float* un;      // and multiplied by *un, or null
-  const float* factor;  // and by *factor, or null
+  const float* factor;  // and multiplied by *factor, or null
   const int64_t* zero;  // rows of out whose target, of zero_n, is `ignore` become zeros; or null
   int zero_n;
   int64_t ignore;
 
   __device__ __forceinline__ float scale() const {
-    return (count ? 1.f / (float)max(1, *count) : 1.f) * (un ? *un : 1.f) * (factor ? *factor : 1.f);
+    return (count ? 1.f / (float)max(1, *count) : 1.f) * (factor ? *factor : 1.f);
   }
   __device__ __forceinline__ void begin(int warp, int warps) const {
     if (!zero) return;
@@ -385,80 +378,20 @@ __device__ __forceinline__ bool vec_rows(const T* p, int64_t ld, int d) {
   return ld % 8 == 0 && d % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-// ---- fp32's scales: largest magnitudes of x (the rows that count), w and the
-// rows' gradients, in kAmax partial maxima each
-__global__ void __launch_bounds__(256) xent_amax(const float* __restrict__ x, int64_t ldx, int n, int d,
-                                                 const int64_t* __restrict__ targets, int64_t ignore,
-                                                 const float* __restrict__ w, int64_t ldw, int vocab,
-                                                 const float* __restrict__ grad_rows, float* __restrict__ part) {
-  __shared__ float red[8];
-  pdl_next();
-  pdl_wait();
-  const int what = blockIdx.x / kAmax, i = blockIdx.x % kAmax, lane = threadIdx.x % 32;
-  float m = 0.f;
-  if (what < 2) {
-    const float* p = what ? w : x;
-    const int64_t ld = what ? ldw : ldx, rows = what ? vocab : n;
-    for (int64_t r = i * 8 + threadIdx.x / 32; r < rows; r += 8 * kAmax) {
-      if (!what && targets[r] == ignore) continue;
-      if (vec_rows(p, ld, d)) {
-        const float4* q = reinterpret_cast<const float4*>(p + r * ld);
-#pragma unroll 8
-        for (int c = lane; c < d / 4; c += 32) {
-          const float4 v = q[c];
-          m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-      } else {
-#pragma unroll 8
-        for (int c = lane; c < d; c += 32) m = fmaxf(m, fabsf(p[r * ld + c]));
-      }
-    }
-  } else {
-    for (int64_t r = i * 256 + threadIdx.x; r < n; r += 256 * kAmax)
-      if (targets[r] != ignore) m = fmaxf(m, grad_rows ? fabsf(grad_rows[r]) : 1.f);
-  }
-  m = block_max<256>(m, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = m;
-}
-
-// the power of two that brings a largest magnitude into [2^14, 2^15); 1 for 0,
-// infinities and NaN
-__device__ __forceinline__ float scale_of(float amax) {
-  return amax > 0.f && amax < INFINITY ? ldexpf(1.f, min(100, max(-100, 14 - ilogbf(amax)))) : 1.f;
-}
-
-// The scales, from the partial maxima, for a whole CTA of 256 (sc: shared); the
-// grid's first CTA leaves them in memory for the kernels after it.
-__device__ __forceinline__ void load_scales(const float* __restrict__ part, float* sc, float* __restrict__ out) {
-  static_assert(kAmax == 256, "eight partials per lane");
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (warp < 3) {
-    const float4* p = reinterpret_cast<const float4*>(part + warp * kAmax);
-    const float4 v = p[lane], u = p[lane + 32];
-    const float m = warp_max(fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w))));
-    if (lane == 0) sc[warp] = scale_of(m);
-  }
-  __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    out[kScX] = sc[0];
-    out[kScW] = sc[1];
-    out[kScG] = sc[2];
-    out[kUnXW] = 1.f / sc[0] / sc[1];
-    out[kUnGW] = 1.f / sc[2] / sc[1];
-    out[kUnGX] = 1.f / sc[2] / sc[0];
+// fp32 pair -> three bf16 planes, whose sum is the value to 2^-24
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&o)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    o[k] = pack_bf16(a, b);
+    a -= __uint_as_float(o[k] << 16);
+    b -= __uint_as_float(o[k] & 0xffff0000u);
   }
 }
 
-// fp32 -> two fp16 planes
-__device__ __forceinline__ void split2(float v, __half& h, __half& l) {
-  h = __float2half_rn(v);
-  l = __float2half_rn(v - __half2float(h));
-}
-
-// A warp's row: dst = src (bf16, or two planes of fp32 times f), zeros from
-// column d to lds, or everywhere where src is null.
+// A warp's row: dst = src (bf16, or three planes of fp32), zeros from column d
+// to lds, or everywhere where src is null.
 template <typename T>
-__device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t lds, int64_t plane, bool vec, float f) {
+__device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t lds, int64_t plane, bool vec) {
   const int lane = threadIdx.x % 32;
   if (sizeof(T) == 2 && (vec || !src)) {  // d a multiple of 8, 16-byte aligned rows
 #pragma unroll 8
@@ -470,12 +403,11 @@ __device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t
 #pragma unroll 8
     for (int c = lane; c < d / 4; c += 32) {
       const float4 v = reinterpret_cast<const float4*>(src)[c];
-      const __half2 h0 = __floats2half2_rn(v.x * f, v.y * f), h1 = __floats2half2_rn(v.z * f, v.w * f);
-      const float2 y0 = __half22float2(h0), y1 = __half22float2(h1);
-      const __half2 l0 = __floats2half2_rn(v.x * f - y0.x, v.y * f - y0.y), l1 = __floats2half2_rn(v.z * f - y1.x, v.w * f - y1.y);
-      reinterpret_cast<uint2*>(dst)[c] = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
-      reinterpret_cast<uint2*>(dst + plane)[c] =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
+      uint32_t a[3], b[3];
+      split3(v.x, v.y, a);
+      split3(v.z, v.w, b);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) reinterpret_cast<uint2*>(dst + k * plane)[c] = make_uint2(a[k], b[k]);
     }
     return;
   }
@@ -485,10 +417,10 @@ __device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t
     if (sizeof(T) == 2) {
       dst[c] = __float2bfloat16_rn(v);
     } else {
-      __half h, l;
-      split2(v * f, h, l);
-      reinterpret_cast<__half*>(dst)[c] = h;
-      reinterpret_cast<__half*>(dst)[plane + c] = l;
+      uint32_t o[3];
+      split3(v, 0.f, o);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) reinterpret_cast<uint16_t*>(dst)[k * plane + c] = (uint16_t)o[k];
     }
   }
 }
@@ -496,14 +428,11 @@ __device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t
 // rows of a matrix, packed; one warp per row
 template <typename T>
 __global__ void __launch_bounds__(256) xent_pack(const T* __restrict__ x, int64_t ldx, int n, int d, bf16* __restrict__ xs,
-                                                 int64_t lds, int64_t plane, const float* __restrict__ amax, int which,
-                                                 float* __restrict__ scales) {
-  __shared__ float sc[3];
+                                                 int64_t lds, int64_t plane) {
   pdl_next();
   pdl_wait();
-  if (sizeof(T) == 4) load_scales(amax, sc, scales);
   const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d), sizeof(T) == 4 ? sc[which] : 1.f);
+  if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d));
 }
 
 // Before the products of a training call. Lists the tokens that count, in
@@ -521,18 +450,14 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
                                                  int per, int* __restrict__ idx, int* __restrict__ tgt,
                                                  float* __restrict__ lt, int* __restrict__ count, bf16* __restrict__ xs,
                                                  int64_t lds, int64_t plane, const T* __restrict__ w, int64_t ldw,
-                                                 bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w,
-                                                 const float* __restrict__ amax, float* __restrict__ scales) {
-  __shared__ float sc[3];
+                                                 bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w) {
   pdl_next();
   pdl_wait();
-  if (sizeof(T) == 4) load_scales(amax, sc, scales);
-  const float fx = sizeof(T) == 4 ? sc[kScX] : 1.f;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if ((int)blockIdx.x < n_w) {
     const bool v = vec_rows(w, ldw, d);
     for (int64_t r = (int64_t)blockIdx.x * 16 + warp; r < min(vocab, ((int)blockIdx.x + 1) * 16); r += 8)
-      pack_row<T>(w + r * ldw, d, wp + r * ldwp, ldwp, wplane, v, sizeof(T) == 4 ? sc[kScW] : 1.f);
+      pack_row<T>(w + r * ldw, d, wp + r * ldwp, ldwp, wplane, v);
     return;
   }
   __shared__ int red[2][8], pos[256];
@@ -585,8 +510,8 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
     __syncthreads();
     for (int k = warp; k < min(256, r1 - c0); k += 8) {
       const int64_t row = c0 + k;
-      if (pos[k] >= 0) pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec, fx);
-      if (row >= all) pack_row<T>(nullptr, d, xs + row * lds, lds, plane, vec, fx);
+      if (pos[k] >= 0) pack_row<T>(x + row * ldx, d, xs + pos[k] * lds, lds, plane, vec);
+      if (row >= all) pack_row<T>(nullptr, d, xs + row * lds, lds, plane, vec);
     }
   }
 }
@@ -656,24 +581,21 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
   if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
 }
 
-// What xent_rows leaves: bf16 in place of the fp16 exponentials, or two planes
-// hi + lo, apart from fp32 exponentials: bf16, or fp16 of G times its scale
-enum class GKind { kInPlace, kBf16s, kHalves };
-
 // One CTA per row of a piece (few rows: SHARES of them, along y, each a share
 // of the columns): joins the tiles, writes the row's loss and rewrites the
-// exponentials as G = g (p - onehot), g = 1 or grad_rows. Rows between the count and the next multiple
+// exponentials as G = g (p - onehot), g = 1 or grad_rows: in place, or, from fp32
+// exponentials, in two or three bf16 planes apart. Rows between the count and the next multiple
 // of 64 become zeros: the third product reads them. The last CTA of the last
 // piece to finish sums the losses (thread t those of index t mod 256, then
 // in thread order: the same bits whichever CTA it is).
-template <GKind KIND, int SHARES>
+template <int PLANES, int SHARES>
 __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stats, int n_tiles, int rows, int vocab,
                                                  int* __restrict__ count, int base, const int* __restrict__ idx,
                                                  const int* __restrict__ tgt, const float* __restrict__ lt,
                                                  const float* __restrict__ grad_rows, int mean, float* losses,
-                                                 void* __restrict__ p, int64_t ldp, void* __restrict__ planes,
-                                                 int64_t plane, const float* __restrict__ scales, float* __restrict__ loss) {
-  constexpr bool SPLIT = KIND != GKind::kInPlace;
+                                                 void* __restrict__ p, int64_t ldp, bf16* __restrict__ planes,
+                                                 int64_t plane, float* __restrict__ loss) {
+  constexpr bool SPLIT = PLANES > 1;
   extern __shared__ float xent_f[];  // [n_tiles]
   __shared__ float red[8];
   __shared__ int last;
@@ -687,7 +609,7 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
       const uint4 z = make_uint4(0, 0, 0, 0);
       for (int64_t c = blockIdx.y * 256 + threadIdx.x; c < ldp / 8; c += 256 * SHARES) {
         if (SPLIT) {
-          for (int k = 0; k < 2; ++k) reinterpret_cast<uint4*>(static_cast<bf16*>(planes) + k * plane + row * ldp)[c] = z;
+          for (int k = 0; k < PLANES; ++k) reinterpret_cast<uint4*>(planes + k * plane + row * ldp)[c] = z;
         } else {
           reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp)[c] = z;
         }
@@ -702,7 +624,6 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
   if (threadIdx.x == 0 && blockIdx.y == 0) losses[base + row] = row_loss(lse, lt[row]);
   float g = grad_rows ? grad_rows[idx[row]] : 1.f;
   if (t < 0) g = __int_as_float(0x7fc00000);
-  if (KIND == GKind::kHalves) g *= scales[kScG];
   // tile factors: g 2^(m_tile - lse)
   for (int i = threadIdx.x; i < n_tiles; i += 256) {
     const float m = st[i].x;
@@ -730,22 +651,12 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = v[q] * f - (c + q == t ? g : 0.f);
     if (SPLIT) {
-      uint32_t o[2][4];
+      uint32_t o[4][3];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float a = v[2 * q], b = v[2 * q + 1];
-        if (KIND == GKind::kHalves) {
-          o[0][q] = pack_half(a, b);
-          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&o[0][q]));
-          o[1][q] = pack_half(a - y.x, b - y.y);
-        } else {
-          o[0][q] = pack_bf16(a, b);
-          o[1][q] = pack_bf16(a - __uint_as_float(o[0][q] << 16), b - __uint_as_float(o[0][q] & 0xffff0000u));
-        }
-      }
+      for (int q = 0; q < 4; ++q) split3(v[2 * q], v[2 * q + 1], o[q]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        *reinterpret_cast<uint4*>(static_cast<bf16*>(planes) + k * plane + row * ldp + c) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+      for (int k = 0; k < PLANES; ++k)
+        *reinterpret_cast<uint4*>(planes + k * plane + row * ldp + c) = make_uint4(o[0][k], o[1][k], o[2][k], o[3][k]);
     } else {
       *reinterpret_cast<uint4*>(static_cast<bf16*>(p) + row * ldp + c) =
           make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
@@ -812,13 +723,12 @@ struct Plan {
   int elt, planes, gplanes, n_tiles, piece, n_pieces;
   int64_t ldx, ldw, ldp, ldd;
   size_t part_bytes;
-  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, g, amax, scales, acc, part, total;
+  size_t xs, ws, stats, lt, idx, tgt, count, losses, p, g, acc, part, total;
 };
 
 MmArgs base_args(const Plan& q, volatile unsigned* fault) {
   MmArgs p = {};
-  p.n_terms = q.f32 ? 3 : 1;
-  p.fp16 = q.f32;
+  p.n_terms = q.f32 ? 6 : 1;
   p.pa = q.f32 ? kTermsA : 0;
   p.pb = q.f32 ? kTermsB : 0;
   p.nz = 1;
@@ -864,9 +774,9 @@ Plan make_plan(const llattn_xent_args& a) {
   Plan q;
   q.f32 = a.dtype == LLATTN_F32;
   q.elt = q.f32 ? 4 : 2;
-  q.planes = q.f32 ? 2 : 1;
+  q.planes = q.f32 ? 3 : 1;
   q.train = a.dx || a.dw || a.stage != LLATTN_XENT_ALL;
-  q.gplanes = q.f32 || a.tokens <= kFineG ? 2 : 1;
+  q.gplanes = q.f32 ? 3 : a.tokens <= kFineG ? 2 : 1;
   q.pack_x = q.f32 || q.train || !aligned_rows(a.x, a.ldx, a.tokens, 2);
   q.pack_w = q.f32 || !aligned_rows(a.w, a.ldw, a.vocab, 2);
   q.ldx = q.pack_x ? up8(a.d) : (a.tokens == 1 ? up8(a.d) : a.ldx);
@@ -877,7 +787,8 @@ Plan make_plan(const llattn_xent_args& a) {
   q.n_tiles = cdiv(a.vocab, q.few ? 32 : kTile);
   // rows of exponentials held at a time: half a GiB of them (V = 32000 in
   // bf16: 8192 rows), whole row tiles
-  const int64_t row_bytes = q.gplanes == 2 ? q.ldp * 8 : q.ldp * 2;
+  const int p_bytes = q.gplanes > 1 ? 4 : 2;  // an exponential's
+  const int64_t row_bytes = q.ldp * (q.gplanes > 1 ? p_bytes + 2 * q.gplanes : p_bytes);
   const int64_t piece = std::max<int64_t>(256, (int64_t)(512u << 20) / row_bytes / 256 * 256);
   q.piece = (int)std::min<int64_t>(piece, a.tokens);
   if (!q.train) q.piece = a.tokens;
@@ -893,10 +804,8 @@ Plan make_plan(const llattn_xent_args& a) {
   q.tgt = take(q.train ? 4 * n : 0);
   q.count = take(8);
   q.losses = take(4 * n);
-  q.p = take(q.train ? (size_t)q.piece * q.ldp * 2 * q.gplanes : 0);
-  q.g = take(q.train && q.gplanes == 2 ? 4 * (size_t)q.piece * q.ldp : 0);
-  q.amax = take(q.f32 ? sizeof(float) * 3 * kAmax : 0);
-  q.scales = take(q.f32 ? sizeof(float) * kScales : 0);
+  q.p = take(q.train ? (size_t)q.piece * q.ldp * p_bytes : 0);
+  q.g = take(q.train && q.gplanes > 1 ? 2 * (size_t)q.gplanes * q.piece * q.ldp : 0);
   q.acc = take(q.train && a.dw && q.n_pieces > 1 ? 4 * (size_t)a.vocab * q.ldd : 0);
   int64_t part = 0;
   if (a.dx) part = mm_part_floats(dx_args(q, a, q.piece, nullptr));
@@ -928,20 +837,12 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   const bool mean = a.reduction == LLATTN_XENT_MEAN;
   const int64_t xplane = (int64_t)n * q.ldx, wplane = (int64_t)V * q.ldw;
   const void* wv = q.pack_w ? wp : a.w;
-  float* amax = reinterpret_cast<float*>(ws + q.amax);
-  float* scales = q.f32 ? reinterpret_cast<float*>(ws + q.scales) : nullptr;
-  auto un = [&](int i) { return scales ? scales + i : nullptr; };
-  if (q.f32 && !grads)
-    TRY(launch_pdl(xent_amax, dim3(3 * kAmax), 256, 0, 1, s, static_cast<const float*>(a.x), a.ldx, n, d, a.targets,
-                   a.ignore_index, static_cast<const float*>(a.w), a.ldw, V, a.grad_rows, amax));
   if (!q.train) {
     if (q.pack_w) {
-      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(V, 8)), 256, 0, 1, s, static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane,
-                     amax, (int)kScW, scales));
+      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(V, 8)), 256, 0, 1, s, static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane));
     }
     if (q.pack_x) {
-      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane,
-                     amax, (int)kScX, scales));
+      TRY(launch_pdl(xent_pack<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane));
     }
     MmArgs p = base_args(q, fault);
     const Operand ox{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0}, ow{wv, V, d, q.ldw, q.planes, wplane, 0};
@@ -951,11 +852,11 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       p.M = V;
       p.N = n;
       std::swap(p.pa, p.pb);
-      TRY(launch_mm_sh<0>(p, ow, ox, EpiScore{stats, q.n_tiles, a.targets, lt, un(kUnXW)}, s));
+      TRY(launch_mm_sh<0>(p, ow, ox, EpiScore{stats, q.n_tiles, a.targets, lt}, s));
     } else {
       p.M = n;
       p.N = V;
-      TRY(launch_mm(p, ox, ow, EpiStats{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0, un(kUnXW)}, s));
+      TRY(launch_mm(p, ox, ow, EpiStats{stats, q.n_tiles, nullptr, a.targets, lt, nullptr, 0, 0}, s));
     }
     float* losses = a.losses ? a.losses : reinterpret_cast<float*>(ws + q.losses);
     TRY(launch_pdl(xent_losses, dim3(n), 128, 0, 1, s, stats, q.n_tiles, lt, a.targets, a.ignore_index, V, losses));
@@ -968,10 +869,10 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   if (!grads)
     TRY(launch_pdl(xent_prep<T>, dim3(n_w + cdiv(n, per)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, d, a.targets, n,
                    a.ignore_index, V, per, idx, tgt, lt, count, xs, q.ldx, xplane, static_cast<const T*>(a.w), a.ldw, wp,
-                   q.ldw, wplane, n_w, amax, scales));
+                   q.ldw, wplane, n_w));
   float* losses = reinterpret_cast<float*>(ws + q.losses);
   void* pbuf = ws + q.p;
-  void* gpl = ws + q.g;
+  bf16* gpl = reinterpret_cast<bf16*>(ws + q.g);
   float* acc = reinterpret_cast<float*>(ws + q.acc);
   float* part = reinterpret_cast<float*>(grads ? static_cast<char*>(a.workspace) : ws + q.part);  // split tiles of one product at a time
   const int64_t gplane = (int64_t)q.piece * q.ldp;
@@ -985,7 +886,7 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
     p.N = V;
     p.K = d;
     p.chain = logits_chain(q, a);
-    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.gplanes == 2, un(kUnXW)};
+    EpiStats ep{stats, q.n_tiles, tgt + base, nullptr, lt + base, pbuf, q.ldp, q.gplanes > 1};
     if (!grads) TRY(launch_mm(p, ox, Operand{wv, V, d, q.ldw, q.planes, wplane, 0}, ep, s));
     const size_t sm = sizeof(float) * q.n_tiles;
     auto rows_pass = [&](auto kernel, int shares) {
@@ -994,23 +895,23 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
         if (e != cudaSuccess) return e;
       }
       return launch_pdl(kernel, dim3(rows, shares), 256, sm, 1, s, stats, q.n_tiles, rows, V, count, base, idx + base, tgt + base,
-                        lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, scales, c + 1 == q.n_pieces ? a.loss : nullptr);
+                        lt + base, a.grad_rows, mean, losses, pbuf, q.ldp, gpl, gplane, c + 1 == q.n_pieces ? a.loss : nullptr);
     };
     const bool share = rows <= 2 * sm_count() && V >= 4096;  // (129 rows of 32000: 12.7 -> 9.1 us)
-    auto rows_as = [&](auto kind) {
-      constexpr GKind kG = decltype(kind)::value;
-      return share ? rows_pass(xent_rows<kG, 4>, 4) : rows_pass(xent_rows<kG, 1>, 1);
+    auto rows_as = [&](auto planes) {
+      constexpr int P = decltype(planes)::value;
+      return share ? rows_pass(xent_rows<P, 4>, 4) : rows_pass(xent_rows<P, 1>, 1);
     };
     using std::integral_constant;
     if (grads) {
     } else if constexpr (sizeof(T) == 4) {
-      TRY(rows_as(integral_constant<GKind, GKind::kHalves>{}));
+      TRY(rows_as(integral_constant<int, 3>{}));
     } else if (q.gplanes == 2) {
-      TRY(rows_as(integral_constant<GKind, GKind::kBf16s>{}));
+      TRY(rows_as(integral_constant<int, 2>{}));
     } else {
-      TRY(rows_as(integral_constant<GKind, GKind::kInPlace>{}));
+      TRY(rows_as(integral_constant<int, 1>{}));
     }
-    const void* g = q.gplanes == 2 ? gpl : pbuf;
+    const void* g = q.gplanes > 1 ? gpl : pbuf;
     if (a.dx) {
       MmArgs m = dx_args(q, a, rows, fault);
       m.m_dev = count;
@@ -1027,7 +928,6 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.ignore = a.ignore_index;
       eo.idx = idx + base;
       eo.count = mean ? count : nullptr;
-      eo.un = un(kUnGW);
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.gplanes, gplane, 0}, Operand{wv, V, d, q.ldw, q.planes, wplane, 1}, eo,
                     s));
     }
@@ -1046,7 +946,6 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
       eo.acc = c && last ? acc : nullptr;
       eo.ldacc = q.ldd;
       eo.count = last && mean ? count : nullptr;
-      eo.un = last ? un(kUnGX) : nullptr;
       eo.factor = a.factor;
       TRY(launch_mm(m, Operand{g, rows, V, q.ldp, q.gplanes, gplane, 1}, Operand{ox.p, rows, d, q.ldx, q.planes, xplane, 1},
                     eo, s));
@@ -1065,9 +964,9 @@ size_t workspace_bytes(const llattn_xent_args& a) {
 
 int launches(const llattn_xent_args& a) {
   const Plan q = make_plan(a);
-  if (!q.train) return q.f32 + q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
+  if (!q.train) return q.pack_w + q.pack_x + 2 + (a.loss ? 1 : 0);
   const int loss = a.stage == LLATTN_XENT_GRADS ? 0 : 1;
-  return loss * (q.f32 + 1) + q.n_pieces * (2 * loss + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
+  return loss + q.n_pieces * (2 * loss + (a.dx ? 1 + joins(dx_args(q, a, q.piece, nullptr)) : 0) +
                            (a.dw ? 1 + joins(dw_args(q, a, q.piece, nullptr)) : 0));
 }
 
