@@ -53,10 +53,10 @@ constexpr int kTile = 128;  // columns per (max, sum) statistic
 constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u, kFineA = 0x01u;
 
 // Calls of few tokens have little to average an error over and time to spare: up
-// to kFineG tokens keep G in two bf16 planes (one plane's rounding of p - 1 is an
+// to kFine tokens keep G in two bf16 planes (one plane's rounding of p - 1 is an
 // error of the whole row, up to 1.5 times the output's own rounding for a
-// single token, 1.2 times over some tens; 20 tokens of V = 32000: 148 us in two
-// planes, 127 in one), and up to kFine tokens' tensor-core sums are short chains
+// single token, 1.2 times over some tens; 20 tokens of V = 32000: 155 us in two
+// planes, 127 in one), and their tensor-core sums are short chains
 // (MmArgs::chain): of 4 K = 64 steps for bf16 logits (the loss of 1 token at d = 2048: 2e-6 off
 // without chains, 4e-7 with; one token's time is the same, 129 tokens of V = 32000
 // would take 150 instead of 143 us), of 1 for fp32's. fp32's sums
@@ -65,7 +65,7 @@ constexpr uint32_t kTermsA = 0x010120u, kTermsB = 0x001102u, kFineA = 0x01u;
 // steps (losses of 1024 tokens, d = 2048: 1.0e-6 off in one sum, 5e-7 in two;
 // d = 1536: 7.7e-7 in one, and two would take 148 instead of 142 us for 2048
 // tokens).
-constexpr int kFineG = 16, kFine = 64, kFineChain = 4, kFineF32Chain = 1, kF32Chain = 8, kChain = 24;
+constexpr int kFine = 64, kFineChain = 4, kFineF32Chain = 1, kF32Chain = 8, kChain = 24;
 
 // ---- first product: statistics and exponentials ----------------------------
 
@@ -776,7 +776,7 @@ Plan make_plan(const llattn_xent_args& a) {
   q.elt = q.f32 ? 4 : 2;
   q.planes = q.f32 ? 3 : 1;
   q.train = a.dx || a.dw || a.stage != LLATTN_XENT_ALL;
-  q.gplanes = q.f32 ? 3 : a.tokens <= kFineG ? 2 : 1;
+  q.gplanes = q.f32 ? 3 : a.tokens <= kFine ? 2 : 1;
   q.pack_x = q.f32 || q.train || !aligned_rows(a.x, a.ldx, a.tokens, 2);
   q.pack_w = q.f32 || !aligned_rows(a.w, a.ldw, a.vocab, 2);
   q.ldx = q.pack_x ? up8(a.d) : (a.tokens == 1 ? up8(a.d) : a.ldx);

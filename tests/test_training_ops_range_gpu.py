@@ -110,3 +110,13 @@ def test_one_bad_token_leaves_the_others_precise(dtype):
         dx, _ = torch.autograd.grad(linear_cross_entropy(xr, wr, t, reduction="none"), (xr, wr), g)
         assert not torch.isfinite(dx[7]).all()
         assert ((dx.double() - rdx).norm(dim=1) <= tol * rdx.norm(dim=1))[keep].all(), what
+
+@pytest.mark.parametrize("n", [17, 33, 64])
+def test_few_tokens_round_once(n):
+    """bf16, up to 64 tokens: a row of dx is off by its own rounding, 2^-9 of each
+    entry, and what G's two planes leave (2^-17): no token's row by more."""
+    x, w, t = make(n, 264, 2000, BF)
+    _, dx, dw = run(x, w, t)
+    _, rdx, rdw = plain(x, w, t)
+    assert ((dx.double() - rdx).norm(dim=1) <= (2**-9 + 2**-15) * rdx.norm(dim=1)).all()
+    assert rel(dw, rdw) <= 2**-9 + 2**-15
