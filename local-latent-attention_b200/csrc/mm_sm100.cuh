@@ -911,15 +911,22 @@ double mm_time(const MmArgs& p) {
   return t + tail;
 }
 
-// fp32 elements of MmArgs::part for a product of at most these sizes
-inline int64_t mm_part_floats(const MmArgs& p) {
-  if (!p.split) return 0;
-  // mm_plan's cap: 4 waves of ranges
-  return 4 * std::max({mm_units(3) * 256 * 512, mm_units(2) * 256 * 256, mm_units(1) * 128 * 128});
-}
-
 // whether mm_plan may split anything, whatever the device-side counts
 inline bool joins(const MmArgs& p) { return p.split && cdiv(p.K, 64) >= 16; }
+
+// fp32 elements of MmArgs::part for a product of at most these sizes: mm_plan
+// splits fewer tiles than units, each into as many ranges as K's steps allow
+// (32 at most), 4 waves of ranges at most
+template <int SH>
+int64_t mm_part_blocks(const MmArgs& p) {
+  const int64_t tiles = (int64_t)cdiv(p.M, MmShape<SH>::BM) * cdiv(p.N, MmShape<SH>::BN) * std::max(p.nz, 1);
+  const int64_t units = mm_units(SH), ranges = std::min(32, cdiv(p.K, 64) / 8);
+  return std::min(4 * units, std::min(tiles, units - 1) * ranges) * MmShape<SH>::BM * MmShape<SH>::BN;
+}
+inline int64_t mm_part_floats(const MmArgs& p) {
+  if (!joins(p)) return 0;
+  return std::max({mm_part_blocks<0>(p), mm_part_blocks<1>(p), mm_part_blocks<2>(p), mm_part_blocks<3>(p), mm_part_blocks<4>(p)});
+}
 
 template <int SH, typename Epi>
 cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t s, decltype(&Epi::quad)) {
@@ -963,7 +970,7 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
   p.b_mn = b.mn;
   if (p.nz < 1) p.nz = 1;
   if (p.n_terms < 1) p.n_terms = 1;
-  if (p.M < 1 || p.N < 1 || p.K < 1 || (p.split && !p.part)) return cudaErrorInvalidValue;
+  if (p.M < 1 || p.N < 1 || p.K < 1 || (joins(p) && !p.part)) return cudaErrorInvalidValue;
   const double t2 = mm_time<2>(p), t1 = mm_time<1>(p);
   if constexpr (Epi::kNarrow) {
     MmArgs q = p;

@@ -4,6 +4,8 @@ linear_cross_entropy hands to the C calls, with stand-ins for them."""
 import contextlib
 import ctypes
 import gc
+import math
+import random
 
 import pytest
 import torch
@@ -103,3 +105,54 @@ def test_backward_computes_again_what_does_not_fit_its_inputs(calls, monkeypatch
                         lambda self, ref: 256 if ref._obj.stage == _lib.XENT_GRADS else 2 * KEPT)
     loss.backward()
     assert [c[0] for c in calls] == ["loss", "loss", "grads"] and calls[2][1] == calls[1][1] and calls[2][2]
+
+
+# --- workspaces, from the host --------------------------------------------------
+
+def sizes(n, d, v, dtype=_lib.BF16, stage=_lib.XENT_GRADS):
+    outs = dict(loss=None, dx=1 << 21, dw=1 << 22, kept=1 << 23) if stage == _lib.XENT_GRADS else dict(dx=1 << 21, dw=1 << 22)
+    a = _lib.XentArgs(n, d, v, dtype, _lib.XENT_MEAN, -100, 1 << 24, d, 1 << 25, d, 1 << 26, None, None)
+    for k, val in {**outs, "stage": stage}.items():
+        setattr(a, k, val)
+    return _lib.lib().llattn_xent_workspace_bytes(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("dtype", [_lib.BF16, _lib.F32])
+def test_small_calls_take_small_workspaces(dtype):
+    """Nothing is reserved for sums that no product of these sizes splits."""
+    assert sizes(1, 64, 97, dtype) <= 256 and sizes(512, 128, 128, dtype) <= 256
+    assert sizes(1, 64, 97, dtype, _lib.XENT_ALL) <= 1 << 18
+    assert sizes(512, 128, 128, dtype, _lib.XENT_ALL) <= 3 << 20  # 512 x 128 of x in planes, exponentials, G
+
+
+SHAPES = {0: (128, 32), 1: (128, 128), 2: (256, 256), 3: (256, 512), 4: (128, 64)}
+
+
+def split_bytes(m, n, k, shape, sms=148):
+    """Partial sums of the product's last wave (mm_plan's rule)."""
+    bm, bn = SHAPES[shape]
+    units = sms // 2 if shape in (2, 3) else sms
+    total, steps = -(-m // bm) * -(-n // bn), -(-k // 64)
+    tail = total % units
+    block = 205 * (bm * bn // 1024) // 64
+    best, cost = 1, None
+    for s in range(1, 33):
+        if s > 1 and (steps < 8 * s or tail * s > 4 * units):
+            break
+        c = 1024 * -(-tail * s // units) * (-(-steps // s) + 6) + (block * tail * s if s > 1 else 0)
+        if cost is None or c < cost:
+            best, cost = s, c
+    return 4 * bm * bn * tail * best if best > 1 else 0
+
+
+def test_workspace_holds_every_split():
+    """Whatever the shape that a product runs in and however few tokens count (the
+    device cuts dx's rows and dw's sums to them)."""
+    rng = random.Random(0)
+    for _ in range(300):
+        n, d, v = (int(math.exp(rng.uniform(math.log(a), math.log(b)))) for a, b in ((1, 8000), (1, 5000), (1, 32000)))
+        have = sizes(n, d, v)
+        for counted in {0, 1, n, n // 2, rng.randint(0, n), rng.randint(0, n)}:
+            for shape in SHAPES:
+                assert split_bytes(counted, d, v, shape) <= have, (n, d, v, counted, shape)
+                assert split_bytes(v, d, counted, shape) <= have, (n, d, v, counted, shape)
