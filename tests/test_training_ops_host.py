@@ -9,6 +9,7 @@ import random
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.utils.checkpoint import checkpoint
 
 import llattn_b200
@@ -105,6 +106,28 @@ def test_backward_computes_again_what_does_not_fit_its_inputs(calls, monkeypatch
                         lambda self, ref: 256 if ref._obj.stage == _lib.XENT_GRADS else 2 * KEPT)
     loss.backward()
     assert [c[0] for c in calls] == ["loss", "loss", "grads"] and calls[2][1] == calls[1][1] and calls[2][2]
+
+
+# --- who watches -----------------------------------------------------------------
+
+def fake_case(grads=False):
+    f = lambda *s: torch.empty(*s, device="cuda", dtype=torch.bfloat16, requires_grad=grads)
+    return f(6, 16), f(10, 16), torch.empty(6, dtype=torch.int64, device="cuda")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_fake_tensors_go_through_the_custom_ops(reduction):
+    with FakeTensorMode():
+        x, w, t = fake_case()
+        out = llattn_b200.linear_cross_entropy(x, w, t, reduction=reduction)
+        assert out.shape == ((6,) if reduction == "none" else ()) and out.dtype == torch.float32
+        x, w, t = fake_case(True)
+        out = llattn_b200.linear_cross_entropy(x, w, t, reduction=reduction)
+        assert out.requires_grad
+        g = llattn_b200.newton_schulz(fake_case()[0].float())
+        assert g.shape == (6, 16) and g.dtype == torch.bfloat16
+        for o, shape in zip(llattn_b200.newton_schulz([x, w, x]), ((6, 16), (10, 16), (6, 16))):
+            assert o.shape == shape and o.dtype == torch.bfloat16
 
 
 # --- workspaces, from the host --------------------------------------------------

@@ -5,9 +5,12 @@ import math
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.checkpoint import checkpoint
 
-from llattn_b200 import linear_cross_entropy
+from llattn_b200 import linear_cross_entropy, newton_schulz
 from test_training_ops_gpu import BF, FP, make
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +74,48 @@ def test_weight_gathered_again_elsewhere(dtype):
     del held
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+class Seen(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_dispatch_modes_see_the_operators(reduction):
+    """Counters and tracers see a custom op, forward and backward; results as without them (fp32: an upstream
+    gradient of 1 rounds nowhere)."""
+    x, w, t = make(90, 64, 256, FP, ignored=0.1)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    f = lambda: gradients(linear_cross_entropy(x, w, t, reduction=reduction).sum(), x, w)
+    want = f()
+    with Seen() as seen:
+        got = f()
+    ours = [n for n in seen.names if n.startswith("llattn_b200.")]
+    assert any(n.startswith("llattn_b200.linear_xent") for n in ours) and (reduction == "mean" or len(ours) == 2)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    g = torch.randn(48, 80, device="cuda")
+    with Seen() as seen:
+        outs = newton_schulz([g, g])
+    assert any(n.startswith("llattn_b200.newton_schulz") for n in seen.names)
+    assert torch.equal(outs[1], newton_schulz(g))
+
+
+def test_fake_and_traced_gradients():
+    with FakeTensorMode():
+        x = torch.empty(6, 16, device="cuda", requires_grad=True)
+        w = torch.empty(10, 16, device="cuda", requires_grad=True)
+        t = torch.empty(6, dtype=torch.int64, device="cuda")
+        for reduction in ("mean", "none"):
+            dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, t, reduction=reduction).sum(), (x, w))
+            assert dx.shape == x.shape and dw.shape == w.shape
+    x, w, t = make(20, 16, 40, FP)
+    f = lambda x, w: linear_cross_entropy(x, w, t)
+    graph = make_fx(f)(x, w)
+    assert "llattn_b200.linear_xent" in graph.code and torch.equal(graph(x, w), f(x, w))
