@@ -281,7 +281,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
     returns, differentiable in x and weight.
 
     x [..., d] and weight [vocab, d], both bfloat16 or both float32 (under
-    autocast both are cast to its dtype, as a linear layer's are); targets
+    autocast both are cast to its dtype, as a linear layer's are, or to float32
+    where that is float16); targets
     [...] int64. Products are summed in fp32; the gradients come back in the
     inputs' dtype. reduction: "mean" over the tokens whose target is not
     ignore_index (0 when there is none), "sum", or "none" (losses [...] fp32,
@@ -301,6 +302,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
         _require(False, f"targets {tuple(targets.shape)} must have x's leading shape {tuple(x.shape[:-1])}")
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
+        dt = torch.float32 if dt == torch.float16 else dt  # (no fp16 kernels)
         x, weight = x.to(dt), weight.to(dt)
     flat = x.dim() == 2
     x2, t = (x, targets) if flat else (x.reshape(-1, x.shape[-1]), targets.reshape(-1))

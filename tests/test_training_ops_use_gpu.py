@@ -11,6 +11,7 @@ from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.checkpoint import checkpoint
 
 from llattn_b200 import linear_cross_entropy, newton_schulz
+from llattn_b200.lm import LocalLatentLM, ModelConfig
 from test_training_ops_gpu import BF, FP, make
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +120,28 @@ def test_fake_and_traced_gradients():
     f = lambda x, w: linear_cross_entropy(x, w, t)
     graph = make_fx(f)(x, w)
     assert "llattn_b200.linear_xent" in graph.code and torch.equal(graph(x, w), f(x, w))
+
+
+def test_autocast_in_fp16_takes_fp32():
+    x, w, t = make(90, 64, 256, FP, ignored=0.1)
+    xh, wr = x.half().requires_grad_(True), w.half().float().requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.float16):
+        loss = linear_cross_entropy(xh, wr, t)
+    dx, dw = torch.autograd.grad(loss, (xh, wr))
+    full = gradients(linear_cross_entropy(xf := xh.detach().float().requires_grad_(True), wr, t), xf, wr)
+    assert torch.equal(loss, full[0]) and torch.equal(dw, full[2]) and torch.equal(dx, full[1].half())
+
+
+def test_fused_loss_under_fp16_autocast_follows_the_plain_head():
+    """The LM's head with a gradient scaler's autocast: fp16 logits in the plain head
+    (2^-11 of logits below 8: 4e-3 of the loss at most)."""
+    torch.manual_seed(0)
+    m = LocalLatentLM(ModelConfig(vocab_size=512, max_seq_len=128, d_model=256, n_heads=2, n_layers=1, d_ff=512, local_window=64,
+                                  latent_tokens=8, latent_d_model=64, latent_heads=2)).cuda()
+    h, t = torch.randn(2, 64, 256, device="cuda"), torch.randint(0, 512, (2, 64), device="cuda")
+    got = {}
+    for fused in (False, True):
+        m.fused_loss = fused
+        with torch.autocast("cuda", dtype=torch.float16):
+            got[fused] = m.loss_head(h, t).item()
+    assert abs(got[True] - got[False]) <= 4e-3 * got[False]
