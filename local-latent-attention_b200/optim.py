@@ -25,10 +25,13 @@ class Muon(torch.optim.Optimizer):
                              f"steps={steps}")
         super().__init__(params, dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps,
                                       coefficients=tuple(coefficients)))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2:
-                    raise ValueError(f"Muon updates matrices; got a parameter of shape {tuple(p.shape)}")
+
+    def add_param_group(self, group: dict) -> None:
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon updates matrices; got a parameter of shape {tuple(p.shape)}")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -56,19 +59,52 @@ class Muon(torch.optim.Optimizer):
         return loss
 
 
-class OptimizerPair:
-    """Optimisers over disjoint parameters that step together."""
+class OptimizerPair(torch.optim.Optimizer):
+    """Optimisers over disjoint parameters that step together, as one optimiser:
+    its groups and states are theirs, so that schedulers and gradient scalers
+    take it. state_dict is the list of theirs. Groups are added to one of them."""
 
     def __init__(self, *optimizers: torch.optim.Optimizer) -> None:
         self.optimizers = optimizers
+        self._made = False
+        super().__init__([g for o in optimizers for g in o.param_groups], {})
+        self._made = True
 
+    # the base class's own copies are never set: a loaded optimiser has new ones
     @property
     def param_groups(self) -> list[dict]:
         return [g for o in self.optimizers for g in o.param_groups]
 
-    def step(self) -> None:
+    @param_groups.setter
+    def param_groups(self, groups) -> None:
+        pass
+
+    @property
+    def state(self) -> dict:
+        return {p: s for o in self.optimizers for p, s in o.state.items()}
+
+    @state.setter
+    def state(self, state) -> None:
+        pass
+
+    def add_param_group(self, group: dict) -> None:
+        if self._made:
+            raise RuntimeError("OptimizerPair: add the group to one of its optimizers")
+
+    def __getstate__(self) -> dict:
+        return {"optimizers": self.optimizers}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__init__(*state["optimizers"])
+
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         for o in self.optimizers:
             o.step()
+        return loss
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for o in self.optimizers:
