@@ -32,6 +32,9 @@
 #include <math.h>
 
 #include <algorithm>
+#include <array>
+#include <map>
+#include <mutex>
 
 #include "mm_sm100.cuh"
 #include "xent.cuh"
@@ -646,25 +649,66 @@ __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Pt
   cluster.sync();  // the others have read this CTA's parts
 }
 
+template <typename T>
+cudaError_t small_attributes(int smem, int cl) {
+  cudaError_t e = set_smem_once(orth_small<T>, smem);
+  if (e == cudaSuccess && cl > 8) e = cudaFuncSetAttribute(orth_small<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
+}
+
+// Whether the current device can hold a cluster of cl CTAs with that much
+// shared memory (a partition of a GPU may not). Asked once per device and form.
+template <typename T>
+bool cluster_fits(int cl, int smem) {
+  static std::mutex mu;
+  static std::map<std::array<int, 3>, bool> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  const std::array<int, 3> key{dev, cl, smem};
+  std::lock_guard<std::mutex> lock(mu);
+  const auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cl);
+  cfg.blockDim = dim3(kSmallT);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim = {(unsigned)cl, 1, 1};
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (small_attributes<T>(smem, cl) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, orth_small<T>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return known[key] = n > 0;
+}
+
 // CTAs per matrix of the one-launch form (more than 8 need an opt-in), 0 where
-// it does not apply. Slices of at most 128 columns: one column tile per warp.
+// it does not apply: as many as give slices of 128 columns, one column tile per
+// warp, or the most that fit the device, 16 at most, with wider slices.
 int small_cluster(const llattn_orth_args& a) {
   const int q = std::min(a.rows, a.cols), L = std::max(a.rows, a.cols);
   if (q > kSmallQ) return 0;
   int cl = 1;
   while (cl < 16 && L > 128 * cl) cl *= 2;
-  return SmallShape(q, L, cl).bytes() <= 220 * 1024 ? cl : 0;
+  for (; cl >= 1; cl /= 2) {
+    const int smem = SmallShape(q, L, cl).bytes();
+    if (smem > 220 * 1024) return 0;
+    if (a.dtype == LLATTN_F32 ? cluster_fits<float>(cl, smem) : cluster_fits<bf16>(cl, smem)) return cl;
+  }
+  return 0;
 }
 
 template <typename T>
 cudaError_t run_small(const llattn_orth_args& a, int cl, cudaStream_t st) {
   const int smem = SmallShape(std::min(a.rows, a.cols), std::max(a.rows, a.cols), cl).bytes();
-  cudaError_t e = set_smem_once(orth_small<T>, smem);
+  cudaError_t e = small_attributes<T>(smem, cl);
   if (e != cudaSuccess) return e;
-  if (cl > 8) {
-    e = cudaFuncSetAttribute(orth_small<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
   for (int i0 = 0; i0 < a.count; i0 += kPtrs) {
     const int cnt = std::min(kPtrs, a.count - i0);
     Ptrs g;

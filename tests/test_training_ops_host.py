@@ -179,3 +179,15 @@ def test_workspace_holds_every_split():
             for shape in SHAPES:
                 assert split_bytes(counted, d, v, shape) <= have, (n, d, v, counted, shape)
                 assert split_bytes(v, d, counted, shape) <= have, (n, d, v, counted, shape)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a device whose clusters fit")
+@pytest.mark.parametrize("rows,cols", [(8, 8), (64, 300), (64, 1536), (3000, 48)])
+def test_matrices_without_a_cluster_get_the_general_kernels(rows, cols):
+    """Where a matrix's cluster of CTAs does not fit the device (here there is
+    none), the call is planned for the kernels that need no cluster."""
+    for dtype in (_lib.BF16, _lib.F32):
+        ptrs = (ctypes.c_void_p * 1)(1 << 20)
+        a = _lib.OrthArgs(rows, cols, 1, 5, dtype, 3.4, -4.7, 2.0, 1e-7, ptrs, 1 << 21, None, 0)
+        up = (cols + 7) // 8 * 8
+        assert _lib.lib().llattn_orth_workspace_bytes(ctypes.byref(a)) >= 3 * 2 * rows * up
