@@ -49,6 +49,12 @@ constexpr float kX = 64.f, kS = 256.f;  // scales of X and of S, B
 constexpr int kFolded = 2;              // last steps that hold B + a I
 constexpr int kParts = 64;              // partial sums of squares per matrix
 constexpr int kPtrs = 64;               // matrices per conversion launch
+// Gram sums of more than kLong K = 64 steps run in chains of kGramChain (MmArgs::chain).
+// In one sum they come out up to 3 x 2^-26 per 16 products short, 5e-5 at the
+// limit and 6e-4 of all of S at 200000, which five steps' polynomials make
+// several times that (a flat 1 x 200000: 4.1e-3 of the result, 2.2e-3 in chains;
+// 5 x 300000 3.6e-3 and 2.8e-3, in the same time).
+constexpr int kLong = 256, kGramChain = 64;
 
 struct Ptrs {
   const void* p[kPtrs];
@@ -67,7 +73,7 @@ __device__ __forceinline__ void store_symmetric(__half* base, int64_t ld, bool m
 
 // S = X X^T (scaled by kS), from hi * 2^6 (or the first step's G * 2^e)
 struct EpiGram {
-  static constexpr bool kNarrow = true, kWide = false, kChain = false, kBegin = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = true, kBegin = false;
   struct Pre {};
   __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
   __half* s;
@@ -799,9 +805,11 @@ cudaError_t run(const llattn_orth_args& a, const Plan& p, volatile unsigned* fau
       gm.M = gm.N = p.q;
       gm.K = p.tall ? m : n;
       gm.sym = 1;
+      gm.chain = cdiv(gm.K, 64) > kLong ? kGramChain : 0;
       const Operand& og = p.tall ? on : ok;
       TRY(launch_mm(gm, og, og, EpiGram{S, p.ldb, p.bz, sc}, st));
       gm.K = p.q;
+      gm.chain = 0;
       const Operand os{S, p.q, p.q, p.ldb, cnt, p.bz, 0}, ob{B, p.q, p.q, p.ldb, cnt, p.bz, 0};
       TRY(launch_mm(gm, os, os, EpiPoly{S, B, p.ldb, p.bz, a.b, a.c / kS, folded ? a.a * kS : 0.f}, st));
       MmArgs um = ma;

@@ -35,3 +35,13 @@ def test_past_one_launch(m, n, dtype):
     gs = [spectrum(m, n, d, dtype, i) for i, d in enumerate((0.0, 0.7))]
     for g, o in zip(gs, newton_schulz(gs)):
         assert rel(o, plain_ns(g)) <= 4e-3
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("m,n", [(1, 200000), (16, 100000), (300000, 5), (70, 150000)])
+def test_long_sums(m, n, dtype):
+    """Gram sums over hundreds of thousands of products: what the tensor cores'
+    additions drop does not grow with the length."""
+    gs = [spectrum(m, n, d, dtype, i) for i, d in enumerate((0.0, 0.7))]
+    for g, o in zip(gs, newton_schulz(gs)):
+        assert rel(o, plain_ns(g)) <= 4e-3
