@@ -10,9 +10,9 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.checkpoint import checkpoint
 
-from llattn_b200 import linear_cross_entropy, newton_schulz
+from llattn_b200 import _lib, linear_cross_entropy, newton_schulz
 from llattn_b200.lm import LocalLatentLM, ModelConfig
-from test_training_ops_gpu import BF, FP, make
+from test_training_ops_gpu import BF, FP, make, plain, rel, spectrum
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +145,141 @@ def test_fused_loss_under_fp16_autocast_follows_the_plain_head():
         with torch.autocast("cuda", dtype=torch.float16):
             got[fused] = m.loss_head(h, t).item()
     assert abs(got[True] - got[False]) <= 4e-3 * got[False]
+
+
+# --- gradients that are made with the loss and scaled in the backward -------------
+
+# bf16: G's rounding, the stored gradient's and the scaled one's, each 2^-9 at most
+THREE = 3 * 2**-9
+PIECES = {BF: (8500, 65, 32771), FP: (1700, 65, 32771)}  # tokens past what is held at a time; V d odd
+
+
+def pieces_case(dtype):
+    n, d, v = PIECES[dtype]
+    x, w, t = make(n, d, v, dtype, ignored=0.1)
+    return x.requires_grad_(True), w.requires_grad_(True), t
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_several_pieces_with_an_upstream_gradient(dtype):
+    x, w, t = pieces_case(dtype)
+    _, rdx, rdw = plain(x, w, t)
+    tol = THREE if dtype == BF else 1e-5
+    for factor in (-1.7, 0.0, 1.0):
+        dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, t) * factor, (x, w))
+        if factor == 0.0:
+            assert not dx.any() and not dw.any()
+            continue
+        assert rel(dx, rdx * factor) <= tol and rel(dw, rdw * factor) <= tol
+        assert not dx[t == -100].any()
+    # (the last one's: factor 1) only one of them wanted
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, w.detach(), t), x)[0], dx)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x.detach(), w, t), w)[0], dw)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_several_pieces_twice_through_a_retained_graph(dtype):
+    x, w, t = pieces_case(dtype)
+    loss = linear_cross_entropy(x, w, t)
+    first = [g.clone() for g in torch.autograd.grad(loss * -1.7, (x, w), retain_graph=True)]
+    again = [g.clone() for g in torch.autograd.grad(loss * -1.7, (x, w), retain_graph=True)]
+    other = torch.autograd.grad(loss * 0.5, (x, w))
+    plain_ones = torch.autograd.grad(linear_cross_entropy(x, w, t), (x, w))
+    for a, b, c, p in zip(first, again, other, plain_ones):
+        assert torch.equal(a, b) and torch.equal(c, p * 0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_several_pieces_under_hooks_and_checkpoints(dtype):
+    x, w, t = pieces_case(dtype)
+    f = lambda x, w: linear_cross_entropy(x, w, t)
+    want = gradients(f(x, w) * 0.7, x, w)
+    with torch.autograd.graph.save_on_cpu():
+        offloaded = f(x, w)
+    for loss in (offloaded, checkpoint(f, x, w, use_reentrant=False)):
+        held = churn()
+        for a, b in zip(gradients(loss * 0.7, x, w), want):
+            assert torch.equal(a, b)
+        del held
+
+
+def test_bad_target_in_a_later_piece():
+    x, w, t = pieces_case(BF)
+    t[8400] = 32771
+    loss = linear_cross_entropy(x, w, t)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert math.isnan(loss.item()) and dx[8400].isnan().all() and dw.isnan().any()
+    ok = torch.arange(8500, device="cuda") != 8400
+    assert torch.isfinite(dx[ok]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_compiled_gradients_with_an_upstream_gradient(dtype):
+    x, w, t = make(90, 64, 256, dtype, ignored=0.1)
+    _, rdx, rdw = plain(x, w, t)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    step = torch.compile(lambda x, w: linear_cross_entropy(x, w, t) * -1.7, backend="aot_eager", fullgraph=True)
+    dx, dw = torch.autograd.grad(step(x, w), (x, w))
+    tol = THREE if dtype == BF else 1e-5
+    assert rel(dx, rdx * -1.7) <= tol and rel(dw, rdw * -1.7) <= tol
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("na,nb,off", [(1, 0, 0), (7, 3, 0), (4096, 5, 0), (100003, 77, 0), (1000, 999, 1), (100003, 100003, 3)])
+def test_scale(dtype, na, nb, off):
+    """llattn_scale: whole chunks and tails, bases without 16-byte alignment, a factor of 1; the elements around stay."""
+    code = _lib.BF16 if dtype == BF else _lib.F32
+    for factor in (-1.7, 0.0, 1.0):
+        a, b = (torch.randn(off + m + 9, device="cuda").to(dtype) for m in (na, nb))
+        f = torch.tensor(factor, device="cuda")
+        want = [v.clone() for v in (a, b)]
+        for v, m in zip(want, (na, nb)):
+            v[off:off + m] = (v[off:off + m].float() * f).to(dtype)
+        s = torch.cuda.current_stream().cuda_stream
+        _lib.check(_lib.lib().llattn_scale(a[off:].data_ptr(), na, b[off:].data_ptr(), nb, code, f.data_ptr(), s), "llattn_scale")
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
+# --- CUDA graphs -------------------------------------------------------------------
+
+def replayed(f):
+    """f in a CUDA graph: what it returns, filled by each replay."""
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            f()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = f()
+    return graph, outs
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n,d,v", [(40, 64, 256), (500, 264, 5003)])
+def test_loss_in_a_cuda_graph(n, d, v, dtype):
+    x, w, t = make(n, d, v, dtype, ignored=0.1)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    per = lambda: linear_cross_entropy(x.detach(), w.detach(), t, reduction="none")
+    step = lambda: (*gradients(linear_cross_entropy(x, w, t) * 0.7, x, w), per())
+    graph, outs = replayed(step)
+    for seed in (1, 2):
+        nx, nw, nt = make(n, d, v, dtype, seed=seed, ignored=0.3 * seed)
+        with torch.no_grad():
+            x.copy_(nx), w.copy_(nw), t.copy_(nt)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("m,n,count", [(64, 1536, 2), (256, 256, 4), (300, 777, 1)])
+def test_newton_schulz_in_a_cuda_graph(m, n, count):
+    gs = [spectrum(m, n, 0.5, FP, i) for i in range(count)]
+    graph, outs = replayed(lambda: newton_schulz(gs))
+    for g in gs:
+        g.copy_(spectrum(m, n, 0.2, FP, 9) * 3)
+    graph.replay()
+    for o, want in zip(outs, newton_schulz(gs)):
+        assert torch.equal(o, want)
