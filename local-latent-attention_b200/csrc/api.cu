@@ -725,7 +725,7 @@ int llattn_xent(const llattn_xent_args* a, void* stream) {
   if (grads && a->losses) return fail(LLATTN_ERR_ARG, "llattn_xent: losses are written without gradients only");
   if (a->loss && a->reduction == LLATTN_XENT_NONE)
     return fail(LLATTN_ERR_ARG, "llattn_xent: reduction none has no scalar loss");
-  if (grads && (a->reduction == LLATTN_XENT_NONE) != (a->grad_rows != nullptr))
+  if ((grads || a->stage == LLATTN_XENT_LOSS) && (a->reduction == LLATTN_XENT_NONE) != (a->grad_rows != nullptr))
     return fail(LLATTN_ERR_ARG, "llattn_xent: grad_rows goes with reduction none");
   const size_t need = xent::workspace_bytes(*a);
   if (need == 0) return fail(LLATTN_ERR_ARG, "llattn_xent: %d tokens do not fit one piece: no stages", a->tokens);

@@ -191,3 +191,13 @@ def test_matrices_without_a_cluster_get_the_general_kernels(rows, cols):
         a = _lib.OrthArgs(rows, cols, 1, 5, dtype, 3.4, -4.7, 2.0, 1e-7, ptrs, 1 << 21, None, 0)
         up = (cols + 7) // 8 * 8
         assert _lib.lib().llattn_orth_workspace_bytes(ctypes.byref(a)) >= 3 * 2 * rows * up
+
+
+def test_stage_loss_refuses_row_gradients():
+    """grad_rows goes with reduction none, which has no stages: given to a stage's
+    loss it would weight the exponentials that are kept."""
+    a = _lib.XentArgs(10, 64, 100, _lib.BF16, _lib.XENT_MEAN, -100, 1 << 20, 64, 2 << 20, 64, 3 << 20, 1 << 22, None, 4 << 20)
+    a.stage = _lib.XENT_LOSS
+    L = _lib.lib()
+    assert L.llattn_xent(ctypes.byref(a), None) != 0
+    assert "grad_rows" in L.llattn_last_error().decode()
