@@ -14,9 +14,10 @@
 // and each CTA ends up with its 128 rows x 256 columns of the accumulator.
 // Per K = 64 step a CTA copies 32 KB for 128 x 256 x 64 products, half the L2
 // traffic per flop of a 128 x 128 tile on one CTA, which smaller products use
-// because it spreads over more SMs. All keep a ring of 6 to 8 stages that
+// because it spreads over more SMs. All keep a ring of stages (6 to 8) that
 // runs on across tiles and two accumulators in TMEM, so one tile's epilogue
-// overlaps the next tile's MMAs.
+// overlaps the next tile's MMAs; the 256 x 512 tile of long sums has 4 stages
+// and one accumulator, in two halves.
 //
 // Warps: 0 copies, 1 issues MMAs, the others (one per 32 rows x 128 columns of
 // the CTA's accumulator) run the epilogue: thread = row, 128 columns.

@@ -11,8 +11,9 @@
 // into exponentials against the tile's own maximum m, keeps (m, sum) per
 // (row, tile), and, when gradients are wanted, stores the exponentials of a
 // bounded piece of the tokens as fp16 scaled by 2^15: relative to the tile's
-// maximum every stored value above 2^-29 keeps 11 bits, so the later
-// normalisation is the only 8-bit rounding G goes through. xent_rows then
+// maximum every stored value above 2^-29 keeps 11 bits, and one above 2^-32
+// bf16's 8 (none below 2^-40: such a word of such a token gets no gradient), so
+// the later normalisation is the only 8-bit rounding G goes through. xent_rows then
 // joins the tiles' (m, sum) to the row's logsumexp and rewrites the
 // piece in place as bf16 G, which the other two products read. One pass over
 // the exponentials (4 bytes per element) replaces a second 2 N V d product.

@@ -283,16 +283,24 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
     x [..., d] and weight [vocab, d], both bfloat16 or both float32 (under
     autocast both are cast to its dtype, as a linear layer's are, or to float32
     where that is float16); targets
-    [...] int64. Products are summed in fp32; the gradients come back in the
-    inputs' dtype. reduction: "mean" over the tokens whose target is not
+    [...] int64 (vocab at most 2^21, d at most 2^20). The gradients come back in
+    the inputs' dtype. reduction: "mean" over the tokens whose target is not
     ignore_index (0 when there is none), "sum", or "none" (losses [...] fp32,
     0 for ignored tokens). Ignored tokens get zero gradients and their rows of x
     are not read for weight's. A target outside [0, vocab) makes the loss NaN.
 
     "mean" and "sum" keep the exponentials until the backward where they take at
-    most half a GiB; for more tokens they compute the gradients together with the
-    loss, half a GiB of exponentials at a time, and keep those. "none" recomputes
-    in the backward. Gradients of gradients are not supported."""
+    most half a GiB; for more tokens, and under torch.compile and dispatch modes,
+    they compute the gradients together with the loss, half a GiB of exponentials
+    at a time, and keep those. "none" recomputes in the backward. Gradients of
+    gradients are not supported.
+
+    Precision: sums are fp32. fp32 inputs keep 24 bits and their range in every
+    product. bfloat16: the exponentials are held in fp16 relative to the largest
+    of 128 neighbouring words (a probability under 2^-40 of it counts as 0 in the
+    gradients), softmax - onehot is rounded to bfloat16 for more than 64 tokens,
+    and the gradients once more; those that were computed with the loss are
+    rounded again by an upstream gradient that is no power of two."""
     code = _REDUCTIONS.get(reduction)
     if code is None:
         _require(False, f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
@@ -367,7 +375,12 @@ def newton_schulz(g, *, steps: int = 5, coefficients: tuple[float, float, float]
     g: a matrix [m, n], a batch [..., m, n], or a list of matrices (of any mix
     of shapes; equal shapes run as one batch), bfloat16 or float32 on CUDA.
     Returns the same structure in bfloat16 (products of 16-bit operands summed
-    in fp32; not differentiable). An all-zero matrix stays zero."""
+    in fp32, also for float32: 1.7 to 2.8e-3 off, 1.7e-3 of it the result's own
+    rounding; not differentiable). An all-zero matrix stays zero.
+
+    Refused: steps outside 1 to 64, coefficients outside [-16, 16] (the fp16
+    operands' range rests on them), eps below 0, sides above 2^20, more than
+    65536 matrices of a shape."""
     a, b, c = (float(v) for v in coefficients)
     steps, eps = int(steps), float(eps)
     if isinstance(g, Tensor):
