@@ -388,6 +388,49 @@ typedef struct llattn_orth_args {
 LLATTN_API size_t llattn_orth_workspace_bytes(const llattn_orth_args* args);
 LLATTN_API int llattn_orth(const llattn_orth_args* args, void* stream);
 
+/* Gated feed-forward block and its gradients (the block of models.py:40-58 with a
+ * second, gating projection; no counterpart in the reference):
+ *   g = x w_gate^T, u = x w_up^T, h = act(g) u, y = h w_down^T
+ *   x [tokens, d] dtype, w_gate and w_up [ff, d], w_down [d_out, ff], row
+ *   strides ldx, ldg, ldu, ldd (elements; unaligned rows are copied into the workspace)
+ * llattn_gated_fwd writes y [tokens, d_out], contiguous, and where kept is not NULL
+ * what the backward needs of g and u: llattn_gated_kept_bytes bytes.
+ * llattn_gated_bwd takes the same inputs, kept and dy [tokens, d_out] (row
+ * stride lddy) and writes, contiguous, each of dx [tokens, d], dw_gate, dw_up [ff, d]
+ * and dw_down [d_out, ff] that is not NULL.
+ * act: silu(g) = g / (1 + exp(-g)), or gelu(g) = g (1 + erf(g / sqrt 2)) / 2.
+ * workspace and kept: 256-byte aligned, no initialisation; the workspace's size
+ * is llattn_gated_workspace_bytes(args, backward). */
+typedef enum llattn_activation { LLATTN_ACT_SILU = 0, LLATTN_ACT_GELU = 1 } llattn_activation;
+
+typedef struct llattn_gated_args {
+  int32_t tokens, d, ff, d_out, dtype, activation;
+  const void* x;
+  int64_t ldx;
+  const void* w_gate;
+  int64_t ldg;
+  const void* w_up;
+  int64_t ldu;
+  const void* w_down;
+  int64_t ldd;
+  void* y;
+  void* kept;
+  const void* dy;
+  int64_t lddy;
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  void* workspace;
+  size_t workspace_bytes;
+} llattn_gated_args;
+
+/* pointers are only tested for NULL and alignment (0 on bad arguments) */
+LLATTN_API size_t llattn_gated_kept_bytes(const llattn_gated_args* args);
+LLATTN_API size_t llattn_gated_workspace_bytes(const llattn_gated_args* args, int backward);
+LLATTN_API int llattn_gated_fwd(const llattn_gated_args* args, void* stream);
+LLATTN_API int llattn_gated_bwd(const llattn_gated_args* args, void* stream);
+
 /* Per-kernel timing with CUDA events on the launching stream, the native
  * side of the module's set_profile/get_profile_stats (models.py:131-157,
  * which times phases with host syncs instead). enable != 0 turns it on;

@@ -10,10 +10,11 @@ first use; it is built by ``csrc/build.py``.
 """
 
 from . import ops
+from .lm_ops import gated_mlp
 from .module import DecodeCache, LocalLatentAttentionB200, build_attention
 from .ops import LLAttnFunction, llattn_attention
 from .optim import Muon
 from .training_ops import linear_cross_entropy, newton_schulz
 
 __all__ = ["LocalLatentAttentionB200", "DecodeCache", "build_attention", "llattn_attention", "LLAttnFunction", "ops",
-           "linear_cross_entropy", "newton_schulz", "Muon"]
+           "linear_cross_entropy", "newton_schulz", "Muon", "gated_mlp"]

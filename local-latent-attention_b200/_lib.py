@@ -22,9 +22,11 @@ EXPORTED = (
     "llattn_profile_enable", "llattn_profile_read", "llattn_profile_name", "llattn_colsum_workspace_bytes",
     "llattn_colsum", "llattn_fault_inject_host", "llattn_pool_proj_fwd", "llattn_pool_proj_bwd",
     "llattn_xent_workspace_bytes", "llattn_xent", "llattn_scale", "llattn_orth_workspace_bytes", "llattn_orth",
+    "llattn_gated_kept_bytes", "llattn_gated_workspace_bytes", "llattn_gated_fwd", "llattn_gated_bwd",
 )
 XENT_NONE, XENT_MEAN, XENT_SUM = 0, 1, 2
 XENT_ALL, XENT_LOSS, XENT_GRADS = 0, 1, 2  # stages
+ACT_SILU, ACT_GELU = 0, 1
 
 
 class Dims(ctypes.Structure):
@@ -85,6 +87,15 @@ class OrthArgs(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class GatedArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int32), ("d", ctypes.c_int32), ("ff", ctypes.c_int32), ("d_out", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("x", _vp), ("ldx", ctypes.c_int64),
+                ("w_gate", _vp), ("ldg", ctypes.c_int64), ("w_up", _vp), ("ldu", ctypes.c_int64), ("w_down", _vp),
+                ("ldd", ctypes.c_int64), ("y", _vp), ("kept", _vp), ("dy", _vp), ("lddy", ctypes.c_int64), ("dx", _vp),
+                ("dw_gate", _vp), ("dw_up", _vp), ("dw_down", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -137,6 +148,14 @@ def lib() -> ctypes.CDLL:
         L.llattn_orth_workspace_bytes.restype = ctypes.c_size_t
         L.llattn_orth.argtypes = [ctypes.POINTER(OrthArgs), _vp]
         L.llattn_orth.restype = ctypes.c_int
+        L.llattn_gated_kept_bytes.argtypes = [ctypes.POINTER(GatedArgs)]
+        L.llattn_gated_kept_bytes.restype = ctypes.c_size_t
+        L.llattn_gated_workspace_bytes.argtypes = [ctypes.POINTER(GatedArgs), ctypes.c_int]
+        L.llattn_gated_workspace_bytes.restype = ctypes.c_size_t
+        for name in ("llattn_gated_fwd", "llattn_gated_bwd"):
+            fn = getattr(L, name)
+            fn.argtypes = [ctypes.POINTER(GatedArgs), _vp]
+            fn.restype = ctypes.c_int
         L.llattn_profile_enable.argtypes = [ctypes.c_int]
         L.llattn_profile_enable.restype = ctypes.c_int
         L.llattn_profile_read.argtypes = [ctypes.POINTER(ctypes.c_double),
@@ -156,7 +175,7 @@ def profile_enable(on: bool) -> None:
 def profile_read() -> dict:
     """{kernel group: (total ms, launches)} since the last profile_enable."""
     L = lib()
-    n = 16
+    n = 32
     ms = (ctypes.c_double * n)()
     cnt = (ctypes.c_longlong * n)()
     k = L.llattn_profile_read(ms, cnt, n)

@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "gated.cuh"
 #include "profile.cuh"
 #include "sm100.cuh"
 #include "xent.cuh"
@@ -506,7 +507,8 @@ extern "C" {
 int llattn_version(void) { return LLATTN_VERSION; }
 
 unsigned llattn_fault_status(int reset) {
-  unsigned v = sm100::read_fault_word(reset != 0) | xent::read_fault_word(reset != 0) | orth::read_fault_word(reset != 0);
+  unsigned v = sm100::read_fault_word(reset != 0) | xent::read_fault_word(reset != 0) | orth::read_fault_word(reset != 0) |
+               gated::read_fault_word(reset != 0);
   volatile unsigned* w = fault_host_word();
   if (w) {
     v |= *w;
@@ -777,6 +779,49 @@ int llattn_orth(const llattn_orth_args* a, void* stream) {
   prof::Scope ps(prof::ORTH, s, orth::launches(*a));
   return check_launch(orth::launch(*a, g.fault_host, s), "orth");
 }
+
+static int check_gated(const llattn_gated_args* a, bool backward) {
+  if (!a) return fail(LLATTN_ERR_ARG, "args is NULL");
+  if (a->tokens < 1 || a->d < 1 || a->ff < 1 || a->d_out < 1)
+    return fail(LLATTN_ERR_ARG, "gated: tokens, d, ff and d_out must be >= 1");
+  if (a->tokens > (1 << 26) || a->d > (1 << 20) || a->ff > (1 << 20) || a->d_out > (1 << 20))
+    return fail(LLATTN_ERR_ARG, "gated: %d tokens, d %d, ff %d or d_out %d too large", a->tokens, a->d, a->ff, a->d_out);
+  if (a->dtype != LLATTN_F32 && a->dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", a->dtype);
+  if (a->activation != LLATTN_ACT_SILU && a->activation != LLATTN_ACT_GELU)
+    return fail(LLATTN_ERR_ARG, "gated: unknown activation %d", a->activation);
+  if (a->ldx < a->d || a->ldg < a->d || a->ldu < a->d || a->ldd < a->ff || (backward && a->lddy < a->d_out))
+    return fail(LLATTN_ERR_ARG, "gated: row strides (%lld, %lld, %lld, %lld, %lld) below the rows' lengths",
+                (long long)a->ldx, (long long)a->ldg, (long long)a->ldu, (long long)a->ldd, (long long)a->lddy);
+  return LLATTN_OK;
+}
+
+size_t llattn_gated_kept_bytes(const llattn_gated_args* a) { return check_gated(a, false) ? 0 : gated::kept_bytes(*a); }
+
+size_t llattn_gated_workspace_bytes(const llattn_gated_args* a, int backward) {
+  return check_gated(a, backward != 0) ? 0 : gated::workspace_bytes(*a, backward != 0);
+}
+
+static int run_gated(const llattn_gated_args* a, bool backward, const char* what, void* stream) {
+  int rc = check_gated(a, backward);
+  if (rc) return rc;
+  if (!a->x || !a->w_gate || !a->w_up || !a->w_down) return fail(LLATTN_ERR_ARG, "%s: NULL pointer in args", what);
+  if (backward ? !a->dy || !a->kept : !a->y) return fail(LLATTN_ERR_ARG, "%s: NULL pointer in args", what);
+  if (backward && !a->dx && !a->dw_gate && !a->dw_up && !a->dw_down)
+    return fail(LLATTN_ERR_ARG, "%s: no output asked for", what);
+  const size_t need = gated::workspace_bytes(*a, backward);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(LLATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, a->workspace_bytes);
+  if (!al(a->workspace, 256) || (a->kept && !al(a->kept, 256)))
+    return fail(LLATTN_ERR_ALIGN, "%s: workspace and kept must be 256-byte aligned", what);
+  Geom g;
+  if ((rc = fault_gate(&g))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prof::Scope ps(prof::GATED, s, gated::launches(*a, backward));
+  return check_launch(gated::launch(*a, backward, g.fault_host, s), what);
+}
+
+int llattn_gated_fwd(const llattn_gated_args* a, void* stream) { return run_gated(a, false, "llattn_gated_fwd", stream); }
+int llattn_gated_bwd(const llattn_gated_args* a, void* stream) { return run_gated(a, true, "llattn_gated_bwd", stream); }
 
 // ---------------------------------------------------------------------------
 // llattn_bwd_noalloc: the backward for callers that must not allocate device

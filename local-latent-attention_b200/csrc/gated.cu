@@ -1,0 +1,584 @@
+// Gated feed-forward block and its gradients:
+//   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T       (act: silu, or gelu by erf)
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// All products run on mm_kernel (mm_sm100.cuh). The first one takes rows of both
+// Wg and Wu into a tile (kSecondHalves), so that a thread of its epilogue
+// holds g[n, j] and u[n, j] and writes h alone. The backward's first product
+// recomputes h from what was kept and turns dh into dg and du in its epilogue: dh
+// is never in memory either. dx is one product over both halves of the inner
+// width (kSecondTerms), dWg and dWu are one product.
+//
+// Roundings, bf16: h, dg and du are rounded to bf16 to be operands, and the
+// result once more, which is sqrt(2) of the result's own rounding. g and u
+// are kept in fp16 with a power of two for every 32 of them (11 bits relative
+// to their largest, 4 bytes an inner column and token as bf16 would take): in bf16 they
+// would add another rounding to dg and du each (dx 1.75 times its own). Up
+// to kFine tokens keep h, dg and du in two bf16 planes, as little averages
+// their errors.
+// fp32: all operands in three bf16 planes and six products (24 bits), g and u
+// in fp32.
+//
+// Up to kFew tokens without gradients take few_kernel instead: weights are read
+// once, in the order that the tensor cores' fragments want, and h stays fp32.
+#include <math.h>
+
+#include <algorithm>
+
+#include "gated.cuh"
+#include "mm_rows.cuh"
+
+namespace llattn {
+namespace gated {
+namespace {
+
+using namespace mm;
+
+constexpr int kFine = 64, kFew = 32;
+// K = 64 steps a tensor-core sum takes (MmArgs::chain) in fp32: as the loss's products (xent.cu)
+constexpr int kFineF32Chain = 1, kF32Chain = 4;
+constexpr int kBlock = 32;  // inner columns of a kept block
+
+// act(g) and act'(g). EXACT: to fp32's last bits; otherwise ex2's and rcp's 2^-22.
+template <int ACT, bool EXACT>
+__device__ __forceinline__ void activation(float g, float& a, float& slope) {
+  if (ACT == LLATTN_ACT_SILU) {
+    const float e = EXACT ? expf(-g) : __expf(-g);
+    const float s = EXACT ? 1.f / (1.f + e) : __fdividef(1.f, 1.f + e);
+    a = g * s;
+    slope = s * (1.f + g * (1.f - s));
+  } else {
+    const float phi = 0.5f * erfcf(g * -0.70710678f);
+    const float p = 0.39894228f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
+    a = g * phi;
+    slope = phi + g * p;
+  }
+}
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float activate(float g) {
+  float a, slope;
+  activation<ACT, EXACT>(g, a, slope);
+  return a;
+}
+
+// Kept g and u of a (token, block of 32 inner columns): 32 values of g, then of u.
+// bf16 inputs: fp16 times 2^(s - 127), s a byte for g and for u each, chosen so
+// that the largest lies in [2^14, 2^15); fp32 inputs: as they are.
+struct Kept {
+  void* gu;         // [tokens][blocks][2][32]
+  uint16_t* scale;  // [tokens][blocks] (bf16)
+  int blocks;
+};
+__device__ __forceinline__ uint32_t block_scale(const float (&v)[32]) {
+  float m = 0.f;
+#pragma unroll
+  for (int q = 0; q < 32; ++q) m = fmaxf(m, fabsf(v[q]));
+  const int e = __float_as_uint(m) >> 23;  // 2^(e - 127) <= m
+  return (uint32_t)min(253, 127 + 14 + 127 - e);
+}
+__device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
+__device__ __forceinline__ float unscale_of(uint32_t s) { return __uint_as_float((254u - s) << 23); }
+
+// rows of n columns in P bf16 planes (P = 1: rounded), 32 columns of a warp's 32 rows
+template <int P>
+__device__ __forceinline__ void store_planes(uint8_t* buf, int lane, float (&v)[32], const Rows& dst, int64_t plane_bytes,
+                                             int n) {
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    uint4 u[4];
+    bf16_row(v, u);
+    block_store(buf, lane, u, Rows{dst.p + k * plane_bytes, dst.stride, dst.rows}, n * 2);
+    if (k + 1 < P) {
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const float2 r = bf16_pair(u, q);
+        v[2 * q] -= r.x;
+        v[2 * q + 1] -= r.y;
+      }
+    }
+  }
+}
+
+// ---- g, u -> h ------------------------------------------------------------------
+
+// P: planes of h (3: fp32 inputs)
+template <int ACT, int P>
+struct EpiGated {
+  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false;
+  static constexpr int kSecond = kSecondHalves;
+  static constexpr bool F32 = P == 3;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
+  int ff;
+  bf16* h;  // [P][tokens][ldh]
+  int64_t ldh, hplane;
+  Kept kept;  // gu null: nothing is kept
+
+  template <int CW>
+  __device__ __forceinline__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
+                                       uint8_t* buf, Pre&) const {
+    static_assert(CW >= 2 * kBlock, "whole blocks of g");
+    constexpr int G = CW / 2;
+    const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0, f0 = col0 / 2;
+#pragma unroll 1
+    for (int cc = 0; cc < G; cc += 32) {
+      const int n = ff - f0 - cc;
+      if (n <= 0) break;  // warp-uniform
+      float g[32], u[32];
+      load32(taddr + cc, zero, g);
+      load32(taddr + G + cc, zero, u);
+      if (kept.gu) {
+        const int64_t at = (int64_t)row0 * kept.blocks + (f0 + cc) / 32;
+        if constexpr (F32) {
+          uint4 w[8];
+          const Rows dst{static_cast<float*>(kept.gu) + at * 64, kept.blocks * (int64_t)256, rows};
+          f32_row(g, w);
+          block_store(buf, lane, w, dst, 128);
+          f32_row(u, w);
+          block_store(buf, lane, w, dst.at(128), 128);
+        } else {
+          const uint32_t sg = block_scale(g), su = block_scale(u);
+          const float fg = scale_of(sg), fu = scale_of(su);
+          uint4 w[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            w[q] = make_uint4(pack_half(g[8 * q] * fg, g[8 * q + 1] * fg), pack_half(g[8 * q + 2] * fg, g[8 * q + 3] * fg),
+                              pack_half(g[8 * q + 4] * fg, g[8 * q + 5] * fg), pack_half(g[8 * q + 6] * fg, g[8 * q + 7] * fg));
+            w[q + 4] = make_uint4(pack_half(u[8 * q] * fu, u[8 * q + 1] * fu), pack_half(u[8 * q + 2] * fu, u[8 * q + 3] * fu),
+                                  pack_half(u[8 * q + 4] * fu, u[8 * q + 5] * fu), pack_half(u[8 * q + 6] * fu, u[8 * q + 7] * fu));
+          }
+          block_store(buf, lane, w, Rows{static_cast<__half*>(kept.gu) + at * 64, kept.blocks * (int64_t)128, rows}, 128);
+          if (row < M) kept.scale[at + (int64_t)lane * kept.blocks] = (uint16_t)(sg | su << 8);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 32; ++q) g[q] = activate<ACT, F32>(g[q]) * u[q];
+      store_planes<P>(buf, lane, g, Rows{h + (int64_t)row0 * ldh + f0 + cc, ldh * 2, rows}, hplane * 2, n);
+    }
+  }
+};
+
+// ---- dh -> dg, du and h again ----------------------------------------------------
+
+template <int ACT, int P>
+struct EpiGrad {
+  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false;
+  static constexpr bool F32 = P == 3;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
+  Kept kept;
+  bf16* dgu;  // [tokens][P][2][ld] (dg, du), or null
+  int64_t ld;
+  bf16* h;  // [P][tokens][ld], or null
+  int64_t hplane;
+
+  template <int CW>
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
+                                       uint8_t* buf, Pre&) const {
+    const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0;
+    constexpr int CH = 8, HALVES = F32 ? 2 : 1;
+    const int64_t at0 = (int64_t)row0 * kept.blocks + col0 / 32;
+    const Rows src{static_cast<uint8_t*>(kept.gu) + at0 * (128 * HALVES), kept.blocks * (int64_t)(128 * HALVES), rows};
+    uint4 x[CH];
+    uint32_t sc = 0;
+    // the next block is asked for before this one is worked on
+    auto ask = [&](int cc) {
+      block_fetch(lane, x, src.at(cc / 32 * 128 * HALVES), 128);
+      if (!F32 && row < M) sc = kept.scale[at0 + (int64_t)lane * kept.blocks + cc / 32];
+    };
+    if (col0 < a.N) ask(0);
+#pragma unroll 1
+    for (int cc = 0; cc < CW; cc += 32) {
+      const int n = a.N - col0 - cc;
+      if (n <= 0) break;  // warp-uniform
+      float g[32], u[32], dh[32];
+      block_spread(buf, lane, x);
+      if constexpr (F32) {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) g[q] = __uint_as_float(word(x, q));
+        block_fetch(lane, x, src.at(cc / 32 * 256 + 128), 128);
+        block_spread(buf, lane, x);
+#pragma unroll
+        for (int q = 0; q < 32; ++q) u[q] = __uint_as_float(word(x, q));
+      } else {
+        const float fg = unscale_of(sc & 255u), fu = unscale_of(sc >> 8);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const uint32_t wg = word(x, q), wu = word(x, q + 16);
+          const float2 pg = __half22float2(*reinterpret_cast<const __half2*>(&wg));
+          const float2 pu = __half22float2(*reinterpret_cast<const __half2*>(&wu));
+          g[2 * q] = pg.x * fg;
+          g[2 * q + 1] = pg.y * fg;
+          u[2 * q] = pu.x * fu;
+          u[2 * q + 1] = pu.y * fu;
+        }
+      }
+      if (cc + 32 < CW && n > 32) ask(cc + 32);
+      load32(taddr + cc, zero, dh);
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        float act, slope;
+        activation<ACT, F32>(g[q], act, slope);
+        g[q] = act * u[q];
+        u[q] = dh[q] * u[q] * slope;
+        dh[q] *= act;
+      }
+      if (h) store_planes<P>(buf, lane, g, Rows{h + (int64_t)row0 * ld + col0 + cc, ld * 2, rows}, hplane * 2, n);
+      if (dgu) {
+        const Rows dst{dgu + (int64_t)row0 * 2 * P * ld + col0 + cc, 4 * P * ld, rows};
+        store_planes<P>(buf, lane, u, dst, 4 * ld, n);
+        store_planes<P>(buf, lane, dh, Rows{dst.p + 2 * ld, dst.stride, rows}, 4 * ld, n);
+      }
+    }
+  }
+};
+
+// ---- dWg and dWu ------------------------------------------------------------------
+
+// Row m of the product is row m of dWg (m < ff) or m - half of dWu.
+struct EpiTwo {
+  static constexpr bool kNarrow = true, kWide = true, kChain = true, kBegin = false;
+  struct Pre {};
+  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
+  void *first, *second;  // each may be null
+  int64_t ldo;
+  int half, ff, out_bf16, vec;
+
+  __device__ __forceinline__ uint8_t* at(int row, int col) const {
+    const int t = row >= half, r = row - t * half;
+    uint8_t* base = static_cast<uint8_t*>(t ? second : first);
+    return base && r < ff ? base + (r * ldo + col) * (out_bf16 ? 2 : 4) : nullptr;
+  }
+  __device__ __forceinline__ void quad(int row, int col, int n, float4 v) const {
+    uint8_t* dst = at(row, col);
+    if (!dst) return;
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    if (out_bf16) {
+      if (vec) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+      } else {
+        for (int q = 0; q < n; ++q) reinterpret_cast<bf16*>(dst)[q] = __float2bfloat16_rn(x[q]);
+      }
+    } else if (vec) {
+      *reinterpret_cast<float4*>(dst) = v;
+    } else {
+      for (int q = 0; q < n; ++q) reinterpret_cast<float*>(dst)[q] = x[q];
+    }
+  }
+  template <int CW>
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
+                                       uint8_t* buf, Pre&) const {
+    const int lane = threadIdx.x % 32;
+    const MappedRows dst{row < M ? at(row, col0) : nullptr};
+    if (CW == 128 && out_bf16 && vec) {  // whole 128-byte lines
+#pragma unroll 1
+      for (int cc = 0; cc < CW; cc += 64) {
+        const int n = a.N - col0 - cc;
+        if (n <= 0) break;
+        uint4 u[8];
+        row64_bf16(taddr + cc, zero, 1.f, u);
+        block_store(buf, lane, u, dst.at(cc * 2), n * 2);
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int cc = 0; cc < CW; cc += 32) {
+      const int n = a.N - col0 - cc;
+      if (n <= 0) break;  // warp-uniform
+      float v[32];
+      load32(taddr + cc, zero, v);
+      if (out_bf16) {
+        uint4 u[4];
+        bf16_row(v, u);
+        if (vec)
+          block_store(buf, lane, u, dst.at(cc * 2), n * 2);
+        else
+          block_store_odd<bf16>(buf, lane, u, dst.at(cc * 2), n);
+      } else {
+        uint4 u[8];
+        f32_row(v, u);
+        if (vec)
+          block_store(buf, lane, u, dst.at(cc * 4), n * 4);
+        else
+          block_store_odd<float>(buf, lane, u, dst.at(cc * 4), n);
+      }
+    }
+  }
+};
+
+// dx: term t of the inner width's halves takes Wg or Wu
+struct EpiDx : EpiOut {
+  static constexpr int kSecond = kSecondTerms;
+};
+
+// ---- host side ------------------------------------------------------------------
+
+struct Plan {
+  bool f32, fine;
+  int elt, planes, hplanes;
+  bool pack_x, pack_g, pack_u, pack_d, pack_dy;
+  int64_t ldx, ldg, ldu, ldd, ldy, ldf;
+  int blocks;
+  size_t x, g, u, d, dy, h, dgu, part, total;
+};
+
+MmArgs product(const Plan& q, int M, int N, int K, volatile unsigned* fault) {
+  MmArgs p = {};
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.nz = 1;
+  p.n_terms = q.f32 ? 6 : 1;
+  p.pa = q.f32 ? kTermsA : 0;
+  p.pb = q.f32 ? kTermsB : 0;
+  p.chain = q.f32 ? (q.fine ? kFineF32Chain : kF32Chain) : 0;
+  p.fault_host = fault;
+  return p;
+}
+// y = h Wd^T
+MmArgs y_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* fault) {
+  MmArgs p = product(q, a.tokens, a.d_out, a.ff, fault);
+  if (q.hplanes == 2) {
+    p.n_terms = 2;
+    p.pa = 0x01u;
+  }
+  p.split = 1;
+  return p;
+}
+// dx = dg Wg + du Wu: for each term of fp32's planes (or of G's two), smallest first, a
+// pass over each half. dgu's z is 2 plane + half.
+MmArgs dx_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* fault) {
+  MmArgs p = product(q, a.tokens, a.d, a.ff, fault);
+  const int n = q.f32 ? 6 : q.hplanes;
+  const uint64_t ta = q.f32 ? kTermsA : q.hplanes == 2 ? 0x01u : 0u, tb = q.f32 ? kTermsB : 0u;
+  p.pa = p.pb = 0;
+  for (int t = 0; t < n; ++t)
+    for (int half = 0; half < 2; ++half) {
+      p.pa |= (2 * ((ta >> (4 * t)) & 15u) + half) << (4 * (2 * t + half));
+      p.pb |= ((tb >> (4 * t)) & 15u) << (4 * (2 * t + half));
+      p.b2 |= (uint32_t)half << (2 * t + half);
+    }
+  p.n_terms = 2 * n;
+  p.majors = 2;
+  p.split = 1;
+  return p;
+}
+// dWd = dy^T h
+MmArgs dwd_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* fault) {
+  MmArgs p = product(q, a.d_out, a.ff, a.tokens, fault);
+  if (q.hplanes == 2) {
+    p.n_terms = 2;
+    p.pb = 0x01u;
+  }
+  p.split = 1;
+  return p;
+}
+// [dWg; dWu] = [dg, du]^T x
+MmArgs dwgu_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* fault) {
+  MmArgs p = product(q, (int)(2 * q.ldf), a.d, a.tokens, fault);
+  if (q.hplanes == 2) {
+    p.n_terms = 2;
+    p.pa = 0x01u;
+  }
+  p.split = 1;
+  return p;
+}
+
+Plan make_plan(const llattn_gated_args& a, bool backward) {
+  Plan q;
+  q.f32 = a.dtype == LLATTN_F32;
+  q.fine = a.tokens <= kFine;
+  q.elt = q.f32 ? 4 : 2;
+  q.planes = q.f32 ? 3 : 1;
+  q.hplanes = q.f32 ? 3 : q.fine ? 2 : 1;
+  const int64_t n = a.tokens;
+  auto pack = [&](const void* p, int64_t ld, int64_t rows) { return q.f32 || !aligned_rows(p, ld, rows, 2); };
+  auto stride = [&](bool packed, int64_t ld, int64_t rows, int cols) { return packed || rows == 1 ? up8(cols) : ld; };
+  q.pack_x = pack(a.x, a.ldx, n);
+  q.pack_g = pack(a.w_gate, a.ldg, a.ff);
+  q.pack_u = pack(a.w_up, a.ldu, a.ff);
+  q.pack_d = pack(a.w_down, a.ldd, a.d_out);
+  q.pack_dy = backward && pack(a.dy, a.lddy, n);
+  q.ldx = stride(q.pack_x, a.ldx, n, a.d);
+  q.ldg = stride(q.pack_g, a.ldg, a.ff, a.d);
+  q.ldu = stride(q.pack_u, a.ldu, a.ff, a.d);
+  q.ldd = stride(q.pack_d, a.ldd, a.d_out, a.ff);
+  q.ldy = stride(q.pack_dy, a.lddy, n, a.d_out);
+  q.ldf = up8(a.ff);
+  q.blocks = cdiv(a.ff, kBlock);
+  const bool need_x = !backward || a.dw_gate || a.dw_up, need_gu = !backward || a.dx, inner = a.dx || a.dw_gate || a.dw_up;
+  size_t off = 0;
+  auto take = [&](size_t b) { size_t o = off; off += up256(b); return o; };
+  const size_t pl = 2 * (size_t)q.planes;
+  q.x = take(q.pack_x && need_x ? pl * n * q.ldx : 0);
+  q.g = take(q.pack_g && need_gu ? pl * a.ff * q.ldg : 0);
+  q.u = take(q.pack_u && need_gu ? pl * a.ff * q.ldu : 0);
+  q.d = take(q.pack_d ? pl * a.d_out * q.ldd : 0);
+  q.dy = take(q.pack_dy ? pl * n * q.ldy : 0);
+  q.h = take(!backward || a.dw_down ? 2 * (size_t)q.hplanes * n * q.ldf : 0);
+  q.dgu = take(backward && inner ? 4 * (size_t)q.hplanes * n * q.ldf : 0);
+  int64_t part = 0;
+  if (!backward) {
+    part = mm_part_floats(y_args(q, a, nullptr));
+  } else {
+    if (a.dx) part = mm_part_floats(dx_args(q, a, nullptr));
+    if (a.dw_down) part = std::max(part, mm_part_floats(dwd_args(q, a, nullptr)));
+    if (a.dw_gate || a.dw_up) part = std::max(part, mm_part_floats(dwgu_args(q, a, nullptr)));
+  }
+  q.part = take(4 * (size_t)part);
+  q.total = off;
+  return q;
+}
+
+Kept kept_at(const Plan& q, const llattn_gated_args& a) {
+  Kept k;
+  k.gu = a.kept;
+  k.blocks = q.blocks;
+  k.scale = reinterpret_cast<uint16_t*>(static_cast<char*>(a.kept) + up256((size_t)a.tokens * q.blocks * 64 * (q.f32 ? 4 : 2)));
+  return k;
+}
+
+template <typename T>
+cudaError_t pack(bool needed, const void* src, int64_t ld, int rows, int cols, void* dst, int64_t lds, cudaStream_t s) {
+  if (!needed) return cudaSuccess;
+  return launch_pdl(pack_kernel<T>, dim3(cdiv(rows, 8)), 256, 0, 1, s, static_cast<const T*>(src), ld, rows, cols,
+                    static_cast<bf16*>(dst), lds, rows * lds);
+}
+
+EpiOut rows_out(const Plan& q, void* out, int cols) {
+  EpiOut o{};
+  o.out = out;
+  o.ldo = cols;
+  o.out_bf16 = !q.f32;
+  o.vec = aligned_rows(out, cols, 2, q.elt);
+  return o;
+}
+
+// The tile of the gated product: at least one kept block of g wide (shape 0 holds 16 columns of g)
+template <int ACT, int P>
+cudaError_t launch_gated(MmArgs p, const Operand& x, const Operand& g, const Operand& u, const EpiGated<ACT, P>& e,
+                         cudaStream_t s) {
+  const double t2 = mm_time<2>(p), t1 = mm_time<1>(p), t4 = mm_time<4>(p);
+  if (t4 < std::min(t1, t2)) return launch_mm_sh<4>(p, x, g, e, s, &u);
+  return t2 <= t1 ? launch_mm_sh<2>(p, x, g, e, s, &u) : launch_mm_sh<1>(p, x, g, e, s, &u);
+}
+
+template <typename T, int ACT, int P>
+cudaError_t run_fwd(const llattn_gated_args& a, const Plan& q, volatile unsigned* fault, cudaStream_t s) {
+  char* ws = static_cast<char*>(a.workspace);
+  const int n = a.tokens;
+  TRY(pack<T>(q.pack_x, a.x, a.ldx, n, a.d, ws + q.x, q.ldx, s));
+  TRY(pack<T>(q.pack_g, a.w_gate, a.ldg, a.ff, a.d, ws + q.g, q.ldg, s));
+  TRY(pack<T>(q.pack_u, a.w_up, a.ldu, a.ff, a.d, ws + q.u, q.ldu, s));
+  TRY(pack<T>(q.pack_d, a.w_down, a.ldd, a.d_out, a.ff, ws + q.d, q.ldd, s));
+  const Operand x{q.pack_x ? ws + q.x : a.x, n, a.d, q.ldx, q.planes, n * q.ldx, 0};
+  const Operand g{q.pack_g ? ws + q.g : a.w_gate, a.ff, a.d, q.ldg, q.planes, a.ff * q.ldg, 0};
+  const Operand u{q.pack_u ? ws + q.u : a.w_up, a.ff, a.d, q.ldu, q.planes, a.ff * q.ldu, 0};
+  const Operand d{q.pack_d ? ws + q.d : a.w_down, a.d_out, a.ff, q.ldd, q.planes, a.d_out * q.ldd, 0};
+  bf16* h = reinterpret_cast<bf16*>(ws + q.h);
+  const int64_t hplane = n * q.ldf;
+  EpiGated<ACT, P> e{};
+  e.ff = a.ff;
+  e.h = h;
+  e.ldh = q.ldf;
+  e.hplane = hplane;
+  if (a.kept) e.kept = kept_at(q, a);
+  TRY(launch_gated(product(q, n, 2 * a.ff, a.d, fault), x, g, u, e, s));
+  MmArgs p = y_args(q, a, fault);
+  p.part = reinterpret_cast<float*>(ws + q.part);
+  return launch_mm(p, Operand{h, n, a.ff, q.ldf, P, hplane, 0}, d, rows_out(q, a.y, a.d_out), s);
+}
+
+template <typename T, int ACT, int P>
+cudaError_t run_bwd(const llattn_gated_args& a, const Plan& q, volatile unsigned* fault, cudaStream_t s) {
+  char* ws = static_cast<char*>(a.workspace);
+  const int n = a.tokens;
+  const bool weights = a.dw_gate || a.dw_up;
+  TRY(pack<T>(q.pack_dy, a.dy, a.lddy, n, a.d_out, ws + q.dy, q.ldy, s));
+  TRY(pack<T>(q.pack_d, a.w_down, a.ldd, a.d_out, a.ff, ws + q.d, q.ldd, s));
+  TRY(pack<T>(q.pack_g && a.dx, a.w_gate, a.ldg, a.ff, a.d, ws + q.g, q.ldg, s));
+  TRY(pack<T>(q.pack_u && a.dx, a.w_up, a.ldu, a.ff, a.d, ws + q.u, q.ldu, s));
+  TRY(pack<T>(q.pack_x && weights, a.x, a.ldx, n, a.d, ws + q.x, q.ldx, s));
+  const void* dy = q.pack_dy ? ws + q.dy : a.dy;
+  const int64_t dyplane = n * q.ldy, hplane = n * q.ldf;
+  bf16 *h = reinterpret_cast<bf16*>(ws + q.h), *dgu = reinterpret_cast<bf16*>(ws + q.dgu);
+  float* part = reinterpret_cast<float*>(ws + q.part);
+  EpiGrad<ACT, P> e{};
+  e.kept = kept_at(q, a);
+  e.dgu = a.dx || weights ? dgu : nullptr;
+  e.ld = q.ldf;
+  e.h = a.dw_down ? h : nullptr;
+  e.hplane = hplane;
+  TRY(launch_mm(product(q, n, a.ff, a.d_out, fault), Operand{dy, n, a.d_out, q.ldy, q.planes, dyplane, 0},
+                Operand{q.pack_d ? ws + q.d : a.w_down, a.d_out, a.ff, q.ldd, q.planes, a.d_out * q.ldd, 1}, e, s));
+  if (a.dx) {
+    MmArgs p = dx_args(q, a, fault);
+    p.part = part;
+    const Operand g{q.pack_g ? ws + q.g : a.w_gate, a.ff, a.d, q.ldg, q.planes, a.ff * q.ldg, 1};
+    const Operand u{q.pack_u ? ws + q.u : a.w_up, a.ff, a.d, q.ldu, q.planes, a.ff * q.ldu, 1};
+    EpiDx o{rows_out(q, a.dx, a.d)};
+    TRY(launch_mm(p, Operand{dgu, n, a.ff, 2 * P * q.ldf, 2 * P, q.ldf, 0}, g, o, s, &u));
+  }
+  if (a.dw_down) {
+    MmArgs p = dwd_args(q, a, fault);
+    p.part = part;
+    TRY(launch_mm(p, Operand{dy, n, a.d_out, q.ldy, q.planes, dyplane, 1}, Operand{h, n, a.ff, q.ldf, P, hplane, 1},
+                  rows_out(q, a.dw_down, a.ff), s));
+  }
+  if (weights) {
+    MmArgs p = dwgu_args(q, a, fault);
+    p.part = part;
+    EpiTwo o{};
+    o.first = a.dw_gate;
+    o.second = a.dw_up;
+    o.ldo = a.d;
+    o.half = (int)q.ldf;
+    o.ff = a.ff;
+    o.out_bf16 = !q.f32;
+    o.vec = (!a.dw_gate || aligned_rows(a.dw_gate, a.d, 2, q.elt)) && (!a.dw_up || aligned_rows(a.dw_up, a.d, 2, q.elt));
+    TRY(launch_mm(p, Operand{dgu, n, 2 * q.ldf, 2 * P * q.ldf, P, 2 * q.ldf, 1},
+                  Operand{q.pack_x ? ws + q.x : a.x, n, a.d, q.ldx, q.planes, n * q.ldx, 1}, o, s));
+  }
+  return cudaSuccess;
+}
+
+template <int ACT>
+cudaError_t run(const llattn_gated_args& a, bool backward, volatile unsigned* fault, cudaStream_t s) {
+  const Plan q = make_plan(a, backward);
+  if (q.f32) return backward ? run_bwd<float, ACT, 3>(a, q, fault, s) : run_fwd<float, ACT, 3>(a, q, fault, s);
+  if (q.hplanes == 2) return backward ? run_bwd<bf16, ACT, 2>(a, q, fault, s) : run_fwd<bf16, ACT, 2>(a, q, fault, s);
+  return backward ? run_bwd<bf16, ACT, 1>(a, q, fault, s) : run_fwd<bf16, ACT, 1>(a, q, fault, s);
+}
+
+}  // namespace
+
+size_t kept_bytes(const llattn_gated_args& a) {
+  const size_t blocks = (size_t)a.tokens * cdiv(a.ff, kBlock);
+  return a.dtype == LLATTN_F32 ? up256(blocks * 256) : up256(blocks * 128) + up256(blocks * 2);
+}
+
+size_t workspace_bytes(const llattn_gated_args& a, bool backward) {
+  return std::max<size_t>(256, make_plan(a, backward).total);
+}
+
+int launches(const llattn_gated_args& a, bool backward) {
+  const Plan q = make_plan(a, backward);
+  const bool weights = a.dw_gate || a.dw_up;
+  if (!backward) return q.pack_x + q.pack_g + q.pack_u + q.pack_d + 2 + joins(y_args(q, a, nullptr));
+  int n = q.pack_dy + q.pack_d + 1;
+  if (a.dx) n += q.pack_g + q.pack_u + 1 + joins(dx_args(q, a, nullptr));
+  if (a.dw_down) n += 1 + joins(dwd_args(q, a, nullptr));
+  if (weights) n += q.pack_x + 1 + joins(dwgu_args(q, a, nullptr));
+  return n;
+}
+
+cudaError_t launch(const llattn_gated_args& a, bool backward, volatile unsigned* fault, cudaStream_t s) {
+  return a.activation == LLATTN_ACT_SILU ? run<LLATTN_ACT_SILU>(a, backward, fault, s)
+                                         : run<LLATTN_ACT_GELU>(a, backward, fault, s);
+}
+
+unsigned read_fault_word(bool reset) { return read_fault(reset); }
+
+}  // namespace gated
+}  // namespace llattn

@@ -28,6 +28,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "sm100.cuh"
 #include "sm100_ptx.cuh"
@@ -92,7 +94,7 @@ struct MmArgs {
   // bits: a sum that grows evenly comes out up to 2^-26 per product of 16 short
   // (measured for bf16 operands, three times that for fp16), always
   // towards zero. chain > 0 bounds each such sum to that many K = 64 steps (of
-  // the last term's; the terms before it, smaller by 2^-8 and less, make one
+  // the last term's, or the last `majors`'; the terms before, smaller by 2^-8 and less, make one
   // more): the epilogue warps add it to the tile's fp32 sum in TMEM, rounded to
   // nearest, while the next one is under way (Epi::kChain; not shape 3).
   int chain;
@@ -101,7 +103,9 @@ struct MmArgs {
   // products over planes: operand z coordinates (pa, pb) of n_terms passes
   // over K, 4 bits each (fp32 operands in three bf16 planes, G in two)
   int n_terms;
-  uint32_t pa, pb;
+  int majors;               // how many of them, the last ones, are the large ones (0: 1)
+  uint64_t pa, pb;
+  uint32_t b2;              // kSecondTerms: bit t set, term t takes B from its second map
   const int* m_dev;
   const int* k_dev;
   int dev_base;
@@ -525,9 +529,9 @@ __device__ __forceinline__ void drain(uint32_t acc, uint32_t sum, bool add) {
 
 // The tensor-core sums of a tile of `steps` K = 64 steps over n_terms terms:
 // the one that starts at step i ends before step chain_end.
-__device__ __forceinline__ int chain_end(int i, int steps, int n_terms, int chain) {
-  const int minor = n_terms > 1 ? steps / n_terms * (n_terms - 1) : 0;
-  return i < minor ? minor : min(steps, i + chain);
+__device__ __forceinline__ int chain_end(const MmArgs& p, int i, int steps) {
+  const int minor = p.n_terms > 1 ? steps / p.n_terms * (p.n_terms - max(p.majors, 1)) : 0;
+  return i < minor ? minor : min(steps, i + p.chain);
 }
 
 // one range's sums of a tile: its fp32 block of part, [BM][BN]
@@ -549,6 +553,19 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
   }
 }
 
+// A second map for B, asked for by Epi::kSecond:
+//   kSecondHalves: both maps' rows in one tile: of every BR columns of C (a CTA's share
+//     of a tile, an epilogue warp's columns) the first half are rows of the first map and
+//     the other half the same rows of the second one, so that a thread holds column
+//     j of both products. C's columns count both: N = 2 x rows, rounded up to
+//     whole BR. K-major only.
+//   kSecondTerms: MmArgs::b2 says which terms take the second map.
+enum { kSecondNone = 0, kSecondHalves = 1, kSecondTerms = 2 };
+template <typename Epi, typename = void>
+struct SecondB : std::integral_constant<int, kSecondNone> {};
+template <typename Epi>
+struct SecondB<Epi, std::void_t<decltype(Epi::kSecond)>> : std::integral_constant<int, Epi::kSecond> {};
+
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
 //                                          bool zero, uint8_t* buf, Pre& pre) const
@@ -566,8 +583,10 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 template <int SH, bool CHAIN, typename Epi>
 __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-              const __grid_constant__ MmArgs p, const __grid_constant__ Epi epi) {
+              const __grid_constant__ CUtensorMap tm_b2, const __grid_constant__ MmArgs p,
+              const __grid_constant__ Epi epi) {
   using S = MmShape<SH>;
+  constexpr int SECOND = SecondB<Epi>::value;
   constexpr int ST = S::ST, CG = S::CG;
   extern __shared__ uint8_t mm_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~uintptr_t(1023));
@@ -593,6 +612,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     fence_barrier_init();
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
+    if (SECOND != kSecondNone) prefetch_tmap(&tm_b2);
   }
   if (warp == 1) {
     __syncwarp();
@@ -628,6 +648,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       int it = 0;
       bool ok = true;
       // the copies of a K = 64 step into stage s
+      const CUtensorMap* mb = &tm_b;
       auto copy = [&](int s, int ma, int nb, int k, int za, int zb, bool first) {
         if (rank == 0) mbar_expect_tx(&full[s], CG * (S::AB + S::NH * (S::BR < 64 && !p.b_mn ? S::BR * 128 : S::BB)));
         uint8_t* sa = smem + S::A + s * S::AB;
@@ -649,11 +670,14 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
         for (int h = 0; h < S::NH; ++h) {
           uint8_t* dst = sb + h * S::BB;
           const int n = nb + h * S::HN;
-          if (p.b_mn) {
-            load(&tm_b, dst, n, k, zb);
-            if (S::BR > 64) load(&tm_b, dst + S::BB / 2, n + 64, k, zb);
+          if (SECOND == kSecondHalves) {
+            load(&tm_b, dst, k, n / 2, zb);
+            load(&tm_b2, dst + S::BR * 64, k, n / 2, zb);
+          } else if (p.b_mn) {
+            load(mb, dst, n, k, zb);
+            if (S::BR > 64) load(mb, dst + S::BB / 2, n + 64, k, zb);
           } else {
-            load(&tm_b, dst, k, n, zb);
+            load(mb, dst, k, n, zb);
           }
         }
       };
@@ -663,6 +687,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
         const int ma = w.m0 + rank * 128, nb = w.n0 + rank * S::BR;
         for (int term = 0; ok && term < p.n_terms; ++term) {
           const int za = w.z + (int)((p.pa >> (4 * term)) & 15u), zb = w.z + (int)((p.pb >> (4 * term)) & 15u);
+          if (SECOND == kSecondTerms) mb = (p.b2 >> term) & 1 ? &tm_b2 : &tm_b;
           int k = x.k0;
           if (!counted && it == 0 && k < x.k1) {  // (apart: a test in the loop costs a long product 3 %)
             copy(0, ma, nb, k, za, zb, true);
@@ -750,7 +775,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
           }
         }
         do {
-          const int end = CHAIN ? chain_end(i, steps, p.n_terms, p.chain) : steps, begin = i;
+          const int end = CHAIN ? chain_end(p, i, steps) : steps, begin = i;
           const int buf = one ? 0 : k & 1, use = one ? k : k >> 1;
           if (S::NH == 1) {
             // the epilogue has read what this accumulator held before
@@ -822,7 +847,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
           if (!ok) break;
           if (steps) drain<S::CW>(t0 + S::HN * buf, sum, i > 0);
           release(buf);
-          i = chain_end(i, steps, p.n_terms, p.chain);
+          i = chain_end(p, i, steps);
         } while (i < steps);
         if (ok) out(S::CW * half, sum);
       } else {
@@ -944,29 +969,43 @@ cudaError_t launch_join(const MmArgs&, const Epi&, int, cudaStream_t, ...) {
   return cudaErrorInvalidValue;  // an epilogue without quad() cannot be split
 }
 
+// b2: the second map's operand (Epi::kSecond; kSecondHalves: N is set here).
 template <int SH, bool CHAIN = false, typename Epi>
-cudaError_t launch_mm_sh(const MmArgs& p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
+cudaError_t launch_mm_sh(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s,
+                         const Operand* b2 = nullptr) {
   if constexpr (Epi::kChain && !CHAIN && SH != 3) {
-    if (p.chain) return launch_mm_sh<SH, true>(p, a, b, epi, s);
+    if (p.chain) return launch_mm_sh<SH, true>(p, a, b, epi, s, b2);
   }
   using S = MmShape<SH>;
-  CUtensorMap ta, tb;
+  constexpr int SECOND = SecondB<Epi>::value;
+  const int br = SECOND == kSecondHalves ? S::BR / 2 : S::BR;
+  CUtensorMap ta, tb, tb2;
   if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
-      !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : S::BR))
+      !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : br))
     return cudaErrorInvalidValue;
+  tb2 = tb;
+  if (SECOND != kSecondNone &&
+      (!b2 || b2->mn != b.mn ||
+       !sm100::make_operand_map(&tb2, b2->p, b2->rows, b2->cols, b2->ld, b2->nz, b2->zs, b2->mn ? 64 : br)))
+    return cudaErrorInvalidValue;
+  if (SECOND == kSecondHalves) {
+    if (b.mn || p.split) return cudaErrorInvalidValue;
+    p.N = cdiv((int)b.rows, br) * S::BR;
+  }
   cudaError_t e = set_smem_once(mm_kernel<SH, CHAIN, Epi>, S::SMEM);
   if (e != cudaSuccess) return e;
   const int64_t m = cdiv(p.M, S::BM), n = cdiv(p.N, S::BN);
   const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
   const int units = p.split ? mm_units(SH) : (int)std::min<int64_t>(tiles, mm_units(SH));
-  e = launch_pdl(mm_kernel<SH, CHAIN, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, p, epi);
+  e = launch_pdl(mm_kernel<SH, CHAIN, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, tb2, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<SH, Epi>(p, epi, units, s, nullptr);
 }
 
 template <typename Epi>
-cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s) {
+cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s,
+                      const Operand* b2 = nullptr) {
   p.a_mn = a.mn;
   p.b_mn = b.mn;
   if (p.nz < 1) p.nz = 1;
@@ -978,12 +1017,12 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
     q.sym = 0;  // not square: every tile is computed
     const double t4 = mm_time<4>(q), t0 = mm_time<0>(q);
     if (std::min(t0, t4) < std::min(t1, t2))
-      return t0 <= t4 ? launch_mm_sh<0>(q, a, b, epi, s) : launch_mm_sh<4>(q, a, b, epi, s);
+      return t0 <= t4 ? launch_mm_sh<0>(q, a, b, epi, s, b2) : launch_mm_sh<4>(q, a, b, epi, s, b2);
   }
   if constexpr (Epi::kWide) {
-    if (!p.chain && mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s);
+    if (!p.chain && mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s, b2);
   }
-  return t2 <= t1 ? launch_mm_sh<2>(p, a, b, epi, s) : launch_mm_sh<1>(p, a, b, epi, s);
+  return t2 <= t1 ? launch_mm_sh<2>(p, a, b, epi, s, b2) : launch_mm_sh<1>(p, a, b, epi, s, b2);
 }
 
 }  // namespace
