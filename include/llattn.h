@@ -431,6 +431,63 @@ LLATTN_API size_t llattn_gated_workspace_bytes(const llattn_gated_args* args, in
 LLATTN_API int llattn_gated_fwd(const llattn_gated_args* args, void* stream);
 LLATTN_API int llattn_gated_bwd(const llattn_gated_args* args, void* stream);
 
+/* Token embedding with its positions (models.py:505-518: embedding + position), and
+ * its gradients:
+ *   out[b, t] = scale w[ids[b, t]] + positions[t]      (positions may be NULL)
+ *   dw[v] = scale sum of dout[b, t] over ids[b, t] = v, dpositions[t] = sum_b dout[b, t]
+ *   ids [batch, length] int64 (ids_wide != 0) or int32; w [vocab, d], positions
+ *   [position_rows >= length, d] dtype, row strides ldw, ldp (elements)
+ *   out, dout [batch, length, d], dw [vocab, d], dpositions [position_rows, d]: contiguous
+ * An id outside [0, vocab) makes its row of out NaN and has no gradient; tokens of the
+ * word `padding` (< 0: none) have no gradient either, in dw. llattn_embed_bwd writes each
+ * of dw and dpositions that is not NULL, whole. workspace: llattn_embed_workspace_bytes
+ * bytes, 256-byte aligned, no initialisation (the forward needs none). */
+typedef struct llattn_embed_args {
+  int32_t batch, length, d, dtype, ids_wide, position_rows;
+  int64_t vocab, padding;
+  float scale;
+  const void* ids;
+  const void* w;
+  int64_t ldw;
+  const void* positions;
+  int64_t ldp;
+  void* out;
+  const void* dout;
+  void* dw;
+  void* dpositions;
+  void* workspace;
+  size_t workspace_bytes;
+} llattn_embed_args;
+
+LLATTN_API size_t llattn_embed_workspace_bytes(const llattn_embed_args* args);
+LLATTN_API int llattn_embed_fwd(const llattn_embed_args* args, void* stream);
+LLATTN_API int llattn_embed_bwd(const llattn_embed_args* args, void* stream);
+
+/* Norm of `count` tensors together, and their scaling in place:
+ *   norm = sqrt(sum of squares) or the largest magnitude (a NaN, where there is one)
+ *   scale != 0: every element times min(1, max_norm / (norm + 1e-6))
+ * tensors, sizes (elements) and dtypes are host arrays, read during the call; a
+ * tensor is sizes[i] consecutive elements, aligned to their own size, on the current
+ * device; empty ones are skipped; with scale none may overlap another. norm: fp32 device
+ * scalar. Sums are fp64, in a fixed order. Replaces torch.nn.utils.clip_grad_norm_
+ * in the reference's training loop. workspace: llattn_clip_workspace_bytes bytes,
+ * 256-byte aligned, no initialisation. */
+typedef enum llattn_norm_type { LLATTN_NORM_2 = 0, LLATTN_NORM_INF = 1 } llattn_norm_type;
+
+typedef struct llattn_clip_args {
+  int32_t count, norm_type, scale;
+  void* const* tensors;
+  const int64_t* sizes;
+  const int32_t* dtypes;
+  double max_norm;
+  float* norm;
+  void* workspace;
+  size_t workspace_bytes;
+} llattn_clip_args;
+
+LLATTN_API size_t llattn_clip_workspace_bytes(const llattn_clip_args* args);
+LLATTN_API int llattn_clip(const llattn_clip_args* args, void* stream);
+
 /* Per-kernel timing with CUDA events on the launching stream, the native
  * side of the module's set_profile/get_profile_stats (models.py:131-157,
  * which times phases with host syncs instead). enable != 0 turns it on;

@@ -10,11 +10,12 @@ first use; it is built by ``csrc/build.py``.
 """
 
 from . import ops
-from .lm_ops import gated_mlp
+from .lm_ops import clip_grad_norm_, gated_mlp, token_embedding, total_norm
 from .module import DecodeCache, LocalLatentAttentionB200, build_attention
 from .ops import LLAttnFunction, llattn_attention
 from .optim import Muon
 from .training_ops import linear_cross_entropy, newton_schulz
 
 __all__ = ["LocalLatentAttentionB200", "DecodeCache", "build_attention", "llattn_attention", "LLAttnFunction", "ops",
-           "linear_cross_entropy", "newton_schulz", "Muon", "gated_mlp"]
+           "linear_cross_entropy", "newton_schulz", "Muon", "gated_mlp", "token_embedding",
+           "clip_grad_norm_", "total_norm"]

@@ -23,10 +23,12 @@ EXPORTED = (
     "llattn_colsum", "llattn_fault_inject_host", "llattn_pool_proj_fwd", "llattn_pool_proj_bwd",
     "llattn_xent_workspace_bytes", "llattn_xent", "llattn_scale", "llattn_orth_workspace_bytes", "llattn_orth",
     "llattn_gated_kept_bytes", "llattn_gated_workspace_bytes", "llattn_gated_fwd", "llattn_gated_bwd",
+    "llattn_embed_workspace_bytes", "llattn_embed_fwd", "llattn_embed_bwd", "llattn_clip_workspace_bytes", "llattn_clip",
 )
 XENT_NONE, XENT_MEAN, XENT_SUM = 0, 1, 2
 XENT_ALL, XENT_LOSS, XENT_GRADS = 0, 1, 2  # stages
 ACT_SILU, ACT_GELU = 0, 1
+NORM_2, NORM_INF = 0, 1
 
 
 class Dims(ctypes.Structure):
@@ -96,6 +98,21 @@ class GatedArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+class EmbedArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("length", ctypes.c_int32), ("d", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("ids_wide", ctypes.c_int32), ("position_rows", ctypes.c_int32), ("vocab", ctypes.c_int64),
+                ("padding", ctypes.c_int64), ("scale", ctypes.c_float), ("ids", _vp), ("w", _vp), ("ldw", ctypes.c_int64),
+                ("positions", _vp), ("ldp", ctypes.c_int64), ("out", _vp), ("dout", _vp), ("dw", _vp),
+                ("dpositions", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class ClipArgs(ctypes.Structure):
+    _fields_ = [("count", ctypes.c_int32), ("norm_type", ctypes.c_int32), ("scale", ctypes.c_int32),
+                ("tensors", ctypes.POINTER(_vp)), ("sizes", ctypes.POINTER(ctypes.c_int64)),
+                ("dtypes", ctypes.POINTER(ctypes.c_int32)), ("max_norm", ctypes.c_double), ("norm", _fp),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -155,6 +172,14 @@ def lib() -> ctypes.CDLL:
         for name in ("llattn_gated_fwd", "llattn_gated_bwd"):
             fn = getattr(L, name)
             fn.argtypes = [ctypes.POINTER(GatedArgs), _vp]
+            fn.restype = ctypes.c_int
+        L.llattn_embed_workspace_bytes.argtypes = [ctypes.POINTER(EmbedArgs)]
+        L.llattn_embed_workspace_bytes.restype = ctypes.c_size_t
+        L.llattn_clip_workspace_bytes.argtypes = [ctypes.POINTER(ClipArgs)]
+        L.llattn_clip_workspace_bytes.restype = ctypes.c_size_t
+        for name, cls in (("llattn_embed_fwd", EmbedArgs), ("llattn_embed_bwd", EmbedArgs), ("llattn_clip", ClipArgs)):
+            fn = getattr(L, name)
+            fn.argtypes = [ctypes.POINTER(cls), _vp]
             fn.restype = ctypes.c_int
         L.llattn_profile_enable.argtypes = [ctypes.c_int]
         L.llattn_profile_enable.restype = ctypes.c_int

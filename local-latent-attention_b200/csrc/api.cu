@@ -9,9 +9,13 @@
 #include <string.h>
 
 #include <algorithm>
+#include <memory>
 #include <mutex>
+#include <new>
 
+#include "clip.cuh"
 #include "common.cuh"
+#include "embed.cuh"
 #include "gated.cuh"
 #include "profile.cuh"
 #include "sm100.cuh"
@@ -822,6 +826,107 @@ static int run_gated(const llattn_gated_args* a, bool backward, const char* what
 
 int llattn_gated_fwd(const llattn_gated_args* a, void* stream) { return run_gated(a, false, "llattn_gated_fwd", stream); }
 int llattn_gated_bwd(const llattn_gated_args* a, void* stream) { return run_gated(a, true, "llattn_gated_bwd", stream); }
+
+static int check_embed(const llattn_embed_args* a) {
+  if (!a) return fail(LLATTN_ERR_ARG, "args is NULL");
+  if (a->batch < 1 || a->length < 1 || a->d < 1 || a->vocab < 1)
+    return fail(LLATTN_ERR_ARG, "embed: batch, length, d and vocab must be >= 1");
+  if ((int64_t)a->batch * a->length > (1 << 30) || a->d > (1 << 20) || a->vocab > (1 << 24))
+    return fail(LLATTN_ERR_ARG, "embed: %d x %d tokens, d %d or vocab %lld too large", a->batch, a->length, a->d,
+                (long long)a->vocab);
+  if (a->dtype != LLATTN_F32 && a->dtype != LLATTN_BF16) return fail(LLATTN_ERR_ARG, "unknown dtype %d", a->dtype);
+  if (a->padding >= a->vocab) return fail(LLATTN_ERR_ARG, "embed: padding %lld outside the vocabulary", (long long)a->padding);
+  if ((a->positions || a->dpositions) && a->position_rows < a->length)
+    return fail(LLATTN_ERR_ARG, "embed: %d position rows for a length of %d", a->position_rows, a->length);
+  return LLATTN_OK;
+}
+
+size_t llattn_embed_workspace_bytes(const llattn_embed_args* a) { return check_embed(a) ? 0 : embed::workspace_bytes(*a); }
+
+int llattn_embed_fwd(const llattn_embed_args* a, void* stream) {
+  int rc = check_embed(a);
+  if (rc) return rc;
+  if (!a->ids || !a->w || !a->out) return fail(LLATTN_ERR_ARG, "llattn_embed_fwd: NULL pointer in args");
+  if (a->ldw < a->d || (a->positions && a->ldp < a->d))
+    return fail(LLATTN_ERR_ARG, "embed: row strides (%lld, %lld) below d = %d", (long long)a->ldw, (long long)a->ldp, a->d);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prof::Scope ps(prof::EMBED, s);
+  return check_launch(embed::launch_fwd(*a, s), "embed_fwd");
+}
+
+int llattn_embed_bwd(const llattn_embed_args* a, void* stream) {
+  int rc = check_embed(a);
+  if (rc) return rc;
+  if (!a->dout || (a->dw && !a->ids)) return fail(LLATTN_ERR_ARG, "llattn_embed_bwd: NULL pointer in args");
+  if (!a->dw && !a->dpositions) return fail(LLATTN_ERR_ARG, "llattn_embed_bwd: no output asked for");
+  const size_t need = embed::workspace_bytes(*a);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_bwd: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
+  if (!al(a->workspace, 256)) return fail(LLATTN_ERR_ALIGN, "llattn_embed_bwd: workspace must be 256-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prof::Scope ps(prof::EMBED, s, embed::launches(*a, true));
+  return check_launch(embed::launch_bwd(*a, s), "embed_bwd");
+}
+
+static int check_clip(const llattn_clip_args* a) {
+  if (!a) return fail(LLATTN_ERR_ARG, "args is NULL");
+  if (a->count < 0) return fail(LLATTN_ERR_ARG, "clip: count must be >= 0");
+  if (a->count && (!a->tensors || !a->sizes || !a->dtypes)) return fail(LLATTN_ERR_ARG, "clip: NULL pointer in args");
+  if (a->norm_type != LLATTN_NORM_2 && a->norm_type != LLATTN_NORM_INF)
+    return fail(LLATTN_ERR_ARG, "clip: unknown norm %d", a->norm_type);
+  if (a->scale && !(a->max_norm >= 0.0)) return fail(LLATTN_ERR_ARG, "clip: max_norm must be >= 0");
+  for (int i = 0; i < a->count; ++i) {
+    if (a->dtypes[i] != LLATTN_F32 && a->dtypes[i] != LLATTN_BF16)
+      return fail(LLATTN_ERR_ARG, "clip: tensor %d has unknown dtype %d", i, a->dtypes[i]);
+    if (a->sizes[i] < 0 || a->sizes[i] > ((int64_t)1 << 42))
+      return fail(LLATTN_ERR_ARG, "clip: tensor %d of %lld elements", i, (long long)a->sizes[i]);
+    if (a->sizes[i] && !a->tensors[i]) return fail(LLATTN_ERR_ARG, "clip: tensor %d is NULL", i);
+    if (a->sizes[i] && !al(a->tensors[i], a->dtypes[i] == LLATTN_BF16 ? 2 : 4))
+      return fail(LLATTN_ERR_ALIGN, "clip: tensor %d is not aligned to its elements", i);
+  }
+  return LLATTN_OK;
+}
+
+// Whether any two of the tensors share memory: an element would be scaled twice, or half way.
+static int check_apart(const llattn_clip_args* a) {
+  struct Run {
+    uintptr_t p, end;
+    int i;
+  };
+  std::unique_ptr<Run[]> r(new (std::nothrow) Run[a->count + 1]);
+  if (!r) return fail(LLATTN_ERR_ARG, "clip: no host memory for %d tensors", a->count);
+  int n = 0;
+  bool sorted = true;  // (as the tensors of one bucket are)
+  for (int i = 0; i < a->count; ++i) {
+    if (!a->sizes[i]) continue;
+    const uintptr_t p = (uintptr_t)a->tensors[i];
+    r[n] = {p, p + (uintptr_t)a->sizes[i] * (a->dtypes[i] == LLATTN_BF16 ? 2 : 4), i};
+    sorted = sorted && (n == 0 || r[n - 1].p <= p);
+    ++n;
+  }
+  if (!sorted) std::sort(r.get(), r.get() + n, [](const Run& x, const Run& y) { return x.p < y.p; });
+  for (int k = 1; k < n; ++k)
+    if (r[k - 1].end > r[k].p)
+      return fail(LLATTN_ERR_ARG, "clip: tensors %d and %d share memory", std::min(r[k - 1].i, r[k].i),
+                  std::max(r[k - 1].i, r[k].i));
+  return LLATTN_OK;
+}
+
+size_t llattn_clip_workspace_bytes(const llattn_clip_args* a) { return check_clip(a) ? 0 : clip::workspace_bytes(*a); }
+
+int llattn_clip(const llattn_clip_args* a, void* stream) {
+  int rc = check_clip(a);
+  if (rc) return rc;
+  if (!a->norm) return fail(LLATTN_ERR_ARG, "llattn_clip: NULL pointer in args");
+  if (a->scale && (rc = check_apart(a))) return rc;
+  const size_t need = clip::workspace_bytes(*a);
+  if (!a->workspace || a->workspace_bytes < need)
+    return fail(LLATTN_ERR_WORKSPACE, "llattn_clip: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
+  if (!al(a->workspace, 256)) return fail(LLATTN_ERR_ALIGN, "llattn_clip: workspace must be 256-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prof::Scope ps(prof::CLIP, s, clip::launches(*a));
+  return check_launch(clip::launch(*a, s), "clip");
+}
 
 // ---------------------------------------------------------------------------
 // llattn_bwd_noalloc: the backward for callers that must not allocate device

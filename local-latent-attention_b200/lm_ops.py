@@ -12,13 +12,13 @@ subclasses, which plain eager calls leave out.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Iterable, Optional, Sequence, Union
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from .ops import _dtype_code, _require
+from .ops import _DT, _dtype_code, _require
 from .training_ops import _direct, _on, _rows, _stream
 
 _PLAIN = torch.contiguous_format
@@ -184,3 +184,261 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     else:
         y = (_gated_fwd if _direct(x2, w_gate, w_up, w_down) else gated_mlp_op)(x2, w_gate, w_up, w_down, act, False)[0]
     return y if flat else y.view(*x.shape[:-1], w_down.shape[0])
+
+
+# --------------------------------------------------------------------------
+# token embedding
+
+_IDS = {torch.int64: 1, torch.int32: 0}
+
+
+def _embed_args(ids: Tensor, w: Tensor, rows: int, scale: float, padding: int):
+    length = ids.shape[1]
+    return _lib.EmbedArgs(ids.shape[0], length, w.shape[1], _dtype_code(w), _IDS[ids.dtype], rows, w.shape[0], padding, scale,
+                          ids.data_ptr())
+
+
+def _check_embed(ids: Tensor, w: Tensor, pos: Optional[Tensor]) -> None:
+    if (w.is_cuda and ids.dim() == 2 and w.dim() == 2 and ids.dtype in _IDS and w.dtype in _TYPES and ids.device == w.device
+            and w.numel() and (pos is None or (pos.dim() == 2 and pos.shape[0] >= ids.shape[1] and pos.shape[1] == w.shape[1]
+                                               and pos.dtype == w.dtype and pos.device == w.device))):
+        return
+    _require(w.is_cuda, "token_embedding needs CUDA tensors")
+    _require(ids.dtype in _IDS, f"ids must be int64 or int32, got {ids.dtype}")
+    _require(w.dim() == 2, f"weight must be [vocab, d], got {tuple(w.shape)}")
+    _dtype_code(w)
+    _require(w.numel() > 0, "weight must have rows and columns")
+    if pos is not None:
+        _require(pos.dim() == 2 and pos.shape[0] >= ids.shape[1] and pos.shape[1] == w.shape[1],
+                 f"positions {tuple(pos.shape)} must be [at least {ids.shape[1]}, {w.shape[1]}]")
+        _require(pos.dtype == w.dtype, f"weight is {w.dtype} and positions {pos.dtype}: one dtype is needed")
+    _require(False, "ids, weight and positions must be on one device")
+
+
+def _embed_fwd(ids: Tensor, w: Tensor, pos: Optional[Tensor], scale: float) -> Tensor:
+    """ids [batch, length] -> [batch, length, d]."""
+    _check_embed(ids, w, pos)
+    out = torch.empty(*ids.shape, w.shape[1], dtype=w.dtype, device=w.device)
+    if out.numel():
+        ids, w = ids.contiguous(), _rows(w)
+        pos = None if pos is None else _rows(pos)
+        args = _embed_args(ids, w, 0 if pos is None else pos.shape[0], scale, -1)
+        args.w, args.ldw, args.out = w.data_ptr(), max(w.stride(0), w.shape[1]), out.data_ptr()
+        if pos is not None:
+            args.positions, args.ldp = pos.data_ptr(), max(pos.stride(0), pos.shape[1])
+        with _on(w.device):
+            _lib.check(_lib.lib().llattn_embed_fwd(ctypes.byref(args), _stream(w)), "llattn_embed_fwd")
+    return out
+
+
+def _embed_bwd(ids: Tensor, dout: Tensor, vocab: int, position_rows: int, scale: float, padding: int, need_w: bool,
+               need_p: bool) -> tuple[Tensor, Tensor]:
+    """dweight and dpositions where needed (else empty)."""
+    d = dout.shape[2]
+    make = torch.empty if dout.numel() else torch.zeros
+    dw = make((vocab, d) if need_w else (0,), dtype=dout.dtype, device=dout.device)
+    dp = make((position_rows, d) if need_p else (0,), dtype=dout.dtype, device=dout.device)
+    if dout.numel() and (need_w or need_p):
+        ids, dout = ids.contiguous(), dout.contiguous()
+        args = _lib.EmbedArgs(*ids.shape, d, _dtype_code(dout), _IDS[ids.dtype], position_rows, vocab, padding, scale,
+                              ids.data_ptr())
+        args.dout, args.dw, args.dpositions = (dout.data_ptr(), dw.data_ptr() if need_w else None,
+                                               dp.data_ptr() if need_p else None)
+        L, ref = _lib.lib(), ctypes.byref(args)
+        with _on(dout.device):
+            size = L.llattn_embed_workspace_bytes(ref) or 256
+            ws = torch.empty(size, dtype=torch.uint8, device=dout.device)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), size
+            _lib.check(L.llattn_embed_bwd(ref, _stream(dout)), "llattn_embed_bwd")
+    return dw, dp
+
+
+token_embedding_op = torch.library.custom_op("llattn_b200::token_embedding", _embed_fwd, mutates_args=(), device_types="cuda")
+token_embedding_grads_op = torch.library.custom_op("llattn_b200::token_embedding_grads", _embed_bwd, mutates_args=(),
+                                                   device_types="cuda")
+
+
+@token_embedding_op.register_fake
+def _embed_fake(ids, w, pos, scale):
+    return w.new_empty(*ids.shape, w.shape[1])
+
+
+@token_embedding_grads_op.register_fake
+def _embed_grads_fake(ids, dout, vocab, position_rows, scale, padding, need_w, need_p):
+    d = dout.shape[2]
+    return (dout.new_empty((vocab, d) if need_w else (0,)), dout.new_empty((position_rows, d) if need_p else (0,)))
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, w, pos, scale, padding):
+        f = _embed_fwd if _direct(ids, w, *(() if pos is None else (pos,))) else token_embedding_op
+        ctx.save_for_backward(ids)
+        ctx.cfg = (w.shape[0], 0 if pos is None else pos.shape[0], scale, padding)
+        return f(ids, w, pos, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        _, need_w, need_p = ctx.needs_input_grad[:3]
+        f = _embed_bwd if _direct(ids, dout) else token_embedding_grads_op
+        dw, dp = f(ids, dout, *ctx.cfg, need_w, need_p)
+        return None, dw if need_w else None, dp if need_p else None, None, None
+
+
+def token_embedding(ids: Tensor, weight: Tensor, *, positions: Optional[Tensor] = None, scale: float = 1.0,
+                    padding_idx: Optional[int] = None) -> Tensor:
+    """Rows of an embedding: ``scale * weight[ids]``, plus ``positions[t]`` for the t-th
+    id along ids' last dimension; differentiable in weight and positions
+    (gradients of gradients are not supported).
+
+    ids [...] int64 or int32, weight [vocab, d] bfloat16 or float32, positions
+    [at least ids.shape[-1], d] in weight's dtype; any row strides. Returns [..., d]
+    in weight's dtype (autocast does not change it, as it does not change
+    torch's embedding). At most 2^30 ids, 2^24 words.
+
+    weight's gradient sums the tokens of each word in fp32 in the order of the tokens: the same
+    bits every run. Tokens of the word padding_idx (which may count from the end)
+    do not take part in it. An id outside [0, vocab) makes its row NaN and has no
+    gradient (it is an error that no launch can raise)."""
+    _require(ids.dim() >= 1 or positions is None, "positions need ids with a dimension")
+    if weight.dim() != 2:
+        _require(False, f"weight must be [vocab, d], got {tuple(weight.shape)}")
+    padding = -1
+    if padding_idx is not None:
+        vocab = weight.shape[0]
+        _require(-vocab <= padding_idx < vocab, f"padding_idx {padding_idx} outside the {vocab} words")
+        padding = padding_idx % vocab
+    scale = float(scale)
+    ids2 = ids if ids.dim() == 2 else ids.reshape(-1, ids.shape[-1] if ids.dim() and ids.shape[-1] else 1)
+    if torch.is_grad_enabled() and (weight.requires_grad or (positions is not None and positions.requires_grad)):
+        out = _Embed.apply(ids2, weight, positions, scale, padding)
+    else:
+        f = _embed_fwd if _direct(ids2, weight, *(() if positions is None else (positions,))) else token_embedding_op
+        out = f(ids2, weight, positions, scale)
+    return out if ids.dim() == 2 else out.view(*ids.shape, weight.shape[1])
+
+
+# --------------------------------------------------------------------------
+# norm over many tensors, clipping
+
+_NORMS = {2.0: _lib.NORM_2, float("inf"): _lib.NORM_INF}
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether t's elements are numel() consecutive ones, in whatever order."""
+    if t.is_contiguous():
+        return True
+    run = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def _check_tensors(tensors: Sequence[Tensor], what: str) -> None:
+    device = tensors[0].device
+    _require(device.type == "cuda", f"{what} needs CUDA tensors")
+    for t in tensors:
+        if t.dtype not in _DT or t.device != device or t.layout != torch.strided:
+            _require(t.device == device, f"{what} needs tensors of one device, got {device} and {t.device}")
+            _require(t.layout == torch.strided, f"{what} needs dense tensors, got {t.layout}")
+            _dtype_code(t)
+
+
+def _clip(tensors: Sequence[Tensor], norm_type: int, max_norm: float, scale: bool) -> Tensor:
+    """tensors: dense, of one device and not empty as a list."""
+    n, device = len(tensors), tensors[0].device
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    args = _lib.ClipArgs(n, norm_type, scale, (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
+                         (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
+                         (ctypes.c_int32 * n)(*[_DT[t.dtype] for t in tensors]), max_norm, norm.data_ptr())
+    L, ref = _lib.lib(), ctypes.byref(args)
+    with _on(device):
+        size = L.llattn_clip_workspace_bytes(ref)
+        ws = torch.empty(size or 256, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), size or 256
+        _lib.check(L.llattn_clip(ref, _stream(norm)), "llattn_clip")
+    return norm
+
+
+def _norm_of(tensors: list[Tensor], norm_type: int) -> Tensor:
+    _check_tensors(tensors, "total_norm")
+    return _clip([t if _dense(t) else t.contiguous() for t in tensors], norm_type, 0.0, False)
+
+
+def _clip_of(grads: list[Tensor], max_norm: float, norm_type: int) -> Tensor:
+    _check_tensors(grads, "clip_grad_norm_")
+    dense = [g if _dense(g) else g.contiguous() for g in grads]
+    norm = _clip(dense, norm_type, max_norm, True)
+    for g, c in zip(grads, dense):
+        if c is not g:
+            g.copy_(c)
+    return norm
+
+
+total_norm_op = torch.library.custom_op("llattn_b200::total_norm", _norm_of, mutates_args=(), device_types="cuda",
+                                        schema="(Tensor[] tensors, int norm_type) -> Tensor")
+clip_grads_op = torch.library.custom_op("llattn_b200::clip_grads_", _clip_of, mutates_args=("grads",), device_types="cuda",
+                                        schema="(Tensor(a!)[] grads, float max_norm, int norm_type) -> Tensor")
+
+
+@total_norm_op.register_fake
+def _norm_fake(tensors, norm_type):
+    return tensors[0].new_empty((), dtype=torch.float32)
+
+
+@clip_grads_op.register_fake
+def _clip_fake(grads, max_norm, norm_type):
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+def _norm_code(norm_type) -> int:
+    code = _NORMS.get(float(norm_type))
+    _require(code is not None, f"norm_type must be 2 or inf, got {norm_type!r}")
+    return code
+
+
+@torch.no_grad()
+def total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
+    """The norm of all tensors' elements together, as a float32 scalar on their
+    device: the 2-norm (sums in fp64, in a fixed order; finite for any finite float32
+    result) or, for norm_type=inf, the largest magnitude. NaN where one of them is.
+    Tensors are bfloat16 or float32, of any shapes and mix, on one CUDA device; 0
+    on the CPU for an empty list."""
+    code = _norm_code(norm_type)
+    tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    return (_norm_of if _direct(*tensors) else total_norm_op)(tensors, code)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> Tensor:
+    """torch.nn.utils.clip_grad_norm_ in two launches: the norm of all gradients
+    together (``total_norm``), and every gradient times min(1, max_norm / (norm + 1e-6))
+    in place, untouched where that is 1. Returns the norm, a float32 scalar on the
+    gradients' device.
+
+    Gradients are bfloat16 or float32, of any mix and layout, on one CUDA device; no two may
+    share memory. Parameters without a gradient are skipped, one given twice counts
+    once. norm_type: 2 or inf. A norm that is not finite makes the gradients NaN or 0, as
+    torch's does; error_if_nonfinite raises instead, before they change (it waits for the
+    device)."""
+    code = _norm_code(norm_type)
+    max_norm = float(max_norm)
+    _require(max_norm >= 0, f"max_norm must be >= 0, got {max_norm}")
+    parameters = [parameters] if isinstance(parameters, Tensor) else dict.fromkeys(parameters)
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    direct = _direct(*grads)
+    if error_if_nonfinite:
+        norm = (_norm_of if direct else total_norm_op)(grads, code)
+        if not torch.isfinite(norm):
+            raise RuntimeError(f"llattn: the total norm of order {norm_type} of the gradients is not finite, so they cannot "
+                               "be clipped; error_if_nonfinite=False scales them all the same")
+    return (_clip_of if direct else clip_grads_op)(grads, max_norm, code)

@@ -73,3 +73,81 @@ def test_gated_mlp_on_the_cpu_is_refused():
         llattn_b200.gated_mlp(x, w, w, w)
     with pytest.raises(RuntimeError, match="activation"):
         llattn_b200.gated_mlp(x, w, w, w, activation="tanh")
+
+
+# --- token embedding ------------------------------------------------------------------
+
+def embed_args(**kw):
+    base = dict(batch=3, length=5, d=16, dtype=_lib.F32, ids_wide=1, position_rows=8, vocab=100, padding=-1, scale=1.0, ids=1 << 20,
+                w=2 << 20, ldw=16, positions=3 << 20, ldp=16, out=4 << 20, dout=5 << 20, dw=6 << 20, dpositions=7 << 20,
+                workspace=None, workspace_bytes=0)
+    base.update(kw)
+    return _lib.EmbedArgs(*base.values())
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(batch=0), ">= 1"), (dict(length=0), ">= 1"), (dict(d=0), ">= 1"), (dict(vocab=0), ">= 1"), (dict(dtype=3), "dtype"),
+    (dict(batch=1 << 20, length=1 << 11, position_rows=1 << 11), "too large"), (dict(vocab=(1 << 24) + 1), "too large"),
+    (dict(padding=100), "padding"), (dict(position_rows=4), "position rows"),
+])
+def test_embed_refusals(bad, msg):
+    L = _lib.lib()
+    refused(L.llattn_embed_fwd(ctypes.byref(embed_args(**bad)), None), msg)
+    refused(L.llattn_embed_bwd(ctypes.byref(embed_args(**bad)), None), msg)
+    assert L.llattn_embed_workspace_bytes(ctypes.byref(embed_args(**bad))) == 0
+
+
+@pytest.mark.parametrize("bad,msg", [(dict(ids=None), "NULL"), (dict(w=None), "NULL"), (dict(out=None), "NULL"),
+                                     (dict(ldw=15), "row strides"), (dict(ldp=15), "row strides")])
+def test_embed_forward_refusals(bad, msg):
+    refused(_lib.lib().llattn_embed_fwd(ctypes.byref(embed_args(**bad)), None), msg)
+
+
+@pytest.mark.parametrize("bad,msg", [(dict(dout=None), "NULL"), (dict(ids=None), "NULL"), (dict(dw=None, dpositions=None), "no output"),
+                                     (dict(), "workspace of"),
+                                     (dict(workspace=(1 << 30) + 8, workspace_bytes=1 << 40), "aligned")])
+def test_embed_backward_refusals(bad, msg):
+    refused(_lib.lib().llattn_embed_bwd(ctypes.byref(embed_args(**bad)), None), msg)
+
+
+# --- norm and clipping ----------------------------------------------------------------
+
+def clip_args(ptrs, lens, codes, **kw):
+    n = len(ptrs)
+    base = dict(count=n, norm_type=_lib.NORM_2, scale=1, tensors=(ctypes.c_void_p * n)(*ptrs), sizes=(ctypes.c_int64 * n)(*lens),
+                dtypes=(ctypes.c_int32 * n)(*codes), max_norm=1.0, norm=1 << 20, workspace=None, workspace_bytes=0)
+    base.update(kw)
+    return _lib.ClipArgs(*base.values())
+
+
+@pytest.mark.parametrize("lists,kw,msg", [
+    (([4096], [4], [_lib.F32]), dict(count=-1), "count"), (([4096], [4], [_lib.F32]), dict(norm_type=2), "norm"),
+    (([4096], [4], [_lib.F32]), dict(max_norm=-0.5), "max_norm"), (([4096], [4], [_lib.F32]), dict(max_norm=float("nan")), "max_norm"),
+    (([4096], [4], [5]), {}, "dtype"), (([4096], [-1], [0]), {}, "elements"), (([None], [4], [0]), {}, "NULL"),
+    (([4098], [4], [0]), {}, "aligned"), (([4097], [4], [1]), {}, "aligned"), (([4096], [4], [0]), dict(norm=None), "NULL"),
+    (([4096], [4], [0]), dict(tensors=None), "NULL"), (([4096, 4104], [4, 4], [0, 0]), {}, "tensors 0 and 1 share"),
+    (([8192, 4096, 8190], [4, 100, 2], [1, 1, 1]), {}, "tensors 0 and 2 share"), (([4096, 4112], [4, 4], [0, 0]), {}, "workspace of"),
+    (([4096, 4096], [4, 0], [0, 0]), {}, "workspace of"), (([4096, 4096], [4, 4], [0, 0]), dict(scale=0), "workspace of"),
+    (([4096], [4], [0]), dict(workspace=(1 << 30) + 8, workspace_bytes=1 << 40), "aligned"),
+])
+def test_clip_refusals(lists, kw, msg):
+    refused(_lib.lib().llattn_clip(ctypes.byref(clip_args(*lists, **kw)), None), msg)
+
+
+def test_lm_ops_on_the_cpu_are_refused():
+    with pytest.raises(RuntimeError, match="CUDA"):
+        llattn_b200.token_embedding(torch.zeros(2, 3, dtype=torch.long), torch.randn(4, 8))
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        llattn_b200.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        llattn_b200.total_norm([p])
+
+
+def test_dense_layouts():
+    from llattn_b200.lm_ops import _dense
+    t = torch.zeros(4, 5, 6)
+    assert _dense(t) and _dense(t.permute(2, 0, 1)) and _dense(t[1:3]) and _dense(t[:, :, :1][:, :1]) is False
+    assert not _dense(t[:, 1:3]) and not _dense(torch.zeros(1).expand(3)) and _dense(torch.zeros(3, 1).expand(3, 1))
+    assert _dense(torch.zeros(0, 3)) and not _dense(t[..., ::2])
