@@ -12,7 +12,7 @@
 //
 // Roundings, bf16: h, dg and du are rounded to bf16 to be operands, and the
 // result once more, which is sqrt(2) of the result's own rounding. g and u
-// are kept in fp16 with a power of two for every 32 of them (11 bits relative
+// are kept in fp16 with a power of two for every 16 of them (11 bits relative
 // to their largest, 4 bytes an inner column and token as bf16 would take): in bf16 they
 // would add another rounding to dg and du each (dx 1.75 times its own). Up
 // to kFine tokens keep h, dg and du in two bf16 planes, as little averages
@@ -38,9 +38,10 @@ using namespace mm;
 constexpr int kFine = 64, kFew = 32;
 // K = 64 steps a tensor-core sum takes (MmArgs::chain) in fp32: as the loss's products (xent.cu)
 constexpr int kFineF32Chain = 1, kF32Chain = 4;
-constexpr int kBlock = 32;  // inner columns of a kept block
+constexpr int kBlock = 16;  // inner columns of a kept block
 
-// act(g) and act'(g). EXACT: to fp32's last bits; otherwise ex2's and rcp's 2^-22.
+// act(g) and act'(g). EXACT: to fp32's last bits; otherwise ex2's and rcp's 2^-22, and
+// erf by Abramowitz and Stegun's 7.1.26 (1.5e-7), which shares its exponential with the density.
 template <int ACT, bool EXACT>
 __device__ __forceinline__ void activation(float g, float& a, float& slope) {
   if (ACT == LLATTN_ACT_SILU) {
@@ -48,55 +49,75 @@ __device__ __forceinline__ void activation(float g, float& a, float& slope) {
     const float s = EXACT ? 1.f / (1.f + e) : __fdividef(1.f, 1.f + e);
     a = g * s;
     slope = s * (1.f + g * (1.f - s));
-  } else {
+  } else if (EXACT) {
     const float phi = 0.5f * erfcf(g * -0.70710678f);
-    const float p = 0.39894228f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
     a = g * phi;
-    slope = phi + g * p;
+    slope = phi + g * (0.39894228f * expf(-0.5f * g * g));
+  } else {
+    const float e = fast_exp2(g * g * -0.72134752f);
+    const float t = __fdividef(1.f, fmaf(fabsf(g), 0.3275911f * 0.70710678f, 1.f));
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    q *= 0.5f * t * e;
+    const float phi = g > 0.f ? 1.f - q : q;
+    a = g * phi;
+    slope = phi + g * (0.39894228f * e);
   }
 }
-template <int ACT, bool EXACT>
-__device__ __forceinline__ float activate(float g) {
-  float a, slope;
-  activation<ACT, EXACT>(g, a, slope);
-  return a;
-}
 
-// Kept g and u of a (token, block of 32 inner columns): 32 values of g, then of u.
-// bf16 inputs: fp16 times 2^(s - 127), s a byte for g and for u each, chosen so
-// that the largest lies in [2^14, 2^15); fp32 inputs: as they are.
+// Kept g and u: for every 32 tokens and 16 inner columns a block of 16-byte chunks, lane by
+// lane (token by token), so that the warp that wrote it and the one that reads it
+// each move whole lines without going through shared memory: a token's 16 values of g,
+// then of u. bf16 inputs: fp16 times 2^(s - 127), s a byte for g and for u each,
+// chosen so that the largest of the 16 lies in [2^14, 2^15); fp32 inputs: as they are.
 struct Kept {
-  void* gu;         // [tokens][blocks][2][32]
-  uint16_t* scale;  // [tokens][blocks] (bf16)
+  uint8_t* gu;      // [token groups][blocks][4 or 8 chunks][32][16]
+  uint16_t* scale;  // [token groups][blocks][32] (bf16)
   int blocks;
 };
-__device__ __forceinline__ uint32_t block_scale(const float (&v)[32]) {
+__device__ __forceinline__ uint32_t block_scale(const float (&v)[16]) {
   float m = 0.f;
 #pragma unroll
-  for (int q = 0; q < 32; ++q) m = fmaxf(m, fabsf(v[q]));
+  for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(v[q]));
   const int e = __float_as_uint(m) >> 23;  // 2^(e - 127) <= m
   return (uint32_t)min(253, 127 + 14 + 127 - e);
 }
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
 __device__ __forceinline__ float unscale_of(uint32_t s) { return __uint_as_float((254u - s) << 23); }
 
-// rows of n columns in P bf16 planes (P = 1: rounded), 32 columns of a warp's 32 rows
+// 16 columns of this thread's row
+__device__ __forceinline__ void load16(uint32_t taddr, bool zero, float (&v)[16]) {
+  uint32_t r[16];
+  if (!zero) {
+    tmem_ld16(taddr, r);
+    tmem_ld_wait();
+  }
+#pragma unroll
+  for (int q = 0; q < 16; ++q) v[q] = zero ? 0.f : __uint_as_float(r[q]);
+}
+// v rounded to bf16, and, for more planes, what that leaves of it
+template <bool REST>
+__device__ __forceinline__ void round16(float (&v)[16], uint32_t* w) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
+    if (REST) {
+      v[2 * q] -= __uint_as_float(w[q] << 16);
+      v[2 * q + 1] -= __uint_as_float(w[q] & 0xffff0000u);
+    }
+  }
+}
+// 16 columns in P > 1 planes, z, z + dz, ...
 template <int P>
-__device__ __forceinline__ void store_planes(uint8_t* buf, int lane, float (&v)[32], const Rows& dst, int64_t plane_bytes,
-                                             int n) {
+__device__ __forceinline__ void send_planes(Outgoing<16>& out, const CUtensorMap* map, float (&v)[16], int col, int row, int z,
+                                            int dz) {
 #pragma unroll
   for (int k = 0; k < P; ++k) {
-    uint4 u[4];
-    bf16_row(v, u);
-    block_store(buf, lane, u, Rows{dst.p + k * plane_bytes, dst.stride, dst.rows}, n * 2);
-    if (k + 1 < P) {
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const float2 r = bf16_pair(u, q);
-        v[2 * q] -= r.x;
-        v[2 * q + 1] -= r.y;
-      }
-    }
+    uint32_t w[8];
+    round16<true>(v, w);
+    out.send(map, w, col, row, z + k * dz);
   }
 }
 
@@ -105,56 +126,74 @@ __device__ __forceinline__ void store_planes(uint8_t* buf, int lane, float (&v)[
 // P: planes of h (3: fp32 inputs)
 template <int ACT, int P>
 struct EpiGated {
-  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false, kBulkOut = true;
   static constexpr int kSecond = kSecondHalves;
   static constexpr bool F32 = P == 3;
+  static constexpr int COLS = P == 1 ? 32 : 16;  // of a block sent out
   struct Pre {};
   __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
+  CUtensorMap h;  // [P][tokens][ff]
+  Kept kept;      // gu null: nothing is kept
   int ff;
-  bf16* h;  // [P][tokens][ldh]
-  int64_t ldh, hplane;
-  Kept kept;  // gu null: nothing is kept
 
-  template <int CW>
-  __device__ __forceinline__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
-                                       uint8_t* buf, Pre&) const {
-    static_assert(CW >= 2 * kBlock, "whole blocks of g");
-    constexpr int G = CW / 2;
-    const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0, f0 = col0 / 2;
-#pragma unroll 1
-    for (int cc = 0; cc < G; cc += 32) {
-      const int n = ff - f0 - cc;
-      if (n <= 0) break;  // warp-uniform
-      float g[32], u[32];
-      load32(taddr + cc, zero, g);
-      load32(taddr + G + cc, zero, u);
-      if (kept.gu) {
-        const int64_t at = (int64_t)row0 * kept.blocks + (f0 + cc) / 32;
-        if constexpr (F32) {
-          uint4 w[8];
-          const Rows dst{static_cast<float*>(kept.gu) + at * 64, kept.blocks * (int64_t)256, rows};
-          f32_row(g, w);
-          block_store(buf, lane, w, dst, 128);
-          f32_row(u, w);
-          block_store(buf, lane, w, dst.at(128), 128);
-        } else {
-          const uint32_t sg = block_scale(g), su = block_scale(u);
-          const float fg = scale_of(sg), fu = scale_of(su);
-          uint4 w[8];
+  __device__ __forceinline__ void keep(const float (&g)[16], const float (&u)[16], int row0, int col, int lane) const {
+    const int64_t at = (int64_t)(row0 / 32) * kept.blocks + col / 16;
+    if constexpr (F32) {
+      uint4* dst = reinterpret_cast<uint4*>(kept.gu + at * 4096) + lane;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            w[q] = make_uint4(pack_half(g[8 * q] * fg, g[8 * q + 1] * fg), pack_half(g[8 * q + 2] * fg, g[8 * q + 3] * fg),
-                              pack_half(g[8 * q + 4] * fg, g[8 * q + 5] * fg), pack_half(g[8 * q + 6] * fg, g[8 * q + 7] * fg));
-            w[q + 4] = make_uint4(pack_half(u[8 * q] * fu, u[8 * q + 1] * fu), pack_half(u[8 * q + 2] * fu, u[8 * q + 3] * fu),
-                                  pack_half(u[8 * q + 4] * fu, u[8 * q + 5] * fu), pack_half(u[8 * q + 6] * fu, u[8 * q + 7] * fu));
-          }
-          block_store(buf, lane, w, Rows{static_cast<__half*>(kept.gu) + at * 64, kept.blocks * (int64_t)128, rows}, 128);
-          if (row < M) kept.scale[at + (int64_t)lane * kept.blocks] = (uint16_t)(sg | su << 8);
-        }
+      for (int c = 0; c < 4; ++c) {
+        dst[32 * c] = make_uint4(__float_as_uint(g[4 * c]), __float_as_uint(g[4 * c + 1]), __float_as_uint(g[4 * c + 2]),
+                                 __float_as_uint(g[4 * c + 3]));
+        dst[32 * c + 128] = make_uint4(__float_as_uint(u[4 * c]), __float_as_uint(u[4 * c + 1]), __float_as_uint(u[4 * c + 2]),
+                                       __float_as_uint(u[4 * c + 3]));
       }
+    } else {
+      uint4* dst = reinterpret_cast<uint4*>(kept.gu + at * 2048) + lane;
+      const uint32_t sg = block_scale(g), su = block_scale(u);
+      const float fg = scale_of(sg), fu = scale_of(su);
 #pragma unroll
-      for (int q = 0; q < 32; ++q) g[q] = activate<ACT, F32>(g[q]) * u[q];
-      store_planes<P>(buf, lane, g, Rows{h + (int64_t)row0 * ldh + f0 + cc, ldh * 2, rows}, hplane * 2, n);
+      for (int c = 0; c < 2; ++c) {
+        const float *x = g + 8 * c, *y = u + 8 * c;
+        dst[32 * c] = make_uint4(pack_half(x[0] * fg, x[1] * fg), pack_half(x[2] * fg, x[3] * fg),
+                                 pack_half(x[4] * fg, x[5] * fg), pack_half(x[6] * fg, x[7] * fg));
+        dst[32 * c + 64] = make_uint4(pack_half(y[0] * fu, y[1] * fu), pack_half(y[2] * fu, y[3] * fu),
+                                      pack_half(y[4] * fu, y[5] * fu), pack_half(y[6] * fu, y[7] * fu));
+      }
+      kept.scale[at * 32 + lane] = (uint16_t)(sg | su << 8);
+    }
+  }
+
+  template <int CW, int BR>
+  __device__ __forceinline__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero, uint8_t* buf,
+                                       Pre&) const {
+    constexpr int W = CW / 2;  // of the BR columns: BR / 2 of g, BR / 2 of u; this warp's: W of each
+    static_assert(W >= 32, "whole blocks");
+    const int lane = threadIdx.x % 32, row0 = row - lane, o = col0 % BR, f0 = (col0 - o) / 2 + o / 2;
+    if (row0 >= M) return;  // warp-uniform
+    const uint32_t gt = taddr - o + o / 2, ut = gt + BR / 2;
+    Outgoing<COLS> out(buf, lane);
+#pragma unroll 1
+    for (int cc = 0; cc < W; cc += COLS) {
+      if (f0 + cc >= ff) break;  // warp-uniform
+      uint32_t w[COLS / 2];
+#pragma unroll
+      for (int c = 0; c < COLS; c += 16) {
+        float g[16], u[16];
+        load16(gt + cc + c, zero, g);
+        load16(ut + cc + c, zero, u);
+        if (kept.gu && f0 + cc + c < ff) keep(g, u, row0, f0 + cc + c, lane);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          float a, slope;
+          activation<ACT, F32>(g[q], a, slope);
+          g[q] = a * u[q];
+        }
+        if constexpr (P == 1)
+          round16<false>(g, w + c / 2);
+        else
+          send_planes<P>(out, &h, g, f0 + cc + c, row0, 0, 1);
+      }
+      if constexpr (P == 1) out.send(&h, w, f0 + cc, row0, 0);
     }
   }
 };
@@ -163,72 +202,93 @@ struct EpiGated {
 
 template <int ACT, int P>
 struct EpiGrad {
-  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false;
+  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false, kBulkOut = true;
   static constexpr bool F32 = P == 3;
-  struct Pre {};
-  __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
+  static constexpr int COLS = P == 1 ? 32 : 16;
+  struct Pre {
+    uint4 x[F32 ? 8 : 4];
+    uint32_t scale;
+  };
+  CUtensorMap dgu, h;  // z = 2 plane + (0: dg, 1: du); z = plane
   Kept kept;
-  bf16* dgu;  // [tokens][P][2][ld] (dg, du), or null
-  int64_t ld;
-  bf16* h;  // [P][tokens][ld], or null
-  int64_t hplane;
+  int inner, down;  // which of them are wanted
+
+  __device__ __forceinline__ void ask(Pre& pre, int row0, int col, int lane) const {
+    const int64_t at = (int64_t)(row0 / 32) * kept.blocks + col / 16;
+    const uint4* src = reinterpret_cast<const uint4*>(kept.gu + at * (F32 ? 4096 : 2048)) + lane;
+#pragma unroll
+    for (int c = 0; c < (F32 ? 8 : 4); ++c) pre.x[c] = src[32 * c];
+    if (!F32) pre.scale = kept.scale[at * 32 + lane];
+  }
+  __device__ __forceinline__ void fetch(Pre& pre, const MmArgs& a, MmTile, int row, int col0, int M) const {
+    const int lane = threadIdx.x % 32;
+    if (row - lane < M && col0 < a.N) ask(pre, row - lane, col0, lane);
+  }
+  static __device__ __forceinline__ void values(const Pre& pre, float (&g)[16], float (&u)[16]) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        g[q] = __uint_as_float(word(pre.x, q));
+        u[q] = __uint_as_float(word(pre.x, q + 16));
+      }
+    } else {
+      const float fg = unscale_of(pre.scale & 255u), fu = unscale_of(pre.scale >> 8);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t wg = word(pre.x, q), wu = word(pre.x, q + 8);
+        const float2 pg = __half22float2(*reinterpret_cast<const __half2*>(&wg));
+        const float2 pu = __half22float2(*reinterpret_cast<const __half2*>(&wu));
+        g[2 * q] = pg.x * fg;
+        g[2 * q + 1] = pg.y * fg;
+        u[2 * q] = pu.x * fu;
+        u[2 * q + 1] = pu.y * fu;
+      }
+    }
+  }
 
   template <int CW>
   __device__ __forceinline__ void tile(const MmArgs& a, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
-                                       uint8_t* buf, Pre&) const {
-    const int lane = threadIdx.x % 32, row0 = row - lane, rows = M - row0;
-    constexpr int CH = 8, HALVES = F32 ? 2 : 1;
-    const int64_t at0 = (int64_t)row0 * kept.blocks + col0 / 32;
-    const Rows src{static_cast<uint8_t*>(kept.gu) + at0 * (128 * HALVES), kept.blocks * (int64_t)(128 * HALVES), rows};
-    uint4 x[CH];
-    uint32_t sc = 0;
-    // the next block is asked for before this one is worked on
-    auto ask = [&](int cc) {
-      block_fetch(lane, x, src.at(cc / 32 * 128 * HALVES), 128);
-      if (!F32 && row < M) sc = kept.scale[at0 + (int64_t)lane * kept.blocks + cc / 32];
-    };
-    if (col0 < a.N) ask(0);
+                                       uint8_t* buf, Pre& pre) const {
+    const int lane = threadIdx.x % 32, row0 = row - lane;
+    if (row0 >= M) return;  // warp-uniform
+    Outgoing<COLS> out(buf, lane);
 #pragma unroll 1
-    for (int cc = 0; cc < CW; cc += 32) {
-      const int n = a.N - col0 - cc;
-      if (n <= 0) break;  // warp-uniform
-      float g[32], u[32], dh[32];
-      block_spread(buf, lane, x);
-      if constexpr (F32) {
+    for (int cc = 0; cc < CW; cc += COLS) {
+      if (col0 + cc >= a.N) break;  // warp-uniform
+      uint32_t wh[COLS / 2], wg[COLS / 2], wu[COLS / 2];
 #pragma unroll
-        for (int q = 0; q < 32; ++q) g[q] = __uint_as_float(word(x, q));
-        block_fetch(lane, x, src.at(cc / 32 * 256 + 128), 128);
-        block_spread(buf, lane, x);
-#pragma unroll
-        for (int q = 0; q < 32; ++q) u[q] = __uint_as_float(word(x, q));
-      } else {
-        const float fg = unscale_of(sc & 255u), fu = unscale_of(sc >> 8);
+      for (int c = 0; c < COLS; c += 16) {
+        const int col = col0 + cc + c;
+        float g[16], u[16], dh[16];
+        values(pre, g, u);
+        if (cc + c + 16 < CW && col + 16 < a.N) ask(pre, row0, col + 16, lane);  // while this block is worked on
+        load16(taddr + cc + c, zero, dh);
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          const uint32_t wg = word(x, q), wu = word(x, q + 16);
-          const float2 pg = __half22float2(*reinterpret_cast<const __half2*>(&wg));
-          const float2 pu = __half22float2(*reinterpret_cast<const __half2*>(&wu));
-          g[2 * q] = pg.x * fg;
-          g[2 * q + 1] = pg.y * fg;
-          u[2 * q] = pu.x * fu;
-          u[2 * q + 1] = pu.y * fu;
+          float act, slope;
+          activation<ACT, F32>(g[q], act, slope);
+          g[q] = act * u[q];
+          u[q] = dh[q] * u[q] * slope;
+          dh[q] *= act;
+        }
+        if constexpr (P == 1) {
+          round16<false>(g, wh + c / 2);
+          round16<false>(u, wg + c / 2);
+          round16<false>(dh, wu + c / 2);
+        } else {
+          if (down) send_planes<P>(out, &h, g, col, row0, 0, 1);
+          if (inner) {
+            send_planes<P>(out, &dgu, u, col, row0, 0, 2);
+            send_planes<P>(out, &dgu, dh, col, row0, 1, 2);
+          }
         }
       }
-      if (cc + 32 < CW && n > 32) ask(cc + 32);
-      load32(taddr + cc, zero, dh);
-#pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        float act, slope;
-        activation<ACT, F32>(g[q], act, slope);
-        g[q] = act * u[q];
-        u[q] = dh[q] * u[q] * slope;
-        dh[q] *= act;
-      }
-      if (h) store_planes<P>(buf, lane, g, Rows{h + (int64_t)row0 * ld + col0 + cc, ld * 2, rows}, hplane * 2, n);
-      if (dgu) {
-        const Rows dst{dgu + (int64_t)row0 * 2 * P * ld + col0 + cc, 4 * P * ld, rows};
-        store_planes<P>(buf, lane, u, dst, 4 * ld, n);
-        store_planes<P>(buf, lane, dh, Rows{dst.p + 2 * ld, dst.stride, rows}, 4 * ld, n);
+      if constexpr (P == 1) {
+        if (down) out.send(&h, wh, col0 + cc, row0, 0);
+        if (inner) {
+          out.send(&dgu, wg, col0 + cc, row0, 0);
+          out.send(&dgu, wu, col0 + cc, row0, 1);
+        }
       }
     }
   }
@@ -433,17 +493,16 @@ Plan make_plan(const llattn_gated_args& a, bool backward) {
 
 Kept kept_at(const Plan& q, const llattn_gated_args& a) {
   Kept k;
-  k.gu = a.kept;
+  k.gu = static_cast<uint8_t*>(a.kept);
   k.blocks = q.blocks;
-  k.scale = reinterpret_cast<uint16_t*>(static_cast<char*>(a.kept) + up256((size_t)a.tokens * q.blocks * 64 * (q.f32 ? 4 : 2)));
+  k.scale = reinterpret_cast<uint16_t*>(k.gu + (size_t)cdiv(a.tokens, 32) * q.blocks * 2048);
   return k;
 }
 
 template <typename T>
 cudaError_t pack(bool needed, const void* src, int64_t ld, int rows, int cols, void* dst, int64_t lds, cudaStream_t s) {
   if (!needed) return cudaSuccess;
-  return launch_pdl(pack_kernel<T>, dim3(cdiv(rows, 8)), 256, 0, 1, s, static_cast<const T*>(src), ld, rows, cols,
-                    static_cast<bf16*>(dst), lds, rows * lds);
+  return launch_pack<T>(src, ld, rows, cols, dst, lds, s);
 }
 
 EpiOut rows_out(const Plan& q, void* out, int cols) {
@@ -455,13 +514,20 @@ EpiOut rows_out(const Plan& q, void* out, int cols) {
   return o;
 }
 
-// The tile of the gated product: at least one kept block of g wide (shape 0 holds 16 columns of g)
-template <int ACT, int P>
-cudaError_t launch_gated(MmArgs p, const Operand& x, const Operand& g, const Operand& u, const EpiGated<ACT, P>& e,
-                         cudaStream_t s) {
+// The tiles of the two products with the activation in their epilogues: shape 5
+// instead of 2, and for g and u at least 32 columns of each to a warp (shape 0 holds 16).
+template <typename Epi>
+cudaError_t launch_active(MmArgs p, const Operand& a, const Operand& b, const Epi& e, cudaStream_t s,
+                          const Operand* b2 = nullptr) {
+  p.a_mn = a.mn;
+  p.b_mn = b.mn;
   const double t2 = mm_time<2>(p), t1 = mm_time<1>(p), t4 = mm_time<4>(p);
-  if (t4 < std::min(t1, t2)) return launch_mm_sh<4>(p, x, g, e, s, &u);
-  return t2 <= t1 ? launch_mm_sh<2>(p, x, g, e, s, &u) : launch_mm_sh<1>(p, x, g, e, s, &u);
+  if constexpr (SecondB<Epi>::value != kSecondHalves) {
+    const double t0 = mm_time<0>(p);
+    if (t0 <= t4 && t0 < std::min(t1, t2)) return launch_mm_sh<0>(p, a, b, e, s, b2);
+  }
+  if (t4 < std::min(t1, t2)) return launch_mm_sh<4>(p, a, b, e, s, b2);
+  return t2 <= t1 ? launch_mm_sh<5>(p, a, b, e, s, b2) : launch_mm_sh<1>(p, a, b, e, s, b2);
 }
 
 template <typename T, int ACT, int P>
@@ -480,11 +546,9 @@ cudaError_t run_fwd(const llattn_gated_args& a, const Plan& q, volatile unsigned
   const int64_t hplane = n * q.ldf;
   EpiGated<ACT, P> e{};
   e.ff = a.ff;
-  e.h = h;
-  e.ldh = q.ldf;
-  e.hplane = hplane;
+  if (!sm100::make_block_map(&e.h, h, n, a.ff, q.ldf, P, hplane, e.COLS)) return cudaErrorInvalidValue;
   if (a.kept) e.kept = kept_at(q, a);
-  TRY(launch_gated(product(q, n, 2 * a.ff, a.d, fault), x, g, u, e, s));
+  TRY(launch_active(product(q, n, 2 * a.ff, a.d, fault), x, g, e, s, &u));
   MmArgs p = y_args(q, a, fault);
   p.part = reinterpret_cast<float*>(ws + q.part);
   return launch_mm(p, Operand{h, n, a.ff, q.ldf, P, hplane, 0}, d, rows_out(q, a.y, a.d_out), s);
@@ -506,11 +570,12 @@ cudaError_t run_bwd(const llattn_gated_args& a, const Plan& q, volatile unsigned
   float* part = reinterpret_cast<float*>(ws + q.part);
   EpiGrad<ACT, P> e{};
   e.kept = kept_at(q, a);
-  e.dgu = a.dx || weights ? dgu : nullptr;
-  e.ld = q.ldf;
-  e.h = a.dw_down ? h : nullptr;
-  e.hplane = hplane;
-  TRY(launch_mm(product(q, n, a.ff, a.d_out, fault), Operand{dy, n, a.d_out, q.ldy, q.planes, dyplane, 0},
+  e.inner = a.dx || weights;
+  e.down = a.dw_down != nullptr;
+  if ((e.inner && !sm100::make_block_map(&e.dgu, dgu, n, a.ff, 2 * P * q.ldf, 2 * P, q.ldf, e.COLS)) ||
+      (e.down && !sm100::make_block_map(&e.h, h, n, a.ff, q.ldf, P, hplane, e.COLS)))
+    return cudaErrorInvalidValue;
+  TRY(launch_active(product(q, n, a.ff, a.d_out, fault), Operand{dy, n, a.d_out, q.ldy, q.planes, dyplane, 0},
                 Operand{q.pack_d ? ws + q.d : a.w_down, a.d_out, a.ff, q.ldd, q.planes, a.d_out * q.ldd, 1}, e, s));
   if (a.dx) {
     MmArgs p = dx_args(q, a, fault);
@@ -554,8 +619,7 @@ cudaError_t run(const llattn_gated_args& a, bool backward, volatile unsigned* fa
 }  // namespace
 
 size_t kept_bytes(const llattn_gated_args& a) {
-  const size_t blocks = (size_t)a.tokens * cdiv(a.ff, kBlock);
-  return a.dtype == LLATTN_F32 ? up256(blocks * 256) : up256(blocks * 128) + up256(blocks * 2);
+  return (size_t)cdiv(a.tokens, 32) * cdiv(a.ff, kBlock) * (a.dtype == LLATTN_F32 ? 4096 : 2048 + 64);
 }
 
 size_t workspace_bytes(const llattn_gated_args& a, bool backward) {

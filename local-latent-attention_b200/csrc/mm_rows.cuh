@@ -69,14 +69,58 @@ __device__ __forceinline__ void pack_row(const T* src, int d, bf16* dst, int64_t
   }
 }
 
-// rows of a matrix, packed; one warp per row
+// Rows of a matrix, packed: a thread for 8 columns, whole 16-byte chunks out. (A warp a
+// row, lane by lane, took 51 us for 1408 unaligned rows of 3749, this 6.)
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ x, int64_t ldx, int n, int d, bf16* __restrict__ xs,
-                                                 int64_t lds, int64_t plane) {
+                                                   int64_t lds, int64_t plane) {
   pdl_next();
   pdl_wait();
-  const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (r < n) pack_row<T>(x + r * ldx, d, xs + r * lds, lds, plane, vec_rows(x, ldx, d));
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = lds / 8, total = n * per;
+  if (i >= total) return;
+  const int64_t r = total <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
+  const int c = (int)(i - r * per) * 8;
+  const T* src = x + r * ldx + c;
+  bf16* dst = xs + r * lds + c;
+  if constexpr (sizeof(T) == 2) {
+    uint4 u;
+    if (vec_rows(x, ldx, d)) {
+      u = *reinterpret_cast<const uint4*>(src);
+    } else {
+      T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) e[q] = c + q < d ? src[q] : from_f<T>(0.f);
+    }
+    *reinterpret_cast<uint4*>(dst) = u;
+  } else {
+    float v[8];
+    if (vec_rows(x, ldx, d)) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float4 f = reinterpret_cast<const float4*>(src)[q];
+        v[4 * q] = f.x;
+        v[4 * q + 1] = f.y;
+        v[4 * q + 2] = f.z;
+        v[4 * q + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = c + q < d ? src[q] : 0.f;
+    }
+    uint32_t o[4][3];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) split3(v[2 * q], v[2 * q + 1], o[q]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(dst + k * plane) = make_uint4(o[0][k], o[1][k], o[2][k], o[3][k]);
+  }
+}
+
+template <typename T>
+cudaError_t launch_pack(const void* src, int64_t ld, int rows, int cols, void* dst, int64_t lds, cudaStream_t s) {
+  const int64_t grid = (rows * (lds / 8) + 255) / 256;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  return launch_pdl(pack_kernel<T>, dim3((unsigned)grid), 256, 0, 1, s, static_cast<const T*>(src), ld, rows, cols,
+                    static_cast<bf16*>(dst), lds, rows * lds);
 }
 
 // ---- rows out -----------------------------------------------------------------

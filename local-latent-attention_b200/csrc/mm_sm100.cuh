@@ -190,6 +190,8 @@ __device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
 //      need as long as their products take; 48 KB for twice the products do
 //      not hold the tensor cores up.
 //  2 = 256 x 256 on a pair, two accumulators
+//  5 = the same with 16 epilogue warps instead of 8, at 112 registers a thread and
+//      one stage less: for epilogues that work on every value for long
 //  1 = 128 x 128 on a CTA, two accumulators
 //  4 = 128 x 64 on a CTA, between 1 and 0
 //  0 = 128 x 32 on a CTA, for products too small to occupy the SMs otherwise:
@@ -197,14 +199,14 @@ __device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
 //      1.1 us at the end of a kernel), and a step copies 20 KB instead of 32.
 template <int SH>
 struct MmShape {
-  static constexpr int CG = SH == 2 || SH == 3 ? 2 : 1;
+  static constexpr int CG = SH == 2 || SH == 3 || SH == 5 ? 2 : 1;
   static constexpr int NH = SH == 3 ? 2 : 1;  // column halves of the accumulator, an MMA each
-  static constexpr int BM = 128 * CG, BN = SH == 3 ? 512 : SH == 2 ? 256 : SH == 1 ? 128 : SH == 4 ? 64 : 32;  // tile of the CTA (pair)
+  static constexpr int BM = 128 * CG, BN = SH == 3 ? 512 : SH == 2 || SH == 5 ? 256 : SH == 1 ? 128 : SH == 4 ? 64 : 32;  // tile of the CTA (pair)
   static constexpr int HN = BN / NH;              // columns of an MMA
-  static constexpr int CW = HN < 128 ? HN : 128;  // columns of an epilogue warp (32 rows) in a half
+  static constexpr int CW = SH == 5 ? 64 : HN < 128 ? HN : 128;  // columns of an epilogue warp (32 rows) in a half
   static constexpr int EW = 4 * (HN / CW);        // epilogue warps
   static constexpr int THREADS = 64 + 32 * EW;
-  static constexpr int ST = SH == 3 ? 4 : BN < 128 ? 8 : 6;
+  static constexpr int ST = SH == 3 ? 4 : SH == 5 ? 5 : BN < 128 ? 8 : 6;
   static constexpr int BR = HN / CG;        // rows of B that a CTA copies per half
   static constexpr int AB = 128 * 64 * 2;   // one CTA's A tile: 128 rows x 64 K, 16 KB
   static constexpr int BB = (BR < 64 ? 64 : BR) * 64 * 2;  // B tile of a half (a whole panel of 64 if MN-major)
@@ -479,6 +481,39 @@ __device__ __forceinline__ float2 bf16_pair(const uint4 (&u)[4], int i) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// Blocks of a warp's 32 rows and COLS bf16 columns on their way to memory: laid out
+// in the staging block as the tensor map's swizzle has it, sent by lane 0 (the
+// map's bounds cut what lies outside). 4 KB hold two blocks of 32 columns or four of 16.
+template <int COLS>
+struct Outgoing {
+  static constexpr int BYTES = 64 * COLS, N = 4096 / BYTES, CH = COLS / 8;
+  uint8_t* buf;
+  int lane, k = 0;
+  __device__ __forceinline__ Outgoing(uint8_t* b, int l) : buf(b), lane(l) {
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void send(const CUtensorMap* map, const uint32_t (&w)[COLS / 2], int col, int row, int z) {
+    if (k >= N) {
+      if (lane == 0) bulk_wait_read<N - 1>();
+      __syncwarp();
+    }
+    uint8_t* b = buf + k % N * BYTES;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = CH == 4 ? lane * 64 + (c ^ (lane >> 1 & 3)) * 16 : lane * 32 + (c ^ (lane >> 2 & 1)) * 16;
+      *reinterpret_cast<uint4*>(b + at) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(map, b, col, row, z);
+      tma_store_commit();
+    }
+    ++k;
+  }
+};
+
 // sum (+)= an accumulator's CW columns of this thread's row
 template <int CW>
 __device__ __forceinline__ void drain(uint32_t acc, uint32_t sum, bool add) {
@@ -536,11 +571,18 @@ __device__ __forceinline__ void store_part(const MmArgs& p, const MmItem& x, con
 //     j of both products. C's columns count both: N = 2 x rows, rounded up to
 //     whole BR. K-major only.
 //   kSecondTerms: MmArgs::b2 says which terms take the second map.
+// tile has a second template argument then, BR.
 enum { kSecondNone = 0, kSecondHalves = 1, kSecondTerms = 2 };
 template <typename Epi, typename = void>
 struct SecondB : std::integral_constant<int, kSecondNone> {};
 template <typename Epi>
 struct SecondB<Epi, std::void_t<decltype(Epi::kSecond)>> : std::integral_constant<int, Epi::kSecond> {};
+
+// Epilogues that send blocks out by bulk copies (kBulkOut): lane 0 of each of their warps waits for its own at the end.
+template <typename Epi, typename = void>
+struct BulkOut : std::false_type {};
+template <typename Epi>
+struct BulkOut<Epi, std::void_t<decltype(Epi::kBulkOut)>> : std::bool_constant<Epi::kBulkOut> {};
 
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
@@ -617,7 +659,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   const MmPlan pl = *plan;
   // one accumulator at a time: both halves of shape 3, or, with chains, where
   // the sum takes the place of the second
-  constexpr bool one = S::ACC == 1 || (CHAIN && SH == 2);
+  constexpr bool one = S::ACC == 1 || (CHAIN && S::BN == 256);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -802,7 +844,9 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       typename Epi::Pre pre;
       if (x.block < 0) epi.fetch(pre, p, w, w.m0 + row, w.n0 + S::CW * half, M);
       auto out = [&](int col, uint32_t ta) {
-        if (x.block < 0)
+        if constexpr (SECOND == kSecondHalves)
+          epi.template tile<S::CW, S::BR>(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage, pre);
+        else if (x.block < 0)
           epi.template tile<S::CW>(p, w, w.m0 + row, w.n0 + col, M, ta, x.k1 <= x.k0, stage, pre);
         else
           store_part<SH>(p, x, w, row, col, M, ta, stage);
@@ -816,7 +860,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
       };
       if constexpr (CHAIN) {
         const int steps = x.k1 > x.k0 ? cdiv(x.k1 - x.k0, 64) * p.n_terms : 0;
-        const uint32_t sum = t0 + (SH == 2 ? 1 : 2) * S::HN;
+        const uint32_t sum = t0 + (S::BN == 256 ? 1 : 2) * S::HN;
         int i = 0;
         do {
           const int buf = wait();
@@ -837,6 +881,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
         }
       }
     }
+    if (BulkOut<Epi>::value && lane == 0) bulk_wait<0>();
     if (!ok) mm_raise(p, 8u, abort);
   }
   __syncwarp();
@@ -894,7 +939,7 @@ struct Operand {
   int mn;  // stored MN-major (rows = K, cols = MN) instead of K-major (rows = MN, cols = K)
 };
 
-inline int mm_units(int sh) { return sh == 2 || sh == 3 ? sm_count() / 2 : sm_count(); }
+inline int mm_units(int sh) { return sh == 2 || sh == 3 || sh == 5 ? sm_count() / 2 : sm_count(); }
 
 // Estimated time (us) of a product in a shape: waves of tiles (the last one
 // split where allowed), each K / 64 steps and a gap, and the last tile's

@@ -639,10 +639,10 @@ cudaError_t run(const llattn_xent_args& a, const Plan& q, volatile unsigned* fau
   const void* wv = q.pack_w ? wp : a.w;
   if (!q.train) {
     if (q.pack_w) {
-      TRY(launch_pdl(pack_kernel<T>, dim3(cdiv(V, 8)), 256, 0, 1, s, static_cast<const T*>(a.w), a.ldw, V, d, wp, q.ldw, wplane));
+      TRY(launch_pack<T>(a.w, a.ldw, V, d, wp, q.ldw, s));
     }
     if (q.pack_x) {
-      TRY(launch_pdl(pack_kernel<T>, dim3(cdiv(n, 8)), 256, 0, 1, s, static_cast<const T*>(a.x), a.ldx, n, d, xs, q.ldx, xplane));
+      TRY(launch_pack<T>(a.x, a.ldx, n, d, xs, q.ldx, s));
     }
     MmArgs p = base_args(q, fault);
     const Operand ox{q.pack_x ? xs : a.x, n, d, q.ldx, q.planes, xplane, 0}, ow{wv, V, d, q.ldw, q.planes, wplane, 0};

@@ -112,13 +112,8 @@ gated_mlp_grads_op = torch.library.custom_op("llattn_b200::gated_mlp_grads", _ga
                                              device_types="cuda")
 
 
-def _up256(v):
-    return (v + 255) // 256 * 256
-
-
 def _kept_bytes(n, ff, dtype):
-    blocks = n * ((ff + 31) // 32)
-    return _up256(blocks * 256) if dtype == torch.float32 else _up256(blocks * 128) + _up256(blocks * 2)
+    return (n + 31) // 32 * ((ff + 15) // 16) * (4096 if dtype == torch.float32 else 2048 + 64)
 
 
 @gated_mlp_op.register_fake
@@ -169,7 +164,7 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     Precision: sums are fp32. float32 inputs keep 24 bits in every product.
     bfloat16: the products' operands act(g) u and its gradients are rounded to
     bfloat16 once (for up to 64 tokens to 16 bits, for up to 32 without gradients
-    not below 16 bits), what is kept to 11 bits relative to the largest of 32 neighbours, and
+    not below 16 bits), what is kept to 11 bits relative to the largest of 16 neighbours, and
     the results once."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
