@@ -25,7 +25,7 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(CSRC, "_build")
 LIB = os.path.join(PKG, "libllattn.so")
 SOURCES = ["api.cu", "pool.cu", "latent.cu", "local_simt.cu", "gate.cu", "local_sm100.cu", "decode.cu", "profile.cu",
-           "xent.cu", "orth.cu", "gated.cu", "embed.cu", "clip.cu"]
+           "xent.cu", "orth.cu", "gated.cu", "gated_few.cu", "embed.cu", "clip.cu"]
 NVCC = os.environ.get("NVCC", shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc")
 
 

@@ -20,8 +20,7 @@
 // fp32: all operands in three bf16 planes and six products (24 bits), g and u
 // in fp32.
 //
-// Up to kFew tokens without gradients take few_kernel instead: weights are read
-// once, in the order that the tensor cores' fragments want, and h stays fp32.
+// Up to 8 tokens (16 in fp32) without gradients take gated_few.cu's kernel instead.
 #include <math.h>
 
 #include <algorithm>
@@ -35,7 +34,7 @@ namespace {
 
 using namespace mm;
 
-constexpr int kFine = 64, kFew = 32;
+constexpr int kFine = 64;
 // K = 64 steps a tensor-core sum takes (MmArgs::chain) in fp32: as the loss's products (xent.cu)
 constexpr int kFineF32Chain = 1, kF32Chain = 4;
 constexpr int kBlock = 16;  // inner columns of a kept block
@@ -499,12 +498,6 @@ Kept kept_at(const Plan& q, const llattn_gated_args& a) {
   return k;
 }
 
-template <typename T>
-cudaError_t pack(bool needed, const void* src, int64_t ld, int rows, int cols, void* dst, int64_t lds, cudaStream_t s) {
-  if (!needed) return cudaSuccess;
-  return launch_pack<T>(src, ld, rows, cols, dst, lds, s);
-}
-
 EpiOut rows_out(const Plan& q, void* out, int cols) {
   EpiOut o{};
   o.out = out;
@@ -534,10 +527,12 @@ template <typename T, int ACT, int P>
 cudaError_t run_fwd(const llattn_gated_args& a, const Plan& q, volatile unsigned* fault, cudaStream_t s) {
   char* ws = static_cast<char*>(a.workspace);
   const int n = a.tokens;
-  TRY(pack<T>(q.pack_x, a.x, a.ldx, n, a.d, ws + q.x, q.ldx, s));
-  TRY(pack<T>(q.pack_g, a.w_gate, a.ldg, a.ff, a.d, ws + q.g, q.ldg, s));
-  TRY(pack<T>(q.pack_u, a.w_up, a.ldu, a.ff, a.d, ws + q.u, q.ldu, s));
-  TRY(pack<T>(q.pack_d, a.w_down, a.ldd, a.d_out, a.ff, ws + q.d, q.ldd, s));
+  Packs packs = {};
+  if (q.pack_x) packs.add(a.x, a.ldx, n, a.d, ws + q.x, q.ldx);
+  if (q.pack_g) packs.add(a.w_gate, a.ldg, a.ff, a.d, ws + q.g, q.ldg);
+  if (q.pack_u) packs.add(a.w_up, a.ldu, a.ff, a.d, ws + q.u, q.ldu);
+  if (q.pack_d) packs.add(a.w_down, a.ldd, a.d_out, a.ff, ws + q.d, q.ldd);
+  TRY(launch_packs<T>(packs, s));
   const Operand x{q.pack_x ? ws + q.x : a.x, n, a.d, q.ldx, q.planes, n * q.ldx, 0};
   const Operand g{q.pack_g ? ws + q.g : a.w_gate, a.ff, a.d, q.ldg, q.planes, a.ff * q.ldg, 0};
   const Operand u{q.pack_u ? ws + q.u : a.w_up, a.ff, a.d, q.ldu, q.planes, a.ff * q.ldu, 0};
@@ -559,11 +554,13 @@ cudaError_t run_bwd(const llattn_gated_args& a, const Plan& q, volatile unsigned
   char* ws = static_cast<char*>(a.workspace);
   const int n = a.tokens;
   const bool weights = a.dw_gate || a.dw_up;
-  TRY(pack<T>(q.pack_dy, a.dy, a.lddy, n, a.d_out, ws + q.dy, q.ldy, s));
-  TRY(pack<T>(q.pack_d, a.w_down, a.ldd, a.d_out, a.ff, ws + q.d, q.ldd, s));
-  TRY(pack<T>(q.pack_g && a.dx, a.w_gate, a.ldg, a.ff, a.d, ws + q.g, q.ldg, s));
-  TRY(pack<T>(q.pack_u && a.dx, a.w_up, a.ldu, a.ff, a.d, ws + q.u, q.ldu, s));
-  TRY(pack<T>(q.pack_x && weights, a.x, a.ldx, n, a.d, ws + q.x, q.ldx, s));
+  Packs packs = {};
+  if (q.pack_dy) packs.add(a.dy, a.lddy, n, a.d_out, ws + q.dy, q.ldy);
+  if (q.pack_d) packs.add(a.w_down, a.ldd, a.d_out, a.ff, ws + q.d, q.ldd);
+  if (q.pack_g && a.dx) packs.add(a.w_gate, a.ldg, a.ff, a.d, ws + q.g, q.ldg);
+  if (q.pack_u && a.dx) packs.add(a.w_up, a.ldu, a.ff, a.d, ws + q.u, q.ldu);
+  if (q.pack_x && weights) packs.add(a.x, a.ldx, n, a.d, ws + q.x, q.ldx);
+  TRY(launch_packs<T>(packs, s));
   const void* dy = q.pack_dy ? ws + q.dy : a.dy;
   const int64_t dyplane = n * q.ldy, hplane = n * q.ldf;
   bf16 *h = reinterpret_cast<bf16*>(ws + q.h), *dgu = reinterpret_cast<bf16*>(ws + q.dgu);
@@ -622,22 +619,27 @@ size_t kept_bytes(const llattn_gated_args& a) {
   return (size_t)cdiv(a.tokens, 32) * cdiv(a.ff, kBlock) * (a.dtype == LLATTN_F32 ? 4096 : 2048 + 64);
 }
 
+static bool few(const llattn_gated_args& a, bool backward) { return !backward && !a.kept && a.tokens <= few_tokens(a.dtype); }
+
 size_t workspace_bytes(const llattn_gated_args& a, bool backward) {
+  if (few(a, backward)) return up256(few_workspace_bytes(a));
   return std::max<size_t>(256, make_plan(a, backward).total);
 }
 
 int launches(const llattn_gated_args& a, bool backward) {
+  if (few(a, backward)) return 2;
   const Plan q = make_plan(a, backward);
   const bool weights = a.dw_gate || a.dw_up;
-  if (!backward) return q.pack_x + q.pack_g + q.pack_u + q.pack_d + 2 + joins(y_args(q, a, nullptr));
-  int n = q.pack_dy + q.pack_d + 1;
-  if (a.dx) n += q.pack_g + q.pack_u + 1 + joins(dx_args(q, a, nullptr));
+  if (!backward) return (q.pack_x || q.pack_g || q.pack_u || q.pack_d) + 2 + joins(y_args(q, a, nullptr));
+  int n = (q.pack_dy || q.pack_d || (a.dx && (q.pack_g || q.pack_u)) || (weights && q.pack_x)) + 1;
+  if (a.dx) n += 1 + joins(dx_args(q, a, nullptr));
   if (a.dw_down) n += 1 + joins(dwd_args(q, a, nullptr));
-  if (weights) n += q.pack_x + 1 + joins(dwgu_args(q, a, nullptr));
+  if (weights) n += 1 + joins(dwgu_args(q, a, nullptr));
   return n;
 }
 
 cudaError_t launch(const llattn_gated_args& a, bool backward, volatile unsigned* fault, cudaStream_t s) {
+  if (few(a, backward)) return launch_few(a, s);
   return a.activation == LLATTN_ACT_SILU ? run<LLATTN_ACT_SILU>(a, backward, fault, s)
                                          : run<LLATTN_ACT_GELU>(a, backward, fault, s);
 }
