@@ -23,7 +23,9 @@ namespace llattn {
 namespace clip {
 namespace {
 
-constexpr int kTensors = 1300;  // of 24 bytes: parameters hold 32 KB
+// entries of 24 bytes in the parameters, which hold 32 KB; a short list takes the short form (the
+// parameters are copied with every launch)
+constexpr int kTensors = 1300, kShort = 96;
 constexpr int kThreads = 256, kUnroll = 4, kChunk = kThreads * kUnroll * 16;
 constexpr int kMaxGrid = 1184;
 
@@ -33,11 +35,12 @@ struct Entry {
   int chunk;  // its first chunk
   int bf16;
 };
+template <int CAP>
 struct Table {
   int n, chunks;
-  Entry e[kTensors];
+  Entry e[CAP];
 };
-static_assert(sizeof(Table) <= 32000, "kernel parameters");
+static_assert(sizeof(Table<kTensors>) <= 32000, "kernel parameters");
 
 __device__ __forceinline__ float element(const char* p, int bf) {
   return bf ? __bfloat162float(*reinterpret_cast<const bf16*>(p)) : *reinterpret_cast<const float*>(p);
@@ -57,10 +60,12 @@ __device__ __forceinline__ void unpack(const uint4& u, int bf, float (&v)[8], in
 }
 
 // A CTA's run of chunks [first, last), and the table's entry of a chunk.
-__device__ __forceinline__ int2 run_of(const Table& t) {
+template <int CAP>
+__device__ __forceinline__ int2 run_of(const Table<CAP>& t) {
   return make_int2((int)((int64_t)t.chunks * blockIdx.x / gridDim.x), (int)((int64_t)t.chunks * (blockIdx.x + 1) / gridDim.x));
 }
-__device__ __forceinline__ int entry_of(const Table& t, int chunk) {
+template <int CAP>
+__device__ __forceinline__ int entry_of(const Table<CAP>& t, int chunk) {
   int lo = 0, hi = t.n - 1;  // the last entry that starts at or before chunk
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -162,8 +167,8 @@ __device__ __forceinline__ double block_join(double a, double* red) {
   return a;
 }
 
-template <typename Op>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table t, double* __restrict__ part) {
+template <typename Op, int CAP>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
   __shared__ double red[kThreads / 32];
   const int2 run = run_of(t);
   int e = entry_of(t, run.x);
@@ -188,8 +193,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
 }
 
 // n_part: all batches' sums. scale: 0 writes the norm alone.
-template <typename Op>
-__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ Table t, const double* __restrict__ part,
+template <typename Op, int CAP>
+__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ Table<CAP> t, const double* __restrict__ part,
                                                         int n_part, double max_norm, int scale, float* __restrict__ norm) {
   __shared__ double red[kThreads / 32];
   const int2 run = run_of(t);
@@ -241,10 +246,11 @@ int chunks_of(const llattn_clip_args& a, int i) {
   return (int)(((int64_t)((uintptr_t)a.tensors[i] & 15) + bytes + kChunk - 1) / kChunk);
 }
 
-// The next batch of tensors from *i on: at most kTensors that hold something.
-void fill(const llattn_clip_args& a, int* i, Table* t) {
+// The next batch of tensors from *i on: at most CAP that hold something.
+template <int CAP>
+void fill(const llattn_clip_args& a, int* i, Table<CAP>* t) {
   t->n = t->chunks = 0;
-  for (; *i < a.count && t->n < kTensors; ++*i) {
+  for (; *i < a.count && t->n < CAP; ++*i) {
     if (!a.sizes[*i]) continue;
     const int chunks = chunks_of(a, *i);
     if (t->n && t->chunks > (1 << 30) - chunks) break;
@@ -253,7 +259,8 @@ void fill(const llattn_clip_args& a, int* i, Table* t) {
     t->chunks += chunks;
   }
 }
-int grid_of(const Table& t) { return std::max(1, std::min(t.chunks, std::min(kMaxGrid, 8 * sm_count()))); }
+template <int CAP>
+int grid_of(const Table<CAP>& t) { return std::max(1, std::min(t.chunks, std::min(kMaxGrid, 8 * sm_count()))); }
 
 int batches(const llattn_clip_args& a) {
   int n = 0, full = 0;
@@ -272,15 +279,15 @@ int batches(const llattn_clip_args& a) {
   return n + 1;
 }
 
-template <typename Op>
+template <typename Op, int CAP>
 cudaError_t run(const llattn_clip_args& a, cudaStream_t s) {
   double* part = static_cast<double*>(a.workspace);
-  Table t;
+  Table<CAP> t;
   int n_part = 0, i = 0, n = 0;
   do {
     fill(a, &i, &t);
     const int grid = grid_of(t);
-    const cudaError_t e = launch_pdl(norm_kernel<Op>, dim3(grid), kThreads, 0, 1, s, t, part + n_part);
+    const cudaError_t e = launch_pdl(norm_kernel<Op, CAP>, dim3(grid), kThreads, 0, 1, s, t, part + n_part);
     if (e != cudaSuccess) return e;
     n_part += grid;
     ++n;
@@ -290,7 +297,7 @@ cudaError_t run(const llattn_clip_args& a, cudaStream_t s) {
   float* norm = a.norm;
   do {
     if (again) fill(a, &i, &t);
-    const cudaError_t e = launch_pdl(clip_kernel<Op>, dim3(a.scale ? grid_of(t) : 1), kThreads, 0, 1, s, t, part, n_part,
+    const cudaError_t e = launch_pdl(clip_kernel<Op, CAP>, dim3(a.scale ? grid_of(t) : 1), kThreads, 0, 1, s, t, part, n_part,
                                      a.max_norm, a.scale, norm);
     if (e != cudaSuccess) return e;
     norm = nullptr;
@@ -304,7 +311,8 @@ size_t workspace_bytes(const llattn_clip_args& a) { return (size_t)batches(a) * 
 int launches(const llattn_clip_args& a) { return batches(a) * (a.scale ? 2 : 1) + !a.scale; }
 
 cudaError_t launch(const llattn_clip_args& a, cudaStream_t s) {
-  return a.norm_type == LLATTN_NORM_INF ? run<Largest>(a, s) : run<Squares>(a, s);
+  if (a.count <= kShort) return a.norm_type == LLATTN_NORM_INF ? run<Largest, kShort>(a, s) : run<Squares, kShort>(a, s);
+  return a.norm_type == LLATTN_NORM_INF ? run<Largest, kTensors>(a, s) : run<Squares, kTensors>(a, s);
 }
 
 }  // namespace clip
