@@ -2,18 +2,21 @@
 //   out[b, t] = scale W[ids[b, t]] + P[t]
 //   dW[v] = scale sum_{(b, t): ids[b, t] = v} dout[b, t],  dP[t] = sum_b dout[b, t]
 //
-// dW goes by the tokens sorted by word. The sort is one launch: each CTA
-// owns a range of words and reads all ids (from the L2) for itself, so that no CTA
-// waits for another: it counts its words' tokens and the tokens of smaller words,
-// then writes its tokens, word by word and in their order, to where these
+// dW goes by the tokens sorted by word. The sort runs beside dP's sums, in one
+// launch with them: each of 128 CTAs owns every 128th word (neighbours in a
+// vocabulary are of like frequency) and reads all ids for itself, from the L2, so
+// that no CTA waits for another: it counts its words' tokens and those of the CTAs
+// before it, then writes its tokens, word by word and in their order, to where these
 // start. Rows are then summed in that order, whatever the launch: a warp per word and
-// 2 KB of columns, zeros for a word without tokens. A word of more than kHot tokens
-// is cut at the multiples of kHot of the sorted order; the pieces' sums go
-// through the workspace and are added in order. No atomics on values: the same bits
-// every run.
+// 1 KB of columns, zeros for a word without tokens. A word of more than kHot tokens
+// is cut at the multiples of kHot of the sorted order; these pieces go first, their sums
+// through the workspace, and are added in order. No atomics on values: the same bits
+// every run. Where words and tokens are few (`small`), a CTA a word picks its
+// tokens out of the ids itself, and one launch does it all.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "embed.cuh"
 #include "pdl.cuh"
@@ -22,17 +25,35 @@ namespace llattn {
 namespace embed {
 namespace {
 
-constexpr int kHot = 64;
+// (with pieces of 64 tokens, 2 KB of columns and two rows at a time, 8197 tokens of 1408 bf16 took 84 us
+// for their sums, the longest words' 25 us a warp among them)
+constexpr int kHot = 32;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kMostWords = 1280;  // of a sorting CTA: 32 counters each, 160 KB
-constexpr int kSlice = 4;         // 16-byte vectors a lane takes of a row at a time
+constexpr int kSorters = 128, kSortBits = 7;  // sorting CTAs a round: word v is the (v >> 7)-th of CTA v % 128
+constexpr int kMostBits = 10;                 // at most 1024 words a sorting CTA and round: 32 counters each, 128 KB
+constexpr int kSlice = 2, kRows = 4;          // 16-byte vectors a lane takes of a row, and rows, at a time
+constexpr int kWords = 4;                     // words of a summing warp
+constexpr int kHeld = 40960;                  // tokens whose places the sort keeps, 80 KB
 
 struct Ids {
   const void* p;
   int wide;  // int64, else int32
-  int64_t vocab, padding;
-  __device__ __forceinline__ int64_t at(int64_t i) const {
-    return wide ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int*>(p)[i];
+  int vocab, padding;
+  // the i-th id, -1 where there is no such word
+  __device__ __forceinline__ int at(int64_t i) const {
+    int id, high = 0;
+    if (wide) {
+      const int2 v = static_cast<const int2*>(p)[i];
+      id = v.x;
+      high = v.y;
+    } else {
+      id = static_cast<const int*>(p)[i];
+    }
+    return high == 0 && (unsigned)id < (unsigned)vocab ? id : -1;
+  }
+  __device__ __forceinline__ int counted(int64_t i) const {  // -1 for the padding too
+    const int id = at(i);
+    return id == padding ? -1 : id;
   }
 };
 
@@ -50,6 +71,12 @@ struct Pack {
     } else {
       v[0] = to_f<T>(*p);
     }
+  }
+  using Raw = std::conditional_t<VEC, uint4, T>;  // as it is in memory
+  __device__ __forceinline__ void add(const Raw& u) {
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += to_f<T>(e[i]);
   }
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (VEC) {
@@ -78,257 +105,77 @@ struct Pack {
 
 // ---- forward ----------------------------------------------------------------------
 
-// A thread per pack of columns. per_row: packs of a row.
+// A warp per token and 4 packs a lane of its columns.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) embed_rows(Ids ids, const T* __restrict__ w, int64_t ldw, const T* __restrict__ pos,
-                                                  int64_t ldp, int length, int64_t total, int per_row, int d, float scale,
+                                                  int64_t ldp, int length, int64_t tokens, int slices, int d, float scale,
                                                   T* __restrict__ out) {
   pdl_next();
   pdl_wait();
   using P = Pack<T, VEC>;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int64_t n = total <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
-  const int c = (int)(i - n * per_row) * P::N;
-  const int64_t id = ids.at(n);
-  P r, q;
-  if (id >= 0 && id < ids.vocab) {
-    r.load(w + id * ldw + c);
-    if (pos) {
-      const int t = (int)(n % length);
-      q.load(pos + t * ldp + c);
-#pragma unroll
-      for (int k = 0; k < P::N; ++k) r.v[k] = fmaf(r.v[k], scale, q.v[k]);
-    } else {
-      r.times(scale);
-    }
-  } else {
-    r.fill(__int_as_float(0x7fc00000));  // no such word
-  }
-  r.store(out + n * d + c);
-}
-
-// ---- the sort -----------------------------------------------------------------------
-
-// order: the counted tokens by word, then by index; words: their words; start[v]: a
-// word's first place, start[vocab]: their number.
-__global__ void __launch_bounds__(kSortThreads) embed_sort(Ids ids, int n, int span, int* __restrict__ order,
-                                                           int* __restrict__ words, int* __restrict__ start) {
-  extern __shared__ int counts[];  // [kSortWarps][span]
-  __shared__ int sums[kSortWarps];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int64_t lo = (int64_t)blockIdx.x * span;
-  const int mine = (int)min((int64_t)span, ids.vocab - lo);
-  int* my = counts + warp * span;
-  for (int i = threadIdx.x; i < kSortWarps * span; i += kSortThreads) counts[i] = 0;
-  __syncthreads();
-  pdl_next();
-  pdl_wait();
-  const int per = cdiv(cdiv(n, kSortWarps), 32) * 32, i0 = min(n, warp * per), i1 = min(n, i0 + per);
-  int below = 0;
-  auto each = [&](auto body) {  // groups of 32 ids in order, several loads in flight
-#pragma unroll 1
-    for (int i = i0; i < i1; i += 256) {
-      int64_t id[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int j = i + 32 * k + lane;
-        id[k] = j < i1 ? ids.at(j) : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (id[k] == ids.padding || id[k] >= ids.vocab) id[k] = -1;
-        body(id[k], i + 32 * k + lane);
-      }
-    }
-  };
-  each([&](int64_t id, int) {
-    below += id >= 0 && id < lo;
-    if (id >= lo && id < lo + mine) atomicAdd(my + (int)(id - lo), 1);
-  });
-  below = __reduce_add_sync(0xffffffffu, below);
-  if (lane == 0) sums[warp] = below;
-  __syncthreads();
-  // counters -> places: over the warps of a word, then over the words
-  int base = 0;
-#pragma unroll
-  for (int i = 0; i < kSortWarps; ++i) base += sums[i];
-  __syncthreads();
-  for (int r0 = 0; r0 < mine; r0 += kSortThreads) {
-    const int r = r0 + threadIdx.x;
-    int all = 0;
-    if (r < mine)
-      for (int k = 0; k < kSortWarps; ++k) all += counts[k * span + r];
-    int scan = all;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += v;
-    }
-    if (lane == 31) sums[warp] = scan;
-    __syncthreads();
-    int at = base + scan - all;
-#pragma unroll
-    for (int k = 0; k < kSortWarps; ++k) {
-      at += k < warp ? sums[k] : 0;
-      base += sums[k];
-    }
-    __syncthreads();
-    if (r < mine) {
-      start[lo + r] = at;
-      for (int k = 0; k < kSortWarps; ++k) {
-        const int c = counts[k * span + r];
-        counts[k * span + r] = at;
-        at += c;
-      }
-    }
-  }
-  if (threadIdx.x == 0 && lo + mine == ids.vocab) start[ids.vocab] = base;
-  __syncthreads();
-  each([&](int64_t id, int i) {
-    const bool in = id >= lo && id < lo + mine;
-    const unsigned some = __ballot_sync(0xffffffffu, in);
-    if (!some) return;
-    if (in) {
-      const int r = (int)(id - lo);
-      const unsigned same = __match_any_sync(some, r);
-      const int at = my[r] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp(some);
-      order[at] = i;
-      words[at] = (int)id;
-      if ((same >> lane) == 1u) my[r] = at + 1;  // the last of them
-    }
-    __syncwarp();
-  });
-}
-
-// ---- gradients ------------------------------------------------------------------------
-
-// Columns [c0, c0 + kSlice 32 packs) of the sum of rows order[s, e) of dout, one warp.
-template <typename T, bool VEC>
-__device__ __forceinline__ void sum_rows(Pack<T, VEC> (&a)[kSlice], const T* __restrict__ dout, const int* __restrict__ order,
-                                         int s, int e, int d, int c0) {
-  using P = Pack<T, VEC>;
+  constexpr int U = 4;
   const int lane = threadIdx.x % 32;
+  const int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t n = i <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)slices) : i / slices;
+  if (n >= tokens) return;
+  const int c0 = ((int)(i - n * slices) * U * 32 + lane) * P::N;
+  const int id = ids.at(n);
+  const T* src = w + (int64_t)max(id, 0) * ldw;
+  P r[U], q[U];
 #pragma unroll
-  for (int k = 0; k < kSlice; ++k) a[k].fill(0.f);
-  for (int b = s; b < e; b += 32) {
-    const int mine = b + lane < e ? order[b + lane] : 0, m = min(32, e - b);
-#pragma unroll 2
-    for (int j = 0; j < m; ++j) {
-      const T* row = dout + (int64_t)__shfl_sync(0xffffffffu, mine, j) * d;
-      P r[kSlice];
+  for (int k = 0; k < U; ++k)
+    if (c0 + k * 32 * P::N < d) r[k].load(src + c0 + k * 32 * P::N);
+  if (pos) {
+    const T* at = pos + (int64_t)(n <= INT32_MAX ? (uint32_t)n % (uint32_t)length : n % length) * ldp;
 #pragma unroll
-      for (int k = 0; k < kSlice; ++k) {
-        const int c = c0 + (k * 32 + lane) * P::N;
-        r[k].fill(0.f);
-        if (c < d) r[k].load(row + c);
-      }
+    for (int k = 0; k < U; ++k)
+      if (c0 + k * 32 * P::N < d) q[k].load(at + c0 + k * 32 * P::N);
+  }
 #pragma unroll
-      for (int k = 0; k < kSlice; ++k) a[k].add(r[k]);
+  for (int k = 0; k < U; ++k) {
+    if (c0 + k * 32 * P::N >= d) break;
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) {
+      const float v = pos ? fmaf(r[k].v[e], scale, q[k].v[e]) : r[k].v[e] * scale;
+      r[k].v[e] = id < 0 ? __int_as_float(0x7fc00000) : v;  // no such word
     }
+    r[k].store(out + n * d + c0 + k * 32 * P::N);
   }
 }
 
-// Warps [0, vocab slices) write the words of up to kHot tokens, the next ones the sums
-// of the pieces of the others: slot 2 p holds what interval p of the sorted order has
-// of its first word, slot 2 p + 1 what it has of its last one, where that is another.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) embed_sums(const T* __restrict__ dout, const int* __restrict__ order,
-                                                  const int* __restrict__ words, const int* __restrict__ start, int64_t vocab,
-                                                  int d, int slices, int pieces, float scale, float* __restrict__ part,
-                                                  T* __restrict__ dw) {
-  pdl_next();
-  pdl_wait();
-  using P = Pack<T, VEC>;
-  const int lane = threadIdx.x % 32;
-  const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  const int64_t v = w / slices;
-  const int c0 = (int)(w - v * slices) * (kSlice * 32 * P::N);
-  P a[kSlice];
-  if (v < vocab) {
-    const int s = start[v], e = start[v + 1];
-    if (e - s > kHot) return;
-    sum_rows<T, VEC>(a, dout, order, s, e, d, c0);
-#pragma unroll
-    for (int k = 0; k < kSlice; ++k) {
-      const int c = c0 + (k * 32 + lane) * P::N;
-      a[k].times(scale);
-      if (c < d) a[k].store(dw + v * d + c);
-    }
-    return;
-  }
-  const int64_t p = v - vocab;
-  const int total = start[vocab];
-  if (p >= pieces || p * kHot >= total) return;
-  const int lo = (int)p * kHot, hi = min(lo + kHot, total);
-  for (int last = 0; last < 2; ++last) {
-    const int word = words[last ? hi - 1 : lo];
-    if (last && word == words[lo]) break;
-    const int s = start[word], e = start[word + 1];
-    if (e - s <= kHot) continue;
-    sum_rows<T, VEC>(a, dout, order, max(s, lo), min(e, hi), d, c0);
-#pragma unroll
-    for (int k = 0; k < kSlice; ++k) {
-      const int c = c0 + (k * 32 + lane) * P::N;
-      if (c < d)
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) part[(2 * p + last) * d + c + i] = a[k].v[i];
-    }
-  }
-}
+// ---- dP, beside the sort -------------------------------------------------------------
 
-// The words of more than kHot tokens: a warp for each that starts in interval p (there
-// is one at most: the interval's last word), 32 columns.
+// Sums over a piece of the batch (all of it where `part` is null); rows of P past the
+// length become zeros.
 template <typename T>
-__global__ void __launch_bounds__(256) embed_join(const int* __restrict__ words, const int* __restrict__ start, int64_t vocab,
-                                                  int d, int slices, int pieces, float scale, const float* __restrict__ part,
-                                                  T* __restrict__ dw) {
-  pdl_next();
-  pdl_wait();
-  const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  const int64_t p = w / slices;
-  const int c = (int)(w - p * slices) * 32 + threadIdx.x % 32;
-  const int total = start[vocab];
-  if (p >= pieces || p * kHot >= total) return;
-  const int word = words[min((int)p * kHot + kHot, total) - 1];
-  const int s = start[word], e = start[word + 1];
-  if (e - s <= kHot || s / kHot != p || c >= d) return;
-  const int q1 = (e - 1) / kHot;
-  float a = part[(2 * p + (s % kHot != 0)) * d + c];
-#pragma unroll 8
-  for (int q = (int)p + 1; q <= q1; ++q) a += part[(int64_t)2 * q * d + c];
-  dw[(int64_t)word * d + c] = from_f<T>(a * scale);
-}
-
-// dP: sums over the batch of a piece of its rows (all of them where `part` is null);
-// rows of P past the length become zeros.
+struct Positions {
+  const T* dout;
+  int batch, per, splits;
+  int64_t cols, all;  // length d, position_rows d
+  float* part;
+  T* dp;
+};
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) embed_positions(const T* __restrict__ dout, int batch, int per, int64_t cols,
-                                                       int64_t all, float* __restrict__ part, T* __restrict__ dp) {
-  pdl_next();
-  pdl_wait();
+__device__ __forceinline__ void position_sums(const Positions<T>& q, int64_t thread, int split) {
   using P = Pack<T, VEC>;
-  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * P::N;
-  if (c >= all) return;
+  const int64_t c = thread * P::N;
+  if (c >= q.all) return;
   P a;
   a.fill(0.f);
-  if (c < cols) {
-    const int b1 = min(batch, ((int)blockIdx.y + 1) * per);
-#pragma unroll 8
-    for (int b = blockIdx.y * per; b < b1; ++b) {
+  if (c < q.cols) {
+    const int b1 = min(q.batch, (split + 1) * q.per);
+#pragma unroll 4
+    for (int b = split * q.per; b < b1; ++b) {
       P r;
-      r.load(dout + b * cols + c);
+      r.load(q.dout + b * q.cols + c);
       a.add(r);
     }
   }
-  if (part) {
-    if (c < cols)
-#pragma unroll
-      for (int i = 0; i < P::N; ++i) part[blockIdx.y * cols + c + i] = a.v[i];
-    if (c >= cols && blockIdx.y == 0) a.store(dp + c);
+  if (!q.part || c >= q.cols) {
+    if (split == 0 || !q.part) a.store(q.dp + c);
   } else {
-    a.store(dp + c);
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) q.part[split * q.cols + c + i] = a.v[i];
   }
 }
 template <typename T>
@@ -344,11 +191,315 @@ __global__ void __launch_bounds__(256) embed_positions_join(const float* __restr
   dp[c] = from_f<T>(a);
 }
 
+// ---- the sort -----------------------------------------------------------------------
+
+// A word's slot: those of a sorting CTA and round in a row, so that its tokens are
+// consecutive. start[slot]: its tokens' first place in the sorted order, start[slot + 1]:
+// the place behind them.
+__device__ __forceinline__ int slot_of(int v, int bits) {  // span = 1 << bits
+  const int k = v >> kSortBits;
+  return ((((k >> bits) << kSortBits) + (v & (kSorters - 1))) << bits) + (k & ((1 << bits) - 1));
+}
+
+// CTA: words v with v % 128 = CTA % 128 and (v >> 7) / span = its round. order: the counted
+// tokens by slot, then by index; words: their words; start [rounds 128 span + 1].
+// held: the tokens' places stay in shared memory for the second pass, n of them; otherwise each
+// pass reads the ids. (Places in registers took a loop unrolled 32 times: 11 us of fetching it.)
+__device__ __forceinline__ void sort_tokens(const Ids& ids, int n, int bits, bool held, int cta, int ctas,
+                                            int* __restrict__ order, int* __restrict__ words, int* __restrict__ start) {
+  extern __shared__ int counts[];  // [kSortWarps][span], then the places
+  __shared__ int sums[kSortWarps];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int span = 1 << bits, round = cta >> kSortBits, low = cta & (kSorters - 1);
+  const int per = cdiv(cdiv(n, kSortWarps), 256) * 256, i0 = min(n, warp * per), i1 = min(n, i0 + per);
+  int* my = counts + warp * span;
+  int16_t* places = reinterpret_cast<int16_t*>(counts + kSortWarps * span) + warp * (held ? per : 256);
+  for (int i = threadIdx.x; i < kSortWarps * span; i += kSortThreads) counts[i] = 0;
+  __syncthreads();
+  // 256 ids from i on -> their places: r of this CTA's words, -1: another's, -2: of a CTA before this one
+  auto place = [&](int i, auto body) {
+    int id[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) id[k] = i + 32 * k + lane < i1 ? ids.counted(i + 32 * k + lane) : -1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int q = (id[k] >> kSortBits) - round * span, other = id[k] & (kSorters - 1);
+      const bool here = (unsigned)q < (unsigned)span;
+      const int r = id[k] < 0 ? -1 : q < 0 || (here && other < low) ? -2 : here && other == low ? q : -1;
+      places[(held ? i - i0 : 0) + 32 * k + lane] = (int16_t)r;
+      body(r);
+    }
+  };
+  int below = 0;
+  for (int i = i0; i < i1; i += 256)
+    place(i, [&](int r) {
+      below += r == -2;
+      if (r >= 0) atomicAdd(my + r, 1);
+    });
+  below = __reduce_add_sync(0xffffffffu, below);
+  if (lane == 0) sums[warp] = below;
+  __syncthreads();
+  // counters -> places in the order: over the warps of a word, then over the words
+  int base = 0;
+#pragma unroll
+  for (int i = 0; i < kSortWarps; ++i) base += sums[i];
+  __syncthreads();
+  int* first = start + (int64_t)cta * span;
+  const int r = threadIdx.x;  // (span <= kSortThreads)
+  int all = 0;
+  if (r < span) {
+#pragma unroll 8
+    for (int k = 0; k < kSortWarps; ++k) all += counts[k * span + r];
+  }
+  int scan = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) sums[warp] = scan;
+  __syncthreads();
+  int at = base + scan - all;
+#pragma unroll
+  for (int k = 0; k < kSortWarps; ++k) {
+    at += k < warp ? sums[k] : 0;
+    base += sums[k];
+  }
+  if (r < span) {
+    first[r] = at;
+#pragma unroll 8
+    for (int k = 0; k < kSortWarps; ++k) {
+      const int c = counts[k * span + r];
+      counts[k * span + r] = at;
+      at += c;
+    }
+  }
+  if (threadIdx.x == 0 && cta == ctas - 1) first[span] = base;
+  __syncthreads();
+  for (int i = i0; i < i1; i += 256) {
+    if (!held) {
+      __syncwarp();
+      place(i, [](int) {});
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int k = 0; k < 8; ++k) {
+      const int r = places[(held ? i - i0 : 0) + 32 * k + lane];
+      const unsigned some = __ballot_sync(0xffffffffu, r >= 0);
+      if (r >= 0) {
+        const unsigned same = __match_any_sync(some, r);
+        const int at = my[r] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp(some);
+        order[at] = i + 32 * k + lane;
+        words[at] = ((round * span + r) << kSortBits) + low;
+        if ((same >> lane) == 1u) my[r] = at + 1;  // the last of them
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// The first `sorters` CTAs sort, the others sum dP.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kSortThreads, 2) embed_sort(Ids ids, int n, int bits, int held, int sorters,
+                                                           int* __restrict__ order, int* __restrict__ words,
+                                                           int* __restrict__ start, Positions<T> q, int per_split) {
+  pdl_next();
+  pdl_wait();
+  if ((int)blockIdx.x < sorters) {
+    sort_tokens(ids, n, bits, held, blockIdx.x, sorters, order, words, start);
+    return;
+  }
+  const int b = blockIdx.x - sorters, split = b / per_split;
+  position_sums<T, VEC>(q, (int64_t)(b - split * per_split) * kSortThreads + threadIdx.x, split);
+}
+
+// ---- dW -----------------------------------------------------------------------------
+
+// Columns [c0, c0 + 32 kSlice packs) of rows added to a, the j-th of up to 32 being row index(j) of dout.
+template <typename T, bool VEC, typename Index>
+__device__ __forceinline__ void add_rows(Pack<T, VEC> (&a)[kSlice], const T* __restrict__ dout, int d, int c0, int m, Index index) {
+  using P = Pack<T, VEC>;
+  const int lane = threadIdx.x % 32;
+#pragma unroll 1
+  for (int j0 = 0; j0 < m; j0 += kRows) {
+    typename P::Raw r[kRows][kSlice];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const T* row = dout + (int64_t)index(min(j0 + j, m - 1)) * d;
+#pragma unroll
+      for (int k = 0; k < kSlice; ++k) {
+        const int c = c0 + (k * 32 + lane) * P::N;
+        r[j][k] = typename P::Raw{};
+        if (j0 + j < m && c < d) r[j][k] = *reinterpret_cast<const typename P::Raw*>(row + c);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+#pragma unroll
+      for (int k = 0; k < kSlice; ++k) a[k].add(r[j][k]);
+  }
+}
+
+// Warps [0, pieces slices): the pieces of words of more than kHot tokens: slot 2 p of `part` holds what
+// interval p of the sorted order has of its first word, slot 2 p + 1 what it has of its last
+// one, where that is another. The warps after write the other words, kWords each, a quarter of
+// the vocabulary apart: most words have no token and cost little but the wait for their count.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) embed_sums(const T* __restrict__ dout, const int* __restrict__ order,
+                                                  const int* __restrict__ words, const int* __restrict__ start, int vocab,
+                                                  int bits, int total_at, int d, int slices, int pieces, float scale,
+                                                  float* __restrict__ part, T* __restrict__ dw) {
+  pdl_next();
+  pdl_wait();
+  using P = Pack<T, VEC>;
+  const int lane = threadIdx.x % 32;
+  const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int u = w <= INT32_MAX ? (int)((uint32_t)w / (uint32_t)slices) : (int)(w / slices);
+  const int c0 = (int)(w - (int64_t)u * slices) * (kSlice * 32 * P::N);
+  P a[kSlice];
+  if (u >= pieces) {
+    const int apart = cdiv(vocab, kWords), first = u - pieces;
+    if (first >= apart) return;
+    // lane 2 k: where word k's tokens start, lane 2 k + 1: where they end
+    const int mine = first + lane / 2 * apart;
+    const int bound = lane < 2 * kWords && mine < vocab ? start[slot_of(mine, bits) + lane % 2] : 0;
+    int s[kWords], n[kWords], row[kWords];
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      s[k] = __shfl_sync(0xffffffffu, bound, 2 * k);
+      n[k] = __shfl_sync(0xffffffffu, bound, 2 * k + 1) - s[k];
+      row[k] = lane < n[k] && n[k] <= kHot ? order[s[k] + lane] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const int v = first + k * apart;
+      if (v >= vocab || n[k] > kHot) continue;  // (warp-uniform)
+#pragma unroll
+      for (int i = 0; i < kSlice; ++i) a[i].fill(0.f);
+      add_rows<T, VEC>(a, dout, d, c0, n[k], [&](int j) { return __shfl_sync(0xffffffffu, row[k], j); });
+#pragma unroll
+      for (int i = 0; i < kSlice; ++i) {
+        const int c = c0 + (i * 32 + lane) * P::N;
+        a[i].times(scale);
+        if (c < d) a[i].store(dw + (int64_t)v * d + c);
+      }
+    }
+    return;
+  }
+  const int64_t p = u;
+  const int total = start[total_at];
+  if (p * kHot >= total) return;
+  const int lo = (int)p * kHot, hi = min(lo + kHot, total);
+  for (int last = 0; last < 2; ++last) {
+    const int word = words[last ? hi - 1 : lo];
+    if (last && word == words[lo]) break;
+    const int* at = start + slot_of(word, bits);
+    const int s = max(at[0], lo), e = min(at[1], hi);
+    if (at[1] - at[0] <= kHot) continue;
+    const int row = s + lane < e ? order[s + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < kSlice; ++i) a[i].fill(0.f);
+    add_rows<T, VEC>(a, dout, d, c0, e - s, [&](int j) { return __shfl_sync(0xffffffffu, row, j); });
+#pragma unroll
+    for (int k = 0; k < kSlice; ++k) {
+      const int c = c0 + (k * 32 + lane) * P::N;
+      if (c < d)
+#pragma unroll
+        for (int i = 0; i < P::N; ++i) part[(2 * p + last) * d + c + i] = a[k].v[i];
+    }
+  }
+}
+
+// The words of more than kHot tokens: a warp for each that starts in interval p (there
+// is one at most: the interval's last word), 32 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_join(const int* __restrict__ words, const int* __restrict__ start, int bits,
+                                                  int total_at, int d, int slices, int pieces, float scale,
+                                                  const float* __restrict__ part, T* __restrict__ dw) {
+  pdl_next();
+  pdl_wait();
+  const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t p = w / slices;
+  const int c = (int)(w - p * slices) * 32 + threadIdx.x % 32;
+  const int total = start[total_at];
+  if (p >= pieces || p * kHot >= total) return;
+  const int word = words[min((int)p * kHot + kHot, total) - 1];
+  const int* at = start + slot_of(word, bits);
+  const int s = at[0], e = at[1];
+  if (e - s <= kHot || s / kHot != p || c >= d) return;
+  const int q1 = (e - 1) / kHot;
+  float a = part[(2 * p + (s % kHot != 0)) * d + c];
+  for (int q = (int)p + 1; q <= q1; q += 32) {  // 32 loads at a time: their latency is all there is
+    float x[32];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) x[k] = q + k <= q1 ? part[(int64_t)2 * (q + k) * d + c] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) a += x[k];
+  }
+  dw[(int64_t)word * d + c] = from_f<T>(a * scale);
+}
+
+// Few words and tokens: a CTA per word and 1 KB of columns, whose warps each pick the word's tokens out of
+// an eighth of the ids; then the CTAs of dP.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) embed_small(Ids ids, int n, const T* __restrict__ dout, int d, int slices, float scale,
+                                                   T* __restrict__ dw, int word_ctas, Positions<T> q, int per_split) {
+  pdl_next();
+  pdl_wait();
+  if ((int)blockIdx.x >= word_ctas) {
+    const int b = blockIdx.x - word_ctas, split = b / per_split;
+    position_sums<T, VEC>(q, (int64_t)(b - split * per_split) * 256 + threadIdx.x, split);
+    return;
+  }
+  using P = Pack<T, VEC>;
+  __shared__ float red[8][32][kSlice * P::N];
+  __shared__ int hit[8][32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int v = blockIdx.x / slices, c0 = (blockIdx.x - v * slices) * (kSlice * 32 * P::N);
+  const int per = cdiv(cdiv(n, 8), 32) * 32, i0 = min(n, warp * per), i1 = min(n, i0 + per);
+  P a[kSlice];
+#pragma unroll
+  for (int k = 0; k < kSlice; ++k) a[k].fill(0.f);
+  for (int i = i0; i < i1; i += 256) {
+    int id[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) id[k] = i + 32 * k + lane < i1 ? ids.counted(i + 32 * k + lane) : -1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const unsigned some = __ballot_sync(0xffffffffu, id[k] == v);
+      if (!some) continue;
+      if (id[k] == v) hit[warp][__popc(some & ((1u << lane) - 1u))] = i + 32 * k + lane;
+      __syncwarp();
+      add_rows<T, VEC>(a, dout, d, c0, __popc(some), [&](int j) { return hit[warp][j]; });
+      __syncwarp();
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kSlice; ++k)
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) red[warp][lane][k * P::N + e] = a[k].v[e];
+  __syncthreads();
+  if (warp) return;
+#pragma unroll
+  for (int k = 0; k < kSlice; ++k) {
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) {
+      float x = red[0][lane][k * P::N + e];
+#pragma unroll
+      for (int o = 1; o < 8; ++o) x += red[o][lane][k * P::N + e];
+      a[k].v[e] = x * scale;
+    }
+    const int c = c0 + (k * 32 + lane) * P::N;
+    if (c < d) a[k].store(dw + (int64_t)v * d + c);
+  }
+}
+
 // ---- host side ------------------------------------------------------------------------
 
 struct Plan {
-  int n, elt, span, ctas, slices, pieces, splits, per;
-  bool vec;
+  int n, elt, bits, sorters, total_at, slices, pieces, splits, per;
+  bool vec, small, held;
   int64_t cols;
   size_t order, words, start, part, pos, total;
 };
@@ -362,29 +513,35 @@ Plan make_plan(const llattn_embed_args& a) {
   q.elt = a.dtype == LLATTN_F32 ? 4 : 2;
   q.vec = vectors(a.dout, a.d, q.elt) && vectors(a.dw, a.d, q.elt) && vectors(a.dpositions, a.d, q.elt);
   const int pack = q.vec ? 16 / q.elt : 1;
-  // a range of words for every SM, at least 32 of them
-  q.span = (int)std::min<int64_t>(kMostWords, std::max<int64_t>(32, cdiv64(a.vocab, sm_count())));
-  q.ctas = (int)cdiv64(a.vocab, q.span);
+  q.held = q.n <= kHeld;
+  const int share = (int)cdiv64(a.vocab, kSorters);  // words of a sorting CTA, in rounds
+  q.bits = 0;
+  while (q.bits < kMostBits && 1 << q.bits < share) ++q.bits;
+  q.sorters = cdiv(share, 1 << q.bits) * kSorters;
+  q.total_at = q.sorters << q.bits;
   q.slices = cdiv(a.d, kSlice * 32 * pack);
   q.pieces = q.n > kHot ? cdiv(q.n, kHot) : 0;
+  // one launch while every CTA's words and ids take a few us (4096 CTAs: some 4 rounds of what the GPU holds)
+  q.small = q.n <= 2048 && a.vocab * q.slices <= 4096;
   q.cols = (int64_t)a.length * a.d;
-  // positions: the batch in as many pieces as fill the GPU twice, of at least 16 rows
-  const int64_t ctas = cdiv64(q.cols, 256 * pack);
-  q.splits = (int)std::max<int64_t>(1, std::min<int64_t>(a.batch / 16, cdiv64(16 * sm_count(), ctas)));
+  // positions: the batch in as many pieces as fill the GPU, of at least 16 rows
+  const int64_t ctas = cdiv64(q.cols, 1024 * pack);
+  q.splits = (int)std::max<int64_t>(1, std::min<int64_t>(a.batch / 16, cdiv64(4 * sm_count(), ctas)));
   q.per = cdiv(a.batch, q.splits);
   q.splits = cdiv(a.batch, q.per);
   size_t off = 0;
   auto take = [&](size_t b) { size_t o = off; off += (b + 255) & ~(size_t)255; return o; };
-  q.order = take(a.dw ? 4 * (size_t)q.n : 0);
-  q.words = take(a.dw ? 4 * (size_t)q.n : 0);
-  q.start = take(a.dw ? 4 * (size_t)(a.vocab + 1) : 0);
-  q.part = take(a.dw ? 8 * (size_t)q.pieces * a.d : 0);
+  const bool sorted = a.dw && !q.small;
+  q.order = take(sorted ? 4 * (size_t)q.n : 0);
+  q.words = take(sorted ? 4 * (size_t)q.n : 0);
+  q.start = take(sorted ? 4 * (size_t)(q.total_at + 1) : 0);
+  q.part = take(sorted ? 8 * (size_t)q.pieces * a.d : 0);
   q.pos = take(a.dpositions && q.splits > 1 ? 4 * (size_t)q.splits * q.cols : 0);
   q.total = off;
   return q;
 }
 
-Ids ids_of(const llattn_embed_args& a) { return Ids{a.ids, a.ids_wide, a.vocab, a.padding}; }
+Ids ids_of(const llattn_embed_args& a) { return Ids{a.ids, a.ids_wide, (int)a.vocab, (int)std::max<int64_t>(a.padding, -1)}; }
 
 #define TRY(x)                          \
   do {                                  \
@@ -394,11 +551,11 @@ Ids ids_of(const llattn_embed_args& a) { return Ids{a.ids, a.ids_wide, a.vocab, 
 
 template <typename T, bool VEC>
 cudaError_t fwd(const llattn_embed_args& a, cudaStream_t s) {
-  const int per_row = a.d / Pack<T, VEC>::N;
-  const int64_t total = (int64_t)a.batch * a.length * per_row, grid = cdiv64(total, 256);
+  const int slices = cdiv(a.d, 4 * 32 * Pack<T, VEC>::N);
+  const int64_t tokens = (int64_t)a.batch * a.length, grid = cdiv64(tokens * slices, 8);
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   return launch_pdl(embed_rows<T, VEC>, dim3((unsigned)grid), 256, 0, 1, s, ids_of(a), static_cast<const T*>(a.w), a.ldw,
-                    static_cast<const T*>(a.positions), a.ldp, a.length, total, per_row, a.d, a.scale, static_cast<T*>(a.out));
+                    static_cast<const T*>(a.positions), a.ldp, a.length, tokens, slices, a.d, a.scale, static_cast<T*>(a.out));
 }
 
 template <typename T, bool VEC>
@@ -408,31 +565,37 @@ cudaError_t bwd(const llattn_embed_args& a, const Plan& q, cudaStream_t s) {
   int* start = reinterpret_cast<int*>(ws + q.start);
   float* part = reinterpret_cast<float*>(ws + q.part);
   const T* dout = static_cast<const T*>(a.dout);
-  if (a.dw) {
-    const int smem = 4 * kSortWarps * q.span;
-    TRY(set_smem_once(embed_sort, smem));
-    TRY(launch_pdl(embed_sort, dim3(q.ctas), kSortThreads, smem, 1, s, ids_of(a), q.n, q.span, order, words, start));
-    T* dw = static_cast<T*>(a.dw);
-    const int64_t grid = cdiv64((a.vocab + q.pieces) * q.slices, 8);
-    if (grid > INT32_MAX) return cudaErrorInvalidValue;
-    TRY(launch_pdl(embed_sums<T, VEC>, dim3((unsigned)grid), 256, 0, 1, s, dout, order, words, start, a.vocab, a.d, q.slices,
-                   q.pieces, a.scale, part, dw));
+  T* dw = static_cast<T*>(a.dw);
+  const int64_t all = a.dpositions ? (int64_t)a.position_rows * a.d : 0;
+  float* pos = q.splits > 1 ? reinterpret_cast<float*>(ws + q.pos) : nullptr;
+  const Positions<T> pq{dout, a.batch, q.per, q.splits, q.cols, all, pos, static_cast<T*>(a.dpositions)};
+  const bool small = !dw || q.small;
+  const int threads = small ? 256 : kSortThreads;
+  const int64_t per_split = cdiv64(all, (int64_t)threads * Pack<T, VEC>::N), pos_ctas = per_split * q.splits;
+  const int64_t word_ctas = !dw ? 0 : small ? a.vocab * q.slices : q.sorters;
+  if (pos_ctas + word_ctas > INT32_MAX) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)(word_ctas + pos_ctas));
+  if (small) {
+    TRY(launch_pdl(embed_small<T, VEC>, grid, threads, 0, 1, s, ids_of(a), q.n, dout, a.d, q.slices, a.scale, dw, (int)word_ctas, pq,
+                   (int)per_split));
+  } else {
+    const int smem = (4 * kSortWarps << q.bits) + 2 * kSortWarps * (q.held ? cdiv(cdiv(q.n, kSortWarps), 256) * 256 : 256);
+    TRY(set_smem_once(embed_sort<T, VEC>, smem));
+    TRY(launch_pdl(embed_sort<T, VEC>, grid, threads, smem, 1, s, ids_of(a), q.n, q.bits, q.held, q.sorters, order, words, start, pq,
+                   (int)per_split));
+    const int64_t sums = cdiv64((cdiv64(a.vocab, kWords) + q.pieces) * q.slices, 8);
+    if (sums > INT32_MAX) return cudaErrorInvalidValue;
+    TRY(launch_pdl(embed_sums<T, VEC>, dim3((unsigned)sums), 256, 0, 1, s, dout, order, words, start, (int)a.vocab, q.bits,
+                   q.total_at, a.d, q.slices, q.pieces, a.scale, part, dw));
     if (q.pieces) {
       const int slices = cdiv(a.d, 32);
-      TRY(launch_pdl(embed_join<T>, dim3((unsigned)cdiv64((int64_t)q.pieces * slices, 8)), 256, 0, 1, s, words, start, a.vocab,
-                     a.d, slices, q.pieces, a.scale, part, dw));
+      TRY(launch_pdl(embed_join<T>, dim3((unsigned)cdiv64((int64_t)q.pieces * slices, 8)), 256, 0, 1, s, words, start, q.bits,
+                     q.total_at, a.d, slices, q.pieces, a.scale, part, dw));
     }
   }
-  if (a.dpositions) {
-    const int64_t all = (int64_t)a.position_rows * a.d;
-    float* pos = q.splits > 1 ? reinterpret_cast<float*>(ws + q.pos) : nullptr;
-    const int64_t grid = cdiv64(all, 256 * Pack<T, VEC>::N);
-    TRY(launch_pdl(embed_positions<T, VEC>, dim3((unsigned)grid, q.splits), 256, 0, 1, s, dout, a.batch, q.per, q.cols, all,
-                   pos, static_cast<T*>(a.dpositions)));
-    if (pos)
-      TRY(launch_pdl(embed_positions_join<T>, dim3((unsigned)cdiv64(q.cols, 256)), 256, 0, 1, s, pos, q.splits, q.cols,
-                     static_cast<T*>(a.dpositions)));
-  }
+  if (a.dpositions && pos)
+    TRY(launch_pdl(embed_positions_join<T>, dim3((unsigned)cdiv64(q.cols, 256)), 256, 0, 1, s, pos, q.splits, q.cols,
+                   static_cast<T*>(a.dpositions)));
   return cudaSuccess;
 }
 
@@ -443,7 +606,7 @@ size_t workspace_bytes(const llattn_embed_args& a) { return std::max<size_t>(256
 int launches(const llattn_embed_args& a, bool backward) {
   if (!backward) return 1;
   const Plan q = make_plan(a);
-  return (a.dw ? 2 + (q.pieces > 0) : 0) + (a.dpositions ? 1 + (q.splits > 1) : 0);
+  return (!a.dw || q.small ? 1 : 2 + (q.pieces > 0)) + (a.dpositions && q.splits > 1);
 }
 
 cudaError_t launch_fwd(const llattn_embed_args& a, cudaStream_t s) {

@@ -28,6 +28,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
+from .lm_ops import clip_grad_norm_, gated_mlp, token_embedding
 from .module import LocalLatentAttentionB200
 from .optim import Muon, OptimizerPair
 from .training_ops import linear_cross_entropy
@@ -35,7 +36,9 @@ from .training_ops import linear_cross_entropy
 
 @dataclass
 class ModelConfig:
-    """The reference's ModelConfig fields (models.py:21-37)."""
+    """The reference's ModelConfig fields (models.py:21-37), and ff_gate: "" for
+    its MLP, "silu" or "gelu" for a gated feed-forward block (ff.w1 gates, ff.w3
+    goes up, ff.w2 down, no biases; ``gated_mlp``, CUDA only)."""
 
     vocab_size: int = 128
     max_seq_len: int = 1024
@@ -52,6 +55,7 @@ class ModelConfig:
     latent_query_block_size: int = 0
     checkpoint_blocks: bool = False
     use_triton_kernel: bool = True
+    ff_gate: str = ""
 
 
 RESIDUAL_OUTPUTS = ("out", "r_out", "w2")  # linear layers whose output is added to the residual stream
@@ -60,7 +64,7 @@ RESIDUAL_OUTPUTS = ("out", "r_out", "w2")  # linear layers whose output is added
 class DecoderLayer(nn.Module):
     """norm1 -> LocalLatentAttentionB200 -> residual add, norm2 -> MLP ->
     residual add. The MLP is an nn.ModuleDict {w1, w2} so its parameters
-    keep the reference's ff.w1 / ff.w2 names."""
+    keep the reference's ff.w1 / ff.w2 names; gated, {w1, w3, w2}."""
 
     def __init__(self, config: ModelConfig) -> None:
         super().__init__()
@@ -68,11 +72,19 @@ class DecoderLayer(nn.Module):
         self.norm1 = nn.RMSNorm(d, eps=1e-6)
         self.attn = LocalLatentAttentionB200(config)
         self.norm2 = nn.RMSNorm(d, eps=1e-6)
-        self.ff = nn.ModuleDict({"w1": nn.Linear(d, config.d_ff), "w2": nn.Linear(config.d_ff, d)})
+        self.gate = getattr(config, "ff_gate", "")
+        if self.gate:
+            self.ff = nn.ModuleDict({"w1": nn.Linear(d, config.d_ff, bias=False), "w3": nn.Linear(d, config.d_ff, bias=False),
+                                     "w2": nn.Linear(config.d_ff, d, bias=False)})
+        else:
+            self.ff = nn.ModuleDict({"w1": nn.Linear(d, config.d_ff), "w2": nn.Linear(config.d_ff, d)})
         self.p_drop = config.dropout
 
     def mlp(self, h: torch.Tensor) -> torch.Tensor:
-        h = self.ff["w2"](F.gelu(self.ff["w1"](h)))
+        if self.gate:
+            h = gated_mlp(h, self.ff["w1"].weight, self.ff["w3"].weight, self.ff["w2"].weight, activation=self.gate)
+        else:
+            h = self.ff["w2"](F.gelu(self.ff["w1"](h)))
         return F.dropout(h, self.p_drop, self.training) if self.p_drop else h
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -117,6 +129,9 @@ class LocalLatentLM(nn.Module):
         # never holds the [B T, vocab] logits (CUDA only); False: the logits in
         # memory and F.cross_entropy, as the reference's training loop
         self.fused_loss = False
+        # True: words and positions by token_embedding, in one launch, and their
+        # gradients in the order of the sorted tokens (CUDA only); False: torch's embedding
+        self.fused_embedding = False
 
     def set_profile(self, enabled: bool) -> None:
         for layer in self.blocks:
@@ -132,14 +147,20 @@ class LocalLatentLM(nn.Module):
         """Logits [B, T, vocab]; with `targets` [B, T], the mean next-token
         cross-entropy instead (computed in fp32 by `self.loss_head`, which a
         caller may replace by a compiled version of itself)."""
-        T = input_ids.shape[1]
-        x = self.embedding(input_ids) + self.position.weight[:T].unsqueeze(0)
+        x = self._embed(input_ids)
         remat = self.checkpoint_blocks and self.training
         for layer in self.blocks:
             x = checkpoint(layer, x, use_reentrant=False) if remat else layer(x)
         if targets is not None:
             return self.loss_head(x, targets)
         return self.lm_head(self.norm(x))
+
+    def _embed(self, ids: torch.Tensor, first: int = 0) -> torch.Tensor:
+        """Embeddings of ids [B, T] at positions first, first + 1, ..."""
+        positions = self.position.weight
+        if self.fused_embedding:
+            return token_embedding(ids, self.embedding.weight, positions=positions[first:] if first else positions)
+        return self.embedding(ids) + positions[first:first + ids.shape[1]].unsqueeze(0)
 
     def loss_head(self, x: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         if self.fused_loss:
@@ -180,15 +201,14 @@ class LocalLatentLM(nn.Module):
         return ids
 
     def _prefill(self, ids: torch.Tensor, caches) -> torch.Tensor:
-        T = ids.shape[1]
-        x = self.embedding(ids) + self.position(torch.arange(T, device=ids.device)).unsqueeze(0)
+        x = self._embed(ids)
         for blk, cache in zip(self.blocks, caches):
             x = x + blk.attn.prefill(blk.norm1(x), cache)
             x = x + blk.mlp(blk.norm2(x))
         return self.lm_head(self.norm(x[:, -1]))
 
     def _decode_one(self, tok: torch.Tensor, pos: int, caches) -> torch.Tensor:
-        x = self.embedding(tok) + self.position.weight[pos].view(1, 1, -1)
+        x = self._embed(tok, pos)
         for blk, cache in zip(self.blocks, caches):
             x = x + blk.attn.decode(blk.norm1(x), cache)
             x = x + blk.mlp(blk.norm2(x))
@@ -246,13 +266,14 @@ def build_optimizer(model: nn.Module, lr: float = 3e-4, weight_decay: float = 0.
 
 
 def train_step(model: nn.Module, optimizer, ids: torch.Tensor, targets: torch.Tensor, grad_clip: float = 1.0,
-               autocast_dtype=torch.bfloat16) -> torch.Tensor:
+               autocast_dtype=torch.bfloat16, fused_clip: bool = False) -> torch.Tensor:
     """One optimiser step: bf16 autocast forward, cross-entropy, backward
-    (DDP all-reduces the grads), clip, AdamW. Returns the loss (on device)."""
+    (DDP all-reduces the grads), clip (fused_clip: by this package's clip_grad_norm_),
+    AdamW. Returns the loss (on device)."""
     with torch.autocast(device_type=ids.device.type, dtype=autocast_dtype):
         loss = model(ids, targets)
     loss.backward()
-    torch.nn.utils.clip_grad_norm_(model.parameters(), grad_clip)
+    (clip_grad_norm_ if fused_clip else torch.nn.utils.clip_grad_norm_)(model.parameters(), grad_clip)
     optimizer.step()
     optimizer.zero_grad(set_to_none=True)
     return loss.detach()
