@@ -1,4 +1,5 @@
-"""Build libllattn.so (sm_100a) in-tree with nvcc.
+"""Build libllattn.so (sm_100a) in-tree with nvcc, and _torch_ops.so, the eager path
+of lm_ops.py over it (torch's C++ headers, the host compiler).
 
     python build.py            # incremental: rebuilds objects whose sources changed
     python build.py --clean    # drop objects first
@@ -24,6 +25,7 @@ ROOT = os.path.dirname(PKG)
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(CSRC, "_build")
 LIB = os.path.join(PKG, "libllattn.so")
+TORCH_OPS = os.path.join(PKG, "_torch_ops.so")
 SOURCES = ["api.cu", "pool.cu", "latent.cu", "local_simt.cu", "gate.cu", "local_sm100.cu", "decode.cu", "profile.cu",
            "xent.cu", "orth.cu", "gated.cu", "gated_few.cu", "embed.cu", "clip.cu"]
 NVCC = os.environ.get("NVCC", shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc")
@@ -73,6 +75,37 @@ def _compile(name: str, fl: list[str]) -> str:
     return obj
 
 
+def build_torch_ops() -> None:
+    """_torch_ops.so, where its source, the header or torch changed."""
+    import sysconfig
+
+    import torch
+
+    src, home = os.path.join(CSRC, "torch_ops.cpp"), os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(NVCC))), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-I" + INCLUDE,
+           "-I" + os.path.join(home, "include"), "-I" + os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + cuda, "-L" + os.path.join(home, "lib"), "-L" + PKG,
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-l:libllattn.so",
+           "-Wl,-rpath,$ORIGIN"]
+    h = hashlib.sha256((" ".join(cmd) + torch.__version__ + sys.version).encode())
+    for path in (src, os.path.join(INCLUDE, "llattn.h")):
+        with open(path, "rb") as fh:
+            h.update(fh.read())
+    mark = os.path.join(BUILD, "torch_ops." + h.hexdigest()[:16])
+    if os.path.exists(TORCH_OPS) and os.path.exists(mark):
+        return
+    r = subprocess.run([*cmd, "-o", TORCH_OPS + ".tmp"], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_ops.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
+    for old in os.listdir(BUILD):
+        if old.startswith("torch_ops."):
+            os.remove(os.path.join(BUILD, old))
+    open(mark, "w").close()
+
+
 def build(clean: bool = False) -> str:
     if clean and os.path.isdir(BUILD):
         shutil.rmtree(BUILD)
@@ -87,6 +120,7 @@ def build(clean: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    build_torch_ops()
     return LIB
 
 

@@ -6,7 +6,9 @@ global norm (``clip_grad_norm_``, ``total_norm``).
 As in ``training_ops.py``: CUDA only, torch's current stream, torch-allocated
 outputs and workspaces, ``RuntimeError`` on bad arguments, no CPU implementation;
 custom ops with fake implementations for tracers, dispatch modes and tensor
-subclasses, which plain eager calls leave out.
+subclasses. Plain eager calls leave them out: they go through ``_torch_ops.so``
+(csrc/torch_ops.cpp, built with the library), whose autograd nodes are C++, and what that does
+not handle (empty inputs, bad arguments) comes back to the functions here.
 """
 
 from __future__ import annotations
@@ -22,13 +24,24 @@ from . import _lib
 from .ops import _DT, _dtype_code, _require
 from .training_ops import _direct, _on, _rows, _stream
 
-_PLAIN = torch.contiguous_format
+try:
+    from . import _torch_ops as _native
+except ImportError as missing:  # calls say so: there is no other eager path to fall back to
+    _native, _why = None, missing
+
+
+def _eager():
+    """The native calls, or None where somebody traces or intercepts."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
+        return None
+    if _native is None:
+        raise RuntimeError("llattn: _torch_ops.so is missing or does not load: build it with "
+                           f"`python local-latent-attention_b200/csrc/build.py` ({_why})")
+    return _native
 
 
 def _common_dtype(*tensors: Tensor) -> list[Tensor]:
-    """Under autocast all in its dtype, as a linear layer's inputs are (float32 where that is float16)."""
-    if not torch.is_autocast_enabled("cuda"):
-        return list(tensors)
+    """All in autocast's dtype, as a linear layer's inputs are (float32 where that is float16)."""
     dt = torch.get_autocast_dtype("cuda")
     dt = torch.float32 if dt == torch.float16 else dt  # (no fp16 kernels)
     return [t.to(dt) if t.is_cuda else t for t in tensors]
@@ -170,9 +183,14 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     act = _ACTIVATIONS.get(activation)
     if act is None:
         _require(False, f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if torch.is_autocast_enabled("cuda"):
+        x, w_gate, w_up, w_down = _common_dtype(x, w_gate, w_up, w_down)
+    native = _eager()
+    y = native.gated(x, w_gate, w_up, w_down, act) if native else None
+    if y is not None:
+        return y
     if x.dim() < 1 or w_gate.dim() != 2 or x.shape[-1] != w_gate.shape[1]:
         _require(False, f"x {tuple(x.shape)} must end in w_gate's columns {tuple(w_gate.shape)}")
-    x, w_gate, w_up, w_down = _common_dtype(x, w_gate, w_up, w_down)
     flat = x.dim() == 2
     x2 = x if flat else x.reshape(-1, x.shape[-1])
     if torch.is_grad_enabled() and (x2.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
@@ -298,15 +316,18 @@ def token_embedding(ids: Tensor, weight: Tensor, *, positions: Optional[Tensor] 
     bits every run. Tokens of the word padding_idx (which may count from the end)
     do not take part in it. An id outside [0, vocab) makes its row NaN and has no
     gradient (it is an error that no launch can raise)."""
-    _require(ids.dim() >= 1 or positions is None, "positions need ids with a dimension")
-    if weight.dim() != 2:
-        _require(False, f"weight must be [vocab, d], got {tuple(weight.shape)}")
     padding = -1
     if padding_idx is not None:
-        vocab = weight.shape[0]
+        vocab = weight.shape[0] if weight.dim() else 0
         _require(-vocab <= padding_idx < vocab, f"padding_idx {padding_idx} outside the {vocab} words")
         padding = padding_idx % vocab
     scale = float(scale)
+    native = _eager()
+    out = native.embed(ids, weight, positions, scale, padding) if native else None
+    if out is not None:
+        return out
+    _require(ids.dim() >= 1 or positions is None, "positions need ids with a dimension")
+    _require(weight.dim() == 2, f"weight must be [vocab, d], got {tuple(weight.shape)}")
     ids2 = ids if ids.dim() == 2 else ids.reshape(-1, ids.shape[-1] if ids.dim() and ids.shape[-1] else 1)
     if torch.is_grad_enabled() and (weight.requires_grad or (positions is not None and positions.requires_grad)):
         out = _Embed.apply(ids2, weight, positions, scale, padding)
@@ -339,14 +360,11 @@ _KINDS = {Tensor, torch.nn.Parameter}
 
 
 def _plain(tensors: Sequence[Tensor]) -> bool:
-    """_direct for a long list."""
-    return (set(map(type, tensors)) <= _KINDS and not torch.compiler.is_compiling()
-            and not torch._C._len_torch_dispatch_stack())
+    return set(map(type, tensors)) <= _KINDS
 
 
 def _dense_all(tensors: list[Tensor], what: str) -> list[Tensor]:
-    """The tensors, copies in the place of those that are not dense, checked for `what`. Attribute by attribute over the
-    whole list: a tensor costs 0.3 us of host time, of which a model has hundreds."""
+    """The tensors, copies in the place of those that are not dense, checked for `what`."""
     devices, dtypes, layouts = set(map(Tensor.get_device, tensors)), {t.dtype for t in tensors}, {t.layout for t in tensors}
     if len(devices) != 1 or -1 in devices or not tensors[0].is_cuda:
         _require(tensors[0].is_cuda, f"{what} needs CUDA tensors")
@@ -413,7 +431,6 @@ def _norm_code(norm_type) -> int:
     return code
 
 
-@torch.no_grad()
 def total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
     """The norm of all tensors' elements together, as a float32 scalar on their
     device: the 2-norm (sums in fp64, in a fixed order; finite for any finite float32
@@ -424,10 +441,14 @@ def total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0)
     tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    return (_norm_of if _plain(tensors) else total_norm_op)(tensors, code)
+    native = _eager()
+    norm = native.clip(tensors, False, code, 0.0, False) if native else None
+    if norm is not None:
+        return norm
+    with torch.no_grad():
+        return (_norm_of if native and _plain(tensors) else total_norm_op)(tensors, code)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> Tensor:
     """torch.nn.utils.clip_grad_norm_ in two launches: the norm of all gradients
@@ -444,15 +465,17 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     max_norm = float(max_norm)
     _require(max_norm >= 0, f"max_norm must be >= 0, got {max_norm}")
     parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
-    if len(set(map(id, parameters))) < len(parameters):
-        parameters = list({id(p): p for p in parameters}.values())
-    grads = [g for p in parameters if (g := p.grad) is not None]
-    if not grads:
-        return torch.tensor(0.0)
-    direct = _plain(grads)
+    native = _eager()
     if error_if_nonfinite:
-        norm = (_norm_of if direct else total_norm_op)(grads, code)
+        norm = total_norm([g for p in parameters if (g := p.grad) is not None], norm_type)
         if not torch.isfinite(norm):
             raise RuntimeError(f"llattn: the total norm of order {norm_type} of the gradients is not finite, so they cannot "
                                "be clipped; error_if_nonfinite=False scales them all the same")
-    return (_clip_of if direct else clip_grads_op)(grads, max_norm, code)
+    norm = native.clip(parameters, True, code, max_norm, True) if native else None
+    if norm is not None:
+        return norm
+    grads = [g for p in {id(p): p for p in parameters}.values() if (g := p.grad) is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    with torch.no_grad():
+        return (_clip_of if native and _plain(grads) else clip_grads_op)(grads, max_norm, code)
