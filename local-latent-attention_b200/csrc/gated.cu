@@ -41,20 +41,25 @@ constexpr int kBlock = 16;  // inner columns of a kept block
 
 // act(g) and act'(g). EXACT: to fp32's last bits; otherwise ex2's and rcp's 2^-22, and
 // erf by Abramowitz and Stegun's 7.1.26 (1.5e-7), which shares its exponential with the density.
+// (8 and 19 instructions: the epilogues that use them are as long as their tile's products.)
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <int ACT, bool EXACT>
 __device__ __forceinline__ void activation(float g, float& a, float& slope) {
   if (ACT == LLATTN_ACT_SILU) {
-    const float e = EXACT ? expf(-g) : __expf(-g);
-    const float s = EXACT ? 1.f / (1.f + e) : __fdividef(1.f, 1.f + e);
+    const float s = EXACT ? 1.f / (1.f + expf(-g)) : fast_rcp(1.f + fast_exp2(g * -1.44269504f));
     a = g * s;
-    slope = s * (1.f + g * (1.f - s));
+    slope = fmaf(a, 1.f - s, s);
   } else if (EXACT) {
     const float phi = 0.5f * erfcf(g * -0.70710678f);
     a = g * phi;
     slope = phi + g * (0.39894228f * expf(-0.5f * g * g));
   } else {
     const float e = fast_exp2(g * g * -0.72134752f);
-    const float t = __fdividef(1.f, fmaf(fabsf(g), 0.3275911f * 0.70710678f, 1.f));
+    const float t = fast_rcp(fmaf(fabsf(g), 0.3275911f * 0.70710678f, 1.f));
     float q = fmaf(t, 1.061405429f, -1.453152027f);
     q = fmaf(q, t, 1.421413741f);
     q = fmaf(q, t, -0.284496736f);
@@ -86,7 +91,16 @@ __device__ __forceinline__ uint32_t block_scale(const float (&v)[16]) {
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
 __device__ __forceinline__ float unscale_of(uint32_t s) { return __uint_as_float((254u - s) << 23); }
 
-// 16 columns of this thread's row
+// 8 and 16 columns of this thread's row
+__device__ __forceinline__ void load8(uint32_t taddr, bool zero, float (&v)[8]) {
+  uint32_t r[8];
+  if (!zero) {
+    tmem_ld8(taddr, r);
+    tmem_ld_wait();
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = zero ? 0.f : __uint_as_float(r[q]);
+}
 __device__ __forceinline__ void load16(uint32_t taddr, bool zero, float (&v)[16]) {
   uint32_t r[16];
   if (!zero) {
@@ -96,28 +110,35 @@ __device__ __forceinline__ void load16(uint32_t taddr, bool zero, float (&v)[16]
 #pragma unroll
   for (int q = 0; q < 16; ++q) v[q] = zero ? 0.f : __uint_as_float(r[q]);
 }
-// v rounded to bf16, and, for more planes, what that leaves of it
-template <bool REST>
-__device__ __forceinline__ void round16(float (&v)[16], uint32_t* w) {
+// 8 of this thread's row's columns in P bf16 planes, 16 bytes a store, or all 16 of a block in one
+// plane, 32 bytes a store: a whole sector, so that nothing is gained by bringing rows together in
+// shared memory first (bulk stores of 64-byte rows from there: 145 and 122 us for 142 and 105 at the same
+// point, 8192 x 1536 x 4096).
+template <int P>
+__device__ __forceinline__ void store8(const float* v_, bf16* p, int64_t plane) {
+  float v[8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
-    if (REST) {
+  for (int q = 0; q < 8; ++q) v[q] = v_[q];
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
       v[2 * q] -= __uint_as_float(w[q] << 16);
       v[2 * q + 1] -= __uint_as_float(w[q] & 0xffff0000u);
     }
+    *reinterpret_cast<uint4*>(p + k * plane) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-// 16 columns in P > 1 planes, z, z + dz, ...
-template <int P>
-__device__ __forceinline__ void send_planes(Outgoing<16>& out, const CUtensorMap* map, float (&v)[16], int col, int row, int z,
-                                            int dz) {
+__device__ __forceinline__ void pack8(const float* v, uint32_t* w) {
 #pragma unroll
-  for (int k = 0; k < P; ++k) {
-    uint32_t w[8];
-    round16<true>(v, w);
-    out.send(map, w, col, row, z + k * dz);
-  }
+  for (int q = 0; q < 4; ++q) w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
+}
+__device__ __forceinline__ void store16(const uint32_t (&w)[8], bf16* p) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // ---- g, u -> h ------------------------------------------------------------------
@@ -125,14 +146,14 @@ __device__ __forceinline__ void send_planes(Outgoing<16>& out, const CUtensorMap
 // P: planes of h (3: fp32 inputs)
 template <int ACT, int P>
 struct EpiGated {
-  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false, kBulkOut = true;
+  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false;
   static constexpr int kSecond = kSecondHalves;
   static constexpr bool F32 = P == 3;
-  static constexpr int COLS = P == 1 ? 32 : 16;  // of a block sent out
   struct Pre {};
   __device__ __forceinline__ void fetch(Pre&, const MmArgs&, MmTile, int, int, int) const {}
-  CUtensorMap h;  // [P][tokens][ff]
-  Kept kept;      // gu null: nothing is kept
+  bf16* h;  // [P][tokens][ld]
+  int64_t ld, plane;
+  Kept kept;  // gu null: nothing is kept
   int ff;
 
   __device__ __forceinline__ void keep(const float (&g)[16], const float (&u)[16], int row0, int col, int lane) const {
@@ -163,36 +184,37 @@ struct EpiGated {
   }
 
   template <int CW, int BR>
-  __device__ __forceinline__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero, uint8_t* buf,
+  __device__ __forceinline__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr, bool zero, uint8_t*,
                                        Pre&) const {
     constexpr int W = CW / 2;  // of the BR columns: BR / 2 of g, BR / 2 of u; this warp's: W of each
-    static_assert(W >= 32, "whole blocks");
+    static_assert(W % kBlock == 0, "whole blocks");
     const int lane = threadIdx.x % 32, row0 = row - lane, o = col0 % BR, f0 = (col0 - o) / 2 + o / 2;
     if (row0 >= M) return;  // warp-uniform
     const uint32_t gt = taddr - o + o / 2, ut = gt + BR / 2;
-    Outgoing<COLS> out(buf, lane);
 #pragma unroll 1
-    for (int cc = 0; cc < W; cc += COLS) {
-      if (f0 + cc >= ff) break;  // warp-uniform
-      uint32_t w[COLS / 2];
+    for (int cc = 0; cc < W; cc += 16) {
+      const int col = f0 + cc;
+      if (col >= ff) break;  // warp-uniform
+      float g[16], u[16];
+      load16(gt + cc, zero, g);
+      load16(ut + cc, zero, u);
+      if (kept.gu) keep(g, u, row0, col, lane);
 #pragma unroll
-      for (int c = 0; c < COLS; c += 16) {
-        float g[16], u[16];
-        load16(gt + cc + c, zero, g);
-        load16(ut + cc + c, zero, u);
-        if (kept.gu && f0 + cc + c < ff) keep(g, u, row0, f0 + cc + c, lane);
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          float a, slope;
-          activation<ACT, F32>(g[q], a, slope);
-          g[q] = a * u[q];
-        }
-        if constexpr (P == 1)
-          round16<false>(g, w + c / 2);
-        else
-          send_planes<P>(out, &h, g, f0 + cc + c, row0, 0, 1);
+      for (int q = 0; q < 16; ++q) {
+        float a, slope;
+        activation<ACT, F32>(g[q], a, slope);
+        g[q] = a * u[q];
       }
-      if constexpr (P == 1) out.send(&h, w, f0 + cc, row0, 0);
+      bf16* dst = h + row * ld + col;
+      if constexpr (P == 1) {
+        uint32_t w[8];
+        pack8(g, w);
+        pack8(g + 8, w + 4);
+        if (row < M) store16(w, dst);
+      } else if (row < M) {
+        store8<P>(g, dst, plane);
+        store8<P>(g + 8, dst + 8, plane);
+      }
     }
   }
 };
@@ -201,16 +223,16 @@ struct EpiGated {
 
 template <int ACT, int P>
 struct EpiGrad {
-  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false, kBulkOut = true;
+  static constexpr bool kNarrow = true, kWide = false, kChain = P == 3, kBegin = false;
   static constexpr bool F32 = P == 3;
-  static constexpr int COLS = P == 1 ? 32 : 16;
   struct Pre {
     uint4 x[F32 ? 8 : 4];
     uint32_t scale;
   };
-  CUtensorMap dgu, h;  // z = 2 plane + (0: dg, 1: du); z = plane
+  bf16* dgu;  // [tokens][P][2][ld] (dg, du), or null
+  bf16* h;    // [P][tokens][ld], or null
+  int64_t ld, plane;
   Kept kept;
-  int inner, down;  // which of them are wanted
 
   __device__ __forceinline__ void ask(Pre& pre, int row0, int col, int lane) const {
     const int64_t at = (int64_t)(row0 / 32) * kept.blocks + col / 16;
@@ -223,18 +245,19 @@ struct EpiGrad {
     const int lane = threadIdx.x % 32;
     if (row - lane < M && col0 < a.N) ask(pre, row - lane, col0, lane);
   }
-  static __device__ __forceinline__ void values(const Pre& pre, float (&g)[16], float (&u)[16]) {
+  // columns [8 e, 8 e + 8) of the block
+  static __device__ __forceinline__ void values(const Pre& pre, int e, float (&g)[8], float (&u)[8]) {
     if constexpr (F32) {
 #pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        g[q] = __uint_as_float(word(pre.x, q));
-        u[q] = __uint_as_float(word(pre.x, q + 16));
+      for (int q = 0; q < 8; ++q) {
+        g[q] = __uint_as_float(word(pre.x, 8 * e + q));
+        u[q] = __uint_as_float(word(pre.x, 16 + 8 * e + q));
       }
     } else {
       const float fg = unscale_of(pre.scale & 255u), fu = unscale_of(pre.scale >> 8);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t wg = word(pre.x, q), wu = word(pre.x, q + 8);
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t wg = word(pre.x, 4 * e + q), wu = word(pre.x, 8 + 4 * e + q);
         const float2 pg = __half22float2(*reinterpret_cast<const __half2*>(&wg));
         const float2 pu = __half22float2(*reinterpret_cast<const __half2*>(&wu));
         g[2 * q] = pg.x * fg;
@@ -245,25 +268,28 @@ struct EpiGrad {
     }
   }
 
+  // One block of 16 columns after another, in halves: what a warp holds of it has to fit beside the block
+  // that it has asked for in 96 registers (whole blocks spill 112 bytes, two at a time 208: 8192 x
+  // 1536 x 4096, 122 us).
   template <int CW>
-  __device__ __forceinline__ void tile(const MmArgs& a, MmTile, int row, int col0, int M, uint32_t taddr, bool zero,
-                                       uint8_t* buf, Pre& pre) const {
+  __device__ __forceinline__ void tile(const MmArgs& a, MmTile, int row, int col0, int M, uint32_t taddr, bool zero, uint8_t*,
+                                       Pre& pre) const {
     const int lane = threadIdx.x % 32, row0 = row - lane;
     if (row0 >= M) return;  // warp-uniform
-    Outgoing<COLS> out(buf, lane);
 #pragma unroll 1
-    for (int cc = 0; cc < CW; cc += COLS) {
-      if (col0 + cc >= a.N) break;  // warp-uniform
-      uint32_t wh[COLS / 2], wg[COLS / 2], wu[COLS / 2];
+    for (int cc = 0; cc < CW; cc += 16) {
+      const int col = col0 + cc;
+      if (col >= a.N) break;  // warp-uniform
+      bf16 *hd = h + row * ld + col, *gd = dgu + 2 * P * (row * ld) + col;
+      uint32_t wh[8], wg[8], wu[8];  // (P = 1)
 #pragma unroll
-      for (int c = 0; c < COLS; c += 16) {
-        const int col = col0 + cc + c;
-        float g[16], u[16], dh[16];
-        values(pre, g, u);
-        if (cc + c + 16 < CW && col + 16 < a.N) ask(pre, row0, col + 16, lane);  // while this block is worked on
-        load16(taddr + cc + c, zero, dh);
+      for (int e = 0; e < 2; ++e) {
+        float g[8], u[8], dh[8];
+        values(pre, e, g, u);
+        if (e == 1 && cc + 16 < CW && col + 16 < a.N) ask(pre, row0, col + 16, lane);  // while this block is worked on
+        load8(taddr + cc + 8 * e, zero, dh);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
+        for (int q = 0; q < 8; ++q) {
           float act, slope;
           activation<ACT, F32>(g[q], act, slope);
           g[q] = act * u[q];
@@ -271,22 +297,23 @@ struct EpiGrad {
           dh[q] *= act;
         }
         if constexpr (P == 1) {
-          round16<false>(g, wh + c / 2);
-          round16<false>(u, wg + c / 2);
-          round16<false>(dh, wu + c / 2);
-        } else {
-          if (down) send_planes<P>(out, &h, g, col, row0, 0, 1);
-          if (inner) {
-            send_planes<P>(out, &dgu, u, col, row0, 0, 2);
-            send_planes<P>(out, &dgu, dh, col, row0, 1, 2);
+          pack8(g, wh + 4 * e);
+          pack8(u, wg + 4 * e);
+          pack8(dh, wu + 4 * e);
+        } else if (row < M) {
+          if (h) store8<P>(g, hd + 8 * e, plane);
+          if (dgu) {
+            store8<P>(u, gd + 8 * e, 2 * ld);
+            store8<P>(dh, gd + ld + 8 * e, 2 * ld);
           }
         }
       }
       if constexpr (P == 1) {
-        if (down) out.send(&h, wh, col0 + cc, row0, 0);
-        if (inner) {
-          out.send(&dgu, wg, col0 + cc, row0, 0);
-          out.send(&dgu, wu, col0 + cc, row0, 1);
+        if (row >= M) continue;
+        if (h) store16(wh, hd);
+        if (dgu) {
+          store16(wg, gd);
+          store16(wu, gd + ld);
         }
       }
     }
@@ -464,7 +491,7 @@ Plan make_plan(const llattn_gated_args& a, bool backward) {
   q.ldu = stride(q.pack_u, a.ldu, a.ff, a.d);
   q.ldd = stride(q.pack_d, a.ldd, a.d_out, a.ff);
   q.ldy = stride(q.pack_dy, a.lddy, n, a.d_out);
-  q.ldf = up8(a.ff);
+  q.ldf = cdiv(a.ff, kBlock) * kBlock;
   q.blocks = cdiv(a.ff, kBlock);
   const bool need_x = !backward || a.dw_gate || a.dw_up, need_gu = !backward || a.dx, inner = a.dx || a.dw_gate || a.dw_up;
   size_t off = 0;
@@ -541,7 +568,9 @@ cudaError_t run_fwd(const llattn_gated_args& a, const Plan& q, volatile unsigned
   const int64_t hplane = n * q.ldf;
   EpiGated<ACT, P> e{};
   e.ff = a.ff;
-  if (!sm100::make_block_map(&e.h, h, n, a.ff, q.ldf, P, hplane, e.COLS)) return cudaErrorInvalidValue;
+  e.h = h;
+  e.ld = q.ldf;
+  e.plane = hplane;
   if (a.kept) e.kept = kept_at(q, a);
   TRY(launch_active(product(q, n, 2 * a.ff, a.d, fault), x, g, e, s, &u));
   MmArgs p = y_args(q, a, fault);
@@ -567,11 +596,10 @@ cudaError_t run_bwd(const llattn_gated_args& a, const Plan& q, volatile unsigned
   float* part = reinterpret_cast<float*>(ws + q.part);
   EpiGrad<ACT, P> e{};
   e.kept = kept_at(q, a);
-  e.inner = a.dx || weights;
-  e.down = a.dw_down != nullptr;
-  if ((e.inner && !sm100::make_block_map(&e.dgu, dgu, n, a.ff, 2 * P * q.ldf, 2 * P, q.ldf, e.COLS)) ||
-      (e.down && !sm100::make_block_map(&e.h, h, n, a.ff, q.ldf, P, hplane, e.COLS)))
-    return cudaErrorInvalidValue;
+  e.dgu = a.dx || weights ? dgu : nullptr;
+  e.h = a.dw_down ? h : nullptr;
+  e.ld = q.ldf;
+  e.plane = hplane;
   TRY(launch_active(product(q, n, a.ff, a.d_out, fault), Operand{dy, n, a.d_out, q.ldy, q.planes, dyplane, 0},
                 Operand{q.pack_d ? ws + q.d : a.w_down, a.d_out, a.ff, q.ldd, q.planes, a.d_out * q.ldd, 1}, e, s));
   if (a.dx) {

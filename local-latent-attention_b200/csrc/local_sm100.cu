@@ -528,16 +528,6 @@ bool make_operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t 
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == CUDA_SUCCESS;
 }
 
-bool make_block_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int64_t nz, int64_t zs,
-                    int box_cols) {
-  if (((uintptr_t)base & 15) || ld % 8 || zs % 8) return false;
-  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)nz};
-  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(nz > 1 ? zs : rows * ld) * 2};
-  cuuint32_t box[3] = {(cuuint32_t)box_cols, 32, 1};
-  return encode_cached(map, 3, base, dims, strides, box, box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
-                       CU_TENSOR_MAP_L2_PROMOTION_NONE) == CUDA_SUCCESS;
-}
-
 bool gate_fusable(const Geom& g) { return g.Ld == 64 && g.H <= kGateMaxHeads; }
 
 cudaError_t launch_local_fwd(const Geom& g, const void* qkv, void* local_out, float* lse, const GateEpilogue& ep,

@@ -190,8 +190,9 @@ __device__ __forceinline__ void mm_tmem_dealloc(uint32_t t, uint32_t ncols) {
 //      need as long as their products take; 48 KB for twice the products do
 //      not hold the tensor cores up.
 //  2 = 256 x 256 on a pair, two accumulators
-//  5 = the same with 16 epilogue warps instead of 8, at 112 registers a thread and
-//      one stage less: for epilogues that work on every value for long
+//  5 = the same with 16 epilogue warps instead of 8, at 96 registers a thread, for
+//      epilogues that work on every value for long: they have no staging blocks
+//      (and one stage less: a sixth made dh's product of 8192 x 1536 x 4096 110 us instead of 105)
 //  1 = 128 x 128 on a CTA, two accumulators
 //  4 = 128 x 64 on a CTA, between 1 and 0
 //  0 = 128 x 32 on a CTA, for products too small to occupy the SMs otherwise:
@@ -210,7 +211,7 @@ struct MmShape {
   static constexpr int BR = HN / CG;        // rows of B that a CTA copies per half
   static constexpr int AB = 128 * 64 * 2;   // one CTA's A tile: 128 rows x 64 K, 16 KB
   static constexpr int BB = (BR < 64 ? 64 : BR) * 64 * 2;  // B tile of a half (a whole panel of 64 if MN-major)
-  static constexpr int STG = 4096;          // an epilogue warp's staging block: 32 rows of 128 bytes
+  static constexpr int STG = SH == 5 ? 0 : 4096;  // an epilogue warp's staging block: 32 rows of 128 bytes
   static constexpr int A = 0, B = A + ST * AB, STAGE = B + ST * NH * BB, BAR = STAGE + EW * STG;
   static constexpr int ACC = NH == 2 ? 1 : 2;      // accumulators in TMEM
   static constexpr int BLOCK = 205 * (BM * BN / 1024) / 64;  // mm_plan's `block`
@@ -481,39 +482,6 @@ __device__ __forceinline__ float2 bf16_pair(const uint4 (&u)[4], int i) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// Blocks of a warp's 32 rows and COLS bf16 columns on their way to memory: laid out
-// in the staging block as the tensor map's swizzle has it, sent by lane 0 (the
-// map's bounds cut what lies outside). 4 KB hold two blocks of 32 columns or four of 16.
-template <int COLS>
-struct Outgoing {
-  static constexpr int BYTES = 64 * COLS, N = 4096 / BYTES, CH = COLS / 8;
-  uint8_t* buf;
-  int lane, k = 0;
-  __device__ __forceinline__ Outgoing(uint8_t* b, int l) : buf(b), lane(l) {
-    if (lane == 0) bulk_wait_read<0>();
-    __syncwarp();
-  }
-  __device__ __forceinline__ void send(const CUtensorMap* map, const uint32_t (&w)[COLS / 2], int col, int row, int z) {
-    if (k >= N) {
-      if (lane == 0) bulk_wait_read<N - 1>();
-      __syncwarp();
-    }
-    uint8_t* b = buf + k % N * BYTES;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int at = CH == 4 ? lane * 64 + (c ^ (lane >> 1 & 3)) * 16 : lane * 32 + (c ^ (lane >> 2 & 1)) * 16;
-      *reinterpret_cast<uint4*>(b + at) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-    }
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_3d(map, b, col, row, z);
-      tma_store_commit();
-    }
-    ++k;
-  }
-};
-
 // sum (+)= an accumulator's CW columns of this thread's row
 template <int CW>
 __device__ __forceinline__ void drain(uint32_t acc, uint32_t sum, bool add) {
@@ -577,12 +545,6 @@ template <typename Epi, typename = void>
 struct SecondB : std::integral_constant<int, kSecondNone> {};
 template <typename Epi>
 struct SecondB<Epi, std::void_t<decltype(Epi::kSecond)>> : std::integral_constant<int, Epi::kSecond> {};
-
-// Epilogues that send blocks out by bulk copies (kBulkOut): lane 0 of each of their warps waits for its own at the end.
-template <typename Epi, typename = void>
-struct BulkOut : std::false_type {};
-template <typename Epi>
-struct BulkOut<Epi, std::void_t<decltype(Epi::kBulkOut)>> : std::bool_constant<Epi::kBulkOut> {};
 
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
@@ -881,7 +843,6 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
         }
       }
     }
-    if (BulkOut<Epi>::value && lane == 0) bulk_wait<0>();
     if (!ok) mm_raise(p, 8u, abort);
   }
   __syncwarp();

@@ -103,10 +103,6 @@ cudaError_t launch_gemm(const Geom& g, int M, int N, int K, const void* A, int64
 bool make_operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int64_t nz, int64_t zs,
                       int box_rows);
 
-// The same matrix for stores of blocks of 32 rows and 32 or 16 columns, in the 64- or 32-byte swizzle.
-bool make_block_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int64_t nz, int64_t zs,
-                    int box_cols);
-
 // Reads (and optionally clears) the device fault word of the current device:
 // bits set by a tensor-core kernel whose bounded wait ran out.
 unsigned read_fault_word(bool reset);
