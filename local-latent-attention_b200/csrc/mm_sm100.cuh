@@ -54,6 +54,12 @@ unsigned read_fault(bool reset) {
   return v;
 }
 
+// The schedule: total tiles, of which the first `full` run whole, one after
+// another on each CTA (pair), and the rest in s ranges of K each.
+struct MmPlan {
+  int total, full, s, items;
+};
+
 // One product. M, N, K are the host's sizes; m_dev / k_dev (optional) hold a
 // device-side row count from which M / K are cut: max(0, min(M, *m_dev -
 // dev_base)) (the rows past it are not computed, the K past it not read
@@ -85,6 +91,7 @@ struct MmArgs {
   const int* m_dev;
   const int* k_dev;
   int dev_base;
+  MmPlan plan;              // set by the launch where there is no device-side count
   volatile unsigned* fault_host;
 };
 
@@ -223,12 +230,6 @@ struct MmShape {
 
 struct MmTile {
   int z, m0, n0;
-};
-
-// The schedule: total tiles, of which the first `full` run whole, one after
-// another on each CTA (pair), and the rest in s ranges of K each.
-struct MmPlan {
-  int total, full, s, items;
 };
 
 // s splits the last, partial wave of `units`, each range at least 8 steps of K,
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   // takes it long (4 x 256^2 update: 88 us with the wait here, 66 so).
   const bool counted = p.m_dev || p.k_dev;
   if (counted) pdl_wait();
-  if (threadIdx.x == 0) {
+  if (counted && threadIdx.x == 0) {
     const MmGrid<SH> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
     *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
   }
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const int K = cut_rows(p.K, p.k_dev, p.dev_base);
   const MmGrid<SH> grid(p, M);
-  const MmPlan pl = *plan;
+  const MmPlan pl = counted ? *plan : p.plan;
   // one accumulator at a time: both halves of shape 3, or, with chains, where
   // the sum takes the place of the second
   constexpr bool one = S::ACC == 1 || (CHAIN && S::BN == 256);
@@ -867,10 +868,13 @@ __global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p,
   pdl_wait();
   const int M = cut_rows(p.M, p.m_dev, p.dev_base);
   const MmGrid<SH> grid(p, M);
-  if (threadIdx.x == 0)
-    plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
-  __syncthreads();
-  const MmPlan pl = plan;
+  const bool counted = p.m_dev || p.k_dev;
+  if (counted) {
+    if (threadIdx.x == 0)
+      plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
+    __syncthreads();
+  }
+  const MmPlan pl = counted ? plan : p.plan;
   const int tile = pl.full + blockIdx.x;
   if (tile >= pl.total) return;
   const MmTile w = grid.at(p, tile);
@@ -940,9 +944,8 @@ template <int SH, typename Epi>
 cudaError_t launch_join(const MmArgs& p, const Epi& epi, int units, cudaStream_t s, decltype(&Epi::quad)) {
   using S = MmShape<SH>;
   const MmGrid<SH> g(p, p.M);
-  const int total = g.per_z * p.nz;
-  // the device may have fewer tiles than the host's sizes say, never more
-  const int tail = std::min(total, units - 1);
+  // with counts the device may have fewer tiles than the host's sizes say, never more
+  const int tail = p.m_dev || p.k_dev ? std::min(g.per_z * p.nz, units - 1) : p.plan.s > 1 ? p.plan.total - p.plan.full : 0;
   if (tail < 1) return cudaSuccess;
   return launch_pdl(mm_join<SH, Epi>, dim3(tail, S::BM / 8), 256, 0, 1, s, p, epi, units);
 }
@@ -980,6 +983,8 @@ cudaError_t launch_mm_sh(MmArgs p, const Operand& a, const Operand& b, const Epi
   const int64_t tiles = (p.sym ? m * (m + 1) / 2 : m * n) * p.nz;
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
   const int units = p.split ? mm_units(SH) : (int)std::min<int64_t>(tiles, mm_units(SH));
+  // (on the device the schedule of a split product takes some 2 us, of every CTA of the join as well)
+  if (!p.m_dev && !p.k_dev) p.plan = mm_plan((int)tiles, units, cdiv(p.K, 64), p.split, S::BLOCK);
   e = launch_pdl(mm_kernel<SH, CHAIN, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, tb2, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<SH, Epi>(p, epi, units, s, nullptr);
