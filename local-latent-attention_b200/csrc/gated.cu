@@ -429,7 +429,7 @@ MmArgs y_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* faul
     p.n_terms = 2;
     p.pa = 0x01u;
   }
-  p.split = 1;
+  p.split = 2;
   return p;
 }
 // dx = dg Wg + du Wu: for each term of fp32's planes (or of G's two), smallest first, a
@@ -447,7 +447,7 @@ MmArgs dx_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* fau
     }
   p.n_terms = 2 * n;
   p.majors = 2;
-  p.split = 1;
+  p.split = 2;
   return p;
 }
 // dWd = dy^T h
@@ -457,7 +457,7 @@ MmArgs dwd_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* fa
     p.n_terms = 2;
     p.pb = 0x01u;
   }
-  p.split = 1;
+  p.split = 2;
   return p;
 }
 // [dWg; dWu] = [dg, du]^T x
@@ -467,7 +467,7 @@ MmArgs dwgu_args(const Plan& q, const llattn_gated_args& a, volatile unsigned* f
     p.n_terms = 2;
     p.pa = 0x01u;
   }
-  p.split = 1;
+  p.split = 2;
   return p;
 }
 

@@ -69,7 +69,8 @@ struct MmArgs {
   int a_mn, b_mn;
   int nz;                   // batch elements (tensor-map z)
   // Split K of the tiles that do not fill a wave: each range's sums go to part
-  // (fp32, one BM x BN block per range) and mm_join adds them up. 0: no split.
+  // (fp32, one BM x BN block per range) and mm_join adds them up. 0: no split; 1: ranges of at
+  // least 8 steps of K; 2: of 8 steps counting every term's.
   int split;
   float* part;
   // The tensor cores' additions drop what lies below the running sum's last
@@ -232,20 +233,21 @@ struct MmTile {
   int z, m0, n0;
 };
 
-// s splits the last, partial wave of `units`, each range at least 8 steps of K,
-// by the time of its ceil(tail s / units) rounds in steps: the range's own,
+// s splits the last, partial wave of `units`, each range at least 8 steps of K
+// (`terms` of them a step of the sum, for split = 2), by the time of its ceil(tail s / units) rounds in steps: the range's own,
 // 6 for its epilogue, and the partial sums' way through memory (a 256 x 256
 // block written and read takes the memory 0.2 of a step: `block`, in 1/1024).
-__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int block) {
+__host__ __device__ inline MmPlan mm_plan(int total, int units, int ksteps, int split, int terms, int block) {
   MmPlan r{total, total, 1, total};
   if (!split || total == 0) return r;
+  if (split == 1) terms = 1;
   const int full = total / units * units, tail = total - full;
   if (tail == 0) return r;
   int best = 1;
   int64_t cost = INT64_MAX;  // (integers: the product's and the join's kernel have to agree)
   for (int s = 1; s <= 32; ++s) {
-    if (s > 1 && (ksteps < 8 * s || (int64_t)tail * s > 4 * (int64_t)units)) break;
-    const int64_t c = 1024 * (int64_t)cdiv(tail * s, units) * (cdiv(ksteps, s) + 6) + (s > 1 ? (int64_t)block * tail * s : 0);
+    if (s > 1 && (ksteps < s || ksteps * terms < 8 * s || (int64_t)tail * s > 4 * (int64_t)units)) break;
+    const int64_t c = 1024 * (int64_t)cdiv(tail * s, units) * (cdiv(ksteps, s) * terms + 6) + (s > 1 ? (int64_t)block * tail * s : 0);
     if (c < cost) {
       cost = c;
       best = s;
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
   if (counted) pdl_wait();
   if (counted && threadIdx.x == 0) {
     const MmGrid<SH> g0(p, cut_rows(p.M, p.m_dev, p.dev_base));
-    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
+    *plan = mm_plan(g0.per_z * p.nz, n_units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.n_terms, S::BLOCK);
   }
   tc_fence_before();
   __syncthreads();
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(256) mm_join(const __grid_constant__ MmArgs p,
   const bool counted = p.m_dev || p.k_dev;
   if (counted) {
     if (threadIdx.x == 0)
-      plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, S::BLOCK);
+      plan = mm_plan(grid.per_z * p.nz, units, cdiv(cut_rows(p.K, p.k_dev, p.dev_base), 64), p.split, p.n_terms, S::BLOCK);
     __syncthreads();
   }
   const MmPlan pl = counted ? plan : p.plan;
@@ -916,7 +918,7 @@ double mm_time(const MmArgs& p) {
   constexpr double gap = SH == 3 ? 3.0 : 0.5, tail = SH == 3 ? 8.0 : SH == 2 ? 5.5 : SH == 1 ? 4.3 : SH == 4 ? 2.3 : 1.2;
   const MmGrid<SH> g(p, p.M);
   const int units = mm_units(SH), ks = cdiv(p.K, 64);
-  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, MmShape<SH>::BLOCK);
+  const MmPlan pl = mm_plan(g.per_z * p.nz, units, ks, p.split, p.n_terms, MmShape<SH>::BLOCK);
   double t = (pl.full / units + (pl.full % units ? 1 : 0)) * (ks * p.n_terms * step + gap);
   const int split = pl.items - pl.full;
   if (split) t += cdiv(split, units) * (cdiv(ks, pl.s) * p.n_terms * step + gap) + split * step * MmShape<SH>::BLOCK / 1024;
@@ -924,7 +926,11 @@ double mm_time(const MmArgs& p) {
 }
 
 // whether mm_plan may split anything, whatever the device-side counts
-inline bool joins(const MmArgs& p) { return p.split && cdiv(p.K, 64) >= 16; }
+inline int mm_ranges(const MmArgs& p) {
+  const int ks = cdiv(p.K, 64);
+  return !p.split ? 1 : std::min(32, p.split == 2 ? std::min(ks, ks * p.n_terms / 8) : ks / 8);
+}
+inline bool joins(const MmArgs& p) { return mm_ranges(p) > 1; }
 
 // fp32 elements of MmArgs::part for a product of at most these sizes: mm_plan
 // splits fewer tiles than units, each into as many ranges as K's steps allow
@@ -932,7 +938,7 @@ inline bool joins(const MmArgs& p) { return p.split && cdiv(p.K, 64) >= 16; }
 template <int SH>
 int64_t mm_part_blocks(const MmArgs& p) {
   const int64_t tiles = (int64_t)cdiv(p.M, MmShape<SH>::BM) * cdiv(p.N, MmShape<SH>::BN) * std::max(p.nz, 1);
-  const int64_t units = mm_units(SH), ranges = std::min(32, cdiv(p.K, 64) / 8);
+  const int64_t units = mm_units(SH), ranges = mm_ranges(p);
   return std::min(4 * units, std::min(tiles, units - 1) * ranges) * MmShape<SH>::BM * MmShape<SH>::BN;
 }
 inline int64_t mm_part_floats(const MmArgs& p) {
@@ -984,7 +990,7 @@ cudaError_t launch_mm_sh(MmArgs p, const Operand& a, const Operand& b, const Epi
   if (tiles > 0x1ffffff) return cudaErrorInvalidValue;
   const int units = p.split ? mm_units(SH) : (int)std::min<int64_t>(tiles, mm_units(SH));
   // (on the device the schedule of a split product takes some 2 us, of every CTA of the join as well)
-  if (!p.m_dev && !p.k_dev) p.plan = mm_plan((int)tiles, units, cdiv(p.K, 64), p.split, S::BLOCK);
+  if (!p.m_dev && !p.k_dev) p.plan = mm_plan((int)tiles, units, cdiv(p.K, 64), p.split, p.n_terms, S::BLOCK);
   e = launch_pdl(mm_kernel<SH, CHAIN, Epi>, dim3((unsigned)(units * S::CG)), S::THREADS, S::SMEM, S::CG, s, ta, tb, tb2, p, epi);
   if (e != cudaSuccess || !joins(p)) return e;
   return launch_join<SH, Epi>(p, epi, units, s, nullptr);

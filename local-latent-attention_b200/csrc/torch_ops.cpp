@@ -288,6 +288,8 @@ PyObject* py_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
   pointers.reserve(count);
   sizes.reserve(count);
   dtypes.reserve(count);
+  std::vector<const Tensor*> used;
+  used.reserve(count);
   const Tensor* first = nullptr;
   for (Py_ssize_t i = 0; i < count; ++i) {
     PyObject* o = PyList_GET_ITEM(args[0], i);
@@ -299,6 +301,7 @@ PyObject* py_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int dtype = dtype_of(t);
     if (!plain(t) || dtype < 0 || (first && t.device() != first->device()) || !t.is_non_overlapping_and_dense()) Py_RETURN_NONE;
     if (!first) first = &t;
+    used.push_back(&t);
     pointers.push_back(t.data_ptr());
     sizes.push_back(t.numel());
     dtypes.push_back(dtype);
@@ -322,6 +325,9 @@ PyObject* py_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int rc = llattn_clip(&a, stream(norm));
   if (rc == LLATTN_ERR_ARG) Py_RETURN_NONE;
   check(rc, "llattn_clip");
+  if (scale)  // autograd has to see that they changed
+    for (const Tensor* t : used)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(std::move(norm));
   END_HANDLE_TH_ERRORS
 }

@@ -402,10 +402,11 @@ def _norm_of(tensors: list[Tensor], norm_type: int) -> Tensor:
 def _clip_of(grads: list[Tensor], max_norm: float, norm_type: int) -> Tensor:
     dense = _dense_all(grads, "clip_grad_norm_")
     norm = _clip(dense, norm_type, max_norm, True)
-    if dense is not grads:
-        for g, c in zip(grads, dense):
-            if c is not g:
-                g.copy_(c)
+    for g, c in zip(grads, dense):
+        if c is not g:
+            g.copy_(c)
+        elif not g.is_inference():
+            torch.autograd.graph.increment_version(g)  # autograd has to see that it changed
     return norm
 
 
@@ -434,7 +435,8 @@ def _norm_code(norm_type) -> int:
 def total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
     """The norm of all tensors' elements together, as a float32 scalar on their
     device: the 2-norm (sums in fp64, in a fixed order; finite for any finite float32
-    result) or, for norm_type=inf, the largest magnitude. NaN where one of them is.
+    result) or, for norm_type=inf, the largest magnitude. NaN where one of them is. Not
+    differentiable.
     Tensors are bfloat16 or float32, of any shapes and mix, on one CUDA device; 0
     on the CPU for an empty list."""
     code = _norm_code(norm_type)

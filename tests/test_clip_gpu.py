@@ -181,6 +181,23 @@ def test_same_bits_graphs_streams_and_compile():
     assert torch.equal(f(source), total_norm(source))
 
 
+def test_autograd_sees_the_change():
+    ps = params([(10,), (4, 6)], (FP,))
+    ps[1].grad = torch.randn(6, 4, device="cuda").t()  # (dense)
+    wide = params([(4, 4)], (FP,))[0]
+    wide.grad = torch.randn(4, 9, device="cuda")[:, 2:6]  # (not dense: by way of a copy)
+    w = torch.ones(10, device="cuda", requires_grad=True)
+    y = (w * ps[0].grad).sum()  # saves the gradient
+    before = [p.grad._version for p in (*ps, wide)]
+    clip_grad_norm_([*ps, wide], 0.1)
+    assert all(p.grad._version > v for p, v in zip((*ps, wide), before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    version = ps[0].grad._version
+    total_norm([p.grad for p in ps])
+    assert ps[0].grad._version == version
+
+
 def test_refusals():
     (p, q) = params([(10,), (10,)], (FP,))
     for kw, msg in ((dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"),
