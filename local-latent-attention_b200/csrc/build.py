@@ -83,7 +83,9 @@ def build_torch_ops() -> None:
 
     src, home = os.path.join(CSRC, "torch_ops.cpp"), os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(NVCC))), "include")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    # g++ of the path, as nvcc takes it, whatever CXX says: a newer one may link its libstdc++ in beside
+    # torch's shared one, and the two do not mix (formatting an error message crashed)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-I" + INCLUDE,
            "-I" + os.path.join(home, "include"), "-I" + os.path.join(home, "include", "torch", "csrc", "api", "include"),
            "-I" + sysconfig.get_paths()["include"], "-I" + cuda, "-L" + os.path.join(home, "lib"), "-L" + PKG,

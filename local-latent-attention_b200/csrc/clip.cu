@@ -168,7 +168,7 @@ __device__ __forceinline__ double block_join(double a, double* red) {
 }
 
 template <typename Op, int CAP>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<CAP> t, double* part) {
   __shared__ double red[kThreads / 32];
   const int2 run = run_of(t);
   int e = entry_of(t, run.x);
@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
 
 // n_part: all batches' sums. scale: 0 writes the norm alone.
 template <typename Op, int CAP>
-__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ Table<CAP> t, const double* __restrict__ part,
-                                                        int n_part, double max_norm, int scale, float* __restrict__ norm) {
+__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ Table<CAP> t, const double* part,
+                                                        int n_part, double max_norm, int scale, float* norm) {
   __shared__ double red[kThreads / 32];
   const int2 run = run_of(t);
   int e = scale && run.y > run.x ? entry_of(t, run.y - 1) : 0;

@@ -107,9 +107,9 @@ struct Pack {
 
 // A warp per token and 4 packs a lane of its columns.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) embed_rows(Ids ids, const T* __restrict__ w, int64_t ldw, const T* __restrict__ pos,
+__global__ void __launch_bounds__(256) embed_rows(Ids ids, const T* w, int64_t ldw, const T* pos,
                                                   int64_t ldp, int length, int64_t tokens, int slices, int d, float scale,
-                                                  T* __restrict__ out) {
+                                                  T* out) {
   pdl_next();
   pdl_wait();
   using P = Pack<T, VEC>;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(256) embed_rows(Ids ids, const T* __restrict__
 template <typename T>
 struct Positions {
   const T* dout;
-  int batch, per, splits;
+  int batch, per;
   int64_t cols, all;  // length d, position_rows d
   float* part;
   T* dp;
@@ -179,8 +179,8 @@ __device__ __forceinline__ void position_sums(const Positions<T>& q, int64_t thr
   }
 }
 template <typename T>
-__global__ void __launch_bounds__(256) embed_positions_join(const float* __restrict__ part, int parts, int64_t cols,
-                                                            T* __restrict__ dp) {
+__global__ void __launch_bounds__(256) embed_positions_join(const float* part, int parts, int64_t cols,
+                                                            T* dp) {
   pdl_next();
   pdl_wait();
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -206,7 +206,7 @@ __device__ __forceinline__ int slot_of(int v, int bits) {  // span = 1 << bits
 // held: the tokens' places stay in shared memory for the second pass, n of them; otherwise each
 // pass reads the ids. (Places in registers took a loop unrolled 32 times: 11 us of fetching it.)
 __device__ __forceinline__ void sort_tokens(const Ids& ids, int n, int bits, bool held, int cta, int ctas,
-                                            int* __restrict__ order, int* __restrict__ words, int* __restrict__ start) {
+                                            int* order, int* words, int* start) {
   extern __shared__ int counts[];  // [kSortWarps][span], then the places
   __shared__ int sums[kSortWarps];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -302,8 +302,8 @@ __device__ __forceinline__ void sort_tokens(const Ids& ids, int n, int bits, boo
 // The first `sorters` CTAs sort, the others sum dP.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSortThreads, 2) embed_sort(Ids ids, int n, int bits, int held, int sorters,
-                                                           int* __restrict__ order, int* __restrict__ words,
-                                                           int* __restrict__ start, Positions<T> q, int per_split) {
+                                                           int* order, int* words,
+                                                           int* start, Positions<T> q, int per_split) {
   pdl_next();
   pdl_wait();
   if ((int)blockIdx.x < sorters) {
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kSortThreads, 2) embed_sort(Ids ids, int n, in
 
 // Columns [c0, c0 + 32 kSlice packs) of rows added to a, the j-th of up to 32 being row index(j) of dout.
 template <typename T, bool VEC, typename Index>
-__device__ __forceinline__ void add_rows(Pack<T, VEC> (&a)[kSlice], const T* __restrict__ dout, int d, int c0, int m, Index index) {
+__device__ __forceinline__ void add_rows(Pack<T, VEC> (&a)[kSlice], const T* dout, int d, int c0, int m, Index index) {
   using P = Pack<T, VEC>;
   const int lane = threadIdx.x % 32;
 #pragma unroll 1
@@ -346,10 +346,10 @@ __device__ __forceinline__ void add_rows(Pack<T, VEC> (&a)[kSlice], const T* __r
 // one, where that is another. The warps after write the other words, kWords each, a quarter of
 // the vocabulary apart: most words have no token and cost little but the wait for their count.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) embed_sums(const T* __restrict__ dout, const int* __restrict__ order,
-                                                  const int* __restrict__ words, const int* __restrict__ start, int vocab,
+__global__ void __launch_bounds__(256) embed_sums(const T* dout, const int* order,
+                                                  const int* words, const int* start, int vocab,
                                                   int bits, int total_at, int d, int slices, int pieces, float scale,
-                                                  float* __restrict__ part, T* __restrict__ dw) {
+                                                  float* part, T* dw) {
   pdl_next();
   pdl_wait();
   using P = Pack<T, VEC>;
@@ -414,9 +414,9 @@ __global__ void __launch_bounds__(256) embed_sums(const T* __restrict__ dout, co
 // The words of more than kHot tokens: a warp for each that starts in interval p (there
 // is one at most: the interval's last word), 32 columns.
 template <typename T>
-__global__ void __launch_bounds__(256) embed_join(const int* __restrict__ words, const int* __restrict__ start, int bits,
+__global__ void __launch_bounds__(256) embed_join(const int* words, const int* start, int bits,
                                                   int total_at, int d, int slices, int pieces, float scale,
-                                                  const float* __restrict__ part, T* __restrict__ dw) {
+                                                  const float* part, T* dw) {
   pdl_next();
   pdl_wait();
   const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
@@ -443,8 +443,8 @@ __global__ void __launch_bounds__(256) embed_join(const int* __restrict__ words,
 // Few words and tokens: a CTA per word and 1 KB of columns, whose warps each pick the word's tokens out of
 // an eighth of the ids; then the CTAs of dP.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) embed_small(Ids ids, int n, const T* __restrict__ dout, int d, int slices, float scale,
-                                                   T* __restrict__ dw, int word_ctas, Positions<T> q, int per_split) {
+__global__ void __launch_bounds__(256) embed_small(Ids ids, int n, const T* dout, int d, int slices, float scale,
+                                                   T* dw, int word_ctas, Positions<T> q, int per_split) {
   pdl_next();
   pdl_wait();
   if ((int)blockIdx.x >= word_ctas) {
@@ -568,7 +568,7 @@ cudaError_t bwd(const llattn_embed_args& a, const Plan& q, cudaStream_t s) {
   T* dw = static_cast<T*>(a.dw);
   const int64_t all = a.dpositions ? (int64_t)a.position_rows * a.d : 0;
   float* pos = q.splits > 1 ? reinterpret_cast<float*>(ws + q.pos) : nullptr;
-  const Positions<T> pq{dout, a.batch, q.per, q.splits, q.cols, all, pos, static_cast<T*>(a.dpositions)};
+  const Positions<T> pq{dout, a.batch, q.per, q.cols, all, pos, static_cast<T*>(a.dpositions)};
   const bool small = !dw || q.small;
   const int threads = small ? 256 : kSortThreads;
   const int64_t per_split = cdiv64(all, (int64_t)threads * Pack<T, VEC>::N), pos_ctas = per_split * q.splits;

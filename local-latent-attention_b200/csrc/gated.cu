@@ -658,11 +658,11 @@ int launches(const llattn_gated_args& a, bool backward) {
   if (few(a, backward)) return 2;
   const Plan q = make_plan(a, backward);
   const bool weights = a.dw_gate || a.dw_up;
-  if (!backward) return (q.pack_x || q.pack_g || q.pack_u || q.pack_d) + 2 + joins(y_args(q, a, nullptr));
+  if (!backward) return (q.pack_x || q.pack_g || q.pack_u || q.pack_d) + 1 + mm_launches<EpiOut>(y_args(q, a, nullptr), 0, 0);
   int n = (q.pack_dy || q.pack_d || (a.dx && (q.pack_g || q.pack_u)) || (weights && q.pack_x)) + 1;
-  if (a.dx) n += 1 + joins(dx_args(q, a, nullptr));
-  if (a.dw_down) n += 1 + joins(dwd_args(q, a, nullptr));
-  if (weights) n += 1 + joins(dwgu_args(q, a, nullptr));
+  if (a.dx) n += mm_launches<EpiDx>(dx_args(q, a, nullptr), 0, 1);
+  if (a.dw_down) n += mm_launches<EpiOut>(dwd_args(q, a, nullptr), 1, 1);
+  if (weights) n += mm_launches<EpiTwo>(dwgu_args(q, a, nullptr), 1, 1);
   return n;
 }
 

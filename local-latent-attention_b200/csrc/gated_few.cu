@@ -59,16 +59,22 @@ struct FewShape {
 struct Raw {
   uint4 c[2];
 };
-// [lo, hi): the matrix's bytes
-template <typename T, bool SHIFT>
+// [lo, hi): the matrix's bytes. W: a weight, by the read-only path; otherwise what the kernel before
+// may have written while this one was already there, which the read-only path does not allow for.
+template <bool W>
+__device__ __forceinline__ uint4 load16(uintptr_t q) {
+  const uint4* p = reinterpret_cast<const uint4*>(q);
+  return W ? __ldg(p) : *p;
+}
+template <typename T, bool SHIFT, bool W>
 __device__ __forceinline__ void raw_load(Raw& r, const T* row, int k, int K, bool ok, uintptr_t lo, uintptr_t hi) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(row + k), q = SHIFT ? a & ~uintptr_t(15) : a;
   const uintptr_t b = a + min(16, (K - k) * (int)sizeof(T));  // the end of what is there
   ok = ok && k < K;
   const uint4 z = make_uint4(0, 0, 0, 0);
   const bool first = ok && (!SHIFT || q >= lo) && q + 16 <= hi, second = SHIFT && ok && q + 16 < b && q + 32 <= hi;
-  r.c[0] = first ? __ldg(reinterpret_cast<const uint4*>(q)) : z;
-  if (SHIFT) r.c[1] = second ? __ldg(reinterpret_cast<const uint4*>(q + 16)) : z;
+  r.c[0] = first ? load16<W>(q) : z;
+  if (SHIFT) r.c[1] = second ? load16<W>(q + 16) : z;
   // the matrix's first and last bytes, where a chunk reaches past them
   const bool edge0 = ok && !first, edge1 = SHIFT && ok && !second && q + 16 < b;
   if (edge0 || edge1) {
@@ -179,13 +185,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) raw_load<T, SHIFT>(b[w][h], row[w][h], k, ke, ok[h], lo[w], hi[w]);
+      for (int h = 0; h < 2; ++h) raw_load<T, SHIFT, true>(b[w][h], row[w][h], k, ke, ok[h], lo[w], hi[w]);
   };
   auto issue_x = [&](int j, Raw (&b)[F32 ? 1 : PLANES]) {
     if constexpr (!F32) {
       const int k = kl + j * S::STEP;
       if constexpr (NW == 2) {
-        raw_load<T, XSHIFT>(b[0], xr, k, ke, x_ok, xlo, xhi);
+        raw_load<T, XSHIFT, false>(b[0], xr, k, ke, x_ok, xlo, xhi);
       } else {
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl)

@@ -996,6 +996,20 @@ cudaError_t launch_mm_sh(MmArgs p, const Operand& a, const Operand& b, const Epi
   return launch_join<SH, Epi>(p, epi, units, s, nullptr);
 }
 
+// the shape that launch_mm takes
+template <typename Epi>
+int mm_choose(const MmArgs& p) {
+  const double t2 = mm_time<2>(p), t1 = mm_time<1>(p);
+  if (Epi::kNarrow) {
+    MmArgs q = p;
+    q.sym = 0;
+    const double t4 = mm_time<4>(q), t0 = mm_time<0>(q);
+    if (std::min(t0, t4) < std::min(t1, t2)) return t0 <= t4 ? 0 : 4;
+  }
+  if (Epi::kWide && !p.chain && mm_time<3>(p) < std::min(t1, t2)) return 3;
+  return t2 <= t1 ? 2 : 1;
+}
+
 template <typename Epi>
 cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& epi, cudaStream_t s,
                       const Operand* b2 = nullptr) {
@@ -1004,18 +1018,35 @@ cudaError_t launch_mm(MmArgs p, const Operand& a, const Operand& b, const Epi& e
   if (p.nz < 1) p.nz = 1;
   if (p.n_terms < 1) p.n_terms = 1;
   if (p.M < 1 || p.N < 1 || p.K < 1 || (joins(p) && !p.part)) return cudaErrorInvalidValue;
-  const double t2 = mm_time<2>(p), t1 = mm_time<1>(p);
+  const int shape = mm_choose<Epi>(p);
   if constexpr (Epi::kNarrow) {
-    MmArgs q = p;
-    q.sym = 0;  // not square: every tile is computed
-    const double t4 = mm_time<4>(q), t0 = mm_time<0>(q);
-    if (std::min(t0, t4) < std::min(t1, t2))
-      return t0 <= t4 ? launch_mm_sh<0>(q, a, b, epi, s, b2) : launch_mm_sh<4>(q, a, b, epi, s, b2);
+    if (shape == 0 || shape == 4) p.sym = 0;  // not square: every tile is computed
+    if (shape == 0) return launch_mm_sh<0>(p, a, b, epi, s, b2);
+    if (shape == 4) return launch_mm_sh<4>(p, a, b, epi, s, b2);
   }
   if constexpr (Epi::kWide) {
-    if (!p.chain && mm_time<3>(p) < std::min(t1, t2)) return launch_mm_sh<3>(p, a, b, epi, s, b2);
+    if (shape == 3) return launch_mm_sh<3>(p, a, b, epi, s, b2);
   }
-  return t2 <= t1 ? launch_mm_sh<2>(p, a, b, epi, s, b2) : launch_mm_sh<1>(p, a, b, epi, s, b2);
+  return shape == 2 ? launch_mm_sh<2>(p, a, b, epi, s, b2) : launch_mm_sh<1>(p, a, b, epi, s, b2);
+}
+
+// Kernels of launch_mm without device-side counts: the product's, and the join's where tiles are split.
+template <typename Epi>
+int mm_launches(MmArgs p, bool a_mn, bool b_mn) {
+  p.a_mn = a_mn;
+  p.b_mn = b_mn;
+  auto split = [&](auto shape) {
+    constexpr int SH = decltype(shape)::value;
+    const MmGrid<SH> g(p, p.M);
+    return mm_plan(g.per_z * p.nz, mm_units(SH), cdiv(p.K, 64), p.split, p.n_terms, MmShape<SH>::BLOCK).s > 1;
+  };
+  switch (mm_choose<Epi>(p)) {
+    case 0: return 1 + split(std::integral_constant<int, 0>());
+    case 1: return 1 + split(std::integral_constant<int, 1>());
+    case 2: return 1 + split(std::integral_constant<int, 2>());
+    case 3: return 1 + split(std::integral_constant<int, 3>());
+    default: return 1 + split(std::integral_constant<int, 4>());
+  }
 }
 
 }  // namespace

@@ -231,7 +231,7 @@ struct EpiUpdate {
 
 // partial sums of squares of matrix blockIdx.y, fixed order
 template <typename T>
-__global__ void __launch_bounds__(256) orth_square(const __grid_constant__ Ptrs g, int64_t n, float* __restrict__ part) {
+__global__ void __launch_bounds__(256) orth_square(const __grid_constant__ Ptrs g, int64_t n, float* part) {
   __shared__ float red[8];
   pdl_next();
   pdl_wait();
@@ -276,9 +276,9 @@ __global__ void __launch_bounds__(256) orth_square(const __grid_constant__ Ptrs 
 // hi = fp16(G 2^e), lo = bf16(G 2^e - hi) (optional), s0 = 2^-e / (|G| + eps)
 template <typename T>
 __global__ void __launch_bounds__(256) orth_convert(const __grid_constant__ Ptrs g, int rows, int cols,
-                                                    const float* __restrict__ part, int n_parts, float eps,
-                                                    __half* __restrict__ hi, bf16* __restrict__ lo, int64_t ld, int64_t zs,
-                                                    float* __restrict__ s0) {
+                                                    const float* part, int n_parts, float eps,
+                                                    __half* hi, bf16* lo, int64_t ld, int64_t zs,
+                                                    float* s0) {
   __shared__ float sh[2];
   pdl_next();
   pdl_wait();
@@ -481,7 +481,7 @@ __device__ __forceinline__ void small_read(const T* src, bool tall, int q, int L
 
 template <typename T>
 __global__ void __launch_bounds__(kSmallT) orth_small(const __grid_constant__ Ptrs g, int rows, int cols, int steps,
-                                                      float ca, float cb, float cc, float eps, bf16* __restrict__ out) {
+                                                      float ca, float cb, float cc, float eps, bf16* out) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = cluster.num_blocks(), rank = cluster.block_rank();

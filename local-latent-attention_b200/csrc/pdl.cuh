@@ -9,7 +9,9 @@ namespace {
 // Programmatic dependent launch: a kernel may start (set up its barriers, TMEM
 // and tensor maps) while the one before it in the stream finishes; pdl_wait
 // returns when everything before is complete and visible, so it comes before
-// the first access to global memory; pdl_next lets the kernel after start.
+// the first access to global memory; pdl_next lets the kernel after start. What a
+// kernel before wrote is not read through __restrict__ or __ldg: the read-only path wants it
+// unchanged from this kernel's start on, which is before the wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

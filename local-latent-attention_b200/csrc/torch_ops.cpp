@@ -24,6 +24,9 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// what the library takes
+constexpr int64_t kMostTokens = 1 << 26, kMostIds = 1 << 30, kMostWords = 1 << 24, kMostColumns = 1 << 20;
+
 constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
 
@@ -144,8 +147,8 @@ PyObject* py_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
                &wd = THPVariable_Unpack(args[3]);
   if (!plain(x) || dtype_of(x) < 0 || !like(wg, x) || !like(wu, x) || !like(wd, x) || x.dim() < 1 || x.numel() == 0 || wg.dim() != 2 ||
       wd.dim() != 2 || wg.sizes() != wu.sizes() || x.size(-1) != wg.size(1) || wd.size(1) != wg.size(0) || wg.numel() == 0 ||
-      wd.numel() == 0 || x.numel() / x.size(-1) > INT32_MAX || wg.size(0) > INT32_MAX || wg.size(1) > INT32_MAX ||
-      wd.size(0) > INT32_MAX)
+      wd.numel() == 0 || x.numel() / x.size(-1) > kMostTokens || wg.size(0) > kMostColumns || wg.size(1) > kMostColumns ||
+      wd.size(0) > kMostColumns)
     Py_RETURN_NONE;
   const int act = (int)PyLong_AsLong(args[4]);
   Tensor y;
@@ -208,13 +211,14 @@ struct Embed : torch::autograd::Function<Embed> {
     ctx->saved_data["rows"] = pos ? pos->size(0) : 0;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    ctx->saved_data["need"] = (w.requires_grad() ? 1 : 0) + (pos && pos->requires_grad() ? 2 : 0);
     return embed_forward(ids, w, pos ? *pos : Tensor(), scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(5);
     if (!grads[0].defined()) return out;
-    const int64_t need = ctx->saved_data["need"].toInt(), position_rows = ctx->saved_data["rows"].toInt();
+    const int64_t position_rows = ctx->saved_data["rows"].toInt();
+    const bool need_w = ctx->needs_input_grad(1), need_p = position_rows && ctx->needs_input_grad(2);
+    if (!need_w && !need_p) return out;
     {
       at::NoGradGuard no_grad;
       const c10::cuda::CUDAGuard guard(grads[0].device());
@@ -223,8 +227,8 @@ struct Embed : torch::autograd::Function<Embed> {
       llattn_embed_args a = embed_args(ids, vocab, d, dtype_of(dout), position_rows, ctx->saved_data["scale"].toDouble(),
                                        ctx->saved_data["padding"].toInt());
       const auto opts = dout.options().requires_grad(false);
-      if (need & 1) out[1] = at::empty({vocab, d}, opts);
-      if (need & 2) out[2] = at::empty({position_rows, d}, opts);
+      if (need_w) out[1] = at::empty({vocab, d}, opts);
+      if (need_p) out[2] = at::empty({position_rows, d}, opts);
       a.dout = dout.data_ptr();
       a.dw = data(out[1]);
       a.dpositions = data(out[2]);
@@ -247,8 +251,8 @@ PyObject* py_embed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   std::optional<Tensor> pos;
   if (args[2] != Py_None) pos = THPVariable_Unpack(args[2]);
   if (!plain(ids) || !plain(w) || dtype_of(w) < 0 || ids.device() != w.device() || w.dim() != 2 || w.numel() == 0 ||
-      (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || ids.numel() == 0 || ids.numel() > INT32_MAX ||
-      w.size(1) > INT32_MAX)
+      (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || ids.numel() == 0 || ids.numel() > kMostIds ||
+      w.size(0) > kMostWords || w.size(1) > kMostColumns)
     Py_RETURN_NONE;
   if (pos && (!like(*pos, w) || ids.dim() < 1 || pos->dim() != 2 || pos->size(0) < ids.size(-1) || pos->size(1) != w.size(1) ||
               pos->size(0) > INT32_MAX))

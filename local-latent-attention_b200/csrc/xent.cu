@@ -258,12 +258,12 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // (32768 targets: one CTA's scan alone took 56 us, this launch takes 55 with its
 // 200 MB of packed rows, read and written). The first n_w CTAs pack w instead, 16 rows each.
 template <typename T>
-__global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_t ldx, int d,
-                                                 const int64_t* __restrict__ targets, int n, int64_t ignore, int vocab,
-                                                 int per, int* __restrict__ idx, int* __restrict__ tgt,
-                                                 float* __restrict__ lt, int* __restrict__ count, bf16* __restrict__ xs,
-                                                 int64_t lds, int64_t plane, const T* __restrict__ w, int64_t ldw,
-                                                 bf16* __restrict__ wp, int64_t ldwp, int64_t wplane, int n_w) {
+__global__ void __launch_bounds__(256) xent_prep(const T* x, int64_t ldx, int d,
+                                                 const int64_t* targets, int n, int64_t ignore, int vocab,
+                                                 int per, int* idx, int* tgt,
+                                                 float* lt, int* count, bf16* xs,
+                                                 int64_t lds, int64_t plane, const T* w, int64_t ldw,
+                                                 bf16* wp, int64_t ldwp, int64_t wplane, int n_w) {
   pdl_next();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(256) xent_prep(const T* __restrict__ x, int64_
 
 // logsumexp of a row from its tiles, as (max, log2 of the sum relative to it)
 template <int NT>
-__device__ __forceinline__ float2 join_tiles(const float2* __restrict__ st, int n_tiles, float* red) {
+__device__ __forceinline__ float2 join_tiles(const float2* st, int n_tiles, float* red) {
   // the first 8 NT tiles (all of them up to V = 32 K a tile of 32 columns) are
   // read once, together
   constexpr int KEEP = 8;
@@ -361,9 +361,9 @@ __device__ __forceinline__ float2 join_tiles(const float2* __restrict__ st, int 
 __device__ __forceinline__ float row_loss(float2 lse, float lt) { return (lse.x - lt) + lse.y * kLn2; }
 
 // Losses without gradients: one CTA per row.
-__global__ void __launch_bounds__(128) xent_losses(const float2* __restrict__ stats, int n_tiles,
-                                                   const float* __restrict__ lt, const int64_t* __restrict__ targets,
-                                                   int64_t ignore, int vocab, float* __restrict__ losses) {
+__global__ void __launch_bounds__(128) xent_losses(const float2* stats, int n_tiles,
+                                                   const float* lt, const int64_t* targets,
+                                                   int64_t ignore, int vocab, float* losses) {
   __shared__ float red[4];
   pdl_next();
   pdl_wait();
@@ -402,12 +402,12 @@ __device__ __forceinline__ void sum_losses(int* count, const float* losses, int 
 // piece to finish sums the losses (thread t those of index t mod 256, then
 // in thread order: the same bits whichever CTA it is).
 template <int PLANES, int SHARES>
-__global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stats, int n_tiles, int rows, int vocab,
-                                                 int* __restrict__ count, int base, const int* __restrict__ idx,
-                                                 const int* __restrict__ tgt, const float* __restrict__ lt,
-                                                 const float* __restrict__ grad_rows, int mean, float* losses,
-                                                 void* __restrict__ p, int64_t ldp, bf16* __restrict__ planes,
-                                                 int64_t plane, float* __restrict__ loss) {
+__global__ void __launch_bounds__(256) xent_rows(const float2* stats, int n_tiles, int rows, int vocab,
+                                                 int* count, int base, const int* idx,
+                                                 const int* tgt, const float* lt,
+                                                 const float* grad_rows, int mean, float* losses,
+                                                 void* p, int64_t ldp, bf16* planes,
+                                                 int64_t plane, float* loss) {
   constexpr bool SPLIT = PLANES > 1;
   extern __shared__ float xent_f[];  // [n_tiles]
   __shared__ float red[8];
@@ -480,9 +480,9 @@ __global__ void __launch_bounds__(256) xent_rows(const float2* __restrict__ stat
 
 // loss = sum of the losses (ignored tokens' are 0), over the number that count
 // when mean. One CTA, fixed order.
-__global__ void __launch_bounds__(1024) xent_reduce(const float* __restrict__ losses, int n,
-                                                    const int64_t* __restrict__ targets, int64_t ignore, int mean,
-                                                    float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) xent_reduce(const float* losses, int n,
+                                                    const int64_t* targets, int64_t ignore, int mean,
+                                                    float* loss) {
   pdl_next();
   pdl_wait();
   __shared__ float red[32];
@@ -512,8 +512,8 @@ __device__ __forceinline__ void scale_run(T* p, int64_t n, float f) {
   for (int64_t i = nv * PER + i0; i < n; i += step) p[i] = from_f<T>(to_f<T>(p[i]) * f);
 }
 template <typename T>
-__global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ a, int64_t na, T* __restrict__ b, int64_t nb,
-                                                    const float* __restrict__ s) {
+__global__ void __launch_bounds__(256) scale_kernel(T* a, int64_t na, T* b, int64_t nb,
+                                                    const float* s) {
   pdl_next();
   pdl_wait();
   const float f = *s;

@@ -58,7 +58,8 @@ def _check_gated(x: Tensor, wg: Tensor, wu: Tensor, wd: Tensor) -> None:
     if (x.is_cuda and x.dim() == 2 and wg.dim() == 2 and wd.dim() == 2 and wg.shape == wu.shape
             and x.shape[1] == wg.shape[1] and wd.shape[1] == wg.shape[0] and x.dtype in _TYPES and x.dtype == wg.dtype
             and x.dtype == wu.dtype and x.dtype == wd.dtype and x.device == wg.device and x.device == wu.device
-            and x.device == wd.device and wg.numel() and wd.numel()):
+            and x.device == wd.device and wg.numel() and wd.numel() and x.shape[0] <= 1 << 26
+            and max(*wg.shape, wd.shape[0]) <= 1 << 20):
         return
     _require(x.is_cuda, "gated_mlp needs CUDA tensors")
     _require(x.dim() == 2 and wg.dim() == 2 and wg.shape == wu.shape and x.shape[1] == wg.shape[1],
@@ -69,7 +70,8 @@ def _check_gated(x: Tensor, wg: Tensor, wu: Tensor, wd: Tensor) -> None:
              f"x is {x.dtype}, the weights {wg.dtype}, {wu.dtype} and {wd.dtype}: one dtype (or autocast) is needed")
     _require(x.device == wg.device == wu.device == wd.device, "x and the weights must be on one device")
     _dtype_code(x)
-    _require(False, "the weights must have rows and columns")
+    _require(wg.numel() > 0 and wd.numel() > 0, "the weights must have rows and columns")
+    _require(False, f"{x.shape[0]} tokens or weights {tuple(wg.shape)} and {tuple(wd.shape)} too large (2^26 tokens, sizes of 2^20)")
 
 
 def _gated_args(x: Tensor, wg: Tensor, wu: Tensor, wd: Tensor, act: int):
@@ -179,7 +181,7 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     bfloat16: the products' operands act(g) u and its gradients are rounded to
     bfloat16 once (for up to 64 tokens to 16 bits, for up to 32 without gradients
     not below 16 bits), what is kept to 11 bits relative to the largest of 16 neighbours, and
-    the results once."""
+    the results once. Infinities in a token's inputs make its results infinite or NaN."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
         _require(False, f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
@@ -214,8 +216,9 @@ def _embed_args(ids: Tensor, w: Tensor, rows: int, scale: float, padding: int):
 
 def _check_embed(ids: Tensor, w: Tensor, pos: Optional[Tensor]) -> None:
     if (w.is_cuda and ids.dim() == 2 and w.dim() == 2 and ids.dtype in _IDS and w.dtype in _TYPES and ids.device == w.device
-            and w.numel() and (pos is None or (pos.dim() == 2 and pos.shape[0] >= ids.shape[1] and pos.shape[1] == w.shape[1]
-                                               and pos.dtype == w.dtype and pos.device == w.device))):
+            and w.numel() and ids.numel() <= 1 << 30 and w.shape[0] <= 1 << 24 and w.shape[1] <= 1 << 20
+            and (pos is None or (pos.dim() == 2 and ids.shape[1] <= pos.shape[0] < 1 << 31 and pos.shape[1] == w.shape[1]
+                                 and pos.dtype == w.dtype and pos.device == w.device))):
         return
     _require(w.is_cuda, "token_embedding needs CUDA tensors")
     _require(ids.dtype in _IDS, f"ids must be int64 or int32, got {ids.dtype}")
@@ -226,6 +229,9 @@ def _check_embed(ids: Tensor, w: Tensor, pos: Optional[Tensor]) -> None:
         _require(pos.dim() == 2 and pos.shape[0] >= ids.shape[1] and pos.shape[1] == w.shape[1],
                  f"positions {tuple(pos.shape)} must be [at least {ids.shape[1]}, {w.shape[1]}]")
         _require(pos.dtype == w.dtype, f"weight is {w.dtype} and positions {pos.dtype}: one dtype is needed")
+        _require(pos.shape[0] < 1 << 31, f"{pos.shape[0]} positions: too many")
+    _require(ids.numel() <= 1 << 30 and w.shape[0] <= 1 << 24 and w.shape[1] <= 1 << 20,
+             f"{ids.numel()} ids or weight {tuple(w.shape)} too large (2^30 ids, 2^24 words of 2^20)")
     _require(False, "ids, weight and positions must be on one device")
 
 

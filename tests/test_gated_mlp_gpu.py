@@ -15,7 +15,7 @@ import itertools
 import pytest
 import torch
 
-from llattn_b200 import gated_mlp
+from llattn_b200 import gated_mlp, lm_ops, token_embedding
 
 pytestmark = pytest.mark.gpu
 
@@ -287,6 +287,30 @@ def test_graphs_streams_hooks_and_compile():
         dx.sum().backward()
 
 
+@pytest.mark.parametrize("d", [256, 261])
+@pytest.mark.parametrize("n", [1, 8, 30])
+def test_behind_a_kernel_that_is_still_writing(n, d):
+    """Each of the library's launches may start before the one that writes its input is done."""
+    _, wg, wu, wd, _ = tensors(1, d, 640, d, torch.bfloat16)
+    w = torch.randn(4096, d, device="cuda").bfloat16()
+    ids = torch.randint(0, 4096, (64, n), device="cuda")
+    with torch.no_grad():
+        rows = [token_embedding(i, w) for i in ids]
+        want = []
+        for x in rows:
+            torch.cuda.synchronize()
+            want.append(gated_mlp(x, wg, wu, wd))
+        torch.cuda.synchronize()
+        # x's memory is the same in every step: what an SM has left of the step before is wrong
+        got = [gated_mlp(token_embedding(i, w), wg, wu, wd) for i in ids]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            replayed = [gated_mlp(token_embedding(i, w), wg, wu, wd) for i in ids]
+        for _ in range(3):
+            graph.replay()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, replayed))
+
+
 def test_refusals():
     x, wg, wu, wd, _ = tensors(4, 64, 96, 40, torch.bfloat16)
     for args, kw, msg in (((x, wg, wu, wd), dict(activation="relu"), "activation"), ((x[:, :32], wg, wu, wd), {}, "columns"),
@@ -294,6 +318,11 @@ def test_refusals():
                           ((x.float(), wg, wu, wd), {}, "one dtype"), ((x, wg, wu.float(), wd), {}, "one dtype"),
                           ((x.half(), wg.half(), wu.half(), wd.half()), {}, "dtype"),
                           ((x.cpu(), wg.cpu(), wu.cpu(), wd.cpu()), {}, "CUDA"), ((x, wg, wu, wd.cpu()), {}, "one device"),
-                          ((x, wg[:0], wu[:0], wd[:, :0]), {}, "rows and columns"), ((x, wg, wu, wd[0]), {}, "w_down")):
+                          ((x, wg[:0], wu[:0], wd[:, :0]), {}, "rows and columns"), ((x, wg, wu, wd[0]), {}, "w_down"),
+                          # (sizes that 32 bits would take for small ones; the rows are one row)
+                          ((x[:1].expand(2**32 + 4, 64), wg, wu, wd), {}, "too large"),
+                          ((x, wg, wu, wd[:1].expand(2**32 + 4, 96)), {}, "too large")):
         with pytest.raises(RuntimeError, match=msg):
             gated_mlp(*args, **kw)
+    with pytest.raises(RuntimeError, match=r"status 1\): gated: unknown activation 7"):
+        lm_ops._native.gated(x, wg, wu, wd, 7)  # the library's own refusal, through the native path

@@ -150,6 +150,9 @@ def test_one_gradient_only_and_same_bits():
         assert all(torch.equal(a, b) for a, b in zip(full, again))
     leaf = w.detach().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(token_embedding(ids, leaf, positions=pos), leaf, dout)[0], full[1])
+    both = (leaf, pos.detach().requires_grad_(True))  # of two that have one, one at a time
+    for k in range(2):
+        assert torch.equal(torch.autograd.grad(token_embedding(ids, both[0], positions=both[1]), both[k], dout)[0], full[1 + k])
     leaf = pos.detach().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(token_embedding(ids, w, positions=leaf), leaf, dout)[0], full[2])
 
@@ -199,6 +202,8 @@ def test_refusals():
                           ((ids[0, 0], w), dict(positions=pos), "dimension"), ((ids, w), dict(padding_idx=20), "padding_idx"),
                           ((ids, w), dict(padding_idx=-21), "padding_idx"), ((ids.cpu(), w), {}, "one device"),
                           ((ids.cpu(), w.cpu()), {}, "CUDA"), ((ids, w), dict(positions=pos.cpu()), "one device"),
-                          ((ids, w[:0]), {}, "rows and columns")):
+                          ((ids, w[:0]), {}, "rows and columns"), ((ids[:1].expand(2**32 + 1, 8), w), {}, "too large"),
+                          ((ids, w[:1].expand(2**32 + 4, 16)), {}, "too large"),
+                          ((ids, w), dict(positions=pos[:1].expand(2**32 + 8, 16)), "too many")):
         with pytest.raises(RuntimeError, match=msg):
             token_embedding(*args, **kw)
