@@ -647,7 +647,7 @@ size_t kept_bytes(const llattn_gated_args& a) {
   return (size_t)cdiv(a.tokens, 32) * cdiv(a.ff, kBlock) * (a.dtype == LLATTN_F32 ? 4096 : 2048 + 64);
 }
 
-static bool few(const llattn_gated_args& a, bool backward) { return !backward && !a.kept && a.tokens <= few_tokens(a.dtype); }
+static bool few(const llattn_gated_args& a, bool backward) { return !backward && !a.kept && a.tokens <= few_tokens(a); }
 
 size_t workspace_bytes(const llattn_gated_args& a, bool backward) {
   if (few(a, backward)) return up256(few_workspace_bytes(a));

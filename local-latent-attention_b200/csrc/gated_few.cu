@@ -4,21 +4,28 @@
 //
 // A CTA owns 16 rows of a weight matrix (of both, in the first launch) and a range of K; its 8
 // warps take 64 bytes each of every 512 of a row. A lane reads 16 bytes of row lane / 4 and of the row
-// 8 further straight to registers, several steps ahead: in bf16 they are, in an order of K that
-// x is read in as well, its part of two m16n8k16 fragments (mma.sync: 8 tokens fill its columns, the
-// loads bound the kernel, not the products), and its 16 bytes of token lane / 4 the other operand. No
-// operand is read twice by a CTA, so none goes through shared memory: no barrier before the
-// sums. Rows off a 16-byte boundary are read as the two chunks that hold them and shifted. Rings of
-// asynchronous copies in shared memory with one CTA per SM were slower (1 token: 27 us for 17): what a
-// launch this short waits for is its first loads, its barriers and its last sums, and those pass beside
+// 8 further straight to registers, several steps ahead, across row blocks where a CTA has several: in
+// bf16 they are, in an order of K that x is read in as well, its part of two m16n8k16 fragments (mma.sync:
+// 8 tokens fill its columns, the loads bound the kernel, not the products), and its 16 bytes of token
+// lane / 4 the other operand. No operand is read twice by a CTA, so none goes through shared memory: no
+// barrier before the sums. Rows off a 16-byte boundary are read as the two chunks that hold them and shifted.
+// Rings of asynchronous copies in shared memory with one CTA per SM were slower (1 token: 27 us for 17): what
+// a launch this short waits for is its first loads, its barriers and its last sums, and those pass beside
 // another CTA's loads only where an SM holds several.
 //
 // The ranges of K of a row block are a cluster: their sums meet in the shared memory of its
 // first CTA, which adds them in order. The second launch reads its weights before the first one is
 // done (these do not depend on it: the first launch lets it start only after everything before is
-// complete), and only then waits for h; the first one asks the L2 for its weights before it waits.
+// complete), and only then waits for h; the first one asks the L2 for its weights before it waits. (Asking for
+// the second one's too won nothing: 15.4 us for 15.2.)
 //
 // bf16: h is stored in two bf16 parts and multiplied in both. fp32: products on the SIMT cores, 8 tokens at a time.
+//
+// Measured (us, by CUDA graph over weights that come from memory; floor = the weights at 6.55 TB/s; 33: mm_kernel's
+// way): 1536 x 4096 (5.8): 14.0 for 1 token, 17.2 for 16, 21.5 for 24, 24.5 for 33; 2048 x 8192 (15.4): 26.8, 4096 x
+// 14336 (53.8): 84; 1411 x 3749 (4.8): 20.7, 24 tokens 30, 33: 38; fp32 1536 x 4096 (11.5): 26, 8 tokens 40. The
+// large ones are bound by how evenly the row blocks fill the SMs and by the pauses between CTAs, the small ones by two
+// launches of some 4 us.
 #include <algorithm>
 
 #include "gated.cuh"
@@ -44,15 +51,19 @@ struct FewArgs {
   int act, ranges, per;  // ranges of K, columns of one
 };
 
-// C: tokens that fp32 products are made for (bf16: 8)
+// C: tokens of a CTA
 template <typename T, int C, int NW, bool SHIFT>
 struct FewShape {
   static constexpr bool F32 = sizeof(T) == 4;
-  static constexpr int VALUES = NW * 128;                                // sums of a CTA: 16 rows of 8 tokens
+  static constexpr int NT = F32 ? 1 : C / 8;                             // token groups: columns of a fragment
+  static constexpr int VALUES = NW * NT * 128;                           // sums of a CTA: 16 rows of 8 tokens each
   static constexpr int LANE = 16 / sizeof(T), STEP = 4 * LANE * kWarps;  // columns of 16 bytes, of the CTA's step
   // steps of loads under way: what 128 registers hold (two CTAs to an SM), less where more were slower (bf16, 1
   // token of 1536 x 4096: 15.1 us with 3 and 4 steps, 16.0 with 4 and 6, 16.8 with 2 and 4 and three CTAs)
-  static constexpr int AHEAD = F32 ? (SHIFT || C > 4 ? 2 : NW == 2 ? 4 : 6) : SHIFT ? (NW == 2 ? 2 : 3) : NW == 2 ? 3 : 4;
+  static constexpr int AHEAD = F32       ? (SHIFT || C > 4 ? 2 : NW == 2 ? 4 : 6)
+                               : NT > 1  ? (SHIFT && NW == 2 ? 1 : 2)
+                               : SHIFT   ? (NW == 2 ? 2 : 3)
+                                         : (NW == 2 ? 3 : 4);
 };
 
 // Columns [k, k + 16 bytes) of a row as the aligned chunks that hold them (the second one where the row is off).
@@ -139,64 +150,90 @@ __device__ __forceinline__ float gate(float g, int act) {
   return 0.5f * g * erfcf(g * -0.70710678f);
 }
 
-// SHIFT: rows (of x too) may be off a 16-byte boundary
-template <typename T, int C, int NW, bool SHIFT>
+// SHIFT: rows (of x too) may be off a 16-byte boundary. WHOLE: a row block takes whole turns of the load
+// buffers, the steps past its columns on zeros, so that no branch stands between loads and products and
+// another row block's loads follow; otherwise a CTA has one row block, whose steps stop where it ends.
+template <typename T, int C, int NW, bool SHIFT, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant__ FewArgs p) {
   using S = FewShape<T, C, NW, SHIFT>;
   constexpr bool F32 = S::F32;
   constexpr int PLANES = !F32 && NW == 1 ? 2 : 1;
-  __shared__ float red[kWarps * S::VALUES];
-  extern __shared__ float slots[];  // [ranges][VALUES]
+  constexpr int NT = S::NT, XN = F32 ? 1 : NT * PLANES;
+  constexpr bool XSHIFT = SHIFT && NW == 2;
+  extern __shared__ float few_smem[];  // [2][kWarps][VALUES], [ranges][VALUES]
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
-  const int rank = (int)blockIdx.x % p.ranges, row0 = (int)blockIdx.x / p.ranges * 16;
+  const int rank = (int)blockIdx.x % p.ranges, first = (int)blockIdx.x / p.ranges, stride = (int)gridDim.x / p.ranges;
+  const int blocks = cdiv(p.rows, 16);
   const int tok0 = blockIdx.y * C, tokens = min(C, p.tokens - tok0);
-  const int kb = rank * p.per, ke = min(p.K, kb + p.per), steps = kb < ke ? cdiv(ke - kb, S::STEP) : 0;
-  const int kl = kb + (warp * 4 + t) * S::LANE;  // this lane's first column
+  const int kb = rank * p.per, ke = min(p.K, kb + p.per);
+  constexpr int TURN = WHOLE ? S::AHEAD : 1;
+  const int steps = kb < ke ? cdiv(ke - kb, S::STEP * TURN) * TURN : 0;
+  const int kl = kb + (warp * 4 + t) * S::LANE;                                   // this lane's first column
   if (p.ranges > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  const T* row[NW][2];
   uintptr_t lo[NW], hi[NW];
-  int off[NW][2];
-  bool ok[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) ok[h] = row0 + g + 8 * h < p.rows;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     const T* base = static_cast<const T*>(p.w[w]);
     lo[w] = reinterpret_cast<uintptr_t>(base);
     hi[w] = reinterpret_cast<uintptr_t>(base + (p.rows - 1) * p.ldw[w] + p.K);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      row[w][h] = base + (int64_t)(ok[h] ? row0 + g + 8 * h : 0) * p.ldw[w];
-      off[w][h] = SHIFT ? (int)(reinterpret_cast<uintptr_t>(row[w][h] + kl) & 15) : 0;
-    }
   }
-  // x's row of this lane (bf16): the second launch's has two planes of aligned rows
-  const T* xr = static_cast<const T*>(p.x) + (tok0 + (g < tokens ? g : 0)) * p.ldx;
-  const bool x_ok = g < tokens;
-  constexpr bool XSHIFT = SHIFT && NW == 2;
+  // row h of a block of a matrix, and whether it is there
+  auto row_of = [&](int block, int w, int h) {
+    const int r = block * 16 + g + 8 * h;
+    return static_cast<const T*>(p.w[w]) + (int64_t)(r < p.rows ? r : 0) * p.ldw[w];
+  };
+  // x's rows of this lane (bf16): the second launch's has two planes of aligned rows
+  const T* xr[NT];
+  int xoff[NT];
   const uintptr_t xlo = reinterpret_cast<uintptr_t>(p.x),
                   xhi = reinterpret_cast<uintptr_t>(static_cast<const T*>(p.x) + (p.tokens - 1) * p.ldx + p.K);
-  const int xoff = XSHIFT ? (int)(reinterpret_cast<uintptr_t>(xr + kl) & 15) : 0;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    xr[i] = static_cast<const T*>(p.x) + (tok0 + (8 * i + g < tokens ? 8 * i + g : 0)) * p.ldx;
+    xoff[i] = XSHIFT ? (int)(reinterpret_cast<uintptr_t>(xr[i] + kl) & 15) : 0;
+  }
 
-  Raw buf[S::AHEAD][NW][2], xbuf[S::AHEAD][F32 ? 1 : PLANES];
-  auto issue = [&](int j, Raw (&b)[NW][2]) {
-    const int k = kl + j * S::STEP;
+  // loads run AHEAD steps before the products, into the next row block where this one's are done
+  Raw buf[S::AHEAD][NW][2], xbuf[S::AHEAD][XN];
+  const T* row[NW][2];
+  int next = first, nj = 0, xj = 0;
+  auto set_rows = [&]() {
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) raw_load<T, SHIFT, true>(b[w][h], row[w][h], k, ke, ok[h], lo[w], hi[w]);
+      for (int h = 0; h < 2; ++h) row[w][h] = row_of(next, w, h);
   };
-  auto issue_x = [&](int j, Raw (&b)[F32 ? 1 : PLANES]) {
-    if constexpr (!F32) {
-      const int k = kl + j * S::STEP;
-      if constexpr (NW == 2) {
-        raw_load<T, XSHIFT, false>(b[0], xr, k, ke, x_ok, xlo, xhi);
-      } else {
+  set_rows();
+  auto issue = [&](Raw (&b)[NW][2]) {
+    const int k = kl + nj * S::STEP;
 #pragma unroll
-        for (int pl = 0; pl < PLANES; ++pl)
-          b[pl].c[0] = x_ok && k < ke ? *reinterpret_cast<const uint4*>(xr + pl * p.tokens * p.ldx + k) : make_uint4(0, 0, 0, 0);
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        raw_load<T, SHIFT, true>(b[w][h], row[w][h], k, ke, next * 16 + g + 8 * h < p.rows, lo[w], hi[w]);
+    if (++nj == steps && WHOLE) {
+      nj = 0;
+      next += stride;
+      set_rows();
+    }
+  };
+  auto issue_x = [&](Raw (&b)[XN]) {
+    if constexpr (!F32) {
+      const int k = kl + xj * S::STEP;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const bool x_ok = 8 * i + g < tokens;
+        if constexpr (NW == 2) {
+          raw_load<T, XSHIFT, false>(b[i], xr[i], k, ke, x_ok, xlo, xhi);
+        } else {
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl)
+            b[i * PLANES + pl].c[0] =
+                x_ok && k < ke ? *reinterpret_cast<const uint4*>(xr[i] + pl * p.tokens * p.ldx + k) : make_uint4(0, 0, 0, 0);
+        }
       }
+      if (++xj == steps && WHOLE) xj = 0;
     }
   };
   if (NW == 2) {
@@ -206,29 +243,27 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
       for (int w = 0; w < NW; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (ok[h] && kl + j * S::STEP < ke) asm volatile("prefetch.global.L2 [%0];" ::"l"(row[w][h] + kl + j * S::STEP));
+          if (first * 16 + g + 8 * h < p.rows && kl + j * S::STEP < ke)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(row[w][h] + kl + j * S::STEP));
     pdl_wait();
     pdl_next();  // not before: the second launch's loads rest on it
   }
 #pragma unroll
   for (int u = 0; u < S::AHEAD; ++u) {
-    issue(u, buf[u]);
-    if (NW == 2) issue_x(u, xbuf[u]);
+    issue(buf[u]);
+    if (NW == 2) issue_x(xbuf[u]);
   }
   if (NW == 1) {
     pdl_wait();
     pdl_next();
 #pragma unroll
-    for (int u = 0; u < S::AHEAD; ++u) issue_x(u, xbuf[u]);
+    for (int u = 0; u < S::AHEAD; ++u) issue_x(xbuf[u]);
   }
 
-  constexpr int ACC = F32 ? 2 * C : 4;  // fp32: [row half][token]; else the fragments
+  constexpr int ACC = F32 ? 2 * C : 4 * NT;  // fp32: [row half][token]; else the fragments
   float acc[NW][ACC];
-#pragma unroll
-  for (int w = 0; w < NW; ++w)
-#pragma unroll
-    for (int i = 0; i < ACC; ++i) acc[w][i] = 0.f;
-  auto compute = [&](const Raw (&b)[NW][2], const Raw (&xb)[F32 ? 1 : PLANES], int k) {
+  int off[NW][2];
+  auto compute = [&](const Raw (&b)[NW][2], const Raw (&xb)[XN], int k) {
     uint32_t a[NW][2][4];
 #pragma unroll
     for (int w = 0; w < NW; ++w)
@@ -269,12 +304,12 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
       }
     } else {
 #pragma unroll
-      for (int pl = 0; pl < PLANES; ++pl) {
+      for (int i = 0; i < XN; ++i) {
         uint32_t x[4];
-        words<T, XSHIFT>(xb[pl], xoff, ke - k, x);
+        words<T, XSHIFT>(xb[i], xoff[i / PLANES], ke - k, x);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          float(&c)[4] = *reinterpret_cast<float(*)[4]>(&acc[w][0]);
+          float(&c)[4] = *reinterpret_cast<float(*)[4]>(&acc[w][i / PLANES * 4]);
           mma16816(c, a[w], 0, x[0], x[1]);
           mma16816(c, a[w], 1, x[2], x[3]);
         }
@@ -282,89 +317,107 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
     }
   };
 #pragma unroll 1
-  for (int j0 = 0; j0 < steps; j0 += S::AHEAD) {
-#pragma unroll
-    for (int u = 0; u < S::AHEAD; ++u) {
-      const int j = j0 + u;
-      if (j < steps) {
-        compute(buf[u], xbuf[u], kl + j * S::STEP);
-        issue(j + S::AHEAD, buf[u]);
-        issue_x(j + S::AHEAD, xbuf[u]);
-      }
-    }
-  }
-
-  // sums of the warps, then of the ranges; a value's place: product, fragment register, lane
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if constexpr (F32) {
-#pragma unroll
-      for (int i = 0; i < ACC; ++i) {
-        acc[w][i] += __shfl_xor_sync(0xffffffffu, acc[w][i], 1);
-        acc[w][i] += __shfl_xor_sync(0xffffffffu, acc[w][i], 2);
-      }
-    }
-    for (int r = 0; r < 4; ++r) {
-      float v;
-      if constexpr (F32) {
-        v = 0.f;  // (of no token)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (2 * q + (r & 1) < C) v = t == q ? acc[w][(r >> 1) * C + 2 * q + (r & 1)] : v;
-      } else {
-        v = acc[w][r];
-      }
-      red[warp * S::VALUES + (w * 4 + r) * 32 + lane] = v;
-    }
-  }
-  __syncthreads();
-  if (p.ranges > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA is there
-  for (int i = tid; i < S::VALUES; i += kThreads) {
-    float s = red[i];
-#pragma unroll
-    for (int k = 1; k < kWarps; ++k) s += red[k * S::VALUES + i];
-    float* dst = slots + rank * S::VALUES + i;
-    if (p.ranges > 1)
-      asm volatile(
-          "{\n\t.reg .b32 ra;\n\t"
-          "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
-          "st.shared::cluster.f32 [ra], %1;\n\t}" ::"r"(smem_u32(dst)),
-          "f"(s)
-          : "memory");
-    else
-      *dst = s;
-  }
-  if (p.ranges > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank) return;
-  } else {
-    __syncthreads();
-  }
-  for (int i = tid; i < 128; i += kThreads) {
-    float v[NW];
+  for (int block = first, turn = 0; block < blocks; block += stride, turn ^= 1) {
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      v[w] = slots[w * 128 + i];
-      for (int k = 1; k < p.ranges; ++k) v[w] += slots[k * S::VALUES + w * 128 + i];
+#pragma unroll
+      for (int i = 0; i < ACC; ++i) acc[w][i] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) off[w][h] = SHIFT ? (int)(reinterpret_cast<uintptr_t>(row_of(block, w, h) + kl) & 15) : 0;
     }
-    const int l = i % 32, r = i / 32, tok = 2 * (l % 4) + (r & 1), f = row0 + l / 4 + 8 * (r >> 1);
-    if (tok >= tokens || f >= p.rows) continue;
-    const int64_t at = (tok0 + tok) * p.ldo + f;
-    if constexpr (NW == 2) {
-      const float h = gate(v[0], p.act) * v[1];
-      if constexpr (F32) {
-        static_cast<float*>(p.out)[at] = h;
-      } else {
-        const bf16 hi16 = __float2bfloat16_rn(h);
-        static_cast<bf16*>(p.out)[at] = hi16;
-        static_cast<bf16*>(p.out)[p.tokens * p.ldo + at] = __float2bfloat16_rn(h - __bfloat162float(hi16));
+#pragma unroll 1
+    for (int j0 = 0; j0 < steps; j0 += S::AHEAD) {
+#pragma unroll
+      for (int u = 0; u < S::AHEAD; ++u) {
+        if (WHOLE || j0 + u < steps) {
+          compute(buf[u], xbuf[u], kl + (j0 + u) * S::STEP);
+          issue(buf[u]);
+          issue_x(xbuf[u]);
+        }
       }
-    } else {
-      static_cast<T*>(p.out)[at] = from_f<T>(v[0]);
+    }
+
+    // sums of the warps, then of the ranges; a value's place: product, fragment register, lane
+    float* red = few_smem + turn * kWarps * S::VALUES;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < ACC; ++i) {
+          acc[w][i] += __shfl_xor_sync(0xffffffffu, acc[w][i], 1);
+          acc[w][i] += __shfl_xor_sync(0xffffffffu, acc[w][i], 2);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4 * NT; ++r) {
+        float v;
+        if constexpr (F32) {
+          v = 0.f;  // (of no token)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (2 * q + (r & 1) < C) v = t == q ? acc[w][(r >> 1) * C + 2 * q + (r & 1)] : v;
+        } else {
+          v = acc[w][r];
+        }
+        red[warp * S::VALUES + (w * NT * 4 + r) * 32 + lane] = v;
+      }
+    }
+    __syncthreads();
+    const float* sums = red;
+    int n_sums = kWarps;
+    if (p.ranges > 1) {  // (one row block to a cluster)
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA is there
+      float* slots = few_smem + 2 * kWarps * S::VALUES;
+      for (int i = tid; i < S::VALUES; i += kThreads) {
+        float s = red[i];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) s += red[k * S::VALUES + i];
+        asm volatile(
+            "{\n\t.reg .b32 ra;\n\t"
+            "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
+            "st.shared::cluster.f32 [ra], %1;\n\t}" ::"r"(smem_u32(slots + rank * S::VALUES + i)),
+            "f"(s)
+            : "memory");
+      }
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (rank) return;
+      sums = slots;
+      n_sums = p.ranges;
+    }
+    for (int i = tid; i < 128 * NT; i += kThreads) {
+      float v[NW];
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        v[w] = sums[w * NT * 128 + i];
+#pragma unroll 8
+        for (int k = 1; k < n_sums; ++k) v[w] += sums[k * S::VALUES + w * NT * 128 + i];
+      }
+      const int l = i % 32, r = i / 32 % 4, tok = i / 128 * 8 + 2 * (l % 4) + (r & 1), f = block * 16 + l / 4 + 8 * (r >> 1);
+      if (tok >= tokens || f >= p.rows) continue;
+      const int64_t at = (tok0 + tok) * p.ldo + f;
+      if constexpr (NW == 2) {
+        const float h = gate(v[0], p.act) * v[1];
+        if constexpr (F32) {
+          static_cast<float*>(p.out)[at] = h;
+        } else {
+          const bf16 hi16 = __float2bfloat16_rn(h);
+          static_cast<bf16*>(p.out)[at] = hi16;
+          static_cast<bf16*>(p.out)[p.tokens * p.ldo + at] = __float2bfloat16_rn(h - __bfloat162float(hi16));
+        }
+      } else {
+        static_cast<T*>(p.out)[at] = from_f<T>(v[0]);
+      }
     }
   }
 }
 
+template <typename T, int C, int NW, bool SHIFT, bool WHOLE>
+cudaError_t launch(const FewArgs& p, int grid, cudaStream_t s) {
+  const int smem = (2 * kWarps + p.ranges) * FewShape<T, C, NW, SHIFT>::VALUES * 4;
+  const cudaError_t e = set_smem_once(few_kernel<T, C, NW, SHIFT, WHOLE>, smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(few_kernel<T, C, NW, SHIFT, WHOLE>, dim3(grid, cdiv(p.tokens, C)), kThreads, smem, p.ranges, s, p);
+}
 template <typename T, int C, int NW, bool SHIFT>
 cudaError_t launch(FewArgs p, cudaStream_t s) {
   using S = FewShape<T, C, NW, SHIFT>;
@@ -373,10 +426,11 @@ cudaError_t launch(FewArgs p, cudaStream_t s) {
   p.ranges = 1;
   while (p.ranges < 8 && p.ranges * tiles < sm_count() && p.K >= 4 * p.ranges * S::STEP) p.ranges *= 2;
   p.per = cdiv(cdiv(p.K, p.ranges), S::STEP) * S::STEP;
-  const int smem = p.ranges * S::VALUES * 4;
-  const cudaError_t e = set_smem_once(few_kernel<T, C, NW, SHIFT>, smem);
-  if (e != cudaSuccess) return e;
-  return launch_pdl(few_kernel<T, C, NW, SHIFT>, dim3(tiles * p.ranges, cdiv(p.tokens, C)), kThreads, smem, p.ranges, s, p);
+  const int grid = p.ranges > 1 ? tiles * p.ranges : std::min(tiles, 2 * sm_count());
+  // whole turns (1 token of 2048 x 8192: 26.8 us for 29.8, of 1536 x 4096: 14.0 for 14.6), but not where a single
+  // row block would pay for empty steps (1024 x 2816: 11.8 us for 9.8) or shifted rows spill (1411 x 3749: 22.1 for 20.7)
+  const bool whole = grid < tiles || (!SHIFT && p.per / S::STEP % S::AHEAD == 0);
+  return whole ? launch<T, C, NW, SHIFT, true>(p, grid, s) : launch<T, C, NW, SHIFT, false>(p, grid, s);
 }
 
 template <typename T, int NW>
@@ -384,11 +438,18 @@ cudaError_t launch_as(const FewArgs& p, bool shift, cudaStream_t s) {
   if constexpr (sizeof(T) == 4) {
     if (p.tokens == 1) return shift ? launch<T, 1, NW, true>(p, s) : launch<T, 1, NW, false>(p, s);
     if (p.tokens <= 4) return shift ? launch<T, 4, NW, true>(p, s) : launch<T, 4, NW, false>(p, s);
+  } else {
+    if (p.tokens > 16) return shift ? launch<T, 24, NW, true>(p, s) : launch<T, 24, NW, false>(p, s);
+    if (p.tokens > 8) return shift ? launch<T, 16, NW, true>(p, s) : launch<T, 16, NW, false>(p, s);
   }
   return shift ? launch<T, 8, NW, true>(p, s) : launch<T, 8, NW, false>(p, s);
 }
 
 bool whole(const void* p, int64_t ld, int64_t rows, int elt) { return ((uintptr_t)p & 15) == 0 && (rows == 1 || ld * elt % 16 == 0); }
+bool all_whole(const llattn_gated_args& a) {
+  const int elt = a.dtype == LLATTN_F32 ? 4 : 2;
+  return whole(a.w_gate, a.ldg, a.ff, elt) && whole(a.w_up, a.ldu, a.ff, elt) && whole(a.x, a.ldx, a.tokens, elt);
+}
 int64_t padded(int ff) { return (ff + 7) / 8 * 8; }
 
 template <typename T>
@@ -407,8 +468,7 @@ cudaError_t run(const llattn_gated_args& a, cudaStream_t s) {
   p.ldo = padded(a.ff);
   p.act = a.activation;
   constexpr int elt = sizeof(T);
-  const bool all = whole(a.w_gate, a.ldg, a.ff, elt) && whole(a.w_up, a.ldu, a.ff, elt) && whole(a.x, a.ldx, a.tokens, elt);
-  const cudaError_t e = launch_as<T, 2>(p, !all, s);
+  const cudaError_t e = launch_as<T, 2>(p, !all_whole(a), s);
   if (e != cudaSuccess) return e;
   FewArgs q = {};
   q.x = a.workspace;
@@ -425,7 +485,14 @@ cudaError_t run(const llattn_gated_args& a, cudaStream_t s) {
 
 }  // namespace
 
-int few_tokens(int dtype) { return dtype == LLATTN_F32 ? 16 : 8; }
+// As many tokens as this form is faster for. bf16: beyond 8 it reads x more often than the weights' rows come
+// in, and only small weights, for which mm_kernel's launches are long, make up for that (16 and 24 tokens: 1536 x
+// 4096 17.3 and 21.6 us for 25, 2048 x 8192 32.6 and 40.5 for 33). fp32: 8 at a time, each reading the
+// weights again (16 tokens of 1536 x 4096 71 us for 100, of 1411 x 3749, whose rows are shifted, 106 for 97).
+int few_tokens(const llattn_gated_args& a) {
+  if (a.dtype == LLATTN_F32) return all_whole(a) && whole(a.w_down, a.ldd, a.d_out, 4) ? 16 : 8;
+  return (2 * (int64_t)a.d + a.d_out) * a.ff <= 1 << 25 ? 24 : 8;
+}
 size_t few_workspace_bytes(const llattn_gated_args& a) { return 4 * (size_t)a.tokens * padded(a.ff); }
 cudaError_t launch_few(const llattn_gated_args& a, cudaStream_t s) {
   return a.dtype == LLATTN_F32 ? run<float>(a, s) : run<bf16>(a, s);
