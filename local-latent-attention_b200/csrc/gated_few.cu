@@ -8,8 +8,10 @@
 // bf16 they are, in an order of K that x is read in as well, its part of two m16n8k16 fragments (mma.sync:
 // 8 tokens fill its columns, the loads bound the kernel, not the products), and its 16 bytes of token
 // lane / 4 the other operand. No operand is read twice by a CTA, so none goes through shared memory: no
-// barrier before the sums. Rows off a 16-byte boundary are read as the two chunks that hold them and shifted.
-// Rings of asynchronous copies in shared memory with one CTA per SM were slower (1 token: 27 us for 17): what
+// barrier before the sums. Rows off a 16-byte boundary: bf16 reads the two chunks that hold the 16 bytes and shifts
+// them. fp32 takes rows 4 apart, which are all off it by as much, reads whole chunks that begin before
+// the rows, and shifts x, by elements (1 token of 1411 x 3749: 37 -> 21 us; in bf16 x is in fragments, and
+// two chunks of it for one of the weights cost more than they save: 24 tokens 37 us for 30). Rings of asynchronous copies in shared memory with one CTA per SM were slower (1 token: 27 us for 17): what
 // a launch this short waits for is its first loads, its barriers and its last sums, and those pass beside
 // another CTA's loads only where an SM holds several.
 //
@@ -60,10 +62,11 @@ struct FewShape {
   static constexpr int LANE = 16 / sizeof(T), STEP = 4 * LANE * kWarps;  // columns of 16 bytes, of the CTA's step
   // steps of loads under way: what 128 registers hold (two CTAs to an SM), less where more were slower (bf16, 1
   // token of 1536 x 4096: 15.1 us with 3 and 4 steps, 16.0 with 4 and 6, 16.8 with 2 and 4 and three CTAs)
-  static constexpr int AHEAD = F32       ? (SHIFT || C > 4 ? 2 : NW == 2 ? 4 : 6)
+  static constexpr int AHEAD = F32       ? (C > 4 ? 2 : SHIFT ? 3 : NW == 2 ? 4 : 6)
                                : NT > 1  ? (SHIFT && NW == 2 ? 1 : 2)
                                : SHIFT   ? (NW == 2 ? 2 : 3)
                                          : (NW == 2 ? 3 : 4);
+  static constexpr int GAP = SHIFT && F32 ? LANE : 1;  // rows between those of a CTA
 };
 
 // Columns [k, k + 16 bytes) of a row as the aligned chunks that hold them (the second one where the row is off).
@@ -77,13 +80,14 @@ __device__ __forceinline__ uint4 load16(uintptr_t q) {
   const uint4* p = reinterpret_cast<const uint4*>(q);
   return W ? __ldg(p) : *p;
 }
-template <typename T, bool SHIFT, bool W>
+// GAP: k may lie before the row, by less than a chunk.
+template <typename T, bool SHIFT, bool W, bool GAP>
 __device__ __forceinline__ void raw_load(Raw& r, const T* row, int k, int K, bool ok, uintptr_t lo, uintptr_t hi) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(row + k), q = SHIFT ? a & ~uintptr_t(15) : a;
   const uintptr_t b = a + min(16, (K - k) * (int)sizeof(T));  // the end of what is there
   ok = ok && k < K;
   const uint4 z = make_uint4(0, 0, 0, 0);
-  const bool first = ok && (!SHIFT || q >= lo) && q + 16 <= hi, second = SHIFT && ok && q + 16 < b && q + 32 <= hi;
+  const bool first = ok && (!(SHIFT || GAP) || q >= lo) && q + 16 <= hi, second = SHIFT && ok && q + 16 < b && q + 32 <= hi;
   r.c[0] = first ? load16<W>(q) : z;
   if (SHIFT) r.c[1] = second ? load16<W>(q + 16) : z;
   // the matrix's first and last bytes, where a chunk reaches past them
@@ -96,7 +100,7 @@ __device__ __forceinline__ void raw_load(Raw& r, const T* row, int k, int K, boo
 #pragma unroll
       for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
         const uintptr_t e = q + 16 * c + i * sizeof(T);
-        if (e < a || e >= b) continue;
+        if (e < (GAP ? lo : a) || e >= b) continue;
         if constexpr (sizeof(T) == 2)
           v[i / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(e) << (i % 2 * 16);
         else
@@ -106,10 +110,10 @@ __device__ __forceinline__ void raw_load(Raw& r, const T* row, int k, int K, boo
     }
   }
 }
-// The four words of it, `off` bytes into the chunks, zeros past the n columns that are there.
+// The four words of it, `off` bytes into the chunks, zeros outside the columns [head, n) that are there.
 template <typename T, bool SHIFT>
-__device__ __forceinline__ void words(const Raw& r, int off, int n, uint32_t (&w)[4]) {
-  if (SHIFT) {
+__device__ __forceinline__ void words(const Raw& r, int off, int head, int n, uint32_t (&w)[4]) {
+  if constexpr (SHIFT) {
     uint32_t v[8] = {r.c[0].x, r.c[0].y, r.c[0].z, r.c[0].w, r.c[1].x, r.c[1].y, r.c[1].z, r.c[1].w};
     if (off & 8) {
 #pragma unroll
@@ -127,11 +131,11 @@ __device__ __forceinline__ void words(const Raw& r, int off, int n, uint32_t (&w
     w[2] = r.c[0].z;
     w[3] = r.c[0].w;
   }
-  if (n < 16 / (int)sizeof(T)) {
+  if (n < 16 / (int)sizeof(T) || (sizeof(T) == 4 && head > 0)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 4)
-        w[i] = i < n ? w[i] : 0u;
+        w[i] = i >= head && i < n ? w[i] : 0u;
       else
         w[i] = 2 * i + 1 < n ? w[i] : 2 * i < n ? w[i] & 0xffffu : 0u;
     }
@@ -157,18 +161,20 @@ template <typename T, int C, int NW, bool SHIFT, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant__ FewArgs p) {
   using S = FewShape<T, C, NW, SHIFT>;
   constexpr bool F32 = S::F32;
-  constexpr int PLANES = !F32 && NW == 1 ? 2 : 1;
+  constexpr int PLANES = !F32 && NW == 1 ? 2 : 1, GAP = S::GAP;
+  constexpr bool OFF = SHIFT && GAP == 1;  // rows each off by their own
   constexpr int NT = S::NT, XN = F32 ? 1 : NT * PLANES;
-  constexpr bool XSHIFT = SHIFT && NW == 2;
+  constexpr bool XSHIFT = OFF && NW == 2;
   extern __shared__ float few_smem[];  // [2][kWarps][VALUES], [ranges][VALUES]
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int rank = (int)blockIdx.x % p.ranges, first = (int)blockIdx.x / p.ranges, stride = (int)gridDim.x / p.ranges;
-  const int blocks = cdiv(p.rows, 16);
+  const int blocks = cdiv(p.rows, 16 * GAP) * GAP;
   const int tok0 = blockIdx.y * C, tokens = min(C, p.tokens - tok0);
-  const int kb = rank * p.per, ke = min(p.K, kb + p.per);
+  // columns of a row, with GAP from the chunk on that its first one lies in, the o-th of it: [o, K + o)
+  const int kb = rank * p.per, most = min(p.K + GAP - 1, kb + p.per);
   constexpr int TURN = WHOLE ? S::AHEAD : 1;
-  const int steps = kb < ke ? cdiv(ke - kb, S::STEP * TURN) * TURN : 0;
-  const int kl = kb + (warp * 4 + t) * S::LANE;                                   // this lane's first column
+  const int steps = kb < most ? cdiv(most - kb, S::STEP * TURN) * TURN : 0;
+  const int kl = kb + (warp * 4 + t) * S::LANE;  // this lane's first column
   if (p.ranges > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   uintptr_t lo[NW], hi[NW];
@@ -178,9 +184,11 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
     lo[w] = reinterpret_cast<uintptr_t>(base);
     hi[w] = reinterpret_cast<uintptr_t>(base + (p.rows - 1) * p.ldw[w] + p.K);
   }
-  // row h of a block of a matrix, and whether it is there
-  auto row_of = [&](int block, int w, int h) {
-    const int r = block * 16 + g + 8 * h;
+  auto row_of = [&](int block, int i) { return block / GAP * (16 * GAP) + block % GAP + GAP * i; };  // the i-th of 16
+  auto o_of = [&](int block) { return GAP > 1 ? (int)((lo[0] / sizeof(T) + row_of(block, 0) * p.ldw[0]) % S::LANE) : 0; };
+  auto end_of = [&](int o) { return min(p.K + o, kb + p.per); };
+  auto start_of = [&](int block, int w, int h) {  // of this lane's rows
+    const int r = row_of(block, g + 8 * h);
     return static_cast<const T*>(p.w[w]) + (int64_t)(r < p.rows ? r : 0) * p.ldw[w];
   };
   // x's rows of this lane (bf16): the second launch's has two planes of aligned rows
@@ -197,12 +205,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
   // loads run AHEAD steps before the products, into the next row block where this one's are done
   Raw buf[S::AHEAD][NW][2], xbuf[S::AHEAD][XN];
   const T* row[NW][2];
-  int next = first, nj = 0, xj = 0;
+  int next = first, nj = 0, xj = 0, no = 0;
   auto set_rows = [&]() {
+    no = o_of(next);
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) row[w][h] = row_of(next, w, h);
+      for (int h = 0; h < 2; ++h) row[w][h] = start_of(next, w, h);
   };
   set_rows();
   auto issue = [&](Raw (&b)[NW][2]) {
@@ -211,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
     for (int w = 0; w < NW; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        raw_load<T, SHIFT, true>(b[w][h], row[w][h], k, ke, next * 16 + g + 8 * h < p.rows, lo[w], hi[w]);
+        raw_load<T, OFF, true, (GAP > 1)>(b[w][h], row[w][h], k - no, end_of(no) - no, row_of(next, g + 8 * h) < p.rows, lo[w], hi[w]);
     if (++nj == steps && WHOLE) {
       nj = 0;
       next += stride;
@@ -225,12 +234,12 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
       for (int i = 0; i < NT; ++i) {
         const bool x_ok = 8 * i + g < tokens;
         if constexpr (NW == 2) {
-          raw_load<T, XSHIFT, false>(b[i], xr[i], k, ke, x_ok, xlo, xhi);
+          raw_load<T, XSHIFT, false, false>(b[i], xr[i], k, end_of(0), x_ok, xlo, xhi);
         } else {
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl)
             b[i * PLANES + pl].c[0] =
-                x_ok && k < ke ? *reinterpret_cast<const uint4*>(xr[i] + pl * p.tokens * p.ldx + k) : make_uint4(0, 0, 0, 0);
+                x_ok && k < end_of(0) ? *reinterpret_cast<const uint4*>(xr[i] + pl * p.tokens * p.ldx + k) : make_uint4(0, 0, 0, 0);
         }
       }
       if (++xj == steps && WHOLE) xj = 0;
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
       for (int w = 0; w < NW; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (first * 16 + g + 8 * h < p.rows && kl + j * S::STEP < ke)
+          if (row_of(first, g + 8 * h) < p.rows && kl + j * S::STEP < p.K)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(row[w][h] + kl + j * S::STEP));
     pdl_wait();
     pdl_next();  // not before: the second launch's loads rest on it
@@ -262,13 +271,14 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
 
   constexpr int ACC = F32 ? 2 * C : 4 * NT;  // fp32: [row half][token]; else the fragments
   float acc[NW][ACC];
-  int off[NW][2];
+  int off[NW][2], o = 0, ke = 0;  // of this row block
   auto compute = [&](const Raw (&b)[NW][2], const Raw (&xb)[XN], int k) {
+    const int head = GAP > 1 ? o - k : 0;
     uint32_t a[NW][2][4];
 #pragma unroll
     for (int w = 0; w < NW; ++w)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) words<T, SHIFT>(b[w][h], off[w][h], ke - k, a[w][h]);
+      for (int h = 0; h < 2; ++h) words<T, OFF>(b[w][h], off[w][h], head, ke - k, a[w][h]);
     if constexpr (F32) {
 #pragma unroll
       for (int i0 = 0; i0 < C; i0 += 4) {  // loads of up to 4 tokens together
@@ -276,13 +286,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
         float xv[G][4];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-          const float* src = static_cast<const float*>(p.x) + (int64_t)(tok0 + min(i0 + i, tokens - 1)) * p.ldx + k;
+          const float* src = static_cast<const float*>(p.x) + (int64_t)(tok0 + min(i0 + i, tokens - 1)) * p.ldx + (k - o);
           if (!SHIFT) {  // (a row's last columns are masked in the weights; what lies behind them may not be there)
             const float4 v = k + 4 <= ke ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
             xv[i][0] = v.x; xv[i][1] = v.y; xv[i][2] = v.z; xv[i][3] = v.w;
           } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) xv[i][q] = k + q < ke ? src[q] : 0.f;
+            for (int q = 0; q < 4; ++q) xv[i][q] = q >= head && k + q < ke ? src[q] : 0.f;
           }
         }
         if (!SHIFT && k < ke && k + 4 > ke) {
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < XN; ++i) {
         uint32_t x[4];
-        words<T, XSHIFT>(xb[i], xoff[i / PLANES], ke - k, x);
+        words<T, XSHIFT>(xb[i], xoff[i / PLANES], 0, ke - k, x);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
           float(&c)[4] = *reinterpret_cast<float(*)[4]>(&acc[w][i / PLANES * 4]);
@@ -318,12 +328,14 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
   };
 #pragma unroll 1
   for (int block = first, turn = 0; block < blocks; block += stride, turn ^= 1) {
+    o = o_of(block);
+    ke = end_of(o);
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
 #pragma unroll
       for (int i = 0; i < ACC; ++i) acc[w][i] = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) off[w][h] = SHIFT ? (int)(reinterpret_cast<uintptr_t>(row_of(block, w, h) + kl) & 15) : 0;
+      for (int h = 0; h < 2; ++h) off[w][h] = OFF ? (int)(reinterpret_cast<uintptr_t>(start_of(block, w, h) + kl) & 15) : 0;
     }
 #pragma unroll 1
     for (int j0 = 0; j0 < steps; j0 += S::AHEAD) {
@@ -392,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
 #pragma unroll 8
         for (int k = 1; k < n_sums; ++k) v[w] += sums[k * S::VALUES + w * NT * 128 + i];
       }
-      const int l = i % 32, r = i / 32 % 4, tok = i / 128 * 8 + 2 * (l % 4) + (r & 1), f = block * 16 + l / 4 + 8 * (r >> 1);
+      const int l = i % 32, r = i / 32 % 4, tok = i / 128 * 8 + 2 * (l % 4) + (r & 1), f = row_of(block, l / 4 + 8 * (r >> 1));
       if (tok >= tokens || f >= p.rows) continue;
       const int64_t at = (tok0 + tok) * p.ldo + f;
       if constexpr (NW == 2) {
@@ -422,14 +434,14 @@ template <typename T, int C, int NW, bool SHIFT>
 cudaError_t launch(FewArgs p, cudaStream_t s) {
   using S = FewShape<T, C, NW, SHIFT>;
   // ranges of K while the CTAs do not fill the SMs once, each of at least two steps
-  const int tiles = cdiv(p.rows, 16);
+  const int tiles = cdiv(p.rows, 16 * S::GAP) * S::GAP, K = p.K + S::GAP - 1;
   p.ranges = 1;
-  while (p.ranges < 8 && p.ranges * tiles < sm_count() && p.K >= 4 * p.ranges * S::STEP) p.ranges *= 2;
-  p.per = cdiv(cdiv(p.K, p.ranges), S::STEP) * S::STEP;
+  while (p.ranges < 8 && p.ranges * tiles < sm_count() && K >= 4 * p.ranges * S::STEP) p.ranges *= 2;
+  p.per = cdiv(cdiv(K, p.ranges), S::STEP) * S::STEP;
   const int grid = p.ranges > 1 ? tiles * p.ranges : std::min(tiles, 2 * sm_count());
   // whole turns (1 token of 2048 x 8192: 26.8 us for 29.8, of 1536 x 4096: 14.0 for 14.6), but not where a single
   // row block would pay for empty steps (1024 x 2816: 11.8 us for 9.8) or shifted rows spill (1411 x 3749: 22.1 for 20.7)
-  const bool whole = grid < tiles || (!SHIFT && p.per / S::STEP % S::AHEAD == 0);
+  const bool whole = grid < tiles || ((!SHIFT || S::F32) && p.per / S::STEP % S::AHEAD == 0);
   return whole ? launch<T, C, NW, SHIFT, true>(p, grid, s) : launch<T, C, NW, SHIFT, false>(p, grid, s);
 }
 
@@ -488,9 +500,13 @@ cudaError_t run(const llattn_gated_args& a, cudaStream_t s) {
 // As many tokens as this form is faster for. bf16: beyond 8 it reads x more often than the weights' rows come
 // in, and only small weights, for which mm_kernel's launches are long, make up for that (16 and 24 tokens: 1536 x
 // 4096 17.3 and 21.6 us for 25, 2048 x 8192 32.6 and 40.5 for 33). fp32: 8 at a time, each reading the
-// weights again (16 tokens of 1536 x 4096 71 us for 100, of 1411 x 3749, whose rows are shifted, 106 for 97).
+// weights again (16 tokens of 1536 x 4096 71 us for 100); where w_gate's and w_up's rows are off a 16-byte boundary
+// by different shifts it has none, as a CTA's rows have to be off by the same.
 int few_tokens(const llattn_gated_args& a) {
-  if (a.dtype == LLATTN_F32) return all_whole(a) && whole(a.w_down, a.ldd, a.d_out, 4) ? 16 : 8;
+  if (a.dtype == LLATTN_F32) {
+    const bool alike = (((uintptr_t)a.w_gate ^ (uintptr_t)a.w_up) & 15) == 0 && (a.ldg - a.ldu) % 4 == 0;
+    return alike || all_whole(a) ? 16 : 0;
+  }
   return (2 * (int64_t)a.d + a.d_out) * a.ff <= 1 << 25 ? 24 : 8;
 }
 size_t few_workspace_bytes(const llattn_gated_args& a) { return 4 * (size_t)a.tokens * padded(a.ff); }

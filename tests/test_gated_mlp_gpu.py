@@ -140,6 +140,12 @@ def test_strided_and_unaligned_rows(n, dt):
         with torch.no_grad():
             ins = [inside(t, p, s) for t, p, s in zip((x, wg, wu, wd), pads, shifts)]
             check({"y": gated_mlp(*ins)}, want, f"pads {pads} no grad")
+    # gate and up in one matrix, the rows of one off a 16-byte boundary by another shift than the other's
+    for rows in (ff, ff - 1, 1):
+        both = torch.cat([wg[:rows, :71], wu[:rows, :71]])
+        ins = (x[:, :71], both[:rows], both[rows:], wd[:, :rows])
+        with torch.no_grad():
+            check({"y": gated_mlp(*ins)}, formula(*ins, dy, "silu"), f"{rows} rows of both in one")
     # columns that are not contiguous are copied; one weight in two places; broadcast upstream gradients
     got = run(x.t().contiguous().t(), wg.t().contiguous().t(), wu, wd, dy, "silu")
     check(got, want, "transposed")
