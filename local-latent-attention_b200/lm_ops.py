@@ -179,8 +179,7 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
 
     Precision: sums are fp32. float32 inputs keep 24 bits in every product.
     bfloat16: the products' operands act(g) u and its gradients are rounded to
-    bfloat16 once (for up to 64 tokens to 16 bits, for up to 32 without gradients
-    not below 16 bits), what is kept to 11 bits relative to the largest of 16 neighbours, and
+    bfloat16 once (for up to 64 tokens to 16 bits), what is kept to 11 bits relative to the largest of 16 neighbours, and
     the results once. Infinities in a token's inputs make its results infinite or NaN."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
