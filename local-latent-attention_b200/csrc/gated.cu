@@ -541,7 +541,8 @@ EpiOut rows_out(const Plan& q, void* out, int cols) {
 }
 
 // The tiles of the two products with the activation in their epilogues: shape 5
-// instead of 2, and for g and u at least 32 columns of each to a warp (shape 0 holds 16).
+// instead of 2 for bf16 (fp32's values spill in 96 registers: steps of 2048 x 1024 x 2816 774 us for 710, of 8192 x
+// 1536 x 4096 5600 for 5250), and for g and u at least 32 columns of each to a warp (shape 0 holds 16).
 template <typename Epi>
 cudaError_t launch_active(MmArgs p, const Operand& a, const Operand& b, const Epi& e, cudaStream_t s,
                           const Operand* b2 = nullptr) {
@@ -553,7 +554,8 @@ cudaError_t launch_active(MmArgs p, const Operand& a, const Operand& b, const Ep
     if (t0 <= t4 && t0 < std::min(t1, t2)) return launch_mm_sh<0>(p, a, b, e, s, b2);
   }
   if (t4 < std::min(t1, t2)) return launch_mm_sh<4>(p, a, b, e, s, b2);
-  return t2 <= t1 ? launch_mm_sh<5>(p, a, b, e, s, b2) : launch_mm_sh<1>(p, a, b, e, s, b2);
+  if (t2 <= t1) return launch_mm_sh<Epi::F32 ? 2 : 5>(p, a, b, e, s, b2);
+  return launch_mm_sh<1>(p, a, b, e, s, b2);
 }
 
 template <typename T, int ACT, int P>
