@@ -116,35 +116,31 @@ __device__ __forceinline__ void load16(uint32_t taddr, bool zero, float (&v)[16]
 #pragma unroll
   for (int q = 0; q < 16; ++q) v[q] = zero ? 0.f : __uint_as_float(r[q]);
 }
-// 8 of this thread's row's columns in P bf16 planes, 16 bytes a store, or all 16 of a block in one
-// plane, 32 bytes a store: a whole sector, so that nothing is gained by bringing rows together in
-// shared memory first (bulk stores of 64-byte rows from there: 145 and 122 us for 142 and 105 at the same
-// point, 8192 x 1536 x 4096).
-template <int P>
-__device__ __forceinline__ void store8(const float* v_, bf16* p, int64_t plane) {
-  float v[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = v_[q];
-#pragma unroll
-  for (int k = 0; k < P; ++k) {
-    uint32_t w[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
-      v[2 * q] -= __uint_as_float(w[q] << 16);
-      v[2 * q + 1] -= __uint_as_float(w[q] & 0xffff0000u);
-    }
-    *reinterpret_cast<uint4*>(p + k * plane) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+// A block's 16 columns of this thread's row in P bf16 planes, 32 bytes a store: a whole sector, so that nothing is
+// gained by bringing rows together in shared memory first (bulk stores of 64-byte rows from there: 145 and 122 us for
+// 142 and 105 at the same point, 8192 x 1536 x 4096).
+__device__ __forceinline__ void store16(const uint32_t (&w)[8], bf16* p) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 __device__ __forceinline__ void pack8(const float* v, uint32_t* w) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
 }
-__device__ __forceinline__ void store16(const uint32_t (&w)[8], bf16* p) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
+template <int P>
+__device__ __forceinline__ void store_planes(float (&v)[16], bf16* p, int64_t plane) {
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    uint32_t w[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      w[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
+      v[2 * q] -= __uint_as_float(w[q] << 16);
+      v[2 * q + 1] -= __uint_as_float(w[q] & 0xffff0000u);
+    }
+    store16(w, p + k * plane);
+  }
 }
 
 // ---- g, u -> h ------------------------------------------------------------------
@@ -212,15 +208,7 @@ struct EpiGated {
         g[q] = a * u[q];
       }
       bf16* dst = h + row * ld + col;
-      if constexpr (P == 1) {
-        uint32_t w[8];
-        pack8(g, w);
-        pack8(g + 8, w + 4);
-        if (row < M) store16(w, dst);
-      } else if (row < M) {
-        store8<P>(g, dst, plane);
-        store8<P>(g + 8, dst + 8, plane);
-      }
+      if (row < M) store_planes<P>(g, dst, plane);
     }
   }
 };
@@ -288,6 +276,7 @@ struct EpiGrad {
       if (col >= a.N) break;  // warp-uniform
       bf16 *hd = h + row * ld + col, *gd = dgu + 2 * P * (row * ld) + col;
       uint32_t wh[8], wg[8], wu[8];  // (P = 1)
+      float vh[16], vg[16], vu[16];  // (otherwise)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float g[8], u[8], dh[8];
@@ -306,20 +295,27 @@ struct EpiGrad {
           pack8(g, wh + 4 * e);
           pack8(u, wg + 4 * e);
           pack8(dh, wu + 4 * e);
-        } else if (row < M) {
-          if (h) store8<P>(g, hd + 8 * e, plane);
-          if (dgu) {
-            store8<P>(u, gd + 8 * e, 2 * ld);
-            store8<P>(dh, gd + ld + 8 * e, 2 * ld);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            vh[8 * e + q] = g[q];
+            vg[8 * e + q] = u[q];
+            vu[8 * e + q] = dh[q];
           }
         }
       }
+      if (row >= M) continue;
       if constexpr (P == 1) {
-        if (row >= M) continue;
         if (h) store16(wh, hd);
         if (dgu) {
           store16(wg, gd);
           store16(wu, gd + ld);
+        }
+      } else {
+        if (h) store_planes<P>(vh, hd, plane);
+        if (dgu) {
+          store_planes<P>(vg, gd, 2 * ld);
+          store_planes<P>(vu, gd + ld, 2 * ld);
         }
       }
     }
