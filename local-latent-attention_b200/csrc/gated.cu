@@ -23,8 +23,8 @@
 // Bound by the tensor cores, and by the epilogues with the activation where a tile's products are short:
 // 32768 tokens of 1536 x 4096, bf16: g and u's product 589 us (824 GF: 1.40 PFLOP/s), y 264 + 12 us of joining split
 // tiles (412 GF), dh's 393, dx 514 + 16, dWd 295 + 16, [dWg; dWu] 487 + 18; the training step 3.0 to 3.15 ms, under the
-// power cap. 4095 tokens of 1408 x 3749: 73, 44 + 9, 63, 72 + 8, 51 + 9, 77 + 8. fp32, 1000 of 512 x 1365: 36, 21 + 7,
-// 43, 29 + 11, 23 + 7, 27 + 9 and 9 + 8 of packing.
+// power cap. 4095 tokens of 1408 x 3749: 73, 44 + 9, 63, 72 + 8, 51 + 9, 77 + 8. fp32, 1000 of 512 x 1365: 31, 20 + 6,
+// 37, 28 + 9, 21 + 6, 26 + 7 and 7 + 7 of packing.
 //
 // Few tokens without gradients take gated_few.cu's kernel instead (few_tokens).
 #include <math.h>
@@ -538,7 +538,7 @@ EpiOut rows_out(const Plan& q, void* out, int cols) {
 
 // The tiles of the two products with the activation in their epilogues: shape 5
 // instead of 2 for bf16 (fp32's values spill in 96 registers: steps of 2048 x 1024 x 2816 774 us for 710, of 8192 x
-// 1536 x 4096 5600 for 5250), and for g and u at least 32 columns of each to a warp (shape 0 holds 16).
+// 1536 x 4096 5600 for 5250; 620 and 4650 since with stores of whole sectors), and for g and u at least 32 columns of each to a warp (shape 0 holds 16).
 template <typename Epi>
 cudaError_t launch_active(MmArgs p, const Operand& a, const Operand& b, const Epi& e, cudaStream_t s,
                           const Operand* b2 = nullptr) {
