@@ -194,6 +194,28 @@ def test_graphs_streams_and_compile():
     assert all(torch.equal(a, b) for a, b in zip(got, eager))
 
 
+def test_graph_kept_freed_and_hooked():
+    ids, w, pos, dout = make(3, 40, 24, 30, FP)
+    leaves = (w.requires_grad_(True), pos.requires_grad_(True))
+    out = token_embedding(ids, leaves[0], positions=leaves[1])
+    first = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    again = torch.autograd.grad(out, leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, leaves, dout)
+    with torch.autograd.graph.save_on_cpu():
+        out = token_embedding(ids, leaves[0], positions=leaves[1])
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(out, leaves, dout)))
+    out = token_embedding(ids, leaves[0], positions=leaves[1])
+    (dw,) = torch.autograd.grad(out, leaves[0], dout.requires_grad_(True), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dw.sum().backward()
+    out = token_embedding(ids, leaves[0])
+    ids[0, 0] += 1  # (what the backward reads)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
 def test_refusals():
     ids, w, pos, _ = make(3, 8, 16, 20, BF)
     for args, kw, msg in (((ids.float(), w), {}, "int64"), ((ids.bool(), w), {}, "int64"), ((ids, w[0]), {}, "weight"),
