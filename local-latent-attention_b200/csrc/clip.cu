@@ -250,37 +250,40 @@ int chunks_of(const llattn_clip_args& a, int i) {
   return (int)(((int64_t)((uintptr_t)a.tensors[i] & 15) + bytes + kChunk - 1) / kChunk);
 }
 
-// The next batch of tensors from *i on: at most CAP that hold something.
+// One batch of the list: take(tensor, its first chunk, chunks) for those from i on that hold something, up to
+// `most`. Returns where the next batch starts: behind the empty tensors that follow, so that every batch but an
+// empty list's holds something, and all that walk the list count the same ones.
+template <typename Take>
+int batch(const llattn_clip_args& a, int i, int most, Take take) {
+  for (int n = 0, chunks = 0; i < a.count; ++i) {
+    if (!a.sizes[i]) continue;
+    const int c = chunks_of(a, i);
+    if (n == most || (n && chunks > (1 << 30) - c)) break;
+    take(i, chunks, c);
+    ++n;
+    chunks += c;
+  }
+  return i;
+}
 template <int CAP>
 void fill(const llattn_clip_args& a, int* i, Table<CAP>* t) {
   t->n = t->chunks = 0;
-  for (; *i < a.count && t->n < CAP; ++*i) {
-    if (!a.sizes[*i]) continue;
-    const int chunks = chunks_of(a, *i);
-    if (t->n && t->chunks > (1 << 30) - chunks) break;
-    const int bf = a.dtypes[*i] == LLATTN_BF16;
-    t->e[t->n++] = {static_cast<char*>(a.tensors[*i]), a.sizes[*i] * (bf ? 2 : 4), t->chunks, bf};
-    t->chunks += chunks;
-  }
+  *i = batch(a, *i, CAP, [&](int k, int chunk, int chunks) {
+    const int bf = a.dtypes[k] == LLATTN_BF16;
+    t->e[t->n++] = {static_cast<char*>(a.tensors[k]), a.sizes[k] * (bf ? 2 : 4), chunk, bf};
+    t->chunks = chunk + chunks;
+  });
 }
 template <int CAP>
 int grid_of(const Table<CAP>& t) { return std::max(1, std::min(t.chunks, std::min(kMaxGrid, 8 * sm_count()))); }
 
-int batches(const llattn_clip_args& a) {
-  int n = 0, full = 0;
-  int64_t chunks = 0;
-  for (int i = 0; i < a.count; ++i) {
-    if (!a.sizes[i]) continue;
-    const int c = chunks_of(a, i);
-    if (full == kTensors || (full && chunks > (1 << 30) - c)) {
-      ++n;
-      full = 0;
-      chunks = 0;
-    }
-    ++full;
-    chunks += c;
-  }
-  return n + 1;
+int batches(const llattn_clip_args& a) {  // (the same with the short table, which holds all of a list that takes it)
+  int n = 0, i = 0;
+  do {
+    i = batch(a, i, kTensors, [](int, int, int) {});
+    ++n;
+  } while (i < a.count);
+  return n;
 }
 
 template <typename Op, int CAP>

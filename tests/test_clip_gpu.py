@@ -223,3 +223,37 @@ def test_refusals():
     s.grad = torch.eye(4, device="cuda").to_sparse()
     with pytest.raises(RuntimeError, match="dense"):
         clip_grad_norm_([s], 1.0)
+
+
+def through_c(tensors, norm_type=0, max_norm=1.0, scale=1):
+    """llattn_clip with a workspace of exactly the size that it asks for, between guard bytes; returns the norm."""
+    import ctypes
+
+    from llattn_b200 import _lib
+
+    n = len(tensors)
+    args = _lib.ClipArgs(n, norm_type, scale, (ctypes.c_void_p * n)(*(t.data_ptr() for t in tensors)),
+                         (ctypes.c_int64 * n)(*(t.numel() for t in tensors)),
+                         (ctypes.c_int32 * n)(*(_lib.BF16 if t.dtype == BF else _lib.F32 for t in tensors)), max_norm)
+    norm = torch.empty((), device="cuda")
+    size = _lib.lib().llattn_clip_workspace_bytes(ctypes.byref(args))
+    buf = torch.full((512 + size + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    args.norm, args.workspace, args.workspace_bytes = norm.data_ptr(), buf.data_ptr() + 512, size
+    _lib.check(_lib.lib().llattn_clip(ctypes.byref(args), torch.cuda.current_stream().cuda_stream), "llattn_clip")
+    assert (buf[:512] == 0xA5).all() and (buf[512 + size:] == 0xA5).all()
+    return norm.item()
+
+
+@pytest.mark.parametrize("before,after", ((0, 0), (0, 1), (3, 1500)))
+@pytest.mark.parametrize("count", (0, 1, 96, 1299, 1300, 1301, 2600))
+def test_empty_tensors_and_the_workspaces_size(count, before, after):
+    """Empty tensors behind a full launch's make no further one: its sum would lie behind the workspace."""
+    none = torch.empty(0, device="cuda")
+    held = [p.grad for p in params([(1 + i % 37,) for i in range(count)], (FP, BF), seed=count)]
+    want = norm64(held).item() if held else 0.0
+    lists = [none] * before + held + [none] * after
+    if lists:
+        assert abs(through_c(lists, scale=0) - want) <= NORM * want
+        assert abs(through_c(lists, max_norm=0.5) - want) <= NORM * want
+    if held:  # clipped once (bf16: half a step an element)
+        assert abs(norm64(held).item() / min(want, 0.5) - 1) <= 2.0 ** -8

@@ -134,6 +134,16 @@ def test_clip_refusals(lists, kw, msg):
     refused(_lib.lib().llattn_clip(ctypes.byref(clip_args(*lists, **kw)), None), msg)
 
 
+def test_clip_workspace_counts_what_holds_something():
+    size = lambda lens: _lib.lib().llattn_clip_workspace_bytes(
+        ctypes.byref(clip_args([4096 * (i + 1) for i in range(len(lens))], lens, [_lib.F32] * len(lens))))
+    one = size([])
+    assert one > 0 and size([0] * 5000) == one
+    for n, launches in ((1, 1), (96, 1), (97, 1), (1299, 1), (1300, 1), (1301, 2), (2600, 2), (2601, 3), (3900, 3)):
+        for before, after in ((0, 0), (0, 1), (7, 2000), (1300, 1300)):
+            assert size([0] * before + [5] * n + [0] * after) == launches * one, (n, before, after)
+
+
 def test_lm_ops_on_the_cpu_are_refused():
     with pytest.raises(RuntimeError, match="CUDA"):
         llattn_b200.token_embedding(torch.zeros(2, 3, dtype=torch.long), torch.randn(4, 8))
