@@ -75,23 +75,30 @@ struct FewShape {
 struct Raw {
   uint4 c[2];
 };
-// [lo, hi): the matrix's bytes. W: a weight, by the read-only path; otherwise what the kernel before
-// may have written while this one was already there, which the read-only path does not allow for.
-template <bool W>
+// kConst: by the read-only path, for what was complete before this kernel started: w_down, in the second launch. x
+// and the first launch's weights may come from the kernel ahead, which that path does not allow for. kOnce: past the
+// L1, where the weights leave x its place.
+enum Load { kPlain, kConst, kOnce };
+template <Load L>
 __device__ __forceinline__ uint4 load16(uintptr_t q) {
   const uint4* p = reinterpret_cast<const uint4*>(q);
-  return W ? __ldg(p) : *p;
+  if (L == kConst) return __ldg(p);
+  if (L == kPlain) return *p;
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
+// [lo, hi): the matrix's bytes.
 // GAP: k may lie before the row, by less than a chunk.
-template <typename T, bool SHIFT, bool W, bool GAP>
+template <typename T, bool SHIFT, Load L, bool GAP>
 __device__ __forceinline__ void raw_load(Raw& r, const T* row, int k, int K, bool ok, uintptr_t lo, uintptr_t hi) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(row + k), q = SHIFT ? a & ~uintptr_t(15) : a;
   const uintptr_t b = a + min(16, (K - k) * (int)sizeof(T));  // the end of what is there
   ok = ok && k < K;
   const uint4 z = make_uint4(0, 0, 0, 0);
   const bool first = ok && (!(SHIFT || GAP) || q >= lo) && q + 16 <= hi, second = SHIFT && ok && q + 16 < b && q + 32 <= hi;
-  r.c[0] = first ? load16<W>(q) : z;
-  if (SHIFT) r.c[1] = second ? load16<W>(q + 16) : z;
+  r.c[0] = first ? load16<L>(q) : z;
+  if (SHIFT) r.c[1] = second ? load16<L>(q + 16) : z;
   // the matrix's first and last bytes, where a chunk reaches past them
   const bool edge0 = ok && !first, edge1 = SHIFT && ok && !second && q + 16 < b;
   if (edge0 || edge1) {
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
     for (int w = 0; w < NW; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        raw_load<T, OFF, true, (GAP > 1)>(b[w][h], row[w][h], k - no, end_of(no) - no, row_of(next, g + 8 * h) < p.rows, lo[w], hi[w]);
+        raw_load<T, OFF, NW == 1 ? kConst : kOnce, (GAP > 1)>(b[w][h], row[w][h], k - no, end_of(no) - no, row_of(next, g + 8 * h) < p.rows, lo[w], hi[w]);
     if (++nj == steps && WHOLE) {
       nj = 0;
       next += stride;
@@ -236,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant_
       for (int i = 0; i < NT; ++i) {
         const bool x_ok = 8 * i + g < tokens;
         if constexpr (NW == 2) {
-          raw_load<T, XSHIFT, false, false>(b[i], xr[i], k, end_of(0), x_ok, xlo, xhi);
+          raw_load<T, XSHIFT, kPlain, false>(b[i], xr[i], k, end_of(0), x_ok, xlo, xhi);
         } else {
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl)

@@ -332,3 +332,35 @@ def test_refusals():
             gated_mlp(*args, **kw)
     with pytest.raises(RuntimeError, match=r"status 1\): gated: unknown activation 7"):
         lm_ops._native.gated(x, wg, wu, wd, 7)  # the library's own refusal, through the native path
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=("bf16", "f32"))
+@pytest.mark.parametrize("which", ["w_gate", "w_up", "w_down"])
+@pytest.mark.parametrize("n", [1, 8, 16, 30])
+def test_weights_behind_a_kernel_that_is_still_writing(n, which, dt):
+    """A weight that the library's launch just ahead writes, to the same memory in every step."""
+    d = ff = 520
+    x, *weights, _ = tensors(n, d, ff, d, dt, seed=n)
+    at = ("w_gate", "w_up", "w_down").index(which)
+    table = (torch.randn(2048, d, device="cuda") / d ** 0.5).to(dt)
+    ids = torch.randint(0, 2048, (40, ff), device="cuda")
+
+    def step(i):
+        own = list(weights)
+        own[at] = token_embedding(i, table)
+        return gated_mlp(x, *own)
+
+    with torch.no_grad():
+        want = []
+        for i in ids:
+            weights[at] = token_embedding(i, table)
+            torch.cuda.synchronize()
+            want.append(gated_mlp(x, *weights))
+            torch.cuda.synchronize()
+        got = [step(i) for i in ids]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            replayed = [step(i) for i in ids]
+        for _ in range(3):
+            graph.replay()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, replayed))
