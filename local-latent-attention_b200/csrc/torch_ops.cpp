@@ -36,8 +36,9 @@ constexpr int64_t kMostTokens = 1 << 26, kMostIds = 1 << 30, kMostWords = 1 << 2
 constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize});
 
+// (without a tangent: nothing here carries forward-mode derivatives on)
 bool plain(const Tensor& t) {
-  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(kWrapped);
+  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(kWrapped) && !t._fw_grad(0).defined();
 }
 int dtype_of(const Tensor& t) {
   return t.scalar_type() == at::kFloat ? LLATTN_F32 : t.scalar_type() == at::kBFloat16 ? LLATTN_BF16 : -1;
@@ -60,6 +61,10 @@ struct Once : torch::autograd::Function<Once> {
     TORCH_CHECK(false, "llattn: trying to differentiate twice an operator whose gradients are not differentiable");
   }
 };
+// (calls with dual inputs have gone to lm_ops.py, which refuses them; here it is the upstream gradient that may be one)
+void no_tangent(const Tensor& g, const char* what) {
+  TORCH_CHECK(!g._fw_grad(0).defined(), "llattn: ", what, "'s backward has no forward-mode derivatives (the upstream gradient is a dual tensor)");
+}
 variable_list once(variable_list grads, const variable_list& from) {
   if (!at::GradMode::is_enabled()) return grads;
   const auto leaf = std::find_if(from.begin(), from.end(), [](const Tensor& t) { return t.defined() && t.requires_grad(); });
@@ -119,6 +124,7 @@ struct Gated : torch::autograd::Function<Gated> {
     const variable_list saved = ctx->get_saved_variables();
     variable_list out(5);
     if (!grads[0].defined()) return out;
+    no_tangent(grads[0], "gated_mlp");
     {
       at::NoGradGuard no_grad;
       const c10::cuda::CUDAGuard guard(saved[0].device());
@@ -225,6 +231,7 @@ struct EmbedBackward : torch::autograd::Node {
     variable_list out(2);
     const bool need_w = task_should_compute_output(0), need_p = position_rows && task_should_compute_output(1);
     if (!grads[0].defined() || !(need_w || need_p)) return out;
+    no_tangent(grads[0], "token_embedding");
     {
       at::NoGradGuard no_grad;
       const c10::cuda::CUDAGuard guard(grads[0].device());

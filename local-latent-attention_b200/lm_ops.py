@@ -22,7 +22,7 @@ from torch import Tensor
 
 from . import _lib
 from .ops import _DT, _dtype_code, _require
-from .training_ops import _direct, _on, _rows, _stream
+from .training_ops import _direct, _no_tangents, _on, _rows, _stream
 
 try:
     from . import _torch_ops as _native
@@ -156,6 +156,7 @@ class _GatedMlp(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_tangents("gated_mlp's backward", dy)
         x, wg, wu, wd, kept = ctx.saved_tensors
         need = ctx.needs_input_grad[:4]
         f = _gated_bwd if _direct(x, wg, wu, wd, dy) else gated_mlp_grads_op
@@ -165,7 +166,8 @@ class _GatedMlp(torch.autograd.Function):
 
 def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activation: str = "silu") -> Tensor:
     """Gated feed-forward block: ``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T``,
-    differentiable in all four (gradients of gradients are not supported).
+    differentiable in all four (gradients of gradients and forward-mode derivatives
+    are not supported).
 
     x [..., d], w_gate and w_up [ff, d], w_down [d_out, ff], all bfloat16 or all
     float32 (under autocast all are cast to its dtype, as a linear layer's inputs
@@ -190,6 +192,7 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     y = native.gated(x, w_gate, w_up, w_down, act) if native else None
     if y is not None:
         return y
+    _no_tangents("gated_mlp", x, w_gate, w_up, w_down)
     if x.dim() < 1 or w_gate.dim() != 2 or x.shape[-1] != w_gate.shape[1]:
         _require(False, f"x {tuple(x.shape)} must end in w_gate's columns {tuple(w_gate.shape)}")
     flat = x.dim() == 2
@@ -299,6 +302,7 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _no_tangents("token_embedding's backward", dout)
         (ids,) = ctx.saved_tensors
         _, need_w, need_p = ctx.needs_input_grad[:3]
         f = _embed_bwd if _direct(ids, dout) else token_embedding_grads_op
@@ -310,7 +314,7 @@ def token_embedding(ids: Tensor, weight: Tensor, *, positions: Optional[Tensor] 
                     padding_idx: Optional[int] = None) -> Tensor:
     """Rows of an embedding: ``scale * weight[ids]``, plus ``positions[t]`` for the t-th
     id along ids' last dimension; differentiable in weight and positions
-    (gradients of gradients are not supported).
+    (gradients of gradients and forward-mode derivatives are not supported).
 
     ids [...] int64 or int32, weight [vocab, d] bfloat16 or float32, positions
     [at least ids.shape[-1], d] in weight's dtype; any row strides. Returns [..., d]
@@ -331,6 +335,7 @@ def token_embedding(ids: Tensor, weight: Tensor, *, positions: Optional[Tensor] 
     out = native.embed(ids, weight, positions, scale, padding) if native else None
     if out is not None:
         return out
+    _no_tangents("token_embedding", weight, positions)
     _require(ids.dim() >= 1 or positions is None, "positions need ids with a dimension")
     _require(weight.dim() == 2, f"weight must be [vocab, d], got {tuple(weight.shape)}")
     ids2 = ids if ids.dim() == 2 else ids.reshape(-1, ids.shape[-1] if ids.dim() and ids.shape[-1] else 1)
@@ -484,5 +489,6 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = [g for p in {id(p): p for p in parameters}.values() if (g := p.grad) is not None]
     if not grads:
         return torch.tensor(0.0)
+    _no_tangents("clip_grad_norm_", *grads)
     with torch.no_grad():
         return (_clip_of if native and _plain(grads) else clip_grads_op)(grads, max_norm, code)

@@ -20,6 +20,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _dtype_code, _ptr, _require
@@ -38,6 +39,15 @@ _HERE = nullcontext()
 def _on(device: torch.device):
     """Makes `device` current where it is not."""
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _no_tangents(what: str, *tensors: Optional[Tensor]) -> None:
+    """Refuses forward-mode derivatives, which the kernels would drop (an autograd.Function refuses
+    them itself, but calls without gradients do not go through one)."""
+    if not torch.compiler.is_compiling() and forward_ad._current_level >= 0:
+        for t in tensors:
+            _require(t is None or forward_ad.unpack_dual(t).tangent is None,
+                     f"{what} has no forward-mode derivatives (an input is a dual tensor)")
 
 
 _TENSORS = (Tensor, torch.nn.Parameter)
@@ -235,6 +245,7 @@ class _XentReduced(torch.autograd.Function):
 
 
 def _reduced_backward(ctx, grad):
+    _no_tangents("linear_cross_entropy's backward", grad)
     need = ctx.needs_input_grad
     if ctx.args is not None:
         x, w, targets, kept = ctx.saved_tensors
@@ -267,6 +278,7 @@ class _XentNone(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _no_tangents("linear_cross_entropy's backward", grad)
         x, w, targets = ctx.saved_tensors
         need = ctx.needs_input_grad
         f = _linear_xent_none_grads if _direct(x, w, targets, grad) else linear_xent_none_grads_op
@@ -293,7 +305,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
     most half a GiB; for more tokens, and under torch.compile and dispatch modes,
     they compute the gradients together with the loss, half a GiB of exponentials
     at a time, and keep those. "none" recomputes in the backward. Gradients of
-    gradients are not supported.
+    gradients and forward-mode derivatives are not supported.
 
     Precision: sums are fp32. fp32 inputs keep 24 bits and their range in every
     product. bfloat16: the exponentials are held in fp16 relative to the largest
@@ -312,6 +324,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, *, ignore_i
         dt = torch.get_autocast_dtype("cuda")
         dt = torch.float32 if dt == torch.float16 else dt  # (no fp16 kernels)
         x, weight = x.to(dt), weight.to(dt)
+    _no_tangents("linear_cross_entropy", x, weight)
     flat = x.dim() == 2
     x2, t = (x, targets) if flat else (x.reshape(-1, x.shape[-1]), targets.reshape(-1))
     grads = torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad)
