@@ -74,9 +74,9 @@ struct MmArgs {
   int split;
   float* part;
   // The tensor cores' additions drop what lies below the running sum's last
-  // bits: a sum that grows evenly comes out up to 2^-26 per product of 16 short
-  // (measured for bf16 operands, three times that for fp16), always
-  // towards zero. chain > 0 bounds each such sum to that many K = 64 steps (of
+  // bits: a sum that grows evenly comes out 2^-30 (a few thousand products) to
+  // 2^-27 (2^19) per product short (measured for bf16 operands, three times
+  // that for fp16), always towards zero. chain > 0 bounds each such sum to that many K = 64 steps (of
   // the last term's, or the last `majors`'; the terms before, smaller by 2^-8 and less, make one
   // more): the epilogue warps add it to the tile's fp32 sum in TMEM, rounded to
   // nearest, while the next one is under way (Epi::kChain; not shape 3).

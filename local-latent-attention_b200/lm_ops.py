@@ -179,7 +179,9 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     returned to memory in full: with gradients the call keeps 4 bytes (bfloat16; 8
     for float32) a token and inner column for its backward.
 
-    Precision: sums are fp32. float32 inputs keep 24 bits in every product.
+    Precision: sums are fp32, by the tensor cores, whose additions drop what lies below a sum's last
+    bits: bfloat16 products of one sign come out up to 2^-27 each short, in sums of at most 2^17
+    that are added up in fp32 (float32: of 256). float32 inputs keep 24 bits in every product.
     bfloat16: the products' operands act(g) u and its gradients are rounded to
     bfloat16 once (for up to 64 tokens to 16 bits), what is kept to 11 bits relative to the largest of 16 neighbours, and
     the results once. Infinities in a token's inputs make its results infinite or NaN."""
