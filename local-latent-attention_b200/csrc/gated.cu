@@ -32,6 +32,7 @@
 #include <algorithm>
 
 #include "gated.cuh"
+#include "gated_act.cuh"
 #include "mm_rows.cuh"
 
 namespace llattn {
@@ -49,33 +50,47 @@ constexpr int kFineF32Chain = 1, kF32Chain = 4;
 constexpr int kLongSum = 1 << 17, kLongChain = 1024;
 constexpr int kBlock = 16;  // inner columns of a kept block
 
-// act(g) and act'(g). EXACT: to fp32's last bits; otherwise ex2's and rcp's 2^-22, and
-// erf by Abramowitz and Stegun's 7.1.26 (1.5e-7), which shares its exponential with the density.
-// (8 and 19 instructions: the epilogues that use them are as long as their tile's products.)
+// act(g) and act'(g) for h in P planes. 3: to fp32's last bits. Otherwise ex2's and rcp's 2^-22, and phi(-|g|) =
+// exp(-g^2 / 2) t P(t) with t = 1 / (1 + p |g|), which shares its exponential with the density: P fitted to 9e-7 of the
+// value over all of [0, 19], as the tail's values are rounded relative to themselves (an approximation of erf to 1.5e-7
+// was off by 1 % at -8). ex2's rounded argument costs 3e-6 at -8, 8e-6 at -13, which h in two planes
+// would show: what it lost comes back there.
+// (8 and 21 instructions: the epilogues that use them are as long as their tile's products. For 48 tokens of 1536 x 4096
+// erfc and exp take 99 us a step for 89.)
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <int ACT, bool EXACT>
+template <int ACT, int P>
 __device__ __forceinline__ void activation(float g, float& a, float& slope) {
   if (ACT == LLATTN_ACT_SILU) {
-    const float s = EXACT ? 1.f / (1.f + expf(-g)) : fast_rcp(1.f + fast_exp2(g * -1.44269504f));
+    const float s = P == 3 ? 1.f / (1.f + expf(-g)) : fast_rcp(1.f + fast_exp2(g * -1.44269504f));
     a = g * s;
     slope = fmaf(a, 1.f - s, s);
-  } else if (EXACT) {
-    const float phi = 0.5f * erfcf(g * -0.70710678f);
-    a = g * phi;
-    slope = phi + g * (0.39894228f * expf(-0.5f * g * g));
   } else {
-    const float e = fast_exp2(g * g * -0.72134752f);
-    const float t = fast_rcp(fmaf(fabsf(g), 0.3275911f * 0.70710678f, 1.f));
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    q *= 0.5f * t * e;
-    const float phi = g > 0.f ? 1.f - q : q;
+    float phi, e;
+    if (P == 3) {
+      gaussian(g, phi, e);
+    } else {
+      if (P == 1) {
+        e = fast_exp2(g * g * -0.72134752f);
+      } else {
+        const float b = fminf(fabsf(g), 40.f), h = b * b, y = h * -0.72134752f;
+        const float lost = fmaf(fmaf(b, b, -h), -0.72134752f, fmaf(h, -0.72134752f, -y)) + h * -9.6298e-9f;
+        e = fast_exp2(y);
+        e = fmaf(e, lost * 0.69314718f, e);
+      }
+      const float t = fast_rcp(fmaf(fabsf(g), 0.2675534f, 1.f));
+      float q = fmaf(t, -0.06421818f, 0.17602679f);
+      q = fmaf(q, t, -0.04389216f);
+      q = fmaf(q, t, 0.1290285f);
+      q = fmaf(q, t, 0.08829407f);
+      q = fmaf(q, t, 0.1080908f);
+      q = fmaf(q, t, 0.10666981f);
+      q *= t * e;
+      phi = g > 0.f ? 1.f - q : q;
+    }
     a = g * phi;
     slope = phi + g * (0.39894228f * e);
   }
@@ -208,7 +223,7 @@ struct EpiGated {
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
         float a, slope;
-        activation<ACT, F32>(g[q], a, slope);
+        activation<ACT, P>(g[q], a, slope);
         g[q] = a * u[q];
       }
       bf16* dst = h + row * ld + col;
@@ -290,7 +305,7 @@ struct EpiGrad {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           float act, slope;
-          activation<ACT, F32>(g[q], act, slope);
+          activation<ACT, P>(g[q], act, slope);
           g[q] = act * u[q];
           u[q] = dh[q] * u[q] * slope;
           dh[q] *= act;

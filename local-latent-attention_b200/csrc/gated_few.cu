@@ -33,6 +33,7 @@
 #include <algorithm>
 
 #include "gated.cuh"
+#include "gated_act.cuh"
 #include "pdl.cuh"
 #include "sm100_ptx.cuh"
 
@@ -160,7 +161,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[2][4
 
 __device__ __forceinline__ float gate(float g, int act) {
   if (act == LLATTN_ACT_SILU) return g / (1.f + expf(-g));
-  return 0.5f * g * erfcf(g * -0.70710678f);
+  float phi, e;
+  gaussian(g, phi, e);
+  return g * phi;
 }
 
 // SHIFT: rows (of x too) may be off a 16-byte boundary. WHOLE: a row block takes whole turns of the load
