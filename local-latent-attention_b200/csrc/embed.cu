@@ -10,7 +10,7 @@
 // start. Rows are then summed in that order, whatever the launch: a warp per word and
 // 1 KB of columns, zeros for a word without tokens. A word of more than kHot tokens
 // is cut at the multiples of kHot of the sorted order; these pieces go first, their sums
-// through the workspace, and are added in order. No atomics on values: the same bits
+// through the workspace, and are added in order, 32 and 32: no sum is one long chain. No atomics on values: the same bits
 // every run. Where words and tokens are few (`small`), a CTA a word picks its
 // tokens out of the ids itself, and one launch does it all.
 //
@@ -79,10 +79,11 @@ struct Pack {
     }
   }
   using Raw = std::conditional_t<VEC, uint4, T>;  // as it is in memory
-  __device__ __forceinline__ void add(const Raw& u) {
-    const T* e = reinterpret_cast<const T*>(&u);
+  __device__ __forceinline__ void add(const Raw& p, const Raw& q, const Raw& r, const Raw& s) {
+    const T *a = reinterpret_cast<const T*>(&p), *b = reinterpret_cast<const T*>(&q), *c = reinterpret_cast<const T*>(&r),
+            *d = reinterpret_cast<const T*>(&s);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += to_f<T>(e[i]);
+    for (int i = 0; i < N; ++i) v[i] += (to_f<T>(a[i]) + to_f<T>(b[i])) + (to_f<T>(c[i]) + to_f<T>(d[i]));
   }
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (VEC) {
@@ -340,10 +341,9 @@ __device__ __forceinline__ void add_rows(Pack<T, VEC> (&a)[kSlice], const T* dou
         if (j0 + j < m && c < d) r[j][k] = *reinterpret_cast<const typename P::Raw*>(row + c);
       }
     }
+    static_assert(kRows == 4, "rows in pairs, so that m of them are m / 4 additions in a row");
 #pragma unroll
-    for (int j = 0; j < kRows; ++j)
-#pragma unroll
-      for (int k = 0; k < kSlice; ++k) a[k].add(r[j][k]);
+    for (int k = 0; k < kSlice; ++k) a[k].add(r[0][k], r[1][k], r[2][k], r[3][k]);
   }
 }
 
@@ -441,7 +441,8 @@ __global__ void __launch_bounds__(256) embed_join(const int* words, const int* s
 #pragma unroll
     for (int k = 0; k < 32; ++k) x[k] = q + k <= q1 ? part[(int64_t)2 * (q + k) * d + c] : 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) a += x[k];
+    for (int k = 1; k < 32; ++k) x[0] += x[k];
+    a += x[0];  // (c tokens are 10, 31 and c / 1024 additions in a row)
   }
   dw[(int64_t)word * d + c] = from_f<T>(a * scale);
 }

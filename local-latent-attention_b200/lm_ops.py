@@ -323,7 +323,7 @@ def token_embedding(ids: Tensor, weight: Tensor, *, positions: Optional[Tensor] 
     in weight's dtype (autocast does not change it, as it does not change
     torch's embedding). At most 2^30 ids, 2^24 words.
 
-    weight's gradient sums the tokens of each word in fp32 in the order of the tokens: the same
+    weight's gradient sums the tokens of each word in fp32 in an order of their places: the same
     bits every run. Tokens of the word padding_idx (which may count from the end)
     do not take part in it. An id outside [0, vocab) makes its row NaN and has no
     gradient (it is an error that no launch can raise)."""

@@ -229,3 +229,20 @@ def test_refusals():
                           ((ids, w), dict(positions=pos[:1].expand(2**32 + 8, 16)), "too many")):
         with pytest.raises(RuntimeError, match=msg):
             token_embedding(*args, **kw)
+
+
+@pytest.mark.parametrize("n,v", [(256, 4), (2048, 4), (2048, 5000), (4096, 4), (65536, 5000), (1 << 20, 40)])
+@pytest.mark.parametrize("large", ["first", "each 256th", "last"])
+def test_a_words_sum_is_not_one_chain(n, v, large):
+    """Rows that vanish one by one beside a large one, and not together: a sum of n additions in a row would be off by n
+    half steps. Rows in pairs of pairs (8 and 2 additions for 32 of them), then such sums 32 at a time (31), then
+    c / 1024; small calls n / 32, 2 and 8: within 66 + c / 64."""
+    for small in (0.99 * 2.0 ** -24, 0.99 * 2.0 ** -29):  # of the large row: below its half step alone, or 32 of them
+        dout = torch.full((1, n, 8), small, device="cuda")
+        dout[0, {"first": slice(0, 1), "each 256th": slice(0, None, 256), "last": slice(-1, None)}[large]] = 1.0
+        ids = torch.full((1, n), 1, device="cuda")
+        w = torch.zeros(v, 8, device="cuda", requires_grad=True)
+        (dw,) = torch.autograd.grad(token_embedding(ids, w), w, dout)
+        want = dout.double().sum((0, 1))
+        assert ((dw[1].double() - want).abs() <= 2.0 ** -24 * (67 + n / 64) * want).all()
+        assert (dw[0] == 0).all() and (dw[2:] == 0).all()
