@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   const double total = Op::norm(block_join<Op>(a, red));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
   if (!scale) return;
-  const double c = max_norm / (total + 1e-6);
+  // by the norm that the call returns where that is infinite: a finite one above fp32's range counts as infinity
+  const double c = max_norm / ((isinf((float)total) ? (double)INFINITY : total) + 1e-6);
   const float f = c > 1.0 ? 1.f : (float)c;  // (a NaN stays one)
   if (f == 1.f) return;
   for (int k = run.y - 1; k >= run.x; --k) {

@@ -257,3 +257,28 @@ def test_empty_tensors_and_the_workspaces_size(count, before, after):
         assert abs(through_c(lists, max_norm=0.5) - want) <= NORM * want
     if held:  # clipped once (bf16: half a step an element)
         assert abs(norm64(held).item() / min(want, 0.5) - 1) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("dt", (BF, FP), ids=("bf16", "f32"))
+def test_a_norm_above_fp32s_range_is_infinite(dt):
+    """Finite gradients whose norm no fp32 holds: infinity is returned and the gradients are 0, as torch's."""
+    ps, ref = (params([(333, 77), (5,)], (dt,), seed=3) for _ in range(2))
+    for p in (*ps, *ref):
+        p.grad.fill_(3e38)
+    for kind in (2.0, float("inf")):
+        norm, want = clip_grad_norm_(ps, 1.0, kind), torch.nn.utils.clip_grad_norm_(ref, 1.0, kind)
+        if kind == 2.0:
+            assert norm.isinf() and want.isinf()
+            assert all((p.grad == 0).all() for p in (*ps, *ref))
+            with pytest.raises(RuntimeError, match="not finite"):
+                ps[0].grad.fill_(3e38)
+                clip_grad_norm_(ps, 1.0, kind, error_if_nonfinite=True)
+            assert (ps[0].grad == torch.tensor(3e38, dtype=dt, device="cuda")).all()
+        else:  # (the largest magnitude is finite)
+            assert abs(norm.item() / 3e38 - 1) <= 2.0 ** -8
+        for p in (*ps, *ref):
+            p.grad.fill_(3e38)
+    # just inside: as any other
+    p = params([(4,)], (dt,))[0]
+    p.grad.fill_(1e38)
+    check([p], 3.0)
