@@ -481,7 +481,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     native = _eager()
     if error_if_nonfinite:
-        norm = total_norm([g for p in parameters if (g := p.grad) is not None], norm_type)
+        norm = total_norm([g for p in {id(p): p for p in parameters}.values() if (g := p.grad) is not None], norm_type)
         if not torch.isfinite(norm):
             raise RuntimeError(f"llattn: the total norm of order {norm_type} of the gradients is not finite, so they cannot "
                                "be clipped; error_if_nonfinite=False scales them all the same")

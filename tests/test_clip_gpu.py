@@ -282,3 +282,11 @@ def test_a_norm_above_fp32s_range_is_infinite(dt):
     p = params([(4,)], (dt,))[0]
     p.grad.fill_(1e38)
     check([p], 3.0)
+
+
+def test_given_twice_counts_once_in_the_check_too():
+    p = torch.nn.Parameter(torch.zeros(1, device="cuda"))
+    for kw in ({}, dict(error_if_nonfinite=True)):  # (twice it would be above fp32's range)
+        p.grad = torch.full((1,), 3e38, device="cuda")
+        norm = clip_grad_norm_([p, p], 1e38, **kw)
+        assert abs(norm.item() / 3e38 - 1) <= NORM and abs(p.grad.item() / 1e38 - 1) <= 8 * 2.0 ** -24
