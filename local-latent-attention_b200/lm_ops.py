@@ -41,10 +41,11 @@ def _eager():
 
 
 def _common_dtype(*tensors: Tensor) -> list[Tensor]:
-    """All in autocast's dtype, as a linear layer's inputs are (float32 where that is float16)."""
+    """All in autocast's dtype, as a linear layer's inputs are (float32 where that is float16): float64 and
+    integers are not, and are refused then."""
     dt = torch.get_autocast_dtype("cuda")
     dt = torch.float32 if dt == torch.float16 else dt  # (no fp16 kernels)
-    return [t.to(dt) if t.is_cuda else t for t in tensors]
+    return [t.to(dt) if t.is_cuda and t.is_floating_point() and t.dtype != torch.float64 else t for t in tensors]
 
 
 # --------------------------------------------------------------------------

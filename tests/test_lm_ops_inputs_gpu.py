@@ -70,3 +70,18 @@ def test_dual_gradients_are_not_clipped():
             clip_grad_norm_([p], 0.1)
         assert torch.equal(fwAD.unpack_dual(p.grad).primal, before)
         assert abs(total_norm([p.grad]).item() / before.norm().item() - 1) < 1e-6  # (not differentiable)
+
+
+def test_autocast_casts_what_it_casts_for_a_linear_layer():
+    ins = randn(5, 16), randn(24, 16), randn(24, 16), randn(16, 24)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want = gated_mlp(*ins)
+        assert torch.equal(gated_mlp(*(t.bfloat16() for t in ins)), want) and want.dtype == torch.bfloat16
+        assert gated_mlp(*(t.half() for t in ins)).dtype == torch.bfloat16
+        for k in range(4):
+            for dt in (torch.float64, torch.long):
+                own = [t.to(dt) if i == k else t for i, t in enumerate(ins)]
+                with pytest.raises(RuntimeError, match="dtype"):
+                    gated_mlp(*own)
+        with pytest.raises(RuntimeError, match="dtype"):
+            gated_mlp(*(t.double() for t in ins))
