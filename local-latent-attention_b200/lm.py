@@ -160,7 +160,10 @@ class LocalLatentLM(nn.Module):
         positions = self.position.weight
         if self.fused_embedding:
             return token_embedding(ids, self.embedding.weight, positions=positions[first:] if first else positions)
-        return self.embedding(ids) + positions[first:first + ids.shape[1]].unsqueeze(0)
+        rows = positions[first:first + ids.shape[1]]
+        if first and rows.shape[0] < ids.shape[1]:
+            raise IndexError(f"positions {first} to {first + ids.shape[1] - 1} of {positions.shape[0]}")
+        return self.embedding(ids) + rows.unsqueeze(0)
 
     def loss_head(self, x: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         if self.fused_loss:
@@ -201,7 +204,10 @@ class LocalLatentLM(nn.Module):
         return ids
 
     def _prefill(self, ids: torch.Tensor, caches) -> torch.Tensor:
-        x = self._embed(ids)
+        if self.fused_embedding:
+            x = self._embed(ids)
+        else:
+            x = self.embedding(ids) + self.position(torch.arange(ids.shape[1], device=ids.device)).unsqueeze(0)
         for blk, cache in zip(self.blocks, caches):
             x = x + blk.attn.prefill(blk.norm1(x), cache)
             x = x + blk.mlp(blk.norm2(x))

@@ -54,6 +54,14 @@ def test_the_reference_config_has_no_gate():
     assert list(a.state_dict()) == list(b.state_dict())
 
 
+def test_positions_past_the_table_are_refused():
+    m, ids = LocalLatentLM(small_cfg()), torch.zeros(2, 3, dtype=torch.long)
+    assert m._embed(ids, 157).shape == (2, 3, 128)
+    for tok, first in ((ids[:, :1], 160), (ids, 158), (ids[:, :1], 1000)):
+        with pytest.raises(IndexError):
+            m._embed(tok, first)
+
+
 # --- on the GPU ----------------------------------------------------------------------
 
 def model(**kw):
@@ -176,3 +184,27 @@ def test_example_runs(flags):
     spec.loader.exec_module(mod)
     losses = mod.main(["--steps", "3", "--layers", "1", *flags])
     assert len(losses) == 3 and all(v == v for v in losses)
+
+
+@pytest.mark.gpu
+def test_decoding_past_the_last_position_is_refused():
+    m = model().eval()
+    ids = tokens(159, 2)
+    caches = [blk.attn.new_decode_cache(160) for blk in m.blocks]
+    with torch.no_grad():
+        m._prefill(ids, caches)
+        m._decode_one(ids[:, :1], 159, caches)
+        with pytest.raises(IndexError):
+            m._decode_one(ids[:, :1], 160, caches)
+        m.fused_embedding = True
+        with pytest.raises(RuntimeError, match="positions"):
+            m._decode_one(ids[:, :1], 160, caches)
+
+
+@pytest.mark.gpu
+def test_generation_calls_the_position_module():
+    """A forward hook on model.position sees the prompt's rows, as it does in torch's own call."""
+    m, seen = model().eval(), []
+    m.position.register_forward_hook(lambda mod, args, out: seen.append(out.shape))
+    m.generate(tokens(20, 2), 3)
+    assert seen == [(20, 128)]
