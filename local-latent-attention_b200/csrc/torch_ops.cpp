@@ -44,8 +44,11 @@ int dtype_of(const Tensor& t) {
   return t.scalar_type() == at::kFloat ? LLATTN_F32 : t.scalar_type() == at::kBFloat16 ? LLATTN_BF16 : -1;
 }
 bool like(const Tensor& t, const Tensor& o) { return plain(t) && t.scalar_type() == o.scalar_type() && t.device() == o.device(); }
+// a view whose sign is still to be applied (imag of a conjugate) with it applied: the kernels read the memory
+Tensor signs(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 // contiguous columns and rows that do not overlap
-Tensor rows(const Tensor& t) {
+Tensor rows(const Tensor& u) {
+  const Tensor t = signs(u);
   return t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1)) ? t : t.contiguous();
 }
 int64_t stride_of(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
@@ -235,7 +238,7 @@ struct EmbedBackward : torch::autograd::Node {
     {
       at::NoGradGuard no_grad;
       const c10::cuda::CUDAGuard guard(grads[0].device());
-      const Tensor ids = ids_.unpack().contiguous(), dout = grads[0].contiguous();
+      const Tensor ids = ids_.unpack().contiguous(), dout = signs(grads[0]).contiguous();
       const int64_t d = dout.size(2);
       llattn_embed_args a = embed_args(ids, vocab, d, dtype_of(dout), position_rows, scale, padding);
       const auto opts = dout.options().requires_grad(false);

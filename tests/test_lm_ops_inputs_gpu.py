@@ -85,3 +85,38 @@ def test_autocast_casts_what_it_casts_for_a_linear_layer():
                     gated_mlp(*own)
         with pytest.raises(RuntimeError, match="dtype"):
             gated_mlp(*(t.double() for t in ins))
+
+
+def pending(t):
+    """-t as a view that has its sign still to be applied: what imag of a conjugate is."""
+    return torch._neg_view(t)
+
+
+def test_signs_that_are_still_to_be_applied():
+    one, z = torch.ones(1, 1, device="cuda"), torch.complex(*torch.full((2, 1, 1), 2.0, device="cuda")).conj().imag
+    assert z.is_neg() and z.item() == -2.0
+    assert torch.equal(gated_mlp(z, one, one, one), gated_mlp(z.clone(), one, one, one))
+    ins = [randn(5, 16), randn(24, 16), randn(24, 16), randn(16, 24)]
+    for k in range(4):
+        got = []
+        for f in (pending, torch.neg):
+            leaves = [t.clone().requires_grad_(True) for t in ins]
+            y = gated_mlp(*(f(t) if i == k else t for i, t in enumerate(leaves)))
+            dy = torch.ones_like(y)
+            grads = torch.autograd.grad(y, leaves, f(dy))
+            with torch.no_grad():
+                got.append((y, gated_mlp(*(f(t) if i == k else t for i, t in enumerate(ins))), *grads))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+    table, pos, ids = randn(50, 16), randn(7, 16), torch.randint(0, 50, (2, 7), device="cuda")
+    got = []
+    for f in (pending, torch.neg):
+        leaves = [t.clone().requires_grad_(True) for t in (table, pos)]
+        out = token_embedding(ids, f(leaves[0]), positions=f(leaves[1]))
+        got.append((out, *torch.autograd.grad(out, leaves, f(torch.ones_like(out)))))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    p = torch.nn.Parameter(randn(9))
+    p.grad = pending(randn(9) * 3)
+    before = p.grad.clone()
+    norm = clip_grad_norm_([p], 0.5)
+    assert abs(norm.item() / before.norm().item() - 1) < 1e-6
+    assert torch.allclose(p.grad, before * (0.5 / before.norm()), rtol=1e-5)
