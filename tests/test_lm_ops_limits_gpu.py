@@ -162,3 +162,36 @@ def test_changes_in_place():
         leaf.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_gated_mlp_loses_no_row_past_32_bits():
+    """Gradients of a few rows alone, around element 2^31 of h and in the last, partial step of the sums over the tokens: a
+    row that is lost or read elsewhere shows, which sums over all of them would hide."""
+    n, d, ff = 540_000, 24, 4000
+    rows = torch.tensor([0, 63, 2**31 // ff - 1, 2**31 // ff, 2**31 // ff + 1, n - 65, n - 64, n - 32, n - 2, n - 1], device="cuda")
+    assert n % 64 == 32
+    x, dy = randn(n, d, dtype=BF), torch.zeros(n, d, device="cuda", dtype=BF)
+    dy[rows] = randn(len(rows), d, dtype=BF)
+    weights = [randn(ff, d, dtype=BF, scale=d**-0.5), randn(ff, d, dtype=BF, scale=d**-0.5), randn(d, ff, dtype=BF, scale=ff**-0.5)]
+    leaves = [t.requires_grad_(True) for t in (x, *weights)]
+    y = gated_mlp(*leaves)
+    dx, *dws = torch.autograd.grad(y, leaves, dy)
+    xs, ds, wg, wu, wd = (t.detach().double() for t in (x[rows], dy[rows], *weights))
+    g, u = xs @ wg.T, xs @ wu.T
+    sig = torch.sigmoid(g)
+    a, slope, dh = g * sig, sig * (1 + g * (1 - sig)), ds @ wd
+    # operands rounded (2^-8) and kept values (2^-11 of each, |slope| and |g act''| below 1.2), results rounded (2^-8), sums:
+    # 2^-6 of the absolute terms
+    assert ((y[rows].double() - (a * u) @ wd.T).abs() <= 2.0**-6 * ((a * u).abs() @ wd.T.abs())).all()
+    dg, du = dh * u * slope, dh * a
+    size = 1.2 * (dh * u).abs() @ wg.abs() + (1.2 * (dh * g).abs() + du.abs()) @ wu.abs()
+    assert ((dx[rows].double() - dg @ wg - du @ wu).abs() <= 2.0**-6 * size).all()
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[rows] = False
+    assert (dx[rest] == 0).all()
+    for got, left, big, right in zip(dws, (dg, du, ds), ((dh * u).abs(), (dh * g).abs(), ds.abs()), (xs, xs, a * u)):
+        extra = 1.2 * (g * u).abs() if right is not xs else right.abs()
+        bound = 2.0**-6 * (1.2 * big.T @ extra.abs() + left.abs().T @ right.abs())
+        assert ((got.double() - left.T @ right).abs() <= bound).all()
+        # what any one of the rows adds is beyond the bound somewhere
+        assert all(((left[r, :, None] * right[r]).abs() > 2 * bound).any() for r in range(len(rows)))
