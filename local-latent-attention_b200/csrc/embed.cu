@@ -528,8 +528,12 @@ Plan make_plan(const llattn_embed_args& a) {
   q.total_at = q.sorters << q.bits;
   q.slices = cdiv(a.d, kSlice * 32 * pack);
   q.pieces = q.n > kHot ? cdiv(q.n, kHot) : 0;
-  // one launch while every CTA's words and ids take a few us (4096 CTAs: some 4 rounds of what the GPU holds)
-  q.small = q.n <= 2048 && a.vocab * q.slices <= 4096;
+  // One launch while its CTAs, 1 KB of a word's columns each, take less time than the launches of the sort (2048 tokens
+  // of 128 fp32: 9.8 us for 18.8 with 2048 CTAs, 15.1 for 19.0 with 4096, 25.9 for 18.9 with 8192; 256 tokens 8.9 for
+  // 13.7, 14.2 for 14.1, 24.9 for 14.0). A CTA of bf16 adds twice the columns (2048 tokens: 12.0 for 19.4 with 1024, 15.2
+  // for 19.2 with 2048, 25.4 for 19.5 with 4096; 256: 10.1 for 14.7, 14.5 for 14.2, 24.8 for 15.0). Past 2048 tokens
+  // each CTA's reading of all ids tells (4096 of 512 columns, 64 words: 26.6 for 26.7).
+  q.small = q.n <= 2048 && a.vocab * q.slices <= (q.elt == 4 ? 4096 : 2048);
   q.cols = (int64_t)a.length * a.d;
   // positions: the batch in as many pieces as fill the GPU, of at least 16 rows
   const int64_t ctas = cdiv64(q.cols, 1024 * pack);
