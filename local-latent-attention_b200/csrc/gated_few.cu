@@ -25,8 +25,8 @@
 // bf16: h is stored in two bf16 parts and multiplied in both. fp32: products on the SIMT cores, 8 tokens at a time.
 //
 // Measured (us, by CUDA graph over weights that come from memory; floor = the weights at 6.55 TB/s; 33: mm_kernel's
-// way): 1536 x 4096 (5.8): 14.0 for 1 token, 17.2 for 16, 21.5 for 24, 24.5 for 33; 2048 x 8192 (15.4): 26.8, 4096 x
-// 14336 (53.8): 84; 1411 x 3749 (4.8): 22, 24 tokens 30, 33: 38; fp32 1536 x 4096 (11.5): 27, 8 tokens
+// way): 1536 x 4096 (5.8): 14.2 for 1 token, 17.9 for 16, 21.7 for 24, 25.3 for 33; 2048 x 8192 (15.4): 28, 4096 x
+// 14336 (53.8): 86; 1411 x 3749 (4.8): 22, 24 tokens 31, 33: 38; fp32 1536 x 4096 (11.5): 27, 8 tokens
 // 40, 1411 x 3749 (9.7): 21. The
 // large ones are bound by how evenly the row blocks fill the SMs and by the pauses between CTAs, the small ones by two
 // launches of some 4 us.
@@ -509,11 +509,14 @@ cudaError_t run(const llattn_gated_args& a, cudaStream_t s) {
 
 }  // namespace
 
-// As many tokens as this form is faster for. bf16: beyond 8 it reads x more often than the weights' rows come
-// in, and only small weights, for which mm_kernel's launches are long, make up for that (16 and 24 tokens: 1536 x
-// 4096 17.3 and 21.6 us for 25, 2048 x 8192 32.6 and 40.5 for 33). fp32: 8 at a time, each reading the
-// weights again (16 tokens of 1536 x 4096 71 us for 100); where w_gate's and w_up's rows are off a 16-byte boundary
-// by different shifts it has none, as a CTA's rows have to be off by the same.
+// As many tokens as this form is faster for (us here, and by mm_kernel). bf16: beyond 8 it reads x more often than the
+// weights' rows come in, and only small weights, for which mm_kernel's launches are long, make up for that: 24 tokens of
+// 1024 x 2816 14.3 for 17.3, 1536 x 4096 21.7 for 25.3, 1800 x 4800 33.5 for 33.1, 2048 x 5461 (2^25 weights) 40.7 for
+// 41.1, 2304 x 6144 41.7 for 35.6, 2048 x 8192 42.3 for 37.8; 25, another group, 36.7 for 24.3 at 1536 x 4096. Past 2^25
+// weights 8 tokens are 26.6 for 36.8 and 28.5 for 38.1, 16 34.1 for 35.5 and 34.7 for 37.8: near enough for one limit.
+// fp32: 8 at a time, each reading the weights again: 16 tokens 40 for 67 (1024 x 2816), 71 for 101, 158 for 204 (2048 x
+// 8192), 17 46 for 67, 86 for 101, 215 for 204; where w_gate's and w_up's rows are off a 16-byte boundary by
+// different shifts it has none, as a CTA's rows have to be off by the same.
 int few_tokens(const llattn_gated_args& a) {
   if (a.dtype == LLATTN_F32) {
     const bool alike = (((uintptr_t)a.w_gate ^ (uintptr_t)a.w_up) & 15) == 0 && (a.ldg - a.ldu) % 4 == 0;
