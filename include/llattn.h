@@ -399,8 +399,8 @@ LLATTN_API int llattn_orth(const llattn_orth_args* args, void* stream);
  * stride lddy) and writes, contiguous, each of dx [tokens, d], dw_gate, dw_up [ff, d]
  * and dw_down [d_out, ff] that is not NULL.
  * act: silu(g) = g / (1 + exp(-g)), or gelu(g) = g (1 + erf(g / sqrt 2)) / 2.
- * workspace and kept: 256-byte aligned, no initialisation; the workspace's size
- * is llattn_gated_workspace_bytes(args, backward). */
+ * Tensors are aligned to their elements. workspace and kept: 256-byte aligned, no
+ * initialisation; the workspace's size is llattn_gated_workspace_bytes(args, backward). */
 typedef enum llattn_activation { LLATTN_ACT_SILU = 0, LLATTN_ACT_GELU = 1 } llattn_activation;
 
 typedef struct llattn_gated_args {
@@ -440,8 +440,9 @@ LLATTN_API int llattn_gated_bwd(const llattn_gated_args* args, void* stream);
  *   out, dout [batch, length, d], dw [vocab, d], dpositions [position_rows, d]: contiguous
  * An id outside [0, vocab) makes its row of out NaN and has no gradient; tokens of the
  * word `padding` (< 0: none) have no gradient either, in dw. llattn_embed_bwd writes each
- * of dw and dpositions that is not NULL, whole. workspace: llattn_embed_workspace_bytes
- * bytes, 256-byte aligned, no initialisation (the forward needs none). */
+ * of dw and dpositions that is not NULL, whole. Tensors are aligned to their elements.
+ * workspace: llattn_embed_workspace_bytes bytes, 256-byte aligned, no initialisation
+ * (the forward needs none). */
 typedef struct llattn_embed_args {
   int32_t batch, length, d, dtype, ids_wide, position_rows;
   int64_t vocab, padding;

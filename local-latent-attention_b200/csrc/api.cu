@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -799,6 +800,11 @@ static int check_gated(const llattn_gated_args* a, bool backward) {
   return LLATTN_OK;
 }
 
+// Whether none of the tensors (those that are not NULL) starts inside an element.
+static bool whole_elements(int dtype, std::initializer_list<const void*> tensors) {
+  return std::all_of(tensors.begin(), tensors.end(), [&](const void* p) { return al(p, dtype == LLATTN_F32 ? 4 : 2); });
+}
+
 size_t llattn_gated_kept_bytes(const llattn_gated_args* a) { return check_gated(a, false) ? 0 : gated::kept_bytes(*a); }
 
 size_t llattn_gated_workspace_bytes(const llattn_gated_args* a, int backward) {
@@ -812,6 +818,9 @@ static int run_gated(const llattn_gated_args* a, bool backward, const char* what
   if (backward ? !a->dy || !a->kept : !a->y) return fail(LLATTN_ERR_ARG, "%s: NULL pointer in args", what);
   if (backward && !a->dx && !a->dw_gate && !a->dw_up && !a->dw_down)
     return fail(LLATTN_ERR_ARG, "%s: no output asked for", what);
+  if (!whole_elements(a->dtype, {a->x, a->w_gate, a->w_up, a->w_down}) ||
+      !(backward ? whole_elements(a->dtype, {a->dy, a->dx, a->dw_gate, a->dw_up, a->dw_down}) : whole_elements(a->dtype, {a->y})))
+    return fail(LLATTN_ERR_ALIGN, "%s: a tensor is not aligned to its elements", what);
   const size_t need = gated::workspace_bytes(*a, backward);
   if (!a->workspace || a->workspace_bytes < need)
     return fail(LLATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, need, a->workspace_bytes);
@@ -849,6 +858,8 @@ int llattn_embed_fwd(const llattn_embed_args* a, void* stream) {
   if (!a->ids || !a->w || !a->out) return fail(LLATTN_ERR_ARG, "llattn_embed_fwd: NULL pointer in args");
   if (a->ldw < a->d || (a->positions && a->ldp < a->d))
     return fail(LLATTN_ERR_ARG, "embed: row strides (%lld, %lld) below d = %d", (long long)a->ldw, (long long)a->ldp, a->d);
+  if (!whole_elements(a->dtype, {a->w, a->positions, a->out}) || !al(a->ids, a->ids_wide ? 8 : 4))
+    return fail(LLATTN_ERR_ALIGN, "llattn_embed_fwd: a tensor is not aligned to its elements");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   prof::Scope ps(prof::EMBED, s);
   return check_launch(embed::launch_fwd(*a, s), "embed_fwd");
@@ -859,6 +870,8 @@ int llattn_embed_bwd(const llattn_embed_args* a, void* stream) {
   if (rc) return rc;
   if (!a->dout || (a->dw && !a->ids)) return fail(LLATTN_ERR_ARG, "llattn_embed_bwd: NULL pointer in args");
   if (!a->dw && !a->dpositions) return fail(LLATTN_ERR_ARG, "llattn_embed_bwd: no output asked for");
+  if (!whole_elements(a->dtype, {a->dout, a->dw, a->dpositions}) || !al(a->ids, a->ids_wide ? 8 : 4))
+    return fail(LLATTN_ERR_ALIGN, "llattn_embed_bwd: a tensor is not aligned to its elements");
   const size_t need = embed::workspace_bytes(*a);
   if (!a->workspace || a->workspace_bytes < need)
     return fail(LLATTN_ERR_WORKSPACE, "llattn_embed_bwd: workspace of %zu bytes needed, %zu given", need, a->workspace_bytes);
@@ -918,6 +931,7 @@ int llattn_clip(const llattn_clip_args* a, void* stream) {
   int rc = check_clip(a);
   if (rc) return rc;
   if (!a->norm) return fail(LLATTN_ERR_ARG, "llattn_clip: NULL pointer in args");
+  if (!al(a->norm, 4)) return fail(LLATTN_ERR_ALIGN, "llattn_clip: norm is not aligned to its 4 bytes");
   if (a->scale && (rc = check_apart(a))) return rc;
   const size_t need = clip::workspace_bytes(*a);
   if (!a->workspace || a->workspace_bytes < need)

@@ -144,6 +144,31 @@ def test_clip_workspace_counts_what_holds_something():
             assert size([0] * before + [5] * n + [0] * after) == launches * one, (n, before, after)
 
 
+@pytest.mark.parametrize("code,off", [(_lib.BF16, 1), (_lib.F32, 1), (_lib.F32, 2)])
+def test_tensors_that_start_inside_an_element(code, off):
+    """A pointer that no element starts at would fault in the kernels' single-element loads and stores."""
+    L, size = _lib.lib(), dict(workspace=1 << 30, workspace_bytes=1 << 40)
+    for name in ("x", "w_gate", "w_up", "w_down", "y"):
+        bad = gated_args(dtype=code, **size)
+        setattr(bad, name, getattr(bad, name) + off)
+        refused(L.llattn_gated_fwd(ctypes.byref(bad), None), "aligned to its elements")
+    for name in ("x", "w_gate", "w_up", "w_down", "dy", "dx", "dw_gate", "dw_up", "dw_down"):
+        bad = gated_args(dtype=code, **size)
+        setattr(bad, name, getattr(bad, name) + off)
+        refused(L.llattn_gated_bwd(ctypes.byref(bad), None), "aligned to its elements")
+    for f, names in ((L.llattn_embed_fwd, ("w", "positions", "out", "ids")), (L.llattn_embed_bwd, ("dout", "dw", "dpositions", "ids"))):
+        for name in names:
+            bad = embed_args(dtype=code, **size)
+            setattr(bad, name, getattr(bad, name) + off)
+            refused(f(ctypes.byref(bad), None), "aligned to its elements")
+    for wide, step in ((1, 4), (0, 2)):
+        bad = embed_args(ids_wide=wide, ids=(1 << 20) + step, **size)
+        refused(L.llattn_embed_fwd(ctypes.byref(bad), None), "aligned to its elements")
+        refused(L.llattn_embed_bwd(ctypes.byref(bad), None), "aligned to its elements")
+    bad = clip_args([4096], [4], [code], norm=(1 << 20) + off, **size)
+    refused(L.llattn_clip(ctypes.byref(bad), None), "norm is not aligned")
+
+
 def test_lm_ops_on_the_cpu_are_refused():
     with pytest.raises(RuntimeError, match="CUDA"):
         llattn_b200.token_embedding(torch.zeros(2, 3, dtype=torch.long), torch.randn(4, 8))
