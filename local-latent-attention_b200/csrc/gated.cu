@@ -51,11 +51,11 @@ constexpr int kLongSum = 1 << 17, kLongChain = 1024;
 constexpr int kBlock = 16;  // inner columns of a kept block
 
 // act(g) and act'(g) for h in P planes. 3: to fp32's last bits. Otherwise ex2's and rcp's 2^-22, and phi(-|g|) =
-// exp(-g^2 / 2) t P(t) with t = 1 / (1 + p |g|), which shares its exponential with the density: P fitted to 9e-7 of the
+// exp(-g^2 / 2) t P(t) with t = 1 / (1 + p |g|), which shares its exponential with the density: P fitted to 1.2e-7 of the
 // value over all of [0, 19], as the tail's values are rounded relative to themselves (an approximation of erf to 1.5e-7
-// was off by 1 % at -8). ex2's rounded argument costs 3e-6 at -8, 8e-6 at -13, which h in two planes
-// would show: what it lost comes back there.
-// (8 and 21 instructions: the epilogues that use them are as long as their tile's products. For 48 tokens of 1536 x 4096
+// was off by 1 % at -8): 2^-20 with all roundings. ex2's rounded argument costs 3e-6 at -8, 8e-6 at -13, which h in two
+// planes would show: what it lost comes back there.
+// (8 and 22 instructions: the epilogues that use them are as long as their tile's products. For 48 tokens of 1536 x 4096
 // erfc and exp take 99 us a step for 89.)
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
@@ -81,13 +81,14 @@ __device__ __forceinline__ void activation(float g, float& a, float& slope) {
         e = fast_exp2(y);
         e = fmaf(e, lost * 0.69314718f, e);
       }
-      const float t = fast_rcp(fmaf(fabsf(g), 0.2675534f, 1.f));
-      float q = fmaf(t, -0.06421818f, 0.17602679f);
-      q = fmaf(q, t, -0.04389216f);
-      q = fmaf(q, t, 0.1290285f);
-      q = fmaf(q, t, 0.08829407f);
-      q = fmaf(q, t, 0.1080908f);
-      q = fmaf(q, t, 0.10666981f);
+      const float t = fast_rcp(fmaf(fabsf(g), 0.23663878f, 1.f));
+      float q = fmaf(t, -0.06061577f, 0.19103926f);
+      q = fmaf(q, t, -0.11808938f);
+      q = fmaf(q, t, 0.15785509f);
+      q = fmaf(q, t, 0.045865543f);
+      q = fmaf(q, t, 0.09585728f);
+      q = fmaf(q, t, 0.093646936f);
+      q = fmaf(q, t, 0.09444093f);
       q *= t * e;
       phi = g > 0.f ? 1.f - q : q;
     }

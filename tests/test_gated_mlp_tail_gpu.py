@@ -1,6 +1,6 @@
 """gated_mlp's gelu where it is close to 0, relative to its value: y = gelu(g) 1 1 for inputs that make the products exact.
 
-Bounds, relative: bf16 rounds h (over 64 tokens, 2^-8; else 2^-16) and y (2^-8); phi is off by 2^-16 (the fit, ex2's
+Bounds, relative: bf16 rounds h (over 64 tokens, 2^-8; else 2^-16) and y (2^-8); phi is off by 2^-16 (ex2's
 argument up to 2^7), up to 64 tokens by 2^-18. dx rounds dg and itself. fp32: erfc's 4 ulp of 2^-23, exp's and the
 correction's two each, two products, and 24 bits of h, 2^-23, down to where its third plane is a bf16 number (1e-18)."""
 
