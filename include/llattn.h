@@ -470,8 +470,9 @@ LLATTN_API int llattn_embed_bwd(const llattn_embed_args* args, void* stream);
  * tensors, sizes (elements) and dtypes are host arrays, read during the call; a
  * tensor is sizes[i] consecutive elements, aligned to their own size, on the current
  * device; empty ones are skipped; with scale none may overlap another. norm: fp32 device
- * scalar. Sums are fp64, in a fixed order. Replaces torch.nn.utils.clip_grad_norm_
- * in the reference's training loop. workspace: llattn_clip_workspace_bytes bytes,
+ * scalar; one above fp32's range is infinite, here and in the factor. Squares are summed in
+ * fp32 within 16 bytes and in fp64 from there on, in a fixed order. Replaces
+ * torch.nn.utils.clip_grad_norm_ in the reference's training loop. workspace: llattn_clip_workspace_bytes bytes,
  * 256-byte aligned, no initialisation. */
 typedef enum llattn_norm_type { LLATTN_NORM_2 = 0, LLATTN_NORM_INF = 1 } llattn_norm_type;
 

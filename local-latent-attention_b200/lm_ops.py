@@ -176,16 +176,19 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     2^20, 2^26 tokens. activation: "silu", or "gelu" (by erf). Returns
     [..., d_out] in x's dtype.
 
-    Neither x @ w_gate.T nor x @ w_up.T nor their gradients before the activation are
-    returned to memory in full: with gradients the call keeps 4 bytes (bfloat16; 8
-    for float32) a token and inner column for its backward.
+    Memory, bytes a token and inner column: with gradients the call keeps x @ w_gate.T and x @ w_up.T
+    for its backward, 4 and 1 / 8 in bfloat16, 8 in float32; its workspace holds act(g) u, 2 in bfloat16 (4 up to
+    64 tokens), 6 in float32; the backward's holds that again, where w_down's gradient is wanted, and both gradients
+    before the activation, 4 (8; 12). Without gradients nothing but act(g) u is in memory; its gradient never is.
+    Rows off a 16-byte boundary, and all float32 operands, are copied besides (2 and 6 bytes an element).
 
     Precision: sums are fp32, by the tensor cores, whose additions drop what lies below a sum's last
     bits: bfloat16 products of one sign come out up to 2^-27 each short, in sums of at most 2^17
-    that are added up in fp32 (float32: of 256). float32 inputs keep 24 bits in every product.
-    bfloat16: the products' operands act(g) u and its gradients are rounded to
-    bfloat16 once (for up to 64 tokens to 16 bits), what is kept to 11 bits relative to the largest of 16 neighbours, and
-    the results once. Infinities in a token's inputs make its results infinite or NaN."""
+    that are added up in fp32 (float32: of 256). float32 inputs keep 24 bits in every product, and the
+    activation is to 2^-19 of its value.
+    bfloat16: the products' operands act(g) u and its gradients are rounded to bfloat16 once (for up to 64 tokens to
+    16 bits, of an activation to 2^-19 of its value), what is kept to 11 bits relative to the largest of 16 neighbours,
+    and the results once. Infinities in a token's inputs make its results infinite or NaN."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
         _require(False, f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
@@ -447,8 +450,8 @@ def _norm_code(norm_type) -> int:
 
 def total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
     """The norm of all tensors' elements together, as a float32 scalar on their
-    device: the 2-norm (sums in fp64, in a fixed order; finite for any finite float32
-    result) or, for norm_type=inf, the largest magnitude. NaN where one of them is. Not
+    device: the 2-norm (squares summed in fp32 within 16 bytes and in fp64 from there on, in a fixed
+    order; finite for any finite float32 result) or, for norm_type=inf, the largest magnitude. NaN where one of them is. Not
     differentiable.
     Tensors are bfloat16 or float32, of any shapes and mix, on one CUDA device; 0
     on the CPU for an empty list."""
