@@ -548,6 +548,9 @@ template <typename Epi, typename = void>
 struct SecondB : std::integral_constant<int, kSecondNone> {};
 template <typename Epi>
 struct SecondB<Epi, std::void_t<decltype(Epi::kSecond)>> : std::integral_constant<int, Epi::kSecond> {};
+struct NoMap {};
+template <typename Epi>
+using SecondMap = std::conditional_t<SecondB<Epi>::value == kSecondNone, NoMap, CUtensorMap>;
 
 // Epi: struct with
 //   template <int CW> __device__ void tile(const MmArgs&, MmTile, int row, int col0, int M, uint32_t taddr,
@@ -566,7 +569,7 @@ struct SecondB<Epi, std::void_t<decltype(Epi::kSecond)>> : std::integral_constan
 template <int SH, bool CHAIN, typename Epi>
 __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     mm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-              const __grid_constant__ CUtensorMap tm_b2, const __grid_constant__ MmArgs p,
+              const __grid_constant__ SecondMap<Epi> tm_b2, const __grid_constant__ MmArgs p,
               const __grid_constant__ Epi epi) {
   using S = MmShape<SH>;
   constexpr int SECOND = SecondB<Epi>::value;
@@ -595,7 +598,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
     fence_barrier_init();
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
-    if (SECOND != kSecondNone) prefetch_tmap(&tm_b2);
+    if constexpr (SECOND != kSecondNone) prefetch_tmap(&tm_b2);
   }
   if (warp == 1) {
     __syncwarp();
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
         for (int h = 0; h < S::NH; ++h) {
           uint8_t* dst = sb + h * S::BB;
           const int n = nb + h * S::HN;
-          if (SECOND == kSecondHalves) {
+          if constexpr (SECOND == kSecondHalves) {
             load(&tm_b, dst, k, n / 2, zb);
             load(&tm_b2, dst + S::BR * 64, k, n / 2, zb);
           } else if (p.b_mn) {
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(MmShape<SH>::THREADS, 1)
         const int ma = w.m0 + rank * 128, nb = w.n0 + rank * S::BR;
         for (int term = 0; ok && term < p.n_terms; ++term) {
           const int za = w.z + (int)((p.pa >> (4 * term)) & 15u), zb = w.z + (int)((p.pb >> (4 * term)) & 15u);
-          if (SECOND == kSecondTerms) mb = (p.b2 >> term) & 1 ? &tm_b2 : &tm_b;
+          if constexpr (SECOND == kSecondTerms) mb = (p.b2 >> term) & 1 ? &tm_b2 : &tm_b;
           int k = x.k0;
           if (!counted && it == 0 && k < x.k1) {  // (apart: a test in the loop costs a long product 3 %)
             copy(0, ma, nb, k, za, zb, true);
@@ -970,15 +973,16 @@ cudaError_t launch_mm_sh(MmArgs p, const Operand& a, const Operand& b, const Epi
   using S = MmShape<SH>;
   constexpr int SECOND = SecondB<Epi>::value;
   const int br = SECOND == kSecondHalves ? S::BR / 2 : S::BR;
-  CUtensorMap ta, tb, tb2;
+  CUtensorMap ta, tb;
+  SecondMap<Epi> tb2;
   if (!sm100::make_operand_map(&ta, a.p, a.rows, a.cols, a.ld, a.nz, a.zs, a.mn ? 64 : 128) ||
       !sm100::make_operand_map(&tb, b.p, b.rows, b.cols, b.ld, b.nz, b.zs, b.mn ? 64 : br))
     return cudaErrorInvalidValue;
-  tb2 = tb;
-  if (SECOND != kSecondNone &&
-      (!b2 || b2->mn != b.mn ||
-       !sm100::make_operand_map(&tb2, b2->p, b2->rows, b2->cols, b2->ld, b2->nz, b2->zs, b2->mn ? 64 : br)))
-    return cudaErrorInvalidValue;
+  if constexpr (SECOND != kSecondNone) {
+    if (!b2 || b2->mn != b.mn ||
+        !sm100::make_operand_map(&tb2, b2->p, b2->rows, b2->cols, b2->ld, b2->nz, b2->zs, b2->mn ? 64 : br))
+      return cudaErrorInvalidValue;
+  }
   if (SECOND == kSecondHalves) {
     if (b.mn || p.split) return cudaErrorInvalidValue;
     p.N = cdiv((int)b.rows, br) * S::BR;
