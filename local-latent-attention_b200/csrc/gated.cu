@@ -111,6 +111,11 @@ __device__ __forceinline__ uint32_t block_scale(const float (&v)[16]) {
   float m = 0.f;
 #pragma unroll
   for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(v[q]));
+  if (m == INFINITY) {  // (a weight's row that overflows leaves its neighbours as they are)
+    m = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) m = fabsf(v[q]) < INFINITY ? fmaxf(m, fabsf(v[q])) : m;
+  }
   const int e = __float_as_uint(m) >> 23;  // 2^(e - 127) <= m
   return (uint32_t)min(253, 127 + 14 + 127 - e);
 }

@@ -60,3 +60,33 @@ def test_far_and_no_numbers(n, dt, name):
         ok = want.isfinite()
         assert torch.equal(y[:len(g), 0].isnan() | y[:len(g), 0].isinf(), ~ok)
         assert ((y[:len(g), 0].double() - want)[ok].abs() <= 2 * 2.0 ** -8 * want[ok].abs() + 1e-38).all()
+
+
+@pytest.mark.parametrize("dt", (BF, FP), ids=("bf16", "f32"))
+@pytest.mark.parametrize("name", ("silu", "gelu"))
+@pytest.mark.parametrize("n", (5, 64, 90))
+@pytest.mark.parametrize("which", (0, 1))
+def test_an_overflowing_row_leaves_its_neighbours_gradients(n, name, dt, which):
+    """Columns of g or u that are infinite are kept beside finite ones, whose weights' gradients are what they are without."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dt)
+    x, ws, dy = r(n, 40) + 3, [r(48, 40) / 8, r(48, 40) / 8, r(24, 48)], r(n, 24)
+    x.abs_()
+    rows = [3, 16, 47]
+    rest = torch.ones(48, dtype=torch.bool, device="cuda")
+    rest[rows] = False
+
+    def grads():
+        leaves = [w.clone().requires_grad_(True) for w in ws]
+        return torch.autograd.grad(gated_mlp(x, *leaves, activation=name), leaves[:2], dy)
+
+    want = grads()
+    ws[which][rows[0]] = float("inf")
+    ws[which][rows[1]] = -float("inf")
+    # above fp32's range with every token (x's rows are positive and sum to more than 2; one entry of 3e38 alone leaves tokens
+    # with x[0] < 1.13 a finite 3e38, of which a block keeps 11 bits and its neighbours, 2^-28 of that and less, nothing)
+    assert x.sum(1).min() > 2
+    ws[which][rows[2]] = 3e38
+    for got, w in zip(grads(), want):
+        assert torch.equal(got[rest], w[rest])
+        assert (w[rest] != 0).any(1).all()
